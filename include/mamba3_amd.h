@@ -390,6 +390,86 @@ int m3_small_linear(const void* x, const void* norm_w, float eps, const void* we
 int m3_small_swiglu(const void* x, const void* norm_w, float eps, const void* w_gate,
                     const void* w_up, void* out, int32_t m, int32_t n, int32_t k, void* stream);
 
+/*
+ * The gated MLP of a block with its residual (mamba3/block.py:16-26, 86-91) for any number of
+ * rows, and its backward:
+ *   g = x W_gate^T, u = x W_up^T, h = silu(g) * u, y = [residual +] scale * (h W_down^T)
+ * x, residual, y, dy, dx [rows, d_model]; w_gate, w_up [d_ff, d_model]; w_down [d_model, d_ff]; all of
+ * one dtype (fp32 or bf16), contiguous; x, dy and the weights 16-byte aligned. Products accumulate in
+ * fp32 (fp32 operands: fp32 MFMA); bf16 rounds h, dg, du and the outputs. saved: what the backward
+ * reads, m3_swiglu_mlp_saved_size() bytes, 256-byte aligned; NULL when none follows. Any of the
+ * gradients may be NULL; the residual's is dy. Sums run in a fixed order. workspace: 256-byte
+ * aligned; `keeps` says whether saved is given. rows <= 2^30, d_model and d_ff <= 2^20.
+ */
+int m3_swiglu_mlp_saved_size(int64_t rows, int32_t d_model, int32_t d_ff, int32_t dtype, size_t* bytes);
+int m3_swiglu_mlp_fwd_workspace_size(int64_t rows, int32_t d_model, int32_t d_ff, int32_t dtype,
+                                     int32_t keeps, size_t* bytes);
+int m3_swiglu_mlp_fwd(int64_t rows, int32_t d_model, int32_t d_ff, int32_t dtype, const void* x,
+                      const void* w_gate, const void* w_up, const void* w_down, const void* residual,
+                      float scale, void* y, void* saved, void* workspace, size_t workspace_bytes,
+                      void* stream);
+int m3_swiglu_mlp_bwd_workspace_size(int64_t rows, int32_t d_model, int32_t d_ff, int32_t dtype,
+                                     size_t* bytes);
+int m3_swiglu_mlp_bwd(int64_t rows, int32_t d_model, int32_t d_ff, int32_t dtype, const void* x,
+                      const void* w_gate, const void* w_up, const void* w_down, float scale,
+                      const void* saved, const void* dy, void* dx, void* dw_gate, void* dw_up,
+                      void* dw_down, void* workspace, size_t workspace_bytes, void* stream);
+
+/* How the rows' losses become one. */
+enum m3_reduction {
+    M3_REDUCTION_NONE = 0,  /* loss [rows] */
+    M3_REDUCTION_MEAN = 1,  /* over the rows that count (NaN where none does) */
+    M3_REDUCTION_SUM = 2
+};
+
+/*
+ * Softmax cross entropy of the vocabulary projection (mamba3/block.py:183-192) without its
+ * logits, and its gradients:
+ *   z = hidden weight^T, lse = log sum exp z, loss = lse - z[target]
+ * hidden [rows, d_model] and weight [vocab, d_model] of one dtype (fp32 or bf16), contiguous,
+ * 16-byte aligned; target [rows]. A row whose target is ignore_index counts nowhere: its loss and
+ * its gradient are zero whatever it holds. Another target outside [0, vocab) gives NaN. The forward
+ * writes loss ([rows], or [1]), and lse [rows] and count [1] (rows that count; unused without a
+ * reduction) for the backward. The backward takes grad_loss of loss's shape; either gradient may
+ * be NULL. Logits and sums are fp32; for bf16 the gradient of the logits is rounded to bf16
+ * before its two products. Sums run in a fixed order. The backward's workspace holds the gradient
+ * of the logits for one piece of the vocabulary (up to 256 MB where 256 columns fit that).
+ * rows <= 2^30, d_model <= 2^20, vocab <= 2^30. workspace: 256-byte aligned.
+ */
+int m3_linear_xent_fwd_workspace_size(int64_t rows, int32_t d_model, int32_t vocab, int32_t dtype,
+                                      size_t* bytes);
+int m3_linear_xent_fwd(int64_t rows, int32_t d_model, int32_t vocab, int32_t dtype, int32_t reduction,
+                       const void* hidden, const void* weight, const int64_t* target,
+                       int64_t ignore_index, float* loss, float* lse, float* count, void* workspace,
+                       size_t workspace_bytes, void* stream);
+int m3_linear_xent_bwd_workspace_size(int64_t rows, int32_t d_model, int32_t vocab, int32_t dtype,
+                                      int32_t want_dhidden, int32_t want_dweight, size_t* bytes);
+int m3_linear_xent_bwd(int64_t rows, int32_t d_model, int32_t vocab, int32_t dtype, int32_t reduction,
+                       const void* hidden, const void* weight, const int64_t* target,
+                       int64_t ignore_index, const float* lse, const float* count,
+                       const float* grad_loss, void* dhidden, void* dweight, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* Norms of m3_clip_grad_norm. */
+enum m3_norm {
+    M3_NORM_L2 = 0,
+    M3_NORM_MAX = 1
+};
+
+/*
+ * The norm over all elements of n tensors together and, with `scale`, their scaling in place:
+ *   norm = (sum g^2)^(1/2) or max |g|; g <- g * min(1, max_norm / (norm + 1e-6))
+ * tensors, numel and dtype are host arrays of n entries (device pointers of contiguous fp32 or
+ * bf16 elements; empty tensors may be NULL), read before the call returns. The tensors must not
+ * overlap. norm [1] fp32 on the device. Squares add up in fp64, in a fixed order. NaN and infinite
+ * elements reach the norm; a NaN norm scales by NaN. A factor of 1 leaves the tensors unwritten.
+ * workspace: 256-byte aligned.
+ */
+int m3_clip_grad_norm_workspace_size(int32_t n, const int64_t* numel, const int32_t* dtype, size_t* bytes);
+int m3_clip_grad_norm(int32_t n, void* const* tensors, const int64_t* numel, const int32_t* dtype,
+                      int32_t norm_kind, int32_t scale, float max_norm, float* norm, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

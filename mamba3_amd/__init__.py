@@ -10,6 +10,11 @@ from .layer import KulaMamba, RMSNorm
 from .block import KulaMambaBlock, KulaMambaLM, SwiGLU
 from .ssd import chunked_ssd, SSDOutput
 from .scan import ssd_scan
+# Training operators beyond the reference's API: attributes of the package, not among the
+# eight names of `__all__`.
+from .clip import clip_grad_norm_
+from .loss import linear_cross_entropy
+from .mlp import swiglu_mlp
 
 __all__ = [
     "KulaMamba",

@@ -46,6 +46,17 @@ EXPORTED_SYMBOLS = (
     "m3_step_bwd_workspace_size",
     "m3_step_bwd",
     "m3_prefill_kernel_name",
+    "m3_swiglu_mlp_saved_size",
+    "m3_swiglu_mlp_fwd_workspace_size",
+    "m3_swiglu_mlp_fwd",
+    "m3_swiglu_mlp_bwd_workspace_size",
+    "m3_swiglu_mlp_bwd",
+    "m3_linear_xent_fwd_workspace_size",
+    "m3_linear_xent_fwd",
+    "m3_linear_xent_bwd_workspace_size",
+    "m3_linear_xent_bwd",
+    "m3_clip_grad_norm_workspace_size",
+    "m3_clip_grad_norm",
 )
 
 M3_ERR_UNSUPPORTED = 3
@@ -163,6 +174,22 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.m3_chunked_ssd_bwd_workspace_size.argtypes = [_i32] * 7 + [ctypes.POINTER(ctypes.c_size_t)]
     lib.m3_chunked_ssd_bwd.restype = ctypes.c_int
     lib.m3_chunked_ssd_bwd.argtypes = [_i32] * 6 + [_vp] * 23 + [ctypes.c_size_t, _vp]
+    size_p, f32 = ctypes.POINTER(ctypes.c_size_t), ctypes.c_float
+    dims = [_i64, _i32, _i32, _i32]  # rows, d_model, d_ff or vocab, dtype
+    for name, args in (
+            ("m3_swiglu_mlp_saved_size", [*dims, size_p]),
+            ("m3_swiglu_mlp_fwd_workspace_size", [*dims, _i32, size_p]),
+            ("m3_swiglu_mlp_fwd", [*dims] + [_vp] * 5 + [f32] + [_vp] * 3 + [ctypes.c_size_t, _vp]),
+            ("m3_swiglu_mlp_bwd_workspace_size", [*dims, size_p]),
+            ("m3_swiglu_mlp_bwd", [*dims] + [_vp] * 4 + [f32] + [_vp] * 7 + [ctypes.c_size_t, _vp]),
+            ("m3_linear_xent_fwd_workspace_size", [*dims, size_p]),
+            ("m3_linear_xent_fwd", [*dims, _i32] + [_vp] * 3 + [_i64] + [_vp] * 4 + [ctypes.c_size_t, _vp]),
+            ("m3_linear_xent_bwd_workspace_size", [*dims, _i32, _i32, size_p]),
+            ("m3_linear_xent_bwd", [*dims, _i32] + [_vp] * 3 + [_i64] + [_vp] * 6 + [ctypes.c_size_t, _vp]),
+            ("m3_clip_grad_norm_workspace_size", [_i32, _vp, _vp, size_p]),
+            ("m3_clip_grad_norm", [_i32, _vp, _vp, _vp, _i32, _i32, f32] + [_vp] * 2 + [ctypes.c_size_t, _vp])):
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = ctypes.c_int, args
 
 
 def lib() -> ctypes.CDLL:
@@ -432,3 +459,82 @@ def rmsnorm_bwd(x, weight, rstd, grad, dx, dweight) -> None:
     check(lib().m3_rmsnorm_bwd(ptr(x), dtype_code(x.dtype), ptr(weight), dtype_code(weight.dtype),
                                ptr(rstd), ptr(grad), dtype_code(grad.dtype), ptr(dx), ptr(dweight),
                                ptr(ws), n.value, rows, d, stream_of(x)), "m3_rmsnorm_bwd")
+
+
+# ---------------------------------------------------------------- training operators
+def _bytes_of(name: str, *args) -> int:
+    n = ctypes.c_size_t(0)
+    check(getattr(lib(), name)(*args, ctypes.byref(n)), name)
+    return n.value
+
+
+def _workspace(nbytes: int, device) -> torch.Tensor | None:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def swiglu_mlp_saved_bytes(rows: int, d: int, ff: int, dtype: torch.dtype) -> int:
+    return _bytes_of("m3_swiglu_mlp_saved_size", rows, d, ff, dtype_code(dtype))
+
+
+def swiglu_mlp_fwd(x, w_gate, w_up, w_down, residual, scale, y, saved) -> None:
+    """m3_swiglu_mlp_fwd on contiguous x (rows, d); allocates the workspace."""
+    rows, d = x.shape
+    dims = (rows, d, w_gate.shape[0], dtype_code(x.dtype))
+    n = _bytes_of("m3_swiglu_mlp_fwd_workspace_size", *dims, int(saved is not None))
+    ws = _workspace(n, x.device)
+    check(lib().m3_swiglu_mlp_fwd(*dims, ptr(x), ptr(w_gate), ptr(w_up), ptr(w_down), ptr(residual), scale,
+                                  ptr(y), ptr(saved), ptr(ws), n, stream_of(x)), "m3_swiglu_mlp_fwd")
+
+
+def swiglu_mlp_bwd(x, w_gate, w_up, w_down, scale, saved, dy, dx, dw_gate, dw_up, dw_down) -> None:
+    """m3_swiglu_mlp_bwd on contiguous (rows, d) tensors; allocates the workspace."""
+    rows, d = x.shape
+    dims = (rows, d, w_gate.shape[0], dtype_code(x.dtype))
+    n = _bytes_of("m3_swiglu_mlp_bwd_workspace_size", *dims)
+    ws = _workspace(n, x.device)
+    check(lib().m3_swiglu_mlp_bwd(*dims, ptr(x), ptr(w_gate), ptr(w_up), ptr(w_down), scale, ptr(saved),
+                                  ptr(dy), ptr(dx), ptr(dw_gate), ptr(dw_up), ptr(dw_down), ptr(ws), n,
+                                  stream_of(x)), "m3_swiglu_mlp_bwd")
+
+
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def linear_xent_fwd(hidden, weight, target, ignore_index, reduction, loss, lse, count) -> None:
+    """m3_linear_xent_fwd on contiguous hidden (rows, d); allocates the workspace."""
+    rows, d = hidden.shape
+    dims = (rows, d, weight.shape[0], dtype_code(hidden.dtype))
+    n = _bytes_of("m3_linear_xent_fwd_workspace_size", *dims)
+    ws = _workspace(n, hidden.device)
+    check(lib().m3_linear_xent_fwd(*dims, reduction, ptr(hidden), ptr(weight), ptr(target), ignore_index,
+                                   ptr(loss), ptr(lse), ptr(count), ptr(ws), n, stream_of(hidden)),
+          "m3_linear_xent_fwd")
+
+
+def linear_xent_bwd(hidden, weight, target, ignore_index, reduction, lse, count, grad, dhidden,
+                    dweight) -> None:
+    """m3_linear_xent_bwd on contiguous hidden (rows, d); allocates the workspace."""
+    rows, d = hidden.shape
+    dims = (rows, d, weight.shape[0], dtype_code(hidden.dtype))
+    n = _bytes_of("m3_linear_xent_bwd_workspace_size", *dims, int(dhidden is not None), int(dweight is not None))
+    ws = _workspace(n, hidden.device)
+    check(lib().m3_linear_xent_bwd(*dims, reduction, ptr(hidden), ptr(weight), ptr(target), ignore_index,
+                                   ptr(lse), ptr(count), ptr(grad), ptr(dhidden), ptr(dweight), ptr(ws), n,
+                                   stream_of(hidden)), "m3_linear_xent_bwd")
+
+
+NORM_L2, NORM_MAX = 0, 1
+
+
+def clip_grad_norm(tensors, kind: int, max_norm: float | None, norm) -> None:
+    """m3_clip_grad_norm on contiguous tensors; max_norm None: the norm alone. Allocates the
+    workspace."""
+    n = len(tensors)
+    ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors])
+    numel = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
+    dtype = (ctypes.c_int32 * n)(*[dtype_code(t.dtype) for t in tensors])
+    nbytes = _bytes_of("m3_clip_grad_norm_workspace_size", n, numel, dtype)
+    ws = _workspace(nbytes, norm.device)
+    check(lib().m3_clip_grad_norm(n, ptrs, numel, dtype, kind, int(max_norm is not None),
+                                  0.0 if max_norm is None else max_norm, ptr(norm), ptr(ws), nbytes,
+                                  stream_of(norm)), "m3_clip_grad_norm")

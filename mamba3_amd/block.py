@@ -18,6 +18,8 @@ from torch.utils.checkpoint import checkpoint as grad_checkpoint
 
 from . import _native, ops
 from .layer import KulaMamba, RMSNorm
+from .loss import linear_cross_entropy
+from .mlp import swiglu_mlp
 
 
 def add_scaled_linear(x: torch.Tensor, lin: nn.Linear, inp: torch.Tensor, scale: float,
@@ -79,6 +81,16 @@ class SwiGLU(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return self.w_down(self.hidden(x))
 
+    def fusable(self, x: torch.Tensor) -> bool:
+        """swiglu_mlp takes these projections and x: no biases, one dtype of its two."""
+        lins = (self.w_gate, self.w_up, self.w_down)
+        return (x.is_cuda and x.dtype in (torch.float32, torch.bfloat16) and not torch.is_autocast_enabled("cuda")
+                and all(p.bias is None and p.weight.dtype == x.dtype and p.weight.device == x.device for p in lins))
+
+    def fused(self, x: torch.Tensor, residual: torch.Tensor | None = None, scale: float = 1.0) -> torch.Tensor:
+        """[residual +] scale * w_down(silu(w_gate x) * w_up x) as one operator (swiglu_mlp)."""
+        return swiglu_mlp(x, self.w_gate.weight, self.w_up.weight, self.w_down.weight, residual, scale)
+
 
 class KulaMambaBlock(nn.Module):
     """Pre-norm residual block: x + s*ssm(norm(x)), then x + s*mlp(norm(x))
@@ -117,10 +129,17 @@ class KulaMambaBlock(nn.Module):
             self.mlp_norm = RMSNorm(d_model, eps=norm_eps)
             self.mlp = SwiGLU(d_model, d_ff, bias=bias)
 
+    # Run the MLP and its residual as one operator (swiglu_mlp: forward and backward on kernels of
+    # this package) instead of library products around element-wise passes. Off by default: its
+    # roundings differ (g, u and, in the backward, dh are not rounded to bf16).
+    fused_mlp: bool = False
+
     def _ssm_forward(self, x_normed):
         return self.ssm(x_normed)
 
     def _mlp_forward(self, x_normed):
+        if self.fused_mlp and self.mlp.fusable(x_normed):
+            return self.mlp.fused(x_normed)
         return self.mlp(x_normed)
 
     # The residual adds run as the beta = 1 input of the out_proj / w_down GEMMs
@@ -147,6 +166,10 @@ class KulaMambaBlock(nn.Module):
         return x
 
     def _mlp_residual(self, x: torch.Tensor, inplace: bool = False) -> torch.Tensor:
+        if self.fused_mlp:
+            n = self.mlp_norm(x)
+            if n.dtype == x.dtype and self.mlp.fusable(n):
+                return self.mlp.fused(n, x, self.residual_scale)
         return add_scaled_linear(x, self.mlp.w_down, self.mlp.hidden(self.mlp_norm(x)),
                                  self.residual_scale, inplace=inplace)
 
@@ -263,6 +286,28 @@ class KulaMambaLM(nn.Module):
         for m in self.modules():
             if isinstance(m, KulaMamba):
                 m._init_weights(dt_min=0.001, dt_max=0.1)
+
+    def fuse_mlp(self, on: bool = True) -> "KulaMambaLM":
+        """Switches every block's MLP to the fused operator (KulaMambaBlock.fused_mlp) or back."""
+        for layer in self.layers:
+            layer.fused_mlp = on
+        return self
+
+    def loss(self, input_ids: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
+        """The mean next-token cross entropy that forward returns as "loss" (fp32), without the
+        logits: the head and the loss are one operator (linear_cross_entropy), so a training step
+        holds neither the (tokens, vocab) logits nor their gradient. labels: (B, T), position t is
+        predicted from t - 1; those equal to ignore_index do not count."""
+        if labels.shape != input_ids.shape:
+            raise ValueError(f"labels have shape {tuple(labels.shape)}, expected {tuple(input_ids.shape)}")
+        x = self.embedding(input_ids)
+        for layer in self.layers:
+            x = layer(x, _own_input=True)
+        # the last position predicts nothing: it is ignored rather than cut off, which would copy
+        # the hidden states
+        target = torch.full_like(labels, ignore_index)
+        target[:, :-1] = labels[:, 1:]
+        return linear_cross_entropy(self.norm(x), self.lm_head.weight, target, ignore_index)
 
     def forward(self, input_ids: torch.Tensor, labels: torch.Tensor | None = None) -> dict:
         x = self.embedding(input_ids)

@@ -582,4 +582,165 @@ int m3_chunked_ssd_bwd(int32_t batch, int32_t seqlen, int32_t nheads, int32_t he
                : M3_ERR_LAUNCH;
 }
 
+// ---- training operators
+static int check_product(int64_t rows, int64_t d, int64_t cols, int64_t most_cols, int32_t dtype) {
+    if (rows <= 0 || d <= 0 || cols <= 0) return M3_ERR_INVALID_SHAPE;
+    if (rows > ((int64_t)1 << 30) || d > (1 << 20) || cols > most_cols) return M3_ERR_UNSUPPORTED;
+    if (dtype != M3_DTYPE_F32 && dtype != M3_DTYPE_BF16) return M3_ERR_UNSUPPORTED;
+    return M3_OK;
+}
+static int check_swiglu(int64_t rows, int32_t d_model, int32_t d_ff, int32_t dtype) {
+    return check_product(rows, d_model, d_ff, 1 << 20, dtype);
+}
+static int check_xent(int64_t rows, int32_t d_model, int32_t vocab, int32_t dtype) {
+    return check_product(rows, d_model, vocab, (int64_t)1 << 30, dtype);
+}
+static int check_workspace(const void* ws, size_t have, size_t need) {
+    if (need == 0) return M3_OK;
+    if (!ws || have < need) return M3_ERR_WORKSPACE;
+    return aligned(ws, 256) ? M3_OK : M3_ERR_MISALIGNED;
+}
+
+int m3_swiglu_mlp_saved_size(int64_t rows, int32_t d_model, int32_t d_ff, int32_t dtype, size_t* bytes) {
+    if (!bytes) return M3_ERR_NULL_POINTER;
+    const int st = check_swiglu(rows, d_model, d_ff, dtype);
+    if (st == M3_OK) *bytes = m3::swiglu_saved(rows, d_model, d_ff, dtype);
+    return st;
+}
+
+int m3_swiglu_mlp_fwd_workspace_size(int64_t rows, int32_t d_model, int32_t d_ff, int32_t dtype,
+                                     int32_t keeps, size_t* bytes) {
+    if (!bytes) return M3_ERR_NULL_POINTER;
+    const int st = check_swiglu(rows, d_model, d_ff, dtype);
+    if (st == M3_OK) *bytes = m3::swiglu_fwd_workspace(rows, d_model, d_ff, dtype, keeps != 0);
+    return st;
+}
+
+int m3_swiglu_mlp_fwd(int64_t rows, int32_t d_model, int32_t d_ff, int32_t dtype, const void* x,
+                      const void* w_gate, const void* w_up, const void* w_down, const void* residual,
+                      float scale, void* y, void* saved, void* workspace, size_t workspace_bytes,
+                      void* stream) {
+    if (!x || !w_gate || !w_up || !w_down || !y) return M3_ERR_NULL_POINTER;
+    int st = check_swiglu(rows, d_model, d_ff, dtype);
+    if (st != M3_OK) return st;
+    if (!aligned(x, 16) || !aligned(w_gate, 16) || !aligned(w_up, 16) || !aligned(w_down, 16) ||
+        (saved && !aligned(saved, 256)))
+        return M3_ERR_MISALIGNED;
+    st = check_workspace(workspace, workspace_bytes,
+                         m3::swiglu_fwd_workspace(rows, d_model, d_ff, dtype, saved != nullptr));
+    if (st != M3_OK) return st;
+    return m3::launch_swiglu_fwd(rows, d_model, d_ff, dtype, x, w_gate, w_up, w_down, residual, scale, y,
+                                 saved, workspace, as_stream(stream));
+}
+
+int m3_swiglu_mlp_bwd_workspace_size(int64_t rows, int32_t d_model, int32_t d_ff, int32_t dtype,
+                                     size_t* bytes) {
+    if (!bytes) return M3_ERR_NULL_POINTER;
+    const int st = check_swiglu(rows, d_model, d_ff, dtype);
+    if (st == M3_OK) *bytes = m3::swiglu_bwd_workspace(rows, d_model, d_ff, dtype);
+    return st;
+}
+
+int m3_swiglu_mlp_bwd(int64_t rows, int32_t d_model, int32_t d_ff, int32_t dtype, const void* x,
+                      const void* w_gate, const void* w_up, const void* w_down, float scale,
+                      const void* saved, const void* dy, void* dx, void* dw_gate, void* dw_up,
+                      void* dw_down, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!x || !w_gate || !w_up || !w_down || !saved || !dy) return M3_ERR_NULL_POINTER;
+    int st = check_swiglu(rows, d_model, d_ff, dtype);
+    if (st != M3_OK) return st;
+    if (!aligned(x, 16) || !aligned(w_gate, 16) || !aligned(w_up, 16) || !aligned(w_down, 16) ||
+        !aligned(dy, 16) || !aligned(saved, 256))
+        return M3_ERR_MISALIGNED;
+    st = check_workspace(workspace, workspace_bytes, m3::swiglu_bwd_workspace(rows, d_model, d_ff, dtype));
+    if (st != M3_OK) return st;
+    return m3::launch_swiglu_bwd(rows, d_model, d_ff, dtype, x, w_gate, w_up, w_down, scale, saved, dy, dx,
+                                 dw_gate, dw_up, dw_down, workspace, as_stream(stream));
+}
+
+int m3_linear_xent_fwd_workspace_size(int64_t rows, int32_t d_model, int32_t vocab, int32_t dtype,
+                                      size_t* bytes) {
+    if (!bytes) return M3_ERR_NULL_POINTER;
+    const int st = check_xent(rows, d_model, vocab, dtype);
+    if (st == M3_OK) *bytes = m3::xent_fwd_workspace(rows, d_model, vocab, dtype);
+    return st;
+}
+
+int m3_linear_xent_fwd(int64_t rows, int32_t d_model, int32_t vocab, int32_t dtype, int32_t reduction,
+                       const void* hidden, const void* weight, const int64_t* target,
+                       int64_t ignore_index, float* loss, float* lse, float* count, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+    if (!hidden || !weight || !target || !loss || !lse || !count) return M3_ERR_NULL_POINTER;
+    int st = check_xent(rows, d_model, vocab, dtype);
+    if (st != M3_OK) return st;
+    if (reduction < M3_REDUCTION_NONE || reduction > M3_REDUCTION_SUM) return M3_ERR_INVALID_SHAPE;
+    if (!aligned(hidden, 16) || !aligned(weight, 16)) return M3_ERR_MISALIGNED;
+    st = check_workspace(workspace, workspace_bytes, m3::xent_fwd_workspace(rows, d_model, vocab, dtype));
+    if (st != M3_OK) return st;
+    return m3::launch_xent_fwd(rows, d_model, vocab, dtype, reduction, hidden, weight, target, ignore_index,
+                               loss, lse, count, workspace, as_stream(stream));
+}
+
+int m3_linear_xent_bwd_workspace_size(int64_t rows, int32_t d_model, int32_t vocab, int32_t dtype,
+                                      int32_t want_dhidden, int32_t want_dweight, size_t* bytes) {
+    if (!bytes) return M3_ERR_NULL_POINTER;
+    const int st = check_xent(rows, d_model, vocab, dtype);
+    if (st == M3_OK)
+        *bytes = m3::xent_bwd_workspace(rows, d_model, vocab, dtype, want_dhidden != 0, want_dweight != 0);
+    return st;
+}
+
+int m3_linear_xent_bwd(int64_t rows, int32_t d_model, int32_t vocab, int32_t dtype, int32_t reduction,
+                       const void* hidden, const void* weight, const int64_t* target,
+                       int64_t ignore_index, const float* lse, const float* count,
+                       const float* grad_loss, void* dhidden, void* dweight, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+    if (!hidden || !weight || !target || !lse || !count || !grad_loss) return M3_ERR_NULL_POINTER;
+    int st = check_xent(rows, d_model, vocab, dtype);
+    if (st != M3_OK) return st;
+    if (reduction < M3_REDUCTION_NONE || reduction > M3_REDUCTION_SUM) return M3_ERR_INVALID_SHAPE;
+    if (!aligned(hidden, 16) || !aligned(weight, 16)) return M3_ERR_MISALIGNED;
+    if (!dhidden && !dweight) return M3_OK;
+    st = check_workspace(workspace, workspace_bytes,
+                         m3::xent_bwd_workspace(rows, d_model, vocab, dtype, dhidden != nullptr, dweight != nullptr));
+    if (st != M3_OK) return st;
+    return m3::launch_xent_bwd(rows, d_model, vocab, dtype, reduction, hidden, weight, target, ignore_index,
+                               lse, count, grad_loss, dhidden, dweight, workspace, as_stream(stream));
+}
+
+static int check_tensors(int32_t n, const int64_t* numel, const int32_t* dtype) {
+    if (n < 0) return M3_ERR_INVALID_SHAPE;
+    if (n > 0 && (!numel || !dtype)) return M3_ERR_NULL_POINTER;
+    for (int i = 0; i < n; ++i) {
+        if (numel[i] < 0) return M3_ERR_INVALID_SHAPE;
+        if (dtype[i] != M3_DTYPE_F32 && dtype[i] != M3_DTYPE_BF16) return M3_ERR_UNSUPPORTED;
+        if (numel[i] > ((int64_t)1 << 36)) return M3_ERR_UNSUPPORTED;
+    }
+    return m3::clip_total_blocks(n, numel, dtype) <= 0x3fffffff ? M3_OK : M3_ERR_UNSUPPORTED;
+}
+
+int m3_clip_grad_norm_workspace_size(int32_t n, const int64_t* numel, const int32_t* dtype, size_t* bytes) {
+    if (!bytes) return M3_ERR_NULL_POINTER;
+    const int st = check_tensors(n, numel, dtype);
+    if (st == M3_OK) *bytes = 256 + 8 * (size_t)m3::clip_total_blocks(n, numel, dtype);
+    return st;
+}
+
+int m3_clip_grad_norm(int32_t n, void* const* tensors, const int64_t* numel, const int32_t* dtype,
+                      int32_t norm_kind, int32_t scale, float max_norm, float* norm, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+    if (!norm || (n > 0 && !tensors)) return M3_ERR_NULL_POINTER;
+    int st = check_tensors(n, numel, dtype);
+    if (st != M3_OK) return st;
+    if (norm_kind != M3_NORM_L2 && norm_kind != M3_NORM_MAX) return M3_ERR_UNSUPPORTED;
+    for (int i = 0; i < n; ++i) {
+        if (numel[i] == 0) continue;
+        if (!tensors[i]) return M3_ERR_NULL_POINTER;
+        if (!aligned(tensors[i], dtype[i] == M3_DTYPE_BF16 ? 2 : 4)) return M3_ERR_MISALIGNED;
+    }
+    st = check_workspace(workspace, workspace_bytes, 256 + 8 * (size_t)m3::clip_total_blocks(n, numel, dtype));
+    if (st != M3_OK) return st;
+    return m3::launch_clip(n, tensors, numel, dtype, norm_kind == M3_NORM_MAX, scale != 0, max_norm, norm,
+                           workspace, as_stream(stream));
+}
+
 }  // extern "C"

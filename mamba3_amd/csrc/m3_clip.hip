@@ -1,0 +1,216 @@
+// The norm of many tensors together and their scaling by it (gfx950), for gradients before an
+// optimiser's step:
+//   norm = (sum over all elements of g^2)^(1/2) or max |g|;  g <- g * min(1, max_norm / (norm + 1e-6)).
+// Bound by HBM: one read for the norm, one read and write for the scaling. A launch takes the
+// pointers and sizes of up to kClipTensors tensors in its arguments (no table in device memory, so
+// a call allocates and copies nothing and can be captured), and its blocks walk pieces of kClipPiece
+// bytes that a tensor's blocks share out in order. Squares are added in fp64 (bound by memory all
+// the same): no overflow for gradients past 2^64, and no order to choose; a block's sum, then all
+// blocks' sums, are added in a fixed order.
+#include <algorithm>
+
+#include "m3_common.h"
+#include "m3_kernels.h"
+#include "mamba3_amd.h"
+
+namespace m3 {
+
+constexpr int kClipThreads = 256;
+constexpr int kClipTensors = 144;
+constexpr int64_t kClipPiece = 128 << 10;
+
+struct ClipTensors {
+    void* p[kClipTensors];
+    int64_t n[kClipTensors];      // elements
+    int first[kClipTensors + 1];  // first block of each; [count] the number of blocks
+    int count;
+    int block0;                   // blocks of earlier launches
+};
+
+// The tensor of this block, and its elements [begin, end) there.
+template <typename T>
+__device__ __forceinline__ int clip_piece(const ClipTensors& t, int64_t& begin, int64_t& end) {
+    const int b = (int)blockIdx.x;
+    int lo = 0, hi = t.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (t.first[mid] <= b) lo = mid;
+        else hi = mid - 1;
+    }
+    constexpr int64_t per = kClipPiece / (int64_t)sizeof(T);
+    begin = (int64_t)(b - t.first[lo]) * per;
+    end = begin + per < t.n[lo] ? begin + per : t.n[lo];
+    return lo;
+}
+
+template <bool kInf>
+__device__ __forceinline__ double clip_join(double a, double b) {
+    if constexpr (kInf) return (b <= a) || a != a ? a : b;  // NaN on either side stays
+    else return a + b;
+}
+template <bool kInf>
+__device__ __forceinline__ void clip_add(double& acc, float v) {
+    if constexpr (kInf) acc = clip_join<true>(acc, fabs((double)v));
+    else acc = fma((double)v, (double)v, acc);
+}
+
+template <bool kInf>
+__device__ __forceinline__ double clip_block(double v, double* red) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v = clip_join<kInf>(v, __shfl_xor(v, off, kWave));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll
+    for (int w = 1; w < kClipThreads / 64; ++w) v = clip_join<kInf>(v, red[w]);
+    return v;
+}
+
+template <typename T, bool kInf>
+__global__ __launch_bounds__(kClipThreads) void clip_norm_kernel(ClipTensors t, double* __restrict__ part) {
+    constexpr int E = 16 / sizeof(T);
+    typedef T Piece __attribute__((ext_vector_type(E)));
+    __shared__ double red[kClipThreads / 64];
+    int64_t begin, end;
+    const int k = clip_piece<T>(t, begin, end);
+    const T* p = reinterpret_cast<const T*>(t.p[k]) + begin;
+    const int n = (int)(end - begin);
+    // single elements up to the first 16-byte border and behind the last
+    int head = (int)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / (int)sizeof(T);
+    head = head < n ? head : n;
+    const int pieces = (n - head) / E, tail = head + pieces * E;
+    double acc[2] = {0.0, 0.0};
+    for (int i = threadIdx.x; i < head; i += kClipThreads) clip_add<kInf>(acc[0], (float)p[i]);
+    const Piece* q = reinterpret_cast<const Piece*>(p + head);
+#pragma unroll 8
+    for (int i = threadIdx.x; i < pieces; i += kClipThreads) {
+        const Piece v = q[i];
+#pragma unroll
+        for (int e = 0; e < E; ++e) clip_add<kInf>(acc[e & 1], (float)v[e]);
+    }
+    for (int i = tail + threadIdx.x; i < n; i += kClipThreads) clip_add<kInf>(acc[1], (float)p[i]);
+    const double v = clip_block<kInf>(clip_join<kInf>(acc[0], acc[1]), red);
+    if (threadIdx.x == 0) part[t.block0 + blockIdx.x] = v;
+}
+
+// The blocks' sums -> norm and, with a bound, the factor. One block.
+template <bool kInf>
+__global__ __launch_bounds__(kClipThreads) void clip_total_kernel(const double* __restrict__ part, int n, float max_norm,
+                                                                  float* __restrict__ norm, float* __restrict__ factor) {
+    __shared__ double red[kClipThreads / 64];
+    double v = 0.0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += kClipThreads) v = clip_join<kInf>(v, part[i]);
+    v = clip_block<kInf>(v, red);
+    if (threadIdx.x == 0) {
+        if constexpr (!kInf) v = sqrt(v);
+        norm[0] = (float)v;
+        if (factor) {
+            const double f = (double)max_norm / (v + 1e-6);
+            factor[0] = f > 1.0 ? 1.f : (float)f;  // NaN stays
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(ClipTensors t, const float* __restrict__ factor) {
+    constexpr int E = 16 / sizeof(T);
+    typedef T Piece __attribute__((ext_vector_type(E)));
+    const float f = factor[0];
+    if (f == 1.f) return;  // within the bound: every element stays as it is
+    int64_t begin, end;
+    const int k = clip_piece<T>(t, begin, end);
+    T* p = reinterpret_cast<T*>(t.p[k]) + begin;
+    const int n = (int)(end - begin);
+    int head = (int)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / (int)sizeof(T);
+    head = head < n ? head : n;
+    const int pieces = (n - head) / E, tail = head + pieces * E;
+    for (int i = threadIdx.x; i < head; i += kClipThreads) p[i] = (T)((float)p[i] * f);
+    Piece* q = reinterpret_cast<Piece*>(p + head);
+#pragma unroll 8
+    for (int i = threadIdx.x; i < pieces; i += kClipThreads) {
+        Piece v = q[i];
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = (T)((float)v[e] * f);
+        q[i] = v;
+    }
+    for (int i = tail + threadIdx.x; i < n; i += kClipThreads) p[i] = (T)((float)p[i] * f);
+}
+
+static int64_t clip_blocks(int64_t numel, int dtype) {
+    const int64_t per = kClipPiece / (dtype == M3_DTYPE_BF16 ? 2 : 4);
+    return (numel + per - 1) / per;
+}
+
+// Calls `f(tensors, dtype)` for groups of up to kClipTensors non-empty tensors of one type.
+template <typename F>
+static int clip_groups(int n, void* const* p, const int64_t* numel, const int32_t* dtype, F f) {
+    int block0 = 0;
+    for (int type : {M3_DTYPE_F32, M3_DTYPE_BF16}) {
+        ClipTensors t;
+        t.count = 0;
+        t.block0 = block0;
+        int blocks = 0;
+        auto flush = [&]() -> int {
+            if (t.count == 0) return M3_OK;
+            t.first[t.count] = blocks;
+            const int st = f(t, type, blocks);
+            block0 += blocks;
+            t.count = 0, t.block0 = block0, blocks = 0;
+            return st;
+        };
+        for (int i = 0; i < n; ++i) {
+            if (dtype[i] != type || numel[i] == 0) continue;
+            if (t.count == kClipTensors || blocks + clip_blocks(numel[i], type) > (1 << 23)) {
+                const int st = flush();
+                if (st != M3_OK) return st;
+            }
+            t.p[t.count] = p[i];
+            t.n[t.count] = numel[i];
+            t.first[t.count] = blocks;
+            blocks += (int)clip_blocks(numel[i], type);
+            ++t.count;
+        }
+        const int st = flush();
+        if (st != M3_OK) return st;
+    }
+    return M3_OK;
+}
+
+int64_t clip_total_blocks(int n, const int64_t* numel, const int32_t* dtype) {
+    int64_t blocks = 0;
+    for (int i = 0; i < n; ++i) blocks += clip_blocks(numel[i], dtype[i]);
+    return blocks;
+}
+
+static int clip_status() { return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH; }
+
+int launch_clip(int n, void* const* p, const int64_t* numel, const int32_t* dtype, bool inf_norm, bool scale,
+                float max_norm, float* norm, void* ws, hipStream_t stream) {
+    float* factor = reinterpret_cast<float*>(ws);
+    double* part = reinterpret_cast<double*>(reinterpret_cast<char*>(ws) + 256);
+    int st = clip_groups(n, p, numel, dtype, [&](const ClipTensors& t, int type, int blocks) {
+        const dim3 grid((unsigned)blocks), block(kClipThreads);
+        if (type == M3_DTYPE_BF16) {
+            if (inf_norm) hipLaunchKernelGGL((clip_norm_kernel<bf16, true>), grid, block, 0, stream, t, part);
+            else hipLaunchKernelGGL((clip_norm_kernel<bf16, false>), grid, block, 0, stream, t, part);
+        } else {
+            if (inf_norm) hipLaunchKernelGGL((clip_norm_kernel<float, true>), grid, block, 0, stream, t, part);
+            else hipLaunchKernelGGL((clip_norm_kernel<float, false>), grid, block, 0, stream, t, part);
+        }
+        return clip_status();
+    });
+    if (st != M3_OK) return st;
+    const int blocks = (int)clip_total_blocks(n, numel, dtype);
+    if (inf_norm) hipLaunchKernelGGL((clip_total_kernel<true>), dim3(1), dim3(kClipThreads), 0, stream, part, blocks, max_norm, norm, scale ? factor : nullptr);
+    else hipLaunchKernelGGL((clip_total_kernel<false>), dim3(1), dim3(kClipThreads), 0, stream, part, blocks, max_norm, norm, scale ? factor : nullptr);
+    if ((st = clip_status()) != M3_OK || !scale) return st;
+    return clip_groups(n, p, numel, dtype, [&](const ClipTensors& t, int type, int blocks) {
+        const dim3 grid((unsigned)blocks), block(kClipThreads);
+        if (type == M3_DTYPE_BF16) hipLaunchKernelGGL((clip_scale_kernel<bf16>), grid, block, 0, stream, t, factor);
+        else hipLaunchKernelGGL((clip_scale_kernel<float>), grid, block, 0, stream, t, factor);
+        return clip_status();
+    });
+}
+
+}  // namespace m3

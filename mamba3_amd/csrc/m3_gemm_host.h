@@ -1,0 +1,104 @@
+// Host side of the tiled products: tile and split choice, launches (m3_gemm.h).
+#pragma once
+
+#include <algorithm>
+
+#include "m3_gemm.h"
+
+namespace m3 {
+
+// Tiles: 256 x 256 by 8 waves (bf16 only; one block a CU), 128 x 128 by 4 waves (two blocks a
+// CU), 64 x 64 by 4 waves, four steps deep (two blocks a CU).
+typedef GemmTile<256, 256, 2, 4, 2> TileL;
+typedef GemmTile<128, 128, 2, 2, 2> TileM;
+typedef GemmTile<64, 64, 2, 2, 4> TileS;
+enum { kTileL = 0, kTileM = 1, kTileS = 2 };
+
+struct GemmPlan {
+    int tile;
+    int splits;
+    int bm, bn;
+};
+
+// The tile and the number of k parts with the least estimated time. rows x cols: C (for a
+// gated product, cols counts both halves); steps: k steps of 128 bytes; batch: products in one
+// launch; max_splits: 1 where the epilogue needs the whole sum.
+GemmPlan gemm_plan(int dtype, int64_t rows, int64_t cols, int64_t steps, int batch, int max_splits);
+
+inline int64_t gemm_steps(int64_t k, int dtype) {
+    const int bk = dtype == M3_DTYPE_BF16 ? 64 : 32;
+    return (k + bk - 1) / bk;
+}
+inline int64_t gemm_pad(int64_t n, int dtype) {  // to 16 bytes
+    const int e = dtype == M3_DTYPE_BF16 ? 8 : 4;
+    return (n + e - 1) / e * e;
+}
+inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+
+template <typename T, typename Tile, bool kAKc, bool kBKc, int kMode, typename Epi>
+int gemm_launch(GemmArgs a, const Epi& epi, int64_t rows, int64_t cols, int batch, hipStream_t stream) {
+    a.tiles_m = (int)((rows + Tile::BM - 1) / Tile::BM);
+    a.tiles_n = (int)((cols + Tile::BN - 1) / Tile::BN);
+    const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
+    if (tiles * Tile::NT >= ((int64_t)1 << 32)) return M3_ERR_UNSUPPORTED;
+    auto* k = gemm_kernel<T, Tile, kAKc, kBKc, kMode, Epi>;
+    if (Tile::kLds > 64 * 1024 &&
+        hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, Tile::kLds) != hipSuccess)
+        return M3_ERR_LAUNCH;
+    hipLaunchKernelGGL(k, dim3((unsigned)tiles, (unsigned)batch, (unsigned)a.splits), dim3(Tile::NT), Tile::kLds, stream, a, epi);
+    return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH;
+}
+
+template <bool kAKc, bool kBKc, int kMode, typename Epi>
+int gemm_dispatch(int dtype, const GemmPlan& p, const GemmArgs& a, const Epi& epi, int64_t rows, int64_t cols,
+                  int batch, hipStream_t stream) {
+    if (dtype == M3_DTYPE_BF16) {
+        if (p.tile == kTileL) return gemm_launch<bf16, TileL, kAKc, kBKc, kMode>(a, epi, rows, cols, batch, stream);
+        if (p.tile == kTileM) return gemm_launch<bf16, TileM, kAKc, kBKc, kMode>(a, epi, rows, cols, batch, stream);
+        return gemm_launch<bf16, TileS, kAKc, kBKc, kMode>(a, epi, rows, cols, batch, stream);
+    }
+    if (p.tile == kTileM) return gemm_launch<float, TileM, kAKc, kBKc, kMode>(a, epi, rows, cols, batch, stream);
+    return gemm_launch<float, TileS, kAKc, kBKc, kMode>(a, epi, rows, cols, batch, stream);
+}
+
+// Stores a product (m3_gemm_store.hip): out[z] (rows x cols, row stride ldo) = alpha * (A B) [+ res],
+// or, split or accumulated over calls, fp32 partial sums in `part` that gemm_reduce joins.
+struct GemmStore {
+    void* out[2];
+    int64_t ldo;
+    const void* res;  // rows x cols, row stride ldo, or nullptr
+    float alpha;
+    float* part;      // [splits][batch][rows][cols]
+    int add;          // the partial sums of an earlier call stay in `part`
+    int rows, cols;
+};
+enum GemmForm {
+    kFormNT,  // A rows of k, B rows of k
+    kFormNN,  // A rows of k, B [k][n], one or two terms
+    kFormTN   // A [k][m], B [k][n], `batch` products
+};
+int gemm_store(GemmForm form, int dtype, const GemmPlan& p, GemmArgs a, const GemmStore& st, int batch,
+               hipStream_t stream);
+// out[z] = alpha * sum over s of part[s][z] [+ res]
+int gemm_reduce(int dtype, const GemmStore& st, int splits, int batch, hipStream_t stream);
+inline size_t gemm_part_bytes(const GemmPlan& p, int batch, int64_t rows, int64_t cols) {
+    return p.splits > 1 ? (size_t)up256((int64_t)p.splits * batch * rows * cols * 4) : 0;
+}
+// dst [rows][ldd] = src [rows][cols] with zeros in the columns past cols; rows whose target is
+// `ignore` are zero where a target is given. ldd * size is a multiple of 16.
+int gemm_pad_copy(int dtype, const void* src, void* dst, int64_t rows, int64_t cols, int64_t ldd,
+                  const int64_t* target, int64_t ignore, hipStream_t stream);
+
+inline GemmArgs gemm_args(GemmOp a, GemmOp b, int64_t m, int64_t n, int64_t k, int splits) {
+    GemmArgs g;
+    g.a[0] = g.a[1] = a;
+    g.b[0] = g.b[1] = b;
+    g.M = (int)m, g.N = (int)n;
+    g.K[0] = g.KB[0] = (int)k;
+    g.K[1] = g.KB[1] = 0;
+    g.splits = splits;
+    g.tiles_m = g.tiles_n = 0;
+    return g;
+}
+
+}  // namespace m3

@@ -1,0 +1,193 @@
+// Products whose result is stored as it is (m3_gemm.h): the MLP's down projection with its
+// residual, the input and weight gradients, and the joining of partial sums.
+#include "m3_gemm_host.h"
+#include "m3_kernels.h"
+
+namespace m3 {
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, f32x4 v) {
+    if constexpr (sizeof(T) == 2) {
+        bf16x4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (bf16)v[e];
+        *reinterpret_cast<bf16x4*>(p) = o;
+    } else {
+        *reinterpret_cast<f32x4*>(p) = v;
+    }
+}
+
+struct EpiStore {
+    GemmStore s;
+    bool vec;  // four columns at once
+
+    template <typename T, typename Tile, int kMode>
+    __device__ __forceinline__ void run(const GemmArgs& a, const GemmPlace<Tile, kMode>& at,
+                                        f32x4 (&acc)[Tile::FM][Tile::FN], char*, int, int, int z) const {
+        T* out = reinterpret_cast<T*>(s.out[z]);
+        const T* res = reinterpret_cast<const T*>(s.res);
+        float* part = s.part ? s.part + ((int64_t)blockIdx.z * gridDim.y + z) * s.rows * s.cols : nullptr;
+#pragma unroll
+        for (int i = 0; i < Tile::FM; ++i) {
+            const int m = at.m(i);
+            if (m >= s.rows) continue;
+#pragma unroll
+            for (int j = 0; j < Tile::FN; ++j) {
+                const int n = at.n(j);
+                if (n >= s.cols) continue;
+                f32x4 v = acc[i][j];
+                if (part) {
+                    float* p = part + (int64_t)m * s.cols + n;
+                    if (vec) {
+                        if (s.add) v += *reinterpret_cast<const f32x4*>(p);
+                        *reinterpret_cast<f32x4*>(p) = v;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (n + e < s.cols) p[e] = s.add ? p[e] + v[e] : v[e];
+                    }
+                    continue;
+                }
+                const int64_t o = (int64_t)m * s.ldo + n;
+                if (vec) {
+                    v *= s.alpha;
+                    if (res) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] += (float)res[o + e];
+                    }
+                    store4(out + o, v);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (n + e < s.cols) out[o + e] = (T)(v[e] * s.alpha + (res ? (float)res[o + e] : 0.f));
+                }
+            }
+        }
+    }
+};
+
+static bool four_columns(const GemmStore& s) {
+    auto al = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    return s.cols % 4 == 0 && s.ldo % 4 == 0 && al(s.out[0]) && al(s.out[1]) && al(s.res);
+}
+
+int gemm_store(GemmForm form, int dtype, const GemmPlan& p, GemmArgs a, const GemmStore& st, int batch,
+               hipStream_t stream) {
+    a.splits = p.splits;
+    EpiStore e{st, four_columns(st)};
+    if (p.splits == 1 && !st.add && st.out[0]) e.s.part = nullptr;
+    int r;
+    if (form == kFormNT) r = gemm_dispatch<true, true, kPlain>(dtype, p, a, e, st.rows, st.cols, 1, stream);
+    else if (form == kFormNN) r = gemm_dispatch<true, false, kSeg2>(dtype, p, a, e, st.rows, st.cols, 1, stream);
+    else r = gemm_dispatch<false, false, kBatch2>(dtype, p, a, e, st.rows, st.cols, batch, stream);
+    if (r != M3_OK || !e.s.part || !st.out[0]) return r;
+    return gemm_reduce(dtype, st, p.splits, batch, stream);
+}
+
+// One thread joins four columns of a row; parts are added in order.
+template <typename T, bool kVec>
+__global__ __launch_bounds__(256) void gemm_reduce_kernel(GemmStore s, int splits) {
+    const int z = blockIdx.y;
+    const int64_t each = (int64_t)s.rows * s.cols, stride = each * gridDim.y;
+    const float* part = s.part + z * each;
+    T* out = reinterpret_cast<T*>(s.out[z]);
+    const T* res = reinterpret_cast<const T*>(s.res);
+    const int64_t pieces = kVec ? each / 4 : each;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * 256) {
+        const int64_t at = kVec ? i * 4 : i;
+        const int64_t m = at / s.cols, o = m * s.ldo + (at - m * s.cols);
+        if constexpr (kVec) {
+            f32x4 v{0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < splits; ++k) v += *reinterpret_cast<const f32x4*>(part + k * stride + at);
+            v *= s.alpha;
+            if (res)
+                for (int e = 0; e < 4; ++e) v[e] += (float)res[o + e];
+            store4(out + o, v);
+        } else {
+            float v = 0.f;
+            for (int k = 0; k < splits; ++k) v += part[k * stride + at];
+            out[o] = (T)(v * s.alpha + (res ? (float)res[o] : 0.f));
+        }
+    }
+}
+
+int gemm_reduce(int dtype, const GemmStore& st, int splits, int batch, hipStream_t stream) {
+    const bool vec = four_columns(st);
+    const int64_t pieces = (int64_t)st.rows * st.cols / (vec ? 4 : 1);
+    const dim3 grid((unsigned)std::min<int64_t>((pieces + 255) / 256, 8192), (unsigned)batch);
+    if (dtype == M3_DTYPE_BF16) {
+        if (vec) hipLaunchKernelGGL((gemm_reduce_kernel<bf16, true>), grid, dim3(256), 0, stream, st, splits);
+        else hipLaunchKernelGGL((gemm_reduce_kernel<bf16, false>), grid, dim3(256), 0, stream, st, splits);
+    } else {
+        if (vec) hipLaunchKernelGGL((gemm_reduce_kernel<float, true>), grid, dim3(256), 0, stream, st, splits);
+        else hipLaunchKernelGGL((gemm_reduce_kernel<float, false>), grid, dim3(256), 0, stream, st, splits);
+    }
+    return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH;
+}
+
+// One thread writes 16 bytes of a row; src rows of whole, aligned pieces are read the same way.
+template <typename T>
+__global__ __launch_bounds__(256) void gemm_pad_kernel(const T* __restrict__ src, T* __restrict__ dst, int64_t rows,
+                                                       int cols, int ldd, const int64_t* __restrict__ target,
+                                                       int64_t ignore) {
+    constexpr int E = 16 / sizeof(T);
+    typedef T Piece __attribute__((ext_vector_type(E)));
+    const int per = ldd / E;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per;
+        const int c = (int)(i - r * per) * E;
+        Piece v;
+        if (target && target[r] == ignore) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = (T)0.f;
+        } else if (cols % E == 0) {
+            v = *reinterpret_cast<const Piece*>(src + r * cols + c);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = c + e < cols ? src[r * cols + c + e] : (T)0.f;
+        }
+        *reinterpret_cast<Piece*>(dst + r * ldd + c) = v;
+    }
+}
+
+int gemm_pad_copy(int dtype, const void* src, void* dst, int64_t rows, int64_t cols, int64_t ldd,
+                  const int64_t* target, int64_t ignore, hipStream_t stream) {
+    const int64_t pieces = rows * (ldd / (dtype == M3_DTYPE_BF16 ? 8 : 4));
+    const dim3 grid((unsigned)std::min<int64_t>((pieces + 255) / 256, 16384));
+    if (dtype == M3_DTYPE_BF16)
+        hipLaunchKernelGGL(gemm_pad_kernel<bf16>, grid, dim3(256), 0, stream, reinterpret_cast<const bf16*>(src),
+                           reinterpret_cast<bf16*>(dst), rows, (int)cols, (int)ldd, target, ignore);
+    else
+        hipLaunchKernelGGL(gemm_pad_kernel<float>, grid, dim3(256), 0, stream, reinterpret_cast<const float*>(src),
+                           reinterpret_cast<float*>(dst), rows, (int)cols, (int)ldd, target, ignore);
+    return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH;
+}
+
+GemmPlan gemm_plan(int dtype, int64_t rows, int64_t cols, int64_t steps, int batch, int max_splits) {
+    // us of one k step of a tile alone on its CU, and of as many as run at once
+    struct Cost { int bm, bn, at_once; double one, all, fixed; };
+    static const Cost bf[3] = {{256, 256, 1, 1.9, 1.9, 6.0}, {128, 128, 2, 0.65, 1.0, 4.0}, {64, 64, 2, 0.30, 0.41, 3.0}};
+    static const Cost fp[3] = {{0, 0, 0, 0, 0, 0}, {128, 128, 2, 2.0, 3.9, 4.0}, {64, 64, 2, 0.6, 1.1, 3.0}};
+    const Cost* c = dtype == M3_DTYPE_BF16 ? bf : fp;
+    GemmPlan best{kTileS, 1, 64, 64};
+    double least = 1e30;
+    for (int t = dtype == M3_DTYPE_BF16 ? kTileL : kTileM; t <= kTileS; ++t) {
+        const int64_t tiles = ((rows + c[t].bm - 1) / c[t].bm) * ((cols + c[t].bn - 1) / c[t].bn) * batch;
+        for (int s = 1; s <= max_splits && s <= steps; ++s) {
+            const int64_t blocks = tiles * s;
+            const int64_t slots = (int64_t)256 * c[t].at_once;
+            const double per = (double)((steps + s - 1) / s);
+            const int64_t rounds = blocks / slots, rest = blocks % slots;
+            double us = rounds * (per * c[t].all + c[t].fixed);
+            if (rest) us += per * (rest > 256 ? c[t].all : c[t].one) + c[t].fixed;
+            if (s > 1) us += 4.0 + (double)rows * cols * batch * 8.0 * s / 4.0e6;
+            if (us < least) {
+                least = us;
+                best = GemmPlan{t, s, c[t].bm, c[t].bn};
+            }
+        }
+    }
+    return best;
+}
+
+}  // namespace m3

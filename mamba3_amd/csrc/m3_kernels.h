@@ -196,6 +196,38 @@ int launch_rmsnorm_bwd(const void* x, int xdtype, const void* w, int wdtype, con
                        const void* g, int gdtype, void* dx, void* dw, void* workspace,
                        int64_t rows, int d, hipStream_t stream);
 
+// The gated MLP with its residual (m3_mlp.hip): bytes of what the forward keeps for the backward
+// (saved), of the workspaces (the forward's without `saved` also holds h), and launchers
+// (m3_status).
+size_t swiglu_saved(int64_t rows, int64_t d, int64_t ff, int dtype);
+size_t swiglu_fwd_workspace(int64_t rows, int64_t d, int64_t ff, int dtype, bool keeps);
+size_t swiglu_bwd_workspace(int64_t rows, int64_t d, int64_t ff, int dtype);
+int launch_swiglu_fwd(int64_t rows, int64_t d, int64_t ff, int dtype, const void* x, const void* wg,
+                      const void* wu, const void* wd, const void* res, float scale, void* y,
+                      void* saved, void* ws, hipStream_t stream);
+int launch_swiglu_bwd(int64_t rows, int64_t d, int64_t ff, int dtype, const void* x, const void* wg,
+                      const void* wu, const void* wd, float scale, const void* saved,
+                      const void* dy, void* dx, void* dwg, void* dwu, void* dwd, void* ws,
+                      hipStream_t stream);
+
+// Cross entropy of a vocabulary projection (m3_xent.hip): workspace bytes and launchers
+// (m3_status).
+size_t xent_fwd_workspace(int64_t rows, int64_t d, int64_t vocab, int dtype);
+size_t xent_bwd_workspace(int64_t rows, int64_t d, int64_t vocab, int dtype, bool want_dh, bool want_dw);
+int launch_xent_fwd(int64_t rows, int64_t d, int64_t vocab, int dtype, int reduction,
+                    const void* hidden, const void* weight, const int64_t* target, int64_t ignore,
+                    float* loss, float* lse, float* count, void* ws, hipStream_t stream);
+int launch_xent_bwd(int64_t rows, int64_t d, int64_t vocab, int dtype, int reduction,
+                    const void* hidden, const void* weight, const int64_t* target, int64_t ignore,
+                    const float* lse, const float* count, const float* grad_loss, void* dhidden,
+                    void* dweight, void* ws, hipStream_t stream);
+
+// Norm over many tensors and their scaling (m3_clip.hip): blocks of one pass (8 bytes of
+// workspace each, behind 256) and launcher (m3_status).
+int64_t clip_total_blocks(int n, const int64_t* numel, const int32_t* dtype);
+int launch_clip(int n, void* const* p, const int64_t* numel, const int32_t* dtype, bool inf_norm,
+                bool scale, float max_norm, float* norm, void* ws, hipStream_t stream);
+
 // Returns 1 when the step kernel supports (N, R), else 0.
 int step_supported(int N, int R);
 int launch_step(const m3_layer_desc& d, const m3_layer_params& p, const void* proj,

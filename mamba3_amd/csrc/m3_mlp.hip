@@ -1,0 +1,301 @@
+// The gated MLP of a residual block and its backward (gfx950):
+//   g = x Wg^T, u = x Wu^T, h = silu(g) * u, y = [res +] s (h Wd^T)
+//   dh = s dy Wd, du = dh silu(g), dg = dh u silu'(g), silu'(g) = sig(g) (1 + g (1 - sig(g)))
+//   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = s dy^T h
+// on the tiled products of m3_gemm.h. Both projections, the activation and the product are one
+// kernel: a tile holds the gate and the up columns of the same hidden units, so g and u meet in
+// a lane's registers in fp32 and only h is stored. The backward's dh is never stored either: its
+// epilogue reads g and u and writes dg and du, the operands of the four gradient products (dx
+// is one product of two terms; dWg and dWu are one launch).
+//
+// For the backward the forward keeps g and u. bf16: their upper 24 bits as three planes of
+// 16 bits (g's upper 16, u's upper 16, the next 8 of both): a bf16 copy alone would put a rounding
+// of g and one of u (2^-9 each) into dg and du next to their own; 24 bits leave 2^-16 for 2 more
+// bytes an element. fp32: as they are.
+#include "m3_gemm_host.h"
+#include "m3_kernels.h"
+
+namespace m3 {
+
+typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
+
+template <typename T> __device__ __forceinline__ float sigmoid_of(float g);
+template <> __device__ __forceinline__ float sigmoid_of<bf16>(float g) { return __builtin_amdgcn_rcpf(1.f + fast_exp(-g)); }
+template <> __device__ __forceinline__ float sigmoid_of<float>(float g) { return sigmoid_f(g); }
+
+template <typename T>
+__device__ __forceinline__ void keep_gu(void* saved, int64_t at, int64_t plane, f32x4 g, f32x4 u) {
+    if constexpr (sizeof(T) == 2) {
+        unsigned short* p = reinterpret_cast<unsigned short*>(saved) + at;
+        u16x4 gh, uh, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            // (__builtin_bit_cast of a vector's component takes component 0 on this compiler)
+            const float ge = g[e], ue = u[e];
+            const unsigned gb = __builtin_bit_cast(unsigned, ge), ub = __builtin_bit_cast(unsigned, ue);
+            gh[e] = (unsigned short)(gb >> 16);
+            uh[e] = (unsigned short)(ub >> 16);
+            lo[e] = (unsigned short)((gb >> 8 & 0xff) | (ub & 0xff00));
+        }
+        *reinterpret_cast<u16x4*>(p) = gh;
+        *reinterpret_cast<u16x4*>(p + plane) = uh;
+        *reinterpret_cast<u16x4*>(p + 2 * plane) = lo;
+    } else {
+        float* p = reinterpret_cast<float*>(saved) + at;
+        *reinterpret_cast<f32x4*>(p) = g;
+        *reinterpret_cast<f32x4*>(p + plane) = u;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void kept_gu(const void* saved, int64_t at, int64_t plane, f32x4& g, f32x4& u) {
+    if constexpr (sizeof(T) == 2) {
+        const unsigned short* p = reinterpret_cast<const unsigned short*>(saved) + at;
+        const u16x4 gh = *reinterpret_cast<const u16x4*>(p), uh = *reinterpret_cast<const u16x4*>(p + plane),
+                    lo = *reinterpret_cast<const u16x4*>(p + 2 * plane);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            g[e] = __builtin_bit_cast(float, (unsigned)gh[e] << 16 | (lo[e] & 0xffu) << 8);
+            u[e] = __builtin_bit_cast(float, (unsigned)uh[e] << 16 | (lo[e] & 0xff00u));
+        }
+    } else {
+        const float* p = reinterpret_cast<const float*>(saved) + at;
+        g = *reinterpret_cast<const f32x4*>(p);
+        u = *reinterpret_cast<const f32x4*>(p + plane);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void put4(T* p, f32x4 v) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (T)v[e];
+    *reinterpret_cast<T4*>(p) = o;
+}
+
+// Columns come in fours: the hidden width is padded to 16 bytes, its pad columns are zero (their
+// weight rows read as zero) and are stored as zeros.
+struct EpiGated {
+    void* h;      // rows x ldh
+    void* saved;  // nullptr: no backward
+    int rows, ldh;
+
+    template <typename T, typename Tile, int kMode>
+    __device__ __forceinline__ void run(const GemmArgs&, const GemmPlace<Tile, kMode>& at,
+                                        f32x4 (&acc)[Tile::FM][Tile::FN], char*, int, int, int) const {
+        const int64_t plane = (int64_t)rows * ldh;
+#pragma unroll
+        for (int i = 0; i < Tile::FM; ++i) {
+            const int m = at.m(i);
+            if (m >= rows) continue;
+#pragma unroll
+            for (int j = 0; j < Tile::FN / 2; ++j) {
+                const int n = at.n(j);
+                if (n >= ldh) continue;
+                const f32x4 g = acc[i][j], u = acc[i][j + Tile::FN / 2];
+                const int64_t o = (int64_t)m * ldh + n;
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = g[e] * sigmoid_of<T>(g[e]) * u[e];
+                put4(reinterpret_cast<T*>(h) + o, v);
+                if (saved) keep_gu<T>(saved, o, plane, g, u);
+            }
+        }
+    }
+};
+
+struct EpiGateBwd {
+    void *dg, *du;
+    const void* saved;
+    float alpha;
+    int rows, ldh;
+
+    template <typename T, typename Tile, int kMode>
+    __device__ __forceinline__ void run(const GemmArgs&, const GemmPlace<Tile, kMode>& at,
+                                        f32x4 (&acc)[Tile::FM][Tile::FN], char*, int, int, int) const {
+        const int64_t plane = (int64_t)rows * ldh;
+#pragma unroll
+        for (int i = 0; i < Tile::FM; ++i) {
+            const int m = at.m(i);
+            if (m >= rows) continue;
+#pragma unroll
+            for (int j = 0; j < Tile::FN; ++j) {
+                const int n = at.n(j);
+                if (n >= ldh) continue;
+                const int64_t o = (int64_t)m * ldh + n;
+                f32x4 g, u, a, b;
+                kept_gu<T>(saved, o, plane, g, u);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float s = sigmoid_of<T>(g[e]), dh = acc[i][j][e] * alpha;
+                    a[e] = dh * u[e] * s * (1.f + g[e] * (1.f - s));
+                    b[e] = dh * g[e] * s;
+                }
+                put4(reinterpret_cast<T*>(dg) + o, a);
+                put4(reinterpret_cast<T*>(du) + o, b);
+            }
+        }
+    }
+};
+
+namespace {
+
+constexpr int kMaxSplits = 16;
+
+struct MlpShape {
+    int64_t rows, d, ff, dp, fp;
+    int dtype;
+    int64_t size;
+    bool pad_d, pad_f;  // rows of d (ff) are not whole 16-byte pieces
+};
+MlpShape mlp_shape(int64_t rows, int64_t d, int64_t ff, int dtype) {
+    MlpShape s{rows, d, ff, gemm_pad(d, dtype), gemm_pad(ff, dtype), dtype, dtype == M3_DTYPE_BF16 ? 2 : 4, false, false};
+    s.pad_d = s.dp != d, s.pad_f = s.fp != ff;
+    return s;
+}
+
+// A running pointer through the workspace.
+struct Bump {
+    char* p;
+    size_t used = 0;
+    void* take(int64_t bytes) {
+        void* r = p ? p + used : nullptr;
+        used += (size_t)up256(bytes);
+        return r;
+    }
+};
+
+struct MlpFwd {
+    GemmPlan up, down;
+    void *x, *wg, *wu, *wd, *h;
+    float* part;
+    size_t bytes;
+};
+MlpFwd mlp_fwd_layout(const MlpShape& s, bool keeps_h, void* ws) {
+    MlpFwd f;
+    Bump b{reinterpret_cast<char*>(ws)};
+    f.up = gemm_plan(s.dtype, s.rows, 2 * s.ff, gemm_steps(s.d, s.dtype), 1, 1);
+    f.down = gemm_plan(s.dtype, s.rows, s.d, gemm_steps(s.ff, s.dtype), 1, kMaxSplits);
+    f.x = s.pad_d ? b.take(s.rows * s.dp * s.size) : nullptr;
+    f.wg = s.pad_d ? b.take(s.ff * s.dp * s.size) : nullptr;
+    f.wu = s.pad_d ? b.take(s.ff * s.dp * s.size) : nullptr;
+    f.wd = s.pad_f ? b.take(s.d * s.fp * s.size) : nullptr;
+    f.h = keeps_h ? nullptr : b.take(s.rows * s.fp * s.size);
+    f.part = reinterpret_cast<float*>(b.take((int64_t)gemm_part_bytes(f.down, 1, s.rows, s.d)));
+    f.bytes = b.used;
+    return f;
+}
+
+struct MlpBwd {
+    GemmPlan dh, dx, dw, dwd;
+    void *x, *dy, *wg, *wu, *wd, *dg, *du;
+    float* part;
+    size_t bytes;
+};
+MlpBwd mlp_bwd_layout(const MlpShape& s, void* ws) {
+    MlpBwd f;
+    Bump b{reinterpret_cast<char*>(ws)};
+    f.dh = gemm_plan(s.dtype, s.rows, s.ff, gemm_steps(s.d, s.dtype), 1, 1);
+    f.dx = gemm_plan(s.dtype, s.rows, s.d, 2 * gemm_steps(s.fp, s.dtype), 1, kMaxSplits);
+    f.dw = gemm_plan(s.dtype, s.ff, s.d, gemm_steps(s.rows, s.dtype), 2, kMaxSplits);
+    f.dwd = gemm_plan(s.dtype, s.d, s.ff, gemm_steps(s.rows, s.dtype), 1, kMaxSplits);
+    f.x = s.pad_d ? b.take(s.rows * s.dp * s.size) : nullptr;
+    f.dy = s.pad_d ? b.take(s.rows * s.dp * s.size) : nullptr;
+    f.wg = s.pad_d ? b.take(s.ff * s.dp * s.size) : nullptr;
+    f.wu = s.pad_d ? b.take(s.ff * s.dp * s.size) : nullptr;
+    f.wd = s.pad_f ? b.take(s.d * s.fp * s.size) : nullptr;
+    f.dg = b.take(s.rows * s.fp * s.size);
+    f.du = b.take(s.rows * s.fp * s.size);
+    const size_t part = std::max(std::max(gemm_part_bytes(f.dx, 1, s.rows, s.d), gemm_part_bytes(f.dw, 2, s.ff, s.d)),
+                                 gemm_part_bytes(f.dwd, 1, s.d, s.ff));
+    f.part = reinterpret_cast<float*>(b.take((int64_t)part));
+    f.bytes = b.used;
+    return f;
+}
+
+// h behind the planes of g and u
+int64_t gu_bytes(const MlpShape& s) { return up256(s.rows * s.fp * (s.dtype == M3_DTYPE_BF16 ? 6 : 8)); }
+
+// src as it is, or its padded copy
+int padded(const MlpShape& s, const void* src, void* dst, int64_t rows, int64_t cols, int64_t ldd, const void** out,
+           hipStream_t stream) {
+    *out = dst ? dst : src;
+    return dst ? gemm_pad_copy(s.dtype, src, dst, rows, cols, ldd, nullptr, 0, stream) : M3_OK;
+}
+
+}  // namespace
+
+size_t swiglu_saved(int64_t rows, int64_t d, int64_t ff, int dtype) {
+    const MlpShape s = mlp_shape(rows, d, ff, dtype);
+    return (size_t)(gu_bytes(s) + up256(rows * s.fp * s.size));
+}
+size_t swiglu_fwd_workspace(int64_t rows, int64_t d, int64_t ff, int dtype, bool keeps) {
+    return mlp_fwd_layout(mlp_shape(rows, d, ff, dtype), keeps, nullptr).bytes;
+}
+size_t swiglu_bwd_workspace(int64_t rows, int64_t d, int64_t ff, int dtype) {
+    return mlp_bwd_layout(mlp_shape(rows, d, ff, dtype), nullptr).bytes;
+}
+
+#define M3_TRY(e)                       \
+    do {                                \
+        const int st_ = (e);            \
+        if (st_ != M3_OK) return st_;   \
+    } while (0)
+
+int launch_swiglu_fwd(int64_t rows, int64_t d, int64_t ff, int dtype, const void* x, const void* wg, const void* wu,
+                      const void* wd, const void* res, float scale, void* y, void* saved, void* ws,
+                      hipStream_t stream) {
+    const MlpShape s = mlp_shape(rows, d, ff, dtype);
+    const MlpFwd f = mlp_fwd_layout(s, saved != nullptr, ws);
+    M3_TRY(padded(s, x, f.x, rows, d, s.dp, &x, stream));
+    M3_TRY(padded(s, wg, f.wg, ff, d, s.dp, &wg, stream));
+    M3_TRY(padded(s, wu, f.wu, ff, d, s.dp, &wu, stream));
+    M3_TRY(padded(s, wd, f.wd, d, ff, s.fp, &wd, stream));
+    void* h = saved ? reinterpret_cast<char*>(saved) + gu_bytes(s) : f.h;
+    GemmArgs a = gemm_args({x, s.dp}, {wg, s.dp}, rows, ff, s.dp, 1);
+    a.b[1] = {wu, s.dp};
+    M3_TRY((gemm_dispatch<true, true, kGated>(dtype, f.up, a, EpiGated{h, saved, (int)rows, (int)s.fp}, rows, 2 * s.fp, 1, stream)));
+    const GemmStore st{{y, nullptr}, d, res, scale, f.part, 0, (int)rows, (int)d};
+    return gemm_store(kFormNT, dtype, f.down, gemm_args({h, s.fp}, {wd, s.fp}, rows, d, s.fp, 1), st, 1, stream);
+}
+
+int launch_swiglu_bwd(int64_t rows, int64_t d, int64_t ff, int dtype, const void* x, const void* wg, const void* wu,
+                      const void* wd, float scale, const void* saved, const void* dy, void* dx, void* dwg, void* dwu,
+                      void* dwd, void* ws, hipStream_t stream) {
+    const MlpShape s = mlp_shape(rows, d, ff, dtype);
+    const MlpBwd f = mlp_bwd_layout(s, ws);
+    const void* h = reinterpret_cast<const char*>(saved) + gu_bytes(s);
+    M3_TRY(padded(s, dy, f.dy, rows, d, s.dp, &dy, stream));
+    if (dx || dwg || dwu) {
+        M3_TRY(padded(s, wd, f.wd, d, ff, s.fp, &wd, stream));
+        // rows of Wd past d do not exist: A's pad columns meet zeros
+        GemmArgs a = gemm_args({dy, s.dp}, {wd, s.fp}, rows, s.fp, s.dp, 1);
+        a.KB[0] = (int)d;
+        M3_TRY((gemm_dispatch<true, false, kPlain>(dtype, f.dh, a, EpiGateBwd{f.dg, f.du, saved, scale, (int)rows, (int)s.fp}, rows, s.fp, 1, stream)));
+    }
+    if (dx) {
+        M3_TRY(padded(s, wg, f.wg, ff, d, s.dp, &wg, stream));
+        M3_TRY(padded(s, wu, f.wu, ff, d, s.dp, &wu, stream));
+        GemmArgs a = gemm_args({f.dg, s.fp}, {wg, s.dp}, rows, s.dp, s.fp, 1);
+        a.a[1] = {f.du, s.fp}, a.b[1] = {wu, s.dp};
+        a.K[1] = (int)s.fp;
+        a.KB[0] = a.KB[1] = (int)ff;
+        const GemmStore st{{dx, nullptr}, d, nullptr, 1.f, f.part, 0, (int)rows, (int)d};
+        M3_TRY(gemm_store(kFormNN, dtype, f.dx, a, st, 1, stream));
+    }
+    if (dwg || dwu) {
+        M3_TRY(padded(s, x, f.x, rows, d, s.dp, &x, stream));
+        GemmArgs a = gemm_args({dwg ? f.dg : f.du, s.fp}, {x, s.dp}, s.fp, s.dp, rows, 1);
+        if (dwg && dwu) a.a[1] = {f.du, s.fp};
+        const GemmStore st{{dwg ? dwg : dwu, dwg ? dwu : nullptr}, d, nullptr, 1.f, f.part, 0, (int)ff, (int)d};
+        M3_TRY(gemm_store(kFormTN, dtype, f.dw, a, st, dwg && dwu ? 2 : 1, stream));
+    }
+    if (dwd) {
+        const GemmStore st{{dwd, nullptr}, ff, nullptr, scale, f.part, 0, (int)d, (int)ff};
+        M3_TRY(gemm_store(kFormTN, dtype, f.dwd, gemm_args({dy, s.dp}, {h, s.fp}, s.dp, s.fp, rows, 1), st, 1, stream));
+    }
+    return M3_OK;
+}
+
+}  // namespace m3

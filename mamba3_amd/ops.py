@@ -705,6 +705,157 @@ def _(gate_up, d_ff):
     return gate_up.new_empty(*gate_up.shape[:-1], d_ff)
 
 
+# ---------------------------------------------------------------- training operators
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    """t as contiguous, 16-byte aligned rows of its last dimension."""
+    t = t.detach().reshape(-1, t.shape[-1]).contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def check_alike(what: str, *tensors: torch.Tensor) -> None:
+    """Raises unless the tensors share a dtype that the kernels take and a GPU."""
+    first = tensors[0]
+    _native.dtype_code(first.dtype)
+    for t in tensors[1:]:
+        if t.dtype != first.dtype:
+            raise TypeError(f"{what} takes tensors of one dtype, got {first.dtype} and {t.dtype}")
+        if t.device != first.device:
+            raise ValueError(f"{what} takes tensors on one GPU, got {first.device} and {t.device}")
+    _native.require_gpu(first)
+
+
+def _swiglu_mlp_eager(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+                      residual: Optional[torch.Tensor], scale: float,
+                      keep: bool) -> tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """m3_swiglu_mlp_fwd over the last dimension of x: y in x's shape and, with `keep`, what the
+    backward reads (else None)."""
+    _native.require_gpu(x, w_gate, w_up, w_down, residual)
+    with torch.cuda.device(x.device):
+        x2 = _flat(x)
+        y = torch.empty(x2.shape, device=x.device, dtype=x.dtype)
+        n = _native.swiglu_mlp_saved_bytes(*x2.shape, w_gate.shape[0], x.dtype) if keep else 0
+        saved = torch.empty(n, device=x.device, dtype=torch.uint8) if keep else None
+        _native.swiglu_mlp_fwd(x2, _flat(w_gate), _flat(w_up), _flat(w_down),
+                               None if residual is None else _flat(residual), scale, y, saved)
+    return y.view(x.shape), saved
+
+
+@torch.library.custom_op(f"{NS}::swiglu_mlp", mutates_args=())
+def swiglu_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+               residual: Optional[torch.Tensor], scale: float,
+               keep: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """_swiglu_mlp_eager as an op; the second output is empty without `keep`."""
+    y, saved = _swiglu_mlp_eager(x, w_gate, w_up, w_down, residual, scale, keep)
+    return y, x.new_empty(0, dtype=torch.uint8) if saved is None else saved
+
+
+@swiglu_mlp.register_fake
+def _(x, w_gate, w_up, w_down, residual, scale, keep):
+    d = x.shape[-1]
+    n = _native.swiglu_mlp_saved_bytes(x.numel() // d, d, w_gate.shape[0], x.dtype) if keep else 0
+    return x.new_empty(x.shape), x.new_empty(n, dtype=torch.uint8)
+
+
+@torch.library.custom_op(f"{NS}::swiglu_mlp_bwd", mutates_args=())
+def swiglu_mlp_bwd(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+                   scale: float, saved: torch.Tensor, dy: torch.Tensor,
+                   want: list[bool]) -> list[torch.Tensor]:
+    """m3_swiglu_mlp_bwd: gradients of x, w_gate, w_up and w_down in their shapes; those that
+    `want` leaves out are empty."""
+    with torch.cuda.device(x.device):
+        x2, dy2 = _flat(x), _flat(dy.to(x.dtype))
+        out = [torch.empty(t.shape, device=x.device, dtype=x.dtype) if w else None
+               for t, w in zip((x, w_gate, w_up, w_down), want)]
+        _native.swiglu_mlp_bwd(x2, _flat(w_gate), _flat(w_up), _flat(w_down), scale, saved, dy2, *out)
+    return [x.new_empty(0) if t is None else t for t in out]
+
+
+@swiglu_mlp_bwd.register_fake
+def _(x, w_gate, w_up, w_down, scale, saved, dy, want):
+    return [x.new_empty(t.shape if w else (0,)) for t, w in zip((x, w_gate, w_up, w_down), want)]
+
+
+def _swiglu_mlp_setup(ctx, inputs, output):
+    *tensors, _, scale, keep = inputs
+    ctx.scale, ctx.keep = scale, keep
+    ctx.save_for_backward(*tensors, output[1])
+    ctx.set_materialize_grads(False)
+
+
+def _swiglu_mlp_backward(ctx, dy, _):
+    if dy is None:
+        return (None,) * 7
+    if not ctx.keep:
+        raise RuntimeError("swiglu_mlp was run without keeping what its backward reads")
+    *tensors, saved = ctx.saved_tensors
+    want = list(ctx.needs_input_grad[:4])
+    g = swiglu_mlp_bwd(*tensors, ctx.scale, saved, dy, want) if any(want) else [None] * 4
+    return (*[t if w else None for t, w in zip(g, want)], dy if ctx.needs_input_grad[4] else None, None, None)
+
+
+swiglu_mlp.register_autograd(_swiglu_mlp_backward, setup_context=_swiglu_mlp_setup)
+
+
+def _linear_xent_eager(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor,
+                       ignore_index: int,
+                       reduction: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """m3_linear_xent_fwd: (loss, fp32, of target's shape or a scalar; lse (rows,); count (1,))."""
+    _native.require_gpu(hidden, weight, target)
+    with torch.cuda.device(hidden.device):
+        h2, t1 = _flat(hidden), target.reshape(-1).contiguous()
+        new = lambda *s: torch.empty(s, device=hidden.device, dtype=torch.float32)  # noqa: E731
+        loss = new(*target.shape) if reduction == 0 else new()
+        lse, count = new(h2.shape[0]), new(1)
+        _native.linear_xent_fwd(h2, _flat(weight), t1, ignore_index, reduction, loss, lse, count)
+    return loss, lse, count
+
+
+linear_xent = torch.library.custom_op(f"{NS}::linear_xent", _linear_xent_eager, mutates_args=())
+
+
+@linear_xent.register_fake
+def _(hidden, weight, target, ignore_index, reduction):
+    f = torch.float32
+    return (hidden.new_empty(target.shape if reduction == 0 else (), dtype=f),
+            hidden.new_empty(target.numel(), dtype=f), hidden.new_empty(1, dtype=f))
+
+
+@torch.library.custom_op(f"{NS}::linear_xent_bwd", mutates_args=())
+def linear_xent_bwd(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int,
+                    reduction: int, lse: torch.Tensor, count: torch.Tensor, grad: torch.Tensor,
+                    want: list[bool]) -> list[torch.Tensor]:
+    """m3_linear_xent_bwd: gradients of hidden and weight; those that `want` leaves out are empty."""
+    with torch.cuda.device(hidden.device):
+        out = [torch.empty(t.shape, device=t.device, dtype=t.dtype) if w else None
+               for t, w in zip((hidden, weight), want)]
+        _native.linear_xent_bwd(_flat(hidden), _flat(weight), target.reshape(-1).contiguous(), ignore_index,
+                                reduction, lse, count, grad.float().contiguous(), *out)
+    return [hidden.new_empty(0) if t is None else t for t in out]
+
+
+@linear_xent_bwd.register_fake
+def _(hidden, weight, target, ignore_index, reduction, lse, count, grad, want):
+    return [hidden.new_empty(t.shape if w else (0,)) for t, w in zip((hidden, weight), want)]
+
+
+def _linear_xent_setup(ctx, inputs, output):
+    hidden, weight, target, ctx.ignore_index, ctx.reduction = inputs
+    ctx.save_for_backward(hidden, weight, target, output[1], output[2])
+    ctx.set_materialize_grads(False)
+
+
+def _linear_xent_backward(ctx, g_loss, g_lse, g_count):
+    if g_loss is None:
+        return (None,) * 5
+    hidden, weight, target, lse, count = ctx.saved_tensors
+    want = list(ctx.needs_input_grad[:2])
+    g = linear_xent_bwd(hidden, weight, target, ctx.ignore_index, ctx.reduction, lse, count, g_loss, want)
+    return (*[t if w else None for t, w in zip(g, want)], None, None, None)
+
+
+linear_xent.register_autograd(_linear_xent_backward, setup_context=_linear_xent_setup)
+
+
 # ---------------------------------------------------------------- eager calls
 # What a direct call may be given: a subclass's own dispatch has to see it.
 _PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
@@ -760,3 +911,13 @@ def silu_mul_fast(gate_up, d_ff):
 
 def rmsnorm_fast(x, weight, eps):
     return (_rmsnorm_eager if _direct(x, weight) else rmsnorm)(x, weight, eps)[0]
+
+
+def swiglu_mlp_fast(x, w_gate, w_up, w_down, residual, scale, keep):
+    fn = _swiglu_mlp_eager if _direct(x, w_gate, w_up, w_down, residual) else swiglu_mlp
+    return fn(x, w_gate, w_up, w_down, residual, scale, keep)[0]
+
+
+def linear_xent_fast(hidden, weight, target, ignore_index, reduction):
+    fn = _linear_xent_eager if _direct(hidden, weight, target) else linear_xent
+    return fn(hidden, weight, target, ignore_index, reduction)[0]

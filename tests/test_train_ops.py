@@ -1,0 +1,173 @@
+"""Refusals of the training operators (gated MLP, linear cross entropy, gradient clipping), on the
+host: nothing here launches a kernel."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+import mamba3_amd
+from mamba3_amd import _native
+
+FAKE = 1 << 12  # an address that is never dereferenced: the call is refused first
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not _native.LIB_PATH.exists():
+        from mamba3_amd import build
+        build.build(verbose=False)
+    return _native.lib()
+
+
+def _size(fn, *args):
+    n = ctypes.c_size_t(0)
+    return fn(*args, ctypes.byref(n)), n.value
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("rows,d,ff", [(1, 1, 1), (7, 33, 65), (8192, 768, 2112), (1 << 20, 2048, 5504)])
+def test_swiglu_sizes_cover_what_is_kept(lib, dtype, rows, d, ff):
+    st, saved = _size(lib.m3_swiglu_mlp_saved_size, rows, d, ff, dtype)
+    size = 2 if dtype else 4
+    # gate and up (24 bits each, or fp32) and h
+    assert st == 0 and saved >= rows * ff * ((6 + 2) if dtype else (8 + 4)) and saved % 256 == 0
+    st, kept = _size(lib.m3_swiglu_mlp_fwd_workspace_size, rows, d, ff, dtype, 1)
+    assert st == 0
+    st, alone = _size(lib.m3_swiglu_mlp_fwd_workspace_size, rows, d, ff, dtype, 0)
+    assert st == 0 and alone >= kept + rows * ff * size
+    st, back = _size(lib.m3_swiglu_mlp_bwd_workspace_size, rows, d, ff, dtype)
+    assert st == 0 and back >= 2 * rows * ff * size
+
+
+def test_swiglu_refuses_bad_arguments(lib):
+    def fwd(rows=4, d=64, ff=128, dtype=1, x=FAKE, wg=FAKE, wu=FAKE, wd=FAKE, res=None, y=FAKE, saved=None,
+            ws=FAKE, n=1 << 40):
+        return lib.m3_swiglu_mlp_fwd(rows, d, ff, dtype, x, wg, wu, wd, res, 1.0, y, saved, ws, n, None)
+
+    for name in ("x", "wg", "wu", "wd", "y"):
+        assert fwd(**{name: None}) == 1
+    assert fwd(rows=0) == 2 and fwd(d=0) == 2 and fwd(ff=-1) == 2
+    assert fwd(rows=(1 << 30) + 1) == 3 and fwd(d=(1 << 20) + 1) == 3 and fwd(ff=(1 << 20) + 1) == 3
+    assert fwd(dtype=2) == 3
+    for name in ("x", "wg", "wu", "wd", "ws"):
+        assert fwd(**{name: FAKE + 8}) == 5
+    assert fwd(saved=FAKE + 16) == 5
+    assert fwd(ws=None) == 4 and fwd(n=16) == 4
+
+    def bwd(rows=4, dtype=1, x=FAKE, saved=FAKE, dy=FAKE, ws=FAKE, n=1 << 40):
+        return lib.m3_swiglu_mlp_bwd(rows, 64, 128, dtype, x, FAKE, FAKE, FAKE, 1.0, saved, dy, FAKE, FAKE, FAKE,
+                                     FAKE, ws, n, None)
+
+    assert bwd(x=None) == 1 and bwd(saved=None) == 1 and bwd(dy=None) == 1
+    assert bwd(rows=-1) == 2 and bwd(dtype=7) == 3
+    assert bwd(dy=FAKE + 2) == 5 and bwd(saved=FAKE + 16) == 5 and bwd(n=0) == 4
+
+
+def test_xent_refuses_bad_arguments(lib):
+    def fwd(rows=4, d=64, vocab=100, dtype=1, red=1, h=FAKE, w=FAKE, t=FAKE, loss=FAKE, lse=FAKE, count=FAKE,
+            ws=FAKE, n=1 << 40):
+        return lib.m3_linear_xent_fwd(rows, d, vocab, dtype, red, h, w, t, -100, loss, lse, count, ws, n, None)
+
+    for name in ("h", "w", "t", "loss", "lse", "count"):
+        assert fwd(**{name: None}) == 1
+    assert fwd(rows=0) == 2 and fwd(vocab=0) == 2 and fwd(red=3) == 2 and fwd(red=-1) == 2
+    assert fwd(dtype=2) == 3 and fwd(vocab=(1 << 30) + 1) == 3 and fwd(d=(1 << 20) + 1) == 3
+    assert fwd(h=FAKE + 8) == 5 and fwd(w=FAKE + 8) == 5 and fwd(ws=None) == 4 and fwd(n=100) == 4
+
+    def bwd(rows=4, red=1, grad=FAKE, dh=FAKE, dw=FAKE, n=1 << 40):
+        return lib.m3_linear_xent_bwd(rows, 64, 100, 1, red, FAKE, FAKE, FAKE, -100, FAKE, FAKE, grad, dh, dw, FAKE,
+                                      n, None)
+
+    assert bwd(grad=None) == 1 and bwd(rows=0) == 2 and bwd(red=9) == 2 and bwd(n=0) == 4
+    assert bwd(dh=None, dw=None) == 0  # nothing asked for, nothing launched
+
+
+def test_xent_backward_holds_one_piece_of_the_vocabulary(lib):
+    st, n = _size(lib.m3_linear_xent_bwd_workspace_size, 8192, 768, 128000, 1, 1, 1)
+    # far below the 2.1 GB of bf16 logits: a piece of at most 256 MiB, hidden, fp32 sums
+    assert st == 0 and (256 << 20) < n < (1 << 30)
+
+
+def test_clip_refuses_bad_arguments(lib):
+    i64, i32 = ctypes.c_int64, ctypes.c_int32
+
+    def clip(ptrs=(FAKE,), numel=(8,), dtype=(0,), kind=0, norm=FAKE, ws=FAKE, nbytes=1 << 30, n=None):
+        n = len(ptrs) if n is None else n
+        return lib.m3_clip_grad_norm(n, (ctypes.c_void_p * len(ptrs))(*ptrs), (i64 * len(numel))(*numel),
+                                     (i32 * len(dtype))(*dtype), kind, 1, 1.0, norm, ws, nbytes, None)
+
+    assert clip(norm=None) == 1 and clip(ptrs=(None,)) == 1
+    assert clip(n=-1) == 2 and clip(numel=(-1,)) == 2
+    assert clip(dtype=(5,)) == 3 and clip(kind=2) == 3 and clip(numel=((1 << 36) + 1,)) == 3
+    assert clip(ptrs=(FAKE + 2,)) == 5 and clip(ptrs=(FAKE + 1,), dtype=(1,)) == 5
+    assert clip(ws=None) == 4 and clip(nbytes=8) == 4 and clip(ws=FAKE + 64) == 5
+    assert lib.m3_clip_grad_norm(1, None, None, None, 0, 1, 1.0, FAKE, FAKE, 1 << 30, None) == 1
+
+
+def _weights(d=8, ff=16, dtype=torch.float32):
+    return torch.ones(ff, d, dtype=dtype), torch.ones(ff, d, dtype=dtype), torch.ones(d, ff, dtype=dtype)
+
+
+def test_swiglu_mlp_refuses():
+    wg, wu, wd = _weights()
+    x = torch.ones(3, 8)
+    with pytest.raises(RuntimeError, match="GPU"):
+        mamba3_amd.swiglu_mlp(x, wg, wu, wd)
+    with pytest.raises(ValueError, match="do not fit"):
+        mamba3_amd.swiglu_mlp(torch.ones(3, 9), wg, wu, wd)
+    with pytest.raises(ValueError, match="do not fit"):
+        mamba3_amd.swiglu_mlp(x, wg, wu, wd.t())
+    with pytest.raises(ValueError, match="two-dimensional"):
+        mamba3_amd.swiglu_mlp(x, wg[0], wu, wd)
+    with pytest.raises(ValueError, match="residual"):
+        mamba3_amd.swiglu_mlp(x, wg, wu, wd, residual=torch.ones(1, 8))
+    with pytest.raises(TypeError, match="one dtype"):
+        mamba3_amd.swiglu_mlp(x.bfloat16(), wg, wu, wd)
+    with pytest.raises(TypeError, match="float32 and bfloat16"):
+        mamba3_amd.swiglu_mlp(x.half(), wg.half(), wu.half(), wd.half())
+
+
+def test_linear_cross_entropy_refuses():
+    h, w, t = torch.ones(3, 8), torch.ones(11, 8), torch.zeros(3, dtype=torch.long)
+    with pytest.raises(RuntimeError, match="GPU"):
+        mamba3_amd.linear_cross_entropy(h, w, t)
+    with pytest.raises(ValueError, match="do not fit"):
+        mamba3_amd.linear_cross_entropy(h, w.t(), t)
+    with pytest.raises(ValueError, match="target has shape"):
+        mamba3_amd.linear_cross_entropy(h, w, t[:2])
+    with pytest.raises(TypeError, match="int64"):
+        mamba3_amd.linear_cross_entropy(h, w, t.int())
+    with pytest.raises(ValueError, match="reduction"):
+        mamba3_amd.linear_cross_entropy(h, w, t, reduction="median")
+    with pytest.raises(TypeError, match="one dtype"):
+        mamba3_amd.linear_cross_entropy(h.bfloat16(), w, t)
+
+
+def test_clip_grad_norm_refuses():
+    p = torch.nn.Parameter(torch.ones(4))
+    assert mamba3_amd.clip_grad_norm_([p], 1.0).item() == 0.0  # no gradient, nothing to do
+    p.grad = torch.ones(4)
+    with pytest.raises(RuntimeError, match="GPU"):
+        mamba3_amd.clip_grad_norm_([p], 1.0)
+    for bad in (1.0, 0.0, math.nan):
+        with pytest.raises(ValueError, match="norm_type"):
+            mamba3_amd.clip_grad_norm_(p, 1.0, norm_type=bad)
+    for bad in (-1.0, math.nan):
+        with pytest.raises(ValueError, match="max_norm"):
+            mamba3_amd.clip_grad_norm_(p, bad)
+    p.grad = torch.ones(4).to_sparse()
+    with pytest.raises(TypeError, match="dense"):
+        mamba3_amd.clip_grad_norm_(p, 1.0)
+    q = torch.nn.Parameter(torch.ones(4, dtype=torch.float16))
+    q.grad = torch.ones(4, dtype=torch.float16)
+    with pytest.raises(TypeError, match="float32 and bfloat16"):
+        mamba3_amd.clip_grad_norm_(q, 1.0)
+
+
+def test_new_names_are_attributes_beside_the_eight():
+    for name in ("swiglu_mlp", "linear_cross_entropy", "clip_grad_norm_"):
+        assert callable(getattr(mamba3_amd, name)) and name not in mamba3_amd.__all__
