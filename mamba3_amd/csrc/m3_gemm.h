@@ -26,18 +26,39 @@ namespace m3 {
 
 constexpr unsigned kOob = 0x80000000u;  // a byte offset past every descriptor's bound
 
-template <typename T> struct GemmType;
-template <> struct GemmType<bf16> {
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// The MFMA of a type: MF x MF results (MF 16 or 32) of 32 or 16 k (bf16), fp32 four times 4 or 2.
+template <typename T, int MF> struct GemmType;
+template <> struct GemmType<bf16, 16> {
     typedef bf16x8 Frag;  // 8 consecutive k of one row
-    static __device__ __forceinline__ f32x4 mma(Frag b, Frag a, f32x4 c) {
+    typedef f32x4 Acc;
+    static __device__ __forceinline__ Acc mma(Frag b, Frag a, Acc c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, a, c, 0, 0, 0);
     }
 };
-template <> struct GemmType<float> {
-    typedef f32x4 Frag;  // 4 consecutive k of one row: MFMA j takes element j of every lane
-    static __device__ __forceinline__ f32x4 mma(Frag b, Frag a, f32x4 c) {
+template <> struct GemmType<bf16, 32> {
+    typedef bf16x8 Frag;
+    typedef f32x16 Acc;
+    static __device__ __forceinline__ Acc mma(Frag b, Frag a, Acc c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(b, a, c, 0, 0, 0);
+    }
+};
+template <> struct GemmType<float, 16> {
+    typedef f32x4 Frag;
+    typedef f32x4 Acc;
+    static __device__ __forceinline__ Acc mma(Frag b, Frag a, Acc c) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(b[j], a[j], c, 0, 0, 0);
+        return c;
+    }
+};
+template <> struct GemmType<float, 32> {
+    typedef f32x4 Frag;  // 4 consecutive k of one row: MFMA j takes element j of every lane
+    typedef f32x16 Acc;
+    static __device__ __forceinline__ Acc mma(Frag b, Frag a, Acc c) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(b[j], a[j], c, 0, 0, 0);
         return c;
     }
 };
@@ -63,7 +84,7 @@ struct GemmArgs {
 };
 
 // Global -> LDS copies of one operand's tile by the whole block.
-template <typename T, bool kKc, int BX, int NW>
+template <typename T, bool kKc, int BX, int NW, int MF>
 struct GemmLoader {
     static constexpr int kInstr = BX * 128 / 1024;  // wave instructions a tile
     static constexpr int NI = kInstr / NW;          // of which each wave issues NI
@@ -72,52 +93,60 @@ struct GemmLoader {
     static constexpr int RPI = 64 / CPR;                // rows an instruction
     static_assert(kInstr % NW == 0 && NI >= 1, "tile too small for the block");
     unsigned voff[NI];
-    int piece;  // kKc: the lane's 16-byte piece of the row
 
-    // row0: first row of this wave's part when it differs from its place in the tile (kGated)
-    __device__ __forceinline__ void init(int wave, int lane, int64_t ld, int row_shift) {
+    // ld: row stride in elements; row_shift: rows before this wave's in the tile (kGated); pieces: valid
+    // 16-byte pieces of the rows (kKc), the others are read out of bounds, as zeros
+    __device__ __forceinline__ void init(int wave, int lane, int ld, int row_shift, int pieces) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int r = (wave * NI + i) * RPI + lane / CPR, c = lane % CPR;
             if constexpr (kKc) {
-                piece = c ^ (r & 7);
-                voff[i] = (unsigned)((r - row_shift) * (int)ld * SZ + piece * 16);
+                const int piece = c ^ (r & 7);
+                voff[i] = piece < pieces ? (unsigned)((r - row_shift) * ld * SZ + piece * 16) : kOob;
             } else if constexpr (SZ == 2) {
-                const int key = ((r & 3) | ((r >> 3) & 3) << 2) & (BX / 16 - 1);
-                voff[i] = (unsigned)(r * (int)ld * SZ + (((c >> 1) ^ key) << 1 | (c & 1)) * 16);
+                const int key = MF == 16 ? (r & 3) | ((r >> 3) & 3) << 2 : (r & 3) << 1 | ((r >> 3) & 1) << 3;
+                voff[i] = (unsigned)(r * ld * SZ + (((c >> 1) ^ (key & (BX / 16 - 1))) << 1 | (c & 1)) * 16);
             } else {
-                const int key = (r >> 2) & 3;
-                voff[i] = (unsigned)(r * (int)ld * SZ + (((c >> 2) ^ key) << 2 | (c & 3)) * 16);
+                constexpr int U = MF / 4;  // pieces of a unit
+                const int key = (r >> 2) & (64 / MF - 1);
+                voff[i] = (unsigned)(r * ld * SZ + ((c / U ^ key) * U + c % U) * 16);
             }
         }
     }
-    // bytes: what the descriptor spans; pieces: valid 16-byte pieces of the rows (kKc)
-    __device__ __forceinline__ void issue(const char* base, int64_t bytes, int pieces, char* lds, int wave) const {
-        const __amdgpu_buffer_rsrc_t rs = make_rsrc(base, bytes < 0 ? 0 : bytes);
-        const bool live = !kKc || piece < pieces;
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const unsigned v = live ? voff[i] : kOob;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                rs, (__attribute__((address_space(3))) void*)(lds + (wave * NI + i) * 1024), 16, (int)v, 0, 0, 0);
-        }
+    // Instruction i of this wave; bytes is what lies behind base. In assembly because the compiler takes
+    // every later ds_read_b64_tr_b16 for a reader of what the builtin copies and waits for all copies
+    // before it; the kernel waits itself (wait_vm_lds). No register is written, so none is
+    // live while the copy runs.
+    __device__ __forceinline__ void issue(int i, const char* base, int bytes, unsigned lds, int wave) const {
+        const u32x4 rs{(unsigned)reinterpret_cast<uintptr_t>(base), (unsigned)(reinterpret_cast<uintptr_t>(base) >> 32),
+                       (unsigned)bytes, (unsigned)kRsrcFlags};
+        const unsigned at = lds + (wave * NI + i) * 1024;
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                     :
+                     : "s"(at), "v"(voff[i]), "s"(rs)
+                     : "memory", "m0");
     }
 };
 
-// LDS -> MFMA operand: 16 rows (unit u of the tile), k step ks (of two).
-template <typename T, bool kKc, int BX>
+// LDS -> MFMA operand: MF rows (unit u of the tile), k step ks (of 2 for MF 16, of 4 for MF 32).
+template <typename T, bool kKc, int BX, int MF>
 struct GemmReader {
-    typedef typename GemmType<T>::Frag Frag;
-    int off[2];
+    typedef typename GemmType<T, MF>::Frag Frag;
+    static constexpr int KS = MF == 16 ? 2 : 4, G = 64 / MF;  // lane groups along k
+    int off[KS];
     int key;
     __device__ __forceinline__ void init(int lane) {
-        const int r = lane & 15, g = lane >> 4;
+        const int r = lane % MF, g = lane / MF;
         if constexpr (kKc) {
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) off[ks] = r * 128 + (((ks * 4 + g) ^ (r & 7)) * 16);
+            for (int ks = 0; ks < KS; ++ks) off[ks] = r * 128 + (((ks * G + g) ^ (r & 7)) * 16);
         } else if constexpr (sizeof(T) == 2) {
-            key = (r >> 2 | g << 2) & (BX / 16 - 1);
-            off[0] = (g * 8 + (r >> 2)) * (BX * 2) + (r & 3) * 8;
+            // 16 lanes read a 4 x 16 block and get its columns (MF 32: lanes 0-15 and 16-31 take the
+            // two column halves of the unit)
+            const int j = lane & 15;
+            key = (MF == 16 ? (j >> 2) | g << 2 : (j >> 2) << 1 | g << 3) & (BX / 16 - 1);
+            off[0] = (g * 8 + (j >> 2)) * (BX * 2) + (j & 3) * 8;
+            off[1] = (lane >> 4) & 1;
         } else {
             key = g;
             off[0] = g * 4 * (BX * 4) + r * 4;
@@ -125,16 +154,17 @@ struct GemmReader {
     }
     __device__ __forceinline__ Frag read(const char* tile, int u, int ks) const {
         if constexpr (kKc) {
-            return *reinterpret_cast<const Frag*>(tile + u * 2048 + off[ks]);
+            return *reinterpret_cast<const Frag*>(tile + u * (MF * 128) + off[ks]);
         } else if constexpr (sizeof(T) == 2) {
-            const char* p = tile + off[0] + ((u ^ key) << 5) + ks * 32 * (BX * 2);
+            const int unit = MF == 16 ? u : u * 2 + off[1];
+            const char* p = tile + off[0] + ((unit ^ key) << 5) + ks * (8 * G) * (BX * 2);
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                 (__attribute__((address_space(3))) s16x4*)(p + 4 * (BX * 2)));
             const bf16x4 l4 = __builtin_bit_cast(bf16x4, lo), h4 = __builtin_bit_cast(bf16x4, hi);
             return __builtin_shufflevector(l4, h4, 0, 1, 2, 3, 4, 5, 6, 7);
         } else {
-            const char* p = tile + off[0] + ((u ^ key) << 6) + ks * 16 * (BX * 4);
+            const char* p = tile + off[0] + (u ^ key) * (MF * 4) + ks * (4 * G) * (BX * 4);
             Frag f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) f[j] = *reinterpret_cast<const float*>(p + j * (BX * 4));
@@ -144,31 +174,39 @@ struct GemmReader {
 };
 
 template <int kN>
-__device__ __forceinline__ void wait_vm_lds() {  // at most kN loads in flight, no LDS read
-    __builtin_amdgcn_s_waitcnt((kN & 15) | (7 << 4) | ((kN >> 4) << 14));
+__device__ __forceinline__ void wait_vm_lds() {  // at most kN copies in flight, no LDS read
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(kN) : "memory");
 }
 
-template <int BM_, int BN_, int WGM_, int WGN_, int STAGES_>
+template <int BM_, int BN_, int WGM_, int WGN_, int STAGES_, int MF_>
 struct GemmTile {
-    static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, STAGES = STAGES_;
+    static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, STAGES = STAGES_, MF = MF_;
     static constexpr int NW = WGM * WGN, NT = NW * 64;
-    static constexpr int FM = BM / WGM / 16, FN = BN / WGN / 16;  // 16 x 16 pieces of a wave
+    static constexpr int FM = BM / WGM / MF, FN = BN / WGN / MF;  // MF x MF pieces of a wave
+    static constexpr int Q = MF * MF / 256;                       // fours of columns a lane holds of a piece
     static constexpr int kStageBytes = (BM + BN) * 128;
     static constexpr int kLds = STAGES * kStageBytes;
+    typedef typename GemmType<bf16, MF>::Acc Acc;
 };
 
-// Where a wave's accumulators lie: piece (fm, fn), lane: row m(fm), columns n(fn) .. n(fn) + 3.
+// Where a wave's accumulators lie: piece (fm, fn), four q, lane: row m(fm), columns n(fn, q) ..
+// n(fn, q) + 3.
 template <typename Tile, int kMode>
 struct GemmPlace {
+    static constexpr int MF = Tile::MF;
     int m0, n0, wm, wn, lane;
-    __device__ __forceinline__ int local_m(int fm) const { return (wm * Tile::FM + fm) * 16 + (lane & 15); }
+    __device__ __forceinline__ int local_m(int fm) const { return (wm * Tile::FM + fm) * MF + lane % MF; }
     __device__ __forceinline__ int m(int fm) const { return m0 + local_m(fm); }
     // kGated: fn < FN / 2 of the gate; the up piece of the same columns is fn + FN / 2
-    __device__ __forceinline__ int n(int fn) const {
+    __device__ __forceinline__ int n(int fn, int q) const {
         constexpr int F = kMode == kGated ? Tile::FN / 2 : Tile::FN;
-        return n0 + (wn * F + fn) * 16 + (lane >> 4) * 4;
+        return n0 + (wn * F + fn) * MF + q * 8 + lane / MF * 4;
     }
 };
+template <typename Acc>
+__device__ __forceinline__ f32x4 four(const Acc& v, int q) {
+    return f32x4{v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]};
+}
 
 // Block -> tile: the blocks of one XCD (dispatch is round robin over 8) take a contiguous run of
 // tiles, and runs walk groups of 8 row tiles column by column, so that an XCD's L2 serves
@@ -187,10 +225,11 @@ __device__ __forceinline__ void gemm_tile_of(int tiles_m, int tiles_n, int& tm, 
 
 template <typename T, typename Tile, bool kAKc, bool kBKc, int kMode, typename Epi>
 __global__ __launch_bounds__(Tile::NT, Tile::NT >= 512 ? 2 : 1) void gemm_kernel(GemmArgs a, Epi epi) {
-    constexpr int BM = Tile::BM, BN = Tile::BN, FM = Tile::FM, FN = Tile::FN, ST = Tile::STAGES;
+    constexpr int BM = Tile::BM, BN = Tile::BN, FM = Tile::FM, FN = Tile::FN, ST = Tile::STAGES, MF = Tile::MF;
     constexpr int BK = 128 / sizeof(T), SZ = sizeof(T);
-    typedef GemmLoader<T, kAKc, BM, Tile::NW> LA;
-    typedef GemmLoader<T, kBKc, BN, Tile::NW> LB;
+    typedef GemmLoader<T, kAKc, BM, Tile::NW, MF> LA;
+    typedef GemmLoader<T, kBKc, BN, Tile::NW, MF> LB;
+    typedef GemmType<T, MF> Type;
     constexpr int NLD = LA::NI + LB::NI;
     extern __shared__ __align__(16) char gemm_smem[];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -207,80 +246,137 @@ __global__ __launch_bounds__(Tile::NT, Tile::NT >= 512 ? 2 : 1) void gemm_kernel
 
     const bool second = kMode == kGated && wave * LB::NI >= LB::kInstr / 2;
     static_assert(kMode != kGated || (LB::kInstr / 2) % LB::NI == 0, "a wave fetches from one half");
+    // rows that exist in this tile: spans end with the last one's last valid element (< 2^31 bytes)
+    const int ra_rows = a.M - m0 < BM ? a.M - m0 : BM, rb_rows = a.N - n0 < BN ? a.N - n0 : BN;
     LA la;
     LB lb;
-    la.init(wave, lane, a.a[z].ld, 0);
-    lb.init(wave, lane, a.b[z].ld, second ? BN / 2 : 0);
-
-    auto issue = [&](int s, int slot) {
+    // Where the step to be fetched next lies, and the bytes behind it. From step to step the
+    // pointers advance by pa_step and pb_step; at step `turn` (the end, a term's last, partial step or
+    // the second term's first) everything is set up anew.
+    const char *pa, *pb;
+    int64_t pa_step, pb_step;
+    int ba, bb, turn;
+    auto set_up = [&](int s) {
         const int seg = kMode == kSeg2 && s >= st0 ? 1 : 0;
         const int k0 = (seg ? s - st0 : s) * BK;
-        const int krem = s < s1 ? a.K[seg] - k0 : 0;
+        const int left = a.K[seg] - k0, krem = s >= s1 ? 0 : left < BK ? left : BK;
         const int ia = kMode == kSeg2 ? seg : z, ib = kMode == kGated ? (second ? 1 : 0) : ia;
-        char* sl = gemm_smem + slot * Tile::kStageBytes;
-        const int64_t lda = a.a[ia].ld, ldb = a.b[ib].ld;
-        const char* pa = reinterpret_cast<const char*>(a.a[ia].p);
-        const char* pb = reinterpret_cast<const char*>(a.b[ib].p);
-        // spans end with the last valid row's last valid element
-        if constexpr (kAKc) pa += (m0 * lda + k0) * SZ;
-        else pa += (k0 * lda + m0) * SZ;
-        if constexpr (kBKc) pb += (n0 * ldb + k0) * SZ;
-        else pb += (k0 * ldb + n0) * SZ;
-        const int64_t ba = krem <= 0 ? 0 : kAKc ? ((int64_t)(a.M - m0 - 1) * lda + krem) * SZ : ((int64_t)(krem - 1) * lda + (a.M - m0)) * SZ;
-        const int kb = kBKc || krem <= 0 ? krem : a.KB[seg] - k0;
-        const int64_t bb = kb <= 0 ? 0 : kBKc ? ((int64_t)(a.N - n0 - 1) * ldb + kb) * SZ : ((int64_t)(kb - 1) * ldb + (a.N - n0)) * SZ;
-        const int pieces = krem <= 0 ? 0 : (krem * SZ) >> 4;
-        la.issue(pa, ba, pieces, sl, wave);
-        lb.issue(pb, bb, pieces, sl + BM * 128, wave);
+        const int bleft = a.KB[seg] - k0;
+        const int brem = kBKc || krem < bleft ? krem : bleft;  // may be negative
+        const int lda = (int)a.a[ia].ld, ldb = (int)a.b[ib].ld;
+        pa = reinterpret_cast<const char*>(a.a[ia].p) + (kAKc ? (int64_t)m0 * lda + k0 : (int64_t)k0 * lda + m0) * SZ;
+        pb = reinterpret_cast<const char*>(a.b[ib].p) + (kBKc ? (int64_t)n0 * ldb + k0 : (int64_t)k0 * ldb + n0) * SZ;
+        pa_step = kAKc ? 128 : (int64_t)BK * lda * SZ;
+        pb_step = kBKc ? 128 : (int64_t)BK * ldb * SZ;
+        ba = krem <= 0 || ra_rows <= 0 ? 0 : (kAKc ? (ra_rows - 1) * lda + krem : (krem - 1) * lda + ra_rows) * SZ;
+        bb = brem <= 0 || rb_rows <= 0 ? 0 : (kBKc ? (rb_rows - 1) * ldb + brem : (brem - 1) * ldb + rb_rows) * SZ;
+        const int pieces = krem < BK ? (krem * SZ) >> 4 : 8;
+        la.init(wave, lane, lda, 0, pieces);
+        lb.init(wave, lane, ldb, second ? BN / 2 : 0, pieces);
+        // whole steps of this term for both operands, then the next turn
+        const int whole = (kBKc || a.K[seg] < a.KB[seg] ? a.K[seg] : a.KB[seg]) / BK + (seg ? st0 : 0);
+        const int end = seg || kMode != kSeg2 ? steps : st0;
+        turn = s >= s1 ? 0x7fffffff : s < whole ? whole : s + 1 < end ? s + 1 : end;
+        if (turn > s1 && s < s1) turn = s1;
+    };
+    auto advance = [&](int s) {  // to step s, one past the last set up
+        if (s == turn) {
+            set_up(s);
+        } else {
+            pa += pa_step;
+            pb += pb_step;
+        }
+    };
+    const unsigned lds0 = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)gemm_smem);
+    auto fetch = [&](int i, int slot) {  // instruction i of NLD
+        const unsigned sl = lds0 + slot * Tile::kStageBytes;
+        if (i < LA::NI) la.issue(i, pa, ba, sl, wave);
+        else lb.issue(i - LA::NI, pb, bb, sl + BM * 128, wave);
     };
 
-    GemmReader<T, kAKc, BM> ra;
-    GemmReader<T, kBKc, BN> rb;
+    GemmReader<T, kAKc, BM, MF> ra;
+    GemmReader<T, kBKc, BN, MF> rb;
     ra.init(lane);
     rb.init(lane);
     const int wm = wave / Tile::WGN, wn = wave % Tile::WGN;
     auto unit_b = [&](int fn) {
         if constexpr (kMode == kGated)
-            return fn < FN / 2 ? wn * (FN / 2) + fn : BN / 32 + wn * (FN / 2) + fn - FN / 2;
+            return fn < FN / 2 ? wn * (FN / 2) + fn : BN / (2 * MF) + wn * (FN / 2) + fn - FN / 2;
         else
             return wn * FN + fn;
     };
 
-    f32x4 acc[FM][FN];
+    typename Type::Acc acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
+        for (int j = 0; j < FN; ++j)
 #pragma unroll
-    for (int s = 0; s < ST - 1; ++s) issue(s0 + s, s);
+            for (int e = 0; e < MF * MF / 64; ++e) acc[i][j][e] = 0.f;
+
+    // A step is two halves of KH k steps. While one half's fragments are multiplied, the next half's
+    // are read from LDS; all of step s has been read halfway through it, which frees its slot
+    // for step s + ST. Copies and reads are issued between groups of FN MFMAs, which cover them, two
+    // a group: early in the half, so that they have landed when they are waited for.
+    typedef typename Type::Frag Frag;
+    constexpr int KH = MF == 16 ? 1 : 2;
+    constexpr int kGroups = KH * FM, kReads = KH * (FM + FN);
+    Frag fa[2][KH][FM], fb[2][KH][FN];
+    auto read = [&](int half, int slot, int i) {  // fragment i of a half
+        const char* ta = gemm_smem + slot * Tile::kStageBytes;
+        const int ks = i / (FM + FN), r = i % (FM + FN);
+        if (r < FN) fb[half][ks][r] = rb.read(ta + BM * 128, unit_b(r), half * KH + ks);
+        else fa[half][ks][r - FN] = ra.read(ta, wm * FM + r - FN, half * KH + ks);
+    };
+    auto group = [&](int half, int g) {
+        const int ks = g / FM, i = g % FM;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = Type::mma(fb[half][ks][j], fa[half][ks][i], acc[i][j]);
+    };
+    constexpr int kPer = (kReads + kGroups - 1) / kGroups < 2 ? 2 : (kReads + kGroups - 1) / kGroups;
+    constexpr int kPerLd = (NLD + kGroups - 1) / kGroups < 2 ? 2 : (NLD + kGroups - 1) / kGroups;
+
+    set_up(s0);
+#pragma unroll
+    for (int s = 0; s < ST; ++s) {
+        if (s) advance(s0 + s);
+#pragma unroll
+        for (int i = 0; i < NLD; ++i) fetch(i, s);
+    }
+    wait_vm_lds<NLD * (ST - 1)>();
+    M3_LDS_FENCE();
+    __builtin_amdgcn_s_barrier();
+    M3_LDS_FENCE();
+#pragma unroll
+    for (int i = 0; i < kReads; ++i) read(0, 0, i);
     int slot = 0;
     for (int s = s0; s < s1; ++s) {
-        // step s has landed, and every wave has read step s - 1 out of the slot to be refilled
-        wait_vm_lds<NLD * (ST - 2)>();
+        M3_FENCE();
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+            for (int i = g * kPer; i < (g + 1) * kPer && i < kReads; ++i) read(1, slot, i);
+            M3_FENCE();
+            group(0, g);
+            M3_FENCE();
+        }
+        advance(s + ST);
+        const int next = slot + 1 == ST ? 0 : slot + 1;
+        wait_vm_lds<NLD * (ST - 2)>();  // step s + 1 has landed, this wave has read step s
         M3_LDS_FENCE();
         __builtin_amdgcn_s_barrier();
         M3_LDS_FENCE();
-        {
-            int next = slot + ST - 1;
-            next = next >= ST ? next - ST : next;
-            issue(s + ST - 1, next);
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+            for (int i = g * kPerLd; i < (g + 1) * kPerLd && i < NLD; ++i) fetch(i, slot);
+#pragma unroll
+            for (int i = g * kPer; i < (g + 1) * kPer && i < kReads; ++i) read(0, next, i);
+            M3_FENCE();
+            group(1, g);
+            M3_FENCE();
         }
-        const char* ta = gemm_smem + slot * Tile::kStageBytes;
-        const char* tb = ta + BM * 128;
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            typename GemmType<T>::Frag fa[FM], fb[FN];
-#pragma unroll
-            for (int j = 0; j < FN; ++j) fb[j] = rb.read(tb, unit_b(j), ks);
-#pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = ra.read(ta, wm * FM + i, ks);
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = GemmType<T>::mma(fb[j], fa[i], acc[i][j]);
-        }
-        slot = slot + 1 == ST ? 0 : slot + 1;
+        slot = next;
     }
     wait_vm_lds<0>();  // nothing writes LDS once the epilogue uses it
     M3_LDS_FENCE();

@@ -9,9 +9,9 @@ namespace m3 {
 
 // Tiles: 256 x 256 by 8 waves (bf16 only; one block a CU), 128 x 128 by 4 waves (two blocks a
 // CU), 64 x 64 by 4 waves, four steps deep (two blocks a CU).
-typedef GemmTile<256, 256, 2, 4, 2> TileL;
-typedef GemmTile<128, 128, 2, 2, 2> TileM;
-typedef GemmTile<64, 64, 2, 2, 4> TileS;
+typedef GemmTile<256, 256, 2, 4, 2, 16> TileL;
+template <typename T> using TileM = GemmTile<128, 128, 2, 2, 2, sizeof(T) == 2 ? 16 : 32>;
+typedef GemmTile<64, 64, 2, 2, 4, 16> TileS;
 enum { kTileL = 0, kTileM = 1, kTileS = 2 };
 
 struct GemmPlan {
@@ -54,10 +54,10 @@ int gemm_dispatch(int dtype, const GemmPlan& p, const GemmArgs& a, const Epi& ep
                   int batch, hipStream_t stream) {
     if (dtype == M3_DTYPE_BF16) {
         if (p.tile == kTileL) return gemm_launch<bf16, TileL, kAKc, kBKc, kMode>(a, epi, rows, cols, batch, stream);
-        if (p.tile == kTileM) return gemm_launch<bf16, TileM, kAKc, kBKc, kMode>(a, epi, rows, cols, batch, stream);
+        if (p.tile == kTileM) return gemm_launch<bf16, TileM<bf16>, kAKc, kBKc, kMode>(a, epi, rows, cols, batch, stream);
         return gemm_launch<bf16, TileS, kAKc, kBKc, kMode>(a, epi, rows, cols, batch, stream);
     }
-    if (p.tile == kTileM) return gemm_launch<float, TileM, kAKc, kBKc, kMode>(a, epi, rows, cols, batch, stream);
+    if (p.tile == kTileM) return gemm_launch<float, TileM<float>, kAKc, kBKc, kMode>(a, epi, rows, cols, batch, stream);
     return gemm_launch<float, TileS, kAKc, kBKc, kMode>(a, epi, rows, cols, batch, stream);
 }
 

@@ -23,7 +23,7 @@ struct EpiStore {
 
     template <typename T, typename Tile, int kMode>
     __device__ __forceinline__ void run(const GemmArgs& a, const GemmPlace<Tile, kMode>& at,
-                                        f32x4 (&acc)[Tile::FM][Tile::FN], char*, int, int, int z) const {
+                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char*, int, int, int z) const {
         T* out = reinterpret_cast<T*>(s.out[z]);
         const T* res = reinterpret_cast<const T*>(s.res);
         float* part = s.part ? s.part + ((int64_t)blockIdx.z * gridDim.y + z) * s.rows * s.cols : nullptr;
@@ -32,10 +32,10 @@ struct EpiStore {
             const int m = at.m(i);
             if (m >= s.rows) continue;
 #pragma unroll
-            for (int j = 0; j < Tile::FN; ++j) {
-                const int n = at.n(j);
+            for (int j = 0; j < Tile::FN * Tile::Q; ++j) {
+                const int n = at.n(j / Tile::Q, j % Tile::Q);
                 if (n >= s.cols) continue;
-                f32x4 v = acc[i][j];
+                f32x4 v = four(acc[i][j / Tile::Q], j % Tile::Q);
                 if (part) {
                     float* p = part + (int64_t)m * s.cols + n;
                     if (vec) {

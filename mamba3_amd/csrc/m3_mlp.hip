@@ -83,17 +83,18 @@ struct EpiGated {
 
     template <typename T, typename Tile, int kMode>
     __device__ __forceinline__ void run(const GemmArgs&, const GemmPlace<Tile, kMode>& at,
-                                        f32x4 (&acc)[Tile::FM][Tile::FN], char*, int, int, int) const {
+                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char*, int, int, int) const {
         const int64_t plane = (int64_t)rows * ldh;
 #pragma unroll
         for (int i = 0; i < Tile::FM; ++i) {
             const int m = at.m(i);
             if (m >= rows) continue;
 #pragma unroll
-            for (int j = 0; j < Tile::FN / 2; ++j) {
-                const int n = at.n(j);
+            for (int jq = 0; jq < Tile::FN / 2 * Tile::Q; ++jq) {
+                const int j = jq / Tile::Q, q = jq % Tile::Q;
+                const int n = at.n(j, q);
                 if (n >= ldh) continue;
-                const f32x4 g = acc[i][j], u = acc[i][j + Tile::FN / 2];
+                const f32x4 g = four(acc[i][j], q), u = four(acc[i][j + Tile::FN / 2], q);
                 const int64_t o = (int64_t)m * ldh + n;
                 f32x4 v;
 #pragma unroll
@@ -113,22 +114,23 @@ struct EpiGateBwd {
 
     template <typename T, typename Tile, int kMode>
     __device__ __forceinline__ void run(const GemmArgs&, const GemmPlace<Tile, kMode>& at,
-                                        f32x4 (&acc)[Tile::FM][Tile::FN], char*, int, int, int) const {
+                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char*, int, int, int) const {
         const int64_t plane = (int64_t)rows * ldh;
 #pragma unroll
         for (int i = 0; i < Tile::FM; ++i) {
             const int m = at.m(i);
             if (m >= rows) continue;
 #pragma unroll
-            for (int j = 0; j < Tile::FN; ++j) {
-                const int n = at.n(j);
+            for (int j = 0; j < Tile::FN * Tile::Q; ++j) {
+                const int n = at.n(j / Tile::Q, j % Tile::Q);
                 if (n >= ldh) continue;
                 const int64_t o = (int64_t)m * ldh + n;
+                const f32x4 v = four(acc[i][j / Tile::Q], j % Tile::Q);
                 f32x4 g, u, a, b;
                 kept_gu<T>(saved, o, plane, g, u);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float s = sigmoid_of<T>(g[e]), dh = acc[i][j][e] * alpha;
+                    const float s = sigmoid_of<T>(g[e]), dh = v[e] * alpha;
                     a[e] = dh * u[e] * s * (1.f + g[e] * (1.f - s));
                     b[e] = dh * g[e] * s;
                 }

@@ -41,7 +41,7 @@ struct EpiXentFwd {
 
     template <typename T, typename Tile, int kMode>
     __device__ __forceinline__ void run(const GemmArgs&, const GemmPlace<Tile, kMode>& at,
-                                        f32x4 (&acc)[Tile::FM][Tile::FN], char* smem, int tm, int tn, int) const {
+                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, int tm, int tn, int) const {
         float2* red = reinterpret_cast<float2*>(smem);  // [WGN][BM]
 #pragma unroll
         for (int i = 0; i < Tile::FM; ++i) {
@@ -49,30 +49,32 @@ struct EpiXentFwd {
             const int64_t t = m < rows ? target[m] : -1;
             float top = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < Tile::FN; ++j) {
-                const int n = at.n(j);
+            for (int j = 0; j < Tile::FN * Tile::Q; ++j) {
+                const int n = at.n(j / Tile::Q, j % Tile::Q);
+                const f32x4 v = four(acc[i][j / Tile::Q], j % Tile::Q);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if (n + e < vocab) {
-                        top = fmaxf(top, acc[i][j][e]);
-                        if (t == n + e) zt[m] = acc[i][j][e];
+                        top = fmaxf(top, v[e]);
+                        if (t == n + e) zt[m] = v[e];
                     }
                 }
             }
-            top = fmaxf(top, __shfl_xor(top, 16, kWave));
-            top = fmaxf(top, __shfl_xor(top, 32, kWave));
+#pragma unroll
+            for (int off = Tile::MF; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off, kWave));
             float sum = 0.f;
             const float ref = top == -INFINITY ? 0.f : top;  // a row without finite logits
 #pragma unroll
-            for (int j = 0; j < Tile::FN; ++j) {
-                const int n = at.n(j);
+            for (int j = 0; j < Tile::FN * Tile::Q; ++j) {
+                const int n = at.n(j / Tile::Q, j % Tile::Q);
+                const f32x4 v = four(acc[i][j / Tile::Q], j % Tile::Q);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (n + e < vocab) sum += exp_of<T>(acc[i][j][e] - ref);
+                    if (n + e < vocab) sum += exp_of<T>(v[e] - ref);
             }
-            sum += __shfl_xor(sum, 16, kWave);
-            sum += __shfl_xor(sum, 32, kWave);
-            if (at.lane < 16) red[at.wn * Tile::BM + at.local_m(i)] = make_float2(top, sum);
+#pragma unroll
+            for (int off = Tile::MF; off < 64; off *= 2) sum += __shfl_xor(sum, off, kWave);
+            if (at.lane < Tile::MF) red[at.wn * Tile::BM + at.local_m(i)] = make_float2(top, sum);
         }
         __syncthreads();
         for (int r = threadIdx.x; r < Tile::BM; r += Tile::NT) {
@@ -99,7 +101,7 @@ struct EpiXentBwd {
 
     template <typename T, typename Tile, int kMode>
     __device__ __forceinline__ void run(const GemmArgs&, const GemmPlace<Tile, kMode>& at,
-                                        f32x4 (&acc)[Tile::FM][Tile::FN], char*, int, int, int) const {
+                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char*, int, int, int) const {
         typedef T T4 __attribute__((ext_vector_type(4)));
         const float all = reduction == M3_REDUCTION_NONE ? 0.f : gl[0];
         const float each = reduction == M3_REDUCTION_MEAN ? all / count[0] : all;
@@ -113,13 +115,14 @@ struct EpiXentBwd {
             if (t < 0 || t >= vocab) g = NAN;
             const float l = lse[m];
 #pragma unroll
-            for (int j = 0; j < Tile::FN; ++j) {
-                const int n = at.n(j);
+            for (int j = 0; j < Tile::FN * Tile::Q; ++j) {
+                const int n = at.n(j / Tile::Q, j % Tile::Q);
                 if (n >= ld) continue;
+                const f32x4 v = four(acc[i][j / Tile::Q], j % Tile::Q);
                 T4 o;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float p = exp_of<T>(acc[i][j][e] - l);
+                    float p = exp_of<T>(v[e] - l);
                     if (t == v0 + n + e) p -= 1.f;
                     o[e] = (T)(live && v0 + n + e < vocab ? p * g : 0.f);
                 }
