@@ -197,6 +197,12 @@ struct GemmPlace {
     int m0, n0, wm, wn, lane;
     __device__ __forceinline__ int local_m(int fm) const { return (wm * Tile::FM + fm) * MF + lane % MF; }
     __device__ __forceinline__ int m(int fm) const { return m0 + local_m(fm); }
+    __device__ __forceinline__ int wave() const { return wm * Tile::WGN + wn; }
+    __device__ __forceinline__ int row0(int fm) const { return m0 + (wm * Tile::FM + fm) * MF; }  // of the piece
+    __device__ __forceinline__ int col0() const {  // of the wave
+        constexpr int F = kMode == kGated ? Tile::FN / 2 : Tile::FN;
+        return n0 + wn * F * MF;
+    }
     // kGated: fn < FN / 2 of the gate; the up piece of the same columns is fn + FN / 2
     __device__ __forceinline__ int n(int fn, int q) const {
         constexpr int F = kMode == kGated ? Tile::FN / 2 : Tile::FN;
@@ -207,6 +213,42 @@ template <typename Acc>
 __device__ __forceinline__ f32x4 four(const Acc& v, int q) {
     return f32x4{v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]};
 }
+
+// Stores MF rows of a wave's results as whole rows: fours go into a wave-private part of LDS and leave it
+// as 16 bytes a lane, kCols columns of a row side by side (64 to 256 bytes), where storing them as
+// the MFMA leaves them would write 8 bytes to each of 16 rows. LDS operations of one wave run in
+// order, so no barrier is needed.
+template <typename T, typename Tile, int kCols>
+struct GemmRows {
+    static constexpr int MF = Tile::MF, E = 16 / sizeof(T);
+    static constexpr int kPitch = kCols * (int)sizeof(T) + 16;
+    static constexpr int LPR = kCols / E, RPI = 64 / LPR;  // lanes a row, rows an instruction
+    static_assert(Tile::NW * MF * kPitch <= Tile::kLds, "rows fit LDS");
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    typedef T Piece __attribute__((ext_vector_type(E)));
+    char* mine;
+    int lane;
+    __device__ __forceinline__ GemmRows(char* smem, int wave, int lane_) : mine(smem + wave * (MF * kPitch)), lane(lane_) {}
+    // columns fn * MF + q * 8 + ... of row lane % MF
+    __device__ __forceinline__ void put(int fn, int q, f32x4 v) const {
+        T4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (T)v[e];
+        *reinterpret_cast<T4*>(mine + lane % MF * kPitch + (fn * MF + q * 8 + lane / MF * 4) * (int)sizeof(T)) = o;
+    }
+    // row r of the MF to out + r * ld for r < rows; columns come in whole pieces, cols of them exist
+    __device__ __forceinline__ void store(T* out, int64_t ld, int rows, int cols) const {
+        const int r0 = lane / LPR, c = lane % LPR * E;
+        M3_LDS_FENCE();  // the fours and the pieces are other types to the compiler
+#pragma unroll
+        for (int i = 0; i < (MF + RPI - 1) / RPI; ++i) {
+            const int r = i * RPI + r0;
+            if (r < MF && r < rows && c < cols)
+                *reinterpret_cast<Piece*>(out + r * ld + c) = *reinterpret_cast<const Piece*>(mine + r * kPitch + c * (int)sizeof(T));
+        }
+        M3_LDS_FENCE();
+    }
+};
 
 // Block -> tile: the blocks of one XCD (dispatch is round robin over 8) take a contiguous run of
 // tiles, and runs walk groups of 8 row tiles column by column, so that an XCD's L2 serves

@@ -61,7 +61,7 @@ int gemm_dispatch(int dtype, const GemmPlan& p, const GemmArgs& a, const Epi& ep
     return gemm_launch<float, TileS, kAKc, kBKc, kMode>(a, epi, rows, cols, batch, stream);
 }
 
-// Stores a product (m3_gemm_store.hip): out[z] (rows x cols, row stride ldo) = alpha * (A B) [+ res],
+// Stores a product (m3_gemm_store.hip): out[z] (rows x cols, row stride ldo) = alpha * num / den * (A B) [+ res],
 // or, split or accumulated over calls, fp32 partial sums in `part` that gemm_reduce joins.
 struct GemmStore {
     void* out[2];
@@ -71,6 +71,7 @@ struct GemmStore {
     float* part;      // [splits][batch][rows][cols]
     int add;          // the partial sums of an earlier call stay in `part`
     int rows, cols;
+    const float *num = nullptr, *den = nullptr;  // on the device: a factor num / den (0 where den is 0)
 };
 enum GemmForm {
     kFormNT,  // A rows of k, B rows of k
@@ -79,7 +80,7 @@ enum GemmForm {
 };
 int gemm_store(GemmForm form, int dtype, const GemmPlan& p, GemmArgs a, const GemmStore& st, int batch,
                hipStream_t stream);
-// out[z] = alpha * sum over s of part[s][z] [+ res]
+// out[z] = alpha * num / den * sum over s of part[s][z] [+ res]
 int gemm_reduce(int dtype, const GemmStore& st, int splits, int batch, hipStream_t stream);
 inline size_t gemm_part_bytes(const GemmPlan& p, int batch, int64_t rows, int64_t cols) {
     return p.splits > 1 ? (size_t)up256((int64_t)p.splits * batch * rows * cols * 4) : 0;

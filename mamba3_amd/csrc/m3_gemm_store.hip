@@ -17,64 +17,95 @@ __device__ __forceinline__ void store4(T* p, f32x4 v) {
     }
 }
 
+// alpha with the factor that lies on the device
+__device__ __forceinline__ float store_scale(const GemmStore& s) {
+    float f = s.alpha;
+    if (s.num) f *= s.num[0];
+    if (s.den) f = s.den[0] == 0.f ? 0.f : f / s.den[0];
+    return f;
+}
+
 struct EpiStore {
     GemmStore s;
-    bool vec;  // four columns at once
+    bool vec;  // whole 16-byte pieces
 
     template <typename T, typename Tile, int kMode>
     __device__ __forceinline__ void run(const GemmArgs& a, const GemmPlace<Tile, kMode>& at,
-                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char*, int, int, int z) const {
+                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, int, int, int z) const {
         T* out = reinterpret_cast<T*>(s.out[z]);
         const T* res = reinterpret_cast<const T*>(s.res);
-        float* part = s.part ? s.part + ((int64_t)blockIdx.z * gridDim.y + z) * s.rows * s.cols : nullptr;
-#pragma unroll
-        for (int i = 0; i < Tile::FM; ++i) {
-            const int m = at.m(i);
-            if (m >= s.rows) continue;
-#pragma unroll
-            for (int j = 0; j < Tile::FN * Tile::Q; ++j) {
-                const int n = at.n(j / Tile::Q, j % Tile::Q);
-                if (n >= s.cols) continue;
-                f32x4 v = four(acc[i][j / Tile::Q], j % Tile::Q);
-                if (part) {
-                    float* p = part + (int64_t)m * s.cols + n;
-                    if (vec) {
-                        if (s.add) v += *reinterpret_cast<const f32x4*>(p);
-                        *reinterpret_cast<f32x4*>(p) = v;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (n + e < s.cols) p[e] = s.add ? p[e] + v[e] : v[e];
-                    }
-                    continue;
-                }
-                const int64_t o = (int64_t)m * s.ldo + n;
+        const float alpha = s.part ? 1.f : store_scale(s);
+        if (s.part) {
+            float* part = s.part + ((int64_t)blockIdx.z * gridDim.y + z) * s.rows * s.cols;
+            each(at, acc, [&](int m, int n, f32x4 v) {
+                float* p = part + (int64_t)m * s.cols + n;
                 if (vec) {
-                    v *= s.alpha;
-                    if (res) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] += (float)res[o + e];
-                    }
-                    store4(out + o, v);
+                    if (s.add) v += *reinterpret_cast<const f32x4*>(p);
+                    *reinterpret_cast<f32x4*>(p) = v;
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (n + e < s.cols) out[o + e] = (T)(v[e] * s.alpha + (res ? (float)res[o + e] : 0.f));
+                        if (n + e < s.cols) p[e] = s.add ? p[e] + v[e] : v[e];
                 }
+            });
+        } else if (vec) {
+            const GemmRows<T, Tile, Tile::FN * Tile::MF> rows(smem, at.wave(), at.lane);
+#pragma unroll
+            for (int i = 0; i < Tile::FM; ++i) {
+                const int m = at.m(i), r0 = at.row0(i), c0 = at.col0();
+#pragma unroll
+                for (int j = 0; j < Tile::FN; ++j)
+#pragma unroll
+                    for (int q = 0; q < Tile::Q; ++q) {
+                        f32x4 v = four(acc[i][j], q) * alpha;
+                        const int n = at.n(j, q);
+                        if (res && m < s.rows && n < s.cols) {
+                            typedef T T4 __attribute__((ext_vector_type(4)));
+                            const T4 r = *reinterpret_cast<const T4*>(res + (int64_t)m * s.ldo + n);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[e] += (float)r[e];
+                        }
+                        rows.put(j, q, v);
+                    }
+                rows.store(out + (int64_t)r0 * s.ldo + c0, s.ldo, s.rows - r0, s.cols - c0);
+            }
+        } else {
+            each(at, acc, [&](int m, int n, f32x4 v) {
+                const int64_t o = (int64_t)m * s.ldo + n;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < s.cols) out[o + e] = (T)(v[e] * alpha + (res ? (float)res[o + e] : 0.f));
+            });
+        }
+    }
+
+    // f(m, n, four) for the fours that begin inside the result
+    template <typename Place, typename Acc, int FM, int FN, typename F>
+    __device__ __forceinline__ void each(const Place& at, Acc (&acc)[FM][FN], F f) const {
+        constexpr int Q = sizeof(Acc) / 16;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const int m = at.m(i);
+            if (m >= s.rows) continue;
+#pragma unroll
+            for (int j = 0; j < FN * Q; ++j) {
+                const int n = at.n(j / Q, j % Q);
+                if (n < s.cols) f(m, n, four(acc[i][j / Q], j % Q));
             }
         }
     }
 };
 
-static bool four_columns(const GemmStore& s) {
+static bool whole_pieces(int dtype, const GemmStore& s) {
+    const int e = dtype == M3_DTYPE_BF16 ? 8 : 4;
     auto al = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-    return s.cols % 4 == 0 && s.ldo % 4 == 0 && al(s.out[0]) && al(s.out[1]) && al(s.res);
+    return s.cols % e == 0 && s.ldo % e == 0 && al(s.out[0]) && al(s.out[1]) && al(s.res);
 }
 
 int gemm_store(GemmForm form, int dtype, const GemmPlan& p, GemmArgs a, const GemmStore& st, int batch,
                hipStream_t stream) {
     a.splits = p.splits;
-    EpiStore e{st, four_columns(st)};
+    EpiStore e{st, whole_pieces(dtype, st)};
     if (p.splits == 1 && !st.add && st.out[0]) e.s.part = nullptr;
     int r;
     if (form == kFormNT) r = gemm_dispatch<true, true, kPlain>(dtype, p, a, e, st.rows, st.cols, 1, stream);
@@ -92,6 +123,7 @@ __global__ __launch_bounds__(256) void gemm_reduce_kernel(GemmStore s, int split
     const float* part = s.part + z * each;
     T* out = reinterpret_cast<T*>(s.out[z]);
     const T* res = reinterpret_cast<const T*>(s.res);
+    const float alpha = store_scale(s);
     const int64_t pieces = kVec ? each / 4 : each;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * 256) {
         const int64_t at = kVec ? i * 4 : i;
@@ -99,20 +131,20 @@ __global__ __launch_bounds__(256) void gemm_reduce_kernel(GemmStore s, int split
         if constexpr (kVec) {
             f32x4 v{0.f, 0.f, 0.f, 0.f};
             for (int k = 0; k < splits; ++k) v += *reinterpret_cast<const f32x4*>(part + k * stride + at);
-            v *= s.alpha;
+            v *= alpha;
             if (res)
                 for (int e = 0; e < 4; ++e) v[e] += (float)res[o + e];
             store4(out + o, v);
         } else {
             float v = 0.f;
             for (int k = 0; k < splits; ++k) v += part[k * stride + at];
-            out[o] = (T)(v * s.alpha + (res ? (float)res[o] : 0.f));
+            out[o] = (T)(v * alpha + (res ? (float)res[o] : 0.f));
         }
     }
 }
 
 int gemm_reduce(int dtype, const GemmStore& st, int splits, int batch, hipStream_t stream) {
-    const bool vec = four_columns(st);
+    const bool vec = whole_pieces(dtype, st);
     const int64_t pieces = (int64_t)st.rows * st.cols / (vec ? 4 : 1);
     const dim3 grid((unsigned)std::min<int64_t>((pieces + 255) / 256, 8192), (unsigned)batch);
     if (dtype == M3_DTYPE_BF16) {

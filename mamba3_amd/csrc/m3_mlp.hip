@@ -8,8 +8,8 @@
 // epilogue reads g and u and writes dg and du, the operands of the four gradient products (dx
 // is one product of two terms; dWg and dWu are one launch).
 //
-// For the backward the forward keeps g and u. bf16: their upper 24 bits as three planes of
-// 16 bits (g's upper 16, u's upper 16, the next 8 of both): a bf16 copy alone would put a rounding
+// For the backward the forward keeps g and u. bf16: their upper 24 bits (the upper 16 of each, and the
+// next 8 of both in another 16): a bf16 copy alone would put a rounding
 // of g and one of u (2^-9 each) into dg and du next to their own; 24 bits leave 2^-16 for 2 more
 // bytes an element. fp32: as they are.
 #include "m3_gemm_host.h"
@@ -18,125 +18,154 @@
 namespace m3 {
 
 typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
 
 template <typename T> __device__ __forceinline__ float sigmoid_of(float g);
 template <> __device__ __forceinline__ float sigmoid_of<bf16>(float g) { return __builtin_amdgcn_rcpf(1.f + fast_exp(-g)); }
 template <> __device__ __forceinline__ float sigmoid_of<float>(float g) { return sigmoid_f(g); }
 
+// Where g and u of four columns n .. n + 3 of row m are kept: blocks of 16 x 16 elements in a row of
+// blocks, in a block the fours of 16 rows side by side for each four columns. The 16 lanes that
+// hold the same columns of a piece (m3_gemm.h) then write and read a contiguous run, where rows
+// would take 8 bytes of each of 16 rows.
+struct KeptGu {
+    void* p;
+    int64_t elements;  // rows and columns rounded up to 16
+    int blocks;        // a row of blocks
+    __device__ __forceinline__ int64_t at(int m, int n) const {
+        return ((int64_t)(m >> 4) * blocks + (n >> 4)) * 256 + ((n & 15) >> 2) * 64 + (m & 15) * 4;
+    }
+};
+
+// bf16: [element fours][g upper 16 x 4, u upper 16 x 4], then [element fours][the next 8 of both x 4].
+// fp32: g, then u.
 template <typename T>
-__device__ __forceinline__ void keep_gu(void* saved, int64_t at, int64_t plane, f32x4 g, f32x4 u) {
+__device__ __forceinline__ void keep_gu(const KeptGu& k, int64_t at, f32x4 g, f32x4 u) {
     if constexpr (sizeof(T) == 2) {
-        unsigned short* p = reinterpret_cast<unsigned short*>(saved) + at;
-        u16x4 gh, uh, lo;
+        u16x8 hi;
+        u16x4 lo;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             // (__builtin_bit_cast of a vector's component takes component 0 on this compiler)
             const float ge = g[e], ue = u[e];
             const unsigned gb = __builtin_bit_cast(unsigned, ge), ub = __builtin_bit_cast(unsigned, ue);
-            gh[e] = (unsigned short)(gb >> 16);
-            uh[e] = (unsigned short)(ub >> 16);
+            hi[e] = (unsigned short)(gb >> 16);
+            hi[4 + e] = (unsigned short)(ub >> 16);
             lo[e] = (unsigned short)((gb >> 8 & 0xff) | (ub & 0xff00));
         }
-        *reinterpret_cast<u16x4*>(p) = gh;
-        *reinterpret_cast<u16x4*>(p + plane) = uh;
-        *reinterpret_cast<u16x4*>(p + 2 * plane) = lo;
+        unsigned short* p = reinterpret_cast<unsigned short*>(k.p);
+        *reinterpret_cast<u16x8*>(p + 2 * at) = hi;
+        *reinterpret_cast<u16x4*>(p + 2 * k.elements + at) = lo;
     } else {
-        float* p = reinterpret_cast<float*>(saved) + at;
+        float* p = reinterpret_cast<float*>(k.p) + at;
         *reinterpret_cast<f32x4*>(p) = g;
-        *reinterpret_cast<f32x4*>(p + plane) = u;
+        *reinterpret_cast<f32x4*>(p + k.elements) = u;
     }
 }
 
 template <typename T>
-__device__ __forceinline__ void kept_gu(const void* saved, int64_t at, int64_t plane, f32x4& g, f32x4& u) {
-    if constexpr (sizeof(T) == 2) {
-        const unsigned short* p = reinterpret_cast<const unsigned short*>(saved) + at;
-        const u16x4 gh = *reinterpret_cast<const u16x4*>(p), uh = *reinterpret_cast<const u16x4*>(p + plane),
-                    lo = *reinterpret_cast<const u16x4*>(p + 2 * plane);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            g[e] = __builtin_bit_cast(float, (unsigned)gh[e] << 16 | (lo[e] & 0xffu) << 8);
-            u[e] = __builtin_bit_cast(float, (unsigned)uh[e] << 16 | (lo[e] & 0xff00u));
+struct KeptFour {
+    u16x8 hi;
+    u16x4 lo;
+    f32x4 g, u;
+    __device__ __forceinline__ void load(const KeptGu& k, int64_t at) {
+        if constexpr (sizeof(T) == 2) {
+            const unsigned short* p = reinterpret_cast<const unsigned short*>(k.p);
+            hi = *reinterpret_cast<const u16x8*>(p + 2 * at);
+            lo = *reinterpret_cast<const u16x4*>(p + 2 * k.elements + at);
+        } else {
+            const float* p = reinterpret_cast<const float*>(k.p) + at;
+            g = *reinterpret_cast<const f32x4*>(p);
+            u = *reinterpret_cast<const f32x4*>(p + k.elements);
         }
-    } else {
-        const float* p = reinterpret_cast<const float*>(saved) + at;
-        g = *reinterpret_cast<const f32x4*>(p);
-        u = *reinterpret_cast<const f32x4*>(p + plane);
     }
-}
+    __device__ __forceinline__ void get(int e, float& ge, float& ue) const {
+        if constexpr (sizeof(T) == 2) {
+            ge = __builtin_bit_cast(float, (unsigned)hi[e] << 16 | (lo[e] & 0xffu) << 8);
+            ue = __builtin_bit_cast(float, (unsigned)hi[4 + e] << 16 | (lo[e] & 0xff00u));
+        } else {
+            ge = g[e];
+            ue = u[e];
+        }
+    }
+};
 
-template <typename T>
-__device__ __forceinline__ void put4(T* p, f32x4 v) {
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    T4 o;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = (T)v[e];
-    *reinterpret_cast<T4*>(p) = o;
-}
-
-// Columns come in fours: the hidden width is padded to 16 bytes, its pad columns are zero (their
-// weight rows read as zero) and are stored as zeros.
+// Columns come in whole 16-byte pieces: the hidden width is padded to 16 bytes, its pad columns are
+// zero (their weight rows read as zero) and are stored as zeros.
 struct EpiGated {
     void* h;      // rows x ldh
-    void* saved;  // nullptr: no backward
+    KeptGu kept;  // p nullptr: no backward
     int rows, ldh;
 
     template <typename T, typename Tile, int kMode>
     __device__ __forceinline__ void run(const GemmArgs&, const GemmPlace<Tile, kMode>& at,
-                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char*, int, int, int) const {
-        const int64_t plane = (int64_t)rows * ldh;
+                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, int, int, int) const {
+        const GemmRows<T, Tile, Tile::FN / 2 * Tile::MF> out(smem, at.wave(), at.lane);
 #pragma unroll
         for (int i = 0; i < Tile::FM; ++i) {
-            const int m = at.m(i);
-            if (m >= rows) continue;
+            const int m = at.m(i), r0 = at.row0(i), c0 = at.col0();
 #pragma unroll
             for (int jq = 0; jq < Tile::FN / 2 * Tile::Q; ++jq) {
                 const int j = jq / Tile::Q, q = jq % Tile::Q;
                 const int n = at.n(j, q);
-                if (n >= ldh) continue;
                 const f32x4 g = four(acc[i][j], q), u = four(acc[i][j + Tile::FN / 2], q);
-                const int64_t o = (int64_t)m * ldh + n;
                 f32x4 v;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = g[e] * sigmoid_of<T>(g[e]) * u[e];
-                put4(reinterpret_cast<T*>(h) + o, v);
-                if (saved) keep_gu<T>(saved, o, plane, g, u);
+                out.put(j, q, v);
+                if (kept.p && m < rows && n < ldh) keep_gu<T>(kept, kept.at(m, n), g, u);
             }
+            out.store(reinterpret_cast<T*>(h) + (int64_t)r0 * ldh + c0, ldh, rows - r0, ldh - c0);
         }
     }
 };
 
 struct EpiGateBwd {
     void *dg, *du;
-    const void* saved;
+    KeptGu kept;
     float alpha;
     int rows, ldh;
 
     template <typename T, typename Tile, int kMode>
     __device__ __forceinline__ void run(const GemmArgs&, const GemmPlace<Tile, kMode>& at,
-                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char*, int, int, int) const {
-        const int64_t plane = (int64_t)rows * ldh;
+                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, int, int, int) const {
+        constexpr int J = Tile::FN * Tile::Q;
+        const GemmRows<T, Tile, Tile::FN * Tile::MF> out(smem, at.wave(), at.lane);
+        // the kept values of a piece's row are fetched while the one before is worked on
+        KeptFour<T> k[2][J];
+        auto fetch = [&](int i) {
+            const int m = at.m(i) < rows ? at.m(i) : rows - 1;
+#pragma unroll
+            for (int jq = 0; jq < J; ++jq) {
+                const int n = at.n(jq / Tile::Q, jq % Tile::Q);
+                k[i & 1][jq].load(kept, kept.at(m, n < ldh ? n : 0));
+            }
+        };
+        fetch(0);
 #pragma unroll
         for (int i = 0; i < Tile::FM; ++i) {
-            const int m = at.m(i);
-            if (m >= rows) continue;
+            const int r0 = at.row0(i), c0 = at.col0();
+            if (i + 1 < Tile::FM) fetch(i + 1);
+            f32x4 b[J];
 #pragma unroll
-            for (int j = 0; j < Tile::FN * Tile::Q; ++j) {
-                const int n = at.n(j / Tile::Q, j % Tile::Q);
-                if (n >= ldh) continue;
-                const int64_t o = (int64_t)m * ldh + n;
-                const f32x4 v = four(acc[i][j / Tile::Q], j % Tile::Q);
-                f32x4 g, u, a, b;
-                kept_gu<T>(saved, o, plane, g, u);
+            for (int jq = 0; jq < J; ++jq) {
+                const f32x4 v = four(acc[i][jq / Tile::Q], jq % Tile::Q);
+                f32x4 a;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float s = sigmoid_of<T>(g[e]), dh = v[e] * alpha;
-                    a[e] = dh * u[e] * s * (1.f + g[e] * (1.f - s));
-                    b[e] = dh * g[e] * s;
+                    float g, u;
+                    k[i & 1][jq].get(e, g, u);
+                    const float s = sigmoid_of<T>(g), dh = v[e] * alpha;
+                    a[e] = dh * u * s * (1.f + g * (1.f - s));
+                    b[jq][e] = dh * g * s;
                 }
-                put4(reinterpret_cast<T*>(dg) + o, a);
-                put4(reinterpret_cast<T*>(du) + o, b);
+                out.put(jq / Tile::Q, jq % Tile::Q, a);
             }
+            const int64_t o = (int64_t)r0 * ldh + c0;
+            out.store(reinterpret_cast<T*>(dg) + o, ldh, rows - r0, ldh - c0);
+#pragma unroll
+            for (int jq = 0; jq < J; ++jq) out.put(jq / Tile::Q, jq % Tile::Q, b[jq]);
+            out.store(reinterpret_cast<T*>(du) + o, ldh, rows - r0, ldh - c0);
         }
     }
 };
@@ -216,8 +245,12 @@ MlpBwd mlp_bwd_layout(const MlpShape& s, void* ws) {
     return f;
 }
 
-// h behind the planes of g and u
-int64_t gu_bytes(const MlpShape& s) { return up256(s.rows * s.fp * (s.dtype == M3_DTYPE_BF16 ? 6 : 8)); }
+// h behind what is kept of g and u
+KeptGu kept_gu(const MlpShape& s, const void* saved) {
+    const int64_t blocks = (s.fp + 15) / 16, rows = (s.rows + 15) / 16 * 16;
+    return KeptGu{const_cast<void*>(saved), rows * blocks * 16, (int)blocks};
+}
+int64_t gu_bytes(const MlpShape& s) { return up256(kept_gu(s, nullptr).elements * (s.dtype == M3_DTYPE_BF16 ? 6 : 8)); }
 
 // src as it is, or its padded copy
 int padded(const MlpShape& s, const void* src, void* dst, int64_t rows, int64_t cols, int64_t ldd, const void** out,
@@ -257,7 +290,7 @@ int launch_swiglu_fwd(int64_t rows, int64_t d, int64_t ff, int dtype, const void
     void* h = saved ? reinterpret_cast<char*>(saved) + gu_bytes(s) : f.h;
     GemmArgs a = gemm_args({x, s.dp}, {wg, s.dp}, rows, ff, s.dp, 1);
     a.b[1] = {wu, s.dp};
-    M3_TRY((gemm_dispatch<true, true, kGated>(dtype, f.up, a, EpiGated{h, saved, (int)rows, (int)s.fp}, rows, 2 * s.fp, 1, stream)));
+    M3_TRY((gemm_dispatch<true, true, kGated>(dtype, f.up, a, EpiGated{h, kept_gu(s, saved), (int)rows, (int)s.fp}, rows, 2 * s.fp, 1, stream)));
     const GemmStore st{{y, nullptr}, d, res, scale, f.part, 0, (int)rows, (int)d};
     return gemm_store(kFormNT, dtype, f.down, gemm_args({h, s.fp}, {wd, s.fp}, rows, d, s.fp, 1), st, 1, stream);
 }
@@ -274,7 +307,7 @@ int launch_swiglu_bwd(int64_t rows, int64_t d, int64_t ff, int dtype, const void
         // rows of Wd past d do not exist: A's pad columns meet zeros
         GemmArgs a = gemm_args({dy, s.dp}, {wd, s.fp}, rows, s.fp, s.dp, 1);
         a.KB[0] = (int)d;
-        M3_TRY((gemm_dispatch<true, false, kPlain>(dtype, f.dh, a, EpiGateBwd{f.dg, f.du, saved, scale, (int)rows, (int)s.fp}, rows, s.fp, 1, stream)));
+        M3_TRY((gemm_dispatch<true, false, kPlain>(dtype, f.dh, a, EpiGateBwd{f.dg, f.du, kept_gu(s, saved), scale, (int)rows, (int)s.fp}, rows, s.fp, 1, stream)));
     }
     if (dx) {
         M3_TRY(padded(s, wg, f.wg, ff, d, s.dp, &wg, stream));

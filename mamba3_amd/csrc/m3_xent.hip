@@ -1,7 +1,9 @@
 // Softmax cross entropy of a vocabulary projection without its logits (gfx950): for rows h_m and a
 // weight W of V rows,
 //   z = h W^T, lse_m = log sum over v of exp z_mv, loss_m = lse_m - z_m,target,
-//   dz_mv = (exp(z_mv - lse_m) - [v = target]) gl_m, dh = dz W, dW = dz^T h.
+//   dz_mv = (exp(z_mv - lse_m) - [v = target]) gl_m, dh = dz W, dW = dz^T h,
+// where one gl for all rows (a mean or a sum) is left to the products' results: dz then holds
+// softmax - 1 in the target's place, not rounded multiples of 1 / rows.
 // Forward: the product's epilogue (m3_gemm.h) reduces each tile's columns to a maximum and a sum
 // of exponentials per row, so one pair per row and tile of the vocabulary leaves the kernel
 // instead of the logits; a second kernel joins a row's pairs, a third the rows. Backward, in
@@ -43,39 +45,8 @@ struct EpiXentFwd {
     __device__ __forceinline__ void run(const GemmArgs&, const GemmPlace<Tile, kMode>& at,
                                         typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, int tm, int tn, int) const {
         float2* red = reinterpret_cast<float2*>(smem);  // [WGN][BM]
-#pragma unroll
-        for (int i = 0; i < Tile::FM; ++i) {
-            const int m = at.m(i);
-            const int64_t t = m < rows ? target[m] : -1;
-            float top = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < Tile::FN * Tile::Q; ++j) {
-                const int n = at.n(j / Tile::Q, j % Tile::Q);
-                const f32x4 v = four(acc[i][j / Tile::Q], j % Tile::Q);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (n + e < vocab) {
-                        top = fmaxf(top, v[e]);
-                        if (t == n + e) zt[m] = v[e];
-                    }
-                }
-            }
-#pragma unroll
-            for (int off = Tile::MF; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off, kWave));
-            float sum = 0.f;
-            const float ref = top == -INFINITY ? 0.f : top;  // a row without finite logits
-#pragma unroll
-            for (int j = 0; j < Tile::FN * Tile::Q; ++j) {
-                const int n = at.n(j / Tile::Q, j % Tile::Q);
-                const f32x4 v = four(acc[i][j / Tile::Q], j % Tile::Q);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n + e < vocab) sum += exp_of<T>(v[e] - ref);
-            }
-#pragma unroll
-            for (int off = Tile::MF; off < 64; off *= 2) sum += __shfl_xor(sum, off, kWave);
-            if (at.lane < Tile::MF) red[at.wn * Tile::BM + at.local_m(i)] = make_float2(top, sum);
-        }
+        if (at.n0 + Tile::BN <= vocab) rows_of<T, Tile, kMode, true>(at, acc, red);
+        else rows_of<T, Tile, kMode, false>(at, acc, red);
         __syncthreads();
         for (int r = threadIdx.x; r < Tile::BM; r += Tile::NT) {
             const int m = tm * Tile::BM + r;
@@ -86,48 +57,115 @@ struct EpiXentFwd {
             part[(int64_t)tn * rows + m] = v;
         }
     }
+
+    // The lanes of a row hold 4 columns of each piece; kAll: every column of the tile exists.
+    template <typename T, typename Tile, int kMode, bool kAll>
+    __device__ __forceinline__ void rows_of(const GemmPlace<Tile, kMode>& at, typename Tile::Acc (&acc)[Tile::FM][Tile::FN],
+                                            float2* red) const {
+        constexpr int J = Tile::FN * Tile::Q;
+        const int first = at.n(0, 0);
+        // the target's place among this wave's columns, of all pieces' rows
+        int rel[Tile::FM];
+#pragma unroll
+        for (int i = 0; i < Tile::FM; ++i) {
+            const int m = at.m(i);
+            const int64_t t = m < rows ? target[m] : -1;
+            rel[i] = t >= 0 && t < vocab ? (int)t - first : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < Tile::FM; ++i) {
+            float z[J][4];
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const f32x4 v = four(acc[i][j / Tile::Q], j % Tile::Q);
+                const int n = at.n(j / Tile::Q, j % Tile::Q);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    z[j][e] = kAll || n + e < vocab ? v[e] : -INFINITY;
+                    top = fmaxf(top, z[j][e]);
+                }
+            }
+            // few waves hold the target of one of their rows
+            if (__any(rel[i] >= 0 && rel[i] < Tile::FN * Tile::MF)) {
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (rel[i] == at.n(j / Tile::Q, j % Tile::Q) - first + e) zt[at.m(i)] = z[j][e];
+            }
+#pragma unroll
+            for (int off = Tile::MF; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off, kWave));
+            const float ref = top == -INFINITY ? 0.f : top;  // a row without finite logits
+            float sum = 0.f;
+            if constexpr (sizeof(T) == 2) {
+                const float low = -ref * kLog2e;
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(z[j][e], kLog2e, low));
+            } else {
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum += expf(z[j][e] - ref);
+            }
+#pragma unroll
+            for (int off = Tile::MF; off < 64; off *= 2) sum += __shfl_xor(sum, off, kWave);
+            if (at.lane < Tile::MF) red[at.wn * Tile::BM + at.local_m(i)] = make_float2(top, sum);
+        }
+    }
 };
 
 struct EpiXentBwd {
     void* dz;  // rows x ld: the piece's columns, zero past the vocabulary
     int ld;
     const float* lse;
-    const float* count;      // [1]: rows that count
-    const float* gl;         // dL/dloss: [1], or [rows] for no reduction
+    const float* gl;         // dL/dloss [rows] without a reduction, else nullptr
     const int64_t* target;
     int64_t ignore;
-    int reduction;
-    int v0, vocab, rows;     // first column of the piece
+    int v0, have, vocab, rows;  // first column of the piece, its columns that exist
 
     template <typename T, typename Tile, int kMode>
     __device__ __forceinline__ void run(const GemmArgs&, const GemmPlace<Tile, kMode>& at,
-                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char*, int, int, int) const {
-        typedef T T4 __attribute__((ext_vector_type(4)));
-        const float all = reduction == M3_REDUCTION_NONE ? 0.f : gl[0];
-        const float each = reduction == M3_REDUCTION_MEAN ? all / count[0] : all;
+                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, int, int, int) const {
+        constexpr int J = Tile::FN * Tile::Q;
+        const GemmRows<T, Tile, Tile::FN * Tile::MF> out(smem, at.wave(), at.lane);
+        const int first = at.n(0, 0);
+        const bool all = at.n0 + Tile::BN <= have;  // every column of the tile exists
+        float low[Tile::FM], g[Tile::FM];
+        int rel[Tile::FM];  // the target's place among this wave's columns
 #pragma unroll
         for (int i = 0; i < Tile::FM; ++i) {
-            const int m = at.m(i);
-            if (m >= rows) continue;
+            const int m = at.m(i) < rows ? at.m(i) : rows - 1;
             const int64_t t = target[m];
             const bool live = t != ignore;
-            float g = reduction == M3_REDUCTION_NONE ? gl[m] : each;
-            if (t < 0 || t >= vocab) g = NAN;
-            const float l = lse[m];
+            low[i] = live ? lse[m] : INFINITY;  // exp(z - inf) = 0: hidden reads as zero where it is ignored
+            g[i] = gl && live ? gl[m] : 1.f;
+            if (live && (t < 0 || t >= vocab)) g[i] = NAN;
+            rel[i] = live && t >= v0 && t < v0 + have ? (int)(t - v0) - first : -1;
+        }
 #pragma unroll
-            for (int j = 0; j < Tile::FN * Tile::Q; ++j) {
+        for (int i = 0; i < Tile::FM; ++i) {
+            const bool hit = __any(rel[i] >= 0 && rel[i] < Tile::FN * Tile::MF);
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
                 const int n = at.n(j / Tile::Q, j % Tile::Q);
-                if (n >= ld) continue;
-                const f32x4 v = four(acc[i][j / Tile::Q], j % Tile::Q);
-                T4 o;
+                const f32x4 z = four(acc[i][j / Tile::Q], j % Tile::Q);
+                f32x4 p;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float p = exp_of<T>(v[e] - l);
-                    if (t == v0 + n + e) p -= 1.f;
-                    o[e] = (T)(live && v0 + n + e < vocab ? p * g : 0.f);
-                }
-                *reinterpret_cast<T4*>(reinterpret_cast<T*>(dz) + (int64_t)m * ld + n) = o;
+                for (int e = 0; e < 4; ++e) p[e] = exp_of<T>(z[e] - low[i]);
+                if (hit)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[e] -= rel[i] == n - first + e ? 1.f : 0.f;
+                p *= g[i];
+                if (!all)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[e] = n + e < have ? p[e] : 0.f;
+                out.put(j / Tile::Q, j % Tile::Q, p);
             }
+            const int r0 = at.row0(i), c0 = at.col0();
+            out.store(reinterpret_cast<T*>(dz) + (int64_t)r0 * ld + c0, ld, rows - r0, ld - c0);
         }
     }
 };
@@ -319,14 +357,17 @@ int launch_xent_bwd(int64_t rows, int64_t d, int64_t vocab, int dtype, int reduc
         weight = f.w;
     }
     const int r = (int)rows;
+    const bool none = reduction == M3_REDUCTION_NONE;
     GemmStore dh{{nullptr, nullptr}, d, nullptr, 1.f, f.part, 0, r, (int)d};
+    if (!none) dh.num = grad_loss;
+    if (reduction == M3_REDUCTION_MEAN) dh.den = count;
     for (int64_t v0 = 0; v0 < vocab; v0 += f.piece) {
         const int64_t have = std::min(f.piece, vocab - v0);
         const char* w = reinterpret_cast<const char*>(weight) + v0 * dp * size;
         // dz of the piece; columns past the vocabulary, up to the row stride, are written as zeros
         M3_TRY((gemm_dispatch<true, true, kPlain>(
             dtype, f.z, gemm_args({f.h, dp}, {w, dp}, rows, have, dp, 1),
-            EpiXentBwd{f.dz, (int)f.piece, lse, count, grad_loss, target, ignore, reduction, (int)v0, (int)vocab, r},
+            EpiXentBwd{f.dz, (int)f.piece, lse, none ? grad_loss : nullptr, target, ignore, (int)v0, (int)have, (int)vocab, r},
             rows, f.piece, 1, stream)));
         if (dhidden) {
             GemmArgs a = gemm_args({f.dz, f.piece}, {w, dp}, rows, dp, f.piece, 1);
@@ -336,7 +377,8 @@ int launch_xent_bwd(int64_t rows, int64_t d, int64_t vocab, int dtype, int reduc
         }
         if (dweight) {
             void* out = reinterpret_cast<char*>(dweight) + v0 * d * size;
-            const GemmStore dw{{out, nullptr}, d, nullptr, 1.f, f.part_dw, 0, (int)have, (int)d};
+            GemmStore dw{{out, nullptr}, d, nullptr, 1.f, f.part_dw, 0, (int)have, (int)d};
+            dw.num = dh.num, dw.den = dh.den;
             M3_TRY(gemm_store(kFormTN, dtype, f.dw, gemm_args({f.dz, f.piece}, {f.h, dp}, f.piece, dp, rows, 1), dw, 1, stream));
         }
     }
