@@ -70,7 +70,7 @@ struct GemmOp {
     int64_t ld;
 };
 
-// Two terms (kSeg2: C = A0 B0 + A1 B1), two problems (kBatch2: blockIdx.y) or two B halves
+// Two terms (kSeg2: C = A0 B0 + A1 B1), two products (kBatch2) or two B halves
 // of a tile (kGated: columns [0, BN/2) from B0 and [BN/2, BN) from B1).
 enum GemmMode { kPlain, kSeg2, kBatch2, kGated };
 
@@ -79,7 +79,8 @@ struct GemmArgs {
     int M, N;    // rows of A and of B (kGated: of one half): what the tiles may read
     int K[2];    // inner lengths of the terms; multiples of 16 bytes for k-contiguous operands
     int KB[2];   // rows of B that exist where B is not k-contiguous (<= K: the rest reads as zero)
-    int splits;  // k is cut into so many parts (blockIdx.z)
+    int splits;  // k is cut into so many parts
+    int batch;   // products (1 or 2)
     int tiles_m, tiles_n;
 };
 
@@ -185,7 +186,10 @@ struct GemmTile {
     static constexpr int FM = BM / WGM / MF, FN = BN / WGN / MF;  // MF x MF pieces of a wave
     static constexpr int Q = MF * MF / 256;                       // fours of columns a lane holds of a piece
     static constexpr int kStageBytes = (BM + BN) * 128;
-    static constexpr int kLds = STAGES * kStageBytes;
+    // behind the stages: the epilogue's rows, in fp32 where the tile serves fp32 products
+    static constexpr int kStages = STAGES * kStageBytes;
+    static constexpr int kEpi = NW * MF * (FN * MF * (MF == 32 || BN == 64 ? 4 : 2) + 16);
+    static constexpr int kLds = kStages + kEpi;
     typedef typename GemmType<bf16, MF>::Acc Acc;
 };
 
@@ -223,7 +227,7 @@ struct GemmRows {
     static constexpr int MF = Tile::MF, E = 16 / sizeof(T);
     static constexpr int kPitch = kCols * (int)sizeof(T) + 16;
     static constexpr int LPR = kCols / E, RPI = 64 / LPR;  // lanes a row, rows an instruction
-    static_assert(Tile::NW * MF * kPitch <= Tile::kLds, "rows fit LDS");
+    static_assert(Tile::NW * MF * kPitch <= Tile::kEpi, "rows fit LDS");
     typedef T T4 __attribute__((ext_vector_type(4)));
     typedef T Piece __attribute__((ext_vector_type(E)));
     char* mine;
@@ -250,23 +254,31 @@ struct GemmRows {
     }
 };
 
-// Block -> tile: the blocks of one XCD (dispatch is round robin over 8) take a contiguous run of
-// tiles, and runs walk groups of 8 row tiles column by column, so that an XCD's L2 serves
-// both operands.
-__device__ __forceinline__ void gemm_tile_of(int tiles_m, int tiles_n, int& tm, int& tn) {
-    const int total = tiles_m * tiles_n, b = (int)blockIdx.x;
+// A block's piece of work: one tile of one product, one part of its k.
+struct GemmItem {
+    int tm, tn, batch, split;
+};
+// Work id -> item. Ids go to the XCDs round robin (blocks are dispatched so, and a block's later ids are
+// a multiple of 8 further on): those of one XCD take a contiguous run of tiles, and runs walk
+// groups of 8 row tiles column by column, so that an XCD's L2 serves both operands.
+// (Quotients come from the vector unit: readfirstlane brings these back to scalar registers, which the
+// copies' operands have to be in.)
+__device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ GemmItem gemm_item(const GemmArgs& a, int id) {
+    const int total = a.tiles_m * a.tiles_n;
+    const int outer = scalar(id / total), b = id - outer * total;
     const int x = b & 7, per = total >> 3, rest = total & 7;
-    const int id = x * per + (x < rest ? x : rest) + (b >> 3);
+    const int at = x * per + (x < rest ? x : rest) + (b >> 3);
     constexpr int G = 8;
-    const int group = id / (G * tiles_n), first = group * G;
-    const int rows = tiles_m - first < G ? tiles_m - first : G;
-    const int in = id - group * (G * tiles_n);
-    tm = first + in % rows;
-    tn = in / rows;
+    const int group = scalar(at / (G * a.tiles_n)), first = group * G;
+    const int rows = a.tiles_m - first < G ? a.tiles_m - first : G;
+    const int in = at - group * (G * a.tiles_n);
+    const int tn = scalar(in / rows), split = a.batch == 1 ? outer : outer >> 1;
+    return GemmItem{first + in - tn * rows, tn, outer - split * a.batch, split};
 }
 
 template <typename T, typename Tile, bool kAKc, bool kBKc, int kMode, typename Epi>
-__global__ __launch_bounds__(Tile::NT, Tile::NT >= 512 ? 2 : 1) void gemm_kernel(GemmArgs a, Epi epi) {
+__global__ __launch_bounds__(Tile::NT, 2) void gemm_kernel(GemmArgs a, Epi epi) {
     constexpr int BM = Tile::BM, BN = Tile::BN, FM = Tile::FM, FN = Tile::FN, ST = Tile::STAGES, MF = Tile::MF;
     constexpr int BK = 128 / sizeof(T), SZ = sizeof(T);
     typedef GemmLoader<T, kAKc, BM, Tile::NW, MF> LA;
@@ -276,33 +288,38 @@ __global__ __launch_bounds__(Tile::NT, Tile::NT >= 512 ? 2 : 1) void gemm_kernel
     extern __shared__ __align__(16) char gemm_smem[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int tm, tn;
-    gemm_tile_of(a.tiles_m, a.tiles_n, tm, tn);
-    const int m0 = tm * BM, n0 = tn * (kMode == kGated ? BN / 2 : BN);
-    const int z = kMode == kBatch2 ? (int)blockIdx.y : 0;
+    const int items = a.tiles_m * a.tiles_n * a.batch * a.splits;
 
-    // the k steps of this block: steps [s0, s1) of the terms' steps in a row
+    // the k steps of an item: a part of the terms' steps in a row
     const int st0 = (a.K[0] + BK - 1) / BK;
     const int steps = st0 + (kMode == kSeg2 ? (a.K[1] + BK - 1) / BK : 0);
-    const int s0 = (int)((int64_t)steps * blockIdx.z / a.splits), s1 = (int)((int64_t)steps * (blockIdx.z + 1) / a.splits);
+    auto first_step = [&](int split) { return scalar((int)((unsigned)steps * (unsigned)split / (unsigned)a.splits)); };  // steps < 2^26, splits <= 16
 
     const bool second = kMode == kGated && wave * LB::NI >= LB::kInstr / 2;
     static_assert(kMode != kGated || (LB::kInstr / 2) % LB::NI == 0, "a wave fetches from one half");
-    // rows that exist in this tile: spans end with the last one's last valid element (< 2^31 bytes)
-    const int ra_rows = a.M - m0 < BM ? a.M - m0 : BM, rb_rows = a.N - n0 < BN ? a.N - n0 : BN;
     LA la;
     LB lb;
-    // Where the step to be fetched next lies, and the bytes behind it. From step to step the
-    // pointers advance by pa_step and pb_step; at step `turn` (the end, a term's last, partial step or
-    // the second term's first) everything is set up anew.
+    // What is fetched next: step fs of item f_id, which ends before step f_end. From step to step
+    // the pointers advance by pa_step and pb_step; at step `turn` (the end, a term's last, partial step
+    // or the second term's first) everything is set up anew. Behind the last item nothing is read.
     const char *pa, *pb;
     int64_t pa_step, pb_step;
-    int ba, bb, turn;
-    auto set_up = [&](int s) {
-        const int seg = kMode == kSeg2 && s >= st0 ? 1 : 0;
-        const int k0 = (seg ? s - st0 : s) * BK;
-        const int left = a.K[seg] - k0, krem = s >= s1 ? 0 : left < BK ? left : BK;
-        const int ia = kMode == kSeg2 ? seg : z, ib = kMode == kGated ? (second ? 1 : 0) : ia;
+    int ba, bb, turn, fs, f_id, f_end;
+    auto set_up = [&]() {
+        if (f_id >= items) {
+            ba = bb = 0;
+            pa_step = pb_step = 0;
+            turn = 0x7fffffff;
+            return;
+        }
+        const GemmItem it = gemm_item(a, f_id);
+        const int m0 = it.tm * BM, n0 = it.tn * (kMode == kGated ? BN / 2 : BN);
+        // rows that exist in this tile: spans end with the last one's last valid element (< 2^31 bytes)
+        const int ra_rows = a.M - m0 < BM ? a.M - m0 : BM, rb_rows = a.N - n0 < BN ? a.N - n0 : BN;
+        const int seg = kMode == kSeg2 && fs >= st0 ? 1 : 0;
+        const int k0 = (seg ? fs - st0 : fs) * BK;
+        const int left = a.K[seg] - k0, krem = left < BK ? left : BK;
+        const int ia = kMode == kSeg2 ? seg : kMode == kBatch2 ? it.batch : 0, ib = kMode == kGated ? (second ? 1 : 0) : ia;
         const int bleft = a.KB[seg] - k0;
         const int brem = kBKc || krem < bleft ? krem : bleft;  // may be negative
         const int lda = (int)a.a[ia].ld, ldb = (int)a.b[ib].ld;
@@ -310,7 +327,7 @@ __global__ __launch_bounds__(Tile::NT, Tile::NT >= 512 ? 2 : 1) void gemm_kernel
         pb = reinterpret_cast<const char*>(a.b[ib].p) + (kBKc ? (int64_t)n0 * ldb + k0 : (int64_t)k0 * ldb + n0) * SZ;
         pa_step = kAKc ? 128 : (int64_t)BK * lda * SZ;
         pb_step = kBKc ? 128 : (int64_t)BK * ldb * SZ;
-        ba = krem <= 0 || ra_rows <= 0 ? 0 : (kAKc ? (ra_rows - 1) * lda + krem : (krem - 1) * lda + ra_rows) * SZ;
+        ba = ra_rows <= 0 ? 0 : (kAKc ? (ra_rows - 1) * lda + krem : (krem - 1) * lda + ra_rows) * SZ;
         bb = brem <= 0 || rb_rows <= 0 ? 0 : (kBKc ? (rb_rows - 1) * ldb + brem : (brem - 1) * ldb + rb_rows) * SZ;
         const int pieces = krem < BK ? (krem * SZ) >> 4 : 8;
         la.init(wave, lane, lda, 0, pieces);
@@ -318,12 +335,21 @@ __global__ __launch_bounds__(Tile::NT, Tile::NT >= 512 ? 2 : 1) void gemm_kernel
         // whole steps of this term for both operands, then the next turn
         const int whole = (kBKc || a.K[seg] < a.KB[seg] ? a.K[seg] : a.KB[seg]) / BK + (seg ? st0 : 0);
         const int end = seg || kMode != kSeg2 ? steps : st0;
-        turn = s >= s1 ? 0x7fffffff : s < whole ? whole : s + 1 < end ? s + 1 : end;
-        if (turn > s1 && s < s1) turn = s1;
+        turn = fs < whole ? whole : fs + 1 < end ? fs + 1 : end;
+        turn = turn < f_end ? turn : f_end;
     };
-    auto advance = [&](int s) {  // to step s, one past the last set up
-        if (s == turn) {
-            set_up(s);
+    auto enter = [&](int id) {  // the first step of an item
+        f_id = id;
+        const int split = id < items ? gemm_item(a, id).split : 0;
+        fs = first_step(split);
+        f_end = first_step(split + 1);
+        set_up();
+    };
+    auto advance = [&]() {
+        ++fs;
+        if (fs == turn) {
+            if (fs == f_end) enter(f_id + (int)gridDim.x);
+            else set_up();
         } else {
             pa += pa_step;
             pb += pb_step;
@@ -347,19 +373,12 @@ __global__ __launch_bounds__(Tile::NT, Tile::NT >= 512 ? 2 : 1) void gemm_kernel
         else
             return wn * FN + fn;
     };
-
     typename Type::Acc acc[FM][FN];
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-            for (int e = 0; e < MF * MF / 64; ++e) acc[i][j][e] = 0.f;
 
     // A step is two halves of KH k steps. While one half's fragments are multiplied, the next half's
-    // are read from LDS; all of step s has been read halfway through it, which frees its slot
-    // for step s + ST. Copies and reads are issued between groups of FN MFMAs, which cover them, two
-    // a group: early in the half, so that they have landed when they are waited for.
+    // are read from LDS; all of a step has been read halfway through it, which frees its slot
+    // for the step ST further on. Copies and reads are issued between groups of FN MFMAs, which cover
+    // them, two a group: early in the half, so that they have landed when they are waited for.
     typedef typename Type::Frag Frag;
     constexpr int KH = MF == 16 ? 1 : 2;
     constexpr int kGroups = KH * FM, kReads = KH * (FM + FN);
@@ -378,54 +397,62 @@ __global__ __launch_bounds__(Tile::NT, Tile::NT >= 512 ? 2 : 1) void gemm_kernel
     constexpr int kPer = (kReads + kGroups - 1) / kGroups < 2 ? 2 : (kReads + kGroups - 1) / kGroups;
     constexpr int kPerLd = (NLD + kGroups - 1) / kGroups < 2 ? 2 : (NLD + kGroups - 1) / kGroups;
 
-    set_up(s0);
+    enter((int)blockIdx.x);
 #pragma unroll
     for (int s = 0; s < ST; ++s) {
-        if (s) advance(s0 + s);
+        if (s) advance();
 #pragma unroll
         for (int i = 0; i < NLD; ++i) fetch(i, s);
     }
-    wait_vm_lds<NLD * (ST - 1)>();
-    M3_LDS_FENCE();
-    __builtin_amdgcn_s_barrier();
-    M3_LDS_FENCE();
-#pragma unroll
-    for (int i = 0; i < kReads; ++i) read(0, 0, i);
     int slot = 0;
-    for (int s = s0; s < s1; ++s) {
-        M3_FENCE();
+    // The steps of all items form one row: an item's last steps already fetch the next one's first,
+    // which land during the epilogue.
+    for (int id = (int)blockIdx.x; id < items; id += (int)gridDim.x) {
+        const GemmItem it = gemm_item(a, id);
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
+        for (int i = 0; i < FM; ++i)
 #pragma unroll
-            for (int i = g * kPer; i < (g + 1) * kPer && i < kReads; ++i) read(1, slot, i);
-            M3_FENCE();
-            group(0, g);
-            M3_FENCE();
-        }
-        advance(s + ST);
-        const int next = slot + 1 == ST ? 0 : slot + 1;
-        wait_vm_lds<NLD * (ST - 2)>();  // step s + 1 has landed, this wave has read step s
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int e = 0; e < MF * MF / 64; ++e) acc[i][j][e] = 0.f;
+        wait_vm_lds<0>();  // also the last epilogue's stores, which count with the copies
         M3_LDS_FENCE();
         __builtin_amdgcn_s_barrier();
         M3_LDS_FENCE();
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-#pragma unroll
-            for (int i = g * kPerLd; i < (g + 1) * kPerLd && i < NLD; ++i) fetch(i, slot);
-#pragma unroll
-            for (int i = g * kPer; i < (g + 1) * kPer && i < kReads; ++i) read(0, next, i);
+        for (int i = 0; i < kReads; ++i) read(0, slot, i);
+        for (int n = first_step(it.split + 1) - first_step(it.split); n > 0; --n) {
             M3_FENCE();
-            group(1, g);
-            M3_FENCE();
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+                for (int i = g * kPer; i < (g + 1) * kPer && i < kReads; ++i) read(1, slot, i);
+                M3_FENCE();
+                group(0, g);
+                M3_FENCE();
+            }
+            advance();
+            const int next = slot + 1 == ST ? 0 : slot + 1;
+            wait_vm_lds<NLD * (ST - 2)>();  // the next step has landed, this wave has read this one
+            M3_LDS_FENCE();
+            __builtin_amdgcn_s_barrier();
+            M3_LDS_FENCE();
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+                for (int i = g * kPerLd; i < (g + 1) * kPerLd && i < NLD; ++i) fetch(i, slot);
+#pragma unroll
+                for (int i = g * kPer; i < (g + 1) * kPer && i < kReads; ++i) read(0, next, i);
+                M3_FENCE();
+                group(1, g);
+                M3_FENCE();
+            }
+            slot = next;
         }
-        slot = next;
+        const GemmPlace<Tile, kMode> at{it.tm * BM, it.tn * (kMode == kGated ? BN / 2 : BN), wm, wn, lane};
+        epi.template run<T, Tile, kMode>(a, at, acc, gemm_smem + Tile::kStages, it);
     }
-    wait_vm_lds<0>();  // nothing writes LDS once the epilogue uses it
-    M3_LDS_FENCE();
-    __builtin_amdgcn_s_barrier();
-    M3_LDS_FENCE();
-    const GemmPlace<Tile, kMode> at{m0, n0, wm, wn, lane};
-    epi.template run<T, Tile, kMode>(a, at, acc, gemm_smem, tm, tn, z);
+    wait_vm_lds<0>();  // no copy outlives its block
 }
 
 }  // namespace m3

@@ -39,13 +39,15 @@ template <typename T, typename Tile, bool kAKc, bool kBKc, int kMode, typename E
 int gemm_launch(GemmArgs a, const Epi& epi, int64_t rows, int64_t cols, int batch, hipStream_t stream) {
     a.tiles_m = (int)((rows + Tile::BM - 1) / Tile::BM);
     a.tiles_n = (int)((cols + Tile::BN - 1) / Tile::BN);
-    const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
-    if (tiles * Tile::NT >= ((int64_t)1 << 32)) return M3_ERR_UNSUPPORTED;
+    a.batch = batch;
+    const int64_t items = (int64_t)a.tiles_m * a.tiles_n * batch * a.splits;
+    if (items > 0x3fffffff) return M3_ERR_UNSUPPORTED;
     auto* k = gemm_kernel<T, Tile, kAKc, kBKc, kMode, Epi>;
-    if (Tile::kLds > 64 * 1024 &&
-        hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, Tile::kLds) != hipSuccess)
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, Tile::kLds) != hipSuccess)
         return M3_ERR_LAUNCH;
-    hipLaunchKernelGGL(k, dim3((unsigned)tiles, (unsigned)batch, (unsigned)a.splits), dim3(Tile::NT), Tile::kLds, stream, a, epi);
+    // as many blocks as run at once; each takes every grid-th item
+    constexpr int64_t kAtOnce = 256 * (Tile::NT >= 512 ? 1 : 2);
+    hipLaunchKernelGGL(k, dim3((unsigned)std::min(items, kAtOnce)), dim3(Tile::NT), Tile::kLds, stream, a, epi);
     return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH;
 }
 
@@ -98,6 +100,7 @@ inline GemmArgs gemm_args(GemmOp a, GemmOp b, int64_t m, int64_t n, int64_t k, i
     g.K[0] = g.KB[0] = (int)k;
     g.K[1] = g.KB[1] = 0;
     g.splits = splits;
+    g.batch = 1;
     g.tiles_m = g.tiles_n = 0;
     return g;
 }

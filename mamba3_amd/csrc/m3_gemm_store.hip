@@ -31,12 +31,13 @@ struct EpiStore {
 
     template <typename T, typename Tile, int kMode>
     __device__ __forceinline__ void run(const GemmArgs& a, const GemmPlace<Tile, kMode>& at,
-                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, int, int, int z) const {
+                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, const GemmItem& it) const {
+        const int z = it.batch;
         T* out = reinterpret_cast<T*>(s.out[z]);
         const T* res = reinterpret_cast<const T*>(s.res);
         const float alpha = s.part ? 1.f : store_scale(s);
         if (s.part) {
-            float* part = s.part + ((int64_t)blockIdx.z * gridDim.y + z) * s.rows * s.cols;
+            float* part = s.part + ((int64_t)it.split * a.batch + z) * s.rows * s.cols;
             each(at, acc, [&](int m, int n, f32x4 v) {
                 float* p = part + (int64_t)m * s.cols + n;
                 if (vec) {

@@ -99,7 +99,7 @@ struct EpiGated {
 
     template <typename T, typename Tile, int kMode>
     __device__ __forceinline__ void run(const GemmArgs&, const GemmPlace<Tile, kMode>& at,
-                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, int, int, int) const {
+                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, const GemmItem&) const {
         const GemmRows<T, Tile, Tile::FN / 2 * Tile::MF> out(smem, at.wave(), at.lane);
 #pragma unroll
         for (int i = 0; i < Tile::FM; ++i) {
@@ -128,7 +128,7 @@ struct EpiGateBwd {
 
     template <typename T, typename Tile, int kMode>
     __device__ __forceinline__ void run(const GemmArgs&, const GemmPlace<Tile, kMode>& at,
-                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, int, int, int) const {
+                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, const GemmItem&) const {
         constexpr int J = Tile::FN * Tile::Q;
         const GemmRows<T, Tile, Tile::FN * Tile::MF> out(smem, at.wave(), at.lane);
         // the kept values of a piece's row are fetched while the one before is worked on

@@ -43,18 +43,18 @@ struct EpiXentFwd {
 
     template <typename T, typename Tile, int kMode>
     __device__ __forceinline__ void run(const GemmArgs&, const GemmPlace<Tile, kMode>& at,
-                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, int tm, int tn, int) const {
+                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, const GemmItem& it) const {
         float2* red = reinterpret_cast<float2*>(smem);  // [WGN][BM]
         if (at.n0 + Tile::BN <= vocab) rows_of<T, Tile, kMode, true>(at, acc, red);
         else rows_of<T, Tile, kMode, false>(at, acc, red);
         __syncthreads();
         for (int r = threadIdx.x; r < Tile::BM; r += Tile::NT) {
-            const int m = tm * Tile::BM + r;
+            const int m = it.tm * Tile::BM + r;
             if (m >= rows) break;
             float2 v = red[r];
 #pragma unroll
             for (int w = 1; w < Tile::WGN; ++w) join(v.x, v.y, red[w * Tile::BM + r].x, red[w * Tile::BM + r].y);
-            part[(int64_t)tn * rows + m] = v;
+            part[(int64_t)it.tn * rows + m] = v;
         }
     }
 
@@ -128,7 +128,7 @@ struct EpiXentBwd {
 
     template <typename T, typename Tile, int kMode>
     __device__ __forceinline__ void run(const GemmArgs&, const GemmPlace<Tile, kMode>& at,
-                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, int, int, int) const {
+                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, const GemmItem&) const {
         constexpr int J = Tile::FN * Tile::Q;
         const GemmRows<T, Tile, Tile::FN * Tile::MF> out(smem, at.wave(), at.lane);
         const int first = at.n(0, 0);
