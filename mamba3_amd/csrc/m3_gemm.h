@@ -116,7 +116,8 @@ struct GemmLoader {
     }
     // Instruction i of this wave; bytes is what lies behind base. In assembly because the compiler takes
     // every later ds_read_b64_tr_b16 for a reader of what the builtin copies and waits for all copies
-    // before it; the kernel waits itself (wait_vm_lds). No register is written, so none is
+    // before it; the kernel waits itself (wait_vm_lds). m0 holds no value of the compiler between
+    // instructions (a reserved register). No vector register is written, so none is
     // live while the copy runs.
     __device__ __forceinline__ void issue(int i, const char* base, int bytes, unsigned lds, int wave) const {
         const u32x4 rs{(unsigned)reinterpret_cast<uintptr_t>(base), (unsigned)(reinterpret_cast<uintptr_t>(base) >> 32),
@@ -125,7 +126,7 @@ struct GemmLoader {
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                      :
                      : "s"(at), "v"(voff[i]), "s"(rs)
-                     : "memory", "m0");
+                     : "memory");
     }
 };
 
