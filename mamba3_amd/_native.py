@@ -526,15 +526,13 @@ def linear_xent_bwd(hidden, weight, target, ignore_index, reduction, lse, count,
 NORM_L2, NORM_MAX = 0, 1
 
 
-def clip_grad_norm(tensors, kind: int, max_norm: float | None, norm) -> None:
-    """m3_clip_grad_norm on contiguous tensors; max_norm None: the norm alone. Allocates the
-    workspace."""
-    n = len(tensors)
-    ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors])
-    numel = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
-    dtype = (ctypes.c_int32 * n)(*[dtype_code(t.dtype) for t in tensors])
-    nbytes = _bytes_of("m3_clip_grad_norm_workspace_size", n, numel, dtype)
+def clip_grad_norm(ptrs, numel, dtypes, kind: int, max_norm: float | None, norm) -> None:
+    """m3_clip_grad_norm on contiguous tensors, given as lists of addresses, sizes and dtype codes;
+    max_norm None: the norm alone. Allocates the workspace."""
+    n = len(ptrs)
+    ptrs, numel, dtypes = (_vp * n)(*ptrs), (_i64 * n)(*numel), (_i32 * n)(*dtypes)
+    nbytes = _bytes_of("m3_clip_grad_norm_workspace_size", n, numel, dtypes)
     ws = _workspace(nbytes, norm.device)
-    check(lib().m3_clip_grad_norm(n, ptrs, numel, dtype, kind, int(max_norm is not None),
+    check(lib().m3_clip_grad_norm(n, ptrs, numel, dtypes, kind, int(max_norm is not None),
                                   0.0 if max_norm is None else max_norm, ptr(norm), ptr(ws), nbytes,
                                   stream_of(norm)), "m3_clip_grad_norm")

@@ -7,7 +7,7 @@ from typing import Iterable
 
 import torch
 
-from . import _native
+from . import _native, ops
 
 
 def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float,
@@ -18,13 +18,9 @@ def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm:
     mixture, on one GPU; parameters without one are left out, and one that is listed twice counts
     once. Nothing waits for the GPU, unless error_if_nonfinite asks to raise, before anything is
     scaled, where the norm is NaN or infinite; otherwise such a norm scales by NaN or 0."""
-    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    grads, seen = [], set()
-    for p in params:
-        g = p.grad
-        if g is not None and id(g) not in seen:
-            seen.add(id(g))
-            grads.append(g)
+    params = (parameters,) if isinstance(parameters, torch.Tensor) else parameters
+    # the same gradient listed twice counts once
+    grads = list({id(g): g for g in [p.grad for p in params] if g is not None}.values())
     max_norm, norm_type = float(max_norm), float(norm_type)
     if norm_type == 2.0:
         kind = _native.NORM_L2
@@ -38,30 +34,37 @@ def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm:
         return torch.tensor(0.0)
     device = grads[0].device
     for g in grads:
-        if g.layout != torch.strided:
+        if g.layout is not torch.strided:
             raise TypeError(f"clip_grad_norm_ takes dense gradients, got {g.layout}")
-        _native.dtype_code(g.dtype)
         if g.device != device:
             raise ValueError(f"gradients must be on one GPU, got {device} and {g.device}")
+    codes = [_native.dtype_code(g.dtype) for g in grads]
     _native.require_gpu(grads[0])
-    whole = []  # what the kernels work on: the gradients themselves or contiguous copies
-    for g in grads:
-        if not g.is_contiguous() and any(n > 1 and s == 0 for n, s in zip(g.shape, g.stride())):
-            raise ValueError("a gradient whose elements share memory (expanded) cannot be clipped in place")
-        whole.append(g.detach().contiguous())
-    spans = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in whole)
-    for (a, n), (b, m) in zip(spans, spans[1:]):
-        if n and m and a + n > b:
-            raise ValueError("gradients that overlap in memory cannot be clipped in place")
-    with torch.cuda.device(device), torch.no_grad():
+    whole = grads  # what the kernels work on: the gradients themselves or contiguous copies
+    strided = [g for g in grads if not g.is_contiguous()]
+    if strided:
+        for g in strided:
+            if any(n > 1 and s == 0 for n, s in zip(g.shape, g.stride())):
+                raise ValueError("a gradient whose elements share memory (expanded) cannot be clipped in place")
+        whole = [g.detach().contiguous() for g in grads]
+    ptrs, sizes = [t.data_ptr() for t in whole], [t.numel() for t in whole]
+    end = 0
+    for at, n, code in sorted(zip(ptrs, sizes, codes)):
+        if n:
+            if at < end:
+                raise ValueError("gradients that overlap in memory cannot be clipped in place")
+            end = at + n * (2 if code == _native.M3_DTYPE_BF16 else 4)
+    with ops.on_device(grads[0]):
         norm = torch.empty((), dtype=torch.float32, device=device)
         if error_if_nonfinite:
-            _native.clip_grad_norm(whole, kind, None, norm)
+            _native.clip_grad_norm(ptrs, sizes, codes, kind, None, norm)
             if not math.isfinite(norm.item()):
                 raise RuntimeError(f"the norm of the gradients is {norm.item()}: they were not clipped")
-        _native.clip_grad_norm(whole, kind, max_norm, norm)
+        _native.clip_grad_norm(ptrs, sizes, codes, kind, max_norm, norm)
         torch.autograd.graph.increment_version(grads)
-        for g, t in zip(grads, whole):
-            if t.data_ptr() != g.data_ptr():
-                g.copy_(t)
+        if strided:
+            with torch.no_grad():
+                for g, t in zip(grads, whole):
+                    if t.data_ptr() != g.data_ptr():
+                        g.copy_(t)
     return norm

@@ -2,6 +2,7 @@
 #pragma once
 
 #include <algorithm>
+#include <atomic>
 
 #include "m3_gemm.h"
 
@@ -43,8 +44,16 @@ int gemm_launch(GemmArgs a, const Epi& epi, int64_t rows, int64_t cols, int batc
     const int64_t items = (int64_t)a.tiles_m * a.tiles_n * batch * a.splits;
     if (items > 0x3fffffff) return M3_ERR_UNSUPPORTED;
     auto* k = gemm_kernel<T, Tile, kAKc, kBKc, kMode, Epi>;
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, Tile::kLds) != hipSuccess)
-        return M3_ERR_LAUNCH;
+    // once for each device (a bit of `done`; devices past 63 set it every time)
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return M3_ERR_DEVICE;
+    const uint64_t bit = dev < 63 ? (uint64_t)1 << dev : 0;
+    if (!(done.load(std::memory_order_relaxed) & bit)) {
+        if (hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, Tile::kLds) != hipSuccess)
+            return M3_ERR_LAUNCH;
+        done.fetch_or(bit, std::memory_order_relaxed);
+    }
     // as many blocks as run at once; each takes every grid-th item
     constexpr int64_t kAtOnce = 256 * (Tile::NT >= 512 ? 1 : 2);
     hipLaunchKernelGGL(k, dim3((unsigned)std::min(items, kAtOnce)), dim3(Tile::NT), Tile::kLds, stream, a, epi);
@@ -87,10 +96,28 @@ int gemm_reduce(int dtype, const GemmStore& st, int splits, int batch, hipStream
 inline size_t gemm_part_bytes(const GemmPlan& p, int batch, int64_t rows, int64_t cols) {
     return p.splits > 1 ? (size_t)up256((int64_t)p.splits * batch * rows * cols * 4) : 0;
 }
-// dst [rows][ldd] = src [rows][cols] with zeros in the columns past cols; rows whose target is
-// `ignore` are zero where a target is given. ldd * size is a multiple of 16.
-int gemm_pad_copy(int dtype, const void* src, void* dst, int64_t rows, int64_t cols, int64_t ldd,
-                  const int64_t* target, int64_t ignore, hipStream_t stream);
+// dst [rows][ldd] = src [rows][cols] with zeros in the columns past cols, for up to kPadCopies arrays in
+// one launch; rows whose target is `ignore` are zero where a target is given. ldd * size is a
+// multiple of 16.
+constexpr int kPadCopies = 5;
+struct GemmPad {
+    const void* src;
+    void* dst;
+    int64_t rows;
+    int cols, ldd;
+};
+struct GemmPads {
+    GemmPad p[kPadCopies];
+    int64_t first[kPadCopies + 1];  // first 16-byte piece of each in a row of all pieces
+    int n = 0;
+    void add(int dtype, const void* src, void* dst, int64_t rows, int64_t cols, int64_t ldd) {
+        p[n] = GemmPad{src, dst, rows, (int)cols, (int)ldd};
+        first[0] = 0;
+        first[n + 1] = first[n] + rows * (ldd / (dtype == M3_DTYPE_BF16 ? 8 : 4));
+        ++n;
+    }
+};
+int gemm_pad_copy(int dtype, const GemmPads& pads, const int64_t* target, int64_t ignore, hipStream_t stream);
 
 inline GemmArgs gemm_args(GemmOp a, GemmOp b, int64_t m, int64_t n, int64_t k, int splits) {
     GemmArgs g;

@@ -160,39 +160,41 @@ int gemm_reduce(int dtype, const GemmStore& st, int splits, int batch, hipStream
 
 // One thread writes 16 bytes of a row; src rows of whole, aligned pieces are read the same way.
 template <typename T>
-__global__ __launch_bounds__(256) void gemm_pad_kernel(const T* __restrict__ src, T* __restrict__ dst, int64_t rows,
-                                                       int cols, int ldd, const int64_t* __restrict__ target,
-                                                       int64_t ignore) {
+__global__ __launch_bounds__(256) void gemm_pad_kernel(GemmPads pads, const int64_t* __restrict__ target, int64_t ignore) {
     constexpr int E = 16 / sizeof(T);
     typedef T Piece __attribute__((ext_vector_type(E)));
-    const int per = ldd / E;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / per;
-        const int c = (int)(i - r * per) * E;
+    const int64_t all = pads.first[pads.n];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+        GemmPad p = pads.p[0];
+        int64_t at = i;
+#pragma unroll
+        for (int k = 1; k < kPadCopies; ++k)
+            if (k < pads.n && i >= pads.first[k]) p = pads.p[k], at = i - pads.first[k];
+        const int per = p.ldd / E;
+        const int64_t r = at / per;
+        const int c = (int)(at - r * per) * E;
+        const T* src = reinterpret_cast<const T*>(p.src) + r * p.cols + c;
         Piece v;
         if (target && target[r] == ignore) {
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] = (T)0.f;
-        } else if (cols % E == 0) {
-            v = *reinterpret_cast<const Piece*>(src + r * cols + c);
+        } else if (p.cols % E == 0) {
+            v = *reinterpret_cast<const Piece*>(src);
         } else {
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = c + e < cols ? src[r * cols + c + e] : (T)0.f;
+            for (int e = 0; e < E; ++e) v[e] = c + e < p.cols ? src[e] : (T)0.f;
         }
-        *reinterpret_cast<Piece*>(dst + r * ldd + c) = v;
+        *reinterpret_cast<Piece*>(reinterpret_cast<T*>(p.dst) + r * p.ldd + c) = v;
     }
 }
 
-int gemm_pad_copy(int dtype, const void* src, void* dst, int64_t rows, int64_t cols, int64_t ldd,
-                  const int64_t* target, int64_t ignore, hipStream_t stream) {
-    const int64_t pieces = rows * (ldd / (dtype == M3_DTYPE_BF16 ? 8 : 4));
-    const dim3 grid((unsigned)std::min<int64_t>((pieces + 255) / 256, 16384));
+int gemm_pad_copy(int dtype, const GemmPads& pads, const int64_t* target, int64_t ignore, hipStream_t stream) {
+    if (pads.n == 0) return M3_OK;
+    const dim3 grid((unsigned)std::min<int64_t>((pads.first[pads.n] + 255) / 256, 16384));
     if (dtype == M3_DTYPE_BF16)
-        hipLaunchKernelGGL(gemm_pad_kernel<bf16>, grid, dim3(256), 0, stream, reinterpret_cast<const bf16*>(src),
-                           reinterpret_cast<bf16*>(dst), rows, (int)cols, (int)ldd, target, ignore);
+        hipLaunchKernelGGL(gemm_pad_kernel<bf16>, grid, dim3(256), 0, stream, pads, target, ignore);
     else
-        hipLaunchKernelGGL(gemm_pad_kernel<float>, grid, dim3(256), 0, stream, reinterpret_cast<const float*>(src),
-                           reinterpret_cast<float*>(dst), rows, (int)cols, (int)ldd, target, ignore);
+        hipLaunchKernelGGL(gemm_pad_kernel<float>, grid, dim3(256), 0, stream, pads, target, ignore);
     return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH;
 }
 

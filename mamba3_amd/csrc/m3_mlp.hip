@@ -252,11 +252,11 @@ KeptGu kept_gu(const MlpShape& s, const void* saved) {
 }
 int64_t gu_bytes(const MlpShape& s) { return up256(kept_gu(s, nullptr).elements * (s.dtype == M3_DTYPE_BF16 ? 6 : 8)); }
 
-// src as it is, or its padded copy
-int padded(const MlpShape& s, const void* src, void* dst, int64_t rows, int64_t cols, int64_t ldd, const void** out,
-           hipStream_t stream) {
-    *out = dst ? dst : src;
-    return dst ? gemm_pad_copy(s.dtype, src, dst, rows, cols, ldd, nullptr, 0, stream) : M3_OK;
+// src as it is, or its padded copy, which `pads` will make
+const void* padded(const MlpShape& s, GemmPads& pads, const void* src, void* dst, int64_t rows, int64_t cols, int64_t ldd) {
+    if (!dst) return src;
+    pads.add(s.dtype, src, dst, rows, cols, ldd);
+    return dst;
 }
 
 }  // namespace
@@ -283,10 +283,12 @@ int launch_swiglu_fwd(int64_t rows, int64_t d, int64_t ff, int dtype, const void
                       hipStream_t stream) {
     const MlpShape s = mlp_shape(rows, d, ff, dtype);
     const MlpFwd f = mlp_fwd_layout(s, saved != nullptr, ws);
-    M3_TRY(padded(s, x, f.x, rows, d, s.dp, &x, stream));
-    M3_TRY(padded(s, wg, f.wg, ff, d, s.dp, &wg, stream));
-    M3_TRY(padded(s, wu, f.wu, ff, d, s.dp, &wu, stream));
-    M3_TRY(padded(s, wd, f.wd, d, ff, s.fp, &wd, stream));
+    GemmPads pads;
+    x = padded(s, pads, x, f.x, rows, d, s.dp);
+    wg = padded(s, pads, wg, f.wg, ff, d, s.dp);
+    wu = padded(s, pads, wu, f.wu, ff, d, s.dp);
+    wd = padded(s, pads, wd, f.wd, d, ff, s.fp);
+    M3_TRY(gemm_pad_copy(dtype, pads, nullptr, 0, stream));
     void* h = saved ? reinterpret_cast<char*>(saved) + gu_bytes(s) : f.h;
     GemmArgs a = gemm_args({x, s.dp}, {wg, s.dp}, rows, ff, s.dp, 1);
     a.b[1] = {wu, s.dp};
@@ -301,17 +303,23 @@ int launch_swiglu_bwd(int64_t rows, int64_t d, int64_t ff, int dtype, const void
     const MlpShape s = mlp_shape(rows, d, ff, dtype);
     const MlpBwd f = mlp_bwd_layout(s, ws);
     const void* h = reinterpret_cast<const char*>(saved) + gu_bytes(s);
-    M3_TRY(padded(s, dy, f.dy, rows, d, s.dp, &dy, stream));
-    if (dx || dwg || dwu) {
-        M3_TRY(padded(s, wd, f.wd, d, ff, s.fp, &wd, stream));
+    const bool gates = dx || dwg || dwu;
+    GemmPads pads;
+    dy = padded(s, pads, dy, f.dy, rows, d, s.dp);
+    if (gates) wd = padded(s, pads, wd, f.wd, d, ff, s.fp);
+    if (dx) {
+        wg = padded(s, pads, wg, f.wg, ff, d, s.dp);
+        wu = padded(s, pads, wu, f.wu, ff, d, s.dp);
+    }
+    if (dwg || dwu) x = padded(s, pads, x, f.x, rows, d, s.dp);
+    M3_TRY(gemm_pad_copy(dtype, pads, nullptr, 0, stream));
+    if (gates) {
         // rows of Wd past d do not exist: A's pad columns meet zeros
         GemmArgs a = gemm_args({dy, s.dp}, {wd, s.fp}, rows, s.fp, s.dp, 1);
         a.KB[0] = (int)d;
         M3_TRY((gemm_dispatch<true, false, kPlain>(dtype, f.dh, a, EpiGateBwd{f.dg, f.du, kept_gu(s, saved), scale, (int)rows, (int)s.fp}, rows, s.fp, 1, stream)));
     }
     if (dx) {
-        M3_TRY(padded(s, wg, f.wg, ff, d, s.dp, &wg, stream));
-        M3_TRY(padded(s, wu, f.wu, ff, d, s.dp, &wu, stream));
         GemmArgs a = gemm_args({f.dg, s.fp}, {wg, s.dp}, rows, s.dp, s.fp, 1);
         a.a[1] = {f.du, s.fp}, a.b[1] = {wu, s.dp};
         a.K[1] = (int)s.fp;
@@ -320,7 +328,6 @@ int launch_swiglu_bwd(int64_t rows, int64_t d, int64_t ff, int dtype, const void
         M3_TRY(gemm_store(kFormNN, dtype, f.dx, a, st, 1, stream));
     }
     if (dwg || dwu) {
-        M3_TRY(padded(s, x, f.x, rows, d, s.dp, &x, stream));
         GemmArgs a = gemm_args({dwg ? f.dg : f.du, s.fp}, {x, s.dp}, s.fp, s.dp, rows, 1);
         if (dwg && dwu) a.a[1] = {f.du, s.fp};
         const GemmStore st{{dwg ? dwg : dwu, dwg ? dwu : nullptr}, d, nullptr, 1.f, f.part, 0, (int)ff, (int)d};

@@ -305,7 +305,7 @@ XentBwd xent_bwd_layout(int64_t rows, int64_t d, int64_t vocab, int dtype, bool 
     f.h = b.take(rows * dp * size);
     f.w = dp != d ? b.take(vocab * dp * size) : nullptr;
     f.dz = b.take(rows * f.piece * size);
-    f.part = want_dh ? reinterpret_cast<float*>(b.take((int64_t)f.dh.splits * rows * d * 4)) : nullptr;
+    f.part = want_dh && (pieces > 1 || f.dh.splits > 1) ? reinterpret_cast<float*>(b.take((int64_t)f.dh.splits * rows * d * 4)) : nullptr;
     f.part_dw = want_dw ? reinterpret_cast<float*>(b.take((int64_t)gemm_part_bytes(f.dw, 1, f.piece, d))) : nullptr;
     f.bytes = b.used;
     return f;
@@ -332,8 +332,10 @@ int launch_xent_fwd(int64_t rows, int64_t d, int64_t vocab, int dtype, int reduc
     const XentFwd f = xent_fwd_layout(rows, d, vocab, dtype, ws);
     const int64_t dp = gemm_pad(d, dtype);
     if (f.h) {
-        M3_TRY(gemm_pad_copy(dtype, hidden, f.h, rows, d, dp, nullptr, 0, stream));
-        M3_TRY(gemm_pad_copy(dtype, weight, f.w, vocab, d, dp, nullptr, 0, stream));
+        GemmPads pads;
+        pads.add(dtype, hidden, f.h, rows, d, dp);
+        pads.add(dtype, weight, f.w, vocab, d, dp);
+        M3_TRY(gemm_pad_copy(dtype, pads, nullptr, 0, stream));
         hidden = f.h, weight = f.w;
     }
     M3_TRY((gemm_dispatch<true, true, kPlain>(dtype, f.z, gemm_args({hidden, dp}, {weight, dp}, rows, vocab, dp, 1),
@@ -351,9 +353,12 @@ int launch_xent_bwd(int64_t rows, int64_t d, int64_t vocab, int dtype, int reduc
                     const float* grad_loss, void* dhidden, void* dweight, void* ws, hipStream_t stream) {
     const XentBwd f = xent_bwd_layout(rows, d, vocab, dtype, dhidden != nullptr, dweight != nullptr, ws);
     const int64_t dp = gemm_pad(d, dtype), size = dtype == M3_DTYPE_BF16 ? 2 : 4;
-    M3_TRY(gemm_pad_copy(dtype, hidden, f.h, rows, d, dp, target, ignore, stream));
+    GemmPads live, pads;
+    live.add(dtype, hidden, f.h, rows, d, dp);
+    M3_TRY(gemm_pad_copy(dtype, live, target, ignore, stream));
     if (f.w) {
-        M3_TRY(gemm_pad_copy(dtype, weight, f.w, vocab, d, dp, nullptr, 0, stream));
+        pads.add(dtype, weight, f.w, vocab, d, dp);
+        M3_TRY(gemm_pad_copy(dtype, pads, nullptr, 0, stream));
         weight = f.w;
     }
     const int r = (int)rows;
@@ -372,6 +377,7 @@ int launch_xent_bwd(int64_t rows, int64_t d, int64_t vocab, int dtype, int reduc
         if (dhidden) {
             GemmArgs a = gemm_args({f.dz, f.piece}, {w, dp}, rows, dp, f.piece, 1);
             a.KB[0] = (int)have;
+            if (f.piece >= vocab) dh.out[0] = dhidden;  // one piece: no sum over calls
             M3_TRY(gemm_store(kFormNN, dtype, f.dh, a, dh, 1, stream));
             dh.add = 1;
         }
@@ -382,7 +388,7 @@ int launch_xent_bwd(int64_t rows, int64_t d, int64_t vocab, int dtype, int reduc
             M3_TRY(gemm_store(kFormTN, dtype, f.dw, gemm_args({f.dz, f.piece}, {f.h, dp}, f.piece, dp, rows, 1), dw, 1, stream));
         }
     }
-    if (dhidden) {
+    if (dhidden && f.piece < vocab) {
         dh.out[0] = dhidden;
         M3_TRY(gemm_reduce(dtype, dh, f.dh.splits, 1, stream));
     }

@@ -16,6 +16,7 @@ source tensor and version.
 
 from __future__ import annotations
 
+import contextlib
 import weakref
 from collections import OrderedDict
 from typing import Optional
@@ -708,8 +709,17 @@ def _(gate_up, d_ff):
 # ---------------------------------------------------------------- training operators
 def _flat(t: torch.Tensor) -> torch.Tensor:
     """t as contiguous, 16-byte aligned rows of its last dimension."""
-    t = t.detach().reshape(-1, t.shape[-1]).contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    if t.dim() != 2 or not t.is_contiguous():
+        t = t.detach().reshape(-1, t.shape[-1]).contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.detach().clone()
+
+
+def on_device(t: torch.Tensor):
+    """t's device as the current one (kernels are launched, and workspaces allocated, there)."""
+    return _NO_SWITCH if _C._cuda_getDevice() == t.get_device() else torch.cuda.device(t.device)
+
+
+_NO_SWITCH = contextlib.nullcontext()
 
 
 def check_alike(what: str, *tensors: torch.Tensor) -> None:
@@ -730,7 +740,7 @@ def _swiglu_mlp_eager(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     """m3_swiglu_mlp_fwd over the last dimension of x: y in x's shape and, with `keep`, what the
     backward reads (else None)."""
     _native.require_gpu(x, w_gate, w_up, w_down, residual)
-    with torch.cuda.device(x.device):
+    with on_device(x):
         x2 = _flat(x)
         y = torch.empty(x2.shape, device=x.device, dtype=x.dtype)
         n = _native.swiglu_mlp_saved_bytes(*x2.shape, w_gate.shape[0], x.dtype) if keep else 0
@@ -756,17 +766,23 @@ def _(x, w_gate, w_up, w_down, residual, scale, keep):
     return x.new_empty(x.shape), x.new_empty(n, dtype=torch.uint8)
 
 
+def _swiglu_mlp_bwd_eager(x, w_gate, w_up, w_down, scale, saved, dy, want) -> list:
+    """m3_swiglu_mlp_bwd: gradients of x, w_gate, w_up and w_down in their shapes, None for those that
+    `want` leaves out."""
+    with on_device(x):
+        out = [torch.empty(t.shape, device=x.device, dtype=x.dtype) if w else None
+               for t, w in zip((x, w_gate, w_up, w_down), want)]
+        dy2 = _flat(dy if dy.dtype == x.dtype else dy.to(x.dtype))
+        _native.swiglu_mlp_bwd(_flat(x), _flat(w_gate), _flat(w_up), _flat(w_down), scale, saved, dy2, *out)
+    return out
+
+
 @torch.library.custom_op(f"{NS}::swiglu_mlp_bwd", mutates_args=())
 def swiglu_mlp_bwd(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
                    scale: float, saved: torch.Tensor, dy: torch.Tensor,
                    want: list[bool]) -> list[torch.Tensor]:
-    """m3_swiglu_mlp_bwd: gradients of x, w_gate, w_up and w_down in their shapes; those that
-    `want` leaves out are empty."""
-    with torch.cuda.device(x.device):
-        x2, dy2 = _flat(x), _flat(dy.to(x.dtype))
-        out = [torch.empty(t.shape, device=x.device, dtype=x.dtype) if w else None
-               for t, w in zip((x, w_gate, w_up, w_down), want)]
-        _native.swiglu_mlp_bwd(x2, _flat(w_gate), _flat(w_up), _flat(w_down), scale, saved, dy2, *out)
+    """_swiglu_mlp_bwd_eager as an op; gradients that `want` leaves out are empty."""
+    out = _swiglu_mlp_bwd_eager(x, w_gate, w_up, w_down, scale, saved, dy, want)
     return [x.new_empty(0) if t is None else t for t in out]
 
 
@@ -796,12 +812,32 @@ def _swiglu_mlp_backward(ctx, dy, _):
 swiglu_mlp.register_autograd(_swiglu_mlp_backward, setup_context=_swiglu_mlp_setup)
 
 
+class _SwigluMlp(torch.autograd.Function):
+    """swiglu_mlp under eager autograd: the same calls without the dispatcher's host time (the op and
+    its formula cost 150 us a training step, this 40)."""
+
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, residual, scale):
+        y, saved = _swiglu_mlp_eager(x, w_gate, w_up, w_down, residual, scale, True)
+        ctx.scale = scale
+        ctx.save_for_backward(x, w_gate, w_up, w_down, saved)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        *tensors, saved = ctx.saved_tensors
+        want = ctx.needs_input_grad
+        g = _swiglu_mlp_bwd_eager(*tensors, ctx.scale, saved, dy, want[:4]) if any(want[:4]) else [None] * 4
+        return (*g, dy if want[4] else None, None)
+
+
 def _linear_xent_eager(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor,
                        ignore_index: int,
                        reduction: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """m3_linear_xent_fwd: (loss, fp32, of target's shape or a scalar; lse (rows,); count (1,))."""
     _native.require_gpu(hidden, weight, target)
-    with torch.cuda.device(hidden.device):
+    with on_device(hidden):
         h2, t1 = _flat(hidden), target.reshape(-1).contiguous()
         new = lambda *s: torch.empty(s, device=hidden.device, dtype=torch.float32)  # noqa: E731
         loss = new(*target.shape) if reduction == 0 else new()
@@ -820,16 +856,24 @@ def _(hidden, weight, target, ignore_index, reduction):
             hidden.new_empty(target.numel(), dtype=f), hidden.new_empty(1, dtype=f))
 
 
+def _linear_xent_bwd_eager(hidden, weight, target, ignore_index, reduction, lse, count, grad, want) -> list:
+    """m3_linear_xent_bwd: gradients of hidden and weight, None for those that `want` leaves out."""
+    with on_device(hidden):
+        out = [torch.empty(t.shape, device=t.device, dtype=t.dtype) if w else None
+               for t, w in zip((hidden, weight), want)]
+        if grad.dtype != torch.float32 or not grad.is_contiguous():
+            grad = grad.float().contiguous()
+        _native.linear_xent_bwd(_flat(hidden), _flat(weight), target.reshape(-1).contiguous(), ignore_index,
+                                reduction, lse, count, grad, *out)
+    return out
+
+
 @torch.library.custom_op(f"{NS}::linear_xent_bwd", mutates_args=())
 def linear_xent_bwd(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int,
                     reduction: int, lse: torch.Tensor, count: torch.Tensor, grad: torch.Tensor,
                     want: list[bool]) -> list[torch.Tensor]:
-    """m3_linear_xent_bwd: gradients of hidden and weight; those that `want` leaves out are empty."""
-    with torch.cuda.device(hidden.device):
-        out = [torch.empty(t.shape, device=t.device, dtype=t.dtype) if w else None
-               for t, w in zip((hidden, weight), want)]
-        _native.linear_xent_bwd(_flat(hidden), _flat(weight), target.reshape(-1).contiguous(), ignore_index,
-                                reduction, lse, count, grad.float().contiguous(), *out)
+    """_linear_xent_bwd_eager as an op; gradients that `want` leaves out are empty."""
+    out = _linear_xent_bwd_eager(hidden, weight, target, ignore_index, reduction, lse, count, grad, want)
     return [hidden.new_empty(0) if t is None else t for t in out]
 
 
@@ -856,6 +900,24 @@ def _linear_xent_backward(ctx, g_loss, g_lse, g_count):
 linear_xent.register_autograd(_linear_xent_backward, setup_context=_linear_xent_setup)
 
 
+class _LinearXent(torch.autograd.Function):
+    """linear_xent under eager autograd, without the dispatcher's host time."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, target, ignore_index, reduction):
+        loss, lse, count = _linear_xent_eager(hidden, weight, target, ignore_index, reduction)
+        ctx.cfg = ignore_index, reduction
+        ctx.save_for_backward(hidden, weight, target, lse, count)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        hidden, weight, target, lse, count = ctx.saved_tensors
+        g = _linear_xent_bwd_eager(hidden, weight, target, *ctx.cfg, lse, count, grad, ctx.needs_input_grad[:2])
+        return (*g, None, None, None)
+
+
 # ---------------------------------------------------------------- eager calls
 # What a direct call may be given: a subclass's own dispatch has to see it.
 _PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
@@ -867,7 +929,12 @@ def _direct(*tensors) -> bool:
     calls under autograd, a dispatch or function mode, a functorch transform or forward-mode
     AD, and calls with a tensor subclass among `tensors` (all tensor arguments of the op) go
     through the registered ops and their formulas."""
-    if _is_grad_enabled() or _is_compiling():
+    return not _is_grad_enabled() and _plain(*tensors)
+
+
+def _plain(*tensors) -> bool:
+    """_direct's conditions but for autograd: what a torch.autograd.Function may stand in for."""
+    if _is_compiling():
         return False
     if (_in_dispatch_mode() or _in_function_mode() or _tracing_state() is not None
             or _functorch_stack() is not None or _forward_ad._current_level >= 0):
@@ -883,7 +950,7 @@ try:
     _tracing_state, _functorch_stack = _C._get_tracing_state, _C._functorch.peek_interpreter_stack
     _forward_ad._current_level
 except AttributeError:
-    def _direct(*tensors) -> bool:
+    def _plain(*tensors) -> bool:
         return False
 
 
@@ -914,10 +981,16 @@ def rmsnorm_fast(x, weight, eps):
 
 
 def swiglu_mlp_fast(x, w_gate, w_up, w_down, residual, scale, keep):
-    fn = _swiglu_mlp_eager if _direct(x, w_gate, w_up, w_down, residual) else swiglu_mlp
-    return fn(x, w_gate, w_up, w_down, residual, scale, keep)[0]
+    if not _plain(x, w_gate, w_up, w_down, residual):
+        return swiglu_mlp(x, w_gate, w_up, w_down, residual, scale, keep)[0]
+    if keep:
+        return _SwigluMlp.apply(x, w_gate, w_up, w_down, residual, scale)
+    return _swiglu_mlp_eager(x, w_gate, w_up, w_down, residual, scale, False)[0]
 
 
 def linear_xent_fast(hidden, weight, target, ignore_index, reduction):
-    fn = _linear_xent_eager if _direct(hidden, weight, target) else linear_xent
-    return fn(hidden, weight, target, ignore_index, reduction)[0]
+    if not _plain(hidden, weight, target):
+        return linear_xent(hidden, weight, target, ignore_index, reduction)[0]
+    if _is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return _LinearXent.apply(hidden, weight, target, ignore_index, reduction)
+    return _linear_xent_eager(hidden, weight, target, ignore_index, reduction)[0]
