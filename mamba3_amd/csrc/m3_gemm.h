@@ -95,12 +95,18 @@ struct GemmLoader {
     static_assert(kInstr % NW == 0 && NI >= 1, "tile too small for the block");
     unsigned voff[NI];
 
+    // Which of the tile's instructions is a wave's i-th: with rows of m or n the first half of them
+    // fetches the first half of the step's k.
+    static __device__ __forceinline__ int instr(int wave, int i) {
+        if constexpr (kKc || NI == 1) return wave * NI + i;
+        else return i / (NI / 2) * (kInstr / 2) + wave * (NI / 2) + i % (NI / 2);
+    }
     // ld: row stride in elements; row_shift: rows before this wave's in the tile (kGated); pieces: valid
     // 16-byte pieces of the rows (kKc), the others are read out of bounds, as zeros
     __device__ __forceinline__ void init(int wave, int lane, int ld, int row_shift, int pieces) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const int r = (wave * NI + i) * RPI + lane / CPR, c = lane % CPR;
+            const int r = instr(wave, i) * RPI + lane / CPR, c = lane % CPR;
             if constexpr (kKc) {
                 const int piece = c ^ (r & 7);
                 voff[i] = piece < pieces ? (unsigned)((r - row_shift) * ld * SZ + piece * 16) : kOob;
@@ -122,7 +128,7 @@ struct GemmLoader {
     __device__ __forceinline__ void issue(int i, const char* base, int bytes, unsigned lds, int wave) const {
         const u32x4 rs{(unsigned)reinterpret_cast<uintptr_t>(base), (unsigned)(reinterpret_cast<uintptr_t>(base) >> 32),
                        (unsigned)bytes, (unsigned)kRsrcFlags};
-        const unsigned at = lds + (wave * NI + i) * 1024;
+        const unsigned at = lds + instr(wave, i) * 1024;
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                      :
                      : "s"(at), "v"(voff[i]), "s"(rs)
@@ -377,9 +383,14 @@ __global__ __launch_bounds__(Tile::NT, 2) void gemm_kernel(GemmArgs a, Epi epi) 
     typename Type::Acc acc[FM][FN];
 
     // A step is two halves of KH k steps. While one half's fragments are multiplied, the next half's
-    // are read from LDS; all of a step has been read halfway through it, which frees its slot
-    // for the step ST further on. Copies and reads are issued between groups of FN MFMAs, which cover
-    // them, two a group: early in the half, so that they have landed when they are waited for.
+    // are read from LDS. A barrier in front of a half says that all waves have read what lies before it,
+    // and that the next half's data has landed; what has been read makes room for the step ST further
+    // on. With rows of m or n a half of the copies fetches a half of the k, so each half has its
+    // barrier and refills its own place: copies then have one and a half steps to land. Rows of k
+    // would come in pieces of 64 bytes that way, which costs more than it gives (8192^3 x W^T 783 ->
+    // 827 us; dy^T x 823 -> 800): there the whole step's place is refilled halfway through it.
+    // Copies and reads are issued between groups of FN MFMAs, which cover them, early in the half.
+    constexpr bool kHalves = !kAKc && !kBKc && LA::NI > 1 && LB::NI > 1;
     typedef typename Type::Frag Frag;
     constexpr int KH = MF == 16 ? 1 : 2;
     constexpr int kGroups = KH * FM, kReads = KH * (FM + FN);
@@ -396,7 +407,16 @@ __global__ __launch_bounds__(Tile::NT, 2) void gemm_kernel(GemmArgs a, Epi epi) 
         for (int j = 0; j < FN; ++j) acc[i][j] = Type::mma(fb[half][ks][j], fa[half][ks][i], acc[i][j]);
     };
     constexpr int kPer = (kReads + kGroups - 1) / kGroups < 2 ? 2 : (kReads + kGroups - 1) / kGroups;
-    constexpr int kPerLd = (NLD + kGroups - 1) / kGroups < 2 ? 2 : (NLD + kGroups - 1) / kGroups;
+    constexpr int kLd = kHalves ? NLD / 2 : NLD;  // copies behind a barrier
+    constexpr int kPerLd = (kLd + kGroups - 1) / kGroups < 2 && !kHalves ? 2 : (kLd + kGroups - 1) / kGroups;
+    auto fetch_half = [&](int half, int i, int slot) {  // copy i of the kLd behind the barrier before `half`
+        if constexpr (kHalves) {
+            constexpr int A = LA::NI / 2;
+            fetch(i < A ? half * A + i : LA::NI + half * (LB::NI / 2) + i - A, slot);
+        } else {
+            fetch(i, slot);
+        }
+    };
 
     enter((int)blockIdx.x);
 #pragma unroll
@@ -423,30 +443,29 @@ __global__ __launch_bounds__(Tile::NT, 2) void gemm_kernel(GemmArgs a, Epi epi) 
 #pragma unroll
         for (int i = 0; i < kReads; ++i) read(0, slot, i);
         for (int n = first_step(it.split + 1) - first_step(it.split); n > 0; --n) {
+            const int next = slot + 1 == ST ? 0 : slot + 1;
             M3_FENCE();
 #pragma unroll
-            for (int g = 0; g < kGroups; ++g) {
+            for (int half = 0; half < 2; ++half) {
+                if (half == (kHalves ? 0 : 1)) advance();
+                if (kHalves || half == 1) {
+                    wait_vm_lds<NLD * (kHalves ? ST - 1 : ST - 2)>();
+                    M3_LDS_FENCE();
+                    __builtin_amdgcn_s_barrier();
+                    M3_LDS_FENCE();
+                }
 #pragma unroll
-                for (int i = g * kPer; i < (g + 1) * kPer && i < kReads; ++i) read(1, slot, i);
-                M3_FENCE();
-                group(0, g);
-                M3_FENCE();
-            }
-            advance();
-            const int next = slot + 1 == ST ? 0 : slot + 1;
-            wait_vm_lds<NLD * (ST - 2)>();  // the next step has landed, this wave has read this one
-            M3_LDS_FENCE();
-            __builtin_amdgcn_s_barrier();
-            M3_LDS_FENCE();
+                for (int g = 0; g < kGroups; ++g) {
+                    if (kHalves || half == 1) {
 #pragma unroll
-            for (int g = 0; g < kGroups; ++g) {
+                        for (int i = g * kPerLd; i < (g + 1) * kPerLd && i < kLd; ++i) fetch_half(half, i, slot);
+                    }
 #pragma unroll
-                for (int i = g * kPerLd; i < (g + 1) * kPerLd && i < NLD; ++i) fetch(i, slot);
-#pragma unroll
-                for (int i = g * kPer; i < (g + 1) * kPer && i < kReads; ++i) read(0, next, i);
-                M3_FENCE();
-                group(1, g);
-                M3_FENCE();
+                    for (int i = g * kPer; i < (g + 1) * kPer && i < kReads; ++i) read(half ^ 1, half ? next : slot, i);
+                    M3_FENCE();
+                    group(half, g);
+                    M3_FENCE();
+                }
             }
             slot = next;
         }

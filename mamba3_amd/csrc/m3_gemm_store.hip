@@ -200,14 +200,14 @@ int gemm_pad_copy(int dtype, const GemmPads& pads, const int64_t* target, int64_
 
 // Estimated us of each choice, from launches of 256, 512 and 1024 tiles of 8 and 64 k steps (torch on the
 // same card: 8192^3 bf16 668 us): a step of a 256 x 256 tile takes 1.45 us, of a 128 x 128 tile 0.62 us
-// alone on its CU and 0.85 us next to another, of a 64 x 64 tile 0.20 and 0.37 us; to that come a
+// alone on its CU and 0.90 us next to another, of a 64 x 64 tile 0.20 and 0.37 us; to that come a
 // tile's start and epilogue. Parts of k cost the fp32 partial sums' write and read and a launch.
 // What it decides, both sides measured: the gated product of 8192 x 11008 x 2048 takes 80 us less on 256 x 256
 // tiles than on 128 x 128, that of 8192 x 4224 x 768 8 us more; the 8192 x 768 product over 16128 takes
 // 70 us less in two parts on 256 x 256 tiles than in two on 128 x 128.
 GemmPlan gemm_plan(int dtype, int64_t rows, int64_t cols, int64_t steps, int batch, int max_splits) {
     struct Cost { int size, at_once; double alone, all, fixed; };
-    static const Cost bf[3] = {{256, 1, 1.45, 1.45, 8.0}, {128, 2, 0.62, 0.85, 4.5}, {64, 2, 0.20, 0.37, 3.5}};
+    static const Cost bf[3] = {{256, 1, 1.45, 1.45, 8.0}, {128, 2, 0.62, 0.90, 4.5}, {64, 2, 0.20, 0.37, 3.5}};
     static const Cost fp[3] = {{0, 0, 0, 0, 0}, {128, 2, 1.90, 3.60, 5.0}, {64, 2, 0.65, 1.07, 4.0}};
     const Cost* c = dtype == M3_DTYPE_BF16 ? bf : fp;
     GemmPlan best{kTileS, 1, 64, 64};
@@ -220,7 +220,7 @@ GemmPlan gemm_plan(int dtype, int64_t rows, int64_t cols, int64_t steps, int bat
             const int64_t rest = items % slots;
             double us = items / slots * (per * c[t].all + c[t].fixed);
             if (rest) us += per * (rest > 256 ? c[t].all : c[t].alone) + c[t].fixed;
-            if (s > 1) us += 4.0 + (double)rows * cols * batch * 8.0 * s / 4.0e6;
+            if (s > 1) us += 4.0 + (double)rows * cols * batch * 8.0 * s / 5.0e6;
             if (us < least) {
                 least = us;
                 best = GemmPlan{t, s, c[t].size, c[t].size};
