@@ -70,9 +70,9 @@ struct GemmOp {
     int64_t ld;
 };
 
-// Two terms (kSeg2: C = A0 B0 + A1 B1), two products (kBatch2) or two B halves
-// of a tile (kGated: columns [0, BN/2) from B0 and [BN/2, BN) from B1).
-enum GemmMode { kPlain, kSeg2, kBatch2, kGated };
+// Two terms (kSeg2: C = A0 B0 + A1 B1) or two B halves of a tile (kGated: columns [0, BN/2) from B0
+// and [BN/2, BN) from B1).
+enum GemmMode { kPlain, kSeg2, kGated };
 
 struct GemmArgs {
     GemmOp a[2], b[2];
@@ -80,9 +80,51 @@ struct GemmArgs {
     int K[2];    // inner lengths of the terms; multiples of 16 bytes for k-contiguous operands
     int KB[2];   // rows of B that exist where B is not k-contiguous (<= K: the rest reads as zero)
     int splits;  // k is cut into so many parts
-    int batch;   // products (1 or 2)
     int tiles_m, tiles_n;
 };
+
+// Products of one launch: product p has the work ids [first[p], first[p + 1]).
+template <int kN>
+struct GemmGroup {
+    GemmArgs a[kN];
+    int first[kN + 1];
+};
+// One of four scalars, field by field: an index known at run time only, a loop over the products or a
+// struct chosen as a whole would put the kernel argument into scratch memory.
+template <typename V>
+__device__ __forceinline__ V pick4(int p, V a, V b, V c, V d) {
+    const V lo = p == 1 ? b : a, hi = p == 3 ? d : c;
+    return p < 2 ? lo : hi;
+}
+#define M3_PICK(r, v, p, f) (r).f = pick4(p, (v)[0].f, (v)[1].f, (v)[2].f, (v)[3].f)
+
+template <int kN>
+__device__ __forceinline__ GemmArgs pick_args(const GemmArgs (&v)[kN], int p) {
+    if constexpr (kN == 1) {
+        return v[0];
+    } else {
+        static_assert(kN == 4, "one product or four");
+        GemmArgs r;
+        M3_PICK(r, v, p, a[0].p);
+        M3_PICK(r, v, p, a[0].ld);
+        M3_PICK(r, v, p, a[1].p);
+        M3_PICK(r, v, p, a[1].ld);
+        M3_PICK(r, v, p, b[0].p);
+        M3_PICK(r, v, p, b[0].ld);
+        M3_PICK(r, v, p, b[1].p);
+        M3_PICK(r, v, p, b[1].ld);
+        M3_PICK(r, v, p, K[0]);
+        M3_PICK(r, v, p, K[1]);
+        M3_PICK(r, v, p, KB[0]);
+        M3_PICK(r, v, p, KB[1]);
+        M3_PICK(r, v, p, M);
+        M3_PICK(r, v, p, N);
+        M3_PICK(r, v, p, splits);
+        M3_PICK(r, v, p, tiles_m);
+        M3_PICK(r, v, p, tiles_n);
+        return r;
+    }
+}
 
 // Global -> LDS copies of one operand's tile by the whole block.
 template <typename T, bool kKc, int BX, int NW, int MF>
@@ -263,29 +305,39 @@ struct GemmRows {
 
 // A block's piece of work: one tile of one product, one part of its k.
 struct GemmItem {
-    int tm, tn, batch, split;
+    int prob, tm, tn, split;
 };
-// Work id -> item. Ids go to the XCDs round robin (blocks are dispatched so, and a block's later ids are
-// a multiple of 8 further on): those of one XCD take a contiguous run of tiles, and runs walk
-// groups of 8 row tiles column by column, so that an XCD's L2 serves both operands.
+// Work id (counted from the product's first) -> item. Ids go to the XCDs round robin (blocks are
+// dispatched so, and a block's later ids are a multiple of 8 further on): those of one XCD take a
+// contiguous run of tiles, and runs walk groups of 8 row tiles column by column, so that an
+// XCD's L2 serves both operands.
 // (Quotients come from the vector unit: readfirstlane brings these back to scalar registers, which the
 // copies' operands have to be in.)
 __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ GemmItem gemm_item(const GemmArgs& a, int id) {
+__device__ __forceinline__ GemmItem gemm_item(const GemmArgs& a, int prob, int id) {
     const int total = a.tiles_m * a.tiles_n;
-    const int outer = scalar(id / total), b = id - outer * total;
+    const int split = scalar(id / total), b = id - split * total;
     const int x = b & 7, per = total >> 3, rest = total & 7;
     const int at = x * per + (x < rest ? x : rest) + (b >> 3);
     constexpr int G = 8;
     const int group = scalar(at / (G * a.tiles_n)), first = group * G;
     const int rows = a.tiles_m - first < G ? a.tiles_m - first : G;
     const int in = at - group * (G * a.tiles_n);
-    const int tn = scalar(in / rows), split = a.batch == 1 ? outer : outer >> 1;
-    return GemmItem{first + in - tn * rows, tn, outer - split * a.batch, split};
+    const int tn = scalar(in / rows);
+    return GemmItem{prob, first + in - tn * rows, tn, split};
+}
+// The k steps of a product, and where part `split` of them begins (steps < 2^26, splits <= 16).
+template <int kMode, int BK>
+__device__ __forceinline__ int gemm_steps_of(const GemmArgs& a) {
+    return (a.K[0] + BK - 1) / BK + (kMode == kSeg2 ? (a.K[1] + BK - 1) / BK : 0);
+}
+__device__ __forceinline__ int gemm_first_step(int steps, int splits, int split) {
+    return scalar((int)((unsigned)steps * (unsigned)split / (unsigned)splits));
 }
 
-template <typename T, typename Tile, bool kAKc, bool kBKc, int kMode, typename Epi>
-__global__ __launch_bounds__(Tile::NT, 2) void gemm_kernel(GemmArgs a, Epi epi) {
+// The items of products [kP0, kP1) of a group that fall to this block: ids congruent to its own.
+template <typename T, typename Tile, bool kAKc, bool kBKc, int kMode, int kP0, int kP1, int kN, typename Epi>
+__device__ __forceinline__ void gemm_run(const GemmGroup<kN>& grp, const Epi& epi) {
     constexpr int BM = Tile::BM, BN = Tile::BN, FM = Tile::FM, FN = Tile::FN, ST = Tile::STAGES, MF = Tile::MF;
     constexpr int BK = 128 / sizeof(T), SZ = sizeof(T);
     typedef GemmLoader<T, kAKc, BM, Tile::NW, MF> LA;
@@ -295,12 +347,29 @@ __global__ __launch_bounds__(Tile::NT, 2) void gemm_kernel(GemmArgs a, Epi epi) 
     extern __shared__ __align__(16) char gemm_smem[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int items = a.tiles_m * a.tiles_n * a.batch * a.splits;
-
-    // the k steps of an item: a part of the terms' steps in a row
-    const int st0 = (a.K[0] + BK - 1) / BK;
-    const int steps = st0 + (kMode == kSeg2 ? (a.K[1] + BK - 1) / BK : 0);
-    auto first_step = [&](int split) { return scalar((int)((unsigned)steps * (unsigned)split / (unsigned)a.splits)); };  // steps < 2^26, splits <= 16
+    const int grid = (int)gridDim.x, id_end = grp.first[kP1];
+    int id0 = grp.first[kP0];
+    if constexpr (kP0 > 0) {
+        const int r = id0 - scalar(id0 / grid) * grid;  // whose turn it is
+        id0 += ((int)blockIdx.x >= r ? 0 : grid) + (int)blockIdx.x - r;
+    } else {
+        id0 = (int)blockIdx.x;
+    }
+    if (id0 >= id_end) return;
+    auto args_of = [&](int p) __attribute__((always_inline)) {
+        if constexpr (kP1 - kP0 == 1) return grp.a[kP0];
+        else return pick_args(grp.a, p);
+    };
+    static_assert(kP1 - kP0 <= 1 || (kP0 == 1 && kP1 == 4), "one product, or the last three of four");
+    auto item_of = [&](int id) __attribute__((always_inline)) {
+        int p = kP0, first = grp.first[kP0];
+        if constexpr (kP1 - kP0 == 3) {
+            const int f2 = grp.first[2], f3 = grp.first[3];
+            p = id >= f3 ? 3 : id >= f2 ? 2 : 1;
+            first = id >= f3 ? f3 : id >= f2 ? f2 : first;
+        }
+        return gemm_item(args_of(p), p, id - first);
+    };
 
     const bool second = kMode == kGated && wave * LB::NI >= LB::kInstr / 2;
     static_assert(kMode != kGated || (LB::kInstr / 2) % LB::NI == 0, "a wave fetches from one half");
@@ -312,26 +381,23 @@ __global__ __launch_bounds__(Tile::NT, 2) void gemm_kernel(GemmArgs a, Epi epi) 
     const char *pa, *pb;
     int64_t pa_step, pb_step;
     int ba, bb, turn, fs, f_id, f_end;
-    auto set_up = [&]() {
-        if (f_id >= items) {
-            ba = bb = 0;
-            pa_step = pb_step = 0;
-            turn = 0x7fffffff;
-            return;
-        }
-        const GemmItem it = gemm_item(a, f_id);
+    auto set_up = [&]() __attribute__((always_inline)) {
+        const GemmItem it = item_of(f_id);
+        const GemmArgs a = args_of(it.prob);
+        const int st0 = (a.K[0] + BK - 1) / BK, steps = gemm_steps_of<kMode, BK>(a);
         const int m0 = it.tm * BM, n0 = it.tn * (kMode == kGated ? BN / 2 : BN);
         // rows that exist in this tile: spans end with the last one's last valid element (< 2^31 bytes)
         const int ra_rows = a.M - m0 < BM ? a.M - m0 : BM, rb_rows = a.N - n0 < BN ? a.N - n0 : BN;
         const int seg = kMode == kSeg2 && fs >= st0 ? 1 : 0;
         const int k0 = (seg ? fs - st0 : fs) * BK;
-        const int left = a.K[seg] - k0, krem = left < BK ? left : BK;
-        const int ia = kMode == kSeg2 ? seg : kMode == kBatch2 ? it.batch : 0, ib = kMode == kGated ? (second ? 1 : 0) : ia;
-        const int bleft = a.KB[seg] - k0;
+        const int K = seg ? a.K[1] : a.K[0], KB = seg ? a.KB[1] : a.KB[0];
+        const int left = K - k0, krem = left < BK ? left : BK;
+        const GemmOp oa = seg ? a.a[1] : a.a[0], ob = seg || second ? a.b[1] : a.b[0];
+        const int bleft = KB - k0;
         const int brem = kBKc || krem < bleft ? krem : bleft;  // may be negative
-        const int lda = (int)a.a[ia].ld, ldb = (int)a.b[ib].ld;
-        pa = reinterpret_cast<const char*>(a.a[ia].p) + (kAKc ? (int64_t)m0 * lda + k0 : (int64_t)k0 * lda + m0) * SZ;
-        pb = reinterpret_cast<const char*>(a.b[ib].p) + (kBKc ? (int64_t)n0 * ldb + k0 : (int64_t)k0 * ldb + n0) * SZ;
+        const int lda = (int)oa.ld, ldb = (int)ob.ld;
+        pa = reinterpret_cast<const char*>(oa.p) + (kAKc ? (int64_t)m0 * lda + k0 : (int64_t)k0 * lda + m0) * SZ;
+        pb = reinterpret_cast<const char*>(ob.p) + (kBKc ? (int64_t)n0 * ldb + k0 : (int64_t)k0 * ldb + n0) * SZ;
         pa_step = kAKc ? 128 : (int64_t)BK * lda * SZ;
         pb_step = kBKc ? 128 : (int64_t)BK * ldb * SZ;
         ba = ra_rows <= 0 ? 0 : (kAKc ? (ra_rows - 1) * lda + krem : (krem - 1) * lda + ra_rows) * SZ;
@@ -340,22 +406,30 @@ __global__ __launch_bounds__(Tile::NT, 2) void gemm_kernel(GemmArgs a, Epi epi) 
         la.init(wave, lane, lda, 0, pieces);
         lb.init(wave, lane, ldb, second ? BN / 2 : 0, pieces);
         // whole steps of this term for both operands, then the next turn
-        const int whole = (kBKc || a.K[seg] < a.KB[seg] ? a.K[seg] : a.KB[seg]) / BK + (seg ? st0 : 0);
+        const int whole = (kBKc || K < KB ? K : KB) / BK + (seg ? st0 : 0);
         const int end = seg || kMode != kSeg2 ? steps : st0;
         turn = fs < whole ? whole : fs + 1 < end ? fs + 1 : end;
         turn = turn < f_end ? turn : f_end;
     };
-    auto enter = [&](int id) {  // the first step of an item
+    auto enter = [&](int id) __attribute__((always_inline)) {  // the first step of an item
         f_id = id;
-        const int split = id < items ? gemm_item(a, id).split : 0;
-        fs = first_step(split);
-        f_end = first_step(split + 1);
+        if (id >= id_end) {
+            ba = bb = 0;
+            pa_step = pb_step = 0;
+            turn = f_end = 0x7fffffff;
+            return;
+        }
+        const GemmItem it = item_of(id);
+        const GemmArgs a = args_of(it.prob);
+        const int steps = gemm_steps_of<kMode, BK>(a);
+        fs = gemm_first_step(steps, a.splits, it.split);
+        f_end = gemm_first_step(steps, a.splits, it.split + 1);
         set_up();
     };
-    auto advance = [&]() {
+    auto advance = [&]() __attribute__((always_inline)) {
         ++fs;
         if (fs == turn) {
-            if (fs == f_end) enter(f_id + (int)gridDim.x);
+            if (fs == f_end) enter(f_id + grid);
             else set_up();
         } else {
             pa += pa_step;
@@ -363,7 +437,7 @@ __global__ __launch_bounds__(Tile::NT, 2) void gemm_kernel(GemmArgs a, Epi epi) 
         }
     };
     const unsigned lds0 = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)gemm_smem);
-    auto fetch = [&](int i, int slot) {  // instruction i of NLD
+    auto fetch = [&](int i, int slot) __attribute__((always_inline)) {  // instruction i of NLD
         const unsigned sl = lds0 + slot * Tile::kStageBytes;
         if (i < LA::NI) la.issue(i, pa, ba, sl, wave);
         else lb.issue(i - LA::NI, pb, bb, sl + BM * 128, wave);
@@ -374,7 +448,7 @@ __global__ __launch_bounds__(Tile::NT, 2) void gemm_kernel(GemmArgs a, Epi epi) 
     ra.init(lane);
     rb.init(lane);
     const int wm = wave / Tile::WGN, wn = wave % Tile::WGN;
-    auto unit_b = [&](int fn) {
+    auto unit_b = [&](int fn) __attribute__((always_inline)) {
         if constexpr (kMode == kGated)
             return fn < FN / 2 ? wn * (FN / 2) + fn : BN / (2 * MF) + wn * (FN / 2) + fn - FN / 2;
         else
@@ -395,13 +469,13 @@ __global__ __launch_bounds__(Tile::NT, 2) void gemm_kernel(GemmArgs a, Epi epi) 
     constexpr int KH = MF == 16 ? 1 : 2;
     constexpr int kGroups = KH * FM, kReads = KH * (FM + FN);
     Frag fa[2][KH][FM], fb[2][KH][FN];
-    auto read = [&](int half, int slot, int i) {  // fragment i of a half
+    auto read = [&](int half, int slot, int i) __attribute__((always_inline)) {  // fragment i of a half
         const char* ta = gemm_smem + slot * Tile::kStageBytes;
         const int ks = i / (FM + FN), r = i % (FM + FN);
         if (r < FN) fb[half][ks][r] = rb.read(ta + BM * 128, unit_b(r), half * KH + ks);
         else fa[half][ks][r - FN] = ra.read(ta, wm * FM + r - FN, half * KH + ks);
     };
-    auto group = [&](int half, int g) {
+    auto group = [&](int half, int g) __attribute__((always_inline)) {
         const int ks = g / FM, i = g % FM;
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = Type::mma(fb[half][ks][j], fa[half][ks][i], acc[i][j]);
@@ -409,7 +483,7 @@ __global__ __launch_bounds__(Tile::NT, 2) void gemm_kernel(GemmArgs a, Epi epi) 
     constexpr int kPer = (kReads + kGroups - 1) / kGroups < 2 ? 2 : (kReads + kGroups - 1) / kGroups;
     constexpr int kLd = kHalves ? NLD / 2 : NLD;  // copies behind a barrier
     constexpr int kPerLd = (kLd + kGroups - 1) / kGroups < 2 && !kHalves ? 2 : (kLd + kGroups - 1) / kGroups;
-    auto fetch_half = [&](int half, int i, int slot) {  // copy i of the kLd behind the barrier before `half`
+    auto fetch_half = [&](int half, int i, int slot) __attribute__((always_inline)) {  // copy i of the kLd behind the barrier before `half`
         if constexpr (kHalves) {
             constexpr int A = LA::NI / 2;
             fetch(i < A ? half * A + i : LA::NI + half * (LB::NI / 2) + i - A, slot);
@@ -418,7 +492,7 @@ __global__ __launch_bounds__(Tile::NT, 2) void gemm_kernel(GemmArgs a, Epi epi) 
         }
     };
 
-    enter((int)blockIdx.x);
+    enter(id0);
 #pragma unroll
     for (int s = 0; s < ST; ++s) {
         if (s) advance();
@@ -428,8 +502,14 @@ __global__ __launch_bounds__(Tile::NT, 2) void gemm_kernel(GemmArgs a, Epi epi) 
     int slot = 0;
     // The steps of all items form one row: an item's last steps already fetch the next one's first,
     // which land during the epilogue.
-    for (int id = (int)blockIdx.x; id < items; id += (int)gridDim.x) {
-        const GemmItem it = gemm_item(a, id);
+    for (int id = id0; id < id_end; id += grid) {
+        const GemmItem it = item_of(id);
+        int n_steps;
+        {
+            const GemmArgs a = args_of(it.prob);
+            const int steps = gemm_steps_of<kMode, BK>(a);
+            n_steps = gemm_first_step(steps, a.splits, it.split + 1) - gemm_first_step(steps, a.splits, it.split);
+        }
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -442,7 +522,7 @@ __global__ __launch_bounds__(Tile::NT, 2) void gemm_kernel(GemmArgs a, Epi epi) 
         M3_LDS_FENCE();
 #pragma unroll
         for (int i = 0; i < kReads; ++i) read(0, slot, i);
-        for (int n = first_step(it.split + 1) - first_step(it.split); n > 0; --n) {
+        for (int n = n_steps; n > 0; --n) {
             const int next = slot + 1 == ST ? 0 : slot + 1;
             M3_FENCE();
 #pragma unroll
@@ -470,9 +550,18 @@ __global__ __launch_bounds__(Tile::NT, 2) void gemm_kernel(GemmArgs a, Epi epi) 
             slot = next;
         }
         const GemmPlace<Tile, kMode> at{it.tm * BM, it.tn * (kMode == kGated ? BN / 2 : BN), wm, wn, lane};
-        epi.template run<T, Tile, kMode>(a, at, acc, gemm_smem + Tile::kStages, it);
+        epi.template run<T, Tile, kMode>(at, acc, gemm_smem + Tile::kStages, it);
     }
-    wait_vm_lds<0>();  // no copy outlives its block
+    // no copy outlives its block, and none meets what the block does next in LDS
+    wait_vm_lds<0>();
+    M3_LDS_FENCE();
+    __builtin_amdgcn_s_barrier();
+    M3_LDS_FENCE();
+}
+
+template <typename T, typename Tile, bool kAKc, bool kBKc, int kMode, typename Epi>
+__global__ __launch_bounds__(Tile::NT, 2) void gemm_kernel(GemmGroup<1> grp, Epi epi) {
+    gemm_run<T, Tile, kAKc, kBKc, kMode, 0, 1>(grp, epi);
 }
 
 }  // namespace m3

@@ -21,10 +21,23 @@ struct GemmPlan {
     int bm, bn;
 };
 
-// The tile and the number of k parts with the least estimated time. rows x cols: C (for a
-// gated product, cols counts both halves); steps: k steps of 128 bytes; batch: products in one
-// launch; max_splits: 1 where the epilogue needs the whole sum.
-GemmPlan gemm_plan(int dtype, int64_t rows, int64_t cols, int64_t steps, int batch, int max_splits);
+// One product to be planned: rows x cols results (for a gated product, cols counts both halves) over
+// k steps of 128 bytes; max_splits 1 where the epilogue needs the whole sum; tn: both operands in rows of
+// m and n; sums: fp32 partial sums are written whatever the split.
+struct GemmTask {
+    int64_t rows, cols, steps;
+    int max_splits;
+    bool tn;
+};
+constexpr int kGroupMax = 4;
+constexpr int kMaxSplits = 16;
+struct GemmGroupPlan {
+    int tile;
+    int splits[kGroupMax];
+};
+// The tile for products of one launch and the number of k parts of each with the least estimated time.
+GemmGroupPlan gemm_group_plan(int dtype, const GemmTask* tasks, int n);
+GemmPlan gemm_plan(int dtype, int64_t rows, int64_t cols, int64_t steps, int max_splits);
 
 inline int64_t gemm_steps(int64_t k, int dtype) {
     const int bk = dtype == M3_DTYPE_BF16 ? 64 : 32;
@@ -36,16 +49,20 @@ inline int64_t gemm_pad(int64_t n, int dtype) {  // to 16 bytes
 }
 inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
-template <typename T, typename Tile, bool kAKc, bool kBKc, int kMode, typename Epi>
-int gemm_launch(GemmArgs a, const Epi& epi, int64_t rows, int64_t cols, int batch, hipStream_t stream) {
-    a.tiles_m = (int)((rows + Tile::BM - 1) / Tile::BM);
-    a.tiles_n = (int)((cols + Tile::BN - 1) / Tile::BN);
-    a.batch = batch;
-    const int64_t items = (int64_t)a.tiles_m * a.tiles_n * batch * a.splits;
-    if (items > 0x3fffffff) return M3_ERR_UNSUPPORTED;
-    auto* k = gemm_kernel<T, Tile, kAKc, kBKc, kMode, Epi>;
+// Launches k over the items of a group: as many blocks as run at once, each takes every grid-th item.
+template <typename Tile, int kN, typename... Rest>
+int gemm_launch_group(void (*k)(GemmGroup<kN>, Rest...), GemmGroup<kN> g, const int64_t (&rows)[kN], const int64_t (&cols)[kN],
+                      std::atomic<uint64_t>& done, hipStream_t stream, const Rest&... rest) {
+    int64_t items = 0;
+    for (int p = 0; p < kN; ++p) {
+        g.first[p] = (int)items;
+        g.a[p].tiles_m = (int)((rows[p] + Tile::BM - 1) / Tile::BM);
+        g.a[p].tiles_n = (int)((cols[p] + Tile::BN - 1) / Tile::BN);
+        items += (int64_t)g.a[p].tiles_m * g.a[p].tiles_n * g.a[p].splits;
+        if (items > 0x3fffffff) return M3_ERR_UNSUPPORTED;
+    }
+    g.first[kN] = (int)items;
     // once for each device (a bit of `done`; devices past 63 set it every time)
-    static std::atomic<uint64_t> done{0};
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) return M3_ERR_DEVICE;
     const uint64_t bit = dev < 63 ? (uint64_t)1 << dev : 0;
@@ -54,47 +71,65 @@ int gemm_launch(GemmArgs a, const Epi& epi, int64_t rows, int64_t cols, int batc
             return M3_ERR_LAUNCH;
         done.fetch_or(bit, std::memory_order_relaxed);
     }
-    // as many blocks as run at once; each takes every grid-th item
     constexpr int64_t kAtOnce = 256 * (Tile::NT >= 512 ? 1 : 2);
-    hipLaunchKernelGGL(k, dim3((unsigned)std::min(items, kAtOnce)), dim3(Tile::NT), Tile::kLds, stream, a, epi);
+    hipLaunchKernelGGL(k, dim3((unsigned)std::min(items, kAtOnce)), dim3(Tile::NT), Tile::kLds, stream, g, rest...);
     return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH;
+}
+
+template <typename T, typename Tile, bool kAKc, bool kBKc, int kMode, typename Epi>
+int gemm_launch(const GemmArgs& a, const Epi& epi, int64_t rows, int64_t cols, hipStream_t stream) {
+    static std::atomic<uint64_t> done{0};
+    GemmGroup<1> g;
+    g.a[0] = a;
+    return gemm_launch_group<Tile, 1, Epi>(gemm_kernel<T, Tile, kAKc, kBKc, kMode, Epi>, g, {rows}, {cols}, done, stream, epi);
 }
 
 template <bool kAKc, bool kBKc, int kMode, typename Epi>
 int gemm_dispatch(int dtype, const GemmPlan& p, const GemmArgs& a, const Epi& epi, int64_t rows, int64_t cols,
-                  int batch, hipStream_t stream) {
+                  hipStream_t stream) {
     if (dtype == M3_DTYPE_BF16) {
-        if (p.tile == kTileL) return gemm_launch<bf16, TileL, kAKc, kBKc, kMode>(a, epi, rows, cols, batch, stream);
-        if (p.tile == kTileM) return gemm_launch<bf16, TileM<bf16>, kAKc, kBKc, kMode>(a, epi, rows, cols, batch, stream);
-        return gemm_launch<bf16, TileS, kAKc, kBKc, kMode>(a, epi, rows, cols, batch, stream);
+        if (p.tile == kTileL) return gemm_launch<bf16, TileL, kAKc, kBKc, kMode>(a, epi, rows, cols, stream);
+        if (p.tile == kTileM) return gemm_launch<bf16, TileM<bf16>, kAKc, kBKc, kMode>(a, epi, rows, cols, stream);
+        return gemm_launch<bf16, TileS, kAKc, kBKc, kMode>(a, epi, rows, cols, stream);
     }
-    if (p.tile == kTileM) return gemm_launch<float, TileM<float>, kAKc, kBKc, kMode>(a, epi, rows, cols, batch, stream);
-    return gemm_launch<float, TileS, kAKc, kBKc, kMode>(a, epi, rows, cols, batch, stream);
+    if (p.tile == kTileM) return gemm_launch<float, TileM<float>, kAKc, kBKc, kMode>(a, epi, rows, cols, stream);
+    return gemm_launch<float, TileS, kAKc, kBKc, kMode>(a, epi, rows, cols, stream);
 }
 
-// Stores a product (m3_gemm_store.hip): out[z] (rows x cols, row stride ldo) = alpha * num / den * (A B) [+ res],
-// or, split or accumulated over calls, fp32 partial sums in `part` that gemm_reduce joins.
+// Stores a product (m3_gemm_store.hip): out (rows x cols, row stride ldo) = alpha * num / den * (A B)
+// [+ res], or, split or accumulated over calls, fp32 partial sums in `part` that gemm_reduce joins.
 struct GemmStore {
-    void* out[2];
+    void* out;
     int64_t ldo;
     const void* res;  // rows x cols, row stride ldo, or nullptr
     float alpha;
-    float* part;      // [splits][batch][rows][cols]
+    float* part;      // [splits][rows][cols]
     int add;          // the partial sums of an earlier call stay in `part`
     int rows, cols;
     const float *num = nullptr, *den = nullptr;  // on the device: a factor num / den (0 where den is 0)
+    int splits = 1;
 };
-enum GemmForm {
-    kFormNT,  // A rows of k, B rows of k
-    kFormNN,  // A rows of k, B [k][n], one or two terms
-    kFormTN   // A [k][m], B [k][n], `batch` products
+// x W^T: A and B rows of k
+int gemm_store(int dtype, const GemmPlan& p, GemmArgs a, GemmStore st, hipStream_t stream);
+// Gradient products of one launch: the first (which may be left out, rows 0) dy W, A rows of k and B
+// [k][n], of one or two terms; up to three dy^T x, A [k][m] and B [k][n]. A product whose `out` is nullptr
+// leaves its partial sums; the others' are joined here.
+struct GemmGrads {
+    GemmArgs a[kGroupMax];
+    GemmStore st[kGroupMax];
+    int n = 1;  // entry 0 is dy W's
+    GemmGrads() {
+        for (int p = 0; p < kGroupMax; ++p) {
+            a[p] = GemmArgs{};
+            st[p] = GemmStore{};
+        }
+    }
 };
-int gemm_store(GemmForm form, int dtype, const GemmPlan& p, GemmArgs a, const GemmStore& st, int batch,
-               hipStream_t stream);
-// out[z] = alpha * num / den * sum over s of part[s][z] [+ res]
-int gemm_reduce(int dtype, const GemmStore& st, int splits, int batch, hipStream_t stream);
-inline size_t gemm_part_bytes(const GemmPlan& p, int batch, int64_t rows, int64_t cols) {
-    return p.splits > 1 ? (size_t)up256((int64_t)p.splits * batch * rows * cols * 4) : 0;
+int gemm_grads(int dtype, const GemmGroupPlan& plan, GemmGrads g, hipStream_t stream);
+// out = alpha * num / den * sum over s of part[s] [+ res], for each entry with an `out` and parts
+int gemm_reduce(int dtype, const GemmStore* st, int n, hipStream_t stream);
+inline size_t gemm_part_bytes(int splits, int64_t rows, int64_t cols) {
+    return splits > 1 ? (size_t)up256((int64_t)splits * rows * cols * 4) : 0;
 }
 // dst [rows][ldd] = src [rows][cols] with zeros in the columns past cols, for up to kPadCopies arrays in
 // one launch; rows whose target is `ignore` are zero where a target is given. ldd * size is a
@@ -127,7 +162,6 @@ inline GemmArgs gemm_args(GemmOp a, GemmOp b, int64_t m, int64_t n, int64_t k, i
     g.K[0] = g.KB[0] = (int)k;
     g.K[1] = g.KB[1] = 0;
     g.splits = splits;
-    g.batch = 1;
     g.tiles_m = g.tiles_n = 0;
     return g;
 }

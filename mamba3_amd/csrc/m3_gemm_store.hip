@@ -17,6 +17,27 @@ __device__ __forceinline__ void store4(T* p, f32x4 v) {
     }
 }
 
+template <int kN>
+__device__ __forceinline__ GemmStore pick_store(const GemmStore (&v)[kN], int p) {
+    if constexpr (kN == 1) {
+        return v[0];
+    } else {
+        GemmStore r;
+        M3_PICK(r, v, p, out);
+        M3_PICK(r, v, p, ldo);
+        M3_PICK(r, v, p, res);
+        M3_PICK(r, v, p, alpha);
+        M3_PICK(r, v, p, part);
+        M3_PICK(r, v, p, add);
+        M3_PICK(r, v, p, rows);
+        M3_PICK(r, v, p, cols);
+        M3_PICK(r, v, p, num);
+        M3_PICK(r, v, p, den);
+        M3_PICK(r, v, p, splits);
+        return r;
+    }
+}
+
 // alpha with the factor that lies on the device
 __device__ __forceinline__ float store_scale(const GemmStore& s) {
     float f = s.alpha;
@@ -25,20 +46,24 @@ __device__ __forceinline__ float store_scale(const GemmStore& s) {
     return f;
 }
 
+template <int kN>
 struct EpiStore {
-    GemmStore s;
-    bool vec;  // whole 16-byte pieces
+    GemmStore st[kN];
+    bool whole[kN];  // results come in whole, aligned 16-byte pieces
 
     template <typename T, typename Tile, int kMode>
-    __device__ __forceinline__ void run(const GemmArgs& a, const GemmPlace<Tile, kMode>& at,
-                                        typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, const GemmItem& it) const {
-        const int z = it.batch;
-        T* out = reinterpret_cast<T*>(s.out[z]);
+    __device__ __forceinline__ void run(const GemmPlace<Tile, kMode>& at, typename Tile::Acc (&acc)[Tile::FM][Tile::FN],
+                                        char* smem, const GemmItem& it) const {
+        const GemmStore s = pick_store(st, it.prob);
+        bool vec;
+        if constexpr (kN == 1) vec = whole[0];
+        else vec = pick4(it.prob, whole[0], whole[1], whole[2], whole[3]);
+        T* out = reinterpret_cast<T*>(s.out);
         const T* res = reinterpret_cast<const T*>(s.res);
         const float alpha = s.part ? 1.f : store_scale(s);
         if (s.part) {
-            float* part = s.part + ((int64_t)it.split * a.batch + z) * s.rows * s.cols;
-            each(at, acc, [&](int m, int n, f32x4 v) {
+            float* part = s.part + (int64_t)it.split * s.rows * s.cols;
+            each(s, at, acc, [&](int m, int n, f32x4 v) {
                 float* p = part + (int64_t)m * s.cols + n;
                 if (vec) {
                     if (s.add) v += *reinterpret_cast<const f32x4*>(p);
@@ -71,7 +96,7 @@ struct EpiStore {
                 rows.store(out + (int64_t)r0 * s.ldo + c0, s.ldo, s.rows - r0, s.cols - c0);
             }
         } else {
-            each(at, acc, [&](int m, int n, f32x4 v) {
+            each(s, at, acc, [&](int m, int n, f32x4 v) {
                 const int64_t o = (int64_t)m * s.ldo + n;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
@@ -82,7 +107,7 @@ struct EpiStore {
 
     // f(m, n, four) for the fours that begin inside the result
     template <typename Place, typename Acc, int FM, int FN, typename F>
-    __device__ __forceinline__ void each(const Place& at, Acc (&acc)[FM][FN], F f) const {
+    static __device__ __forceinline__ void each(const GemmStore& s, const Place& at, Acc (&acc)[FM][FN], F f) {
         constexpr int Q = sizeof(Acc) / 16;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
@@ -100,61 +125,114 @@ struct EpiStore {
 static bool whole_pieces(int dtype, const GemmStore& s) {
     const int e = dtype == M3_DTYPE_BF16 ? 8 : 4;
     auto al = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-    return s.cols % e == 0 && s.ldo % e == 0 && al(s.out[0]) && al(s.out[1]) && al(s.res);
+    return s.cols % e == 0 && s.ldo % e == 0 && al(s.out) && al(s.res);
 }
 
-int gemm_store(GemmForm form, int dtype, const GemmPlan& p, GemmArgs a, const GemmStore& st, int batch,
-               hipStream_t stream) {
-    a.splits = p.splits;
-    EpiStore e{st, whole_pieces(dtype, st)};
-    if (p.splits == 1 && !st.add && st.out[0]) e.s.part = nullptr;
+// Where one part of a whole result goes: straight to `out`, unless sums are kept or joined.
+static void direct(GemmStore& st) {
+    if (st.splits == 1 && !st.add && st.out) st.part = nullptr;
+}
+
+int gemm_store(int dtype, const GemmPlan& p, GemmArgs a, GemmStore st, hipStream_t stream) {
+    a.splits = st.splits = p.splits;
+    EpiStore<1> e{{st}, {whole_pieces(dtype, st)}};
+    direct(e.st[0]);
+    const int r = gemm_dispatch<true, true, kPlain>(dtype, p, a, e, st.rows, st.cols, stream);
+    if (r != M3_OK || !e.st[0].part) return r;
+    return gemm_reduce(dtype, &st, 1, stream);
+}
+
+template <typename T, typename Tile>
+__global__ __launch_bounds__(Tile::NT, 2) void gemm_grads_kernel(GemmGroup<kGroupMax> grp, EpiStore<kGroupMax> epi) {
+    gemm_run<T, Tile, true, false, kSeg2, 0, 1>(grp, epi);
+    gemm_run<T, Tile, false, false, kPlain, 1, kGroupMax>(grp, epi);
+}
+
+template <typename T, typename Tile>
+static int launch_grads(const GemmGroup<kGroupMax>& grp, const EpiStore<kGroupMax>& e, hipStream_t stream) {
+    static std::atomic<uint64_t> done{0};
+    int64_t rows[kGroupMax], cols[kGroupMax];
+    for (int p = 0; p < kGroupMax; ++p) rows[p] = e.st[p].rows, cols[p] = e.st[p].cols;
+    return gemm_launch_group<Tile, kGroupMax, EpiStore<kGroupMax>>(gemm_grads_kernel<T, Tile>, grp, rows, cols, done, stream, e);
+}
+
+// The products share one launch: what one of them leaves of the last round of tiles the next one takes,
+// and there is one reduction. Apart, the four products of 8192 x 768 x 2112 took 178 us with their
+// reductions.
+int gemm_grads(int dtype, const GemmGroupPlan& plan, GemmGrads g, hipStream_t stream) {
+    GemmGroup<kGroupMax> grp;
+    EpiStore<kGroupMax> e;
+    bool join = false;
+    for (int p = 0; p < kGroupMax; ++p) {
+        g.st[p].splits = plan.splits[p];
+        grp.a[p] = g.a[p];
+        grp.a[p].splits = plan.splits[p];
+        e.st[p] = g.st[p];
+        e.whole[p] = whole_pieces(dtype, g.st[p]);
+        direct(e.st[p]);
+        join = join || (e.st[p].part && e.st[p].out && e.st[p].rows);
+        if (!e.st[p].part) g.st[p].part = nullptr;
+    }
     int r;
-    if (form == kFormNT) r = gemm_dispatch<true, true, kPlain>(dtype, p, a, e, st.rows, st.cols, 1, stream);
-    else if (form == kFormNN) r = gemm_dispatch<true, false, kSeg2>(dtype, p, a, e, st.rows, st.cols, 1, stream);
-    else r = gemm_dispatch<false, false, kBatch2>(dtype, p, a, e, st.rows, st.cols, batch, stream);
-    if (r != M3_OK || !e.s.part || !st.out[0]) return r;
-    return gemm_reduce(dtype, st, p.splits, batch, stream);
+    if (dtype == M3_DTYPE_BF16) {
+        r = plan.tile == kTileL   ? launch_grads<bf16, TileL>(grp, e, stream)
+            : plan.tile == kTileM ? launch_grads<bf16, TileM<bf16>>(grp, e, stream)
+                                  : launch_grads<bf16, TileS>(grp, e, stream);
+    } else {
+        r = plan.tile == kTileM ? launch_grads<float, TileM<float>>(grp, e, stream) : launch_grads<float, TileS>(grp, e, stream);
+    }
+    return r != M3_OK || !join ? r : gemm_reduce(dtype, g.st, kGroupMax, stream);
 }
 
-// One thread joins four columns of a row; parts are added in order.
-template <typename T, bool kVec>
-__global__ __launch_bounds__(256) void gemm_reduce_kernel(GemmStore s, int splits) {
-    const int z = blockIdx.y;
-    const int64_t each = (int64_t)s.rows * s.cols, stride = each * gridDim.y;
-    const float* part = s.part + z * each;
-    T* out = reinterpret_cast<T*>(s.out[z]);
+struct GemmReduce {
+    GemmStore st[kGroupMax];
+    bool whole[kGroupMax];
+};
+
+// One thread joins four columns of a row (or one element); parts are added in order. A grid row for each
+// result.
+template <typename T>
+__global__ __launch_bounds__(256) void gemm_reduce_kernel(GemmReduce r) {
+    const GemmStore s = pick_store(r.st, (int)blockIdx.y);
+    if (!s.part || !s.out) return;
+    const bool vec = pick4((int)blockIdx.y, r.whole[0], r.whole[1], r.whole[2], r.whole[3]);
+    const int64_t each = (int64_t)s.rows * s.cols;
+    T* out = reinterpret_cast<T*>(s.out);
     const T* res = reinterpret_cast<const T*>(s.res);
     const float alpha = store_scale(s);
-    const int64_t pieces = kVec ? each / 4 : each;
+    const int64_t pieces = vec ? each / 4 : each;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * 256) {
-        const int64_t at = kVec ? i * 4 : i;
+        const int64_t at = vec ? i * 4 : i;
         const int64_t m = at / s.cols, o = m * s.ldo + (at - m * s.cols);
-        if constexpr (kVec) {
+        if (vec) {
             f32x4 v{0.f, 0.f, 0.f, 0.f};
-            for (int k = 0; k < splits; ++k) v += *reinterpret_cast<const f32x4*>(part + k * stride + at);
+#pragma unroll 4
+            for (int k = 0; k < s.splits; ++k) v += *reinterpret_cast<const f32x4*>(s.part + k * each + at);
             v *= alpha;
             if (res)
                 for (int e = 0; e < 4; ++e) v[e] += (float)res[o + e];
             store4(out + o, v);
         } else {
             float v = 0.f;
-            for (int k = 0; k < splits; ++k) v += part[k * stride + at];
+            for (int k = 0; k < s.splits; ++k) v += s.part[k * each + at];
             out[o] = (T)(v * alpha + (res ? (float)res[o] : 0.f));
         }
     }
 }
 
-int gemm_reduce(int dtype, const GemmStore& st, int splits, int batch, hipStream_t stream) {
-    const bool vec = whole_pieces(dtype, st);
-    const int64_t pieces = (int64_t)st.rows * st.cols / (vec ? 4 : 1);
-    const dim3 grid((unsigned)std::min<int64_t>((pieces + 255) / 256, 8192), (unsigned)batch);
-    if (dtype == M3_DTYPE_BF16) {
-        if (vec) hipLaunchKernelGGL((gemm_reduce_kernel<bf16, true>), grid, dim3(256), 0, stream, st, splits);
-        else hipLaunchKernelGGL((gemm_reduce_kernel<bf16, false>), grid, dim3(256), 0, stream, st, splits);
-    } else {
-        if (vec) hipLaunchKernelGGL((gemm_reduce_kernel<float, true>), grid, dim3(256), 0, stream, st, splits);
-        else hipLaunchKernelGGL((gemm_reduce_kernel<float, false>), grid, dim3(256), 0, stream, st, splits);
+int gemm_reduce(int dtype, const GemmStore* st, int n, hipStream_t stream) {
+    GemmReduce r;
+    int64_t most = 0;
+    for (int p = 0; p < kGroupMax; ++p) {
+        r.st[p] = p < n ? st[p] : GemmStore{};
+        r.whole[p] = whole_pieces(dtype, r.st[p]);
+        if (r.st[p].part && r.st[p].out)
+            most = std::max(most, (int64_t)r.st[p].rows * r.st[p].cols / (r.whole[p] ? 4 : 1));
     }
+    if (most == 0) return M3_OK;
+    const dim3 grid((unsigned)std::min<int64_t>((most + 255) / 256, 8192), (unsigned)n);
+    if (dtype == M3_DTYPE_BF16) hipLaunchKernelGGL(gemm_reduce_kernel<bf16>, grid, dim3(256), 0, stream, r);
+    else hipLaunchKernelGGL(gemm_reduce_kernel<float>, grid, dim3(256), 0, stream, r);
     return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH;
 }
 
@@ -199,35 +277,126 @@ int gemm_pad_copy(int dtype, const GemmPads& pads, const int64_t* target, int64_
 }
 
 // Estimated us of each choice, from launches of 256, 512 and 1024 tiles of 8 and 64 k steps (torch on the
-// same card: 8192^3 bf16 668 us): a step of a 256 x 256 tile takes 1.45 us, of a 128 x 128 tile 0.62 us
-// alone on its CU and 0.90 us next to another, of a 64 x 64 tile 0.20 and 0.37 us; to that come a
-// tile's start and epilogue. Parts of k cost the fp32 partial sums' write and read and a launch.
+// same card: 8192^3 bf16 668 us): a step of a 256 x 256 tile takes 1.45 us (1.38 where both operands
+// are rows of m and n), of a 128 x 128 tile 0.62 us alone on its CU and 0.90 us (1.05) next to another, of a
+// 64 x 64 tile 0.20 and 0.37 us; to that come a tile's start and epilogue. Parts of k cost the
+// fp32 partial sums' write and read and a launch.
 // What it decides, both sides measured: the gated product of 8192 x 11008 x 2048 takes 80 us less on 256 x 256
 // tiles than on 128 x 128, that of 8192 x 4224 x 768 8 us more; the 8192 x 768 product over 16128 takes
-// 70 us less in two parts on 256 x 256 tiles than in two on 128 x 128.
-GemmPlan gemm_plan(int dtype, int64_t rows, int64_t cols, int64_t steps, int batch, int max_splits) {
-    struct Cost { int size, at_once; double alone, all, fixed; };
-    static const Cost bf[3] = {{256, 1, 1.45, 1.45, 8.0}, {128, 2, 0.62, 0.90, 4.5}, {64, 2, 0.20, 0.37, 3.5}};
-    static const Cost fp[3] = {{0, 0, 0, 0, 0}, {128, 2, 1.90, 3.60, 5.0}, {64, 2, 0.65, 1.07, 4.0}};
-    const Cost* c = dtype == M3_DTYPE_BF16 ? bf : fp;
-    GemmPlan best{kTileS, 1, 64, 64};
+// 33 us less in two parts on 256 x 256 tiles than whole on 128 x 128.
+namespace {
+struct TileCost { int size, at_once; double alone, all, tn, fixed; };
+const TileCost kCostBf16[3] = {{256, 1, 1.45, 1.45, 1.38, 8.0}, {128, 2, 0.62, 0.90, 1.05, 4.5}, {64, 2, 0.20, 0.37, 0.38, 3.5}};
+const TileCost kCostF32[3] = {{0, 0, 0, 0, 0, 0}, {128, 2, 1.90, 3.60, 3.60, 5.0}, {64, 2, 0.65, 1.07, 1.07, 4.0}};
+
+int64_t group_items(const TileCost& c, const GemmTask& t, int splits) {
+    return ((t.rows + c.size - 1) / c.size) * ((t.cols + c.size - 1) / c.size) * splits;
+}
+
+// Rounds of as many items as run at once, each as long as its longest item.
+double group_us(const TileCost& c, const GemmTask* t, const int* splits, int n) {
+    const int64_t slots = (int64_t)256 * c.at_once;
+    double us = 0, longest = 0, alone = 0;  // of the current round's items, and with a CU to themselves
+    int64_t room = slots;                   // left in the current round
+    bool joined = false;
+    for (int p = 0; p < n; ++p) {
+        int64_t items = group_items(c, t[p], splits[p]);
+        if (items == 0) continue;
+        const double steps = (double)((t[p].steps + splits[p] - 1) / splits[p]);
+        const double one = steps * (t[p].tn ? c.tn : c.all) + c.fixed, own = std::min(one, steps * c.alone + c.fixed);
+        if (splits[p] > 1) {
+            us += (double)t[p].rows * t[p].cols * 8.0 * splits[p] / 5.0e6;
+            joined = true;
+        }
+        const int64_t in = std::min(items, room);
+        longest = std::max(longest, one), alone = std::max(alone, own);
+        room -= in, items -= in;
+        if (room == 0) us += longest, longest = alone = 0, room = slots;
+        us += items / slots * one;
+        items %= slots;
+        if (items) longest = one, alone = own, room = slots - items;
+    }
+    // the last round may leave each item a CU to itself
+    return us + (slots - room <= 256 ? alone : longest) + (joined ? 4.0 : 0.0);
+}
+}  // namespace
+
+static GemmGroupPlan search_plan(int dtype, const GemmTask* tasks, int n) {
+    const TileCost* c = dtype == M3_DTYPE_BF16 ? kCostBf16 : kCostF32;
+    static const int kTry[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16};
+    GemmGroupPlan best{kTileS, {1, 1, 1, 1}};
     double least = 1e30;
     for (int t = dtype == M3_DTYPE_BF16 ? kTileL : kTileM; t <= kTileS; ++t) {
-        const int64_t tiles = ((rows + c[t].size - 1) / c[t].size) * ((cols + c[t].size - 1) / c[t].size) * batch;
-        for (int s = 1; s <= max_splits && s <= steps; ++s) {
-            const int64_t items = tiles * s, slots = (int64_t)256 * c[t].at_once;
-            const double per = (double)((steps + s - 1) / s);
-            const int64_t rest = items % slots;
-            double us = items / slots * (per * c[t].all + c[t].fixed);
-            if (rest) us += per * (rest > 256 ? c[t].all : c[t].alone) + c[t].fixed;
-            if (s > 1) us += 4.0 + (double)rows * cols * batch * 8.0 * s / 5.0e6;
-            if (us < least) {
-                least = us;
-                best = GemmPlan{t, s, c[t].size, c[t].size};
+        int s[kGroupMax] = {1, 1, 1, 1};
+        double us = group_us(c[t], tasks, s, n);
+        // all dy^T x alike first, then one product after the other; a launch of many rounds gains nothing
+        // from parts
+        int64_t items = 0;
+        for (int p = 0; p < n; ++p) items += group_items(c[t], tasks[p], 1);
+        if (items <= (int64_t)256 * c[t].at_once * 6) {
+            auto fits = [&](int p, int k) { return k <= tasks[p].max_splits && k <= tasks[p].steps; };
+            int alike = 1;
+            for (int k : kTry) {
+                int v[kGroupMax] = {1, 1, 1, 1};
+                for (int p = 0; p < n; ++p)
+                    if (tasks[p].tn && fits(p, k)) v[p] = k;
+                const double u = group_us(c[t], tasks, v, n);
+                if (u < us) us = u, alike = k;
             }
+            for (int p = 0; p < n; ++p)
+                if (tasks[p].tn && fits(p, alike)) s[p] = alike;
+            for (int pass = 0; pass < 2; ++pass)
+                for (int p = 0; p < n; ++p) {
+                    int keep = s[p];
+                    for (int k : kTry) {
+                        if (!fits(p, k)) break;
+                        s[p] = k;
+                        const double u = group_us(c[t], tasks, s, n);
+                        if (u < us) us = u, keep = k;
+                    }
+                    s[p] = keep;
+                }
+        }
+        if (us < least) {
+            least = us;
+            best.tile = t;
+            for (int p = 0; p < kGroupMax; ++p) best.splits[p] = s[p];
         }
     }
     return best;
+}
+
+// The search takes 20 us of host time, and a call asks three times (the workspace's size, its check, the
+// launch): each thread keeps its last plans.
+GemmGroupPlan gemm_group_plan(int dtype, const GemmTask* tasks, int n) {
+    struct Kept {
+        int dtype = -1, n = 0;
+        GemmTask t[kGroupMax];
+        GemmGroupPlan plan;
+    };
+    static thread_local Kept kept[64];
+    uint64_t h = (uint64_t)dtype * 31 + (uint64_t)n;
+    for (int p = 0; p < n; ++p)
+        h = (h * 0x9e3779b97f4a7c15ull + (uint64_t)tasks[p].rows * 3 + (uint64_t)tasks[p].cols * 5 + (uint64_t)tasks[p].steps * 7) ^ (h >> 29);
+    Kept& k = kept[h >> 58];
+    auto same = [](const GemmTask& a, const GemmTask& b) {
+        return a.rows == b.rows && a.cols == b.cols && a.steps == b.steps && a.max_splits == b.max_splits && a.tn == b.tn;
+    };
+    bool hit = k.dtype == dtype && k.n == n;
+    for (int p = 0; hit && p < n; ++p) hit = same(k.t[p], tasks[p]);
+    if (!hit) {
+        k.plan = search_plan(dtype, tasks, n);
+        k.dtype = dtype, k.n = n;
+        for (int p = 0; p < n; ++p) k.t[p] = tasks[p];
+    }
+    return k.plan;
+}
+
+GemmPlan gemm_plan(int dtype, int64_t rows, int64_t cols, int64_t steps, int max_splits) {
+    const GemmTask t{rows, cols, steps, max_splits, false};
+    const GemmGroupPlan g = gemm_group_plan(dtype, &t, 1);
+    const int size = g.tile == kTileL ? 256 : g.tile == kTileM ? 128 : 64;
+    return GemmPlan{g.tile, g.splits[0], size, size};
 }
 
 }  // namespace m3

@@ -98,7 +98,7 @@ struct EpiGated {
     int rows, ldh;
 
     template <typename T, typename Tile, int kMode>
-    __device__ __forceinline__ void run(const GemmArgs&, const GemmPlace<Tile, kMode>& at,
+    __device__ __forceinline__ void run(const GemmPlace<Tile, kMode>& at,
                                         typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, const GemmItem&) const {
         const GemmRows<T, Tile, Tile::FN / 2 * Tile::MF> out(smem, at.wave(), at.lane);
 #pragma unroll
@@ -127,7 +127,7 @@ struct EpiGateBwd {
     int rows, ldh;
 
     template <typename T, typename Tile, int kMode>
-    __device__ __forceinline__ void run(const GemmArgs&, const GemmPlace<Tile, kMode>& at,
+    __device__ __forceinline__ void run(const GemmPlace<Tile, kMode>& at,
                                         typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, const GemmItem&) const {
         constexpr int J = Tile::FN * Tile::Q;
         const GemmRows<T, Tile, Tile::FN * Tile::MF> out(smem, at.wave(), at.lane);
@@ -172,8 +172,6 @@ struct EpiGateBwd {
 
 namespace {
 
-constexpr int kMaxSplits = 16;
-
 struct MlpShape {
     int64_t rows, d, ff, dp, fp;
     int dtype;
@@ -206,31 +204,37 @@ struct MlpFwd {
 MlpFwd mlp_fwd_layout(const MlpShape& s, bool keeps_h, void* ws) {
     MlpFwd f;
     Bump b{reinterpret_cast<char*>(ws)};
-    f.up = gemm_plan(s.dtype, s.rows, 2 * s.ff, gemm_steps(s.d, s.dtype), 1, 1);
-    f.down = gemm_plan(s.dtype, s.rows, s.d, gemm_steps(s.ff, s.dtype), 1, kMaxSplits);
+    f.up = gemm_plan(s.dtype, s.rows, 2 * s.ff, gemm_steps(s.d, s.dtype), 1);
+    f.down = gemm_plan(s.dtype, s.rows, s.d, gemm_steps(s.ff, s.dtype), kMaxSplits);
     f.x = s.pad_d ? b.take(s.rows * s.dp * s.size) : nullptr;
     f.wg = s.pad_d ? b.take(s.ff * s.dp * s.size) : nullptr;
     f.wu = s.pad_d ? b.take(s.ff * s.dp * s.size) : nullptr;
     f.wd = s.pad_f ? b.take(s.d * s.fp * s.size) : nullptr;
     f.h = keeps_h ? nullptr : b.take(s.rows * s.fp * s.size);
-    f.part = reinterpret_cast<float*>(b.take((int64_t)gemm_part_bytes(f.down, 1, s.rows, s.d)));
+    f.part = reinterpret_cast<float*>(b.take((int64_t)gemm_part_bytes(f.down.splits, s.rows, s.d)));
     f.bytes = b.used;
     return f;
 }
 
+// What the backward computes, in the order of the grouped launch.
+enum { kDx, kDwGate, kDwUp, kDwDown };
 struct MlpBwd {
-    GemmPlan dh, dx, dw, dwd;
+    GemmPlan dh;
+    GemmGroupPlan grads;
     void *x, *dy, *wg, *wu, *wd, *dg, *du;
-    float* part;
+    float* part[kGroupMax];
     size_t bytes;
 };
 MlpBwd mlp_bwd_layout(const MlpShape& s, void* ws) {
     MlpBwd f;
     Bump b{reinterpret_cast<char*>(ws)};
-    f.dh = gemm_plan(s.dtype, s.rows, s.ff, gemm_steps(s.d, s.dtype), 1, 1);
-    f.dx = gemm_plan(s.dtype, s.rows, s.d, 2 * gemm_steps(s.fp, s.dtype), 1, kMaxSplits);
-    f.dw = gemm_plan(s.dtype, s.ff, s.d, gemm_steps(s.rows, s.dtype), 2, kMaxSplits);
-    f.dwd = gemm_plan(s.dtype, s.d, s.ff, gemm_steps(s.rows, s.dtype), 1, kMaxSplits);
+    f.dh = gemm_plan(s.dtype, s.rows, s.ff, gemm_steps(s.d, s.dtype), 1);
+    const int64_t over_rows = gemm_steps(s.rows, s.dtype);
+    const GemmTask tasks[kGroupMax] = {{s.rows, s.d, 2 * gemm_steps(s.fp, s.dtype), kMaxSplits, false},
+                                       {s.ff, s.d, over_rows, kMaxSplits, true},
+                                       {s.ff, s.d, over_rows, kMaxSplits, true},
+                                       {s.d, s.ff, over_rows, kMaxSplits, true}};
+    f.grads = gemm_group_plan(s.dtype, tasks, kGroupMax);
     f.x = s.pad_d ? b.take(s.rows * s.dp * s.size) : nullptr;
     f.dy = s.pad_d ? b.take(s.rows * s.dp * s.size) : nullptr;
     f.wg = s.pad_d ? b.take(s.ff * s.dp * s.size) : nullptr;
@@ -238,9 +242,8 @@ MlpBwd mlp_bwd_layout(const MlpShape& s, void* ws) {
     f.wd = s.pad_f ? b.take(s.d * s.fp * s.size) : nullptr;
     f.dg = b.take(s.rows * s.fp * s.size);
     f.du = b.take(s.rows * s.fp * s.size);
-    const size_t part = std::max(std::max(gemm_part_bytes(f.dx, 1, s.rows, s.d), gemm_part_bytes(f.dw, 2, s.ff, s.d)),
-                                 gemm_part_bytes(f.dwd, 1, s.d, s.ff));
-    f.part = reinterpret_cast<float*>(b.take((int64_t)part));
+    for (int p = 0; p < kGroupMax; ++p)
+        f.part[p] = reinterpret_cast<float*>(b.take((int64_t)gemm_part_bytes(f.grads.splits[p], tasks[p].rows, tasks[p].cols)));
     f.bytes = b.used;
     return f;
 }
@@ -292,9 +295,9 @@ int launch_swiglu_fwd(int64_t rows, int64_t d, int64_t ff, int dtype, const void
     void* h = saved ? reinterpret_cast<char*>(saved) + gu_bytes(s) : f.h;
     GemmArgs a = gemm_args({x, s.dp}, {wg, s.dp}, rows, ff, s.dp, 1);
     a.b[1] = {wu, s.dp};
-    M3_TRY((gemm_dispatch<true, true, kGated>(dtype, f.up, a, EpiGated{h, kept_gu(s, saved), (int)rows, (int)s.fp}, rows, 2 * s.fp, 1, stream)));
-    const GemmStore st{{y, nullptr}, d, res, scale, f.part, 0, (int)rows, (int)d};
-    return gemm_store(kFormNT, dtype, f.down, gemm_args({h, s.fp}, {wd, s.fp}, rows, d, s.fp, 1), st, 1, stream);
+    M3_TRY((gemm_dispatch<true, true, kGated>(dtype, f.up, a, EpiGated{h, kept_gu(s, saved), (int)rows, (int)s.fp}, rows, 2 * s.fp, stream)));
+    const GemmStore st{y, d, res, scale, f.part, 0, (int)rows, (int)d};
+    return gemm_store(dtype, f.down, gemm_args({h, s.fp}, {wd, s.fp}, rows, d, s.fp, 1), st, stream);
 }
 
 int launch_swiglu_bwd(int64_t rows, int64_t d, int64_t ff, int dtype, const void* x, const void* wg, const void* wu,
@@ -317,27 +320,30 @@ int launch_swiglu_bwd(int64_t rows, int64_t d, int64_t ff, int dtype, const void
         // rows of Wd past d do not exist: A's pad columns meet zeros
         GemmArgs a = gemm_args({dy, s.dp}, {wd, s.fp}, rows, s.fp, s.dp, 1);
         a.KB[0] = (int)d;
-        M3_TRY((gemm_dispatch<true, false, kPlain>(dtype, f.dh, a, EpiGateBwd{f.dg, f.du, kept_gu(s, saved), scale, (int)rows, (int)s.fp}, rows, s.fp, 1, stream)));
+        M3_TRY((gemm_dispatch<true, false, kPlain>(dtype, f.dh, a, EpiGateBwd{f.dg, f.du, kept_gu(s, saved), scale, (int)rows, (int)s.fp}, rows, s.fp, stream)));
     }
+    // a gradient that is not wanted has no rows, and no items
+    GemmGrads g;
     if (dx) {
-        GemmArgs a = gemm_args({f.dg, s.fp}, {wg, s.dp}, rows, s.dp, s.fp, 1);
-        a.a[1] = {f.du, s.fp}, a.b[1] = {wu, s.dp};
-        a.K[1] = (int)s.fp;
-        a.KB[0] = a.KB[1] = (int)ff;
-        const GemmStore st{{dx, nullptr}, d, nullptr, 1.f, f.part, 0, (int)rows, (int)d};
-        M3_TRY(gemm_store(kFormNN, dtype, f.dx, a, st, 1, stream));
+        g.a[kDx] = gemm_args({f.dg, s.fp}, {wg, s.dp}, rows, s.dp, s.fp, 1);
+        g.a[kDx].a[1] = {f.du, s.fp}, g.a[kDx].b[1] = {wu, s.dp};
+        g.a[kDx].K[1] = (int)s.fp;
+        g.a[kDx].KB[0] = g.a[kDx].KB[1] = (int)ff;
+        g.st[kDx] = GemmStore{dx, d, nullptr, 1.f, f.part[kDx], 0, (int)rows, (int)d};
     }
-    if (dwg || dwu) {
-        GemmArgs a = gemm_args({dwg ? f.dg : f.du, s.fp}, {x, s.dp}, s.fp, s.dp, rows, 1);
-        if (dwg && dwu) a.a[1] = {f.du, s.fp};
-        const GemmStore st{{dwg ? dwg : dwu, dwg ? dwu : nullptr}, d, nullptr, 1.f, f.part, 0, (int)ff, (int)d};
-        M3_TRY(gemm_store(kFormTN, dtype, f.dw, a, st, dwg && dwu ? 2 : 1, stream));
+    if (dwg) {
+        g.a[kDwGate] = gemm_args({f.dg, s.fp}, {x, s.dp}, s.fp, s.dp, rows, 1);
+        g.st[kDwGate] = GemmStore{dwg, d, nullptr, 1.f, f.part[kDwGate], 0, (int)ff, (int)d};
+    }
+    if (dwu) {
+        g.a[kDwUp] = gemm_args({f.du, s.fp}, {x, s.dp}, s.fp, s.dp, rows, 1);
+        g.st[kDwUp] = GemmStore{dwu, d, nullptr, 1.f, f.part[kDwUp], 0, (int)ff, (int)d};
     }
     if (dwd) {
-        const GemmStore st{{dwd, nullptr}, ff, nullptr, scale, f.part, 0, (int)d, (int)ff};
-        M3_TRY(gemm_store(kFormTN, dtype, f.dwd, gemm_args({dy, s.dp}, {h, s.fp}, s.dp, s.fp, rows, 1), st, 1, stream));
+        g.a[kDwDown] = gemm_args({dy, s.dp}, {h, s.fp}, s.dp, s.fp, rows, 1);
+        g.st[kDwDown] = GemmStore{dwd, ff, nullptr, scale, f.part[kDwDown], 0, (int)d, (int)ff};
     }
-    return M3_OK;
+    return gates || dwd ? gemm_grads(dtype, f.grads, g, stream) : M3_OK;
 }
 
 }  // namespace m3

@@ -19,7 +19,6 @@
 
 namespace m3 {
 
-constexpr int kXentSplits = 16;
 constexpr int64_t kXentPieceBytes = (int64_t)256 << 20;
 constexpr int64_t kXentPieceMost = (int64_t)1 << 20;  // columns: a tile's rows stay within 32-bit offsets
 
@@ -42,7 +41,7 @@ struct EpiXentFwd {
     int rows, vocab;
 
     template <typename T, typename Tile, int kMode>
-    __device__ __forceinline__ void run(const GemmArgs&, const GemmPlace<Tile, kMode>& at,
+    __device__ __forceinline__ void run(const GemmPlace<Tile, kMode>& at,
                                         typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, const GemmItem& it) const {
         float2* red = reinterpret_cast<float2*>(smem);  // [WGN][BM]
         if (at.n0 + Tile::BN <= vocab) rows_of<T, Tile, kMode, true>(at, acc, red);
@@ -127,7 +126,7 @@ struct EpiXentBwd {
     int v0, have, vocab, rows;  // first column of the piece, its columns that exist
 
     template <typename T, typename Tile, int kMode>
-    __device__ __forceinline__ void run(const GemmArgs&, const GemmPlace<Tile, kMode>& at,
+    __device__ __forceinline__ void run(const GemmPlace<Tile, kMode>& at,
                                         typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, const GemmItem&) const {
         constexpr int J = Tile::FN * Tile::Q;
         const GemmRows<T, Tile, Tile::FN * Tile::MF> out(smem, at.wave(), at.lane);
@@ -275,7 +274,7 @@ XentFwd xent_fwd_layout(int64_t rows, int64_t d, int64_t vocab, int dtype, void*
     XentFwd f;
     Bump b{reinterpret_cast<char*>(ws)};
     const int64_t dp = gemm_pad(d, dtype), size = dtype == M3_DTYPE_BF16 ? 2 : 4;
-    f.z = gemm_plan(dtype, rows, vocab, gemm_steps(d, dtype), 1, 1);
+    f.z = gemm_plan(dtype, rows, vocab, gemm_steps(d, dtype), 1);
     f.tiles = (int)((vocab + f.z.bn - 1) / f.z.bn);
     f.h = dp != d ? b.take(rows * dp * size) : nullptr;
     f.w = dp != d ? b.take(vocab * dp * size) : nullptr;
@@ -288,7 +287,8 @@ XentFwd xent_fwd_layout(int64_t rows, int64_t d, int64_t vocab, int dtype, void*
 
 struct XentBwd {
     int64_t piece;  // columns of a piece (its row stride)
-    GemmPlan z, dh, dw;
+    GemmPlan z;
+    GemmGroupPlan grads;  // dh, dW
     void *h, *w, *dz;
     float* part;      // dh's sums
     float* part_dw;
@@ -302,14 +302,16 @@ XentBwd xent_bwd_layout(int64_t rows, int64_t d, int64_t vocab, int dtype, bool 
     const int64_t most = std::min<int64_t>(std::max<int64_t>(kXentPieceBytes / (rows * size) / 256 * 256, 256), kXentPieceMost);
     const int64_t pieces = (vocab + most - 1) / most;
     f.piece = pieces == 1 ? gemm_pad(vocab, dtype) : ((vocab + pieces - 1) / pieces + 255) / 256 * 256;
-    f.z = gemm_plan(dtype, rows, f.piece, gemm_steps(d, dtype), 1, 1);
-    f.dh = gemm_plan(dtype, rows, d, gemm_steps(f.piece, dtype), 1, kXentSplits);
-    f.dw = gemm_plan(dtype, f.piece, d, gemm_steps(rows, dtype), 1, kXentSplits);
+    f.z = gemm_plan(dtype, rows, f.piece, gemm_steps(d, dtype), 1);
+    const GemmTask tasks[2] = {{want_dh ? rows : 0, d, gemm_steps(f.piece, dtype), kMaxSplits, false},
+                               {want_dw ? f.piece : 0, d, gemm_steps(rows, dtype), kMaxSplits, true}};
+    f.grads = gemm_group_plan(dtype, tasks, 2);
+    const int dh_splits = f.grads.splits[0];
     f.h = b.take(rows * dp * size);
     f.w = dp != d ? b.take(vocab * dp * size) : nullptr;
     f.dz = b.take(rows * f.piece * size);
-    f.part = want_dh && (pieces > 1 || f.dh.splits > 1) ? reinterpret_cast<float*>(b.take((int64_t)f.dh.splits * rows * d * 4)) : nullptr;
-    f.part_dw = want_dw ? reinterpret_cast<float*>(b.take((int64_t)gemm_part_bytes(f.dw, 1, f.piece, d))) : nullptr;
+    f.part = want_dh && (pieces > 1 || dh_splits > 1) ? reinterpret_cast<float*>(b.take((int64_t)dh_splits * rows * d * 4)) : nullptr;
+    f.part_dw = want_dw ? reinterpret_cast<float*>(b.take((int64_t)gemm_part_bytes(f.grads.splits[1], f.piece, d))) : nullptr;
     f.bytes = b.used;
     return f;
 }
@@ -342,7 +344,7 @@ int launch_xent_fwd(int64_t rows, int64_t d, int64_t vocab, int dtype, int reduc
         hidden = f.h, weight = f.w;
     }
     M3_TRY((gemm_dispatch<true, true, kPlain>(dtype, f.z, gemm_args({hidden, dp}, {weight, dp}, rows, vocab, dp, 1),
-                                              EpiXentFwd{f.part, f.zt, target, (int)rows, (int)vocab}, rows, vocab, 1, stream)));
+                                              EpiXentFwd{f.part, f.zt, target, (int)rows, (int)vocab}, rows, vocab, stream)));
     const bool none = reduction == M3_REDUCTION_NONE;
     const int blocks = (int)((rows + kXentRows - 1) / kXentRows);
     hipLaunchKernelGGL(xent_rows_kernel, dim3(blocks), dim3(256), 0, stream, f.part, f.zt, target, ignore, f.tiles,
@@ -366,7 +368,9 @@ int launch_xent_bwd(int64_t rows, int64_t d, int64_t vocab, int dtype, int reduc
     }
     const int r = (int)rows;
     const bool none = reduction == M3_REDUCTION_NONE;
-    GemmStore dh{{nullptr, nullptr}, d, nullptr, 1.f, f.part, 0, r, (int)d};
+    GemmGrads g;
+    GemmStore& dh = g.st[0];
+    if (dhidden) dh = GemmStore{nullptr, d, nullptr, 1.f, f.part, 0, r, (int)d};
     if (!none) dh.num = grad_loss;
     if (reduction == M3_REDUCTION_MEAN) dh.den = count;
     for (int64_t v0 = 0; v0 < vocab; v0 += f.piece) {
@@ -376,24 +380,24 @@ int launch_xent_bwd(int64_t rows, int64_t d, int64_t vocab, int dtype, int reduc
         M3_TRY((gemm_dispatch<true, true, kPlain>(
             dtype, f.z, gemm_args({f.h, dp}, {w, dp}, rows, have, dp, 1),
             EpiXentBwd{f.dz, (int)f.piece, lse, none ? grad_loss : nullptr, target, ignore, (int)v0, (int)have, (int)vocab, r},
-            rows, f.piece, 1, stream)));
+            rows, f.piece, stream)));
         if (dhidden) {
-            GemmArgs a = gemm_args({f.dz, f.piece}, {w, dp}, rows, dp, f.piece, 1);
-            a.KB[0] = (int)have;
-            if (f.piece >= vocab) dh.out[0] = dhidden;  // one piece: no sum over calls
-            M3_TRY(gemm_store(kFormNN, dtype, f.dh, a, dh, 1, stream));
-            dh.add = 1;
+            g.a[0] = gemm_args({f.dz, f.piece}, {w, dp}, rows, dp, f.piece, 1);
+            g.a[0].KB[0] = (int)have;
+            if (f.piece >= vocab) dh.out = dhidden;  // one piece: no sum over calls
         }
         if (dweight) {
-            void* out = reinterpret_cast<char*>(dweight) + v0 * d * size;
-            GemmStore dw{{out, nullptr}, d, nullptr, 1.f, f.part_dw, 0, (int)have, (int)d};
-            dw.num = dh.num, dw.den = dh.den;
-            M3_TRY(gemm_store(kFormTN, dtype, f.dw, gemm_args({f.dz, f.piece}, {f.h, dp}, f.piece, dp, rows, 1), dw, 1, stream));
+            g.a[1] = gemm_args({f.dz, f.piece}, {f.h, dp}, f.piece, dp, rows, 1);
+            g.st[1] = GemmStore{reinterpret_cast<char*>(dweight) + v0 * d * size, d, nullptr, 1.f, f.part_dw, 0, (int)have, (int)d};
+            g.st[1].num = dh.num, g.st[1].den = dh.den;
         }
+        M3_TRY(gemm_grads(dtype, f.grads, g, stream));
+        dh.add = 1;
     }
     if (dhidden && f.piece < vocab) {
-        dh.out[0] = dhidden;
-        M3_TRY(gemm_reduce(dtype, dh, f.dh.splits, 1, stream));
+        dh.out = dhidden;
+        dh.splits = f.grads.splits[0];
+        M3_TRY(gemm_reduce(dtype, &dh, 1, stream));
     }
     return M3_OK;
 }
