@@ -434,7 +434,7 @@ enum m3_reduction {
  * be NULL. Logits and sums are fp32; for bf16 the gradient of the logits is rounded to bf16
  * before its two products. Sums run in a fixed order. The backward's workspace holds the gradient
  * of the logits for one piece of the vocabulary (up to 256 MB where 256 columns fit that).
- * rows <= 2^30, d_model <= 2^20, vocab <= 2^30. workspace: 256-byte aligned.
+ * rows <= 2^27, d_model <= 2^20, vocab <= 2^30. workspace: 256-byte aligned.
  */
 int m3_linear_xent_fwd_workspace_size(int64_t rows, int32_t d_model, int32_t vocab, int32_t dtype,
                                       size_t* bytes);

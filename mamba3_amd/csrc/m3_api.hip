@@ -593,7 +593,8 @@ static int check_swiglu(int64_t rows, int32_t d_model, int32_t d_ff, int32_t dty
     return check_product(rows, d_model, d_ff, 1 << 20, dtype);
 }
 static int check_xent(int64_t rows, int32_t d_model, int32_t vocab, int32_t dtype) {
-    return check_product(rows, d_model, vocab, (int64_t)1 << 30, dtype);
+    const int st = check_product(rows, d_model, vocab, (int64_t)1 << 30, dtype);
+    return st == M3_OK && rows > ((int64_t)1 << 27) ? M3_ERR_UNSUPPORTED : st;  // 16 rows a block, 32-bit grid
 }
 static int check_workspace(const void* ws, size_t have, size_t need) {
     if (need == 0) return M3_OK;

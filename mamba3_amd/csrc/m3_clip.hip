@@ -143,10 +143,12 @@ static int64_t clip_blocks(int64_t numel, int dtype) {
 }
 
 // Calls `f(tensors, dtype)` for groups of up to kClipTensors non-empty tensors of one type.
+// `back`: from the last tensor to the first.
 template <typename F>
-static int clip_groups(int n, void* const* p, const int64_t* numel, const int32_t* dtype, F f) {
+static int clip_groups(int n, void* const* p, const int64_t* numel, const int32_t* dtype, bool back, F f) {
     int block0 = 0;
-    for (int type : {M3_DTYPE_F32, M3_DTYPE_BF16}) {
+    const int types[2] = {back ? M3_DTYPE_BF16 : M3_DTYPE_F32, back ? M3_DTYPE_F32 : M3_DTYPE_BF16};
+    for (int type : types) {
         ClipTensors t;
         t.count = 0;
         t.block0 = block0;
@@ -159,7 +161,8 @@ static int clip_groups(int n, void* const* p, const int64_t* numel, const int32_
             t.count = 0, t.block0 = block0, blocks = 0;
             return st;
         };
-        for (int i = 0; i < n; ++i) {
+        for (int j = 0; j < n; ++j) {
+            const int i = back ? n - 1 - j : j;
             if (dtype[i] != type || numel[i] == 0) continue;
             if (t.count == kClipTensors || blocks + clip_blocks(numel[i], type) > (1 << 23)) {
                 const int st = flush();
@@ -189,7 +192,7 @@ int launch_clip(int n, void* const* p, const int64_t* numel, const int32_t* dtyp
                 float max_norm, float* norm, void* ws, hipStream_t stream) {
     float* factor = reinterpret_cast<float*>(ws);
     double* part = reinterpret_cast<double*>(reinterpret_cast<char*>(ws) + 256);
-    int st = clip_groups(n, p, numel, dtype, [&](const ClipTensors& t, int type, int blocks) {
+    int st = clip_groups(n, p, numel, dtype, false, [&](const ClipTensors& t, int type, int blocks) {
         const dim3 grid((unsigned)blocks), block(kClipThreads);
         if (type == M3_DTYPE_BF16) {
             if (inf_norm) hipLaunchKernelGGL((clip_norm_kernel<bf16, true>), grid, block, 0, stream, t, part);
@@ -205,7 +208,8 @@ int launch_clip(int n, void* const* p, const int64_t* numel, const int32_t* dtyp
     if (inf_norm) hipLaunchKernelGGL((clip_total_kernel<true>), dim3(1), dim3(kClipThreads), 0, stream, part, blocks, max_norm, norm, scale ? factor : nullptr);
     else hipLaunchKernelGGL((clip_total_kernel<false>), dim3(1), dim3(kClipThreads), 0, stream, part, blocks, max_norm, norm, scale ? factor : nullptr);
     if ((st = clip_status()) != M3_OK || !scale) return st;
-    return clip_groups(n, p, numel, dtype, [&](const ClipTensors& t, int type, int blocks) {
+    // what the norm read last is still in the last-level cache
+    return clip_groups(n, p, numel, dtype, true, [&](const ClipTensors& t, int type, int blocks) {
         const dim3 grid((unsigned)blocks), block(kClipThreads);
         if (type == M3_DTYPE_BF16) hipLaunchKernelGGL((clip_scale_kernel<bf16>), grid, block, 0, stream, t, factor);
         else hipLaunchKernelGGL((clip_scale_kernel<float>), grid, block, 0, stream, t, factor);

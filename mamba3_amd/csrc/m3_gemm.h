@@ -235,9 +235,9 @@ struct GemmTile {
     static constexpr int FM = BM / WGM / MF, FN = BN / WGN / MF;  // MF x MF pieces of a wave
     static constexpr int Q = MF * MF / 256;                       // fours of columns a lane holds of a piece
     static constexpr int kStageBytes = (BM + BN) * 128;
-    // behind the stages: the epilogue's rows, in fp32 where the tile serves fp32 products
+    // behind the stages: an epilogue's bf16 rows, or a pair of floats for each row and column of waves
     static constexpr int kStages = STAGES * kStageBytes;
-    static constexpr int kEpi = NW * MF * (FN * MF * (MF == 32 || BN == 64 ? 4 : 2) + 16);
+    static constexpr int kEpi = MF == 32 ? WGN * BM * 8 : NW * MF * (FN * MF * 2 + 16);
     static constexpr int kLds = kStages + kEpi;
     typedef typename GemmType<bf16, MF>::Acc Acc;
 };
@@ -267,39 +267,53 @@ __device__ __forceinline__ f32x4 four(const Acc& v, int q) {
     return f32x4{v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]};
 }
 
-// Stores MF rows of a wave's results as whole rows: fours go into a wave-private part of LDS and leave it
-// as 16 bytes a lane, kCols columns of a row side by side (64 to 256 bytes), where storing them as
-// the MFMA leaves them would write 8 bytes to each of 16 rows. LDS operations of one wave run in
-// order, so no barrier is needed.
+// Stores MF rows of a wave's results. bf16: as whole rows, fours go into a wave-private part of LDS and
+// leave it as 16 bytes a lane, kCols columns of a row side by side (64 or 128 bytes), where storing
+// them as the MFMA leaves them would write 8 bytes to each of 16 rows; LDS operations of one wave run
+// in order, so no barrier is needed. fp32: 16 bytes a lane at once (the LDS would cost the second block on
+// a CU).
 template <typename T, typename Tile, int kCols>
 struct GemmRows {
     static constexpr int MF = Tile::MF, E = 16 / sizeof(T);
     static constexpr int kPitch = kCols * (int)sizeof(T) + 16;
     static constexpr int LPR = kCols / E, RPI = 64 / LPR;  // lanes a row, rows an instruction
-    static_assert(Tile::NW * MF * kPitch <= Tile::kEpi, "rows fit LDS");
+    static_assert(sizeof(T) == 4 || Tile::NW * MF * kPitch <= Tile::kEpi, "rows fit LDS");
     typedef T T4 __attribute__((ext_vector_type(4)));
     typedef T Piece __attribute__((ext_vector_type(E)));
     char* mine;
     int lane;
+    T* out;
+    int64_t ld;
+    int rows, cols;
     __device__ __forceinline__ GemmRows(char* smem, int wave, int lane_) : mine(smem + wave * (MF * kPitch)), lane(lane_) {}
+    // the next MF rows go to out_ + r * ld_ for r < rows_; columns come in whole 16-byte pieces, cols_ of them exist
+    __device__ __forceinline__ void begin(T* out_, int64_t ld_, int rows_, int cols_) {
+        out = out_, ld = ld_, rows = rows_, cols = cols_;
+    }
     // columns fn * MF + q * 8 + ... of row lane % MF
     __device__ __forceinline__ void put(int fn, int q, f32x4 v) const {
+        const int r = lane % MF, c = fn * MF + q * 8 + lane / MF * 4;
         T4 o;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = (T)v[e];
-        *reinterpret_cast<T4*>(mine + lane % MF * kPitch + (fn * MF + q * 8 + lane / MF * 4) * (int)sizeof(T)) = o;
-    }
-    // row r of the MF to out + r * ld for r < rows; columns come in whole pieces, cols of them exist
-    __device__ __forceinline__ void store(T* out, int64_t ld, int rows, int cols) const {
-        const int r0 = lane / LPR, c = lane % LPR * E;
-        M3_LDS_FENCE();  // the fours and the pieces are other types to the compiler
-#pragma unroll
-        for (int i = 0; i < (MF + RPI - 1) / RPI; ++i) {
-            const int r = i * RPI + r0;
-            if (r < MF && r < rows && c < cols)
-                *reinterpret_cast<Piece*>(out + r * ld + c) = *reinterpret_cast<const Piece*>(mine + r * kPitch + c * (int)sizeof(T));
+        if constexpr (sizeof(T) == 4) {
+            if (r < rows && c < cols) *reinterpret_cast<T4*>(out + r * ld + c) = o;
+        } else {
+            *reinterpret_cast<T4*>(mine + r * kPitch + c * (int)sizeof(T)) = o;
         }
-        M3_LDS_FENCE();
+    }
+    __device__ __forceinline__ void store() const {
+        if constexpr (sizeof(T) == 2) {
+            const int r0 = lane / LPR, c = lane % LPR * E;
+            M3_LDS_FENCE();  // the fours and the pieces are other types to the compiler
+#pragma unroll
+            for (int i = 0; i < (MF + RPI - 1) / RPI; ++i) {
+                const int r = i * RPI + r0;
+                if (r < MF && r < rows && c < cols)
+                    *reinterpret_cast<Piece*>(out + r * ld + c) = *reinterpret_cast<const Piece*>(mine + r * kPitch + c * (int)sizeof(T));
+            }
+            M3_LDS_FENCE();
+        }
     }
 };
 

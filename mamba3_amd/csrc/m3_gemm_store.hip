@@ -75,10 +75,11 @@ struct EpiStore {
                 }
             });
         } else if (vec) {
-            const GemmRows<T, Tile, Tile::FN * Tile::MF> rows(smem, at.wave(), at.lane);
+            GemmRows<T, Tile, Tile::FN * Tile::MF> rows(smem, at.wave(), at.lane);
 #pragma unroll
             for (int i = 0; i < Tile::FM; ++i) {
                 const int m = at.m(i), r0 = at.row0(i), c0 = at.col0();
+                rows.begin(out + (int64_t)r0 * s.ldo + c0, s.ldo, s.rows - r0, s.cols - c0);
 #pragma unroll
                 for (int j = 0; j < Tile::FN; ++j)
 #pragma unroll
@@ -93,7 +94,7 @@ struct EpiStore {
                         }
                         rows.put(j, q, v);
                     }
-                rows.store(out + (int64_t)r0 * s.ldo + c0, s.ldo, s.rows - r0, s.cols - c0);
+                rows.store();
             }
         } else {
             each(s, at, acc, [&](int m, int n, f32x4 v) {

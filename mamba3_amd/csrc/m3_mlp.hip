@@ -100,10 +100,11 @@ struct EpiGated {
     template <typename T, typename Tile, int kMode>
     __device__ __forceinline__ void run(const GemmPlace<Tile, kMode>& at,
                                         typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, const GemmItem&) const {
-        const GemmRows<T, Tile, Tile::FN / 2 * Tile::MF> out(smem, at.wave(), at.lane);
+        GemmRows<T, Tile, Tile::FN / 2 * Tile::MF> out(smem, at.wave(), at.lane);
 #pragma unroll
         for (int i = 0; i < Tile::FM; ++i) {
             const int m = at.m(i), r0 = at.row0(i), c0 = at.col0();
+            out.begin(reinterpret_cast<T*>(h) + (int64_t)r0 * ldh + c0, ldh, rows - r0, ldh - c0);
 #pragma unroll
             for (int jq = 0; jq < Tile::FN / 2 * Tile::Q; ++jq) {
                 const int j = jq / Tile::Q, q = jq % Tile::Q;
@@ -115,7 +116,7 @@ struct EpiGated {
                 out.put(j, q, v);
                 if (kept.p && m < rows && n < ldh) keep_gu<T>(kept, kept.at(m, n), g, u);
             }
-            out.store(reinterpret_cast<T*>(h) + (int64_t)r0 * ldh + c0, ldh, rows - r0, ldh - c0);
+            out.store();
         }
     }
 };
@@ -130,7 +131,7 @@ struct EpiGateBwd {
     __device__ __forceinline__ void run(const GemmPlace<Tile, kMode>& at,
                                         typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, const GemmItem&) const {
         constexpr int J = Tile::FN * Tile::Q;
-        const GemmRows<T, Tile, Tile::FN * Tile::MF> out(smem, at.wave(), at.lane);
+        GemmRows<T, Tile, Tile::FN * Tile::MF> out(smem, at.wave(), at.lane);
         // the kept values of a piece's row are fetched while the one before is worked on
         KeptFour<T> k[2][J];
         auto fetch = [&](int i) {
@@ -145,7 +146,9 @@ struct EpiGateBwd {
 #pragma unroll
         for (int i = 0; i < Tile::FM; ++i) {
             const int r0 = at.row0(i), c0 = at.col0();
+            const int64_t o = (int64_t)r0 * ldh + c0;
             if (i + 1 < Tile::FM) fetch(i + 1);
+            out.begin(reinterpret_cast<T*>(dg) + o, ldh, rows - r0, ldh - c0);
             f32x4 b[J];
 #pragma unroll
             for (int jq = 0; jq < J; ++jq) {
@@ -161,11 +164,11 @@ struct EpiGateBwd {
                 }
                 out.put(jq / Tile::Q, jq % Tile::Q, a);
             }
-            const int64_t o = (int64_t)r0 * ldh + c0;
-            out.store(reinterpret_cast<T*>(dg) + o, ldh, rows - r0, ldh - c0);
+            out.store();
+            out.begin(reinterpret_cast<T*>(du) + o, ldh, rows - r0, ldh - c0);
 #pragma unroll
             for (int jq = 0; jq < J; ++jq) out.put(jq / Tile::Q, jq % Tile::Q, b[jq]);
-            out.store(reinterpret_cast<T*>(du) + o, ldh, rows - r0, ldh - c0);
+            out.store();
         }
     }
 };

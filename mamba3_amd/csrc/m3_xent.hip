@@ -129,7 +129,7 @@ struct EpiXentBwd {
     __device__ __forceinline__ void run(const GemmPlace<Tile, kMode>& at,
                                         typename Tile::Acc (&acc)[Tile::FM][Tile::FN], char* smem, const GemmItem&) const {
         constexpr int J = Tile::FN * Tile::Q;
-        const GemmRows<T, Tile, Tile::FN * Tile::MF> out(smem, at.wave(), at.lane);
+        GemmRows<T, Tile, Tile::FN * Tile::MF> out(smem, at.wave(), at.lane);
         const int first = at.n(0, 0);
         const bool all = at.n0 + Tile::BN <= have;  // every column of the tile exists
         float low[Tile::FM], g[Tile::FM];
@@ -147,6 +147,8 @@ struct EpiXentBwd {
 #pragma unroll
         for (int i = 0; i < Tile::FM; ++i) {
             const bool hit = __any(rel[i] >= 0 && rel[i] < Tile::FN * Tile::MF);
+            const int r0 = at.row0(i), c0 = at.col0();
+            out.begin(reinterpret_cast<T*>(dz) + (int64_t)r0 * ld + c0, ld, rows - r0, ld - c0);
 #pragma unroll
             for (int j = 0; j < J; ++j) {
                 const int n = at.n(j / Tile::Q, j % Tile::Q);
@@ -163,8 +165,7 @@ struct EpiXentBwd {
                     for (int e = 0; e < 4; ++e) p[e] = n + e < have ? p[e] : 0.f;
                 out.put(j / Tile::Q, j % Tile::Q, p);
             }
-            const int r0 = at.row0(i), c0 = at.col0();
-            out.store(reinterpret_cast<T*>(dz) + (int64_t)r0 * ld + c0, ld, rows - r0, ld - c0);
+            out.store();
         }
     }
 };

@@ -19,7 +19,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     """Cross entropy of softmax(hidden weight^T) against target: hidden (..., d_model) and weight
     (vocab, d_model), both fp32 or both bf16, target (...) int64, on one GPU. Returns an fp32 scalar
     ("mean" over the rows that count, NaN where none does, or "sum") or a loss per row ("none").
-    Differentiable in hidden and weight; sums are fp32 and run in a fixed order.
+    Differentiable in hidden and weight; sums are fp32 and run in a fixed order. Under bf16 autocast both
+    are taken in bf16.
 
     A row whose target is `ignore_index` counts nowhere: its loss and its gradients are zero whatever
     `hidden` holds there. Any other target outside [0, vocab) is not checked on the host: it makes the
@@ -35,6 +36,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
         raise ValueError(f"reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
     if weight.numel() == 0:
         raise ValueError("linear_cross_entropy needs a vocabulary and d_model of at least 1")
+    hidden, weight = ops.autocast(hidden, weight)
     ops.check_alike("linear_cross_entropy", hidden, weight)
     if target.device != hidden.device:
         raise ValueError(f"target is on {target.device}, hidden on {hidden.device}")

@@ -19,8 +19,8 @@ def swiglu_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down
                residual: torch.Tensor | None = None, scale: float = 1.0) -> torch.Tensor:
     """x (..., d_model), w_gate and w_up (d_ff, d_model), w_down (d_model, d_ff), residual of x's
     shape; all fp32 or all bf16, on one GPU. Returns x's shape and dtype. Differentiable in every
-    tensor; sums are fp32 and run in a fixed order. Without gradients, at most 8 bf16 rows run on
-    the decode kernels (`m3_small_swiglu`, `m3_small_linear`) where they take the shape."""
+    tensor; sums are fp32 and run in a fixed order. Under bf16 autocast the products run in bf16 and the
+    residual is added in its own type. Without gradients, at most 8 bf16 rows run on the decode kernels (`m3_small_swiglu`, `m3_small_linear`) where they take the shape."""
     if x.dim() < 1 or w_gate.dim() != 2 or w_up.dim() != 2 or w_down.dim() != 2:
         raise ValueError("swiglu_mlp expects x (..., d_model) and two-dimensional weights")
     ff, d = w_gate.shape
@@ -29,6 +29,10 @@ def swiglu_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down
                          f"w_down {tuple(w_down.shape)} do not fit (..., d), (f, d), (f, d), (d, f)")
     if residual is not None and residual.shape != x.shape:
         raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {tuple(x.shape)}")
+    x, w_gate, w_up, w_down = ops.autocast(x, w_gate, w_up, w_down)
+    if residual is not None and residual.dtype != x.dtype and torch.is_autocast_enabled("cuda"):
+        # the residual stream keeps its type
+        return residual + swiglu_mlp(x, w_gate, w_up, w_down, None, scale)
     ins = (x, w_gate, w_up, w_down) if residual is None else (x, w_gate, w_up, w_down, residual)
     ops.check_alike("swiglu_mlp", *ins)
     if d == 0 or ff == 0:

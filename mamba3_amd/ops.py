@@ -734,6 +734,13 @@ def check_alike(what: str, *tensors: torch.Tensor) -> None:
     _native.require_gpu(first)
 
 
+def autocast(*tensors):
+    """The tensors in the type that torch.autocast runs products in, where that is bf16."""
+    if not torch.is_autocast_enabled("cuda") or torch.get_autocast_dtype("cuda") is not torch.bfloat16:
+        return tensors
+    return tuple(t.to(torch.bfloat16) for t in tensors)
+
+
 def _swiglu_mlp_eager(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
                       residual: Optional[torch.Tensor], scale: float,
                       keep: bool) -> tuple[torch.Tensor, Optional[torch.Tensor]]:

@@ -669,6 +669,56 @@ def test_compiled_step():
     assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
+def test_autocast():
+    """fp32 tensors under bf16 autocast: the products of their bf16 copies, the residual added in fp32."""
+    t = mlp_inputs(20, 64, 96, torch.float32)
+    low = {k: v.bfloat16() for k, v in t.items()}
+    hidden, weight, target = xent_inputs(20, 64, 50, torch.float32)
+    args = [low[k] for k in ("x", "w_gate", "w_up", "w_down")]
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = mamba3_amd.swiglu_mlp(**t, scale=0.5)
+        loss = mamba3_amd.linear_cross_entropy(hidden, weight, target)
+    assert y.dtype == torch.float32
+    assert torch.equal(y, t["residual"] + mamba3_amd.swiglu_mlp(*args, scale=0.5))
+    assert torch.equal(loss, mamba3_amd.linear_cross_entropy(hidden.bfloat16(), weight.bfloat16(), target))
+    lm = _lm(torch.float32).fuse_mlp()
+    ids = torch.randint(300, (2, 20), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        loss = lm.loss(ids, ids)
+    loss.backward()
+    assert loss.dtype == torch.float32 and torch.isfinite(loss) and lm.embedding.weight.grad.dtype == torch.float32
+
+
+def test_two_streams_at_once():
+    """The same two steps side by side on two streams, and after one another: nothing is shared."""
+    sets = [_step_inputs(seed=s, rows=900) for s in (0, 100)]
+    want = [[t.clone() for t in (*_step(*_step_inputs(seed=s, rows=900)),)] for s in (0, 100)]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for st, args in zip(streams, sets):
+        with torch.cuda.stream(st):
+            got.append(_step(*args))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_second_backward_and_changed_inputs_are_refused():
+    t = mlp_inputs(6, 16, 24, torch.float32)
+    x = t["x"].requires_grad_()
+    y = mamba3_amd.swiglu_mlp(**t)
+    (g,) = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    hidden, weight, target = xent_inputs(6, 16, 20, torch.float32)
+    loss = mamba3_amd.linear_cross_entropy(hidden, weight.requires_grad_(), target)
+    with torch.no_grad():
+        weight.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
 # ---------------------------------------------------------------- the language model
 def _lm(dtype, **kw):
     torch.manual_seed(0)
