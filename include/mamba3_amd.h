@@ -40,7 +40,8 @@ enum m3_status {
     M3_ERR_MISALIGNED = 5,        /* a pointer violates the documented alignment */
     M3_ERR_LAUNCH = 6,            /* the HIP runtime rejected a kernel launch */
     M3_ERR_DEVICE = 7,            /* device query failed (no device / wrong arch) */
-    M3_ERR_SCRATCH_LIMIT = 8      /* m3_prefill_fwd_noalloc: workspace need exceeds its scratch */
+    M3_ERR_SCRATCH_LIMIT = 8,     /* m3_prefill_fwd_noalloc: workspace need exceeds its scratch */
+    M3_ERR_OVERLAP = 9            /* m3_clip_grad_norm: tensors to be written overlap in memory */
 };
 
 /* Size of the static per-device scratch of m3_prefill_fwd_noalloc (64 MiB). */
@@ -460,8 +461,8 @@ enum m3_norm {
  * The norm over all elements of n tensors together and, with `scale`, their scaling in place:
  *   norm = (sum g^2)^(1/2) or max |g|; g <- g * min(1, max_norm / (norm + 1e-6))
  * tensors, numel and dtype are host arrays of n entries (device pointers of contiguous fp32 or
- * bf16 elements; empty tensors may be NULL), read before the call returns. The tensors must not
- * overlap. norm [1] fp32 on the device. Squares add up in fp64, in a fixed order. NaN and infinite
+ * bf16 elements; empty tensors may be NULL), read before the call returns. Tensors to be scaled must
+ * not overlap (M3_ERR_OVERLAP; sorting them takes host memory for the call). norm [1] fp32 on the device. Squares add up in fp64, in a fixed order. NaN and infinite
  * elements reach the norm; a NaN norm scales by NaN. A factor of 1 leaves the tensors unwritten.
  * workspace: 256-byte aligned.
  */

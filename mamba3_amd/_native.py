@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
+from array import array
 from pathlib import Path
 
 import torch
@@ -62,6 +63,7 @@ EXPORTED_SYMBOLS = (
 M3_ERR_UNSUPPORTED = 3
 M3_ERR_WORKSPACE = 4
 M3_ERR_SCRATCH_LIMIT = 8
+M3_ERR_OVERLAP = 9
 NOALLOC_SCRATCH_BYTES = 64 << 20
 
 
@@ -530,9 +532,13 @@ def clip_grad_norm(ptrs, numel, dtypes, kind: int, max_norm: float | None, norm)
     """m3_clip_grad_norm on contiguous tensors, given as lists of addresses, sizes and dtype codes;
     max_norm None: the norm alone. Allocates the workspace."""
     n = len(ptrs)
-    ptrs, numel, dtypes = (_vp * n)(*ptrs), (_i64 * n)(*numel), (_i32 * n)(*dtypes)
-    nbytes = _bytes_of("m3_clip_grad_norm_workspace_size", n, numel, dtypes)
+    ptrs, numel, dtypes = array("Q", ptrs), array("q", numel), array("i", dtypes)
+    p, k, d = (a.buffer_info()[0] for a in (ptrs, numel, dtypes))
+    nbytes = _bytes_of("m3_clip_grad_norm_workspace_size", n, k, d)
     ws = _workspace(nbytes, norm.device)
-    check(lib().m3_clip_grad_norm(n, ptrs, numel, dtypes, kind, int(max_norm is not None),
-                                  0.0 if max_norm is None else max_norm, ptr(norm), ptr(ws), nbytes,
-                                  stream_of(norm)), "m3_clip_grad_norm")
+    st = lib().m3_clip_grad_norm(n, p, k, d, kind, int(max_norm is not None),
+                                 0.0 if max_norm is None else max_norm, ptr(norm), ptr(ws), nbytes,
+                                 stream_of(norm))
+    if st == M3_ERR_OVERLAP:
+        raise ValueError("gradients that overlap in memory cannot be clipped in place")
+    check(st, "m3_clip_grad_norm")

@@ -19,8 +19,10 @@ def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm:
     once. Nothing waits for the GPU, unless error_if_nonfinite asks to raise, before anything is
     scaled, where the norm is NaN or infinite; otherwise such a norm scales by NaN or 0."""
     params = (parameters,) if isinstance(parameters, torch.Tensor) else parameters
-    # the same gradient listed twice counts once
-    grads = list({id(g): g for g in [p.grad for p in params] if g is not None}.values())
+    # A model has hundreds of small gradients: each of these passes over them is one C call per tensor.
+    grads = [g for g in [p.grad for p in params] if g is not None]
+    if len(set(map(id, grads))) < len(grads):
+        grads = list({id(g): g for g in grads}.values())
     max_norm, norm_type = float(max_norm), float(norm_type)
     if norm_type == 2.0:
         kind = _native.NORM_L2
@@ -32,37 +34,31 @@ def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     if not grads:
         return torch.tensor(0.0)
-    device = grads[0].device
-    for g in grads:
-        if g.layout is not torch.strided:
-            raise TypeError(f"clip_grad_norm_ takes dense gradients, got {g.layout}")
-        if g.device != device:
-            raise ValueError(f"gradients must be on one GPU, got {device} and {g.device}")
-    codes = [_native.dtype_code(g.dtype) for g in grads]
+    for layout in {g.layout for g in grads}:
+        if layout is not torch.strided:
+            raise TypeError(f"clip_grad_norm_ takes dense gradients, got {layout}")
+    dtypes = [g.dtype for g in grads]
+    codes = {d: _native.dtype_code(d) for d in set(dtypes)}
     _native.require_gpu(grads[0])
+    if len(set(map(torch.Tensor.get_device, grads))) > 1:
+        raise ValueError(f"gradients must be on one GPU, got {sorted({str(g.device) for g in grads})}")
     whole = grads  # what the kernels work on: the gradients themselves or contiguous copies
-    strided = [g for g in grads if not g.is_contiguous()]
-    if strided:
-        for g in strided:
-            if any(n > 1 and s == 0 for n, s in zip(g.shape, g.stride())):
+    if not all(map(torch.Tensor.is_contiguous, grads)):
+        for g in grads:
+            if not g.is_contiguous() and any(n > 1 and s == 0 for n, s in zip(g.shape, g.stride())):
                 raise ValueError("a gradient whose elements share memory (expanded) cannot be clipped in place")
         whole = [g.detach().contiguous() for g in grads]
-    ptrs, sizes = [t.data_ptr() for t in whole], [t.numel() for t in whole]
-    end = 0
-    for at, n, code in sorted(zip(ptrs, sizes, codes)):
-        if n:
-            if at < end:
-                raise ValueError("gradients that overlap in memory cannot be clipped in place")
-            end = at + n * (2 if code == _native.M3_DTYPE_BF16 else 4)
+    args = (list(map(torch.Tensor.data_ptr, whole)), list(map(torch.Tensor.numel, whole)),
+            [codes[d] for d in dtypes], kind)
     with ops.on_device(grads[0]):
-        norm = torch.empty((), dtype=torch.float32, device=device)
+        norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
         if error_if_nonfinite:
-            _native.clip_grad_norm(ptrs, sizes, codes, kind, None, norm)
+            _native.clip_grad_norm(*args, None, norm)
             if not math.isfinite(norm.item()):
                 raise RuntimeError(f"the norm of the gradients is {norm.item()}: they were not clipped")
-        _native.clip_grad_norm(ptrs, sizes, codes, kind, max_norm, norm)
+        _native.clip_grad_norm(*args, max_norm, norm)
         torch.autograd.graph.increment_version(grads)
-        if strided:
+        if whole is not grads:
             with torch.no_grad():
                 for g, t in zip(grads, whole):
                     if t.data_ptr() != g.data_ptr():

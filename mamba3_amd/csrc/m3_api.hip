@@ -1,10 +1,11 @@
 // C-ABI entry points (declared in include/mamba3_amd.h). Validates every argument on
-// the host, then calls the launchers. Never throws, never allocates, never syncs. The one
+// the host, then calls the launchers. Never throws, allocates nothing on the device, never syncs. The one
 // piece of global state is the static scratch of m3_prefill_fwd_noalloc (below).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <mutex>
+#include <new>
 
 #include "m3_kernels.h"
 
@@ -197,6 +198,7 @@ const char* m3_status_string(int status) {
         case M3_ERR_MISALIGNED: return "pointer alignment violated";
         case M3_ERR_LAUNCH: return "kernel launch failed";
         case M3_ERR_DEVICE: return "device query failed";
+        case M3_ERR_OVERLAP: return "tensors to be written overlap in memory";
         case M3_ERR_SCRATCH_LIMIT:
             return "workspace need exceeds the static scratch of m3_prefill_fwd_noalloc "
                    "(M3_NOALLOC_SCRATCH_BYTES); use m3_prefill_fwd with a caller workspace";
@@ -719,6 +721,25 @@ static int check_tensors(int32_t n, const int64_t* numel, const int32_t* dtype) 
     return m3::clip_total_blocks(n, numel, dtype) <= 0x3fffffff ? M3_OK : M3_ERR_UNSUPPORTED;
 }
 
+// No two of the tensors share memory.
+static int check_apart(int32_t n, void* const* tensors, const int64_t* numel, const int32_t* dtype) {
+    struct Span { uintptr_t at, end; };
+    Span* v = new (std::nothrow) Span[n > 0 ? n : 1];
+    if (!v) return M3_ERR_WORKSPACE;
+    int m = 0;
+    for (int i = 0; i < n; ++i)
+        if (numel[i]) {
+            const uintptr_t at = reinterpret_cast<uintptr_t>(tensors[i]);
+            v[m++] = Span{at, at + (uintptr_t)numel[i] * (dtype[i] == M3_DTYPE_BF16 ? 2 : 4)};
+        }
+    std::sort(v, v + m, [](const Span& a, const Span& b) { return a.at < b.at; });
+    int st = M3_OK;
+    for (int i = 1; i < m; ++i)
+        if (v[i - 1].end > v[i].at) st = M3_ERR_OVERLAP;
+    delete[] v;
+    return st;
+}
+
 int m3_clip_grad_norm_workspace_size(int32_t n, const int64_t* numel, const int32_t* dtype, size_t* bytes) {
     if (!bytes) return M3_ERR_NULL_POINTER;
     const int st = check_tensors(n, numel, dtype);
@@ -740,6 +761,10 @@ int m3_clip_grad_norm(int32_t n, void* const* tensors, const int64_t* numel, con
     }
     st = check_workspace(workspace, workspace_bytes, 256 + 8 * (size_t)m3::clip_total_blocks(n, numel, dtype));
     if (st != M3_OK) return st;
+    if (scale) {
+        st = check_apart(n, tensors, numel, dtype);
+        if (st != M3_OK) return st;
+    }
     return m3::launch_clip(n, tensors, numel, dtype, norm_kind == M3_NORM_MAX, scale != 0, max_norm, norm,
                            workspace, as_stream(stream));
 }

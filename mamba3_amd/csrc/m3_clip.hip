@@ -16,16 +16,17 @@
 namespace m3 {
 
 constexpr int kClipThreads = 256;
-constexpr int kClipTensors = 144;
+constexpr int kClipTensors = 240;
 constexpr int64_t kClipPiece = 128 << 10;
 
-struct ClipTensors {
+struct ClipTensors {  // 3.8 KB of kernel arguments
     void* p[kClipTensors];
-    int64_t n[kClipTensors];      // elements
-    int first[kClipTensors + 1];  // first block of each; [count] the number of blocks
+    uint32_t n[kClipTensors];     // elements (larger tensors take several entries)
+    int first[kClipTensors];      // first block of each
     int count;
     int block0;                   // blocks of earlier launches
 };
+constexpr int64_t kClipMost = (int64_t)1 << 30;  // elements of an entry: whole pieces of either type
 
 // The tensor of this block, and its elements [begin, end) there.
 template <typename T>
@@ -39,7 +40,7 @@ __device__ __forceinline__ int clip_piece(const ClipTensors& t, int64_t& begin, 
     }
     constexpr int64_t per = kClipPiece / (int64_t)sizeof(T);
     begin = (int64_t)(b - t.first[lo]) * per;
-    end = begin + per < t.n[lo] ? begin + per : t.n[lo];
+    end = begin + per < (int64_t)t.n[lo] ? begin + per : (int64_t)t.n[lo];
     return lo;
 }
 
@@ -155,24 +156,27 @@ static int clip_groups(int n, void* const* p, const int64_t* numel, const int32_
         int blocks = 0;
         auto flush = [&]() -> int {
             if (t.count == 0) return M3_OK;
-            t.first[t.count] = blocks;
             const int st = f(t, type, blocks);
             block0 += blocks;
             t.count = 0, t.block0 = block0, blocks = 0;
             return st;
         };
+        const int size = type == M3_DTYPE_BF16 ? 2 : 4;
         for (int j = 0; j < n; ++j) {
             const int i = back ? n - 1 - j : j;
-            if (dtype[i] != type || numel[i] == 0) continue;
-            if (t.count == kClipTensors || blocks + clip_blocks(numel[i], type) > (1 << 23)) {
-                const int st = flush();
-                if (st != M3_OK) return st;
+            if (dtype[i] != type) continue;
+            for (int64_t at = 0; at < numel[i]; at += kClipMost) {
+                const int64_t here = std::min(numel[i] - at, kClipMost);
+                if (t.count == kClipTensors || blocks + clip_blocks(here, type) > (1 << 23)) {
+                    const int st = flush();
+                    if (st != M3_OK) return st;
+                }
+                t.p[t.count] = reinterpret_cast<char*>(p[i]) + at * size;
+                t.n[t.count] = (uint32_t)here;
+                t.first[t.count] = blocks;
+                blocks += (int)clip_blocks(here, type);
+                ++t.count;
             }
-            t.p[t.count] = p[i];
-            t.n[t.count] = numel[i];
-            t.first[t.count] = blocks;
-            blocks += (int)clip_blocks(numel[i], type);
-            ++t.count;
         }
         const int st = flush();
         if (st != M3_OK) return st;
