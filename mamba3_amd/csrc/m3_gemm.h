@@ -477,7 +477,7 @@ __device__ __forceinline__ void gemm_run(const GemmGroup<kN>& grp, const Epi& ep
     // barrier and refills its own place: copies then have one and a half steps to land. Rows of k
     // would come in pieces of 64 bytes that way, which costs more than it gives (8192^3 x W^T 783 ->
     // 827 us; dy^T x 823 -> 800): there the whole step's place is refilled halfway through it.
-    // Copies and reads are issued between groups of FN MFMAs, which cover them, early in the half.
+    // Copies and reads are issued between groups of FN MFMAs, which cover them.
     constexpr bool kHalves = !kAKc && !kBKc && LA::NI > 1 && LB::NI > 1;
     typedef typename Type::Frag Frag;
     constexpr int KH = MF == 16 ? 1 : 2;
@@ -494,9 +494,13 @@ __device__ __forceinline__ void gemm_run(const GemmGroup<kN>& grp, const Epi& ep
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = Type::mma(fb[half][ks][j], fa[half][ks][i], acc[i][j]);
     };
-    constexpr int kPer = (kReads + kGroups - 1) / kGroups < 2 ? 2 : (kReads + kGroups - 1) / kGroups;
+    // Reads and copies between two groups: as few as fit the half, but two reads, and three with eight groups
+    // and rows of k on both sides (256 x 256 tiles, 8192^3 x W^T 777 us at two reads and two copies, 760 at
+    // three and one; dy W 786 at two and two, 765 at two and one; dy^T x 781, and 813 at three).
+    constexpr int kFew = kAKc && kBKc && kGroups >= 8 ? 3 : 2;
+    constexpr int kPer = (kReads + kGroups - 1) / kGroups < kFew ? kFew : (kReads + kGroups - 1) / kGroups;
     constexpr int kLd = kHalves ? NLD / 2 : NLD;  // copies behind a barrier
-    constexpr int kPerLd = (kLd + kGroups - 1) / kGroups < 2 && !kHalves ? 2 : (kLd + kGroups - 1) / kGroups;
+    constexpr int kPerLd = (kLd + kGroups - 1) / kGroups;
     auto fetch_half = [&](int half, int i, int slot) __attribute__((always_inline)) {  // copy i of the kLd behind the barrier before `half`
         if constexpr (kHalves) {
             constexpr int A = LA::NI / 2;
