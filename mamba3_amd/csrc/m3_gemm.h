@@ -494,13 +494,13 @@ __device__ __forceinline__ void gemm_run(const GemmGroup<kN>& grp, const Epi& ep
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = Type::mma(fb[half][ks][j], fa[half][ks][i], acc[i][j]);
     };
-    // Reads and copies between two groups: as few as fit the half, but two reads, and three with eight groups
-    // and rows of k on both sides (256 x 256 tiles, 8192^3 x W^T 777 us at two reads and two copies, 760 at
-    // three and one; dy W 786 at two and two, 765 at two and one; dy^T x 781, and 813 at three).
-    constexpr int kFew = kAKc && kBKc && kGroups >= 8 ? 3 : 2;
-    constexpr int kPer = (kReads + kGroups - 1) / kGroups < kFew ? kFew : (kReads + kGroups - 1) / kGroups;
+    // Reads and copies between two groups: two, and with B in rows of n as few copies as fit the half
+    // (256 x 256 tiles, 8192^3: dy W 786 us at two copies, 765 at one; dy^T x 781 us, and 813 at three
+    // reads; x W^T 777, and 760 at three reads and one copy, which over short k is slower: cross
+    // entropy of 8192 x 768 against 32000 tokens, forward and backward, 1609 us and 1627).
+    constexpr int kPer = (kReads + kGroups - 1) / kGroups < 2 ? 2 : (kReads + kGroups - 1) / kGroups;
     constexpr int kLd = kHalves ? NLD / 2 : NLD;  // copies behind a barrier
-    constexpr int kPerLd = (kLd + kGroups - 1) / kGroups;
+    constexpr int kPerLd = (kLd + kGroups - 1) / kGroups < 2 && kBKc ? 2 : (kLd + kGroups - 1) / kGroups;
     auto fetch_half = [&](int half, int i, int slot) __attribute__((always_inline)) {  // copy i of the kLd behind the barrier before `half`
         if constexpr (kHalves) {
             constexpr int A = LA::NI / 2;

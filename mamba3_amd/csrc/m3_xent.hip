@@ -22,6 +22,10 @@ namespace m3 {
 constexpr int64_t kXentPieceBytes = (int64_t)256 << 20;
 constexpr int64_t kXentPieceMost = (int64_t)1 << 20;  // columns: a tile's rows stay within 32-bit offsets
 
+template <typename T> __device__ __forceinline__ float exp_of(float x);
+template <> __device__ __forceinline__ float exp_of<bf16>(float x) { return fast_exp(x); }
+template <> __device__ __forceinline__ float exp_of<float>(float x) { return expf(x); }
+
 // (max, sum of exp(z - max)) of two disjoint sets. An empty set is (-inf, 0).
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
     const float top = fmaxf(m, m2);
@@ -135,10 +139,9 @@ struct EpiXentBwd {
             const int m = at.m(i) < rows ? at.m(i) : rows - 1;
             const int64_t t = target[m];
             const bool live = t != ignore;
-            // exp(z - inf) = 0: hidden reads as zero where it is ignored
-            low[i] = !live ? INFINITY : t < 0 || t >= vocab ? NAN : lse[m];
-            if constexpr (sizeof(T) == 2) low[i] *= kLog2e;
+            low[i] = live ? lse[m] : INFINITY;  // exp(z - inf) = 0: hidden reads as zero where it is ignored
             g[i] = gl && live ? gl[m] : 1.f;
+            if (live && (t < 0 || t >= vocab)) g[i] = NAN;
             rel[i] = live && t >= v0 && t < v0 + have ? (int)(t - v0) - first : -1;
         }
 #pragma unroll
@@ -152,14 +155,11 @@ struct EpiXentBwd {
                 const f32x4 z = four(acc[i][j / Tile::Q], j % Tile::Q);
                 f32x4 p;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (sizeof(T) == 2) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], kLog2e, -low[i]));
-                    else p[e] = expf(z[e] - low[i]);
-                }
+                for (int e = 0; e < 4; ++e) p[e] = exp_of<T>(z[e] - low[i]);
                 if (hit)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) p[e] -= rel[i] == n - first + e ? 1.f : 0.f;
-                if (gl) p *= g[i];
+                p *= g[i];
                 if (!all)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) p[e] = n + e < have ? p[e] : 0.f;
