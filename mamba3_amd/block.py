@@ -166,12 +166,10 @@ class KulaMambaBlock(nn.Module):
         return x
 
     def _mlp_residual(self, x: torch.Tensor, inplace: bool = False) -> torch.Tensor:
-        if self.fused_mlp:
-            n = self.mlp_norm(x)
-            if n.dtype == x.dtype and self.mlp.fusable(n):
-                return self.mlp.fused(n, x, self.residual_scale)
-        return add_scaled_linear(x, self.mlp.w_down, self.mlp.hidden(self.mlp_norm(x)),
-                                 self.residual_scale, inplace=inplace)
+        n = self.mlp_norm(x)
+        if self.fused_mlp and n.dtype == x.dtype and self.mlp.fusable(n):
+            return self.mlp.fused(n, x, self.residual_scale)
+        return add_scaled_linear(x, self.mlp.w_down, self.mlp.hidden(n), self.residual_scale, inplace=inplace)
 
     def _small_step_usable(self, x: torch.Tensor) -> bool:
         """The decode step runs on the small-batch projection kernels (norm + in_proj,

@@ -23,7 +23,7 @@ struct GemmPlan {
 
 // One product to be planned: rows x cols results (for a gated product, cols counts both halves) over
 // k steps of 128 bytes; max_splits 1 where the epilogue needs the whole sum; tn: both operands in rows of
-// m and n; sums: fp32 partial sums are written whatever the split.
+// m and n.
 struct GemmTask {
     int64_t rows, cols, steps;
     int max_splits;

@@ -5,8 +5,13 @@
 // on the tiled products of m3_gemm.h. Both projections, the activation and the product are one
 // kernel: a tile holds the gate and the up columns of the same hidden units, so g and u meet in
 // a lane's registers in fp32 and only h is stored. The backward's dh is never stored either: its
-// epilogue reads g and u and writes dg and du, the operands of the four gradient products (dx
-// is one product of two terms; dWg and dWu are one launch).
+// epilogue reads g and u and writes dg and du, the operands of the four gradient products, which
+// are one launch (dx is one product of two terms).
+//
+// Measured, bf16, 8192 rows, d 768, ff 2112 (forward + backward 346 us, 239 GFLOP): gated product 73 us,
+// down 46, dh 67, gradients 165; d 2048, ff 5504 (1.49 ms, 1,120 TF/s): 329, 167, 226, 766. Bound by
+// the MFMAs; the small size by 4.1 and 2.1 rounds of tiles that take 5 and 3, and by the kept values'
+// bytes next to twelve k steps a tile.
 //
 // For the backward the forward keeps g and u. bf16: their upper 24 bits (the upper 16 of each, and the
 // next 8 of both in another 16): a bf16 copy alone would put a rounding
