@@ -656,6 +656,99 @@ def test_captured_step_replays():
             _step(*_step_inputs(seed=7))  # eager work of its own between the replays
 
 
+# ---------------------------------------------------------------- offsets past 32 bits
+def test_mlp_offsets_past_32_bits():
+    """h, and what is kept for the backward, pass 4 GiB: the last rows against the definition. Only
+    they have a dy, so the weights' gradients are theirs."""
+    rows, d, ff, last = (1 << 21) + 37, 64, 1088, 300
+    print(rows, d, ff, flush=True)
+    t = mlp_inputs(rows, d, ff, torch.bfloat16)
+    dy = torch.zeros(rows, d, device="cuda", dtype=torch.bfloat16)
+    dy[-last:] = randn(last, d, dtype=torch.bfloat16, seed=9)
+    leaves = {k: v.requires_grad_() for k, v in t.items()}
+    y = mamba3_amd.swiglu_mlp(**t, scale=0.5)
+    grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)))
+    end = {k: v.detach()[-last:] if k in ("x", "residual") else v.detach() for k, v in t.items()}
+    want = mlp_expected(end, 0.5, dy[-last:], torch.bfloat16)
+    hold("y", y[-last:], want["y"])
+    for k in leaves:
+        hold(k, grads[k][-last:] if k in ("x", "residual") else grads[k], want[k])
+    assert not grads["x"][:-last].any()
+
+
+def test_xent_row_offsets_past_32_bits():
+    rows, d, vocab, last = (1 << 25) + 5, 64, 200, 300
+    print(rows, d, vocab, flush=True)
+    hidden, weight, target = xent_inputs(rows, d, vocab, torch.bfloat16)
+    grad = torch.zeros(rows, device="cuda")
+    grad[-last:] = randn(last, dtype=torch.float32, seed=5)
+    hidden.requires_grad_()
+    weight.requires_grad_()
+    loss = mamba3_amd.linear_cross_entropy(hidden, weight, target, reduction="none")
+    dh, dw = torch.autograd.grad(loss, [hidden, weight], grad)
+    want = xent_expected(hidden.detach()[-last:], weight, target[-last:], "none", grad[-last:], torch.bfloat16)
+    for name, got, w in zip(("loss", "dhidden", "dweight"), (loss[-last:], dh[-last:], dw), want):
+        hold(name, got, w)
+    assert not dh[:-last].any()
+
+
+def test_xent_vocabulary_offsets_past_32_bits():
+    """A weight of 4 GiB whose last rows are not zero, and hold the targets."""
+    rows, d, vocab, last = 5, 64, (1 << 25) + 3, 70
+    print(rows, d, vocab, flush=True)
+    hidden, end, target = xent_inputs(rows, d, last, torch.bfloat16, ignored=0.0)
+    weight = torch.zeros(vocab, d, device="cuda", dtype=torch.bfloat16)
+    weight[-last:] = end * 4  # exact; some logits of these rows outweigh the zeros of all others
+    hidden.requires_grad_()
+    weight.requires_grad_()
+    loss = mamba3_amd.linear_cross_entropy(hidden, weight, target + vocab - last, reduction="sum")
+    dh, dw = torch.autograd.grad(loss, [hidden, weight])
+    h, w = Num(hidden), Num(weight.detach()[-last:])
+    z = h.dot(w)
+    lse = torch.logaddexp(torch.logsumexp(z.v, 1), torch.full((rows,), math.log(vocab - last), device="cuda").double())[:, None]
+    # a row's sum: at most 256 terms in a lane's and a tile's order, then the tiles' pairs one by one
+    e_lse = z.e.amax(1, keepdim=True) + (64 + vocab / 64 + (z.top.amax(1, keepdim=True) + 4) * 2) * STEP + lse.abs() * STEP * 2
+    at = target[:, None]
+    want = (lse - z.v.gather(1, at)).sum()
+    assert abs(loss.item() - want.item()) <= (e_lse + z.e.gather(1, at) + 2 * STEP * (lse.abs() + z.top.gather(1, at))).sum().item()
+    p = torch.exp(z.v - lse)
+    dz = Num(p - torch.zeros_like(p).scatter_(1, at, 1.0), p * torch.expm1(z.e + e_lse + ((z.v - lse).abs() + 4) * 2.0 ** -22) + STEP)
+    dz = dz.rounded(torch.bfloat16)
+    # the other rows of the weight are zero: they add nothing to dhidden
+    hold("dhidden", dh, dz.dot(w.t()).rounded(torch.bfloat16))
+    hold("dweight", dw[-last:], dz.t().dot(h.t()).rounded(torch.bfloat16))
+    rest = torch.exp(-lse) * torch.ones(1, 1000, device="cuda").double()
+    rest = Num(rest, rest * torch.expm1(e_lse + (lse.abs() + 4) * 2.0 ** -22)).rounded(torch.bfloat16)
+    for begin in (0, (1 << 25) - 2000):
+        hold("dweight", dw[begin:begin + 1000], rest.t().dot(h.t()).rounded(torch.bfloat16))
+
+
+def test_clip_offsets_past_32_bits():
+    n = (1 << 32) + 12345
+    print(n, flush=True)
+    p = torch.nn.Parameter(torch.empty(n, device="cuda", dtype=torch.bfloat16))
+    p.grad = torch.zeros(n, device="cuda", dtype=torch.bfloat16)
+    p.grad[0], p.grad[1 << 32], p.grad[-1] = 2.0, 3.0, 6.0
+    assert mamba3_amd.clip_grad_norm_(p, 3.5).item() == 7.0
+    # the factor is 0.5 but for 1e-6 / 7: the halves are the nearest bf16
+    assert (p.grad[0].item(), p.grad[1 << 32].item(), p.grad[-1].item()) == (1.0, 1.5, 3.0)
+    assert p.grad.count_nonzero().item() == 3
+
+
+def test_compiled_for_other_row_counts():
+    x, weights, head, target = _step_inputs()
+
+    def f(x, target):
+        return mamba3_amd.linear_cross_entropy(mamba3_amd.swiglu_mlp(x, *weights, residual=x), head, target)
+
+    leaves = [*weights, head]
+    step = torch.compile(f, fullgraph=True, dynamic=True)
+    for n in (x.shape[0], x.shape[0] // 2 + 1, 3):
+        want = torch.autograd.grad(f(x[:n], target[:n]), leaves)
+        got = torch.autograd.grad(step(x[:n], target[:n]), leaves)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 def test_compiled_step():
     x, weights, head, target = _step_inputs()
 
