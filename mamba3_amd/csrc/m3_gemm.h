@@ -340,7 +340,7 @@ __device__ __forceinline__ GemmItem gemm_item(const GemmArgs& a, int prob, int i
     const int tn = scalar(in / rows);
     return GemmItem{prob, first + in - tn * rows, tn, split};
 }
-// The k steps of a product, and where part `split` of them begins (steps < 2^26, splits <= 16).
+// The k steps of a product, and where part `split` of them begins (steps < 2^26, splits <= 64).
 template <int kMode, int BK>
 __device__ __forceinline__ int gemm_steps_of(const GemmArgs& a) {
     return (a.K[0] + BK - 1) / BK + (kMode == kSeg2 ? (a.K[1] + BK - 1) / BK : 0);

@@ -5,6 +5,7 @@
 #include <atomic>
 
 #include "m3_gemm.h"
+#include "m3_gemm_plan.h"
 
 namespace m3 {
 
@@ -13,7 +14,6 @@ namespace m3 {
 typedef GemmTile<256, 256, 2, 4, 2, 16> TileL;
 template <typename T> using TileM = GemmTile<128, 128, 2, 2, 2, sizeof(T) == 2 ? 16 : 32>;
 typedef GemmTile<64, 64, 2, 2, 4, 16> TileS;
-enum { kTileL = 0, kTileM = 1, kTileS = 2 };
 
 struct GemmPlan {
     int tile;
@@ -21,21 +21,7 @@ struct GemmPlan {
     int bm, bn;
 };
 
-// One product to be planned: rows x cols results (for a gated product, cols counts both halves) over
-// k steps of 128 bytes; max_splits 1 where the epilogue needs the whole sum; tn: both operands in rows of
-// m and n.
-struct GemmTask {
-    int64_t rows, cols, steps;
-    int max_splits;
-    bool tn;
-};
-constexpr int kGroupMax = 4;
-constexpr int kMaxSplits = 16;
-struct GemmGroupPlan {
-    int tile;
-    int splits[kGroupMax];
-};
-// The tile for products of one launch and the number of k parts of each with the least estimated time.
+// search_plan (m3_gemm_plan.h), kept for the next calls of the same sizes.
 GemmGroupPlan gemm_group_plan(int dtype, const GemmTask* tasks, int n);
 GemmPlan gemm_plan(int dtype, int64_t rows, int64_t cols, int64_t steps, int max_splits);
 

@@ -279,96 +279,6 @@ int gemm_pad_copy(int dtype, const GemmPads& pads, const int64_t* target, int64_
     return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH;
 }
 
-// Estimated us of each choice, from launches of 256, 512 and 1024 tiles of 8 and 64 k steps (torch on the
-// same card: 8192^3 bf16 668 us): a step of a 256 x 256 tile takes 1.45 us (1.38 where both operands
-// are rows of m and n), of a 128 x 128 tile 0.62 us alone on its CU and 0.90 us (1.05) next to another, of a
-// 64 x 64 tile 0.20 and 0.37 us; to that come a tile's start and epilogue. Parts of k cost the
-// fp32 partial sums' write and read and a launch.
-// What it decides, both sides measured: the gated product of 8192 x 11008 x 2048 takes 80 us less on 256 x 256
-// tiles than on 128 x 128, that of 8192 x 4224 x 768 8 us more; the 8192 x 768 product over 16128 takes
-// 33 us less in two parts on 256 x 256 tiles than whole on 128 x 128.
-namespace {
-struct TileCost { int size, at_once; double alone, all, tn, fixed; };
-const TileCost kCostBf16[3] = {{256, 1, 1.45, 1.45, 1.38, 8.0}, {128, 2, 0.62, 0.90, 1.05, 4.5}, {64, 2, 0.20, 0.37, 0.38, 3.5}};
-const TileCost kCostF32[3] = {{0, 0, 0, 0, 0, 0}, {128, 2, 1.90, 3.60, 3.60, 5.0}, {64, 2, 0.65, 1.07, 1.07, 4.0}};
-
-int64_t group_items(const TileCost& c, const GemmTask& t, int splits) {
-    return ((t.rows + c.size - 1) / c.size) * ((t.cols + c.size - 1) / c.size) * splits;
-}
-
-// Rounds of as many items as run at once, each as long as its longest item.
-double group_us(const TileCost& c, const GemmTask* t, const int* splits, int n) {
-    const int64_t slots = (int64_t)256 * c.at_once;
-    double us = 0, longest = 0, alone = 0;  // of the current round's items, and with a CU to themselves
-    int64_t room = slots;                   // left in the current round
-    bool joined = false;
-    for (int p = 0; p < n; ++p) {
-        int64_t items = group_items(c, t[p], splits[p]);
-        if (items == 0) continue;
-        const double steps = (double)((t[p].steps + splits[p] - 1) / splits[p]);
-        const double one = steps * (t[p].tn ? c.tn : c.all) + c.fixed, own = std::min(one, steps * c.alone + c.fixed);
-        if (splits[p] > 1) {
-            us += (double)t[p].rows * t[p].cols * 8.0 * splits[p] / 5.0e6;
-            joined = true;
-        }
-        const int64_t in = std::min(items, room);
-        longest = std::max(longest, one), alone = std::max(alone, own);
-        room -= in, items -= in;
-        if (room == 0) us += longest, longest = alone = 0, room = slots;
-        us += items / slots * one;
-        items %= slots;
-        if (items) longest = one, alone = own, room = slots - items;
-    }
-    // the last round may leave each item a CU to itself
-    return us + (slots - room <= 256 ? alone : longest) + (joined ? 4.0 : 0.0);
-}
-}  // namespace
-
-static GemmGroupPlan search_plan(int dtype, const GemmTask* tasks, int n) {
-    const TileCost* c = dtype == M3_DTYPE_BF16 ? kCostBf16 : kCostF32;
-    static const int kTry[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16};
-    GemmGroupPlan best{kTileS, {1, 1, 1, 1}};
-    double least = 1e30;
-    for (int t = dtype == M3_DTYPE_BF16 ? kTileL : kTileM; t <= kTileS; ++t) {
-        int s[kGroupMax] = {1, 1, 1, 1};
-        double us = group_us(c[t], tasks, s, n);
-        // all dy^T x alike first, then one product after the other; a launch of many rounds gains nothing
-        // from parts
-        int64_t items = 0;
-        for (int p = 0; p < n; ++p) items += group_items(c[t], tasks[p], 1);
-        if (items <= (int64_t)256 * c[t].at_once * 6) {
-            auto fits = [&](int p, int k) { return k <= tasks[p].max_splits && k <= tasks[p].steps; };
-            int alike = 1;
-            for (int k : kTry) {
-                int v[kGroupMax] = {1, 1, 1, 1};
-                for (int p = 0; p < n; ++p)
-                    if (tasks[p].tn && fits(p, k)) v[p] = k;
-                const double u = group_us(c[t], tasks, v, n);
-                if (u < us) us = u, alike = k;
-            }
-            for (int p = 0; p < n; ++p)
-                if (tasks[p].tn && fits(p, alike)) s[p] = alike;
-            for (int pass = 0; pass < 2; ++pass)
-                for (int p = 0; p < n; ++p) {
-                    int keep = s[p];
-                    for (int k : kTry) {
-                        if (!fits(p, k)) break;
-                        s[p] = k;
-                        const double u = group_us(c[t], tasks, s, n);
-                        if (u < us) us = u, keep = k;
-                    }
-                    s[p] = keep;
-                }
-        }
-        if (us < least) {
-            least = us;
-            best.tile = t;
-            for (int p = 0; p < kGroupMax; ++p) best.splits[p] = s[p];
-        }
-    }
-    return best;
-}
-
 // The search takes 20 us of host time, and a call asks three times (the workspace's size, its check, the
 // launch): each thread keeps its last plans.
 GemmGroupPlan gemm_group_plan(int dtype, const GemmTask* tasks, int n) {
@@ -388,7 +298,7 @@ GemmGroupPlan gemm_group_plan(int dtype, const GemmTask* tasks, int n) {
     bool hit = k.dtype == dtype && k.n == n;
     for (int p = 0; hit && p < n; ++p) hit = same(k.t[p], tasks[p]);
     if (!hit) {
-        k.plan = search_plan(dtype, tasks, n);
+        k.plan = search_plan(dtype == M3_DTYPE_BF16, tasks, n);
         k.dtype = dtype, k.n = n;
         for (int p = 0; p < n; ++p) k.t[p] = tasks[p];
     }

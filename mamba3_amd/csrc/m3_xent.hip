@@ -296,7 +296,7 @@ XentFwd xent_fwd_layout(int64_t rows, int64_t d, int64_t vocab, int dtype, void*
 struct XentBwd {
     int64_t piece;  // columns of a piece (its row stride)
     GemmPlan z;
-    GemmGroupPlan grads;  // dh, dW
+    GemmPairPlan grads;  // dh, dW
     void *h, *w, *dz;
     float* part;      // dh's sums
     float* part_dw;
@@ -311,15 +311,15 @@ XentBwd xent_bwd_layout(int64_t rows, int64_t d, int64_t vocab, int dtype, bool 
     const int64_t pieces = (vocab + most - 1) / most;
     f.piece = pieces == 1 ? gemm_pad(vocab, dtype) : ((vocab + pieces - 1) / pieces + 255) / 256 * 256;
     f.z = gemm_plan(dtype, rows, f.piece, gemm_steps(d, dtype), 1);
-    const GemmTask tasks[2] = {{want_dh ? rows : 0, d, gemm_steps(f.piece, dtype), kMaxSplits, false},
+    const GemmTask tasks[2] = {{want_dh ? rows : 0, d, gemm_steps(f.piece, dtype), kMostSplits, false},
                                {want_dw ? f.piece : 0, d, gemm_steps(rows, dtype), kMaxSplits, true}};
-    f.grads = gemm_group_plan(dtype, tasks, 2);
-    const int dh_splits = f.grads.splits[0];
+    f.grads = pair_plan(tasks, [&](const GemmTask (&t)[2]) { return gemm_group_plan(dtype, t, 2); });
+    const int dh_splits = f.grads.p[0].splits[0];
     f.h = b.take(rows * dp * size);
     f.w = dp != d ? b.take(vocab * dp * size) : nullptr;
     f.dz = b.take(rows * f.piece * size);
     f.part = want_dh && (pieces > 1 || dh_splits > 1) ? reinterpret_cast<float*>(b.take((int64_t)dh_splits * rows * d * 4)) : nullptr;
-    f.part_dw = want_dw ? reinterpret_cast<float*>(b.take((int64_t)gemm_part_bytes(f.grads.splits[1], f.piece, d))) : nullptr;
+    f.part_dw = want_dw ? reinterpret_cast<float*>(b.take((int64_t)gemm_part_bytes(f.grads.p[1].splits[1], f.piece, d))) : nullptr;
     f.bytes = b.used;
     return f;
 }
@@ -399,12 +399,21 @@ int launch_xent_bwd(int64_t rows, int64_t d, int64_t vocab, int dtype, int reduc
             g.st[1] = GemmStore{reinterpret_cast<char*>(dweight) + v0 * d * size, d, nullptr, 1.f, f.part_dw, 0, (int)have, (int)d};
             g.st[1].num = dh.num, g.st[1].den = dh.den;
         }
-        M3_TRY(gemm_grads(dtype, f.grads, g, stream));
+        if (f.grads.apart) {
+            GemmGrads one;
+            one.a[0] = g.a[0], one.st[0] = g.st[0];
+            M3_TRY(gemm_grads(dtype, f.grads.p[0], one, stream));
+            one = GemmGrads{};
+            one.a[1] = g.a[1], one.st[1] = g.st[1];
+            M3_TRY(gemm_grads(dtype, f.grads.p[1], one, stream));
+        } else {
+            M3_TRY(gemm_grads(dtype, f.grads.p[0], g, stream));
+        }
         dh.add = 1;
     }
     if (dhidden && f.piece < vocab) {
         dh.out = dhidden;
-        dh.splits = f.grads.splits[0];
+        dh.splits = f.grads.p[0].splits[0];
         M3_TRY(gemm_reduce(dtype, &dh, 1, stream));
     }
     return M3_OK;

@@ -471,6 +471,28 @@ def test_xent_gradient_against_differences():
         assert abs((grads[i].double() * way).sum().item() - slope) <= allowed
 
 
+@pytest.mark.parametrize("rows,d,vocab,parts", [(1, 64, 128000, 64), (16, 200, 50021, 48), (16, 64, 128000, 64)])
+def test_xent_few_rows_sum_the_vocabulary_in_parts(rows, d, vocab, parts):
+    """dhidden of few rows is a sum over the whole vocabulary. All its terms but the last are alike and positive
+    (hidden is zero, a column of the weight is one number), so that roundings of one chain of additions fall to the
+    same side; cut into parts, a part's chain is vocab / parts long and the parts' sums come to it."""
+    print(rows, d, vocab, flush=True)
+    weight = (1.0 + torch.rand(1, d, generator=torch.Generator().manual_seed(0)).cuda()).expand(vocab, d).contiguous().requires_grad_()
+    hidden = torch.zeros(rows, d, device="cuda", requires_grad=True)
+    target = torch.full((rows,), vocab - 1, device="cuda")
+    loss = mamba3_amd.linear_cross_entropy(hidden, weight, target, reduction="sum")
+    dh, dw = torch.autograd.grad(loss, [hidden, weight])
+    lse = math.log(vocab)
+    w = weight[0].detach().double()
+    # p = 1 / vocab off by lse's own error (its sum: 64 terms in a lane, 500 tiles' pairs) and the exponential's
+    e_p = (lse + 4) * 2.0 ** -22 + (64 + vocab / 256 + 2 * lse) * STEP
+    # the terms' magnitudes are 2 w in all; the true sum is 0
+    bound = 2 * w * (e_p + (vocab / parts + parts + 2) * STEP)
+    assert abs(loss.item() - rows * lse) <= rows * lse * e_p
+    assert (dh.double().abs() <= bound).all(), (dh.double().abs() / bound).max().item()
+    assert not dw.any()  # products with hidden
+
+
 # ---------------------------------------------------------------- clipping
 def _params(shapes, seed=0, std=1.0):
     out = []
