@@ -164,8 +164,9 @@ struct EpiGateBwd {
                     float g, u;
                     k[i & 1][jq].get(e, g, u);
                     const float s = sigmoid_of<T>(g), dh = v[e] * alpha;
-                    a[e] = dh * u * s * (1.f + g * (1.f - s));
-                    b[jq][e] = dh * g * s;
+                    // s, which is 0 for far gates, meets each large factor before they meet one another
+                    a[e] = dh * (u * (s * (1.f + g * (1.f - s))));
+                    b[jq][e] = dh * (g * s);
                 }
                 out.put(jq / Tile::Q, jq % Tile::Q, a);
             }

@@ -1,0 +1,50 @@
+"""The training operators at the edges of what their documentation allows: saturated and infinite values, a
+vocabulary in several pieces, gradients that share memory, modules that do more than their weights say, other
+row counts under compilation. Bounds as in test_gpu_train_ops."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+import mamba3_amd
+from mamba3_amd import _native
+from test_gpu_train_ops import DTYPES, HALF, STEP, _lm, hold, mlp_inputs, randn, xent_expected, xent_inputs
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- the gated MLP
+def _gates(values, dtype, up=1.0, dy=1.0):
+    """One row through an MLP whose hidden unit j has gate values[j] (the sum of its entries) and the given up
+    value: (y, dg, du) of the units, read off as gradients of the weights' columns that x's 1 meets."""
+    n = len(values)
+    terms = torch.tensor(values, device="cuda").to(dtype).view(n, -1)
+    x = torch.zeros(1, 8, device="cuda", dtype=dtype)
+    x[0, :terms.shape[1]] = 1.0
+    wg = torch.zeros(n, 8, device="cuda", dtype=dtype)
+    wg[:, :terms.shape[1]] = terms
+    wu = torch.zeros(n, 8, device="cuda", dtype=dtype)
+    wu[:, 0] = up
+    wd = torch.eye(8, n, device="cuda", dtype=dtype)
+    wg.requires_grad_(), wu.requires_grad_()
+    y = mamba3_amd.swiglu_mlp(x, wg, wu, wd)
+    dwg, dwu = torch.autograd.grad(y, [wg, wu], torch.full_like(y, dy))
+    return wg.detach().double().sum(1), dwg[:, 0].double(), dwu[:, 0].double()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp32"])
+@pytest.mark.parametrize("up", [1.0, 3e37, -3e37])
+def test_mlp_saturated_gates_meet_large_gradients(dtype, up):
+    """Far-out gates under a gradient of several units: silu and its slope are 0 or as good as 0 there, and their
+    products with large factors 0 as well, not infinity times zero."""
+    gates = [-3e38, -1e38, -1e30, -200.0, 200.0, 1e4, 1e30, 1e37]
+    g, dg, du = _gates([[v] for v in gates], dtype, up, dy=8.0)
+    u = torch.tensor(up).to(dtype).double().item()
+    flat = g < -100.0
+    slope, silu = torch.where(flat, 0.0, 1.0).double(), torch.where(flat, 0.0, g)
+    assert torch.allclose(du, 8.0 * silu, rtol=2 * HALF[dtype] + 8 * STEP, atol=1e-30), du
+    assert torch.allclose(dg, 8.0 * u * slope, rtol=2 * HALF[dtype] + 8 * STEP, atol=1e-30), dg
