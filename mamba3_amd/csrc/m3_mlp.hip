@@ -13,9 +13,9 @@
 // the MFMAs; the small size by 4.1 and 2.1 rounds of tiles that take 5 and 3, and by the kept values'
 // bytes next to twelve k steps a tile.
 //
-// For the backward the forward keeps g and u. bf16: their upper 24 bits (the upper 16 of each, and the
-// next 8 of both in another 16): a bf16 copy alone would put a rounding
-// of g and one of u (2^-9 each) into dg and du next to their own; 24 bits leave 2^-16 for 2 more
+// For the backward the forward keeps g and u. bf16: rounded to 24 bits (the upper 16 of each, and the
+// next 8 of both in another 16), a relative 2^-16: a bf16 copy alone would put a rounding
+// of g and one of u (2^-8 each) into dg and du next to their own; 24 bits cost 2 more
 // bytes an element. fp32: as they are.
 #include "m3_gemm_host.h"
 #include "m3_kernels.h"
@@ -42,6 +42,10 @@ struct KeptGu {
     }
 };
 
+// A float's bits, to be cut to the upper 24: rounded to the nearest (ties away from zero; past the largest, to
+// infinity). Infinities stay, and NaNs: of bf16 operands they have zeros in their low bits.
+__device__ __forceinline__ unsigned round24(float v) { return __builtin_bit_cast(unsigned, v) + 0x80; }
+
 // bf16: [element fours][g upper 16 x 4, u upper 16 x 4], then [element fours][the next 8 of both x 4].
 // fp32: g, then u.
 template <typename T>
@@ -53,7 +57,7 @@ __device__ __forceinline__ void keep_gu(const KeptGu& k, int64_t at, f32x4 g, f3
         for (int e = 0; e < 4; ++e) {
             // (__builtin_bit_cast of a vector's component takes component 0 on this compiler)
             const float ge = g[e], ue = u[e];
-            const unsigned gb = __builtin_bit_cast(unsigned, ge), ub = __builtin_bit_cast(unsigned, ue);
+            const unsigned gb = round24(ge), ub = round24(ue);
             hi[e] = (unsigned short)(gb >> 16);
             hi[4 + e] = (unsigned short)(ub >> 16);
             lo[e] = (unsigned short)((gb >> 8 & 0xff) | (ub & 0xff00));

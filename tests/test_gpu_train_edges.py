@@ -48,3 +48,19 @@ def test_mlp_saturated_gates_meet_large_gradients(dtype, up):
     slope, silu = torch.where(flat, 0.0, 1.0).double(), torch.where(flat, 0.0, g)
     assert torch.allclose(du, 8.0 * silu, rtol=2 * HALF[dtype] + 8 * STEP, atol=1e-30), du
     assert torch.allclose(dg, 8.0 * u * slope, rtol=2 * HALF[dtype] + 8 * STEP, atol=1e-30), dg
+
+
+def test_mlp_kept_gates_are_rounded_to_the_nearest():
+    """What the backward reads of a gate in bf16 has 16 significant bits: half a step of those, 2^-16 in [1, 2), is
+    how far it may be off. Near the zero of silu' (g = -1.2784645) a gate's error is all that is left of dg: gates
+    there whose last bits, 2^-15 and below, are just under a whole step."""
+    root, a, step = 1.2784645427610738, 1.2734375, 2.0 ** -15
+    base = math.floor((root - a) / step)
+    gates = [[-a, -(base + i) * step, -f * step] for i in (-4, -1, 0, 3) for f in (0.96875, 0.5625)]
+    g, dg, _ = _gates(gates, torch.bfloat16)
+    assert ((g + root).abs() < 2.0 ** -12).all()
+    s = torch.sigmoid(g)
+    want = s * (1 + g * (1 - s))
+    # |silu''| <= 0.2195 around here; the slope's own fp32 steps; dg and its gradient are rounded to bf16
+    bound = 0.2195 * 2.0 ** -16 + (g.abs() + 4) * 2.0 ** -21 * s * (1 + g.abs()) + 2 * HALF[torch.bfloat16] * want.abs()
+    assert ((dg - want).abs() <= bound).all(), ((dg - want).abs() / bound).max().item()
