@@ -146,9 +146,9 @@ struct EpiXentBwd {
             const int m = at.m(i) < rows ? at.m(i) : rows - 1;
             const int64_t t = target[m];
             const bool live = t != ignore;
-            low[i] = live ? lse[m] : INFINITY;  // exp(z - inf) = 0: hidden reads as zero where it is ignored
+            // a target outside the vocabulary makes its row NaN
+            low[i] = !live ? INFINITY : t < 0 || t >= vocab ? NAN : lse[m];
             g[i] = gl && live ? gl[m] : 1.f;
-            if (live && (t < 0 || t >= vocab)) g[i] = NAN;
             rel[i] = live && t >= v0 && t < v0 + have ? (int)(t - v0) - first : -1;
         }
 #pragma unroll
@@ -166,7 +166,10 @@ struct EpiXentBwd {
                 if (hit)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) p[e] -= rel[i] == n - first + e ? 1.f : 0.f;
-                p *= g[i];
+                if (gl) p *= g[i];
+                // ignored: zero whatever the weight holds (hidden reads as zero there, and 0 * inf is NaN)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[e] = low[i] == INFINITY ? 0.f : p[e];
                 if (!all)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) p[e] = n + e < have ? p[e] : 0.f;

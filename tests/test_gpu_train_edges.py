@@ -64,3 +64,20 @@ def test_mlp_kept_gates_are_rounded_to_the_nearest():
     # |silu''| <= 0.2195 around here; the slope's own fp32 steps; dg and its gradient are rounded to bf16
     bound = 0.2195 * 2.0 ** -16 + (g.abs() + 4) * 2.0 ** -21 * s * (1 + g.abs()) + 2 * HALF[torch.bfloat16] * want.abs()
     assert ((dg - want).abs() <= bound).all(), ((dg - want).abs() / bound).max().item()
+
+
+# ---------------------------------------------------------------- the linear cross entropy
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp32"])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_xent_ignored_rows_add_nothing_to_a_weight_that_is_not_finite(dtype, value):
+    """dweight is a sum over the rows that count: without any it is zero, whatever the weight holds."""
+    hidden, weight, _ = xent_inputs(40, 48, 300, dtype)
+    weight[7, 3], weight[290] = value, value
+    target = torch.full((40,), -100, device="cuda")
+    for reduction in ("mean", "sum", "none"):
+        h, w = hidden.detach().requires_grad_(), weight.detach().requires_grad_()
+        loss = mamba3_amd.linear_cross_entropy(h, w, target, reduction=reduction)
+        (dw,) = torch.autograd.grad(loss.sum(), [w])
+        assert not dw.any(), reduction
+        if reduction != "mean":
+            assert not loss.any()
