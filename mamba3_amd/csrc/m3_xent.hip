@@ -33,10 +33,12 @@ template <typename T> __device__ __forceinline__ float exp_of(float x);
 template <> __device__ __forceinline__ float exp_of<bf16>(float x) { return fast_exp(x); }
 template <> __device__ __forceinline__ float exp_of<float>(float x) { return expf(x); }
 
-// (max, sum of exp(z - max)) of two disjoint sets. An empty set is (-inf, 0).
-__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+// (max, sum of exp(z - max)) of two disjoint sets. An empty set is (-inf, 0). S: the sum's type; a row's pairs come one
+// after another, hundreds of them for a large vocabulary, and are summed in fp64.
+template <typename S>
+__device__ __forceinline__ void join(float& m, S& s, float m2, S s2) {
     const float top = fmaxf(m, m2);
-    const float a = m == top ? s : s * expf(m - top), b = m2 == top ? s2 : s2 * expf(m2 - top);
+    const S a = m == top ? s : s * (S)expf(m - top), b = m2 == top ? s2 : s2 * (S)expf(m2 - top);
     m = top;
     s = a + b;
 }
@@ -110,6 +112,8 @@ struct EpiXentFwd {
                 for (int j = 0; j < J; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(z[j][e], kLog2e, low));
+                // every term is off by low's rounding, which the fma sees
+                sum *= __builtin_amdgcn_exp2f(-__builtin_fmaf(ref, kLog2e, low));
             } else {
 #pragma unroll
                 for (int j = 0; j < J; ++j)
@@ -190,32 +194,36 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(const float2* __restrict
                                                         int rows, int vocab, float* __restrict__ loss,
                                                         float* __restrict__ lse, double* __restrict__ sums) {
     constexpr int Q = 256 / kXentRows;
-    __shared__ float2 red[Q][kXentRows];
+    __shared__ float red_top[Q][kXentRows];
+    __shared__ double red_sum[Q][kXentRows];
     const int r = threadIdx.x % kXentRows, q = threadIdx.x / kXentRows;
     const int m = blockIdx.x * kXentRows + r;
-    float top = -INFINITY, sum = 0.f;
+    float top = -INFINITY;
+    double sum = 0.0;
     if (m < rows) {
 #pragma unroll 4
         for (int t = q; t < tiles; t += Q) {
             const float2 v = part[(int64_t)t * rows + m];
-            join(top, sum, v.x, v.y);
+            join(top, sum, v.x, (double)v.y);
         }
     }
-    red[q][r] = make_float2(top, sum);
+    red_top[q][r] = top;
+    red_sum[q][r] = sum;
     __syncthreads();
     if (threadIdx.x >= 64) return;
     double mine = 0.0, counts = 0.0;
     if (q == 0 && m < rows) {
 #pragma unroll
-        for (int k = 1; k < Q; ++k) join(top, sum, red[k][r].x, red[k][r].y);
-        const float l = top + logf(sum);
+        for (int k = 1; k < Q; ++k) join(top, sum, red_top[k][r], red_sum[k][r]);
+        // the loss from the difference of the logits, not of numbers as large as they are
+        const float log_sum = logf((float)sum);
         const int64_t t = target[m];
         float v = 0.f;
         if (t != ignore) {
-            v = t >= 0 && t < vocab ? l - zt[m] : NAN;
+            v = t >= 0 && t < vocab ? (top - zt[m]) + log_sum : NAN;
             counts = 1.0;
         }
-        lse[m] = l;
+        lse[m] = top + log_sum;
         if (loss) loss[m] = v;
         mine = (double)v;
     }

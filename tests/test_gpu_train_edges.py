@@ -81,3 +81,23 @@ def test_xent_ignored_rows_add_nothing_to_a_weight_that_is_not_finite(dtype, val
         assert not dw.any(), reduction
         if reduction != "mean":
             assert not loss.any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp32"])
+def test_xent_small_losses_of_large_logits(dtype):
+    """Logits of thousands that lie a few units apart: the loss is their difference, log sum exp(z - top) + (top -
+    z_target), and no number as large as the logits is rounded on the way."""
+    top = 4096.0
+    steps = [0.0, 2.0, 3.0, 5.0, 8.0, 16.0]
+    hidden = torch.full((len(steps), 8), 0.0, device="cuda", dtype=dtype)
+    hidden[:, 0], hidden[:, 1] = 64.0, 1.0
+    weight = torch.zeros(len(steps) + 50, 8, device="cuda", dtype=dtype)
+    weight[:len(steps), 0] = top / 64
+    weight[:len(steps), 1] = -torch.tensor(steps, device="cuda").to(dtype)
+    target = torch.arange(len(steps), device="cuda")
+    loss = mamba3_amd.linear_cross_entropy(hidden, weight, target, reduction="none").double()
+    z = top - torch.tensor(steps, device="cuda").double()
+    log_sum = torch.log(torch.exp(z - top).sum())
+    want = log_sum + (top - z)
+    # the exponentials' and the logarithm's steps, one addition
+    assert ((loss - want).abs() <= (16 + 4) * 2.0 ** -22 + 4 * STEP * want).all(), (loss - want).abs().max().item()
