@@ -21,6 +21,8 @@
 // Rows whose target is ignored count nowhere: their loss and dz are zero by selection, and
 // products over rows read them as zeros, whatever the row holds. A target outside [0, V) that is
 // not the ignored value makes its row's loss, and the gradients it enters, NaN.
+#include <type_traits>
+
 #include "m3_gemm_host.h"
 #include "m3_kernels.h"
 
@@ -80,51 +82,63 @@ struct EpiXentFwd {
             const int64_t t = m < rows ? target[m] : -1;
             rel[i] = t >= 0 && t < vocab ? (int)t - first : -1;
         }
+        auto logit = [&](int i, int j, int e) __attribute__((always_inline)) {
+            const float v = four(acc[i][j / Tile::Q], j % Tile::Q)[e];
+            return kAll || at.n(j / Tile::Q, j % Tile::Q) + e < vocab ? v : -INFINITY;
+        };
+        float top[Tile::FM];
 #pragma unroll
         for (int i = 0; i < Tile::FM; ++i) {
-            float z[J][4];
-            float top = -INFINITY;
+            top[i] = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const f32x4 v = four(acc[i][j / Tile::Q], j % Tile::Q);
-                const int n = at.n(j / Tile::Q, j % Tile::Q);
+            for (int j = 0; j < J; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    z[j][e] = kAll || n + e < vocab ? v[e] : -INFINITY;
-                    top = fmaxf(top, z[j][e]);
-                }
-            }
+                for (int e = 0; e < 4; ++e) top[i] = fmaxf(top[i], logit(i, j, e));
             // few waves hold the target of one of their rows
             if (__any(rel[i] >= 0 && rel[i] < Tile::FN * Tile::MF)) {
 #pragma unroll
                 for (int j = 0; j < J; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (rel[i] == at.n(j / Tile::Q, j % Tile::Q) - first + e) zt[at.m(i)] = z[j][e];
+                        if (rel[i] == at.n(j / Tile::Q, j % Tile::Q) - first + e) zt[at.m(i)] = logit(i, j, e);
             }
-#pragma unroll
-            for (int off = Tile::MF; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off, kWave));
-            const float ref = top == -INFINITY ? 0.f : top;  // a row without finite logits
-            float sum = 0.f;
-            if constexpr (sizeof(T) == 2) {
-                const float low = -ref * kLog2e;
-#pragma unroll
-                for (int j = 0; j < J; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(z[j][e], kLog2e, low));
-                // every term is off by low's rounding, which the fma sees
-                sum *= __builtin_amdgcn_exp2f(-__builtin_fmaf(ref, kLog2e, low));
-            } else {
-#pragma unroll
-                for (int j = 0; j < J; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sum += expf(z[j][e] - ref);
-            }
-#pragma unroll
-            for (int off = Tile::MF; off < 64; off *= 2) sum += __shfl_xor(sum, off, kWave);
-            if (at.lane < Tile::MF) red[at.wn * Tile::BM + at.local_m(i)] = make_float2(top, sum);
         }
+        bool any_far = false;
+#pragma unroll
+        for (int i = 0; i < Tile::FM; ++i) {
+#pragma unroll
+            for (int off = Tile::MF; off < 64; off *= 2) top[i] = fmaxf(top[i], __shfl_xor(top[i], off, kWave));
+            any_far = any_far || far(top[i]);
+        }
+        // The sums of exp(z - top). bf16: as one fma before the instruction, but for far rows; `some`: there are such
+        // rows in this wave (the others' sums do not change by it).
+        auto sums = [&](auto some) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < Tile::FM; ++i) {
+                const float ref = top[i] == -INFINITY ? 0.f : top[i];  // a row without finite logits
+                const float low = -ref * kLog2e;
+                float sum = 0.f, apart = 0.f;
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float z = logit(i, j, e);
+                        if constexpr (sizeof(T) == 2) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, low));
+                        if constexpr (decltype(some)::value) apart += exp_of<T>(z - ref);
+                    }
+                // every term is off by low's rounding, which the fma sees
+                if constexpr (sizeof(T) == 2) sum *= __builtin_amdgcn_exp2f(-__builtin_fmaf(ref, kLog2e, low));
+                if constexpr (decltype(some)::value) sum = sizeof(T) == 4 || far(ref) ? apart : sum;
+#pragma unroll
+                for (int off = Tile::MF; off < 64; off *= 2) sum += __shfl_xor(sum, off, kWave);
+                if (at.lane < Tile::MF) red[at.wn * Tile::BM + at.local_m(i)] = make_float2(top[i], sum);
+            }
+        };
+        if (sizeof(T) == 4 || __any(any_far)) sums(std::true_type{});
+        else sums(std::false_type{});
     }
+    // logits at the type's ends: their product with log2(e) overflows
+    static __device__ __forceinline__ bool far(float top) { return fabsf(top) > 1e38f && top != -INFINITY; }
 };
 
 struct EpiXentBwd {

@@ -101,3 +101,32 @@ def test_xent_small_losses_of_large_logits(dtype):
     want = log_sum + (top - z)
     # the exponentials' and the logarithm's steps, one addition
     assert ((loss - want).abs() <= (16 + 4) * 2.0 ** -22 + 4 * STEP * want).all(), (loss - want).abs().max().item()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp32"])
+@pytest.mark.parametrize("vocab", [64, 700, 1029])
+def test_xent_logits_at_the_types_lowest_value(dtype, vocab):
+    """Whole tiles of columns, and whole rows, at the lowest finite value: they take no part beside others, and are
+    as good as one another alone."""
+    low = torch.finfo(dtype).min
+    hidden = torch.zeros(4, 8, device="cuda", dtype=dtype)
+    hidden[0, 0], hidden[1, 1], hidden[2, 2], hidden[3, 3] = 1.0, 1.0, 1.0, 1.0
+    weight = torch.zeros(vocab, 8, device="cuda", dtype=dtype)
+    weight[:, 0] = low                                # row 0: nothing but the lowest
+    weight[: vocab - 20, 1] = low                     # row 1: all columns but the last
+    weight[30:, 2] = low                              # row 2: all columns but the first
+    weight[::3, 3] = low
+    weight[:, 4] = torch.linspace(-2, 2, vocab).to(dtype)
+    hidden[1:, 4] = 1.0
+    target = torch.tensor([5, vocab - 3, 7, 10], device="cuda")
+    loss = mamba3_amd.linear_cross_entropy(hidden, weight, target, reduction="none")
+    z = hidden.detach().double() @ weight.detach().double().t()
+    want = torch.nn.functional.cross_entropy(z, target, reduction="none")
+    assert ((loss.double() - want).abs() <= 64 * STEP * (1 + want)).all(), (loss, want)
+    # (the gradient takes exp(z - lse) from an lse in fp32: row 0's is no more than its maximum)
+    h, w = hidden.detach()[1:].requires_grad_(), weight.detach().requires_grad_()
+    dw = torch.autograd.grad(mamba3_amd.linear_cross_entropy(h, w, target[1:], reduction="sum"), w)[0].double()
+    dz = torch.softmax(z[1:], 1)
+    dz[torch.arange(3, device="cuda"), target[1:]] -= 1
+    size = dz.abs().t() @ h.detach().double().abs()
+    assert ((dw - dz.t() @ h.detach().double()).abs() <= size * (2 * HALF[dtype] + 64 * STEP) + STEP).all()
