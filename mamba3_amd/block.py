@@ -14,6 +14,7 @@ import math
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.nn.modules.module import _has_any_global_hook
 from torch.utils.checkpoint import checkpoint as grad_checkpoint
 
 from . import _native, ops
@@ -41,6 +42,19 @@ def add_scaled_linear(x: torch.Tensor, lin: nn.Linear, inp: torch.Tensor, scale:
     if lin.bias is not None:
         out = out + lin.bias * scale
     return out.view(x.shape)
+
+
+def _as_written(m: nn.Module, cls: type) -> bool:
+    """Calling `m` runs cls.forward and nothing else: no subclass, no forward of its own, no hooks (its own or those of
+    all modules)."""
+    return (type(m) is cls and "forward" not in m.__dict__
+            and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+            and not _has_any_global_hook())
+
+
+def _only_weight(lin: nn.Module) -> bool:
+    """Calling `lin` is x W^T."""
+    return _as_written(lin, nn.Linear) and lin.bias is None
 
 
 class SwiGLU(nn.Module):
@@ -82,10 +96,11 @@ class SwiGLU(nn.Module):
         return self.w_down(self.hidden(x))
 
     def fusable(self, x: torch.Tensor) -> bool:
-        """swiglu_mlp takes these projections and x: no biases, one dtype of its two."""
+        """swiglu_mlp takes these projections and x (one dtype of its two) and computes what calling them would."""
         lins = (self.w_gate, self.w_up, self.w_down)
         return (x.is_cuda and x.dtype in (torch.float32, torch.bfloat16) and not torch.is_autocast_enabled("cuda")
-                and all(p.bias is None and p.weight.dtype == x.dtype and p.weight.device == x.device for p in lins))
+                and _as_written(self, SwiGLU)
+                and all(_only_weight(p) and p.weight.dtype == x.dtype and p.weight.device == x.device for p in lins))
 
     def fused(self, x: torch.Tensor, residual: torch.Tensor | None = None, scale: float = 1.0) -> torch.Tensor:
         """[residual +] scale * w_down(silu(w_gate x) * w_up x) as one operator (swiglu_mlp)."""
@@ -294,7 +309,8 @@ class KulaMambaLM(nn.Module):
     def loss(self, input_ids: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
         """The mean next-token cross entropy that forward returns as "loss" (fp32), without the
         logits: the head and the loss are one operator (linear_cross_entropy), so a training step
-        holds neither the (tokens, vocab) logits nor their gradient. labels: (B, T), position t is
+        holds neither the (tokens, vocab) logits nor their gradient. A head that is more than its weight
+        (a bias, hooks, a subclass) is called, and its logits kept. labels: (B, T), position t is
         predicted from t - 1; those equal to ignore_index do not count."""
         if labels.shape != input_ids.shape:
             raise ValueError(f"labels have shape {tuple(labels.shape)}, expected {tuple(input_ids.shape)}")
@@ -305,7 +321,10 @@ class KulaMambaLM(nn.Module):
         # the hidden states
         target = torch.full_like(labels, ignore_index)
         target[:, :-1] = labels[:, 1:]
-        return linear_cross_entropy(self.norm(x), self.lm_head.weight, target, ignore_index)
+        x = self.norm(x)
+        if not _only_weight(self.lm_head):
+            return F.cross_entropy(self.lm_head(x).flatten(0, -2).float(), target.flatten(), ignore_index=ignore_index)
+        return linear_cross_entropy(x, self.lm_head.weight, target, ignore_index)
 
     def forward(self, input_ids: torch.Tensor, labels: torch.Tensor | None = None) -> dict:
         x = self.embedding(input_ids)

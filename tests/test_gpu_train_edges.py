@@ -130,3 +130,77 @@ def test_xent_logits_at_the_types_lowest_value(dtype, vocab):
     dz[torch.arange(3, device="cuda"), target[1:]] -= 1
     size = dz.abs().t() @ h.detach().double().abs()
     assert ((dw - dz.t() @ h.detach().double()).abs() <= size * (2 * HALF[dtype] + 64 * STEP) + STEP).all()
+
+
+# ---------------------------------------------------------------- modules
+class _Doubled(torch.nn.Linear):
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+def _mlp_of(lm):
+    return lm.layers[0].mlp
+
+
+@pytest.mark.parametrize("name", ["w_gate", "w_up", "w_down", "lm_head"])
+@pytest.mark.parametrize("how", ["hook", "pre_hook", "subclass", "forward", "global"])
+def test_modules_with_more_than_a_weight_are_called(name, how):
+    """A projection with hooks or a forward of its own: fuse_mlp and loss give what the path without them gives."""
+    ids = torch.randint(300, (2, 20), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    # (without checkpointing the block reads w_down's weight for its residual)
+    lm = _lm(torch.float32, tie_weights=False, gradient_checkpointing=name == "w_down").train()
+    owner = lm if name == "lm_head" else _mlp_of(lm)
+    lin, undo = getattr(owner, name), None
+    if how == "hook":
+        lin.register_forward_hook(lambda m, args, out: 2 * out)
+    elif how == "pre_hook":
+        lin.register_forward_pre_hook(lambda m, args: (2 * args[0],))
+    elif how == "subclass":
+        twice = _Doubled(lin.in_features, lin.out_features, bias=False).cuda()
+        twice.load_state_dict(lin.state_dict())
+        setattr(owner, name, twice)
+    elif how == "forward":
+        plain = lin.forward
+        lin.forward = lambda x: 2 * plain(x)
+    else:
+        undo = torch.nn.modules.module.register_module_forward_hook(lambda m, args, out: 2 * out if m is lin else None)
+    try:
+        want = lm(ids, ids)["loss"]
+        want_g = torch.autograd.grad(want, lm.embedding.weight)[0]
+        got = lm.fuse_mlp().loss(ids, ids)
+        got_g = torch.autograd.grad(got, lm.embedding.weight)[0]
+    finally:
+        if undo is not None:
+            undo.remove()
+    assert abs(got.item() - want.item()) <= 1e-5 * abs(want.item())
+    assert (got_g - want_g).norm() <= 1e-4 * want_g.norm()
+
+
+def test_hooks_of_the_mlp_itself_are_called():
+    ids = torch.randint(300, (2, 20), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    lm = _lm(torch.float32, gradient_checkpointing=True).train()
+    _mlp_of(lm).register_forward_hook(lambda m, args, out: 2 * out)
+    want = lm(ids, ids)["loss"].item()
+    assert abs(lm.fuse_mlp().loss(ids, ids).item() - want) <= 1e-5 * want
+
+
+def test_loss_of_a_head_with_a_bias():
+    ids = torch.randint(300, (2, 20), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    lm = _lm(torch.float32, tie_weights=False)
+    head = torch.nn.Linear(128, 300).cuda()
+    lm.lm_head = head
+    labels = ids.clone()
+    labels[0, 5:9] = 7
+    want = lm(ids, ids)["loss"]
+    assert abs(lm.loss(ids, ids).item() - want.item()) <= 1e-5 * want.item()
+    want = lm(ids, torch.where(labels == 7, -100, labels))["loss"]
+    assert abs(lm.loss(ids, labels, ignore_index=7).item() - want.item()) <= 1e-5 * want.item()
+
+
+def test_language_model_compiles_with_its_fused_mlp():
+    ids = torch.randint(300, (2, 20), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    lm = _lm(torch.bfloat16).train().fuse_mlp()
+    want = torch.autograd.grad(lm.loss(ids, ids), lm.embedding.weight)[0]
+    got = torch.autograd.grad(torch.compile(lm.loss, fullgraph=True)(ids, ids), lm.embedding.weight)[0]
+    # the compiler may keep what eager code rounds between operators
+    assert (got.float() - want.float()).norm() <= 16 * HALF[torch.bfloat16] * want.float().norm()
