@@ -204,3 +204,44 @@ def test_language_model_compiles_with_its_fused_mlp():
     got = torch.autograd.grad(torch.compile(lm.loss, fullgraph=True)(ids, ids), lm.embedding.weight)[0]
     # the compiler may keep what eager code rounds between operators
     assert (got.float() - want.float()).norm() <= 16 * HALF[torch.bfloat16] * want.float().norm()
+
+
+# ---------------------------------------------------------------- clipping
+def _with_grads(*grads):
+    out = []
+    for g in grads:
+        p = torch.nn.Parameter(torch.empty(g.shape, device="cuda", dtype=g.dtype))
+        p.grad = g
+        out.append(p)
+    return out
+
+
+def test_clip_refuses_strided_gradients_that_share_memory():
+    base = randn(64, 40, dtype=torch.float32, seed=3)
+    kept = base.clone()
+    shared = [
+        (base[:, :20], base[:, 19:]),                       # columns that meet in one
+        (base[::2], base[:3]),                              # every second row, and the first rows
+        (base.t(), base[10:11]),                            # all of it transposed, and a row
+        (base.flatten()[::3], base.flatten()[1::2]),        # different steps through the same numbers
+        (base.as_strided((10, 10), (5, 1)),),               # one that meets itself
+        (base[:, 3].expand(4, 64).t(),),
+    ]
+    for grads in shared:
+        with pytest.raises(ValueError, match="overlap|share memory"):
+            mamba3_amd.clip_grad_norm_(_with_grads(*grads), 1.0)
+    assert torch.equal(base, kept)
+
+
+def test_clip_takes_interleaved_gradients():
+    """Views of one buffer that lie between one another's elements: every element counts, and is scaled, once."""
+    for cut in (lambda b: (b[:, :13], b[:, 13:14], b[:, 14:]), lambda b: (b[::2], b[1::2]),
+                lambda b: (b.flatten()[::3], b.flatten()[1::3], b.flatten()[2::3]),
+                lambda b: (b[:32].t(), b[32:]), lambda b: (b.flatten()[::4], b.flatten()[2::4], b.flatten()[1::2])):
+        base = randn(64, 40, dtype=torch.float32, seed=3)
+        want = base.double()
+        norm = want.norm().item()
+        got = mamba3_amd.clip_grad_norm_(_with_grads(*cut(base)), 0.5).item()
+        assert abs(got - norm) <= STEP * norm
+        want = want * (0.5 / (norm + 1e-6))
+        assert ((base.double() - want).abs() <= want.abs() * (HALF[torch.float32] + 2 * STEP)).all()

@@ -5,12 +5,14 @@ from __future__ import annotations
 
 import ctypes
 import math
+import random
 
 import pytest
 import torch
 
 import mamba3_amd
 from mamba3_amd import _native
+from mamba3_amd.clip import _refuse_shared_memory
 
 FAKE = 1 << 12  # an address that is never dereferenced: the call is refused first
 
@@ -171,3 +173,58 @@ def test_clip_grad_norm_refuses():
 def test_new_names_are_attributes_beside_the_eight():
     for name in ("swiglu_mlp", "linear_cross_entropy", "clip_grad_norm_"):
         assert callable(getattr(mamba3_amd, name)) and name not in mamba3_amd.__all__
+
+
+def _elements(g, base):
+    """Byte addresses of g's elements from base, each size of them."""
+    at = torch.zeros((), dtype=torch.long)
+    for k, (n, s) in enumerate(zip(g.shape, g.stride())):
+        at = at + (torch.arange(n) * s).view([-1 if i == k else 1 for i in range(g.dim())])
+    first = (at.flatten() * g.element_size() + g.data_ptr() - base)[:, None]
+    return (first + torch.arange(g.element_size())).flatten()
+
+
+def test_clip_finds_shared_memory_of_strided_gradients():
+    """The host's answer against every byte written down, for small strided views of one buffer in two types."""
+    rng = random.Random(0)
+    fp32 = torch.zeros(20000)
+    bf16 = fp32.view(torch.bfloat16)
+    seen = [0, 0]
+    for _ in range(1500):
+        grads = []
+        for _ in range(rng.randint(1, 3)):
+            base, dims = rng.choice([fp32, fp32, bf16]), rng.randint(1, 3)
+            shape = [rng.randint(1, 9) for _ in range(dims)]
+            if rng.random() < 0.5:
+                strides = [rng.randint(1, 30) for _ in range(dims)]
+            else:  # the axes of one array, in any order
+                strides, step = [], rng.choice([1, 2, 3])
+                for n in shape:
+                    strides.append(step)
+                    step *= n + rng.randint(0, 2)
+                rng.shuffle(strides)
+            grads.append(base.as_strided(shape, strides, rng.randint(0, 120)))
+        used = [_elements(g, fp32.data_ptr()) for g in grads]
+        shared = torch.cat(used).bincount().max().item() > 1
+        whole = [u for g, u in zip(grads, used) if g.is_contiguous()]
+        if whole and torch.cat(whole).bincount().max().item() > 1:
+            continue  # contiguous ones are compared by the library
+        seen[shared] += 1
+        if shared:
+            with pytest.raises(ValueError, match="overlap|share memory"):
+                _refuse_shared_memory(grads)
+        else:
+            _refuse_shared_memory(grads)
+    assert min(seen) > 200
+
+
+def test_clip_tells_large_strided_gradients_apart():
+    """Slices of a weight of 100 M elements, which is never touched: answered from the strides."""
+    flat = torch.empty(8192 * 12288)
+    m = flat.view(8192, 12288)
+    for grads in ((m[:, :4096], m[:, 4096:8192], m[:, 8192:]), (flat[::3], flat[1::3]), (flat[::6], flat[1::2]),
+                  (m[:4096].t(), m[4096:]), (m.view(64, 128, 96, 128)[:, :, ::2], m.view(64, 128, 96, 128)[:, :, 1::2, 5:])):
+        _refuse_shared_memory(list(grads))
+    for grads in ((m[:, :4097], m[:, 4096:8192]), (flat[::7], flat[3::11]), (m.t(), m[8191:]), (flat.as_strided((100, 100), (99, 1)),)):
+        with pytest.raises(ValueError, match="overlap|share memory"):
+            _refuse_shared_memory(list(grads))
