@@ -474,8 +474,13 @@ def _workspace(nbytes: int, device) -> torch.Tensor | None:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
-def swiglu_mlp_saved_bytes(rows: int, d: int, ff: int, dtype: torch.dtype) -> int:
-    return _bytes_of("m3_swiglu_mlp_saved_size", rows, d, ff, dtype_code(dtype))
+def swiglu_mlp_saved_bytes(rows: int, ff: int, dtype: torch.dtype) -> int:
+    """m3_swiglu_mlp_saved_size, in arithmetic that a symbolic number of rows passes through: g and u in blocks of
+    16 x 16 (24 bits each for bf16), then h with rows of whole 16 bytes."""
+    size = dtype.itemsize
+    wide = -(-ff * size // 16) * 16 // size
+    kept = (rows + 15) // 16 * 16 * ((wide + 15) // 16 * 16) * (6 if size == 2 else 8)
+    return (kept + 255) // 256 * 256 + (rows * wide * size + 255) // 256 * 256
 
 
 def swiglu_mlp_fwd(x, w_gate, w_up, w_down, residual, scale, y, saved) -> None:

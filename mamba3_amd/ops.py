@@ -750,7 +750,7 @@ def _swiglu_mlp_eager(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     with on_device(x):
         x2 = _flat(x)
         y = torch.empty(x2.shape, device=x.device, dtype=x.dtype)
-        n = _native.swiglu_mlp_saved_bytes(*x2.shape, w_gate.shape[0], x.dtype) if keep else 0
+        n = _native.swiglu_mlp_saved_bytes(x2.shape[0], w_gate.shape[0], x.dtype) if keep else 0
         saved = torch.empty(n, device=x.device, dtype=torch.uint8) if keep else None
         _native.swiglu_mlp_fwd(x2, _flat(w_gate), _flat(w_up), _flat(w_down),
                                None if residual is None else _flat(residual), scale, y, saved)
@@ -768,8 +768,7 @@ def swiglu_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down
 
 @swiglu_mlp.register_fake
 def _(x, w_gate, w_up, w_down, residual, scale, keep):
-    d = x.shape[-1]
-    n = _native.swiglu_mlp_saved_bytes(x.numel() // d, d, w_gate.shape[0], x.dtype) if keep else 0
+    n = _native.swiglu_mlp_saved_bytes(x.numel() // x.shape[-1], w_gate.shape[0], x.dtype) if keep else 0
     return x.new_empty(x.shape), x.new_empty(n, dtype=torch.uint8)
 
 

@@ -245,3 +245,32 @@ def test_clip_takes_interleaved_gradients():
         assert abs(got - norm) <= STEP * norm
         want = want * (0.5 / (norm + 1e-6))
         assert ((base.double() - want).abs() <= want.abs() * (HALF[torch.float32] + 2 * STEP)).all()
+
+
+# ---------------------------------------------------------------- compilation
+def test_compiled_once_for_all_row_counts():
+    """With rows marked dynamic one compilation serves every number of rows, forward and backward."""
+    t = mlp_inputs(64, 128, 320, torch.bfloat16)
+    _, head, _ = xent_inputs(64, 128, 1000, torch.bfloat16)
+    leaves = [t[k].requires_grad_() for k in ("w_gate", "w_up", "w_down")] + [head.requires_grad_()]
+    from torch._dynamo.backends.common import aot_autograd
+    compiled = []
+
+    def backend(graph, inputs):
+        compiled.append(len(inputs))
+        return graph.forward
+
+    def f(x, target):
+        return mamba3_amd.linear_cross_entropy(mamba3_amd.swiglu_mlp(x, *leaves[:3], residual=x), head, target)
+
+    torch._dynamo.reset()
+    step = torch.compile(f, fullgraph=True, backend=aot_autograd(fw_compiler=backend))
+    for rows in (64, 3, 17, 40, 100, 257, 300, 31, 999, 1000, 8):
+        x = randn(rows, 128, dtype=torch.bfloat16, seed=rows)
+        target = torch.arange(rows, device="cuda")
+        torch._dynamo.mark_dynamic(x, 0)
+        torch._dynamo.mark_dynamic(target, 0)
+        want = torch.autograd.grad(f(x, target), leaves)
+        got = torch.autograd.grad(step(x, target), leaves)
+        assert all(torch.equal(a, b) for a, b in zip(want, got)), rows
+    assert len(compiled) == 2  # a forward and a backward graph

@@ -228,3 +228,34 @@ def test_clip_tells_large_strided_gradients_apart():
     for grads in ((m[:, :4097], m[:, 4096:8192]), (flat[::7], flat[3::11]), (m.t(), m[8191:]), (flat.as_strided((100, 100), (99, 1)),)):
         with pytest.raises(ValueError, match="overlap|share memory"):
             _refuse_shared_memory(list(grads))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_swiglu_saved_size_in_python_equals_the_librarys(lib, dtype):
+    for rows in (1, 2, 15, 16, 17, 300, 777, 4096, 8193, (1 << 20) + 3):
+        for ff in (1, 3, 4, 7, 8, 9, 15, 16, 17, 65, 320, 1363, 2112, 5504):
+            st, n = _size(lib.m3_swiglu_mlp_saved_size, rows, 64, ff, _native.dtype_code(dtype))
+            assert st == 0 and n == _native.swiglu_mlp_saved_bytes(rows, ff, dtype), (rows, ff)
+
+
+def test_swiglu_traces_with_symbolic_sizes():
+    """The ops' fake kernels keep sizes symbolic: no guard says what they are, so one trace serves all row counts."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from mamba3_amd import ops
+
+    def step(x, wg, wd):
+        y, saved = ops.swiglu_mlp(x, wg, wg, wd, None, 1.0, True)
+        return ops.swiglu_mlp_bwd(x, wg, wg, wd, 1.0, saved, y, [True, False, True, True])
+
+    bf16 = torch.bfloat16
+    env = make_fx(step, tracing_mode="symbolic")(torch.empty(300, 128, dtype=bf16), torch.empty(320, 128, dtype=bf16),
+                                                 torch.empty(128, 320, dtype=bf16)).shape_env
+    assert not env.replacements and not env.guards
+
+    def loss(hidden, weight, target):
+        out, lse, count = ops.linear_xent(hidden, weight, target, -100, 1)
+        return ops.linear_xent_bwd(hidden, weight, target, -100, 1, lse, count, out, [True, True])
+
+    env = make_fx(loss, tracing_mode="symbolic")(torch.empty(300, 128), torch.empty(1000, 128),
+                                                 torch.zeros(300, dtype=torch.long)).shape_env
+    assert not env.replacements and not env.guards
