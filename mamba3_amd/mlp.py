@@ -47,7 +47,8 @@ def swiglu_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down
         x2 = x.reshape(-1, d)
         if (ops.small_proj_usable(x2, w_gate, w_up, w_down) and _native.small_proj_ok(x2.shape[0], ff)
                 and (residual is None or residual.is_contiguous())):
-            h = ops.small_swiglu_fast(x2, None, 0.0, w_gate, w_up)
-            res = None if residual is None else residual.reshape(-1, d)
-            return ops.small_linear_fast(h, None, 0.0, w_down, res, scale).view(x.shape)
+            with ops.on_device(x):
+                h = ops.small_swiglu_fast(x2, None, 0.0, w_gate, w_up)
+                res = None if residual is None else residual.reshape(-1, d)
+                return ops.small_linear_fast(h, None, 0.0, w_down, res, scale).view(x.shape)
     return ops.swiglu_mlp_fast(x, w_gate, w_up, w_down, residual, scale, keep)

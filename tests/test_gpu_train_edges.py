@@ -274,3 +274,32 @@ def test_compiled_once_for_all_row_counts():
         got = torch.autograd.grad(step(x, target), leaves)
         assert all(torch.equal(a, b) for a, b in zip(want, got)), rows
     assert len(compiled) == 2  # a forward and a backward graph
+
+
+# ---------------------------------------------------------------- devices
+def test_few_rows_run_on_their_own_device(monkeypatch):
+    """The decode kernels that take few rows run inside ops.on_device, as the tiles do."""
+    from mamba3_amd import ops
+    t = mlp_inputs(4, 128, 320, torch.bfloat16)
+    inside, seen = [], []
+    real = ops.on_device
+
+    class Watched:
+        def __init__(self, x):
+            self.real = real(x)
+
+        def __enter__(self):
+            inside.append(1)
+            return self.real.__enter__()
+
+        def __exit__(self, *a):
+            inside.pop()
+            return self.real.__exit__(*a)
+
+    monkeypatch.setattr(ops, "on_device", Watched)
+    for name in ("small_swiglu_fast", "small_linear_fast"):
+        fn = getattr(ops, name)
+        monkeypatch.setattr(ops, name, lambda *a, fn=fn: (seen.append(len(inside)), fn(*a))[1])
+    with torch.no_grad():
+        mamba3_amd.swiglu_mlp(**t)
+    assert seen == [1, 1]
