@@ -83,6 +83,29 @@ def test_xent_ignored_rows_add_nothing_to_a_weight_that_is_not_finite(dtype, val
             assert not loss.any()
 
 
+@pytest.mark.parametrize("wanted", ["both", "hidden", "weight"])
+@pytest.mark.parametrize("rows,d,vocab,dtype,reduction", [
+    (4096, 100, 40000, torch.bfloat16, "none"), (4096, 64, 40000, torch.bfloat16, "sum"),
+    (4096, 33, 20000, torch.float32, "none"), (4100, 64, 20011, torch.float32, "mean")])
+def test_xent_pieces_of_the_vocabulary(rows, d, vocab, dtype, reduction, wanted):
+    """The backward's loop over pieces: types, reductions, widths that 16 bytes do not divide, one gradient alone."""
+    print(rows, d, vocab, dtype, reduction, wanted, flush=True)
+    n = ctypes.c_size_t(0)
+    assert _native.lib().m3_linear_xent_bwd_workspace_size(rows, d, vocab, _native.dtype_code(dtype), 0, 0, ctypes.byref(n)) == 0
+    assert n.value < rows * vocab * dtype.itemsize  # more than one piece
+    hidden, weight, target = xent_inputs(rows, d, vocab, dtype)
+    target[0] = vocab - 1
+    hidden.requires_grad_(wanted != "weight")
+    weight.requires_grad_(wanted != "hidden")
+    loss = mamba3_amd.linear_cross_entropy(hidden, weight, target, reduction=reduction)
+    grad = randn(rows, dtype=torch.float32, seed=5) if reduction == "none" else torch.tensor(1.5, device="cuda")
+    leaves = [t for t in (hidden, weight) if t.requires_grad]
+    got = dict(zip([k for k, t in (("dhidden", hidden), ("dweight", weight)) if t.requires_grad], torch.autograd.grad(loss, leaves, grad)))
+    want = dict(zip(("loss", "dhidden", "dweight"), xent_expected(hidden, weight, target, reduction, grad, dtype)))
+    for name, g in {"loss": loss, **got}.items():
+        hold(name, g, want[name])
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp32"])
 def test_xent_small_losses_of_large_logits(dtype):
     """Logits of thousands that lie a few units apart: the loss is their difference, log sum exp(z - top) + (top -
