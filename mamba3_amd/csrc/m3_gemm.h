@@ -469,6 +469,11 @@ __device__ __forceinline__ void gemm_run(const GemmGroup<kN>& grp, const Epi& ep
             return wn * FN + fn;
     };
     typename Type::Acc acc[FM][FN];
+    // fp32 tiles of few rows, next to which a library cuts k: every 512 k are summed apart, so that the error of a long
+    // k does not grow with the square root of its length. (The 128 x 128 tile has no registers for it.)
+    constexpr bool kFold = sizeof(T) == 4 && BM == 64;
+    constexpr int kFoldSteps = 16;
+    typename Type::Acc total[kFold ? FM : 1][kFold ? FN : 1];
 
     // A step is two halves of KH k steps. While one half's fragments are multiplied, the next half's
     // are read from LDS. A barrier in front of a half says that all waves have read what lies before it,
@@ -534,6 +539,12 @@ __device__ __forceinline__ void gemm_run(const GemmGroup<kN>& grp, const Epi& ep
             for (int j = 0; j < FN; ++j)
 #pragma unroll
                 for (int e = 0; e < MF * MF / 64; ++e) acc[i][j][e] = 0.f;
+        if constexpr (kFold) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) total[i][j] = typename Type::Acc{};
+        }
         wait_vm_lds<0>();  // also the last epilogue's stores, which count with the copies
         M3_LDS_FENCE();
         __builtin_amdgcn_s_barrier();
@@ -566,6 +577,18 @@ __device__ __forceinline__ void gemm_run(const GemmGroup<kN>& grp, const Epi& ep
                 }
             }
             slot = next;
+            if constexpr (kFold) {
+                if (n_steps > kFoldSteps && (n & (kFoldSteps - 1)) == 1) {
+                    asm volatile("");  // a branch: as selections the sums would wait for the products of every step
+#pragma unroll
+                    for (int i = 0; i < FM; ++i)
+#pragma unroll
+                        for (int j = 0; j < FN; ++j) {
+                            total[i][j] += acc[i][j];
+                            acc[i][j] = n > 1 ? typename Type::Acc{} : total[i][j];
+                        }
+                }
+            }
         }
         const GemmPlace<Tile, kMode> at{it.tm * BM, it.tn * (kMode == kGated ? BN / 2 : BN), wm, wn, lane};
         epi.template run<T, Tile, kMode>(at, acc, gemm_smem + Tile::kStages, it);

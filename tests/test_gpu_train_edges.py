@@ -66,6 +66,24 @@ def test_mlp_kept_gates_are_rounded_to_the_nearest():
     assert ((dg - want).abs() <= bound).all(), ((dg - want).abs() / bound).max().item()
 
 
+@pytest.mark.parametrize("rows", [8, 60])
+def test_mlp_fp32_rounding_of_a_long_sum(rows):
+    """fp32 products of few rows sum every 512 k apart. With random terms of size s the j-th partial sum is about
+    sqrt(j) s, and its rounding at most 2^-24 of it, evenly spread: a variance of (2^-23)^2 / 12 j s^2. Over blocks of n of
+    K terms that is (2^-23)^2 n / 24 of the sum's own variance K s^2, and as much for the K / n sums of blocks. (One chain
+    over all K would be off by sqrt(K / 24) 2^-23.) The up projection is seen through a gate of 32, whose silu is 32,
+    and a down projection that copies."""
+    d, ff, n = 16384, 64, 512
+    x = randn(rows, d, dtype=torch.float32, seed=1)
+    up = randn(ff, d, dtype=torch.float32, seed=2)
+    gate = torch.zeros(ff, d, device="cuda")
+    x[:, 0], gate[:, 0], up[:, 0] = 1.0, 32.0, 0.0
+    y = mamba3_amd.swiglu_mlp(x, gate, up, torch.eye(d, ff, device="cuda"))[:, :ff].double() / 32
+    want = x.double() @ up.double().t()
+    off = (y - want).square().mean().sqrt() / want.square().mean().sqrt()
+    assert off <= STEP * math.sqrt((n + d / n) / 24), off.item() / STEP
+
+
 # ---------------------------------------------------------------- the linear cross entropy
 @pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp32"])
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
