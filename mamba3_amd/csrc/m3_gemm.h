@@ -28,20 +28,13 @@ constexpr unsigned kOob = 0x80000000u;  // a byte offset past every descriptor's
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-// The MFMA of a type: MF x MF results (MF 16 or 32) of 32 or 16 k (bf16), fp32 four times 4 or 2.
+// The MFMA of a type: bf16 16 x 16 results of 32 k; fp32 MF x MF (16 or 32) of four times 4 or 2 k.
 template <typename T, int MF> struct GemmType;
 template <> struct GemmType<bf16, 16> {
     typedef bf16x8 Frag;  // 8 consecutive k of one row
     typedef f32x4 Acc;
     static __device__ __forceinline__ Acc mma(Frag b, Frag a, Acc c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, a, c, 0, 0, 0);
-    }
-};
-template <> struct GemmType<bf16, 32> {
-    typedef bf16x8 Frag;
-    typedef f32x16 Acc;
-    static __device__ __forceinline__ Acc mma(Frag b, Frag a, Acc c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(b, a, c, 0, 0, 0);
     }
 };
 template <> struct GemmType<float, 16> {
@@ -153,7 +146,7 @@ struct GemmLoader {
                 const int piece = c ^ (r & 7);
                 voff[i] = piece < pieces ? (unsigned)((r - row_shift) * ld * SZ + piece * 16) : kOob;
             } else if constexpr (SZ == 2) {
-                const int key = MF == 16 ? (r & 3) | ((r >> 3) & 3) << 2 : (r & 3) << 1 | ((r >> 3) & 1) << 3;
+                const int key = (r & 3) | ((r >> 3) & 3) << 2;
                 voff[i] = (unsigned)(r * ld * SZ + (((c >> 1) ^ (key & (BX / 16 - 1))) << 1 | (c & 1)) * 16);
             } else {
                 constexpr int U = MF / 4;  // pieces of a unit
@@ -191,12 +184,10 @@ struct GemmReader {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) off[ks] = r * 128 + (((ks * G + g) ^ (r & 7)) * 16);
         } else if constexpr (sizeof(T) == 2) {
-            // 16 lanes read a 4 x 16 block and get its columns (MF 32: lanes 0-15 and 16-31 take the
-            // two column halves of the unit)
+            // 16 lanes read a 4 x 16 block and get its columns
             const int j = lane & 15;
-            key = (MF == 16 ? (j >> 2) | g << 2 : (j >> 2) << 1 | g << 3) & (BX / 16 - 1);
+            key = ((j >> 2) | g << 2) & (BX / 16 - 1);
             off[0] = (g * 8 + (j >> 2)) * (BX * 2) + (j & 3) * 8;
-            off[1] = (lane >> 4) & 1;
         } else {
             key = g;
             off[0] = g * 4 * (BX * 4) + r * 4;
@@ -206,8 +197,7 @@ struct GemmReader {
         if constexpr (kKc) {
             return *reinterpret_cast<const Frag*>(tile + u * (MF * 128) + off[ks]);
         } else if constexpr (sizeof(T) == 2) {
-            const int unit = MF == 16 ? u : u * 2 + off[1];
-            const char* p = tile + off[0] + ((unit ^ key) << 5) + ks * (8 * G) * (BX * 2);
+            const char* p = tile + off[0] + ((u ^ key) << 5) + ks * (8 * G) * (BX * 2);
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                 (__attribute__((address_space(3))) s16x4*)(p + 4 * (BX * 2)));
@@ -239,7 +229,7 @@ struct GemmTile {
     static constexpr int kStages = STAGES * kStageBytes;
     static constexpr int kEpi = MF == 32 ? WGN * BM * 8 : NW * MF * (FN * MF * 2 + 16);
     static constexpr int kLds = kStages + kEpi;
-    typedef typename GemmType<bf16, MF>::Acc Acc;
+    typedef typename GemmType<float, MF>::Acc Acc;
 };
 
 // Where a wave's accumulators lie: piece (fm, fn), four q, lane: row m(fm), columns n(fn, q) ..

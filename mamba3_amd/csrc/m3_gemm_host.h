@@ -35,6 +35,23 @@ inline int64_t gemm_pad(int64_t n, int dtype) {  // to 16 bytes
 }
 inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
+// A running pointer through the workspace.
+struct Bump {
+    char* p;
+    size_t used = 0;
+    void* take(int64_t bytes) {
+        void* r = p ? p + used : nullptr;
+        used += (size_t)up256(bytes);
+        return r;
+    }
+};
+
+#define M3_TRY(e)                       \
+    do {                                \
+        const int st_ = (e);            \
+        if (st_ != M3_OK) return st_;   \
+    } while (0)
+
 // Launches k over the items of a group: as many blocks as run at once, each takes every grid-th item.
 template <typename Tile, int kN, typename... Rest>
 int gemm_launch_group(void (*k)(GemmGroup<kN>, Rest...), GemmGroup<kN> g, const int64_t (&rows)[kN], const int64_t (&cols)[kN],

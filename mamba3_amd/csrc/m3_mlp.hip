@@ -197,17 +197,6 @@ MlpShape mlp_shape(int64_t rows, int64_t d, int64_t ff, int dtype) {
     return s;
 }
 
-// A running pointer through the workspace.
-struct Bump {
-    char* p;
-    size_t used = 0;
-    void* take(int64_t bytes) {
-        void* r = p ? p + used : nullptr;
-        used += (size_t)up256(bytes);
-        return r;
-    }
-};
-
 struct MlpFwd {
     GemmPlan up, down;
     void *x, *wg, *wu, *wd, *h;
@@ -287,12 +276,6 @@ size_t swiglu_fwd_workspace(int64_t rows, int64_t d, int64_t ff, int dtype, bool
 size_t swiglu_bwd_workspace(int64_t rows, int64_t d, int64_t ff, int dtype) {
     return mlp_bwd_layout(mlp_shape(rows, d, ff, dtype), nullptr).bytes;
 }
-
-#define M3_TRY(e)                       \
-    do {                                \
-        const int st_ = (e);            \
-        if (st_ != M3_OK) return st_;   \
-    } while (0)
 
 int launch_swiglu_fwd(int64_t rows, int64_t d, int64_t ff, int dtype, const void* x, const void* wg, const void* wu,
                       const void* wd, const void* res, float scale, void* y, void* saved, void* ws,

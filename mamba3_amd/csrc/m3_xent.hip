@@ -284,16 +284,6 @@ __global__ __launch_bounds__(256) void xent_total_kernel(const double* __restric
 
 namespace {
 
-struct Bump {
-    char* p;
-    size_t used = 0;
-    void* take(int64_t bytes) {
-        void* r = p ? p + used : nullptr;
-        used += (size_t)up256(bytes);
-        return r;
-    }
-};
-
 struct XentFwd {
     GemmPlan z;
     int tiles;
@@ -350,12 +340,6 @@ XentBwd xent_bwd_layout(int64_t rows, int64_t d, int64_t vocab, int dtype, bool 
 }
 
 }  // namespace
-
-#define M3_TRY(e)                       \
-    do {                                \
-        const int st_ = (e);            \
-        if (st_ != M3_OK) return st_;   \
-    } while (0)
 
 size_t xent_fwd_workspace(int64_t rows, int64_t d, int64_t vocab, int dtype) {
     return xent_fwd_layout(rows, d, vocab, dtype, nullptr).bytes;
