@@ -21,8 +21,9 @@ struct GemmPlan {
     int bm, bn;
 };
 
-// search_plan (m3_gemm_plan.h), kept for the next calls of the same sizes.
+// search_plan and pair_plan (m3_gemm_plan.h), kept for the next calls of the same sizes.
 GemmGroupPlan gemm_group_plan(int dtype, const GemmTask* tasks, int n);
+GemmPairPlan gemm_pair_plan(int dtype, const GemmTask (&tasks)[2]);
 GemmPlan gemm_plan(int dtype, int64_t rows, int64_t cols, int64_t steps, int max_splits);
 
 inline int64_t gemm_steps(int64_t k, int dtype) {

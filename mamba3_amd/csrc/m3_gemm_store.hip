@@ -279,30 +279,46 @@ int gemm_pad_copy(int dtype, const GemmPads& pads, const int64_t* target, int64_
     return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH;
 }
 
-// The search takes 20 us of host time, and a call asks three times (the workspace's size, its check, the
-// launch): each thread keeps its last plans.
-GemmGroupPlan gemm_group_plan(int dtype, const GemmTask* tasks, int n) {
+// A search takes 20 us of host time or more, and a call asks three times (the workspace's size, its check, the
+// launch): each thread keeps its last plans, in any of four places that follow a hash of their tasks.
+template <typename Plan, typename F>
+static const Plan& kept_plan(int dtype, const GemmTask* tasks, int n, F search) {
     struct Kept {
         int dtype = -1, n = 0;
         GemmTask t[kGroupMax];
-        GemmGroupPlan plan;
+        Plan plan;
     };
     static thread_local Kept kept[64];
+    static thread_local unsigned turn = 0;
     uint64_t h = (uint64_t)dtype * 31 + (uint64_t)n;
     for (int p = 0; p < n; ++p)
         h = (h * 0x9e3779b97f4a7c15ull + (uint64_t)tasks[p].rows * 3 + (uint64_t)tasks[p].cols * 5 + (uint64_t)tasks[p].steps * 7) ^ (h >> 29);
-    Kept& k = kept[h >> 58];
     auto same = [](const GemmTask& a, const GemmTask& b) {
         return a.rows == b.rows && a.cols == b.cols && a.steps == b.steps && a.max_splits == b.max_splits && a.tn == b.tn;
     };
-    bool hit = k.dtype == dtype && k.n == n;
-    for (int p = 0; hit && p < n; ++p) hit = same(k.t[p], tasks[p]);
-    if (!hit) {
-        k.plan = search_plan(dtype == M3_DTYPE_BF16, tasks, n);
-        k.dtype = dtype, k.n = n;
-        for (int p = 0; p < n; ++p) k.t[p] = tasks[p];
+    Kept* at = nullptr;
+    for (unsigned i = 0; i < 4; ++i) {
+        Kept& k = kept[((h >> 58) + i) & 63];
+        bool hit = k.dtype == dtype && k.n == n;
+        for (int p = 0; hit && p < n; ++p) hit = same(k.t[p], tasks[p]);
+        if (hit) return k.plan;
+        if (!at && k.n == 0) at = &k;
     }
-    return k.plan;
+    if (!at) at = &kept[((h >> 58) + turn++ % 4) & 63];
+    at->plan = search();
+    at->dtype = dtype, at->n = n;
+    for (int p = 0; p < n; ++p) at->t[p] = tasks[p];
+    return at->plan;
+}
+
+GemmGroupPlan gemm_group_plan(int dtype, const GemmTask* tasks, int n) {
+    return kept_plan<GemmGroupPlan>(dtype, tasks, n, [&] { return search_plan(dtype == M3_DTYPE_BF16, tasks, n); });
+}
+
+GemmPairPlan gemm_pair_plan(int dtype, const GemmTask (&tasks)[2]) {
+    return kept_plan<GemmPairPlan>(dtype, tasks, 2, [&] {
+        return pair_plan(tasks, [&](const GemmTask (&t)[2]) { return search_plan(dtype == M3_DTYPE_BF16, t, 2); });
+    });
 }
 
 GemmPlan gemm_plan(int dtype, int64_t rows, int64_t cols, int64_t steps, int max_splits) {

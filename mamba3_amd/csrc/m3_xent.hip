@@ -328,7 +328,7 @@ XentBwd xent_bwd_layout(int64_t rows, int64_t d, int64_t vocab, int dtype, bool 
     f.z = gemm_plan(dtype, rows, f.piece, gemm_steps(d, dtype), 1);
     const GemmTask tasks[2] = {{want_dh ? rows : 0, d, gemm_steps(f.piece, dtype), kMostSplits, false},
                                {want_dw ? f.piece : 0, d, gemm_steps(rows, dtype), kMaxSplits, true}};
-    f.grads = pair_plan(tasks, [&](const GemmTask (&t)[2]) { return gemm_group_plan(dtype, t, 2); });
+    f.grads = gemm_pair_plan(dtype, tasks);
     const int dh_splits = f.grads.p[0].splits[0];
     f.h = b.take(rows * dp * size);
     f.w = dp != d ? b.take(vocab * dp * size) : nullptr;
