@@ -11,12 +11,13 @@
 // the two gradient products on it: dW's rows of the piece are final, dh is summed over the
 // pieces in fp32. Recomputing z costs 2 M V d operations (a quarter of the pass) and keeps the memory at one piece.
 //
-// Measured, bf16, forward + backward: 8192 rows, d 768, 32000 tokens 1.61 ms (z 381 us, dz in two pieces
-// 232 us each, gradients 370 us each and 27 for dW's two parts: 1,000 TF/s); 4096 rows, d 2048, 128000 tokens
-// 6.74 ms (1,669, 4 x 446, 4 x 798: 1,275 TF/s). Bound by the MFMAs, and over short k by the epilogues,
+// Measured, bf16, forward + backward: 8192 rows, d 768, 32000 tokens 1.48 - 1.57 ms (z 381 - 398 us, dz in two pieces
+// 234 us each, gradients 360 us each and 18 for dh's parts: 1,050 TF/s); 4096 rows, d 2048, 128000 tokens
+// 6.6 - 6.9 ms (1,701, 4 x 454, 4 x 811: 1,260 TF/s). Bound by the MFMAs, and over short k by the epilogues,
 // which a CU's one block of 256 x 256 does not overlap with products: at d 768 an exponential for each
 // 768 multiply-adds. Two blocks of 128 x 128 overlap them and are slower: z 446 - 464 us, dz 309 - 316.
-// Pieces of 256 MiB: two of 16128 columns at the first size.
+// Pieces of 256 MiB: two of 16128 columns at the first size. 16 rows, d 2048, 128000 tokens, fp32: 1.2 ms (z 335 and
+// 311 us, dh 318, dW 354: 64-row tiles a quarter full, and 1 GB written).
 //
 // Rows whose target is ignored count nowhere: their loss and dz are zero by selection, and
 // products over rows read them as zeros, whatever the row holds. A target outside [0, V) that is
