@@ -87,9 +87,10 @@ def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm:
     """Scales the gradients of `parameters` in place by min(1, max_norm / (norm + 1e-6)) and returns
     norm, the norm of all their elements together before that (an fp32 scalar on their GPU): the
     2-norm, or for norm_type inf the largest absolute value. Gradients are fp32 or bf16, in any
-    mixture, on one GPU; parameters without one are left out, and one that is listed twice counts
-    once; gradients that share memory otherwise are refused. Nothing waits for the GPU, unless error_if_nonfinite asks to raise, before anything is
-    scaled, where the norm is NaN or infinite; otherwise such a norm scales by NaN or 0."""
+    mixture, on one GPU; parameters without one are left out, one that is listed twice counts
+    once, and gradients that share memory otherwise are refused. Nothing waits for the GPU, unless
+    error_if_nonfinite asks to raise, before anything is scaled, where the norm is NaN or infinite;
+    otherwise such a norm scales by NaN or 0."""
     params = (parameters,) if isinstance(parameters, torch.Tensor) else parameters
     # A model has hundreds of small gradients: each of these passes over them is one C call per tensor.
     grads = [g for g in [p.grad for p in params] if g is not None]

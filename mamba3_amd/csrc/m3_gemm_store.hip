@@ -158,9 +158,9 @@ static int launch_grads(const GemmGroup<kGroupMax>& grp, const EpiStore<kGroupMa
 }
 
 // The products share one launch: what one of them leaves of the last round of tiles the next one takes,
-// and there is one reduction. The four products of 8192 x 768 x 2112 take 192 us apart and 165 together,
-// with their reductions (12 us): 133 GFLOP at 870 TF/s in the products' launch; of 8192 x 2048 x 5504
-// 740 us, 1,250 TF/s. Bound by the MFMAs, and at the smaller size by the parts of k, whose fp32 sums are
+// and there is one reduction. The four products of 8192 x 768 x 2112 take 192 us apart and 161 together,
+// with their reductions (12 us): 133 GFLOP at 890 TF/s in the products' launch; of 8192 x 2048 x 5504
+// 757 us, 1,220 TF/s. Bound by the MFMAs, and at the smaller size by the parts of k, whose fp32 sums are
 // written and read.
 int gemm_grads(int dtype, const GemmGroupPlan& plan, GemmGrads g, hipStream_t stream) {
     GemmGroup<kGroupMax> grp;

@@ -8,10 +8,10 @@
 // epilogue reads g and u and writes dg and du, the operands of the four gradient products, which
 // are one launch (dx is one product of two terms).
 //
-// Measured, bf16, 8192 rows, d 768, ff 2112 (forward + backward 346 us, 239 GFLOP): gated product 73 us,
-// down 46, dh 67, gradients 165; d 2048, ff 5504 (1.49 ms, 1,120 TF/s): 329, 167, 226, 766. Bound by
-// the MFMAs; the small size by 4.1 and 2.1 rounds of tiles that take 5 and 3, and by the kept values'
-// bytes next to twelve k steps a tile.
+// Measured, bf16, 8192 rows, d 768, ff 2112 (forward + backward 347 - 362 us, 239 GFLOP): gated product 75 us,
+// down 48, dh 67, gradients 149 and their sums 12; d 2048, ff 5504 (1.47 - 1.53 ms, 1,110 TF/s): 333, 167, 229, 757
+// and 27. Bound by the MFMAs; the small size by 4.1 and 2.1 rounds of tiles that take 5 and 3, and by the kept
+// values' bytes next to twelve k steps a tile.
 //
 // For the backward the forward keeps g and u. bf16: rounded to 24 bits (the upper 16 of each, and the
 // next 8 of both in another 16), a relative 2^-16: a bf16 copy alone would put a rounding
