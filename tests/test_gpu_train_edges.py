@@ -344,3 +344,43 @@ def test_few_rows_run_on_their_own_device(monkeypatch):
     with torch.no_grad():
         mamba3_amd.swiglu_mlp(**t)
     assert seen == [1, 1]
+
+
+# ---------------------------------------------------------------- graphs
+@pytest.mark.parametrize("rows,d,vocab,dtype", [(16, 256, 50021, torch.float32), (4096, 100, 40000, torch.bfloat16)])
+def test_captured_loss_replays(rows, d, vocab, dtype):
+    """Two captured losses with their gradients, one after the other, between eager ones: few rows (dh and dW in launches
+    of their own, dh in parts) and several pieces of the vocabulary (sums kept from piece to piece)."""
+    print(rows, d, vocab, dtype, flush=True)
+
+    def run(h, w, t):
+        loss = mamba3_amd.linear_cross_entropy(h, w, t)
+        return [loss.detach(), *torch.autograd.grad(loss, [h, w])]
+
+    inputs = {s: xent_inputs(rows, d, vocab, dtype, seed=s) for s in (0, 10, 20)}
+    for h, w, t in inputs.values():
+        t[0] = 5
+    eager = {s: run(h.clone().requires_grad_(), w.clone().requires_grad_(), t) for s, (h, w, t) in inputs.items()}
+    graphs = []
+    for _ in range(2):
+        h, w, t = (v.clone() for v in inputs[0])
+        h.requires_grad_(), w.requires_grad_()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run(h, w, t)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run(h, w, t)
+        graphs.append((graph, (h, w, t), out))
+    for seeds in ((10, 20), (20, 0), (0, 10)):
+        for (graph, own, out), s in zip(graphs, seeds):
+            for a, b in zip(own, inputs[s]):
+                with torch.no_grad():
+                    a.copy_(b)
+            graph.replay()
+        torch.cuda.synchronize()
+        for (graph, own, out), s in zip(graphs, seeds):
+            assert all(torch.equal(a, b) for a, b in zip(out, eager[s]))
+        run(*(v.clone().requires_grad_() if v.is_floating_point() else v for v in inputs[0]))
