@@ -238,13 +238,13 @@ def _plain_sample(st):
     before = among.cumsum(1)
     kept &= (before - among < p * before[:, -1:]) | (p >= 1)
     kept[:, 0] = True
-    w = torch.zeros_like(mass).scatter_(1, order, torch.where(kept, mass, 0.0)).cumsum(1)
-    picked = (w <= st["u"].double()[:, None] * w[:, -1:]).sum(1)
-    token = torch.where(t[:, 0] > 0, picked, order[:, 0])
+    w = torch.where(kept, mass, 0.0).cumsum(1)  # from the likeliest token down, ties from the lowest index
+    place = torch.where(t > 0, (w <= st["u"].double()[:, None] * w[:, -1:]).sum(1, keepdim=True), 0)
+    token = order.gather(1, place)[:, 0]
     if not st["logprob"]:
         return {"token": token}
     # among what was kept; a greedy choice is certain
-    gap = (st["logits"].double().gather(1, token[:, None]) - top) / t
+    gap = (z.gather(1, place) - top) / t
     return {"token": token, "logprob": torch.where(t > 0, gap - w[:, -1:].log(), 0.0)[:, 0].float()}
 
 
@@ -377,9 +377,7 @@ def exact(case, seed):
     share = ranked.cumsum(1)
     share = share / share.gather(1, setting["top_k"].long().clamp(max=case["vocab"]) - 1)
     count = torch.minimum(count, 1 + (share < setting["top_p"]).sum(1, keepdim=True)).clamp(min=1, max=case["vocab"])
-    place = torch.empty_like(order).scatter_(1, order, torch.arange(case["vocab"], device=order.device).expand_as(order))
-    left = torch.where(place < count, prob, 0.0)
+    left = torch.where(torch.arange(case["vocab"], device=order.device) < count, ranked, 0.0)
     left = left / left.sum(1, keepdim=True)
-    token = torch.searchsorted(left.cumsum(1), st["u"].double()[:, None], right=True).clamp(max=case["vocab"] - 1)
-    # rounding of probabilities may part tokens of one logit from their order: their log probabilities are the same
-    return {"token": None, "logprob": torch.where(greedy, 0.0, left.gather(1, token).log()[:, 0])}
+    at = torch.searchsorted(left.cumsum(1), st["u"].double()[:, None], right=True).clamp(max=case["vocab"] - 1)
+    return {"token": None, "logprob": torch.where(greedy, 0.0, left.gather(1, at).log()[:, 0])}
