@@ -471,6 +471,73 @@ int m3_clip_grad_norm(int32_t n, void* const* tensors, const int64_t* numel, con
                       int32_t norm_kind, int32_t scale, float max_norm, float* norm, void* workspace,
                       size_t workspace_bytes, void* stream);
 
+/* Element types of microscaled values: 4 bits (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) or 8 (to 448). */
+enum m3_mx_format {
+    M3_MX_E2M1 = 0,
+    M3_MX_E4M3 = 1
+};
+
+/*
+ * Microscaled values: blocks of 32 along a row of k share a power of two 2^E; value = element * 2^E. A row is
+ * stored as kp elements, kp = k rounded up to 128 (zeros behind k): data [rows, kp] bytes (e4m3) or
+ * [rows, kp / 2] (e2m1, the even k in the low half of a byte), 16-byte aligned; scales [rows, kp / 32] bytes
+ * E + 127, 4-byte aligned, 255 for a block that held an infinity or NaN (it is NaN). E is the smallest exponent,
+ * from -127 on, under which the block's largest magnitude rounds to an element (none saturates); 0 for a block
+ * of zeros. Elements round to nearest, ties to even.
+ * m3_mx_quantize: x [rows, k], or with `gated` of silu(x[:, :k]) * x[:, k:] for x [rows, 2 k] (computed in fp32,
+ * mamba3/block.py:16-26). m3_mx_dequantize: out [rows, k] (exact in bf16 but for results below 2^-126 or past the largest number).
+ * rows <= 2^32, k <= 2^24.
+ */
+int m3_mx_quantize(int64_t rows, int32_t k, int32_t dtype, int32_t gated, int32_t format, const void* x, void* data,
+                   void* scales, void* stream);
+int m3_mx_dequantize(int64_t rows, int32_t k, int32_t format, int32_t dtype, const void* data, const void* scales, void* out,
+                     void* stream);
+
+/*
+ * The residual's addition (mamba3/block.py:84-91) and the norm behind it (mamba3/mamba3.py:19-35) in one pass:
+ *   total = residual + scale * x (stored in the inputs' type), r = 1 / sqrt(mean total^2 + eps), y = total r weight
+ * x, residual, total, y [rows, d], weight [d], all of one dtype; y is rounded once. rstd [rows] (r, or NULL) is
+ * for the backward. m3_add_rmsnorm_mx writes y as microscaled values; there residual and total may both be
+ * NULL (total = x).
+ * Backward, with g = weight dy: dt = dtotal + r g - total r^3 sum(g total) / d; dresidual = dt, dx = scale dt,
+ * dweight = sum over rows of dy total r. dtotal may be NULL (zeros); any of the results may be. Sums run in a fixed
+ * order. workspace (for dweight): 256-byte aligned. rows <= 2^32, d <= 2^24.
+ */
+int m3_add_rmsnorm_fwd(int64_t rows, int32_t d, int32_t dtype, const void* x, const void* residual, const void* weight,
+                       float scale, float eps, void* total, void* y, float* rstd, void* stream);
+int m3_add_rmsnorm_mx(int64_t rows, int32_t d, int32_t dtype, const void* x, const void* residual, const void* weight,
+                      float scale, float eps, void* total, int32_t format, void* data, void* scales, void* stream);
+int m3_add_rmsnorm_bwd_workspace_size(int64_t rows, int32_t d, size_t* bytes);
+int m3_add_rmsnorm_bwd(int64_t rows, int32_t d, int32_t dtype, const void* total, const void* weight, const float* rstd,
+                       const void* dtotal, const void* dy, float scale, void* dx, void* dresidual, void* dweight,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * out = [residual +] scale * (x w^T) for microscaled x [rows, k] (either format) and w [n, k] (e2m1); residual and
+ * out [rows, n] in out_dtype. bf16 results come from the instructions that take the elements and scales as they
+ * are, whose sums align e4m3 products at about 2^-13 of the largest of 128; fp32 results from bf16
+ * instructions (the elements with their scales are exact in bf16) with fp32 sums. rows, n <= 2^26, k <= 2^20.
+ */
+int m3_mx_linear(int64_t rows, int32_t n, int32_t k, int32_t x_format, int32_t out_dtype, const void* x_data,
+                 const void* x_scales, const void* w_data, const void* w_scales, const void* residual, float scale, void* out,
+                 void* stream);
+
+/*
+ * The next token of each row of logits [rows, vocab] from a random number u [rows] in [0, 1) (mamba3/block.py:208-222
+ * draws with torch.multinomial). Tokens are ordered by logit, ties from the lowest index. With masses
+ * exp((z - max z) / temperature), kept are the first top_k tokens (0: all), of these the shortest run from the first on whose mass
+ * reaches top_p of theirs (1: all, 0: the first), and of these the ones with at least min_p of the first's mass.
+ * token = the first kept one whose running mass passes u times the kept mass; logprob (or NULL) the log of
+ * its share. A temperature of 0 (or below, or NaN) takes the first token (logprob 0). NaN counts as
+ * -infinity, which is no token: a row without any gives -1 (logprob NaN). u outside [0, 1) is taken to its ends.
+ * Each setting is the array's [rows] entry, or where that is NULL the number. vocab <= 2^22. workspace: 256-byte aligned.
+ */
+int m3_sample_tokens_workspace_size(int64_t rows, int32_t vocab, size_t* bytes);
+int m3_sample_tokens(int64_t rows, int32_t vocab, int32_t dtype, const void* logits, const float* u, const float* temperatures,
+                     double temperature, const int32_t* top_ks, int64_t top_k, const float* top_ps, double top_p,
+                     const float* min_ps, double min_p, int64_t* token, float* logprob, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -58,6 +58,15 @@ EXPORTED_SYMBOLS = (
     "m3_linear_xent_bwd",
     "m3_clip_grad_norm_workspace_size",
     "m3_clip_grad_norm",
+    "m3_mx_quantize",
+    "m3_mx_dequantize",
+    "m3_add_rmsnorm_fwd",
+    "m3_add_rmsnorm_mx",
+    "m3_add_rmsnorm_bwd_workspace_size",
+    "m3_add_rmsnorm_bwd",
+    "m3_mx_linear",
+    "m3_sample_tokens_workspace_size",
+    "m3_sample_tokens",
 )
 
 M3_ERR_UNSUPPORTED = 3
@@ -189,7 +198,17 @@ def _declare(lib: ctypes.CDLL) -> None:
             ("m3_linear_xent_bwd_workspace_size", [*dims, _i32, _i32, size_p]),
             ("m3_linear_xent_bwd", [*dims, _i32] + [_vp] * 3 + [_i64] + [_vp] * 6 + [ctypes.c_size_t, _vp]),
             ("m3_clip_grad_norm_workspace_size", [_i32, _vp, _vp, size_p]),
-            ("m3_clip_grad_norm", [_i32, _vp, _vp, _vp, _i32, _i32, f32] + [_vp] * 2 + [ctypes.c_size_t, _vp])):
+            ("m3_clip_grad_norm", [_i32, _vp, _vp, _vp, _i32, _i32, f32] + [_vp] * 2 + [ctypes.c_size_t, _vp]),
+            ("m3_mx_quantize", [_i64] + [_i32] * 4 + [_vp] * 4),
+            ("m3_mx_dequantize", [_i64] + [_i32] * 3 + [_vp] * 4),
+            ("m3_add_rmsnorm_fwd", [_i64, _i32, _i32] + [_vp] * 3 + [f32, f32] + [_vp] * 4),
+            ("m3_add_rmsnorm_mx", [_i64, _i32, _i32] + [_vp] * 3 + [f32, f32, _vp, _i32] + [_vp] * 3),
+            ("m3_add_rmsnorm_bwd_workspace_size", [_i64, _i32, size_p]),
+            ("m3_add_rmsnorm_bwd", [_i64, _i32, _i32] + [_vp] * 5 + [f32] + [_vp] * 4 + [ctypes.c_size_t, _vp]),
+            ("m3_mx_linear", [_i64] + [_i32] * 4 + [_vp] * 5 + [f32] + [_vp] * 2),
+            ("m3_sample_tokens_workspace_size", [_i64, _i32, size_p]),
+            ("m3_sample_tokens", [_i64, _i32, _i32, _vp, _vp, _vp, ctypes.c_double, _vp, _i64, _vp, ctypes.c_double, _vp,
+                                  ctypes.c_double, _vp, _vp, _vp, ctypes.c_size_t, _vp])):
         fn = getattr(lib, name)
         fn.restype, fn.argtypes = ctypes.c_int, args
 
@@ -547,3 +566,85 @@ def clip_grad_norm(ptrs, numel, dtypes, kind: int, max_norm: float | None, norm)
     if st == M3_ERR_OVERLAP:
         raise ValueError("gradients that overlap in memory cannot be clipped in place")
     check(st, "m3_clip_grad_norm")
+
+
+# ---------------------------------------------------------------- 4-bit serving
+MX_FORMATS = {"e2m1": 0, "e4m3": 1}
+
+
+def mx_padded(k: int) -> int:
+    """Elements of a stored row of k microscaled values."""
+    return -(-k // 128) * 128
+
+
+def mx_row_bytes(k: int, fmt: str) -> int:
+    return mx_padded(k) if fmt == "e4m3" else mx_padded(k) // 2
+
+
+def mx_quantize(x, fmt: str, gated: bool, data, scales) -> None:
+    """m3_mx_quantize on contiguous x (rows, k), or (rows, 2 k) when gated."""
+    rows, k = x.shape
+    st = lib().m3_mx_quantize(rows, k // 2 if gated else k, dtype_code(x.dtype), int(gated), MX_FORMATS[fmt],
+                              x.data_ptr(), data.data_ptr(), scales.data_ptr(), stream_of(x))
+    if st:
+        check(st, "m3_mx_quantize")
+
+
+def mx_dequantize(data, scales, fmt: str, out) -> None:
+    """m3_mx_dequantize into contiguous out (rows, k)."""
+    rows, k = out.shape
+    st = lib().m3_mx_dequantize(rows, k, MX_FORMATS[fmt], dtype_code(out.dtype), data.data_ptr(), scales.data_ptr(),
+                                out.data_ptr(), stream_of(out))
+    if st:
+        check(st, "m3_mx_dequantize")
+
+
+def add_rmsnorm_fwd(x, residual, weight, scale: float, eps: float, total, y, rstd) -> None:
+    """m3_add_rmsnorm_fwd on contiguous (rows, d) tensors."""
+    rows, d = x.shape
+    st = lib().m3_add_rmsnorm_fwd(rows, d, dtype_code(x.dtype), x.data_ptr(), residual.data_ptr(), weight.data_ptr(),
+                                  scale, eps, total.data_ptr(), y.data_ptr(), ptr(rstd), stream_of(x))
+    if st:
+        check(st, "m3_add_rmsnorm_fwd")
+
+
+def add_rmsnorm_mx(x, residual, weight, scale: float, eps: float, total, fmt: str, data, scales) -> None:
+    """m3_add_rmsnorm_mx on contiguous (rows, d) tensors."""
+    rows, d = x.shape
+    st = lib().m3_add_rmsnorm_mx(rows, d, dtype_code(x.dtype), x.data_ptr(), ptr(residual), weight.data_ptr(), scale,
+                                 eps, ptr(total), MX_FORMATS[fmt], data.data_ptr(), scales.data_ptr(), stream_of(x))
+    if st:
+        check(st, "m3_add_rmsnorm_mx")
+
+
+def add_rmsnorm_bwd(total, weight, rstd, dtotal, dy, scale: float, dx, dresidual, dweight) -> None:
+    """m3_add_rmsnorm_bwd on contiguous (rows, d) tensors; allocates the workspace."""
+    rows, d = total.shape
+    n = _bytes_of("m3_add_rmsnorm_bwd_workspace_size", rows, d) if dweight is not None else 0
+    ws = _workspace(n, total.device)
+    check(lib().m3_add_rmsnorm_bwd(rows, d, dtype_code(total.dtype), ptr(total), ptr(weight), ptr(rstd), ptr(dtotal),
+                                   ptr(dy), scale, ptr(dx), ptr(dresidual), ptr(dweight), ptr(ws), n,
+                                   stream_of(total)), "m3_add_rmsnorm_bwd")
+
+
+def mx_linear(x_data, x_scales, x_format: str, w_data, w_scales, k: int, residual, scale: float, out) -> None:
+    """m3_mx_linear into contiguous out (rows, n)."""
+    rows, n = out.shape
+    st = lib().m3_mx_linear(rows, n, k, MX_FORMATS[x_format], dtype_code(out.dtype), x_data.data_ptr(), x_scales.data_ptr(),
+                            w_data.data_ptr(), w_scales.data_ptr(), ptr(residual), scale, out.data_ptr(), stream_of(out))
+    if st:
+        check(st, "m3_mx_linear")
+
+
+def sample_tokens(logits, u, temperature, top_k, top_p, min_p, token, logprob) -> None:
+    """m3_sample_tokens on contiguous logits (rows, vocab); settings are numbers or tensors (rows,), fp32 or for
+    top_k int32. Allocates the workspace."""
+    rows, vocab = logits.shape
+    n = _bytes_of("m3_sample_tokens_workspace_size", rows, vocab)
+    ws = _workspace(n, logits.device)
+    args = []
+    for v in (temperature, top_k, top_p, min_p):
+        args += [v.data_ptr(), 0] if isinstance(v, torch.Tensor) else [None, v]
+    check(lib().m3_sample_tokens(rows, vocab, dtype_code(logits.dtype), logits.data_ptr(), u.data_ptr(), *args,
+                                 token.data_ptr(), ptr(logprob), ws.data_ptr(), n, stream_of(logits)),
+          "m3_sample_tokens")

@@ -769,4 +769,126 @@ int m3_clip_grad_norm(int32_t n, void* const* tensors, const int64_t* numel, con
                            workspace, as_stream(stream));
 }
 
+// ---- 4-bit serving
+static int check_mx(int64_t rows, int64_t k, int32_t format) {
+    if (rows <= 0 || k <= 0) return M3_ERR_INVALID_SHAPE;
+    if (rows > ((int64_t)1 << 32) || k > (1 << 24) || rows > ((int64_t)1 << 50) / k) return M3_ERR_UNSUPPORTED;
+    return format == M3_MX_E2M1 || format == M3_MX_E4M3 ? M3_OK : M3_ERR_UNSUPPORTED;
+}
+static int check_dtype(int32_t dtype) {
+    return dtype == M3_DTYPE_F32 || dtype == M3_DTYPE_BF16 ? M3_OK : M3_ERR_UNSUPPORTED;
+}
+static int size_of(int32_t dtype) { return dtype == M3_DTYPE_BF16 ? 2 : 4; }
+
+int m3_mx_quantize(int64_t rows, int32_t k, int32_t dtype, int32_t gated, int32_t format, const void* x, void* data,
+                   void* scales, void* stream) {
+    if (!x || !data || !scales) return M3_ERR_NULL_POINTER;
+    int st = check_mx(rows, k, format);
+    if (st == M3_OK) st = check_dtype(dtype);
+    if (st != M3_OK) return st;
+    if (!aligned(x, size_of(dtype)) || !aligned(data, 16) || !aligned(scales, 4)) return M3_ERR_MISALIGNED;
+    return m3::launch_mx_quantize(x, dtype, gated != 0, format, data, scales, rows, k, as_stream(stream));
+}
+
+int m3_mx_dequantize(int64_t rows, int32_t k, int32_t format, int32_t dtype, const void* data, const void* scales, void* out,
+                     void* stream) {
+    if (!data || !scales || !out) return M3_ERR_NULL_POINTER;
+    int st = check_mx(rows, k, format);
+    if (st == M3_OK) st = check_dtype(dtype);
+    if (st != M3_OK) return st;
+    if (!aligned(data, 16) || !aligned(scales, 4) || !aligned(out, size_of(dtype))) return M3_ERR_MISALIGNED;
+    return m3::launch_mx_dequantize(data, scales, format, out, dtype, rows, k, as_stream(stream));
+}
+
+int m3_add_rmsnorm_fwd(int64_t rows, int32_t d, int32_t dtype, const void* x, const void* residual, const void* weight,
+                       float scale, float eps, void* total, void* y, float* rstd, void* stream) {
+    if (!x || !residual || !weight || !total || !y) return M3_ERR_NULL_POINTER;
+    int st = check_mx(rows, d, M3_MX_E4M3);
+    if (st == M3_OK) st = check_dtype(dtype);
+    if (st != M3_OK) return st;
+    for (const void* p : {x, residual, weight, (const void*)total, (const void*)y})
+        if (!aligned(p, size_of(dtype))) return M3_ERR_MISALIGNED;
+    return m3::launch_add_norm(x, residual, weight, dtype, scale, eps, total, y, rstd, rows, d, as_stream(stream));
+}
+
+int m3_add_rmsnorm_mx(int64_t rows, int32_t d, int32_t dtype, const void* x, const void* residual, const void* weight,
+                      float scale, float eps, void* total, int32_t format, void* data, void* scales, void* stream) {
+    if (!x || !weight || !data || !scales || (residual != nullptr) != (total != nullptr)) return M3_ERR_NULL_POINTER;
+    int st = check_mx(rows, d, format);
+    if (st == M3_OK) st = check_dtype(dtype);
+    if (st != M3_OK) return st;
+    for (const void* p : {x, residual, weight, (const void*)total})
+        if (p && !aligned(p, size_of(dtype))) return M3_ERR_MISALIGNED;
+    if (!aligned(data, 16) || !aligned(scales, 4)) return M3_ERR_MISALIGNED;
+    return m3::launch_add_norm_mx(x, residual, weight, dtype, scale, eps, total, format, data, scales, rows, d, as_stream(stream));
+}
+
+int m3_add_rmsnorm_bwd_workspace_size(int64_t rows, int32_t d, size_t* bytes) {
+    if (!bytes) return M3_ERR_NULL_POINTER;
+    const int st = check_mx(rows, d, M3_MX_E4M3);
+    if (st == M3_OK) *bytes = m3::add_norm_bwd_workspace(rows, d);
+    return st;
+}
+
+int m3_add_rmsnorm_bwd(int64_t rows, int32_t d, int32_t dtype, const void* total, const void* weight, const float* rstd,
+                       const void* dtotal, const void* dy, float scale, void* dx, void* dresidual, void* dweight,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+    if (!total || !weight || !rstd || !dy) return M3_ERR_NULL_POINTER;
+    int st = check_mx(rows, d, M3_MX_E4M3);
+    if (st == M3_OK) st = check_dtype(dtype);
+    if (st != M3_OK) return st;
+    for (const void* p : {total, weight, dtotal, dy, (const void*)dx, (const void*)dresidual, (const void*)dweight})
+        if (p && !aligned(p, size_of(dtype))) return M3_ERR_MISALIGNED;
+    if (!dx && !dresidual && !dweight) return M3_OK;
+    if (dweight) {
+        st = check_workspace(workspace, workspace_bytes, m3::add_norm_bwd_workspace(rows, d));
+        if (st != M3_OK) return st;
+    }
+    return m3::launch_add_norm_bwd(total, weight, rstd, dtotal, dy, dtype, scale, dx, dresidual, dweight, workspace, rows, d,
+                                   as_stream(stream));
+}
+
+int m3_mx_linear(int64_t rows, int32_t n, int32_t k, int32_t x_format, int32_t out_dtype, const void* x_data,
+                 const void* x_scales, const void* w_data, const void* w_scales, const void* residual, float scale, void* out,
+                 void* stream) {
+    if (!x_data || !x_scales || !w_data || !w_scales || !out) return M3_ERR_NULL_POINTER;
+    int st = check_mx(rows, k, x_format);
+    if (st == M3_OK) st = check_dtype(out_dtype);
+    if (st != M3_OK) return st;
+    if (n <= 0) return M3_ERR_INVALID_SHAPE;
+    if (rows > (1 << 26) || n > (1 << 26) || k > (1 << 20)) return M3_ERR_UNSUPPORTED;
+    if (!aligned(x_data, 16) || !aligned(w_data, 16) || !aligned(x_scales, 4) || !aligned(w_scales, 4) ||
+        !aligned(out, size_of(out_dtype)) || (residual && !aligned(residual, size_of(out_dtype))))
+        return M3_ERR_MISALIGNED;
+    return m3::launch_mx_linear(x_data, x_scales, x_format, w_data, w_scales, residual, scale, out, out_dtype, (int)rows, n, k,
+                                as_stream(stream));
+}
+
+static int check_sample(int64_t rows, int32_t vocab) {
+    if (rows <= 0 || vocab <= 0) return M3_ERR_INVALID_SHAPE;
+    return rows > (1 << 30) || vocab > (1 << 22) ? M3_ERR_UNSUPPORTED : M3_OK;
+}
+
+int m3_sample_tokens_workspace_size(int64_t rows, int32_t vocab, size_t* bytes) {
+    if (!bytes) return M3_ERR_NULL_POINTER;
+    const int st = check_sample(rows, vocab);
+    if (st == M3_OK) *bytes = m3::sample_workspace(rows, vocab);
+    return st;
+}
+
+int m3_sample_tokens(int64_t rows, int32_t vocab, int32_t dtype, const void* logits, const float* u, const float* temperatures,
+                     double temperature, const int32_t* top_ks, int64_t top_k, const float* top_ps, double top_p,
+                     const float* min_ps, double min_p, int64_t* token, float* logprob, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+    if (!logits || !u || !token) return M3_ERR_NULL_POINTER;
+    int st = check_sample(rows, vocab);
+    if (st == M3_OK) st = check_dtype(dtype);
+    if (st != M3_OK) return st;
+    if (!aligned(logits, size_of(dtype))) return M3_ERR_MISALIGNED;
+    st = check_workspace(workspace, workspace_bytes, m3::sample_workspace(rows, vocab));
+    if (st != M3_OK) return st;
+    return m3::launch_sample(logits, dtype, rows, vocab, u, temperatures, temperature, top_ks, top_k, top_ps, top_p, min_ps, min_p,
+                             token, logprob, workspace, as_stream(stream));
+}
+
 }  // extern "C"

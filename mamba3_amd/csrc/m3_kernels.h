@@ -228,6 +228,38 @@ int64_t clip_total_blocks(int n, const int64_t* numel, const int32_t* dtype);
 int launch_clip(int n, void* const* p, const int64_t* numel, const int32_t* dtype, bool inf_norm,
                 bool scale, float max_norm, float* norm, void* ws, hipStream_t stream);
 
+// Microscaled values (m3_mx.hip; formats of m3_mx.h): quantisation of x, or with `gated` of
+// silu(x[:, :k]) * x[:, k:2 k], and its inverse (m3_status).
+int launch_mx_quantize(const void* x, int dtype, bool gated, int format, void* data, void* scales,
+                       int64_t rows, int k, hipStream_t stream);
+int launch_mx_dequantize(const void* data, const void* scales, int format, void* out, int dtype,
+                         int64_t rows, int k, hipStream_t stream);
+
+// The residual's addition and the norm behind it (m3_add_norm.hip): y in the inputs' type or
+// microscaled, the backward's workspace bytes and launcher (m3_status).
+int launch_add_norm(const void* x, const void* res, const void* w, int dtype, float scale, float eps,
+                    void* total, void* y, float* rstd, int64_t rows, int d, hipStream_t stream);
+int launch_add_norm_mx(const void* x, const void* res, const void* w, int dtype, float scale, float eps,
+                       void* total, int format, void* data, void* scales, int64_t rows, int d,
+                       hipStream_t stream);
+size_t add_norm_bwd_workspace(int64_t rows, int d);
+int launch_add_norm_bwd(const void* total, const void* w, const float* rstd, const void* dtotal,
+                        const void* dy, int dtype, float scale, void* dx, void* dres, void* dw, void* ws,
+                        int64_t rows, int d, hipStream_t stream);
+
+// Products of microscaled activations with e2m1 weights (m3_mx_linear.hip; m3_status).
+int launch_mx_linear(const void* x, const void* xs, int x_format, const void* w, const void* ws,
+                     const void* res, float scale, void* out, int out_dtype, int m, int n, int k,
+                     hipStream_t stream);
+
+// The next token of each row of logits (m3_sample.hip): settings by row, or where their pointer is
+// NULL one for all; workspace bytes and launcher (m3_status).
+size_t sample_workspace(int64_t rows, int64_t vocab);
+int launch_sample(const void* logits, int dtype, int64_t rows, int vocab, const float* u,
+                  const float* temperature, double temperature1, const int32_t* top_k, int64_t top_k1,
+                  const float* top_p, double top_p1, const float* min_p, double min_p1, int64_t* token,
+                  float* logprob, void* ws, hipStream_t stream);
+
 // Returns 1 when the step kernel supports (N, R), else 0.
 int step_supported(int N, int R);
 int launch_step(const m3_layer_desc& d, const m3_layer_params& p, const void* proj,

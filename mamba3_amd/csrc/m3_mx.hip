@@ -1,0 +1,131 @@
+// Microscaled quantisation (m3_mx.h), with silu(gate) * up in front of it, and its inverse.
+// Bound by HBM: one read and one write. A lane takes eight elements (one 16-byte read of bf16), four
+// lanes a block of 32, whose largest magnitude they find with two lane moves.
+#include <algorithm>
+
+#include "m3_common.h"
+#include "m3_kernels.h"
+#include "m3_mx.h"
+#include "mamba3_amd.h"
+
+namespace m3 {
+
+constexpr int kMxThreads = 256;
+constexpr int kMxUnits = 2;  // eights a thread
+
+// silu without the overflow of exp(-g): e = exp(-|g|) is at most 1.
+__device__ __forceinline__ float silu_any(float g) {
+    const float e = expf(-fabsf(g));
+    return (g < 0.f ? g * e : g) / (1.f + e);
+}
+
+template <typename T, int F, bool kGated>
+__global__ __launch_bounds__(kMxThreads) void mx_quantize_kernel(const T* __restrict__ x, uint8_t* __restrict__ data,
+                                                                 uint8_t* __restrict__ scales, unsigned units, int k,
+                                                                 int kp, FastDiv per_row) {
+    const unsigned at = blockIdx.x * (kMxThreads * kMxUnits) + threadIdx.x;
+    float v[kMxUnits][8], u[kGated ? kMxUnits : 1][8];
+    unsigned row[kMxUnits];
+    int unit[kMxUnits];
+#pragma unroll
+    for (int i = 0; i < kMxUnits; ++i) {
+        const unsigned id = at + i * kMxThreads;
+        row[i] = per_row.div(id);
+        unit[i] = (int)(id - row[i] * per_row.d);
+        if (id < units) {
+            const T* r = x + (int64_t)row[i] * (kGated ? 2 * (int64_t)k : k);
+            load8(r, unit[i] * 8, k, v[i]);
+            if constexpr (kGated) load8(r + k, unit[i] * 8, k, u[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kMxUnits; ++i) {
+        if (at + i * kMxThreads >= units) continue;  // whole blocks of 32: units of a row come in sixteens
+        if constexpr (kGated) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] = silu_any(v[i][e]) * u[i][e];
+        }
+        mx_store8<F>(v[i], data + (int64_t)row[i] * (F == kE4m3 ? kp : kp / 2), scales + (int64_t)row[i] * (kp / 32), unit[i]);
+    }
+}
+
+template <typename T, int F>
+__global__ __launch_bounds__(kMxThreads) void mx_dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales,
+                                                                   T* __restrict__ out, unsigned units, int k, int kp, FastDiv per_row) {
+    const unsigned at = blockIdx.x * (kMxThreads * kMxUnits) + threadIdx.x;
+    u32x2 w[kMxUnits];
+    unsigned row[kMxUnits], s[kMxUnits];
+    int unit[kMxUnits];
+#pragma unroll
+    for (int i = 0; i < kMxUnits; ++i) {
+        const unsigned id = at + i * kMxThreads;
+        row[i] = per_row.div(id);
+        unit[i] = (int)(id - row[i] * per_row.d);
+        if (id < units) {
+            const uint8_t* p = data + (int64_t)row[i] * (F == kE4m3 ? kp : kp / 2);
+            if constexpr (F == kE4m3) w[i] = *reinterpret_cast<const u32x2*>(p + unit[i] * 8);
+            else w[i] = u32x2{*reinterpret_cast<const unsigned*>(p + unit[i] * 4), 0};
+            s[i] = scales[(int64_t)row[i] * (kp / 32) + (unit[i] >> 2)];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kMxUnits; ++i) {
+        if (at + i * kMxThreads >= units) continue;
+        float v[8];
+        mx_unpack8<F>(w[i], v);
+        const float f = mx_factor(s[i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= f;
+        store8(out + (int64_t)row[i] * k, unit[i] * 8, k, v);
+    }
+}
+
+// Launches of fewer than 2^31 units.
+template <typename Launch>
+static int mx_rows(int64_t rows, int64_t per_row, Launch launch) {
+    const int64_t most = (((int64_t)1 << 31) - 1) / per_row;
+    for (int64_t r = 0; r < rows; r += most) {
+        const unsigned units = (unsigned)(std::min(most, rows - r) * per_row);
+        launch(r, units, dim3((units + kMxThreads * kMxUnits - 1) / (kMxThreads * kMxUnits)));
+        if (hipGetLastError() != hipSuccess) return M3_ERR_LAUNCH;
+    }
+    return M3_OK;
+}
+
+template <typename T, int F, bool kGated>
+static int quantize_t(const void* x, void* data, void* scales, int64_t rows, int k, hipStream_t stream) {
+    const int kp = (int)mx_padded(k);
+    return mx_rows(rows, kp / 8, [&](int64_t r, unsigned units, dim3 grid) {
+        hipLaunchKernelGGL((mx_quantize_kernel<T, F, kGated>), grid, dim3(kMxThreads), 0, stream,
+                           reinterpret_cast<const T*>(x) + r * k * (kGated ? 2 : 1),
+                           reinterpret_cast<uint8_t*>(data) + r * mx_row_bytes(kp, F), reinterpret_cast<uint8_t*>(scales) + r * (kp / 32),
+                           units, k, kp, FastDiv(kp / 8));
+    });
+}
+template <typename T>
+static int quantize_f(const void* x, bool gated, int format, void* data, void* scales, int64_t rows, int k, hipStream_t stream) {
+    if (format == kE4m3)
+        return gated ? quantize_t<T, kE4m3, true>(x, data, scales, rows, k, stream) : quantize_t<T, kE4m3, false>(x, data, scales, rows, k, stream);
+    return gated ? quantize_t<T, kE2m1, true>(x, data, scales, rows, k, stream) : quantize_t<T, kE2m1, false>(x, data, scales, rows, k, stream);
+}
+int launch_mx_quantize(const void* x, int dtype, bool gated, int format, void* data, void* scales, int64_t rows, int k, hipStream_t stream) {
+    return dtype == M3_DTYPE_BF16 ? quantize_f<bf16>(x, gated, format, data, scales, rows, k, stream)
+                                  : quantize_f<float>(x, gated, format, data, scales, rows, k, stream);
+}
+
+template <typename T, int F>
+static int dequantize_t(const void* data, const void* scales, void* out, int64_t rows, int k, hipStream_t stream) {
+    const int kp = (int)mx_padded(k);
+    return mx_rows(rows, kp / 8, [&](int64_t r, unsigned units, dim3 grid) {
+        hipLaunchKernelGGL((mx_dequantize_kernel<T, F>), grid, dim3(kMxThreads), 0, stream,
+                           reinterpret_cast<const uint8_t*>(data) + r * mx_row_bytes(kp, F),
+                           reinterpret_cast<const uint8_t*>(scales) + r * (kp / 32), reinterpret_cast<T*>(out) + r * k, units, k, kp, FastDiv(kp / 8));
+    });
+}
+int launch_mx_dequantize(const void* data, const void* scales, int format, void* out, int dtype, int64_t rows, int k, hipStream_t stream) {
+    if (dtype == M3_DTYPE_BF16)
+        return format == kE4m3 ? dequantize_t<bf16, kE4m3>(data, scales, out, rows, k, stream) : dequantize_t<bf16, kE2m1>(data, scales, out, rows, k, stream);
+    return format == kE4m3 ? dequantize_t<float, kE4m3>(data, scales, out, rows, k, stream) : dequantize_t<float, kE2m1>(data, scales, out, rows, k, stream);
+}
+
+}  // namespace m3

@@ -1000,3 +1000,250 @@ def linear_xent_fast(hidden, weight, target, ignore_index, reduction):
     if _is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         return _LinearXent.apply(hidden, weight, target, ignore_index, reduction)
     return _linear_xent_eager(hidden, weight, target, ignore_index, reduction)[0]
+
+
+# ---------------------------------------------------------------- 4-bit serving
+def _rows_of(t: torch.Tensor) -> torch.Tensor:
+    """t as contiguous rows of its last dimension; these kernels take them at any alignment."""
+    return t if t.dim() == 2 and t.is_contiguous() else t.detach().reshape(-1, t.shape[-1]).contiguous()
+
+
+def _mx_empty(rows: int, k: int, fmt: str, like: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Room for (rows, k) microscaled values: (data, scales)."""
+    return (like.new_empty((rows, _native.mx_row_bytes(k, fmt)), dtype=torch.uint8),
+            like.new_empty((rows, _native.mx_padded(k) // 32), dtype=torch.uint8))
+
+
+def _mx_quantize_eager(x: torch.Tensor, fmt: str, gated: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """m3_mx_quantize over the last dimension of x: (data, scales), one row for each of x's."""
+    _native.require_gpu(x)
+    with on_device(x):
+        x2 = _rows_of(x)
+        out = _mx_empty(x2.shape[0], x2.shape[1] // 2 if gated else x2.shape[1], fmt, x2)
+        if x2.shape[0]:
+            _native.mx_quantize(x2, fmt, gated, *out)
+    return out
+
+
+mx_quantize = torch.library.custom_op(f"{NS}::mx_quantize", _mx_quantize_eager, mutates_args=())
+
+
+@mx_quantize.register_fake
+def _(x, fmt, gated):
+    k = x.shape[-1] // 2 if gated else x.shape[-1]
+    return _mx_empty(x.numel() // x.shape[-1], k, fmt, x)
+
+
+def _mx_dequantize_eager(data: torch.Tensor, scales: torch.Tensor, fmt: str, k: int, dtype: torch.dtype) -> torch.Tensor:
+    """m3_mx_dequantize: (rows, k) in `dtype`."""
+    _native.require_gpu(data, scales)
+    with on_device(data):
+        out = torch.empty((data.shape[0], k), device=data.device, dtype=dtype)
+        if out.shape[0]:
+            _native.mx_dequantize(data, scales, fmt, out)
+    return out
+
+
+mx_dequantize = torch.library.custom_op(f"{NS}::mx_dequantize", _mx_dequantize_eager, mutates_args=())
+
+
+@mx_dequantize.register_fake
+def _(data, scales, fmt, k, dtype):
+    return data.new_empty((data.shape[0], k), dtype=dtype)
+
+
+def _add_rmsnorm_eager(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, scale: float,
+                       eps: float, keep: bool = True) -> tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+    """m3_add_rmsnorm_fwd over the last dimension: (total, y, and with `keep` rstd (rows,) fp32)."""
+    _native.require_gpu(x, residual, weight)
+    with on_device(x):
+        x2 = _rows_of(x)
+        total, y = torch.empty_like(x2), torch.empty_like(x2)
+        rstd = torch.empty(x2.shape[0], device=x.device, dtype=torch.float32) if keep else None
+        _native.add_rmsnorm_fwd(x2, _rows_of(residual), weight.contiguous(), scale, eps, total, y, rstd)
+    return total.view(x.shape), y.view(x.shape), rstd
+
+
+@torch.library.custom_op(f"{NS}::add_rmsnorm", mutates_args=())
+def add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, scale: float,
+                eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """_add_rmsnorm_eager as an op."""
+    return _add_rmsnorm_eager(x, residual, weight, scale, eps)
+
+
+@add_rmsnorm.register_fake
+def _(x, residual, weight, scale, eps):
+    return x.new_empty(x.shape), x.new_empty(x.shape), x.new_empty(x.numel() // x.shape[-1], dtype=torch.float32)
+
+
+def _add_rmsnorm_bwd_eager(total, weight, rstd, dtotal, dy, scale, want) -> list:
+    """m3_add_rmsnorm_bwd: gradients of x, residual and weight, None for those that `want` leaves out."""
+    with on_device(total):
+        out = [torch.empty(t.shape, device=t.device, dtype=t.dtype) if w else None
+               for t, w in zip((total, total, weight), want)]
+        two = lambda t: None if t is None else _rows_of(t if t.dtype == total.dtype else t.to(total.dtype))  # noqa: E731
+        _native.add_rmsnorm_bwd(_rows_of(total), weight.contiguous(), rstd, two(dtotal), two(dy), scale, *out)
+    return out
+
+
+@torch.library.custom_op(f"{NS}::add_rmsnorm_bwd", mutates_args=())
+def add_rmsnorm_bwd(total: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, dtotal: Optional[torch.Tensor],
+                    dy: torch.Tensor, scale: float, want: list[bool]) -> list[torch.Tensor]:
+    """_add_rmsnorm_bwd_eager as an op; gradients that `want` leaves out are empty."""
+    out = _add_rmsnorm_bwd_eager(total, weight, rstd, dtotal, dy, scale, want)
+    return [total.new_empty(0) if t is None else t for t in out]
+
+
+@add_rmsnorm_bwd.register_fake
+def _(total, weight, rstd, dtotal, dy, scale, want):
+    return [t.new_empty(t.shape if w else (0,)) for t, w in zip((total, total, weight), want)]
+
+
+def _add_rmsnorm_grads(bwd, total, weight, rstd, scale, want, dtotal, dy):
+    """The three gradients; either output's may be None."""
+    if dy is None:
+        # the norm's output is unused: the sum alone
+        if dtotal is None:
+            return None, None, None
+        return (dtotal * scale if want[0] else None, dtotal if want[1] else None,
+                torch.zeros_like(weight) if want[2] else None)
+    if not any(want):
+        return None, None, None
+    out = bwd(total, weight, rstd, dtotal, dy, scale, list(want))
+    return tuple(t if w else None for t, w in zip(out, want))
+
+
+def _add_rmsnorm_setup(ctx, inputs, output):
+    _, _, weight, ctx.scale, _ = inputs
+    ctx.save_for_backward(output[0], weight, output[2])
+    ctx.set_materialize_grads(False)
+
+
+def _add_rmsnorm_backward(ctx, dtotal, dy, _):
+    grads = _add_rmsnorm_grads(add_rmsnorm_bwd, *ctx.saved_tensors, ctx.scale, ctx.needs_input_grad[:3], dtotal, dy)
+    return (*grads, None, None)
+
+
+add_rmsnorm.register_autograd(_add_rmsnorm_backward, setup_context=_add_rmsnorm_setup)
+
+
+class _AddRmsNorm(torch.autograd.Function):
+    """add_rmsnorm under eager autograd, without the dispatcher's host time."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, scale, eps):
+        total, y, rstd = _add_rmsnorm_eager(x, residual, weight, scale, eps)
+        ctx.scale = scale
+        ctx.save_for_backward(total, weight, rstd)
+        ctx.set_materialize_grads(False)
+        return total, y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dtotal, dy):
+        grads = _add_rmsnorm_grads(_add_rmsnorm_bwd_eager, *ctx.saved_tensors, ctx.scale, ctx.needs_input_grad[:3], dtotal, dy)
+        return (*grads, None, None)
+
+
+def _add_rmsnorm_mx_eager(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, scale: float,
+                          eps: float, fmt: str) -> tuple[Optional[torch.Tensor], torch.Tensor, torch.Tensor]:
+    """m3_add_rmsnorm_mx over the last dimension: (total, or None without a residual; data, scales)."""
+    _native.require_gpu(x, residual, weight)
+    with on_device(x):
+        x2 = _rows_of(x)
+        total = None if residual is None else torch.empty_like(x2)
+        data, scales = _mx_empty(*x2.shape, fmt, x2)
+        if x2.shape[0]:
+            _native.add_rmsnorm_mx(x2, None if residual is None else _rows_of(residual), weight.contiguous(), scale, eps,
+                                   total, fmt, data, scales)
+    return None if total is None else total.view(x.shape), data, scales
+
+
+@torch.library.custom_op(f"{NS}::add_rmsnorm_mx", mutates_args=())
+def add_rmsnorm_mx(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, scale: float, eps: float,
+                   fmt: str) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """_add_rmsnorm_mx_eager as an op; the first output is empty without a residual."""
+    total, data, scales = _add_rmsnorm_mx_eager(x, residual, weight, scale, eps, fmt)
+    return x.new_empty(0) if total is None else total, data, scales
+
+
+@add_rmsnorm_mx.register_fake
+def _(x, residual, weight, scale, eps, fmt):
+    return (x.new_empty((0,) if residual is None else x.shape), *_mx_empty(x.numel() // x.shape[-1], x.shape[-1], fmt, x))
+
+
+def _mx_linear_eager(x_data: torch.Tensor, x_scales: torch.Tensor, x_format: str, w_data: torch.Tensor,
+                     w_scales: torch.Tensor, k: int, residual: Optional[torch.Tensor], scale: float,
+                     dtype: torch.dtype) -> torch.Tensor:
+    """m3_mx_linear: (rows, n) in `dtype`, the residual's where one is given."""
+    _native.require_gpu(x_data, x_scales, w_data, w_scales, residual)
+    with on_device(x_data):
+        out = torch.empty((x_data.shape[0], w_data.shape[0]), device=x_data.device, dtype=dtype)
+        if out.numel():
+            _native.mx_linear(x_data, x_scales, x_format, w_data, w_scales, k,
+                              None if residual is None else _rows_of(residual), scale, out)
+    return out
+
+
+mx_linear = torch.library.custom_op(f"{NS}::mx_linear", _mx_linear_eager, mutates_args=())
+
+
+@mx_linear.register_fake
+def _(x_data, x_scales, x_format, w_data, w_scales, k, residual, scale, dtype):
+    return x_data.new_empty((x_data.shape[0], w_data.shape[0]), dtype=dtype)
+
+
+def _sample_tokens_eager(logits: torch.Tensor, u: torch.Tensor, temperatures: Optional[torch.Tensor], temperature: float,
+                         top_ks: Optional[torch.Tensor], top_k: int, top_ps: Optional[torch.Tensor], top_p: float,
+                         min_ps: Optional[torch.Tensor], min_p: float, logprob: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """m3_sample_tokens on logits (rows, vocab): (tokens (rows,) int64, log probabilities (rows,), empty unless asked
+    for). A setting is the tensor (rows,), or where that is None the number."""
+    _native.require_gpu(logits, u, temperatures, top_ks, top_ps, min_ps)
+    with on_device(logits):
+        rows = logits.shape[0]
+        token = torch.empty(rows, device=logits.device, dtype=torch.int64)
+        lp = torch.empty(rows if logprob else 0, device=logits.device, dtype=torch.float32)
+        each = [n if t is None else t.contiguous()
+                for t, n in ((temperatures, temperature), (top_ks, top_k), (top_ps, top_p), (min_ps, min_p))]
+        if rows:
+            _native.sample_tokens(_rows_of(logits), u.contiguous(), *each, token, lp if logprob else None)
+    return token, lp
+
+
+sample_tokens = torch.library.custom_op(f"{NS}::sample_tokens", _sample_tokens_eager, mutates_args=())
+
+
+@sample_tokens.register_fake
+def _(logits, u, temperatures, temperature, top_ks, top_k, top_ps, top_p, min_ps, min_p, logprob):
+    rows = logits.shape[0]
+    return logits.new_empty(rows, dtype=torch.int64), logits.new_empty(rows if logprob else 0, dtype=torch.float32)
+
+
+def mx_quantize_fast(x, fmt, gated):
+    return (_mx_quantize_eager if _plain(x) else mx_quantize)(x, fmt, gated)
+
+
+def mx_dequantize_fast(data, scales, fmt, k, dtype):
+    return (_mx_dequantize_eager if _plain(data, scales) else mx_dequantize)(data, scales, fmt, k, dtype)
+
+
+def add_rmsnorm_fast(x, residual, weight, scale, eps):
+    if not _plain(x, residual, weight):
+        return add_rmsnorm(x, residual, weight, scale, eps)[:2]
+    if _is_grad_enabled() and (x.requires_grad or residual.requires_grad or weight.requires_grad):
+        return _AddRmsNorm.apply(x, residual, weight, scale, eps)
+    return _add_rmsnorm_eager(x, residual, weight, scale, eps, False)[:2]
+
+
+def add_rmsnorm_mx_fast(x, residual, weight, scale, eps, fmt):
+    return (_add_rmsnorm_mx_eager if _plain(x, residual, weight) else add_rmsnorm_mx)(x, residual, weight, scale, eps, fmt)
+
+
+def mx_linear_fast(x_data, x_scales, x_format, w_data, w_scales, k, residual, scale, dtype):
+    fn = _mx_linear_eager if _plain(x_data, x_scales, w_data, w_scales, residual) else mx_linear
+    return fn(x_data, x_scales, x_format, w_data, w_scales, k, residual, scale, dtype)
+
+
+def sample_tokens_fast(logits, u, temperatures, temperature, top_ks, top_k, top_ps, top_p, min_ps, min_p, logprob):
+    fn = _sample_tokens_eager if _plain(logits, u, temperatures, top_ks, top_ps, min_ps) else sample_tokens
+    return fn(logits, u, temperatures, temperature, top_ks, top_k, top_ps, top_p, min_ps, min_p, logprob)
