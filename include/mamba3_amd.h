@@ -523,6 +523,15 @@ int m3_mx_linear(int64_t rows, int32_t n, int32_t k, int32_t x_format, int32_t o
                  void* stream);
 
 /*
+ * The same for x [rows, k] in x_dtype, quantised to e4m3 on the way: the bits of m3_mx_quantize and m3_mx_linear, in one
+ * launch, for the sizes for which m3_mx_linear_takes_tensor returns 1 (at most 16 rows of together at most 32768 padded
+ * elements, and so few columns that m3_mx_linear takes its kernel for few rows); others are unsupported.
+ */
+int m3_mx_linear_takes_tensor(int64_t rows, int32_t n, int32_t k, int32_t out_dtype);
+int m3_mx_linear_tensor(int64_t rows, int32_t n, int32_t k, int32_t x_dtype, int32_t out_dtype, const void* x, const void* w_data,
+                        const void* w_scales, const void* residual, float scale, void* out, void* stream);
+
+/*
  * The next token of each row of logits [rows, vocab] from a random number u [rows] in [0, 1) (mamba3/block.py:208-222
  * draws with torch.multinomial). Tokens are ordered by logit, ties from the lowest index. With masses
  * exp((z - max z) / temperature), kept are the first top_k tokens (0: all), of these the shortest run from the first on whose mass
@@ -530,13 +539,11 @@ int m3_mx_linear(int64_t rows, int32_t n, int32_t k, int32_t x_format, int32_t o
  * token = the first kept one whose running mass passes u times the kept mass; logprob (or NULL) the log of
  * its share. A temperature of 0 (or below, or NaN) takes the first token (logprob 0). NaN counts as
  * -infinity, which is no token: a row without any gives -1 (logprob NaN). u outside [0, 1) is taken to its ends.
- * Each setting is the array's [rows] entry, or where that is NULL the number. vocab <= 2^22. workspace: 256-byte aligned.
+ * Each setting is the array's [rows] entry, or where that is NULL the number. rows <= 2^30, vocab <= 2^22.
  */
-int m3_sample_tokens_workspace_size(int64_t rows, int32_t vocab, size_t* bytes);
 int m3_sample_tokens(int64_t rows, int32_t vocab, int32_t dtype, const void* logits, const float* u, const float* temperatures,
                      double temperature, const int32_t* top_ks, int64_t top_k, const float* top_ps, double top_p,
-                     const float* min_ps, double min_p, int64_t* token, float* logprob, void* workspace,
-                     size_t workspace_bytes, void* stream);
+                     const float* min_ps, double min_p, int64_t* token, float* logprob, void* stream);
 
 #ifdef __cplusplus
 }

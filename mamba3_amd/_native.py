@@ -8,6 +8,7 @@ missing library raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 from array import array
 from pathlib import Path
@@ -65,7 +66,8 @@ EXPORTED_SYMBOLS = (
     "m3_add_rmsnorm_bwd_workspace_size",
     "m3_add_rmsnorm_bwd",
     "m3_mx_linear",
-    "m3_sample_tokens_workspace_size",
+    "m3_mx_linear_takes_tensor",
+    "m3_mx_linear_tensor",
     "m3_sample_tokens",
 )
 
@@ -206,9 +208,10 @@ def _declare(lib: ctypes.CDLL) -> None:
             ("m3_add_rmsnorm_bwd_workspace_size", [_i64, _i32, size_p]),
             ("m3_add_rmsnorm_bwd", [_i64, _i32, _i32] + [_vp] * 5 + [f32] + [_vp] * 4 + [ctypes.c_size_t, _vp]),
             ("m3_mx_linear", [_i64] + [_i32] * 4 + [_vp] * 5 + [f32] + [_vp] * 2),
-            ("m3_sample_tokens_workspace_size", [_i64, _i32, size_p]),
+            ("m3_mx_linear_takes_tensor", [_i64] + [_i32] * 3),
+            ("m3_mx_linear_tensor", [_i64] + [_i32] * 4 + [_vp] * 4 + [f32] + [_vp] * 2),
             ("m3_sample_tokens", [_i64, _i32, _i32, _vp, _vp, _vp, ctypes.c_double, _vp, _i64, _vp, ctypes.c_double, _vp,
-                                  ctypes.c_double, _vp, _vp, _vp, ctypes.c_size_t, _vp])):
+                                  ctypes.c_double, _vp, _vp, _vp])):
         fn = getattr(lib, name)
         fn.restype, fn.argtypes = ctypes.c_int, args
 
@@ -617,10 +620,15 @@ def add_rmsnorm_mx(x, residual, weight, scale: float, eps: float, total, fmt: st
         check(st, "m3_add_rmsnorm_mx")
 
 
+@functools.lru_cache(maxsize=256)
+def _add_rmsnorm_bwd_bytes(rows: int, d: int) -> int:
+    return _bytes_of("m3_add_rmsnorm_bwd_workspace_size", rows, d)
+
+
 def add_rmsnorm_bwd(total, weight, rstd, dtotal, dy, scale: float, dx, dresidual, dweight) -> None:
     """m3_add_rmsnorm_bwd on contiguous (rows, d) tensors; allocates the workspace."""
     rows, d = total.shape
-    n = _bytes_of("m3_add_rmsnorm_bwd_workspace_size", rows, d) if dweight is not None else 0
+    n = _add_rmsnorm_bwd_bytes(rows, d) if dweight is not None else 0
     ws = _workspace(n, total.device)
     check(lib().m3_add_rmsnorm_bwd(rows, d, dtype_code(total.dtype), ptr(total), ptr(weight), ptr(rstd), ptr(dtotal),
                                    ptr(dy), scale, ptr(dx), ptr(dresidual), ptr(dweight), ptr(ws), n,
@@ -636,15 +644,27 @@ def mx_linear(x_data, x_scales, x_format: str, w_data, w_scales, k: int, residua
         check(st, "m3_mx_linear")
 
 
+def mx_linear_takes_tensor(rows: int, n: int, k: int, out_dtype: torch.dtype) -> bool:
+    return bool(lib().m3_mx_linear_takes_tensor(rows, n, k, dtype_code(out_dtype)))
+
+
+def mx_linear_tensor(x, w_data, w_scales, residual, scale: float, out) -> None:
+    """m3_mx_linear_tensor on contiguous x (rows, k) into contiguous out (rows, n)."""
+    rows, n = out.shape
+    st = lib().m3_mx_linear_tensor(rows, n, x.shape[1], dtype_code(x.dtype), dtype_code(out.dtype), x.data_ptr(),
+                                   w_data.data_ptr(), w_scales.data_ptr(), ptr(residual), scale, out.data_ptr(), stream_of(out))
+    if st:
+        check(st, "m3_mx_linear_tensor")
+
+
 def sample_tokens(logits, u, temperature, top_k, top_p, min_p, token, logprob) -> None:
     """m3_sample_tokens on contiguous logits (rows, vocab); settings are numbers or tensors (rows,), fp32 or for
-    top_k int32. Allocates the workspace."""
+    top_k int32."""
     rows, vocab = logits.shape
-    n = _bytes_of("m3_sample_tokens_workspace_size", rows, vocab)
-    ws = _workspace(n, logits.device)
     args = []
     for v in (temperature, top_k, top_p, min_p):
         args += [v.data_ptr(), 0] if isinstance(v, torch.Tensor) else [None, v]
-    check(lib().m3_sample_tokens(rows, vocab, dtype_code(logits.dtype), logits.data_ptr(), u.data_ptr(), *args,
-                                 token.data_ptr(), ptr(logprob), ws.data_ptr(), n, stream_of(logits)),
-          "m3_sample_tokens")
+    st = lib().m3_sample_tokens(rows, vocab, dtype_code(logits.dtype), logits.data_ptr(), u.data_ptr(), *args,
+                                token.data_ptr(), ptr(logprob), stream_of(logits))
+    if st:
+        check(st, "m3_sample_tokens")

@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import ops
-from .mx import MXTensor, check_format, refuse_gradients
+from .mx import MXTensor, _mx, check_format, refuse_gradients
 
 
 def _check(what: str, x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor) -> None:
@@ -44,4 +44,4 @@ def add_rms_norm_mx(x: torch.Tensor, residual: torch.Tensor | None, weight: torc
     refuse_gradients("add_rms_norm_mx", x, residual, weight)
     _check("add_rms_norm_mx", x, residual, weight)
     total, data, scales = ops.add_rmsnorm_mx_fast(x, residual, weight, float(scale), float(eps), format)
-    return (x if residual is None else total), MXTensor(data, scales, x.shape, format)
+    return (x if residual is None else total), _mx(data, scales, x.shape, format)

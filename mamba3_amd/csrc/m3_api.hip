@@ -864,31 +864,39 @@ int m3_mx_linear(int64_t rows, int32_t n, int32_t k, int32_t x_format, int32_t o
                                 as_stream(stream));
 }
 
+int m3_mx_linear_takes_tensor(int64_t rows, int32_t n, int32_t k, int32_t out_dtype) {
+    return rows > 0 && n > 0 && k > 0 && m3::mx_linear_takes_tensor(rows, n, k, out_dtype) ? 1 : 0;
+}
+
+int m3_mx_linear_tensor(int64_t rows, int32_t n, int32_t k, int32_t x_dtype, int32_t out_dtype, const void* x, const void* w_data,
+                        const void* w_scales, const void* residual, float scale, void* out, void* stream) {
+    if (!x || !w_data || !w_scales || !out) return M3_ERR_NULL_POINTER;
+    if (rows <= 0 || n <= 0 || k <= 0) return M3_ERR_INVALID_SHAPE;
+    int st = check_dtype(x_dtype);
+    if (st == M3_OK) st = check_dtype(out_dtype);
+    if (st != M3_OK) return st;
+    if (n > (1 << 26) || !m3::mx_linear_takes_tensor(rows, n, k, out_dtype)) return M3_ERR_UNSUPPORTED;
+    if (!aligned(x, size_of(x_dtype)) || !aligned(w_data, 16) || !aligned(w_scales, 4) || !aligned(out, size_of(out_dtype)) ||
+        (residual && !aligned(residual, size_of(out_dtype))))
+        return M3_ERR_MISALIGNED;
+    return m3::launch_mx_linear_tensor(x, x_dtype, w_data, w_scales, residual, scale, out, out_dtype, (int)rows, n, k, as_stream(stream));
+}
+
 static int check_sample(int64_t rows, int32_t vocab) {
     if (rows <= 0 || vocab <= 0) return M3_ERR_INVALID_SHAPE;
     return rows > (1 << 30) || vocab > (1 << 22) ? M3_ERR_UNSUPPORTED : M3_OK;
 }
 
-int m3_sample_tokens_workspace_size(int64_t rows, int32_t vocab, size_t* bytes) {
-    if (!bytes) return M3_ERR_NULL_POINTER;
-    const int st = check_sample(rows, vocab);
-    if (st == M3_OK) *bytes = m3::sample_workspace(rows, vocab);
-    return st;
-}
-
 int m3_sample_tokens(int64_t rows, int32_t vocab, int32_t dtype, const void* logits, const float* u, const float* temperatures,
                      double temperature, const int32_t* top_ks, int64_t top_k, const float* top_ps, double top_p,
-                     const float* min_ps, double min_p, int64_t* token, float* logprob, void* workspace,
-                     size_t workspace_bytes, void* stream) {
+                     const float* min_ps, double min_p, int64_t* token, float* logprob, void* stream) {
     if (!logits || !u || !token) return M3_ERR_NULL_POINTER;
     int st = check_sample(rows, vocab);
     if (st == M3_OK) st = check_dtype(dtype);
     if (st != M3_OK) return st;
     if (!aligned(logits, size_of(dtype))) return M3_ERR_MISALIGNED;
-    st = check_workspace(workspace, workspace_bytes, m3::sample_workspace(rows, vocab));
-    if (st != M3_OK) return st;
     return m3::launch_sample(logits, dtype, rows, vocab, u, temperatures, temperature, top_ks, top_k, top_ps, top_p, min_ps, min_p,
-                             token, logprob, workspace, as_stream(stream));
+                             token, logprob, as_stream(stream));
 }
 
 }  // extern "C"

@@ -251,14 +251,17 @@ int launch_add_norm_bwd(const void* total, const void* w, const float* rstd, con
 int launch_mx_linear(const void* x, const void* xs, int x_format, const void* w, const void* ws,
                      const void* res, float scale, void* out, int out_dtype, int m, int n, int k,
                      hipStream_t stream);
+// ... of a tensor that is quantised to e4m3 on the way, where one launch does both: the same bits.
+bool mx_linear_takes_tensor(int64_t m, int64_t n, int64_t k, int out_dtype);
+int launch_mx_linear_tensor(const void* x, int x_dtype, const void* w, const void* ws, const void* res,
+                            float scale, void* out, int out_dtype, int m, int n, int k, hipStream_t stream);
 
 // The next token of each row of logits (m3_sample.hip): settings by row, or where their pointer is
-// NULL one for all; workspace bytes and launcher (m3_status).
-size_t sample_workspace(int64_t rows, int64_t vocab);
+// NULL one for all (m3_status).
 int launch_sample(const void* logits, int dtype, int64_t rows, int vocab, const float* u,
                   const float* temperature, double temperature1, const int32_t* top_k, int64_t top_k1,
                   const float* top_p, double top_p1, const float* min_p, double min_p1, int64_t* token,
-                  float* logprob, void* ws, hipStream_t stream);
+                  float* logprob, hipStream_t stream);
 
 // Returns 1 when the step kernel supports (N, R), else 0.
 int step_supported(int N, int R);

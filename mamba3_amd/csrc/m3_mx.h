@@ -9,6 +9,8 @@
 // 16-byte pieces and whole steps of the matrix instructions, which take 128 k.
 #pragma once
 
+#include <atomic>
+
 #include "m3_common.h"
 #include "m3_mfma.h"
 
@@ -31,6 +33,17 @@ struct FastDiv {
     }
     __device__ __forceinline__ unsigned div(unsigned n) const { return __umulhi(n, m) >> s; }
 };
+
+// Allows dynamic LDS past 64 KB, once for each device (a bit of `done`; devices past 63 set it every time).
+inline bool allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return false;
+    const uint64_t bit = dev < 63 ? (uint64_t)1 << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return true;
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return false;
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return true;
+}
 
 // Magnitude bits: their order is the magnitudes', an infinity above all numbers and NaN above it.
 __device__ __forceinline__ unsigned mag_bits(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
@@ -86,10 +99,10 @@ __device__ __forceinline__ u32x2 mx_pack8(const float (&v)[8]) {
     return o;
 }
 
-// Quantises the blocks whose 32 elements lie in four consecutive lanes, eight each, and stores this
-// lane's part: `unit` is the index of its eight in the row.
+// Quantises the blocks whose 32 elements lie in four consecutive lanes, eight each: this lane's elements go to `data`,
+// and in the block's first lane its scale to `scale`.
 template <int F>
-__device__ __forceinline__ void mx_store8(float (&v)[8], uint8_t* data_row, uint8_t* scale_row, int unit) {
+__device__ __forceinline__ void mx_store8_at(float (&v)[8], uint8_t* data, uint8_t* scale, bool first) {
     unsigned top = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -100,9 +113,14 @@ __device__ __forceinline__ void mx_store8(float (&v)[8], uint8_t* data_row, uint
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = s.byte == 255 ? 0.f : v[e] * s.inv;
     const u32x2 o = mx_pack8<F>(v);
-    if constexpr (F == kE4m3) *reinterpret_cast<u32x2*>(data_row + unit * 8) = o;
-    else *reinterpret_cast<unsigned*>(data_row + unit * 4) = o[0];
-    if ((unit & 3) == 0) scale_row[unit >> 2] = (uint8_t)s.byte;
+    if constexpr (F == kE4m3) *reinterpret_cast<u32x2*>(data) = o;
+    else *reinterpret_cast<unsigned*>(data) = o[0];
+    if (first) *scale = (uint8_t)s.byte;
+}
+// The same where they lie in a stored row: `unit` is the index of this lane's eight.
+template <int F>
+__device__ __forceinline__ void mx_store8(float (&v)[8], uint8_t* data_row, uint8_t* scale_row, int unit) {
+    mx_store8_at<F>(v, data_row + unit * (F == kE4m3 ? 8 : 4), scale_row + (unit >> 2), (unit & 3) == 0);
 }
 
 // Eight stored elements -> fp32, without their scale.

@@ -11,6 +11,8 @@
 // 16 g .. 16 g + 15 and 64 + 16 g .. (e4m3) or 32 g .. 32 g + 31 (e2m1), and the scale of block g. As in
 // m3_gemm.h the weights come first, so that a lane gets four consecutive n of one row m.
 #include <algorithm>
+#include <atomic>
+#include <utility>
 
 #include "m3_common.h"
 #include "m3_kernels.h"
@@ -93,9 +95,56 @@ __device__ __forceinline__ void mx_out4(const MxLinearArgs& a, int m, int n, f32
     }
 }
 
-// Few rows: a block takes 16 FM rows and 16 FN columns, its four waves every fourth step of k, straight from
-// memory to registers; their sums meet in LDS. Bound by the weights' read.
+// Few rows: a block takes 16 FM rows and 16 FN columns, its four waves every fourth step of k, straight from memory to
+// registers; their sums meet in LDS. Bound by the latency of its few reads, and by the weights' read. Reading two steps
+// ahead, and eight waves a block, gained nothing (4 x 768 x 3696 in a graph 2.6 us; 3.0 and 2.7).
 constexpr int kMlWaves = 4;
+
+// Adds w x^T of one step of k.
+template <int FA, int FM, int FN, bool kExact>
+__device__ __forceinline__ void few_step(const MxFrag<kE2m1> (&w)[FN], const MxFrag<FA> (&x)[FM], f32x4 (&acc)[FM][FN]) {
+    if constexpr (kExact) {
+        float fx[FM], fw[FN];
+#pragma unroll
+        for (int i = 0; i < FM; ++i) fx[i] = mx_factor((unsigned)x[i].s);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) fw[j] = mx_factor((unsigned)w[j].s);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            bf16x8 xq[FM];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) xq[i] = x[i].part(q, fx[i]);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                const bf16x8 wq = w[j].part(q, fw[j]);
+#pragma unroll
+                for (int i = 0; i < FM; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wq, xq[i], acc[i][j], 0, 0, 0);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int i = 0; i < FM; ++i) acc[i][j] = mx_mma<FA>(w[j], x[i], acc[i][j]);
+    }
+}
+// The waves' sums and their store.
+template <int FM, int FN, typename TO>
+__device__ __forceinline__ void few_store(const MxLinearArgs& a, f32x4 (&part)[kMlWaves][FM * FN][64], const f32x4 (&acc)[FM][FN], int m0, int n0, bool whole) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) part[wave][i * FN + j][lane] = acc[i][j];
+    __syncthreads();
+    for (int f = wave; f < FM * FN; f += kMlWaves) {
+        f32x4 v = part[0][f][lane];
+#pragma unroll
+        for (int q = 1; q < kMlWaves; ++q) v += part[q][f][lane];
+        mx_out4<TO>(a, m0 + f / FN * 16 + (lane & 15), n0 + f % FN * 16 + (lane >> 4) * 4, v, whole);
+    }
+}
+
 template <int FA, int FM, int FN, typename TO>
 __global__ __launch_bounds__(kMlWaves * 64) void mx_linear_few_kernel(MxLinearArgs a, int tiles_n, bool whole) {
     constexpr bool kExact = sizeof(TO) == 4;
@@ -127,64 +176,495 @@ __global__ __launch_bounds__(kMlWaves * 64) void mx_linear_few_kernel(MxLinearAr
         for (int j = 0; j < FN; ++j) w[j].template load<kExact>(wp[j], wsp[j], step, g);
 #pragma unroll
         for (int i = 0; i < FM; ++i) x[i].template load<kExact>(xp[i], xsp[i], step, g);
-        if constexpr (kExact) {
-            float fx[FM], fw[FN];
-#pragma unroll
-            for (int i = 0; i < FM; ++i) fx[i] = mx_factor((unsigned)x[i].s);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) fw[j] = mx_factor((unsigned)w[j].s);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                bf16x8 xq[FM];
-#pragma unroll
-                for (int i = 0; i < FM; ++i) xq[i] = x[i].part(q, fx[i]);
-#pragma unroll
-                for (int j = 0; j < FN; ++j) {
-                    const bf16x8 wq = w[j].part(q, fw[j]);
-#pragma unroll
-                    for (int i = 0; i < FM; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wq, xq[i], acc[i][j], 0, 0, 0);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-#pragma unroll
-                for (int i = 0; i < FM; ++i) acc[i][j] = mx_mma<FA>(w[j], x[i], acc[i][j]);
-        }
+        few_step<FA, FM, FN, kExact>(w, x, acc);
     }
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) part[wave][i * FN + j][lane] = acc[i][j];
-    __syncthreads();
-    for (int f = wave; f < FM * FN; f += kMlWaves) {
-        f32x4 v = part[0][f][lane];
-#pragma unroll
-        for (int q = 1; q < kMlWaves; ++q) v += part[q][f][lane];
-        mx_out4<TO>(a, m0 + f / FN * 16 + r, n0 + f % FN * 16 + g * 4, v, whole);
-    }
+    few_store<FM, FN, TO>(a, part, acc, m0, n0, whole);
 }
 
+// The same for at most 16 rows of a tensor, which each block quantises to e4m3 into LDS first: one launch less, and the
+// weights' first reads are on their way meanwhile. Rows of LDS are XOR-swizzled in 16-byte pieces. The sums are those of
+// the kernel above on the quantised rows, bit for bit.
+constexpr int kMlRawRows = 16;
+constexpr int kMlRawBytes = 32768;  // of quantised elements (with more, quantising in every block takes longer than the launch)
+template <typename T, int FN, typename TO>
+__global__ __launch_bounds__(kMlWaves * 64) void mx_linear_raw_kernel(MxLinearArgs a, int k, bool whole) {
+    constexpr bool kExact = sizeof(TO) == 4;
+    extern __shared__ __align__(16) char mx_smem[];  // [M][kp] elements, [M][kp / 32] scales
+    __shared__ f32x4 part[kMlWaves][FN][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    const int n0 = (int)blockIdx.x * 16 * FN, kp = a.steps * kMxStep;
+    const int64_t wb = (int64_t)a.steps * 64, sb = (int64_t)a.steps * 4;
+    const uint8_t *wp[FN], *wsp[FN];
+    MxFrag<kE2m1> w[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const int n = n0 + j * 16 + r < a.N ? n0 + j * 16 + r : a.N - 1;
+        wp[j] = a.w + n * wb, wsp[j] = a.ws + n * sb;
+        w[j].template load<kExact>(wp[j], wsp[j], wave < a.steps ? wave : a.steps - 1, g);
+    }
+    uint8_t* xs = reinterpret_cast<uint8_t*>(mx_smem) + a.M * kp;
+    const int units = kp / 8;
+    for (int i = threadIdx.x; i < a.M * units; i += kMlWaves * 64) {  // whole groups of four: units come in sixteens
+        const int row = i / units, unit = i - row * units;
+        float v[8];
+        load8(reinterpret_cast<const T*>(a.x) + (int64_t)row * k, unit * 8, k, v);
+        const int at = (unit >> 1 ^ (row & 7)) * 2 + (unit & 1);  // its 16-byte piece
+        mx_store8_at<kE4m3>(v, reinterpret_cast<uint8_t*>(mx_smem) + row * kp + at * 8, xs + row * (kp / 32) + (unit >> 2), (unit & 3) == 0);
+    }
+    __syncthreads();
+    f32x4 acc[1][FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int m = r < a.M ? r : a.M - 1;
+    const char* xr = mx_smem + m * kp;
+    const uint8_t* xsr = xs + m * (kp / 32);
+    for (int step = wave; step < a.steps; step += kMlWaves) {
+        if (step != wave) {
+#pragma unroll
+            for (int j = 0; j < FN; ++j) w[j].template load<kExact>(wp[j], wsp[j], step, g);
+        }
+        MxFrag<kE4m3> x[1];
+        const int p0 = step * 8 + (kExact ? 2 * g : g), p1 = step * 8 + (kExact ? 2 * g + 1 : 4 + g);
+        x[0].p[0] = *reinterpret_cast<const i32x4*>(xr + (p0 ^ (m & 7)) * 16);
+        x[0].p[1] = *reinterpret_cast<const i32x4*>(xr + (p1 ^ (m & 7)) * 16);
+        x[0].s = xsr[step * 4 + g];
+        few_step<kE4m3, 1, FN, kExact>(w, x, acc);
+    }
+    few_store<1, FN, TO>(a, part, acc, 0, n0, whole);
+}
+
+// Rows of the result are whole pieces of four.
+template <typename TO>
+static bool out4(const MxLinearArgs& a) {
+    const size_t piece = 4 * sizeof(TO);
+    return a.N % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % piece == 0 && (!a.res || reinterpret_cast<uintptr_t>(a.res) % piece == 0);
+}
 template <int FA, int FM, int FN, typename TO>
 static int few_t(const MxLinearArgs& a, hipStream_t stream) {
     const int64_t tn = (a.N + 16 * FN - 1) / (16 * FN), tm = (a.M + 16 * FM - 1) / (16 * FM);
     if (tn * tm > 0x7fffffff) return M3_ERR_UNSUPPORTED;
-    const size_t piece = 4 * sizeof(TO);
-    const bool whole = a.N % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % piece == 0 && (!a.res || reinterpret_cast<uintptr_t>(a.res) % piece == 0);
-    hipLaunchKernelGGL((mx_linear_few_kernel<FA, FM, FN, TO>), dim3((unsigned)(tn * tm)), dim3(kMlWaves * 64), 0, stream, a, (int)tn, whole);
+    hipLaunchKernelGGL((mx_linear_few_kernel<FA, FM, FN, TO>), dim3((unsigned)(tn * tm)), dim3(kMlWaves * 64), 0, stream, a, (int)tn, out4<TO>(a));
     return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH;
+}
+// Columns of a block: the fewest with which at most 256 blocks (one a CU) cover the result, since every block reads its rows
+// of x anew (M = 64, K = 768: N = 3696 takes 4.4, 5.0 and 6.2 us with 16, 32 and 64 columns, N = 32000 17, 11 and 9.3).
+static int few_columns(const MxLinearArgs& a, int rows) {
+    const int64_t tm = (a.M + rows - 1) / rows;
+    return tm * ((a.N + 15) / 16) <= 256 ? 1 : tm * ((a.N + 31) / 32) <= 256 ? 2 : 4;
+}
+template <int FA, int FM, typename TO>
+static int few_m(const MxLinearArgs& a, hipStream_t stream) {
+    const int fn = few_columns(a, 16 * FM);
+    if (fn == 1) return few_t<FA, FM, 1, TO>(a, stream);
+    if (fn == 2) return few_t<FA, FM, 2, TO>(a, stream);
+    return few_t<FA, FM, 4, TO>(a, stream);
+}
+template <typename T, int FN, typename TO>
+static int raw_t(const MxLinearArgs& a, int k, hipStream_t stream) {
+    const int lds = a.M * a.steps * (kMxStep + 4);
+    hipLaunchKernelGGL((mx_linear_raw_kernel<T, FN, TO>), dim3((unsigned)((a.N + 16 * FN - 1) / (16 * FN))), dim3(kMlWaves * 64), lds, stream, a, k, out4<TO>(a));
+    return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH;
+}
+template <typename T, typename TO>
+static int raw_n(const MxLinearArgs& a, int k, hipStream_t stream) {
+    const int fn = few_columns(a, 16);
+    if (fn == 1) return raw_t<T, 1, TO>(a, k, stream);
+    if (fn == 2) return raw_t<T, 2, TO>(a, k, stream);
+    return raw_t<T, 4, TO>(a, k, stream);
+}
+
+// Many rows: tiles through LDS, as in m3_gemm.h. A block of WGM x WGN waves owns a BM x BN tile (a wave 32 FM x 64)
+// and walks k in steps of 128, fetched straight to LDS three steps ahead; operand rows past the end come as zeros by
+// the descriptors' bounds. The 32 x 32 x 64 instruction takes a step in two halves; half s of a step takes the step's blocks
+// of 32 s and 2 + s, so that a lane's two scales of an operand row are one 16-bit read: group g = lane / 32 holds
+// block 2 g + s (e2m1) or 16 elements of either block (e4m3), and the scale of block 2 g + s.
+//
+// LDS of a step: x rows of 128 (e4m3) or 64 bytes, w rows of 64, then a word of scales for each row of x and of w.
+// 16-byte pieces lie XOR-swizzled, by which piece a lane fetches: piece c of row r at c ^ (r & 7), in rows of 64 bytes at
+// c ^ (r >> 1 & 3), so that eight consecutive rows of a read fall on eight places.
+//
+// A step is 2 FM groups of two instructions, each with a fragment of x; fragments are read two groups ahead, into a ring of
+// four. The barrier lies before the last two groups: by then all waves have read the step, whose place is refilled with
+// the one three further on, and the next step has landed. (With a whole half's fragments ahead the 256 x 256 tile spilled 94
+// registers.) Blocks stay for further tiles, whose first steps are fetched by the last steps of the tile before; the
+// epilogue turns the results into whole rows in a part of LDS of each wave's own.
+template <int FA_, int BM_, int BN_, int WGM_, int WGN_, int STAGES_, int ER_>
+struct MxTile {
+    static constexpr int FA = FA_, BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, STAGES = STAGES_;
+    static constexpr int ER = ER_;  // rows of results a wave turns at once
+    static constexpr int NW = WGM * WGN, NT = NW * 64;
+    static constexpr int FM = BM / WGM / 32, FN = 2;
+    static constexpr int XROW = FA == kE4m3 ? 128 : 64;  // bytes of x a row and step
+    // copies a wave and step: of 1 KB of x and of w, of 64 rows' scales (those past the last row's fetch nothing)
+    static constexpr int NX = BM * XROW / 1024 / NW, NWL = BN * 64 / 1024 / NW, NS = ((BM + BN) / 64 + NW - 1) / NW, NLD = NX + NWL + NS;
+    static constexpr int kX = BM * XROW, kW = BN * 64, kS = NS * NW * 256;
+    static constexpr int kStage = kX + kW + kS;
+    static constexpr int kLds = STAGES * kStage + NW * ER * 128;
+    static constexpr int kStores = FM * 4;  // of an epilogue, a wave
+    static_assert(BN / WGN == 64 && NX * NW * 1024 == kX && NWL * NW * 1024 == kW && (ER == 16 || ER == 32), "whole copies");
+};
+
+template <int... I, typename F>
+__device__ __forceinline__ void mx_each(std::integer_sequence<int, I...>, F f) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+
+template <typename Tile>
+__global__ __launch_bounds__(Tile::NT, 2) void mx_linear_tile_kernel(MxLinearArgs a, int tiles_m, int tiles_n) {
+    constexpr int FA = Tile::FA, FM = Tile::FM, FN = Tile::FN, ST = Tile::STAGES, XROW = Tile::XROW, NLD = Tile::NLD;
+    constexpr int XP = FA == kE4m3 ? 2 : 1;  // 16-byte pieces of an x fragment
+    extern __shared__ __align__(16) char mx_smem[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / Tile::WGN, wn = wave % Tile::WGN;
+    const int total = tiles_m * tiles_n, grid = (int)gridDim.x;
+    const int xld = a.steps * XROW, wld = a.steps * 64, sld = a.steps * 4;
+
+    // ids -> tiles: those of one XCD (every eighth id) are a contiguous run, in groups of 8 row tiles walked column by
+    // column, so that an XCD's L2 serves both operands
+    auto tile_of = [&](int id, int& m0, int& n0) __attribute__((always_inline)) {
+        constexpr int G = 8;
+        const int x = id & 7, per = total >> 3, rest = total & 7;
+        const int at = x * per + (x < rest ? x : rest) + (id >> 3);
+        const int group = __builtin_amdgcn_readfirstlane(at / (G * tiles_n)), first = group * G;
+        const int rows = tiles_m - first < G ? tiles_m - first : G;
+        const int in = at - group * (G * tiles_n);
+        const int tn = __builtin_amdgcn_readfirstlane(in / rows);
+        m0 = (first + in - tn * rows) * Tile::BM, n0 = tn * Tile::BN;
+    };
+
+    // ---- copies: this wave's NX of x, NWL of w and one of the scales (64 rows of x or of w)
+    unsigned xoff[Tile::NX], woff[Tile::NWL];
+#pragma unroll
+    for (int i = 0; i < Tile::NX; ++i) {
+        constexpr int CPR = XROW / 16, RPI = 64 / CPR;
+        const int r = (wave * Tile::NX + i) * RPI + lane / CPR, c = lane % CPR;
+        xoff[i] = (unsigned)(r * xld + ((FA == kE4m3 ? c ^ (r & 7) : c ^ (r >> 1 & 3)) * 16));
+    }
+#pragma unroll
+    for (int i = 0; i < Tile::NWL; ++i) {
+        const int r = (wave * Tile::NWL + i) * 16 + lane / 4, c = lane % 4;
+        woff[i] = (unsigned)(r * wld + ((c ^ (r >> 1 & 3)) * 16));
+    }
+    const unsigned soff = (unsigned)(lane * sld);
+    const char *px, *pw, *ps[Tile::NS];
+    int bx, bw, bs[Tile::NS], f_id, fs;
+    auto enter = [&](int id) __attribute__((always_inline)) {
+        f_id = id, fs = 0;
+        int m0 = 0, n0 = 0;
+        const bool there = id < total;
+        if (there) tile_of(id, m0, n0);
+        const int xr = a.M - m0 < Tile::BM ? a.M - m0 : Tile::BM, wr = a.N - n0 < Tile::BN ? a.N - n0 : Tile::BN;
+        px = reinterpret_cast<const char*>(a.x) + (int64_t)m0 * xld;
+        pw = reinterpret_cast<const char*>(a.w) + (int64_t)n0 * wld;
+        bx = there ? (xr - 1) * xld + XROW : 0;
+        bw = there ? (wr - 1) * wld + 64 : 0;
+#pragma unroll
+        for (int i = 0; i < Tile::NS; ++i) {
+            const int c = wave * Tile::NS + i;  // of BM / 64 copies of x's scales, then BN / 64 of w's
+            const bool sx = c < Tile::BM / 64;
+            const int row = (sx ? c : c - Tile::BM / 64) * 64, left = (sx ? xr : wr) - row;
+            ps[i] = (sx ? reinterpret_cast<const char*>(a.xs) + (int64_t)(m0 + row) * sld : reinterpret_cast<const char*>(a.ws) + (int64_t)(n0 + row) * sld);
+            bs[i] = there && c < (Tile::BM + Tile::BN) / 64 && left > 0 ? ((left < 64 ? left : 64) - 1) * sld + 4 : 0;
+        }
+    };
+    auto advance = [&]() __attribute__((always_inline)) {
+        if (++fs == a.steps) enter(f_id + grid);
+        else {
+            px += XROW, pw += 64;
+#pragma unroll
+            for (int i = 0; i < Tile::NS; ++i) ps[i] += 4;
+        }
+    };
+    const unsigned lds0 = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)mx_smem);
+    auto rsrc = [](const char* base, int bytes) __attribute__((always_inline)) {
+        return u32x4{(unsigned)reinterpret_cast<uintptr_t>(base), (unsigned)(reinterpret_cast<uintptr_t>(base) >> 32), (unsigned)bytes,
+                     (unsigned)kRsrcFlags};
+    };
+    // In assembly for the reason that m3_gemm.h gives: the kernel waits for its copies itself.
+    auto copy16 = [](u32x4 rs, unsigned off, unsigned at) __attribute__((always_inline)) {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(at), "v"(off), "s"(rs) : "memory");
+    };
+    auto copy4 = [](u32x4 rs, unsigned off, unsigned at) __attribute__((always_inline)) {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" : : "s"(at), "v"(off), "s"(rs) : "memory");
+    };
+    auto fetch = [&](int i, int slot) __attribute__((always_inline)) {
+        const unsigned at = lds0 + slot * Tile::kStage;
+        if (i < Tile::NX) copy16(rsrc(px, bx), xoff[i], at + (wave * Tile::NX + i) * 1024);
+        else if (i < Tile::NX + Tile::NWL) copy16(rsrc(pw, bw), woff[i - Tile::NX], at + Tile::kX + (wave * Tile::NWL + i - Tile::NX) * 1024);
+        else copy4(rsrc(ps[i - Tile::NX - Tile::NWL], bs[i - Tile::NX - Tile::NWL]), soff, at + Tile::kX + Tile::kW + (wave * Tile::NS + i - Tile::NX - Tile::NWL) * 256);
+    };
+
+    // ---- fragments
+    const int r = lane & 31, g = lane >> 5;
+    int xat[2][XP], wat[2];  // of the two halves, within 32 rows
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if constexpr (FA == kE4m3) {
+            xat[h][0] = r * 128 + (((2 * h + g) ^ (r & 7)) * 16);
+            xat[h][XP - 1] = r * 128 + (((4 + 2 * h + g) ^ (r & 7)) * 16);
+        } else {
+            xat[h][0] = r * 64 + (((2 * g + h) ^ (r >> 1 & 3)) * 16);
+        }
+        wat[h] = r * 64 + (((2 * g + h) ^ (r >> 1 & 3)) * 16);
+    }
+    const int sat = r * 4 + 2 * g;
+    constexpr int G = 2 * FM;  // groups of a step
+    i32x4 fx[4][XP], fw[2][FN];
+    int sxr[FM], swr[FN], sxn[FM], swn[FN];  // scales of this step and of the next
+    typedef float f32x16 __attribute__((ext_vector_type(16)));
+    f32x16 acc[FM][FN];
+    auto read_x = [&](int gi, int slot) __attribute__((always_inline)) {  // group gi's
+        const char* p = mx_smem + slot * Tile::kStage + (wm * FM + gi % FM) * 32 * XROW;
+#pragma unroll
+        for (int q = 0; q < XP; ++q) fx[gi % 4][q] = *reinterpret_cast<const i32x4*>(p + xat[gi / FM][q]);
+    };
+    auto read_w = [&](int h, int slot) __attribute__((always_inline)) {
+        const char* p = mx_smem + slot * Tile::kStage + Tile::kX + wn * FN * 2048 + wat[h];
+#pragma unroll
+        for (int i = 0; i < FN; ++i) fw[h][i] = *reinterpret_cast<const i32x4*>(p + i * 2048);
+    };
+    auto read_scales = [&](int slot) __attribute__((always_inline)) {
+        const char* p = mx_smem + slot * Tile::kStage + Tile::kX + Tile::kW + sat;
+#pragma unroll
+        for (int i = 0; i < FN; ++i) swn[i] = *reinterpret_cast<const unsigned short*>(p + Tile::BM * 4 + (wn * FN + i) * 128);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) sxn[i] = *reinterpret_cast<const unsigned short*>(p + (wm * FM + i) * 128);
+    };
+    auto take_scales = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i) swr[i] = swn[i];
+#pragma unroll
+        for (int i = 0; i < FM; ++i) sxr[i] = sxn[i];
+    };
+    auto group = [&](auto gc) __attribute__((always_inline)) {
+        constexpr int gi = decltype(gc)::value, h = gi / FM, i = gi % FM;
+        i32x8 x;
+        if constexpr (XP == 2) x = wide(fx[gi % 4][0], fx[gi % 4][XP - 1]);
+        else x = wide(fx[gi % 4][0], i32x4{0, 0, 0, 0});
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(fw[h][j], i32x4{0, 0, 0, 0}), x, acc[i][j], 4,
+                                                                       FA == kE4m3 ? 0 : 4, h, swr[j], h, sxr[i]);
+    };
+
+    // ---- epilogue: ER rows of 64 columns at a time. Stores go out unconditionally, those past the end to an offset
+    // that the descriptor drops, so that their number is known to the next wait.
+    const bool whole = a.N % 8 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && reinterpret_cast<uintptr_t>(a.res) % 16 == 0;
+    auto epilogue = [&](int id, auto with_res) __attribute__((always_inline)) {
+        constexpr bool kRes = decltype(with_res)::value;
+        constexpr int ER = Tile::ER, T = ER / 8;
+        int m0, n0;
+        tile_of(id, m0, n0);
+        m0 += wm * FM * 32, n0 += wn * 64;
+        const int lane = opaque((int)threadIdx.x) & 63, r = lane & 31, g = lane >> 5;  // not held across the steps
+        char* mine = mx_smem + ST * Tile::kStage + wave * (ER * 128);
+        const bf16* res = reinterpret_cast<const bf16*>(a.res);
+        bf16* out = reinterpret_cast<bf16*>(a.out);
+        // scale times the sums of a round's rows, plus what lies in their place
+        auto combine = [&](int round) __attribute__((always_inline)) {
+            const int i = round * ER / 32;
+            if (ER == 32 || (r >> 4) == round % 2) {
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        bf16x4* at = reinterpret_cast<bf16x4*>(mine + (r & (ER - 1)) * 128 + (((j * 4 + q) ^ (r & 7)) * 16) + g * 8);
+                        bf16x4 o{};
+                        if constexpr (kRes) o = *at;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[e] = (bf16)fmaf(a.scale, acc[i][j][q * 4 + e], kRes ? (float)o[e] : 0.f);
+                        *at = o;
+                    }
+            }
+            M3_LDS_FENCE();  // the fours and the rows' pieces are other types to the compiler
+        };
+        if (whole) {
+            const int rr = lane >> 3, n = n0 + (lane & 7) * 8;
+            // the residual's rows as they lie, a round ahead; past the end a neighbour's, which are not stored
+            bf16x8 rv[kRes ? 2 : 1][T];
+            auto read_res = [&](int round, int to) __attribute__((always_inline)) {
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+                    const int m = m0 + round * ER + t * 8 + rr;
+                    rv[kRes ? to : 0][t] = *reinterpret_cast<const bf16x8*>(res + (int64_t)(m < a.M ? m : a.M - 1) * a.N + (n < a.N ? n : a.N - 8));
+                }
+            };
+            if constexpr (kRes) read_res(0, 0);
+#pragma unroll
+            for (int round = 0; round < FM * 32 / ER; ++round) {
+                if constexpr (kRes) {
+                    if (round + 1 < FM * 32 / ER) read_res(round + 1, (round + 1) % 2);
+#pragma unroll
+                    for (int t = 0; t < T; ++t)
+                        *reinterpret_cast<bf16x8*>(mine + (t * 8 + rr) * 128 + (((lane & 7) ^ rr) * 16)) = rv[round % 2][t];
+                    M3_LDS_FENCE();
+                }
+                combine(round);
+                const int m1 = m0 + round * ER, rows = a.M - m1 < ER ? a.M - m1 : ER;
+                const __amdgpu_buffer_rsrc_t to = make_rsrc(out + (int64_t)m1 * a.N, rows > 0 ? (int64_t)rows * a.N * 2 : 0);
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+                    const u32x4 v = *reinterpret_cast<const u32x4*>(mine + (t * 8 + rr) * 128 + (((lane & 7) ^ rr) * 16));
+                    __builtin_amdgcn_raw_buffer_store_b128(v, to, n < a.N ? ((t * 8 + rr) * a.N + n) * 2 : (int)0x80000000u, 0, 0);
+                }
+                M3_LDS_FENCE();
+            }
+        } else {
+            // rows of any alignment: a column a lane
+            const int n = n0 + lane, nc = n < a.N ? n : a.N - 1;
+            bf16* cell = reinterpret_cast<bf16*>(mine) + (lane & 7);
+            auto at = [&](int row) __attribute__((always_inline)) { return cell + row * 64 + (((lane >> 3) ^ (row & 7)) * 8); };
+#pragma unroll
+            for (int round = 0; round < FM * 32 / ER; ++round) {
+                const int m1 = m0 + round * ER;
+                if constexpr (kRes) {
+                    bf16 v[ER];
+#pragma unroll
+                    for (int e = 0; e < ER; ++e) v[e] = res[(int64_t)(m1 + e < a.M ? m1 + e : a.M - 1) * a.N + nc];
+#pragma unroll
+                    for (int e = 0; e < ER; ++e) *at(e) = v[e];
+                    M3_LDS_FENCE();
+                }
+                combine(round);
+#pragma unroll
+                for (int e = 0; e < ER; ++e) {
+                    const bf16 v = *at(e);
+                    if (m1 + e < a.M && n < a.N) out[(int64_t)(m1 + e) * a.N + n] = v;
+                }
+                M3_LDS_FENCE();
+            }
+            asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // the stores' number is not known
+        }
+    };
+
+    if ((int)blockIdx.x >= total) return;
+    enter((int)blockIdx.x);
+#pragma unroll
+    for (int s = 0; s < ST; ++s) {
+        if (s) advance();
+#pragma unroll
+        for (int i = 0; i < NLD; ++i) fetch(i, s);
+    }
+    auto wait = [](auto n) __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(decltype(n)::value) : "memory");
+    };
+    wait(std::integral_constant<int, NLD*(ST - 1)>{});
+    M3_LDS_FENCE();
+    __builtin_amdgcn_s_barrier();
+    M3_LDS_FENCE();
+    int slot = 0;
+    read_scales(0);
+    read_w(0, 0);
+    read_x(0, 0);
+    read_x(1, 0);
+    take_scales();
+    constexpr int kPerLd = (NLD + 1) / 2;
+    // kStored: the epilogue before has just sent its stores, behind the copies that this step waits for
+    auto step = [&](auto stored) __attribute__((always_inline)) {
+        constexpr int kYounger = NLD * (ST - 2) + (decltype(stored)::value ? Tile::kStores : 0);
+        const int next = slot + 1 == ST ? 0 : slot + 1;
+        auto at = [&](auto gc) __attribute__((always_inline)) {
+            constexpr int gi = decltype(gc)::value;
+            if constexpr (gi == G - 2) {
+                // the next step has landed (memory operations end in order: what may be on its way is what was sent
+                // after its copies), and all waves have read this one
+                wait(std::integral_constant<int, kYounger>{});
+                M3_LDS_FENCE();
+                __builtin_amdgcn_s_barrier();
+                M3_LDS_FENCE();
+                read_scales(next);
+                read_w(0, next);
+            }
+            if constexpr (gi >= G - 2) {
+#pragma unroll
+                for (int t = (gi - G + 2) * kPerLd; t < (gi - G + 3) * kPerLd && t < NLD; ++t) fetch(t, slot);
+                read_x(gi + 2 - G, next);
+            } else {
+                if constexpr (gi == FM - 2) read_w(1, slot);
+                read_x(gi + 2, slot);
+            }
+            M3_FENCE();
+            group(gc);
+            M3_FENCE();
+        };
+        advance();
+        M3_FENCE();
+        mx_each(std::make_integer_sequence<int, G>{}, at);  // (no branch: the compiler would move products behind it)
+        take_scales();
+        slot = next;
+    };
+    for (int id = (int)blockIdx.x; id < total; id += grid) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = f32x16{};
+        if (id == (int)blockIdx.x) step(std::false_type{});
+        else step(std::true_type{});
+        for (int n = a.steps; n > 1; --n) step(std::false_type{});
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) asm volatile("" : "+v"(acc[i][j]));  // the last products before the epilogue's branches
+        if (a.res) epilogue(id, std::true_type{});
+        else epilogue(id, std::false_type{});
+    }
+    // no copy outlives its block
+    wait(std::integral_constant<int, 0>{});
+}
+
+template <typename Tile>
+static int tile_t(const MxLinearArgs& a, hipStream_t stream) {
+    const int64_t tm = (a.M + Tile::BM - 1) / Tile::BM, tn = (a.N + Tile::BN - 1) / Tile::BN;
+    if (tm * tn > (1 << 30) || a.N > (1 << 25)) return M3_ERR_UNSUPPORTED;  // 32 rows of results within a descriptor
+    static std::atomic<uint64_t> done{0};
+    if (!allow_lds(reinterpret_cast<const void*>(&mx_linear_tile_kernel<Tile>), Tile::kLds, done)) return M3_ERR_LAUNCH;
+    const int64_t most = 256 * (Tile::NT >= 512 ? 1 : 2);  // blocks at once
+    hipLaunchKernelGGL((mx_linear_tile_kernel<Tile>), dim3((unsigned)std::min(tm * tn, most)), dim3(Tile::NT), Tile::kLds, stream, a,
+                       (int)tm, (int)tn);
+    return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH;
+}
+// Which kernel, by the number of 128 x 128 and 256 x 256 tiles (us in a graph, e4m3, few rows' kernel and 128 x 128 tiles):
+// 16 x 2048 x 11008 7.3 and 9.3, x 128000 41 and 29; 32 x 2048 x 11008 9.1 and 9.2, 32 x 768 x 32000 6.6 and 5.9;
+// 64 x 2048 x 11008 12.4 and 9.8, 64 x 768 x 3696 4.4 and 5.6, 256 x 768 x 3696 6.5 and 5.9, 1000 x 768 x 4224 19 and 9.1.
+// 128 x 128 and 256 x 256 tiles: 8192 x 768 x 4224 32 and 37, 8192 x 2112 x 768 19 and 27, 8192 x 5504 x 2048 105 and 76,
+// 16 x 2048 x 128000 29 and 45.
+static bool takes_tiles(const MxLinearArgs& a) {
+    const int64_t tiles = (int64_t)((a.M + 127) / 128) * ((a.N + 127) / 128);
+    return tiles >= (a.M <= 16 ? 512 : a.M <= 32 ? 200 : 56);
 }
 template <int FA, typename TO>
 static int linear_t(const MxLinearArgs& a, hipStream_t stream) {
-    if (a.M <= 16) return few_t<FA, 1, 1, TO>(a, stream);
-    if (a.M <= 32) return few_t<FA, 2, 2, TO>(a, stream);
-    return few_t<FA, 4, 4, TO>(a, stream);
+    if constexpr (sizeof(TO) == 2) {
+        if (takes_tiles(a)) {
+            const int64_t large = (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256);
+            return large >= 192 && a.steps >= 12 && a.M > 128 ? tile_t<MxTile<FA, 256, 256, 2, 4, 2, 32>>(a, stream) : tile_t<MxTile<FA, 128, 128, 2, 2, 2, 32>>(a, stream);
+        }
+    }
+    if (a.M <= 16) return few_m<FA, 1, TO>(a, stream);
+    if (a.M <= 32) return few_m<FA, 2, TO>(a, stream);
+    return few_m<FA, 4, TO>(a, stream);
 }
 
+static MxLinearArgs linear_args(const void* x, const void* xs, const void* w, const void* ws, const void* res, float scale, void* out,
+                                int m, int n, int k) {
+    const auto b = [](const void* p) { return reinterpret_cast<const uint8_t*>(p); };
+    return MxLinearArgs{b(x), b(xs), b(w), b(ws), res, out, scale, m, n, (int)(mx_padded(k) / kMxStep)};
+}
+bool mx_linear_takes_tensor(int64_t m, int64_t n, int64_t k, int out_dtype) {
+    if (m > kMlRawRows || m * mx_padded(k) > kMlRawBytes) return false;
+    const MxLinearArgs a = linear_args(nullptr, nullptr, nullptr, nullptr, nullptr, 1.f, nullptr, (int)m, (int)n, (int)k);
+    return out_dtype != M3_DTYPE_BF16 || !takes_tiles(a);
+}
+int launch_mx_linear_tensor(const void* x, int x_dtype, const void* w, const void* ws, const void* res, float scale, void* out,
+                            int out_dtype, int m, int n, int k, hipStream_t stream) {
+    const MxLinearArgs a = linear_args(x, nullptr, w, ws, res, scale, out, m, n, k);
+    if (x_dtype == M3_DTYPE_BF16) return out_dtype == M3_DTYPE_BF16 ? raw_n<bf16, bf16>(a, k, stream) : raw_n<bf16, float>(a, k, stream);
+    return out_dtype == M3_DTYPE_BF16 ? raw_n<float, bf16>(a, k, stream) : raw_n<float, float>(a, k, stream);
+}
 int launch_mx_linear(const void* x, const void* xs, int x_format, const void* w, const void* ws, const void* res, float scale,
                      void* out, int out_dtype, int m, int n, int k, hipStream_t stream) {
-    const auto b = [](const void* p) { return reinterpret_cast<const uint8_t*>(p); };
-    const MxLinearArgs a{b(x), b(xs), b(w), b(ws), res, out, scale, m, n, (int)(mx_padded(k) / kMxStep)};
+    const MxLinearArgs a = linear_args(x, xs, w, ws, res, scale, out, m, n, k);
     if (out_dtype == M3_DTYPE_BF16) return x_format == kE4m3 ? linear_t<kE4m3, bf16>(a, stream) : linear_t<kE2m1, bf16>(a, stream);
     return x_format == kE4m3 ? linear_t<kE4m3, float>(a, stream) : linear_t<kE2m1, float>(a, stream);
 }

@@ -3,16 +3,19 @@
 //   kept: the first k of them, of these the shortest run whose mass reaches p of the k's, and of these the
 //   ones with mass >= m; token = the first whose running mass passes u times the kept mass.
 // Every bound cuts the same order, so what is kept is a prefix, and each step is the question which
-// token of the order a count or a mass falls on. It is answered without sorting the row:
-//   sample_top:   each row's largest logit (its lowest index), in slices over many blocks;
-//   sample_bins:  counts and masses by distance from it, 1024 bins of 1/32;
-//   sample_pick:  one block a row finds the bin, gathers its tokens (the row is read once more), sorts them
-//                 and walks on; a bin with more than 2048 tokens is split by its keys' bits first.
-// Masses are added as whole numbers of 2^-45 or so, so that sums do not depend on their order, and come
-// from an exponential in 64 bits (a Taylor series of 2^f, |f| <= 1/2, to 1e-13 of its value): a border is
-// missed with a probability of about 1e-9 a row, as with 64-bit sums over sorted probabilities.
-// Bound by the row's three reads.
+// token of the order a count or a mass falls on. It is answered without sorting the row. One block takes a row and holds
+// its first 126 KB in LDS (the rest is read anew in each pass: 256 rows of 128000 fp32 logits come from the last-level
+// cache). It finds the largest logit; adds up masses (and where top_k asks, counts) by distance from it, in 1024 bins
+// of T / 32; and gathers the tokens of the bins that may be kept, up to 1024, sorts them and reads the answers off. With
+// more, each question gathers the one bin that it falls in, which is split by its keys' bits until it fits.
+// With q = 32 (max z - z) / T in 64 bits, a token's mass is exp(-b / 32) exp(-r / 32), b the bin and r < 1: the bins add up
+// exp(-r / 32), five terms of its series to 1e-12, as whole numbers of 2^-45 or so, so that sums do not depend on their
+// order; exp(-b / 32) comes in once a bin. (An exponential for each token took three times as long.) What lies past the last bin
+// but one, below exp(-32) of the likeliest, is counted but has no mass. A border is missed with a probability of about
+// 1e-10 a row, as with 64-bit sums over sorted probabilities.
+// Bound by the row's read for large batches, by the chain of passes and barriers for few rows.
 #include <algorithm>
+#include <atomic>
 
 #include "m3_common.h"
 #include "m3_kernels.h"
@@ -22,11 +25,11 @@
 namespace m3 {
 
 typedef unsigned long long u64;
-constexpr int kSpThreads = 256;
+constexpr int kSpThreads = 512;
+constexpr int kSpWaves = kSpThreads / 64;
 constexpr int kSpBins = 1024;
-constexpr int kSpList = 2048;
-constexpr int kSpSlices = 64;  // most of a row
-constexpr int kSpPick = 1024;  // threads of sample_pick
+constexpr int kSpList = 1024;
+constexpr int kSpHeld = 126 << 10;  // bytes of a row in LDS
 
 struct SampleArgs {
     const void* z;
@@ -38,17 +41,14 @@ struct SampleArgs {
     int64_t top_k1;
     int64_t* token;
     float* logprob;
-    int rows, vocab, slices, slice;  // slice: logits of each
-    u64* top;       // [rows][slices]
-    u64* mass;      // [rows][kSpBins]
-    unsigned* count;
-    int shift;      // masses are whole numbers of 2^-shift
+    int64_t rows;
+    int vocab;
+    int shift;  // masses are whole numbers of 2^-shift
 };
 
-// Order of logits as whole numbers; -0 as 0, NaN as -infinity, which is no token.
+// Logits as whole numbers that keep their order, -0 as 0.
 __device__ __forceinline__ unsigned sp_key(float z) {
-    z = z != z ? -INFINITY : z + 0.f;
-    const unsigned b = __builtin_bit_cast(unsigned, z);
+    const unsigned b = __builtin_bit_cast(unsigned, z + 0.f);
     return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
 __device__ __forceinline__ float sp_logit(unsigned key) {
@@ -56,37 +56,34 @@ __device__ __forceinline__ float sp_logit(unsigned key) {
 }
 constexpr unsigned kSpNone = 0x007fffffu;  // the key of -infinity
 
-__device__ __forceinline__ int sp_bin(float top, float z) {
-    const float far = (top - z) * 32.f;  // NaN for two infinities, which are the same logit
-    return z == top ? 0 : far < (float)(kSpBins - 1) ? (int)far : kSpBins - 1;
+// Distances from the largest logit in bins, as 64-bit numbers (NaN for NaN).
+struct SampleScale {
+    double top, per;  // per = 32 / T
+    int shift;        // masses are whole numbers of 2^-shift
+    __device__ __forceinline__ double far(float z) const { return (top - (double)z) * per; }
+    // a logit at least as near as q, with room for rounding: what is below it is further
+    __device__ __forceinline__ float near(double q) const {
+        const double z = top - (q + 1e-6) / per;
+        return (float)(z - fabs(z) * 1e-6);
+    }
+};
+__device__ __forceinline__ bool sp_in(double q, int bin) { return q >= (double)bin && (q < (double)(bin + 1) || bin == kSpBins - 1); }
+constexpr double kSpWhole = 4503599627370496.0;  // 2^52: what is added to it is rounded to a whole number, in its low bits
+__device__ __forceinline__ u64 sp_whole(double v) {  // of 0 <= v < 2^52
+    return __builtin_bit_cast(u64, v + kSpWhole) & 0x000fffffffffffffull;
 }
-// 2^shift mass of a logit, rounded: c = log2(e) / T.
-__device__ __forceinline__ u64 sp_mass(float top, float z, double c, int shift) {
-    const double x = z == top ? 0.0 : ((double)z - (double)top) * c;
-    if (!(x > -64.0)) return 0;  // below half of 2^-62; NaN, an infinity times 0, too
-    const double n = rint(x), f = (x - n) * 0.69314718055994530942;
-    double e = 1.0 / 6227020800.0;
-    e = fma(e, f, 1.0 / 479001600.0);
-    e = fma(e, f, 1.0 / 39916800.0);
-    e = fma(e, f, 1.0 / 3628800.0);
-    e = fma(e, f, 1.0 / 362880.0);
-    e = fma(e, f, 1.0 / 40320.0);
-    e = fma(e, f, 1.0 / 5040.0);
-    e = fma(e, f, 1.0 / 720.0);
-    e = fma(e, f, 1.0 / 120.0);
-    e = fma(e, f, 1.0 / 24.0);
-    e = fma(e, f, 1.0 / 6.0);
-    e = fma(e, f, 0.5);
-    e = fma(e, f, 1.0);
-    e = fma(e, f, 1.0);
-    return (u64)(ldexp(e, (int)n + shift) + 0.5);
+// A token's mass, and that times 2^shift as a whole number (shift <= 51), none past the last bin but one.
+__device__ __forceinline__ double sp_exp(const SampleScale& s, float z) { return exp(s.far(z) * (-1.0 / 32.0)); }
+__device__ __forceinline__ u64 sp_mass(const SampleScale& s, float z) {
+    const double q = s.far(z);
+    return q < (double)(kSpBins - 1) ? sp_whole(ldexp(exp(q * (-1.0 / 32.0)), s.shift)) : 0;
 }
 
 struct SampleRow {
     double t, p, m;
     int64_t k;
 };
-__device__ __forceinline__ SampleRow sp_row(const SampleArgs& a, int row) {
+__device__ __forceinline__ SampleRow sp_row(const SampleArgs& a, int64_t row) {
     SampleRow r;
     r.t = a.temperature ? (double)a.temperature[row] : a.temperature1;
     r.p = a.top_p ? (double)a.top_p[row] : a.top_p1;
@@ -96,87 +93,89 @@ __device__ __forceinline__ SampleRow sp_row(const SampleArgs& a, int row) {
     return r;
 }
 
+// A row's logits, in pieces of 16 bytes: the first `held` in LDS, the others in memory.
 template <typename T>
-__global__ __launch_bounds__(kSpThreads) void sample_top_kernel(SampleArgs a) {
-    const int row = blockIdx.y, s = blockIdx.x;
-    const T* z = reinterpret_cast<const T*>(a.z) + (int64_t)row * a.vocab;
-    const int v0 = s * a.slice, v1 = v0 + a.slice < a.vocab ? v0 + a.slice : a.vocab;
-    u64 best = 0;  // key, then the complement of the index
-    for (int v = v0 + (int)threadIdx.x * 8; v < v1; v += kSpThreads * 8) {
-        float f[8];
-        load8(z, v, v1, f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const u64 k = (u64)sp_key(f[e]) << 32 | (unsigned)~(v + e);
-            if (v + e < v1 && k > best) best = k;
-        }
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        const u64 o = __shfl_xor(best, off, kWave);
-        best = o > best ? o : best;
-    }
-    __shared__ u64 red[kSpThreads / 64];
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = best;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-#pragma unroll
-        for (int i = 1; i < kSpThreads / 64; ++i) best = red[i] > best ? red[i] : best;
-        a.top[(int64_t)row * a.slices + s] = best;
-    }
-    // this slice's share of the row's bins, for the next kernel to add to
-    for (int b = s * kSpThreads + (int)threadIdx.x; b < kSpBins; b += a.slices * kSpThreads) {
-        a.mass[(int64_t)row * kSpBins + b] = 0;
-        a.count[(int64_t)row * kSpBins + b] = 0;
-    }
-}
+struct SampleLogits {
+    static constexpr int E = 16 / sizeof(T);
+    u32x4* lds;
+    const T* z;
+    int vocab, held;
 
-// The row's largest logit and its index's complement, by one wave.
-__device__ __forceinline__ u64 sp_top(const SampleArgs& a, int row) {
-    const int lane = threadIdx.x & 63;
-    u64 v = lane < a.slices ? a.top[(int64_t)row * a.slices + lane] : 0;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        const u64 o = __shfl_xor(v, off, kWave);
-        v = o > v ? o : v;
+    static __device__ __forceinline__ float get(const u32x4& w, int e) {
+        // (a bit cast of the vector's component itself takes the first one with this compiler)
+        const unsigned u = w[sizeof(T) == 4 ? e : e / 2];
+        return __builtin_bit_cast(float, sizeof(T) == 4 ? u : e & 1 ? u & 0xffff0000u : u << 16);
     }
-    return v;
-}
-
-template <typename T>
-__global__ __launch_bounds__(kSpThreads) void sample_bins_kernel(SampleArgs a) {
-    __shared__ u64 mass[kSpBins];
-    __shared__ unsigned count[kSpBins];
-    const int row = blockIdx.y;
-    const SampleRow r = sp_row(a, row);
-    const unsigned key = (unsigned)(sp_top(a, row) >> 32);
-    if (!(r.t > 0.0) || key <= kSpNone) return;  // greedy, or no token
-    const float top = sp_logit(key);
-    const double c = 1.4426950408889634074 / r.t;
-    for (int b = threadIdx.x; b < kSpBins; b += kSpThreads) mass[b] = 0, count[b] = 0;
-    __syncthreads();
-    const T* z = reinterpret_cast<const T*>(a.z) + (int64_t)row * a.vocab;
-    const int v0 = (int)blockIdx.x * a.slice, v1 = v0 + a.slice < a.vocab ? v0 + a.slice : a.vocab;
-    for (int v = v0 + (int)threadIdx.x * 8; v < v1; v += kSpThreads * 8) {
-        float f[8];
-        load8(z, v, v1, f);
+    // element e, known at run time only
+    static __device__ __forceinline__ float pick(const u32x4& w, int e) {
+        const int d = sizeof(T) == 4 ? e : e >> 1;
+        const unsigned a = w[0], b = w[1], c = w[2], g = w[3];
+        const unsigned u = d < 2 ? (d == 0 ? a : b) : (d == 2 ? c : g);
+        return __builtin_bit_cast(float, sizeof(T) == 4 ? u : e & 1 ? u & 0xffff0000u : u << 16);
+    }
+    // piece p; past the row's end -infinity
+    __device__ __forceinline__ u32x4 read(int p) const {
+        const int v = p * E;
+        T t[E];
+        if (v + E <= vocab) {
+            __builtin_memcpy(t, z + v, 16);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if (v + e >= v1 || !(f[e] > -INFINITY)) continue;
-            const int b = sp_bin(top, f[e]);
-            atomicAdd(&count[b], 1u);
-            const u64 m = sp_mass(top, f[e], c, a.shift);
-            if (m) atomicAdd(&mass[b], m);
+            for (int e = 0; e < E; ++e) t[e] = v + e < vocab ? z[v + e] : (T)-INFINITY;
+        }
+        return __builtin_bit_cast(u32x4, t);
+    }
+    template <typename F>
+    __device__ __forceinline__ void pieces_from(int p0, int p1, F f) const {  // f(piece, its index), three more in flight
+        const int p = p0 + (int)threadIdx.x;
+        if (p0 >= p1) return;
+        u32x4 w0 = read(p), w1 = read(p + kSpThreads), w2 = read(p + 2 * kSpThreads), w3 = read(p + 3 * kSpThreads);
+#pragma unroll 1
+        for (int i = p; i < p1; i += kSpThreads) {
+            f(w0, i);
+            w0 = w1, w1 = w2, w2 = w3, w3 = read(i + 4 * kSpThreads);
         }
     }
-    __syncthreads();
-    for (int b = threadIdx.x; b < kSpBins; b += kSpThreads) {
-        if (count[b]) {
-            atomicAdd(&a.count[(int64_t)row * kSpBins + b], count[b]);
-            atomicAdd(&a.mass[(int64_t)row * kSpBins + b], mass[b]);
+    // f(logit, index) for all of them, by the whole block; what is past the end comes as -infinity.
+    // kFirst: the pass that fills LDS.
+    template <bool kFirst, typename F>
+    __device__ __forceinline__ void each(F f) const {
+        auto one = [&](const u32x4& w, int p) __attribute__((always_inline)) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) f(get(w, e), p * E + e);
+        };
+        if constexpr (kFirst) {
+            pieces_from(0, held, [&](const u32x4& w, int p) __attribute__((always_inline)) {
+                lds[p] = w;
+                one(w, p);
+            });
+        } else {
+#pragma unroll 2
+            for (int p = threadIdx.x; p < held; p += kSpThreads) one(lds[p], p);
         }
+        pieces_from(held, (vocab + E - 1) / E, one);
     }
-}
+    // The same for the logits in [lo, hi]: a piece's are marked first, without a branch, and then taken one by one.
+    template <typename F>
+    __device__ __forceinline__ void each_in(float lo, float hi, F f) const {
+        auto one = [&](const u32x4& w, int p) __attribute__((always_inline)) {
+            unsigned marks = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float x = get(w, e);
+                marks |= ((x >= lo) & (x <= hi)) ? 1u << e : 0u;
+            }
+            while (marks) {
+                const int e = __builtin_ctz(marks);
+                marks &= marks - 1;
+                f(pick(w, e), p * E + e);
+            }
+        };
+#pragma unroll 2
+        for (int p = threadIdx.x; p < held; p += kSpThreads) one(lds[p], p);
+        pieces_from(held, (vocab + E - 1) / E, one);
+    }
+};
 
 // A place in the row's order: everything before it has `count` tokens and `mass`; it is the tie-th token (from 0)
 // of those with this key.
@@ -188,31 +187,66 @@ struct SamplePlace {
     int index;        // -1: not known yet
 };
 
-// One block's working memory.
+// The block's working memory.
 struct SampleShared {
-    u64 mass[kSpBins];
-    unsigned count[kSpBins];
-    u64 list[kSpList];      // key, complement of the index
-    u64 wmass[kSpPick / 64];
-    unsigned wcount[kSpPick / 64];
-    unsigned n, lo, hi;
+    u64 mass[kSpBins + 64];  // of the row's bins, and a place for each lane's tokens without mass
+    unsigned count[kSpBins + 64];
+    union {
+        struct {
+            u64 list[kSpList];    // key, complement of the index: as gathered, then from the largest down
+            u64 parted[kSpList];  // by parts of the keys' span
+        };
+        struct {            // of a split bin's parts
+            u64 smass[kSpBins];
+            unsigned scount[kSpBins];
+        };
+    };
+    unsigned parts[kSpList];
+    u64 wmass[kSpWaves];
+    unsigned wcount[kSpWaves];
+    unsigned n;
     int at;
-    u64 before_mass, found;
+    u64 before_mass;
     unsigned before_count;
     SamplePlace place;
 };
 
-// Exclusive sums of c and m over the block's threads, in their order.
+// Inclusive sums over a wave's lanes, by lane moves.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ unsigned sp_move(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, kRows, 0xf, true); }
+template <int kCtrl, int kRows = 0xf>
+__device__ __forceinline__ void sp_add(unsigned& c, u64& m) {
+    c += sp_move<kCtrl, kRows>(c);
+    m += (u64)sp_move<kCtrl, kRows>((unsigned)(m >> 32)) << 32 | sp_move<kCtrl, kRows>((unsigned)m);
+}
+// The largest over a wave's lanes.
+__device__ __forceinline__ unsigned sp_max(unsigned v) {
+    auto with = [&](auto ctrl) __attribute__((always_inline)) {
+        const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xF, 0xF, false);
+        v = o > v ? o : v;
+    };
+    with(std::integral_constant<int, 0xB1>{});
+    with(std::integral_constant<int, 0x4E>{});
+    with(std::integral_constant<int, 0x141>{});
+    with(std::integral_constant<int, 0x140>{});
+#pragma unroll
+    for (int off = 16; off < 64; off <<= 1) {
+        const unsigned o = __shfl_xor(v, off, kWave);
+        v = o > v ? o : v;
+    }
+    return v;
+}
+// Exclusive sums of c and m over the block's threads, in their order, and all of them.
 __device__ __forceinline__ void sp_scan(SampleShared& s, unsigned& c, u64& m, unsigned& all_c, u64& all_m) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     unsigned ic = c;
     u64 im = m;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const unsigned oc = __shfl_up(ic, off, kWave);
-        const u64 om = __shfl_up(im, off, kWave);
-        if (lane >= off) ic += oc, im += om;
-    }
+    sp_add<kRowShr + 1>(ic, im);
+    sp_add<kRowShr + 2>(ic, im);
+    sp_add<kRowShr + 4>(ic, im);
+    sp_add<kRowShr + 8>(ic, im);
+    sp_add<kRowBcast15, 0xa>(ic, im);
+    sp_add<kRowBcast31, 0xc>(ic, im);
     __syncthreads();
     if (lane == 63) s.wcount[wave] = ic, s.wmass[wave] = im;
     __syncthreads();
@@ -220,208 +254,271 @@ __device__ __forceinline__ void sp_scan(SampleShared& s, unsigned& c, u64& m, un
     u64 bm = 0;
     all_c = 0, all_m = 0;
 #pragma unroll
-    for (int w = 0; w < kSpPick / 64; ++w) {
+    for (int w = 0; w < kSpWaves; ++w) {
         if (w == wave) bc = all_c, bm = all_m;
         all_c += s.wcount[w], all_m += s.wmass[w];
     }
     c = bc + ic - c, m = bm + im - m;
 }
 
-// Which bin of s.mass / s.count is the first whose end reaches the goal: `goal_c` tokens, or with kByMass a mass
-// of at least (kPast: above) `goal_m`. s.at: the bin (-1: none), s.before_*: what lies before it, base included.
-template <bool kByMass, bool kPast>
-__device__ __forceinline__ void sp_find_bin(SampleShared& s, u64 base_c, u64 base_m, u64 goal_c, double goal_m) {
-    constexpr int kPer = kSpBins / kSpPick;
-    static_assert(kPer * kSpPick == kSpBins && kSpList % kSpPick == 0, "whole shares");
+// What is looked for: the `count`-th token (kCount), or the first whose running mass is at least (kReach), or above
+// (kPass), `mass`.
+enum { kCount, kReach, kPass };
+struct SampleGoal {
+    int kind;
+    u64 count;
+    double mass;
+    __device__ __forceinline__ bool reached(u64 c, u64 m) const {
+        return kind == kCount ? c >= count : kind == kReach ? (double)m >= mass : (double)m > mass;
+    }
+};
+
+// The bin (s.at) whose end reaches the goal and whose start does not, or where none does `otherwise` (-1: none); s.before_*:
+// what lies before it, without base_*.
+__device__ __forceinline__ void sp_find_bin(SampleShared& s, const u64* mass, const unsigned* count, u64 base_c, u64 base_m, const SampleGoal& goal,
+                                            int otherwise) {
+    constexpr int kPer = kSpBins / kSpThreads;
+    static_assert(kPer * kSpThreads == kSpBins && kSpList % kSpThreads == 0, "whole shares");
     unsigned c[kPer], tc = 0, all_c;
     u64 m[kPer], tm = 0, all_m;
-    __syncthreads();
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        c[i] = s.count[threadIdx.x * kPer + i], m[i] = s.mass[threadIdx.x * kPer + i];
+        c[i] = count[threadIdx.x * kPer + i], m[i] = mass[threadIdx.x * kPer + i];
         tc += c[i], tm += m[i];
     }
     if (threadIdx.x == 0) s.at = -1;
-    unsigned pc = tc;
-    u64 pm = tm;
-    sp_scan(s, pc, pm, all_c, all_m);
-    __syncthreads();
-    auto reached = [&](u64 cc, u64 mm) { return kByMass ? (kPast ? (double)mm > goal_m : (double)mm >= goal_m) : cc >= goal_c; };
+    sp_scan(s, tc, tm, all_c, all_m);
+    const bool missed = !goal.reached(base_c + all_c, base_m + all_m);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        // the one bin that is reached and whose start is not
-        if (c[i] && reached(base_c + pc + c[i], base_m + pm + m[i]) && !reached(base_c + pc, base_m + pm)) {
-            s.at = (int)threadIdx.x * kPer + i;
-            s.before_count = pc, s.before_mass = pm;
+        const int b = (int)threadIdx.x * kPer + i;
+        if (missed ? b == otherwise : goal.reached(base_c + tc + c[i], base_m + tm + m[i]) && !goal.reached(base_c + tc, base_m + tm)) {
+            s.at = b;
+            s.before_count = tc, s.before_mass = tm;
         }
-        pc += c[i], pm += m[i];
+        tc += c[i], tm += m[i];
     }
     __syncthreads();
 }
 
-// Calls f(key, index, logit) for the row's tokens, by the whole block: 32 logits a thread are read at once.
-template <typename T, typename F>
-__device__ __forceinline__ void sp_all(const T* z, int vocab, F f) {
-    constexpr int kU = 4;
-    for (int v0 = (int)threadIdx.x * 8; v0 < vocab; v0 += kSpPick * 8 * kU) {
-        float x[kU][8];
+// The smallest lo and the largest hi of the block's threads.
+__device__ __forceinline__ void sp_span(SampleShared& s, unsigned& lo, unsigned& hi) {
+    const unsigned a = ~sp_max(~lo), b = sp_max(hi);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s.wmass[threadIdx.x >> 6] = (u64)a << 32 | b;
+    __syncthreads();
+    lo = 0xffffffffu, hi = 0;
 #pragma unroll
-        for (int i = 0; i < kU; ++i) load8(z, v0 + i * kSpPick * 8, vocab, x[i]);
-#pragma unroll
-        for (int i = 0; i < kU; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int v = v0 + i * kSpPick * 8 + e;
-                const unsigned key = sp_key(x[i][e]);
-                if (v < vocab && key > kSpNone) f(key, v, x[i][e]);
-            }
+    for (int w = 0; w < kSpWaves; ++w) {
+        const unsigned x = (unsigned)(s.wmass[w] >> 32), y = (unsigned)s.wmass[w];
+        lo = x < lo ? x : lo;
+        hi = y > hi ? y : hi;
     }
 }
-// For those of bin `bin` with keys in [lo, hi].
-template <typename T, typename F>
-__device__ __forceinline__ void sp_each(const T* z, int vocab, float top, int bin, unsigned lo, unsigned hi, F f) {
-    sp_all(z, vocab, [&](unsigned key, int v, float x) {
-        if (key >= lo && key <= hi && sp_bin(top, x) == bin) f(key, v, x);
-    });
-}
-
-// The token of the row's order on which a count (`goal_c`: the goal_c-th token is the answer) or a mass falls
-// (kByMass: the first whose running mass is at least, or with kPast above, goal_m). mass0 / count0: the row's bins
-// in global memory. The answer is in s.place; goals lie within the row.
-template <typename T, bool kByMass, bool kPast>
-__device__ void sp_locate(const SampleArgs& a, SampleShared& s, const T* z, int row, float top, double c, u64 goal_c, double goal_m) {
-    __syncthreads();
-    for (int b = threadIdx.x; b < kSpBins; b += kSpPick) {
-        s.mass[b] = a.mass[(int64_t)row * kSpBins + b];
-        s.count[b] = a.count[(int64_t)row * kSpBins + b];
+// Sorts the first n of the list from the largest key (and the lowest index) down: by 1024 parts of the keys' span, and within
+// a part by counting the larger ones; where a part has more than 48 (equal logits), all by exchanges of pairs.
+__device__ __forceinline__ void sp_sort(SampleShared& s, unsigned n) {
+    constexpr int kPer = kSpList / kSpThreads;
+    u64 mine[kPer];
+    unsigned klo = 0xffffffffu, khi = 0, part[kPer], nth[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const unsigned j = threadIdx.x + i * kSpThreads;
+        s.parts[j] = 0;
+        mine[i] = j < n ? s.list[j] : 0;
+        const unsigned key = (unsigned)(mine[i] >> 32);
+        if (j < n) klo = key < klo ? key : klo, khi = key > khi ? key : khi;
     }
-    sp_find_bin<kByMass, kPast>(s, 0, 0, goal_c, goal_m);
-    const int bin = s.at;
-    if (bin < 0) {  // not within the row: the caller's goals rule it out
-        if (threadIdx.x == 0) s.place = SamplePlace{kSpNone, 0, 0, 0, 0, 0};
-        __syncthreads();
-        return;
-    }
-    u64 base_c = s.before_count, base_m = s.before_mass;
-    unsigned lo = 0, hi = 0xffffffffu, n = s.count[bin];
-    // too many to sort: split the keys' span in 1024 until few are left, or one key
-    while (n > kSpList) {
-        __syncthreads();
-        if (threadIdx.x == 0) s.lo = 0xffffffffu, s.hi = 0;
-        for (int b = threadIdx.x; b < kSpBins; b += kSpPick) s.mass[b] = 0, s.count[b] = 0;
-        __syncthreads();
-        unsigned klo = 0xffffffffu, khi = 0;
-        sp_each(z, a.vocab, top, bin, lo, hi, [&](unsigned key, int, float) {
-            klo = key < klo ? key : klo;
-            khi = key > khi ? key : khi;
-        });
-        atomicMin(&s.lo, klo);
-        atomicMax(&s.hi, khi);
-        __syncthreads();
-        lo = s.lo, hi = s.hi;
-        if (lo == hi) break;
-        int shift = 0;
-        while ((hi - lo) >> shift >= (unsigned)kSpBins) ++shift;
-        // from the largest key down
-        sp_each(z, a.vocab, top, bin, lo, hi, [&](unsigned key, int, float x) {
-            const int b = (int)((hi - key) >> shift);
-            atomicAdd(&s.count[b], 1u);
-            atomicAdd(&s.mass[b], sp_mass(top, x, c, a.shift));
-        });
-        sp_find_bin<kByMass, kPast>(s, base_c, base_m, goal_c, goal_m);
-        const unsigned b = s.at < 0 ? 0u : (unsigned)s.at;
-        base_c += s.before_count, base_m += s.before_mass;
-        n = s.count[b];
-        const unsigned new_hi = hi - (b << shift);
-        const unsigned span = (1u << shift) - 1u;
-        lo = new_hi - lo > span ? new_hi - span : lo;
-        hi = new_hi;
+    sp_span(s, klo, khi);
+    int shift = 0;
+    while ((khi - klo) >> shift >= (unsigned)kSpList) ++shift;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        part[i] = (khi - (unsigned)(mine[i] >> 32)) >> shift;
+        nth[i] = threadIdx.x + i * kSpThreads < n ? atomicAdd(&s.parts[part[i]], 1u) : 0;
     }
     __syncthreads();
-    if (n > kSpList) {  // equal logits: which of them, by division
-        if (threadIdx.x == 0) {
-            const u64 own = sp_mass(top, sp_logit(hi), c, a.shift);
-            int64_t tie;
-            if constexpr (!kByMass) {
-                tie = (int64_t)(goal_c - base_c) - 1;
-            } else {
-                auto reached = [&](int64_t t) {  // with t of them
-                    const double m = (double)(base_m + (u64)t * own);
-                    return kPast ? m > goal_m : m >= goal_m;
-                };
-                int64_t few = 0, many = n;  // not reached with few, reached with many
-                while (many - few > 1) {
-                    const int64_t mid = (few + many) / 2;
-                    if (reached(mid)) many = mid;
-                    else few = mid;
+    // the parts' first places: a thread's are consecutive
+    unsigned c[kPer], first = 0, all_c;
+    u64 none = 0, all_m;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) c[i] = s.parts[threadIdx.x * kPer + i], first += c[i];
+    unsigned most = 0, unused = 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) most = c[i] > most ? c[i] : most;
+    sp_span(s, unused, most);
+    if (most > 48) {
+        unsigned size = 128;
+        while (size < n) size <<= 1;
+        for (unsigned i = n + threadIdx.x; i < size; i += kSpThreads) s.list[i] = 0;
+        static_assert(kSpList <= 2 * kSpThreads, "a pair a thread");
+        const unsigned i = threadIdx.x;
+        // pairs up to 64 apart lie with one wave, whose LDS operations run in order: barriers stand only between the others
+        bool apart = true;
+        for (unsigned w = 2; w <= size; w <<= 1)
+            for (unsigned d = w >> 1; d > 0; d >>= 1) {
+                if (apart || d > 64) __syncthreads();
+                apart = d > 64;
+                if (i < size / 2) {
+                    const unsigned x = 2 * i - (i & (d - 1)), y = x + d;
+                    volatile u64* list = s.list;
+                    const u64 p = list[x], q = list[y];
+                    if ((p < q) == ((x & w) == 0)) list[x] = q, list[y] = p;
                 }
-                tie = many - 1;
             }
-            s.place = SamplePlace{hi, tie, base_c + (u64)tie, base_m + (u64)tie * own, own, -1};
-        }
         __syncthreads();
         return;
     }
-    // few: gather, sort from the largest key (and the lowest index) down, add up
-    if (threadIdx.x == 0) s.n = 0;
-    unsigned size = 64;
-    while (size < n) size <<= 1;
-    __syncthreads();
-    sp_each(z, a.vocab, top, bin, lo, hi, [&](unsigned key, int v, float) {
-        const unsigned i = atomicAdd(&s.n, 1u);
-        if (i < (unsigned)kSpList) s.list[i] = (u64)key << 32 | (unsigned)~v;
-    });
-    __syncthreads();
-    for (unsigned i = threadIdx.x; i < size; i += kSpPick)
-        if (i >= n) s.list[i] = 0;
-    for (unsigned w = 2; w <= size; w <<= 1)
-        for (unsigned d = w >> 1; d > 0; d >>= 1) {
-            __syncthreads();
-            for (unsigned i = threadIdx.x; i < size / 2; i += kSpPick) {
-                const unsigned x = 2 * i - (i & (d - 1)), y = x + d;
-                const u64 p = s.list[x], q = s.list[y];
-                if ((p < q) == ((x & w) == 0)) s.list[x] = q, s.list[y] = p;
-            }
-        }
-    __syncthreads();
-    constexpr int kPer = kSpList / kSpPick;
-    u64 m[kPer], tm = 0, all_m;
-    unsigned tc = 0, all_c;
+    sp_scan(s, first, none, all_c, all_m);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const unsigned j = threadIdx.x * kPer + i;
-        m[i] = j < n ? sp_mass(top, sp_logit((unsigned)(s.list[j] >> 32)), c, a.shift) : 0;
-        tm += m[i];
+        s.parts[threadIdx.x * kPer + i] = first;
+        first += c[i];
     }
-    u64 pm = tm;
-    sp_scan(s, tc, pm, all_c, all_m);
-    auto reached = [&](u64 cc, u64 mm) { return kByMass ? (kPast ? (double)mm > goal_m : (double)mm >= goal_m) : cc >= goal_c; };
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        if (threadIdx.x + i * kSpThreads < n) s.parted[s.parts[part[i]] + nth[i]] = mine[i];
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const unsigned j = threadIdx.x * kPer + i;
-        const u64 bm = base_m + pm, bc = base_c + j;
-        if (j < n && reached(bc + 1, bm + m[i]) && !reached(bc, bm)) {
-            const unsigned key = (unsigned)(s.list[j] >> 32);
-            unsigned less = 0, more = j;  // the first of its ties
-            while (less < more) {
-                const unsigned mid = (less + more) / 2;
-                if ((unsigned)(s.list[mid] >> 32) > key) less = mid + 1;
-                else more = mid;
-            }
-            s.place = SamplePlace{key, (int64_t)(j - less), bc, bm, m[i], (int)~(unsigned)s.list[j]};
+        if (threadIdx.x + i * kSpThreads >= n) continue;
+        const unsigned from = s.parts[part[i]], to = part[i] + 1 < (unsigned)kSpList ? s.parts[part[i] + 1] : n;
+        unsigned above = 0;
+        for (unsigned j = from; j < to; ++j) above += s.parted[j] > mine[i];
+        s.list[from + above] = mine[i];
+    }
+    __syncthreads();
+}
+// A thread's part of the sorted list: its tokens' masses and what lies before them.
+struct SampleWalk {
+    static constexpr int kPer = kSpList / kSpThreads;
+    unsigned n;
+    u64 m[kPer], before;
+    __device__ __forceinline__ void start(SampleShared& s, unsigned n_, const SampleScale& scale, u64 base) {
+        n = n_;
+        u64 all_m;
+        unsigned tc = 0, all_c;
+        before = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const unsigned j = threadIdx.x * kPer + i;
+            m[i] = j < n ? sp_mass(scale, sp_logit((unsigned)(s.list[j] >> 32))) : 0;
+            before += m[i];
         }
-        pm += m[i];
+        sp_scan(s, tc, before, all_c, all_m);
+        before += base;
+    }
+    // the token that the goal falls on, in s.place, or the last where none reaches it: the masses of a bin, added up at once,
+    // may differ from their tokens' in the last bits (the caller waits)
+    __device__ __forceinline__ void find(SampleShared& s, const SampleGoal& goal, u64 base_c) const {
+        u64 bm = before;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const unsigned j = threadIdx.x * kPer + i;
+            const u64 bc = base_c + j;
+            if (j < n && !goal.reached(bc, bm) && (j + 1 == n || goal.reached(bc + 1, bm + m[i]))) {
+                const unsigned key = (unsigned)(s.list[j] >> 32);
+                unsigned less = 0, more = j;  // the first of its ties
+                while (less < more) {
+                    const unsigned mid = (less + more) / 2;
+                    if ((unsigned)(s.list[mid] >> 32) > key) less = mid + 1;
+                    else more = mid;
+                }
+                s.place = SamplePlace{key, (int64_t)(j - less), bc, bm, m[i], (int)~(unsigned)s.list[j]};
+            }
+            bm += m[i];
+        }
+    }
+};
+
+// The token of the row's order that the goal falls on, in s.place; goals lie within the row. (Counts are those of the tokens
+// before it only if the row's bins have counts.)
+template <typename L>
+__device__ __forceinline__ void sp_locate(SampleShared& s, const L& z, const SampleScale& scale, const SampleGoal& goal) {
+    __syncthreads();
+    sp_find_bin(s, s.mass, s.count, 0, 0, goal, -1);
+    const int bin = s.at;
+    u64 base_c = s.before_count, base_m = s.before_mass;
+    // first what may lie in the bin, by one comparison each way
+    float lo = bin < kSpBins - 1 ? scale.near((double)(bin + 1)) : -INFINITY, hi = INFINITY;
+    bool few = bin >= 0;
+    if (!few && threadIdx.x == 0) s.place = SamplePlace{kSpNone, 0, 0, 0, 0, 0};  // not within the row: the caller's goals rule it out
+    while (few) {
+        // gather the bin's tokens in [lo, hi]
+        __syncthreads();
+        if (threadIdx.x == 0) s.n = 0;
+        __syncthreads();
+        z.each_in(lo, hi, [&](float x, int v) __attribute__((always_inline)) {
+            if (x > -INFINITY && sp_in(scale.far(x), bin)) {
+                const unsigned i = atomicAdd(&s.n, 1u);
+                if (i < (unsigned)kSpList) s.list[i] = (u64)sp_key(x) << 32 | (unsigned)~v;
+            }
+        });
+        __syncthreads();
+        const unsigned n = s.n;
+        if (n <= (unsigned)kSpList) {
+            sp_sort(s, n);
+            SampleWalk walk;
+            walk.start(s, n, scale, base_m);
+            walk.find(s, goal, base_c);
+            few = false;
+            continue;
+        }
+        // too many to sort: split the keys' span in 1024, or find one key
+        unsigned klo = 0xffffffffu, khi = 0;
+        for (int b = threadIdx.x; b < kSpBins; b += kSpThreads) s.smass[b] = 0, s.scount[b] = 0;  // seen by all behind sp_span's barriers
+        z.each_in(lo, hi, [&](float x, int) __attribute__((always_inline)) {
+            if (x > -INFINITY && sp_in(scale.far(x), bin)) {
+                const unsigned key = sp_key(x);
+                klo = key < klo ? key : klo;
+                khi = key > khi ? key : khi;
+            }
+        });
+        sp_span(s, klo, khi);
+        if (klo == khi) {
+            // equal logits: which of them, by division
+            if (threadIdx.x == 0) {
+                const u64 own = sp_mass(scale, sp_logit(khi));
+                int64_t before = 0, with = n;  // not reached with `before` of them, reached with `with`
+                while (with - before > 1) {
+                    const int64_t mid = (before + with) / 2;
+                    if (goal.reached(base_c + (u64)mid, base_m + (u64)mid * own)) with = mid;
+                    else before = mid;
+                }
+                s.place = SamplePlace{khi, before, base_c + (u64)before, base_m + (u64)before * own, own, -1};
+            }
+            few = false;
+            continue;
+        }
+        int parts = 0;
+        while ((khi - klo) >> parts >= (unsigned)kSpBins) ++parts;
+        // from the largest key down
+        z.each_in(lo, hi, [&](float x, int) __attribute__((always_inline)) {
+            if (x > -INFINITY && sp_in(scale.far(x), bin)) {
+                const int b = (int)((khi - sp_key(x)) >> parts);
+                atomicAdd(&s.scount[b], 1u);
+                atomicAdd(&s.smass[b], sp_mass(scale, x));
+            }
+        });
+        __syncthreads();
+        sp_find_bin(s, s.smass, s.scount, base_c, base_m, goal, (int)((khi - klo) >> parts));
+        const unsigned b = (unsigned)s.at;
+        base_c += s.before_count, base_m += s.before_mass;
+        const unsigned new_hi = khi - (b << parts), span = (1u << parts) - 1u;
+        lo = sp_logit(new_hi - klo > span ? new_hi - span : klo);
+        hi = sp_logit(new_hi);
     }
     __syncthreads();
 }
 
-// The index of the tie-th token with this key.
+// The index of the tie-th token with this logit.
 template <typename T>
-__device__ __forceinline__ int sp_index(SampleShared& s, const T* z, int vocab, unsigned key, int64_t tie) {
+__device__ __forceinline__ int sp_index(SampleShared& s, const T* z, int vocab, float logit, int64_t tie) {
     __syncthreads();
     if (threadIdx.x == 0) s.at = 0;
     int64_t before = 0;
-    for (int v0 = 0; v0 < vocab; v0 += kSpPick * 8) {
+    for (int v0 = 0; v0 < vocab; v0 += kSpThreads * 8) {
         const int v = v0 + (int)threadIdx.x * 8;
         float x[8];
         unsigned mine = 0, c, all_c;
@@ -429,7 +526,7 @@ __device__ __forceinline__ int sp_index(SampleShared& s, const T* z, int vocab, 
         if (v < vocab) {
             load8(z, v, vocab, x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) mine += v + e < vocab && sp_key(x[e]) == key;
+            for (int e = 0; e < 8; ++e) mine += v + e < vocab && x[e] == logit;
         }
         c = mine;
         sp_scan(s, c, none, all_c, all_m);
@@ -437,7 +534,7 @@ __device__ __forceinline__ int sp_index(SampleShared& s, const T* z, int vocab, 
         if (mine && at <= tie && at + mine > tie) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (v + e < vocab && sp_key(x[e]) == key && at++ == tie) s.at = v + e;
+                if (v + e < vocab && x[e] == logit && at++ == tie) s.at = v + e;
         }
         before += all_c;
         if (before > tie) break;
@@ -447,145 +544,279 @@ __device__ __forceinline__ int sp_index(SampleShared& s, const T* z, int vocab, 
 }
 
 template <typename T>
-__global__ __launch_bounds__(kSpPick) void sample_pick_kernel(SampleArgs a) {
+__global__ __launch_bounds__(kSpThreads) void sample_kernel(SampleArgs a, int held) {
+    extern __shared__ __align__(16) char sp_smem[];
     __shared__ SampleShared s;
-    const int row = blockIdx.x;
-    const T* z = reinterpret_cast<const T*>(a.z) + (int64_t)row * a.vocab;
+    const int64_t row = blockIdx.x;
+    const SampleLogits<T> z{reinterpret_cast<u32x4*>(sp_smem), reinterpret_cast<const T*>(a.z) + row * a.vocab, a.vocab, held};
     const SampleRow r = sp_row(a, row);
-    const u64 first = sp_top(a, row);
-    const unsigned key = (unsigned)(first >> 32);
-    if (!(r.t > 0.0) || key <= kSpNone) {
+    for (int b = threadIdx.x; b < kSpBins + 64; b += kSpThreads) s.mass[b] = 0, s.count[b] = 0;
+
+    // the largest logit (NaN is none), for a greedy choice its lowest index
+    float top = -INFINITY;
+    unsigned first = 0xffffffffu;
+    const bool greedy = !(r.t > 0.0);
+    if (greedy)
+        z.template each<true>([&](float x, int v) __attribute__((always_inline)) {
+            if (x > top) top = x, first = (unsigned)v;  // a thread's indexes rise
+        });
+    else z.template each<true>([&](float x, int) __attribute__((always_inline)) { top = x > top ? x : top; });
+    u64 best = (u64)sp_key(top) << 32 | (unsigned)~first;
+    if (greedy) {
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) {
+            const u64 o = __shfl_xor(best, off, kWave);
+            best = o > best ? o : best;
+        }
+    } else {
+        best = (u64)sp_max((unsigned)(best >> 32)) << 32;
+    }
+    if ((threadIdx.x & 63) == 0) s.wmass[threadIdx.x >> 6] = best;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSpWaves; ++w) best = s.wmass[w] > best ? s.wmass[w] : best;
+    top = sp_logit((unsigned)(best >> 32));
+    if (greedy || top == -INFINITY) {
         if (threadIdx.x == 0) {
-            a.token[row] = key <= kSpNone ? -1 : (int64_t)(int)~(unsigned)first;
-            if (a.logprob) a.logprob[row] = key <= kSpNone ? __builtin_nanf("") : 0.f;
+            a.token[row] = top == -INFINITY ? -1 : (int64_t)(int)~(unsigned)best;
+            if (a.logprob) a.logprob[row] = top == -INFINITY ? __builtin_nanf("") : 0.f;
         }
         return;
     }
-    const float top = sp_logit(key);
-    const double c = 1.4426950408889634074 / r.t;
-    // all tokens and their mass
-    unsigned tc = 0, tokens;
-    u64 tm = 0, total;
-    for (int b = threadIdx.x; b < kSpBins; b += kSpPick) {
-        tc += a.count[(int64_t)row * kSpBins + b];
-        tm += a.mass[(int64_t)row * kSpBins + b];
-    }
-    sp_scan(s, tc, tm, tokens, total);
-    // the kept prefix ends behind (end_key, end_tie) and has `kept` of mass
-    unsigned end_key = 0;
-    int64_t end_tie = a.vocab;
-    u64 kept = total;
-    if (r.k < (int64_t)tokens) {
-        sp_locate<T, false, false>(a, s, z, row, top, c, (u64)r.k, 0.0);
-        end_key = s.place.key, end_tie = s.place.tie, kept = s.place.mass + s.place.own;
-    }
-    if (r.p < 1.0) {
-        // the token that reaches p of the k's mass is the last; the first stays whatever p is
-        const double goal = r.p > 0.0 ? r.p * (double)kept : 0.0;
-        sp_locate<T, true, false>(a, s, z, row, top, c, 0, goal > 0.0 ? goal : 1.0);
-        const SamplePlace q = s.place;
-        if (q.key > end_key || (q.key == end_key && q.tie < end_tie)) end_key = q.key, end_tie = q.tie, kept = q.mass + q.own;
-    }
-    if (r.m > 0.0) {
-        const double m = r.m < 1.0 ? r.m : 1.0;
-        // mass falls with the key: the lowest key with mass >= m, found in 64 steps a time
-        unsigned lo = kSpNone + 1, hi = key;  // hi has it
-        while (lo < hi) {
-            const unsigned span = hi - lo, step = span / 64 + 1, lane = threadIdx.x & 63;
-            const u64 probe = (u64)lo + (u64)step * lane;  // 64 places from lo up
-            const bool in = probe < hi;
-            const double x = in ? ((double)sp_logit((unsigned)probe) - (double)top) / r.t : 0.0;
-            const bool has = !in || exp(x) >= m;
-            const u64 votes = __ballot(has);  // from some lane on; lanes past hi have it
-            if (votes == 0) {
-                const u64 next = (u64)lo + (u64)step * 63 + 1;
-                lo = next < hi ? (unsigned)next : hi;
-                continue;
-            }
-            const unsigned firsthas = (unsigned)__ffsll((unsigned long long)votes) - 1;
-            const u64 nh = (u64)lo + (u64)step * firsthas;
-            const unsigned new_hi = nh < hi ? (unsigned)nh : hi;
-            const unsigned new_lo = firsthas ? (unsigned)((u64)lo + (u64)step * (firsthas - 1) + 1) : new_hi;
-            hi = new_hi, lo = new_lo < new_hi ? new_lo : new_hi;
-        }
-        if (hi > end_key) {
-            // the mass down to that key
-            u64 mine = 0;
-            sp_all(z, a.vocab, [&](unsigned k, int, float x) {
-                if (k >= hi) mine += sp_mass(top, x, c, a.shift);
-            });
-            unsigned none = 0, all_c;
-            u64 all;
-            sp_scan(s, none, mine, all_c, all);
-            end_key = hi, end_tie = a.vocab, kept = all;
-        }
-    }
     const double u = (double)a.u[row];
-    // u below 1 falls within the kept mass; others are taken to its ends
-    double goal = u > 0.0 ? u * (double)kept : 0.0;
-    const double most = (double)kept * (1.0 - 0x1p-50);
-    goal = goal < most ? goal : most;
-    sp_locate<T, true, true>(a, s, z, row, top, c, 0, goal);
-    const SamplePlace q = s.place;
-    const int index = q.index >= 0 ? q.index : sp_index(s, z, a.vocab, q.key, q.tie);
+    if (top == INFINITY) {
+        // infinite logits: all have the same mass, the others none
+        unsigned c = 0, all_c;
+        u64 none = 0, all_m;
+        z.template each<false>([&](float x, int) { c += x == top; });
+        sp_scan(s, c, none, all_c, all_m);
+        double n = r.k < (int64_t)all_c ? (double)r.k : (double)all_c;
+        if (r.p < 1.0) n = fmax(ceil(r.p * n), 1.0);
+        const double at = floor(fmax(u, 0.0) * n);
+        const int index = sp_index(s, z.z, a.vocab, top, (int64_t)(at < n ? at : n - 1.0));
+        if (threadIdx.x == 0) {
+            a.token[row] = index;
+            if (a.logprob) a.logprob[row] = (float)-log(n);
+        }
+        return;
+    }
+    const SampleScale scale{(double)top, 32.0 / r.t, a.shift};
+
+    // masses, and counts where a count is asked for
+    const bool counts = r.k < (int64_t)a.vocab;
+    unsigned tail = 0;  // tokens of the last bin, which have no mass
+    {
+        // exp(-r / 32) 2^shift: the series' terms, -1 / 32 to the i over i!
+        const double unit = ldexp(1.0, a.shift);
+        const double c1 = unit * (-1.0 / 32), c2 = unit * (1.0 / 2048), c3 = unit * (-1.0 / 196608), c4 = unit * (1.0 / 25165824), c5 = unit * (-1.0 / 4026531840.0);
+        const int aside = kSpBins + ((int)threadIdx.x & 63);
+        auto add = [&](float x, auto counted) __attribute__((always_inline)) {
+            // without a branch: what has no mass (NaN, too) goes where nobody looks
+            const double q = scale.far(x);
+            const bool in = q < (double)(kSpBins - 1);
+            const int b = (int)q, at = in ? b : aside;
+            const double d = q - (double)b;
+            atomicAdd(&s.mass[at], sp_whole(fma(fma(fma(fma(fma(c5, d, c4), d, c3), d, c2), d, c1), d, unit)));
+            if constexpr (decltype(counted)::value) {
+                atomicAdd(&s.count[at], 1u);
+                tail += !in & (x > -INFINITY);
+            }
+        };
+        if (counts) z.template each<false>([&](float x, int) __attribute__((always_inline)) { add(x, std::true_type{}); });
+        else z.template each<false>([&](float x, int) __attribute__((always_inline)) { add(x, std::false_type{}); });
+    }
+    __syncthreads();
+    u64 total;
+    {
+        // without counts, at least so many tokens are in a bin
+        unsigned all_c;
+        u64 all;
+        if (counts) {
+            u64 none = 0;
+            sp_scan(s, tail, none, all_c, all);
+            if (threadIdx.x == 0) s.count[kSpBins - 1] = all_c;
+        }
+        unsigned c = 0;
+        total = 0;
+        for (int b = threadIdx.x; b < kSpBins; b += kSpThreads) {
+            u64 m = s.mass[b];
+            if (!counts) s.count[b] = (unsigned)((m + ((u64)1 << a.shift) - 1) >> a.shift);
+            m = (u64)((double)m * exp((double)b * (-1.0 / 32.0)) + 0.5);
+            s.mass[b] = m;
+            total += m;
+        }
+        sp_scan(s, c, total, all_c, all);
+        total = all;
+        __syncthreads();
+    }
+    const bool by_p = r.p < 1.0, by_m = r.m > 0.0;
+    const double min_p = r.m < 1.0 ? r.m : 1.0;
+    // min_p keeps what is nearer than this; rounding of the logarithm matters to tokens that are as near as makes no
+    // difference to a bin, and these are asked for their mass itself
+    const double far_m = by_m ? log(min_p) * -32.0 : 0.0;
+    auto kept_by_m = [&](float x) __attribute__((always_inline)) {
+        const double q = scale.far(x);
+        return q < far_m - 1e-6 || (q < far_m + 1e-6 && sp_exp(scale, x) >= min_p);
+    };
+
+    // The bins that hold the answers: up to the k-th token's, which the other bounds are shares of, or without one up to the
+    // first that a bound lies in. Their tokens, if they are few, answer everything.
+    int last = kSpBins;
+    bool by_k = counts;
+    if (by_k) {
+        sp_find_bin(s, s.mass, s.count, 0, 0, SampleGoal{kCount, (u64)r.k, 0.0}, -1);
+        by_k = s.at >= 0;  // the row has so many tokens
+        if (by_k) last = s.at;
+        __syncthreads();
+    }
+    if (by_p && !by_k) {
+        const double m = r.p > 0.0 ? r.p * (double)total : 0.0;
+        sp_find_bin(s, s.mass, s.count, 0, 0, SampleGoal{kReach, 0, m > 0.0 ? m : 1.0}, -1);
+        if (s.at >= 0) last = s.at;
+    }
+    if (by_m && !by_k) {
+        const int b = (int)fmin(far_m + 1e-6, (double)(kSpBins - 1));
+        last = b < last ? b : last;
+    }
+    if (last < kSpBins) {  // more than fit?
+        unsigned c = 0, all_c;
+        u64 none = 0, all_m;
+        for (int b = threadIdx.x; b <= last; b += kSpThreads) c += s.count[b];
+        sp_scan(s, c, none, all_c, all_m);
+        if (all_c > (unsigned)kSpList) last = kSpBins;
+    }
+    unsigned n = kSpList + 1;
+    if (last < kSpBins) {
+        if (threadIdx.x == 0) s.n = 0;
+        __syncthreads();
+        const double end = (double)(last + 1);
+        const float near = last < kSpBins - 1 ? scale.near(end) : -INFINITY;  // first by one comparison
+        z.each_in(near, INFINITY, [&](float x, int v) __attribute__((always_inline)) {
+            if (x > -INFINITY && (scale.far(x) < end || last == kSpBins - 1)) {
+                const unsigned i = atomicAdd(&s.n, 1u);
+                if (i < (unsigned)kSpList) s.list[i] = (u64)sp_key(x) << 32 | (unsigned)~v;
+            }
+        });
+        __syncthreads();
+        n = s.n;
+    }
+
+    u64 kept;
+    float logit;
+    int index;
+    if (n <= (unsigned)kSpList) {
+        // all in the list: the bounds are places in it
+        sp_sort(s, n);
+        SampleWalk walk;
+        walk.start(s, n, scale, 0);
+        constexpr int kPer = SampleWalk::kPer;
+        unsigned end = by_k && (u64)r.k < n ? (unsigned)r.k : n;
+        if (by_m) {
+            unsigned c = 0, all_c;
+            u64 none = 0, all_m;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const unsigned j = threadIdx.x * kPer + i;
+                c += j < n && kept_by_m(sp_logit((unsigned)(s.list[j] >> 32)));
+            }
+            sp_scan(s, c, none, all_c, all_m);
+            s.n = all_c;  // the same from every thread
+        }
+        auto mass_to = [&](unsigned place) __attribute__((always_inline)) {  // of the list's first `place` >= 1
+            __syncthreads();
+            u64 m = walk.before;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                m += walk.m[i];
+                if (threadIdx.x * kPer + i + 1 == place) s.before_mass = m;
+            }
+            __syncthreads();
+            return s.before_mass;
+        };
+        kept = by_k ? mass_to(end) : total;
+        if (by_p) {
+            const double m = r.p > 0.0 ? r.p * (double)kept : 0.0;
+            walk.find(s, SampleGoal{kReach, 0, m > 0.0 ? m : 1.0}, 0);
+            __syncthreads();
+            const unsigned e = (unsigned)s.place.count + 1;
+            end = e < end ? e : end;
+        }
+        if (by_m) {
+            __syncthreads();
+            const unsigned e = s.n > 0 ? s.n : 1;
+            end = e < end ? e : end;
+        }
+        kept = mass_to(end);
+        // u below 1 falls within the kept mass; others are taken to its ends
+        const double goal = u > 0.0 ? u * (double)kept : 0.0, most = (double)kept * (1.0 - 0x1p-30);
+        walk.find(s, SampleGoal{kPass, 0, goal < most ? goal : most}, 0);
+        __syncthreads();
+        logit = sp_logit(s.place.key), index = s.place.index;
+    } else {
+        // the kept prefix ends behind (end_key, end_tie)
+        unsigned end_key = 0;
+        int64_t end_tie = a.vocab;
+        kept = total;
+        SamplePlace q;
+        for (int step = by_k ? 0 : by_p ? 1 : 2; step < 3; step = step == 0 && !by_p ? 2 : step + 1) {
+            SampleGoal goal;
+            if (step == 0) {
+                goal = SampleGoal{kCount, (u64)r.k, 0.0};
+            } else if (step == 1) {
+                // the token that reaches p of the k's mass is the last; the first stays whatever p is
+                const double m = r.p > 0.0 ? r.p * (double)kept : 0.0;
+                goal = SampleGoal{kReach, 0, m > 0.0 ? m : 1.0};
+            } else {
+                if (by_m) {
+                    // what min_p keeps: its mass, and its lowest key
+                    u64 mine = 0, all;
+                    unsigned low = 0xffffffffu, none = 0, all_c;
+                    z.each_in(scale.near(far_m), INFINITY, [&](float x, int) __attribute__((always_inline)) {
+                        if (x > -INFINITY && kept_by_m(x)) {
+                            mine += sp_mass(scale, x);
+                            low = sp_key(x) < low ? sp_key(x) : low;
+                        }
+                    });
+                    sp_scan(s, none, mine, all_c, all);
+                    unsigned unused = 0;
+                    sp_span(s, low, unused);
+                    if (low > end_key) end_key = low, end_tie = a.vocab, kept = all;
+                }
+                const double m = u > 0.0 ? u * (double)kept : 0.0, most = (double)kept * (1.0 - 0x1p-30);
+                goal = SampleGoal{kPass, 0, m < most ? m : most};
+            }
+            sp_locate(s, z, scale, goal);
+            q = s.place;
+            if (step < 2 && (q.key > end_key || (q.key == end_key && q.tie < end_tie))) end_key = q.key, end_tie = q.tie, kept = q.mass + q.own;
+        }
+        logit = sp_logit(q.key);
+        index = q.index >= 0 ? q.index : sp_index(s, z.z, a.vocab, logit, q.tie);
+    }
     if (threadIdx.x == 0) {
         a.token[row] = index;
-        if (a.logprob) {
-            const float x = sp_logit(q.key);
-            a.logprob[row] = (float)((x == top ? 0.0 : ((double)x - (double)top) / r.t) - log(ldexp((double)kept, -a.shift)));
-        }
+        if (a.logprob)
+            a.logprob[row] = (float)((logit == top ? 0.0 : ((double)logit - (double)top) / r.t) - log(ldexp((double)kept, -a.shift)));
     }
-}
-
-// Slices of a row: enough blocks to fill the card (four a CU), none below 2048 logits.
-static int sample_slices(int64_t rows, int64_t vocab) {
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kSpSlices, vocab / 2048));
-    return (int)std::max<int64_t>(1, std::min(most, (1024 + rows - 1) / rows));
-}
-constexpr int64_t kSpRows = 32768;  // of a launch (grids hold 65535)
-size_t sample_workspace(int64_t rows, int64_t vocab) {
-    rows = std::min(rows, kSpRows);
-    return (size_t)rows * ((size_t)sample_slices(rows, vocab) * 8 + kSpBins * 12);
 }
 
 template <typename T>
 static int sample_t(const SampleArgs& a, hipStream_t stream) {
-    const dim3 grid((unsigned)a.slices, (unsigned)a.rows);
-    hipLaunchKernelGGL((sample_top_kernel<T>), grid, dim3(kSpThreads), 0, stream, a);
-    hipLaunchKernelGGL((sample_bins_kernel<T>), grid, dim3(kSpThreads), 0, stream, a);
-    hipLaunchKernelGGL((sample_pick_kernel<T>), dim3((unsigned)a.rows), dim3(kSpPick), 0, stream, a);
+    const int pieces = (int)(((int64_t)a.vocab * (int)sizeof(T) + 15) / 16), held = std::min(pieces, kSpHeld / 16);
+    static std::atomic<uint64_t> done{0};
+    if (!allow_lds(reinterpret_cast<const void*>(&sample_kernel<T>), kSpHeld, done)) return M3_ERR_LAUNCH;
+    hipLaunchKernelGGL((sample_kernel<T>), dim3((unsigned)a.rows), dim3(kSpThreads), held * 16, stream, a, held);
     return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH;
 }
 
 int launch_sample(const void* logits, int dtype, int64_t rows, int vocab, const float* u, const float* temperature,
                   double temperature1, const int32_t* top_k, int64_t top_k1, const float* top_p, double top_p1,
-                  const float* min_p, double min_p1, int64_t* token, float* logprob, void* ws, hipStream_t stream) {
-    SampleArgs a;
-    a.temperature1 = temperature1, a.top_p1 = top_p1, a.min_p1 = min_p1, a.top_k1 = top_k1;
-    a.vocab = vocab;
-    a.slices = sample_slices(std::min(rows, kSpRows), vocab);
-    a.slice = (vocab + a.slices - 1) / a.slices;
-    a.mass = reinterpret_cast<u64*>(ws);
-    a.top = a.mass + std::min(rows, kSpRows) * kSpBins;
-    a.count = reinterpret_cast<unsigned*>(a.top + std::min(rows, kSpRows) * a.slices);
+                  const float* min_p, double min_p1, int64_t* token, float* logprob, hipStream_t stream) {
     int bits = 0;
     while (((int64_t)1 << bits) < vocab) ++bits;
-    a.shift = 62 - bits;  // a whole row's mass stays below 2^62
-    const int size = dtype == M3_DTYPE_BF16 ? 2 : 4;
-    for (int64_t r = 0; r < rows; r += kSpRows) {
-        a.rows = (int)std::min(rows - r, kSpRows);
-        a.z = reinterpret_cast<const char*>(logits) + r * vocab * size;
-        a.u = u + r;
-        a.temperature = temperature ? temperature + r : nullptr;
-        a.top_k = top_k ? top_k + r : nullptr;
-        a.top_p = top_p ? top_p + r : nullptr;
-        a.min_p = min_p ? min_p + r : nullptr;
-        a.token = token + r;
-        a.logprob = logprob ? logprob + r : nullptr;
-        const int st = dtype == M3_DTYPE_BF16 ? sample_t<bf16>(a, stream) : sample_t<float>(a, stream);
-        if (st != M3_OK) return st;
-    }
-    return M3_OK;
+    // a row's mass stays below 2^62, a token's within the 52 bits that sp_mass has
+    const SampleArgs a{logits, u, temperature, top_p, min_p, top_k, temperature1, top_p1, min_p1, top_k1, token, logprob, rows, vocab,
+                       std::min(62 - bits, 51)};
+    return dtype == M3_DTYPE_BF16 ? sample_t<bf16>(a, stream) : sample_t<float>(a, stream);
 }
 
 }  // namespace m3

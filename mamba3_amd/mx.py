@@ -40,7 +40,7 @@ class MXTensor:
             raise ValueError(f"MXTensor needs a last dimension of at least 1, got shape {tuple(shape)}")
         rows, k = math.prod(shape[:-1]), shape[-1]
         for name, t, cols in (("data", data, _native.mx_row_bytes(k, format)), ("scales", scales, _native.mx_padded(k) // 32)):
-            if t.dtype != torch.uint8 or tuple(t.shape) != (rows, cols) or not t.is_contiguous():
+            if t.dtype is not torch.uint8 or t.shape != (rows, cols) or not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous uint8 of shape {(rows, cols)}, got {t.dtype} {tuple(t.shape)}")
         if data.device != scales.device:
             raise ValueError(f"data is on {data.device}, scales on {scales.device}")
@@ -55,10 +55,18 @@ class MXTensor:
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values, in fp32 or bf16 (both hold them exactly, but for results below 2^-126 and past the largest number)."""
         _native.dtype_code(dtype)
-        return ops.mx_dequantize_fast(self.data, self.scales, self.format, self.shape[-1], dtype).view(self.shape)
+        out = ops.mx_dequantize_fast(self.data, self.scales, self.format, self.shape[-1], dtype)
+        return out if len(self.shape) == 2 else out.view(self.shape)
 
     def __repr__(self) -> str:
         return f"MXTensor(shape={tuple(self.shape)}, format={self.format!r}, device={str(self.device)!r})"
+
+
+def _mx(data: torch.Tensor, scales: torch.Tensor, shape, format: str) -> MXTensor:
+    """An MXTensor of what the kernels wrote."""
+    t = MXTensor.__new__(MXTensor)
+    t.data, t.scales, t.shape, t.format = data, scales, torch.Size(shape), format
+    return t
 
 
 def quantize_mx(x: torch.Tensor, format: str = "e2m1") -> MXTensor:
@@ -68,7 +76,7 @@ def quantize_mx(x: torch.Tensor, format: str = "e2m1") -> MXTensor:
         raise ValueError(f"quantize_mx needs a last dimension of at least 1, got shape {tuple(x.shape)}")
     _native.dtype_code(x.dtype)
     refuse_gradients("quantize_mx", x)
-    return MXTensor(*ops.mx_quantize_fast(x, format, False), x.shape, format)
+    return _mx(*ops.mx_quantize_fast(x, format, False), x.shape, format)
 
 
 def silu_mul_mx(gate_up: torch.Tensor, format: str = "e4m3") -> MXTensor:
@@ -79,37 +87,44 @@ def silu_mul_mx(gate_up: torch.Tensor, format: str = "e4m3") -> MXTensor:
         raise ValueError(f"silu_mul_mx needs an even last dimension of at least 2, got shape {tuple(gate_up.shape)}")
     _native.dtype_code(gate_up.dtype)
     refuse_gradients("silu_mul_mx", gate_up)
-    return MXTensor(*ops.mx_quantize_fast(gate_up, format, True), (*gate_up.shape[:-1], gate_up.shape[-1] // 2), format)
+    return _mx(*ops.mx_quantize_fast(gate_up, format, True), (*gate_up.shape[:-1], gate_up.shape[-1] // 2), format)
 
 
 def mx_linear(x: MXTensor | torch.Tensor, weight: MXTensor, residual: torch.Tensor | None = None, scale: float = 1.0,
               out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """[residual +] scale * x weight^T for weight (n, k) in e2m1 and x (..., k): microscaled in either format, or
-    a tensor, which is quantised to e4m3 first. The result (..., n) has out_dtype: by default the residual's type,
+    a tensor, which is quantised to e4m3 on the way. The result (..., n) has out_dtype: by default the residual's type,
     x's, or bf16. No backward.
 
     Sums are fp32. For a bf16 result the matrix instructions align the 128 products that they add at a time at about
     2^-13 of the largest where x is e4m3; an fp32 result has no such step."""
     if not isinstance(weight, MXTensor) or weight.format != "e2m1" or len(weight.shape) != 2:
         raise ValueError("mx_linear needs a two-dimensional e2m1 MXTensor as weight")
-    if isinstance(x, torch.Tensor):
-        if out_dtype is None and residual is None:
-            out_dtype = x.dtype
-        x = quantize_mx(x, "e4m3")
-    if x.shape[-1] != weight.shape[1]:
+    n, k = weight.shape
+    plain = not isinstance(x, MXTensor)
+    if plain:
+        if x.dim() < 1:
+            raise ValueError("mx_linear expects x (..., k)")
+        refuse_gradients("mx_linear", x)
+        _native.dtype_code(x.dtype)
+    if x.shape[-1] != k or n < 1:
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit (..., k) and (n, k)")
-    shape = (*x.shape[:-1], weight.shape[0])
     if out_dtype is None:
-        out_dtype = torch.bfloat16 if residual is None else residual.dtype
+        out_dtype = residual.dtype if residual is not None else x.dtype if plain else torch.bfloat16
     _native.dtype_code(out_dtype)
-    if weight.shape[0] < 1:
-        raise ValueError("mx_linear needs at least one row of weight")
     if x.device != weight.device:
+        # a tensor on the host is refused for what it is
+        _native.require_gpu(x if plain else x.data)
         raise ValueError(f"x is on {x.device}, weight on {weight.device}")
+    shape = (*x.shape[:-1], n)
     if residual is not None:
-        if tuple(residual.shape) != shape or residual.dtype != out_dtype or residual.device != x.device:
+        if residual.shape != shape or residual.dtype != out_dtype or residual.device != weight.device:
             raise ValueError(f"residual must be {out_dtype} of shape {shape} on {x.device}, got {residual.dtype} "
                              f"{tuple(residual.shape)} on {residual.device}")
         refuse_gradients("mx_linear", residual)
-    return ops.mx_linear_fast(x.data, x.scales, x.format, weight.data, weight.scales, weight.shape[1], residual,
-                              float(scale), out_dtype).view(shape)
+    if plain and ops.mx_linear_takes_tensor(x, n, out_dtype):
+        out = ops.mx_linear_tensor_fast(x, weight.data, weight.scales, residual, float(scale), out_dtype)
+    else:
+        q = quantize_mx(x, "e4m3") if plain else x
+        out = ops.mx_linear_fast(q.data, q.scales, q.format, weight.data, weight.scales, k, residual, float(scale), out_dtype)
+    return out if len(shape) == 2 else out.view(shape)

@@ -17,6 +17,7 @@ source tensor and version.
 from __future__ import annotations
 
 import contextlib
+import functools
 import weakref
 from collections import OrderedDict
 from typing import Optional
@@ -1010,8 +1011,9 @@ def _rows_of(t: torch.Tensor) -> torch.Tensor:
 
 def _mx_empty(rows: int, k: int, fmt: str, like: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Room for (rows, k) microscaled values: (data, scales)."""
-    return (like.new_empty((rows, _native.mx_row_bytes(k, fmt)), dtype=torch.uint8),
-            like.new_empty((rows, _native.mx_padded(k) // 32), dtype=torch.uint8))
+    device, kp = like.device, _native.mx_padded(k)
+    return (torch.empty((rows, kp if fmt == "e4m3" else kp // 2), dtype=torch.uint8, device=device),
+            torch.empty((rows, kp // 32), dtype=torch.uint8, device=device))
 
 
 def _mx_quantize_eager(x: torch.Tensor, fmt: str, gated: bool) -> tuple[torch.Tensor, torch.Tensor]:
@@ -1061,7 +1063,7 @@ def _add_rmsnorm_eager(x: torch.Tensor, residual: torch.Tensor, weight: torch.Te
         total, y = torch.empty_like(x2), torch.empty_like(x2)
         rstd = torch.empty(x2.shape[0], device=x.device, dtype=torch.float32) if keep else None
         _native.add_rmsnorm_fwd(x2, _rows_of(residual), weight.contiguous(), scale, eps, total, y, rstd)
-    return total.view(x.shape), y.view(x.shape), rstd
+    return (total, y, rstd) if x.dim() == 2 else (total.view(x.shape), y.view(x.shape), rstd)
 
 
 @torch.library.custom_op(f"{NS}::add_rmsnorm", mutates_args=())
@@ -1079,10 +1081,14 @@ def _(x, residual, weight, scale, eps):
 def _add_rmsnorm_bwd_eager(total, weight, rstd, dtotal, dy, scale, want) -> list:
     """m3_add_rmsnorm_bwd: gradients of x, residual and weight, None for those that `want` leaves out."""
     with on_device(total):
-        out = [torch.empty(t.shape, device=t.device, dtype=t.dtype) if w else None
-               for t, w in zip((total, total, weight), want)]
-        two = lambda t: None if t is None else _rows_of(t if t.dtype == total.dtype else t.to(total.dtype))  # noqa: E731
-        _native.add_rmsnorm_bwd(_rows_of(total), weight.contiguous(), rstd, two(dtotal), two(dy), scale, *out)
+        t2, w1 = _rows_of(total), weight.contiguous()
+        out = [torch.empty_like(t) if w else None for t, w in zip((t2, t2, w1), want)]
+        dy = _rows_of(dy if dy.dtype == total.dtype else dy.to(total.dtype))
+        if dtotal is not None:
+            dtotal = _rows_of(dtotal if dtotal.dtype == total.dtype else dtotal.to(total.dtype))
+        _native.add_rmsnorm_bwd(t2, w1, rstd, dtotal, dy, scale, *out)
+    if total.dim() != 2:
+        out[:2] = [None if t is None else t.view(total.shape) for t in out[:2]]
     return out
 
 
@@ -1139,10 +1145,16 @@ class _AddRmsNorm(torch.autograd.Function):
         return total, y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dtotal, dy):
+    def _grads(ctx, dtotal, dy):
         grads = _add_rmsnorm_grads(_add_rmsnorm_bwd_eager, *ctx.saved_tensors, ctx.scale, ctx.needs_input_grad[:3], dtotal, dy)
         return (*grads, None, None)
+
+    _once = staticmethod(torch.autograd.function.once_differentiable(_grads.__func__))
+
+    @staticmethod
+    def backward(ctx, dtotal, dy):
+        # the wrapper is for a caller that records the backward; without one it is time alone
+        return (_AddRmsNorm._once if _is_grad_enabled() else _AddRmsNorm._grads)(ctx, dtotal, dy)
 
 
 def _add_rmsnorm_mx_eager(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, scale: float,
@@ -1191,6 +1203,36 @@ mx_linear = torch.library.custom_op(f"{NS}::mx_linear", _mx_linear_eager, mutate
 @mx_linear.register_fake
 def _(x_data, x_scales, x_format, w_data, w_scales, k, residual, scale, dtype):
     return x_data.new_empty((x_data.shape[0], w_data.shape[0]), dtype=dtype)
+
+
+@functools.lru_cache(maxsize=1024)
+def _takes_tensor(rows: int, n: int, k: int, dtype: torch.dtype) -> bool:
+    return _native.mx_linear_takes_tensor(rows, n, k, dtype)
+
+
+def mx_linear_takes_tensor(x: torch.Tensor, n: int, dtype: torch.dtype) -> bool:
+    """True where one launch quantises x and multiplies (sizes alone decide; under torch.compile these may be
+    symbolic, and two launches run)."""
+    return not _is_compiling() and x.numel() > 0 and _takes_tensor(x.numel() // x.shape[-1], n, x.shape[-1], dtype)
+
+
+def _mx_linear_tensor_eager(x: torch.Tensor, w_data: torch.Tensor, w_scales: torch.Tensor, residual: Optional[torch.Tensor],
+                            scale: float, dtype: torch.dtype) -> torch.Tensor:
+    """m3_mx_linear_tensor: (rows, n) in `dtype`."""
+    _native.require_gpu(x, w_data, w_scales, residual)
+    with on_device(x):
+        x2 = _rows_of(x)
+        out = torch.empty((x2.shape[0], w_data.shape[0]), device=x.device, dtype=dtype)
+        _native.mx_linear_tensor(x2, w_data, w_scales, None if residual is None else _rows_of(residual), scale, out)
+    return out
+
+
+mx_linear_tensor = torch.library.custom_op(f"{NS}::mx_linear_tensor", _mx_linear_tensor_eager, mutates_args=())
+
+
+@mx_linear_tensor.register_fake
+def _(x, w_data, w_scales, residual, scale, dtype):
+    return x.new_empty((x.numel() // x.shape[-1], w_data.shape[0]), dtype=dtype)
 
 
 def _sample_tokens_eager(logits: torch.Tensor, u: torch.Tensor, temperatures: Optional[torch.Tensor], temperature: float,
@@ -1242,6 +1284,11 @@ def add_rmsnorm_mx_fast(x, residual, weight, scale, eps, fmt):
 def mx_linear_fast(x_data, x_scales, x_format, w_data, w_scales, k, residual, scale, dtype):
     fn = _mx_linear_eager if _plain(x_data, x_scales, w_data, w_scales, residual) else mx_linear
     return fn(x_data, x_scales, x_format, w_data, w_scales, k, residual, scale, dtype)
+
+
+def mx_linear_tensor_fast(x, w_data, w_scales, residual, scale, dtype):
+    fn = _mx_linear_tensor_eager if _plain(x, w_data, w_scales, residual) else mx_linear_tensor
+    return fn(x, w_data, w_scales, residual, scale, dtype)
 
 
 def sample_tokens_fast(logits, u, temperatures, temperature, top_ks, top_k, top_ps, top_p, min_ps, min_p, logprob):

@@ -91,14 +91,12 @@ def test_mx_linear_refuses_bad_arguments(lib):
 
 
 def test_sample_refuses_bad_arguments(lib):
-    def go(rows=4, vocab=64, dtype=1, z=FAKE, u=FAKE, token=FAKE, ws=FAKE, n=1 << 40):
-        return lib.m3_sample_tokens(rows, vocab, dtype, z, u, None, 1.0, None, 0, None, 1.0, None, 0.0, token, None, ws, n, None)
+    def go(rows=4, vocab=64, dtype=1, z=FAKE, u=FAKE, token=FAKE):
+        return lib.m3_sample_tokens(rows, vocab, dtype, z, u, None, 1.0, None, 0, None, 1.0, None, 0.0, token, None, None)
 
     assert go(z=None) == go(u=None) == go(token=None) == 1
-    assert go(rows=0) == go(vocab=0) == 2 and go(vocab=(1 << 22) + 1) == go(dtype=2) == 3
-    assert go(z=FAKE + 1) == go(ws=FAKE + 8) == 5 and go(ws=None) == go(n=100) == 4
-    st, most = _size(lib.m3_sample_tokens_workspace_size, 1 << 30, 128000)
-    assert st == 0 and most < 1 << 30  # rows beyond a launch's take the same workspace
+    assert go(rows=0) == go(vocab=0) == 2 and go(vocab=(1 << 22) + 1) == go(rows=(1 << 30) + 1) == go(dtype=2) == 3
+    assert go(z=FAKE + 1) == 5
 
 
 def test_python_refuses_cpu_tensors_and_bad_shapes():
