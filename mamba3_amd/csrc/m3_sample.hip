@@ -4,13 +4,15 @@
 //   ones with mass >= m; token = the first whose running mass passes u times the kept mass.
 // Every bound cuts the same order, so what is kept is a prefix, and each step is the question which
 // token of the order a count or a mass falls on. It is answered without sorting the row. One block takes a row and holds
-// its first 126 KB in LDS (the rest is read anew in each pass: 256 rows of 128000 fp32 logits come from the last-level
-// cache). It finds the largest logit; adds up masses (and where top_k asks, counts) by distance from it, in 1024 bins
-// of T / 32; and gathers the tokens of the bins that may be kept, up to 1024, sorts them and reads the answers off. With
-// more, each question gathers the one bin that it falls in, which is split by its keys' bits until it fits.
-// With q = 32 (max z - z) / T in 64 bits, a token's mass is exp(-b / 32) exp(-r / 32), b the bin and r < 1: the bins add up
-// exp(-r / 32), five terms of its series to 1e-12, as whole numbers of 2^-45 or so, so that sums do not depend on their
-// order; exp(-b / 32) comes in once a bin. (An exponential for each token took three times as long.) What lies past the last bin
+// its first 112 KB in LDS (the rest is read anew in each pass: 256 rows of 128000 fp32 logits come from the last-level
+// cache). It finds the largest logit; adds up masses (and where top_k asks, counts) by distance from it, in 2048 bins
+// of T / 64; narrows every answer to a few bins, since what lies before and in a bin bounds the mass that the next question takes
+// its share of; gathers the tokens of all these bins in one pass, up to 1024, sorts them and reads the answers off. With
+// more (equal logits, low temperatures), each question gathers the one bin that it falls in, which is split by its keys' bits
+// until it fits.
+// With q = 64 (max z - z) / T in 64 bits, a token's mass is exp(-b / 64) exp(-r / 64), b the bin and r < 1: the bins add up
+// exp(-r / 64), four terms of its series to 1e-11, as whole numbers of 2^-45 or so, so that sums do not depend on their
+// order; exp(-b / 64) comes in once a bin. (An exponential for each token took three times as long.) What lies past the last bin
 // but one, below exp(-32) of the likeliest, is counted but has no mass. A border is missed with a probability of about
 // 1e-10 a row, as with 64-bit sums over sorted probabilities.
 // Bound by the row's read for large batches, by the chain of passes and barriers for few rows.
@@ -27,9 +29,11 @@ namespace m3 {
 typedef unsigned long long u64;
 constexpr int kSpThreads = 512;
 constexpr int kSpWaves = kSpThreads / 64;
-constexpr int kSpBins = 1024;
+constexpr int kSpBins = 2048;
+constexpr double kSpPerT = 64.0;  // bins of T / 64
 constexpr int kSpList = 1024;
-constexpr int kSpHeld = 126 << 10;  // bytes of a row in LDS
+constexpr int kSpParts = 1024;  // of a bin's keys
+constexpr int kSpHeld = 112 << 10;  // bytes of a row in LDS
 
 struct SampleArgs {
     const void* z;
@@ -58,7 +62,7 @@ constexpr unsigned kSpNone = 0x007fffffu;  // the key of -infinity
 
 // Distances from the largest logit in bins, as 64-bit numbers (NaN for NaN).
 struct SampleScale {
-    double top, per;  // per = 32 / T
+    double top, per;  // per = kSpPerT / T
     int shift;        // masses are whole numbers of 2^-shift
     __device__ __forceinline__ double far(float z) const { return (top - (double)z) * per; }
     // a logit at least as near as q, with room for rounding: what is below it is further
@@ -66,17 +70,23 @@ struct SampleScale {
         const double z = top - (q + 1e-6) / per;
         return (float)(z - fabs(z) * 1e-6);
     }
+    // a logit at least as far as q: what is above it is nearer
+    __device__ __forceinline__ float beyond(double q) const {
+        const double z = top - (q - 1e-6) / per;
+        return (float)(z + fabs(z) * 1e-6);
+    }
 };
+__device__ __forceinline__ int sp_bin(double q) { return q < (double)(kSpBins - 1) ? (int)q : kSpBins - 1; }
 __device__ __forceinline__ bool sp_in(double q, int bin) { return q >= (double)bin && (q < (double)(bin + 1) || bin == kSpBins - 1); }
 constexpr double kSpWhole = 4503599627370496.0;  // 2^52: what is added to it is rounded to a whole number, in its low bits
 __device__ __forceinline__ u64 sp_whole(double v) {  // of 0 <= v < 2^52
     return __builtin_bit_cast(u64, v + kSpWhole) & 0x000fffffffffffffull;
 }
 // A token's mass, and that times 2^shift as a whole number (shift <= 51), none past the last bin but one.
-__device__ __forceinline__ double sp_exp(const SampleScale& s, float z) { return exp(s.far(z) * (-1.0 / 32.0)); }
+__device__ __forceinline__ double sp_exp(const SampleScale& s, float z) { return exp(s.far(z) * (-1.0 / kSpPerT)); }
 __device__ __forceinline__ u64 sp_mass(const SampleScale& s, float z) {
     const double q = s.far(z);
-    return q < (double)(kSpBins - 1) ? sp_whole(ldexp(exp(q * (-1.0 / 32.0)), s.shift)) : 0;
+    return q < (double)(kSpBins - 1) ? sp_whole(ldexp(exp(q * (-1.0 / kSpPerT)), s.shift)) : 0;
 }
 
 struct SampleRow {
@@ -155,15 +165,19 @@ struct SampleLogits {
         }
         pieces_from(held, (vocab + E - 1) / E, one);
     }
-    // The same for the logits in [lo, hi]: a piece's are marked first, without a branch, and then taken one by one.
-    template <typename F>
-    __device__ __forceinline__ void each_in(float lo, float hi, F f) const {
+    // The same for the logits in one of kSpans spans [lo, hi]: a piece's are marked first, without a branch, and then taken
+    // one by one.
+    template <int kSpans, typename F>
+    __device__ __forceinline__ void each_in(const float (&lo)[kSpans], const float (&hi)[kSpans], F f) const {
         auto one = [&](const u32x4& w, int p) __attribute__((always_inline)) {
             unsigned marks = 0;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const float x = get(w, e);
-                marks |= ((x >= lo) & (x <= hi)) ? 1u << e : 0u;
+                bool in = false;
+#pragma unroll
+                for (int i = 0; i < kSpans; ++i) in |= (x >= lo[i]) & (x <= hi[i]);
+                marks |= in ? 1u << e : 0u;
             }
             while (marks) {
                 const int e = __builtin_ctz(marks);
@@ -189,7 +203,7 @@ struct SamplePlace {
 
 // The block's working memory.
 struct SampleShared {
-    u64 mass[kSpBins + 64];  // of the row's bins, and a place for each lane's tokens without mass
+    u64 mass[kSpBins + 64];  // of the row's bins, and a place for each lane's tokens without mass; then of all bins up to each
     unsigned count[kSpBins + 64];
     union {
         struct {
@@ -197,17 +211,15 @@ struct SampleShared {
             u64 parted[kSpList];  // by parts of the keys' span
         };
         struct {            // of a split bin's parts
-            u64 smass[kSpBins];
-            unsigned scount[kSpBins];
+            u64 smass[kSpParts];
+            unsigned scount[kSpParts];
         };
     };
     unsigned parts[kSpList];
     u64 wmass[kSpWaves];
     unsigned wcount[kSpWaves];
     unsigned n;
-    int at;
-    u64 before_mass;
-    unsigned before_count;
+    int at, to;
     SamplePlace place;
 };
 
@@ -273,30 +285,41 @@ struct SampleGoal {
     }
 };
 
-// The bin (s.at) whose end reaches the goal and whose start does not, or where none does `otherwise` (-1: none); s.before_*:
-// what lies before it, without base_*.
-__device__ __forceinline__ void sp_find_bin(SampleShared& s, const u64* mass, const unsigned* count, u64 base_c, u64 base_m, const SampleGoal& goal,
-                                            int otherwise) {
-    constexpr int kPer = kSpBins / kSpThreads;
-    static_assert(kPer * kSpThreads == kSpBins && kSpList % kSpThreads == 0, "whole shares");
-    unsigned c[kPer], tc = 0, all_c;
-    u64 m[kPer], tm = 0, all_m;
+// The bins' running sums in place of the bins' own; all of them.
+template <int kBins>
+__device__ __forceinline__ void sp_run(SampleShared& s, u64* mass, unsigned* count, unsigned& all_c, u64& all_m) {
+    constexpr int kPer = kBins / kSpThreads;
+    static_assert(kPer * kSpThreads == kBins && kSpList % kSpThreads == 0, "whole shares");
+    unsigned c[kPer], tc = 0;
+    u64 m[kPer], tm = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        c[i] = count[threadIdx.x * kPer + i], m[i] = mass[threadIdx.x * kPer + i];
-        tc += c[i], tm += m[i];
+        c[i] = tc += count[threadIdx.x * kPer + i];
+        m[i] = tm += mass[threadIdx.x * kPer + i];
     }
-    if (threadIdx.x == 0) s.at = -1;
     sp_scan(s, tc, tm, all_c, all_m);
-    const bool missed = !goal.reached(base_c + all_c, base_m + all_m);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) count[threadIdx.x * kPer + i] = tc + c[i], mass[threadIdx.x * kPer + i] = tm + m[i];
+    __syncthreads();
+}
+// The bins (s.at, s.to) whose end reaches the goals and whose start does not, or where none does `otherwise` (-1: none). `to` is
+// not easier to reach than `at`.
+template <int kBins>
+__device__ __forceinline__ void sp_find_bins(SampleShared& s, const u64* mass, const unsigned* count, u64 base_c, u64 base_m, const SampleGoal& at,
+                                             const SampleGoal& to, int otherwise) {
+    constexpr int kPer = kBins / kSpThreads;
+    if (threadIdx.x == 0) s.at = s.to = otherwise;
+    const int first = (int)threadIdx.x * kPer;
+    u64 c = base_c + (first ? count[first - 1] : 0), m = base_m + (first ? mass[first - 1] : 0);
+    bool at_before = at.reached(c, m), to_before = to.reached(c, m);
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const int b = (int)threadIdx.x * kPer + i;
-        if (missed ? b == otherwise : goal.reached(base_c + tc + c[i], base_m + tm + m[i]) && !goal.reached(base_c + tc, base_m + tm)) {
-            s.at = b;
-            s.before_count = tc, s.before_mass = tm;
-        }
-        tc += c[i], tm += m[i];
+        c = base_c + count[first + i], m = base_m + mass[first + i];
+        const bool at_now = at.reached(c, m), to_now = to.reached(c, m);
+        if (at_now & !at_before) s.at = first + i;
+        if (to_now & !to_before) s.to = first + i;
+        at_before = at_now, to_before = to_now;
     }
     __syncthreads();
 }
@@ -315,9 +338,11 @@ __device__ __forceinline__ void sp_span(SampleShared& s, unsigned& lo, unsigned&
         hi = y > hi ? y : hi;
     }
 }
-// Sorts the first n of the list from the largest key (and the lowest index) down: by 1024 parts of the keys' span, and within
+// Sorts the first n of the list from the largest key (and the lowest index) down: by 1024 parts, and within
 // a part by counting the larger ones; where a part has more than 48 (equal logits), all by exchanges of pairs.
-__device__ __forceinline__ void sp_sort(SampleShared& s, unsigned n) {
+// place(key): its part, below 1024, not falling as keys fall; with kByKeys parts of the keys' span.
+template <bool kByKeys, typename F>
+__device__ __forceinline__ void sp_sort(SampleShared& s, unsigned n, F place) {
     constexpr int kPer = kSpList / kSpThreads;
     u64 mine[kPer];
     unsigned klo = 0xffffffffu, khi = 0, part[kPer], nth[kPer];
@@ -329,12 +354,17 @@ __device__ __forceinline__ void sp_sort(SampleShared& s, unsigned n) {
         const unsigned key = (unsigned)(mine[i] >> 32);
         if (j < n) klo = key < klo ? key : klo, khi = key > khi ? key : khi;
     }
-    sp_span(s, klo, khi);
     int shift = 0;
-    while ((khi - klo) >> shift >= (unsigned)kSpList) ++shift;
+    if constexpr (kByKeys) {
+        sp_span(s, klo, khi);
+        while ((khi - klo) >> shift >= (unsigned)kSpList) ++shift;
+    } else {
+        __syncthreads();
+    }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        part[i] = (khi - (unsigned)(mine[i] >> 32)) >> shift;
+        const unsigned key = (unsigned)(mine[i] >> 32);
+        part[i] = kByKeys ? (khi - key) >> shift : place(key);
         nth[i] = threadIdx.x + i * kSpThreads < n ? atomicAdd(&s.parts[part[i]], 1u) : 0;
     }
     __syncthreads();
@@ -390,34 +420,79 @@ __device__ __forceinline__ void sp_sort(SampleShared& s, unsigned n) {
     }
     __syncthreads();
 }
-// A thread's part of the sorted list: its tokens' masses and what lies before them.
+// A thread's part of the sorted list: each token's count and mass before it, and the mass up to it.
 struct SampleWalk {
     static constexpr int kPer = kSpList / kSpThreads;
     unsigned n;
-    u64 m[kPer], before;
-    __device__ __forceinline__ void start(SampleShared& s, unsigned n_, const SampleScale& scale, u64 base) {
+    u64 count[kPer], before[kPer], after[kPer];
+    // of tokens that follow each other in the row's order, behind base_c and base_m
+    __device__ __forceinline__ void start(SampleShared& s, unsigned n_, const SampleScale& scale, u64 base_c, u64 base_m) {
         n = n_;
-        u64 all_m;
+        u64 m[kPer], all_m, at = 0;
         unsigned tc = 0, all_c;
-        before = 0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const unsigned j = threadIdx.x * kPer + i;
             m[i] = j < n ? sp_mass(scale, sp_logit((unsigned)(s.list[j] >> 32))) : 0;
-            before += m[i];
+            at += m[i];
         }
-        sp_scan(s, tc, before, all_c, all_m);
-        before += base;
+        sp_scan(s, tc, at, all_c, all_m);
+        at += base_m;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            count[i] = base_c + threadIdx.x * kPer + i;
+            before[i] = at;
+            after[i] = at += m[i];
+        }
     }
-    // the token that the goal falls on, in s.place, or the last where none reaches it: the masses of a bin, added up at once,
-    // may differ from their tokens' in the last bits (the caller waits)
-    __device__ __forceinline__ void find(SampleShared& s, const SampleGoal& goal, u64 base_c) const {
-        u64 bm = before;
+    // Of the tokens of whole bins that need not follow each other, by the bins' running sums: a bin's last
+    // token ends where the bin does. (The masses of a bin, added up at once, may differ from its tokens' in the last bits.) The
+    // running sums are lost.
+    __device__ __forceinline__ void start_bins(SampleShared& s, unsigned n_, const SampleScale& scale) {
+        start(s, n_, scale, 0, 0);
+        int bin[kPer], of_before = -1;
+        u64 end[kPer], begin[kPer];
+        unsigned begin_c[kPer];
+        bool first[kPer], last[kPer];
+        auto bin_of = [&](unsigned j) __attribute__((always_inline)) { return sp_bin(scale.far(sp_logit((unsigned)(s.list[j] >> 32)))); };
+        if (threadIdx.x * kPer < n && threadIdx.x > 0) of_before = bin_of(threadIdx.x * kPer - 1);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const unsigned j = threadIdx.x * kPer + i;
-            const u64 bc = base_c + j;
-            if (j < n && !goal.reached(bc, bm) && (j + 1 == n || goal.reached(bc + 1, bm + m[i]))) {
+            bin[i] = j < n ? bin_of(j) : -1;
+            first[i] = bin[i] != of_before;
+            of_before = bin[i];
+            const int b = bin[i] > 0 ? bin[i] : 0;
+            end[i] = s.mass[b];
+            begin[i] = b ? s.mass[b - 1] : 0, begin_c[i] = b ? s.count[b - 1] : 0;
+        }
+        const unsigned next = (threadIdx.x + 1) * kPer;
+        const int of_next = next < n ? bin_of(next) : -1;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) last[i] = bin[i] != (i + 1 < kPer ? bin[i + 1 < kPer ? i + 1 : 0] : of_next);
+        __syncthreads();
+        // what to add to the list's own sums in this bin
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            if (bin[i] >= 0 && first[i]) s.mass[bin[i]] = begin[i] - before[i], s.count[bin[i]] = begin_c[i] - (threadIdx.x * kPer + i);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int b = bin[i] > 0 ? bin[i] : 0;
+            const u64 more = s.mass[b];
+            count[i] = s.count[b] + (threadIdx.x * kPer + i);
+            before[i] += more, after[i] += more;
+            if (before[i] > end[i]) before[i] = end[i];
+            if (after[i] > end[i] || last[i]) after[i] = end[i];
+        }
+    }
+    // the token that the goal falls on, in s.place, or with kLast the last where none reaches it (the caller waits)
+    template <bool kLast>
+    __device__ __forceinline__ void find(SampleShared& s, const SampleGoal& goal) const {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const unsigned j = threadIdx.x * kPer + i;
+            if (j < n && !goal.reached(count[i], before[i]) && ((kLast && j + 1 == n) || goal.reached(count[i] + 1, after[i]))) {
                 const unsigned key = (unsigned)(s.list[j] >> 32);
                 unsigned less = 0, more = j;  // the first of its ties
                 while (less < more) {
@@ -425,9 +500,8 @@ struct SampleWalk {
                     if ((unsigned)(s.list[mid] >> 32) > key) less = mid + 1;
                     else more = mid;
                 }
-                s.place = SamplePlace{key, (int64_t)(j - less), bc, bm, m[i], (int)~(unsigned)s.list[j]};
+                s.place = SamplePlace{key, (int64_t)(j - less), count[i], before[i], after[i] - before[i], (int)~(unsigned)s.list[j]};
             }
-            bm += m[i];
         }
     }
 };
@@ -437,11 +511,11 @@ struct SampleWalk {
 template <typename L>
 __device__ __forceinline__ void sp_locate(SampleShared& s, const L& z, const SampleScale& scale, const SampleGoal& goal) {
     __syncthreads();
-    sp_find_bin(s, s.mass, s.count, 0, 0, goal, -1);
+    sp_find_bins<kSpBins>(s, s.mass, s.count, 0, 0, goal, goal, -1);
     const int bin = s.at;
-    u64 base_c = s.before_count, base_m = s.before_mass;
+    u64 base_c = bin > 0 ? s.count[bin - 1] : 0, base_m = bin > 0 ? s.mass[bin - 1] : 0;
     // first what may lie in the bin, by one comparison each way
-    float lo = bin < kSpBins - 1 ? scale.near((double)(bin + 1)) : -INFINITY, hi = INFINITY;
+    float lo[1] = {bin < kSpBins - 1 ? scale.near((double)(bin + 1)) : -INFINITY}, hi[1] = {bin > 0 ? scale.beyond((double)bin) : INFINITY};
     bool few = bin >= 0;
     if (!few && threadIdx.x == 0) s.place = SamplePlace{kSpNone, 0, 0, 0, 0, 0};  // not within the row: the caller's goals rule it out
     while (few) {
@@ -449,7 +523,7 @@ __device__ __forceinline__ void sp_locate(SampleShared& s, const L& z, const Sam
         __syncthreads();
         if (threadIdx.x == 0) s.n = 0;
         __syncthreads();
-        z.each_in(lo, hi, [&](float x, int v) __attribute__((always_inline)) {
+        z.template each_in<1>(lo, hi, [&](float x, int v) __attribute__((always_inline)) {
             if (x > -INFINITY && sp_in(scale.far(x), bin)) {
                 const unsigned i = atomicAdd(&s.n, 1u);
                 if (i < (unsigned)kSpList) s.list[i] = (u64)sp_key(x) << 32 | (unsigned)~v;
@@ -458,17 +532,17 @@ __device__ __forceinline__ void sp_locate(SampleShared& s, const L& z, const Sam
         __syncthreads();
         const unsigned n = s.n;
         if (n <= (unsigned)kSpList) {
-            sp_sort(s, n);
+            sp_sort<true>(s, n, [](unsigned) { return 0u; });
             SampleWalk walk;
-            walk.start(s, n, scale, base_m);
-            walk.find(s, goal, base_c);
+            walk.start(s, n, scale, base_c, base_m);
+            walk.find<true>(s, goal);
             few = false;
             continue;
         }
         // too many to sort: split the keys' span in 1024, or find one key
         unsigned klo = 0xffffffffu, khi = 0;
-        for (int b = threadIdx.x; b < kSpBins; b += kSpThreads) s.smass[b] = 0, s.scount[b] = 0;  // seen by all behind sp_span's barriers
-        z.each_in(lo, hi, [&](float x, int) __attribute__((always_inline)) {
+        for (int b = threadIdx.x; b < kSpParts; b += kSpThreads) s.smass[b] = 0, s.scount[b] = 0;  // seen by all behind sp_span's barriers
+        z.template each_in<1>(lo, hi, [&](float x, int) __attribute__((always_inline)) {
             if (x > -INFINITY && sp_in(scale.far(x), bin)) {
                 const unsigned key = sp_key(x);
                 klo = key < klo ? key : klo;
@@ -492,9 +566,9 @@ __device__ __forceinline__ void sp_locate(SampleShared& s, const L& z, const Sam
             continue;
         }
         int parts = 0;
-        while ((khi - klo) >> parts >= (unsigned)kSpBins) ++parts;
+        while ((khi - klo) >> parts >= (unsigned)kSpParts) ++parts;
         // from the largest key down
-        z.each_in(lo, hi, [&](float x, int) __attribute__((always_inline)) {
+        z.template each_in<1>(lo, hi, [&](float x, int) __attribute__((always_inline)) {
             if (x > -INFINITY && sp_in(scale.far(x), bin)) {
                 const int b = (int)((khi - sp_key(x)) >> parts);
                 atomicAdd(&s.scount[b], 1u);
@@ -502,12 +576,15 @@ __device__ __forceinline__ void sp_locate(SampleShared& s, const L& z, const Sam
             }
         });
         __syncthreads();
-        sp_find_bin(s, s.smass, s.scount, base_c, base_m, goal, (int)((khi - klo) >> parts));
+        unsigned all_c;
+        u64 all_m;
+        sp_run<kSpParts>(s, s.smass, s.scount, all_c, all_m);
+        sp_find_bins<kSpParts>(s, s.smass, s.scount, base_c, base_m, goal, goal, (int)((khi - klo) >> parts));
         const unsigned b = (unsigned)s.at;
-        base_c += s.before_count, base_m += s.before_mass;
+        if (b) base_c += s.scount[b - 1], base_m += s.smass[b - 1];
         const unsigned new_hi = khi - (b << parts), span = (1u << parts) - 1u;
-        lo = sp_logit(new_hi - klo > span ? new_hi - span : klo);
-        hi = sp_logit(new_hi);
+        lo[0] = sp_logit(new_hi - klo > span ? new_hi - span : klo);
+        hi[0] = sp_logit(new_hi);
     }
     __syncthreads();
 }
@@ -600,15 +677,15 @@ __global__ __launch_bounds__(kSpThreads) void sample_kernel(SampleArgs a, int he
         }
         return;
     }
-    const SampleScale scale{(double)top, 32.0 / r.t, a.shift};
+    const SampleScale scale{(double)top, kSpPerT / r.t, a.shift};
 
     // masses, and counts where a count is asked for
     const bool counts = r.k < (int64_t)a.vocab;
     unsigned tail = 0;  // tokens of the last bin, which have no mass
     {
-        // exp(-r / 32) 2^shift: the series' terms, -1 / 32 to the i over i!
-        const double unit = ldexp(1.0, a.shift);
-        const double c1 = unit * (-1.0 / 32), c2 = unit * (1.0 / 2048), c3 = unit * (-1.0 / 196608), c4 = unit * (1.0 / 25165824), c5 = unit * (-1.0 / 4026531840.0);
+        // exp(-r / 64) 2^shift: the series' terms, -1 / 64 to the i over i!
+        const double unit = ldexp(1.0, a.shift), c1 = unit * (-1.0 / kSpPerT), c2 = c1 * (-1.0 / (2 * kSpPerT)), c3 = c2 * (-1.0 / (3 * kSpPerT)),
+                     c4 = c3 * (-1.0 / (4 * kSpPerT));
         const int aside = kSpBins + ((int)threadIdx.x & 63);
         auto add = [&](float x, auto counted) __attribute__((always_inline)) {
             // without a branch: what has no mass (NaN, too) goes where nobody looks
@@ -616,7 +693,7 @@ __global__ __launch_bounds__(kSpThreads) void sample_kernel(SampleArgs a, int he
             const bool in = q < (double)(kSpBins - 1);
             const int b = (int)q, at = in ? b : aside;
             const double d = q - (double)b;
-            atomicAdd(&s.mass[at], sp_whole(fma(fma(fma(fma(fma(c5, d, c4), d, c3), d, c2), d, c1), d, unit)));
+            atomicAdd(&s.mass[at], sp_whole(fma(fma(fma(fma(c4, d, c3), d, c2), d, c1), d, unit)));
             if constexpr (decltype(counted)::value) {
                 atomicAdd(&s.count[at], 1u);
                 tail += !in & (x > -INFINITY);
@@ -636,63 +713,102 @@ __global__ __launch_bounds__(kSpThreads) void sample_kernel(SampleArgs a, int he
             sp_scan(s, tail, none, all_c, all);
             if (threadIdx.x == 0) s.count[kSpBins - 1] = all_c;
         }
-        unsigned c = 0;
-        total = 0;
         for (int b = threadIdx.x; b < kSpBins; b += kSpThreads) {
-            u64 m = s.mass[b];
+            const u64 m = s.mass[b];
             if (!counts) s.count[b] = (unsigned)((m + ((u64)1 << a.shift) - 1) >> a.shift);
-            m = (u64)((double)m * exp((double)b * (-1.0 / 32.0)) + 0.5);
-            s.mass[b] = m;
-            total += m;
+            s.mass[b] = (u64)((double)m * exp((double)b * (-1.0 / kSpPerT)) + 0.5);
         }
-        sp_scan(s, c, total, all_c, all);
-        total = all;
         __syncthreads();
+        sp_run<kSpBins>(s, s.mass, s.count, all_c, total);
     }
-    const bool by_p = r.p < 1.0, by_m = r.m > 0.0;
+    bool by_p = r.p < 1.0;
     const double min_p = r.m < 1.0 ? r.m : 1.0;
     // min_p keeps what is nearer than this; rounding of the logarithm matters to tokens that are as near as makes no
     // difference to a bin, and these are asked for their mass itself
-    const double far_m = by_m ? log(min_p) * -32.0 : 0.0;
+    const double far_m = r.m > 0.0 ? log(min_p) * -kSpPerT : (double)kSpBins;
+    bool by_m = far_m < (double)(kSpBins - 2);  // what is beyond has no mass
     auto kept_by_m = [&](float x) __attribute__((always_inline)) {
         const double q = scale.far(x);
         return q < far_m - 1e-6 || (q < far_m + 1e-6 && sp_exp(scale, x) >= min_p);
     };
 
-    // The bins that hold the answers: up to the k-th token's, which the other bounds are shares of, or without one up to the
-    // first that a bound lies in. Their tokens, if they are few, answer everything.
-    int last = kSpBins;
+    // The bins in which the answers lie: the k-th token's, that in which p of the k's mass is reached, the bound of min_p and the
+    // token's. What is known of a mass is that it lies between those of all before its bin and of all up to its end.
+    auto mass_to = [&](int bin) __attribute__((always_inline)) { return bin < 0 ? (u64)0 : s.mass[bin]; };
+    const auto share = [&](u64 of) __attribute__((always_inline)) {  // the token that reaches p is the last; the first stays whatever p is
+        const double m = r.p > 0.0 ? r.p * (double)of : 0.0;
+        return SampleGoal{kReach, 0, m > 1.0 ? m : 1.0};
+    };
+    const auto draw = [&](u64 of) __attribute__((always_inline)) {  // u below 1 falls within the kept mass; others are taken to its ends
+        const double m = u > 0.0 ? u * (double)of : 0.0, most = (double)of * (1.0 - 0x1p-30);
+        return SampleGoal{kPass, 0, m < most ? m : most};
+    };
+    constexpr int kSpans = 3;
+    int from[kSpans] = {0, 0, 0}, to[kSpans] = {-1, -1, -1};  // of bins: k's; p's and min_p's; the token's
+    const int m_from = by_m ? (int)fmax(far_m - 1e-6, 0.0) : 0, m_to = by_m ? (int)(far_m + 1e-6) : -1;
+    u64 low = total, high = total, kept = total;
     bool by_k = counts;
     if (by_k) {
-        sp_find_bin(s, s.mass, s.count, 0, 0, SampleGoal{kCount, (u64)r.k, 0.0}, -1);
+        const SampleGoal goal{kCount, (u64)r.k, 0.0};
+        sp_find_bins<kSpBins>(s, s.mass, s.count, 0, 0, goal, goal, -1);
         by_k = s.at >= 0;  // the row has so many tokens
-        if (by_k) last = s.at;
+        if (by_k) {
+            from[0] = to[0] = s.at;
+            low = mass_to(s.at - 1), high = mass_to(s.at);
+            if (low == high) by_k = false, to[0] = -1, kept = low;  // whichever it is
+        }
+    }
+    if (by_p) {
         __syncthreads();
+        sp_find_bins<kSpBins>(s, s.mass, s.count, 0, 0, share(low), share(high), kSpBins - 1);
+        from[1] = s.at, to[1] = s.to;
+        low = mass_to(from[1] - 1), high = mass_to(to[1]);
     }
-    if (by_p && !by_k) {
-        const double m = r.p > 0.0 ? r.p * (double)total : 0.0;
-        sp_find_bin(s, s.mass, s.count, 0, 0, SampleGoal{kReach, 0, m > 0.0 ? m : 1.0}, -1);
-        if (s.at >= 0) last = s.at;
+    u64 before_m = 0;
+    if (by_m) {
+        before_m = mass_to(m_from - 1);
+        const u64 up_to_m = mass_to(m_to);
+        if (before_m >= high) {  // the others leave less
+            by_m = false;
+        } else if (up_to_m <= low) {  // more, of which min_p leaves a part
+            by_k = by_p = false;
+            from[0] = 0, to[0] = -1, from[1] = m_from, to[1] = m_to;
+            kept = total, low = before_m, high = up_to_m;
+        } else {
+            // side by side with p's, a span holds both
+            from[1] = to[1] < 0 ? m_from : min(from[1], m_from), to[1] = max(to[1], m_to);
+            low = min(low, before_m), high = min(high, up_to_m);
+        }
     }
-    if (by_m && !by_k) {
-        const int b = (int)fmin(far_m + 1e-6, (double)(kSpBins - 1));
-        last = b < last ? b : last;
-    }
-    if (last < kSpBins) {  // more than fit?
-        unsigned c = 0, all_c;
-        u64 none = 0, all_m;
-        for (int b = threadIdx.x; b <= last; b += kSpThreads) c += s.count[b];
-        sp_scan(s, c, none, all_c, all_m);
-        if (all_c > (unsigned)kSpList) last = kSpBins;
+    __syncthreads();
+    sp_find_bins<kSpBins>(s, s.mass, s.count, 0, 0, draw(low), draw(high), kSpBins - 1);
+    from[2] = s.at, to[2] = s.to;
+    // the spans one after the other: the token's, p's and min_p's, k's
+    int skipped[kSpans], bins = 0;  // bins that lie before a span and are in none
+    unsigned some = 0;
+    float lo[kSpans], hi[kSpans];
+#pragma unroll
+    for (int i = kSpans - 1, done = 0; i >= 0; --i) {
+        from[i] = max(from[i], done);
+        skipped[i] = from[i] - bins;
+        lo[i] = INFINITY, hi[i] = -INFINITY;
+        if (to[i] < from[i]) continue;
+        bins += to[i] - from[i] + 1, done = to[i] + 1;
+        some += s.count[to[i]] - (from[i] ? s.count[from[i] - 1] : 0);
+        lo[i] = done < kSpBins ? scale.near((double)done) : -INFINITY;
+        hi[i] = from[i] > 0 ? scale.beyond((double)from[i]) : INFINITY;
     }
     unsigned n = kSpList + 1;
-    if (last < kSpBins) {
+    if (some <= (unsigned)kSpList) {
+        __syncthreads();
         if (threadIdx.x == 0) s.n = 0;
         __syncthreads();
-        const double end = (double)(last + 1);
-        const float near = last < kSpBins - 1 ? scale.near(end) : -INFINITY;  // first by one comparison
-        z.each_in(near, INFINITY, [&](float x, int v) __attribute__((always_inline)) {
-            if (x > -INFINITY && (scale.far(x) < end || last == kSpBins - 1)) {
+        z.template each_in<kSpans>(lo, hi, [&](float x, int v) __attribute__((always_inline)) {
+            const int b = sp_bin(scale.far(x));
+            bool in = false;
+#pragma unroll
+            for (int i = 0; i < kSpans; ++i) in |= (b >= from[i]) & (b <= to[i]);
+            if (in && x > -INFINITY) {
                 const unsigned i = atomicAdd(&s.n, 1u);
                 if (i < (unsigned)kSpList) s.list[i] = (u64)sp_key(x) << 32 | (unsigned)~v;
             }
@@ -701,93 +817,64 @@ __global__ __launch_bounds__(kSpThreads) void sample_kernel(SampleArgs a, int he
         n = s.n;
     }
 
-    u64 kept;
     float logit;
     int index;
     if (n <= (unsigned)kSpList) {
-        // all in the list: the bounds are places in it
-        sp_sort(s, n);
+        const double parts = (double)kSpList / (double)bins;
+        sp_sort<false>(s, n, [&](unsigned key) __attribute__((always_inline)) {
+            const double q = scale.far(sp_logit(key));
+            const int b = sp_bin(q);
+            const int less = b <= to[2] ? skipped[2] : b <= to[1] ? skipped[1] : skipped[0];
+            return (unsigned)fmin(fmax((q - (double)less) * parts, 0.0), (double)(kSpList - 1));
+        });
         SampleWalk walk;
-        walk.start(s, n, scale, 0);
-        constexpr int kPer = SampleWalk::kPer;
-        unsigned end = by_k && (u64)r.k < n ? (unsigned)r.k : n;
-        if (by_m) {
-            unsigned c = 0, all_c;
-            u64 none = 0, all_m;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const unsigned j = threadIdx.x * kPer + i;
-                c += j < n && kept_by_m(sp_logit((unsigned)(s.list[j] >> 32)));
-            }
-            sp_scan(s, c, none, all_c, all_m);
-            s.n = all_c;  // the same from every thread
+        walk.start_bins(s, n, scale);
+        if (by_k) {
+            walk.find<false>(s, SampleGoal{kCount, (u64)r.k, 0.0});
+            __syncthreads();
+            kept = s.place.mass + s.place.own;
+            __syncthreads();
         }
-        auto mass_to = [&](unsigned place) __attribute__((always_inline)) {  // of the list's first `place` >= 1
-            __syncthreads();
-            u64 m = walk.before;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                m += walk.m[i];
-                if (threadIdx.x * kPer + i + 1 == place) s.before_mass = m;
-            }
-            __syncthreads();
-            return s.before_mass;
-        };
-        kept = by_k ? mass_to(end) : total;
         if (by_p) {
-            const double m = r.p > 0.0 ? r.p * (double)kept : 0.0;
-            walk.find(s, SampleGoal{kReach, 0, m > 0.0 ? m : 1.0}, 0);
+            walk.find<false>(s, share(kept));
             __syncthreads();
-            const unsigned e = (unsigned)s.place.count + 1;
-            end = e < end ? e : end;
+            kept = s.place.mass + s.place.own;
+            __syncthreads();
         }
         if (by_m) {
-            __syncthreads();
-            const unsigned e = s.n > 0 ? s.n : 1;
-            end = e < end ? e : end;
+            u64 mine = 0, all_m;
+            unsigned none = 0, all_c;
+#pragma unroll
+            for (int i = 0; i < SampleWalk::kPer; ++i) {
+                const unsigned j = threadIdx.x * SampleWalk::kPer + i;
+                if (j >= n) continue;
+                const float x = sp_logit((unsigned)(s.list[j] >> 32));
+                const int b = sp_bin(scale.far(x));
+                if (b >= m_from && b <= m_to && kept_by_m(x)) mine += walk.after[i] - walk.before[i];
+            }
+            sp_scan(s, none, mine, all_c, all_m);
+            kept = min(kept, before_m + all_m);
         }
-        kept = mass_to(end);
-        // u below 1 falls within the kept mass; others are taken to its ends
-        const double goal = u > 0.0 ? u * (double)kept : 0.0, most = (double)kept * (1.0 - 0x1p-30);
-        walk.find(s, SampleGoal{kPass, 0, goal < most ? goal : most}, 0);
+        walk.find<false>(s, draw(kept));
         __syncthreads();
         logit = sp_logit(s.place.key), index = s.place.index;
     } else {
-        // the kept prefix ends behind (end_key, end_tie)
-        unsigned end_key = 0;
-        int64_t end_tie = a.vocab;
-        kept = total;
         SamplePlace q;
         for (int step = by_k ? 0 : by_p ? 1 : 2; step < 3; step = step == 0 && !by_p ? 2 : step + 1) {
-            SampleGoal goal;
-            if (step == 0) {
-                goal = SampleGoal{kCount, (u64)r.k, 0.0};
-            } else if (step == 1) {
-                // the token that reaches p of the k's mass is the last; the first stays whatever p is
-                const double m = r.p > 0.0 ? r.p * (double)kept : 0.0;
-                goal = SampleGoal{kReach, 0, m > 0.0 ? m : 1.0};
-            } else {
-                if (by_m) {
-                    // what min_p keeps: its mass, and its lowest key
-                    u64 mine = 0, all;
-                    unsigned low = 0xffffffffu, none = 0, all_c;
-                    z.each_in(scale.near(far_m), INFINITY, [&](float x, int) __attribute__((always_inline)) {
-                        if (x > -INFINITY && kept_by_m(x)) {
-                            mine += sp_mass(scale, x);
-                            low = sp_key(x) < low ? sp_key(x) : low;
-                        }
-                    });
-                    sp_scan(s, none, mine, all_c, all);
-                    unsigned unused = 0;
-                    sp_span(s, low, unused);
-                    if (low > end_key) end_key = low, end_tie = a.vocab, kept = all;
-                }
-                const double m = u > 0.0 ? u * (double)kept : 0.0, most = (double)kept * (1.0 - 0x1p-30);
-                goal = SampleGoal{kPass, 0, m < most ? m : most};
+            if (step == 2 && by_m) {
+                u64 mine = 0, all_m;
+                unsigned none = 0, all_c;
+                const float least[1] = {scale.near((double)(m_to + 1))}, most[1] = {m_from > 0 ? scale.beyond((double)m_from) : INFINITY};
+                z.template each_in<1>(least, most, [&](float x, int) __attribute__((always_inline)) {
+                    const int b = sp_bin(scale.far(x));
+                    if (b >= m_from && b <= m_to && kept_by_m(x)) mine += sp_mass(scale, x);
+                });
+                sp_scan(s, none, mine, all_c, all_m);
+                kept = min(kept, before_m + all_m);
             }
-            sp_locate(s, z, scale, goal);
+            sp_locate(s, z, scale, step == 0 ? SampleGoal{kCount, (u64)r.k, 0.0} : step == 1 ? share(kept) : draw(kept));
             q = s.place;
-            if (step < 2 && (q.key > end_key || (q.key == end_key && q.tie < end_tie))) end_key = q.key, end_tie = q.tie, kept = q.mass + q.own;
+            if (step < 2) kept = q.mass + q.own;
         }
         logit = sp_logit(q.key);
         index = q.index >= 0 ? q.index : sp_index(s, z.z, a.vocab, logit, q.tie);
