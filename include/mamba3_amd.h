@@ -523,13 +523,19 @@ int m3_mx_linear(int64_t rows, int32_t n, int32_t k, int32_t x_format, int32_t o
                  void* stream);
 
 /*
- * The same for x [rows, k] in x_dtype, quantised to e4m3 on the way: the bits of m3_mx_quantize and m3_mx_linear, in one
- * launch, for the sizes for which m3_mx_linear_takes_tensor returns 1 (at most 16 rows of together at most 32768 padded
- * elements, and so few columns that m3_mx_linear takes its kernel for few rows); others are unsupported.
+ * The same for a tensor x in x_dtype, quantised to e4m3 on the way: the bits of the two calls, in one launch. `before`:
+ *   M3_MX_AS_IS   x [rows, k] as m3_mx_quantize takes it
+ *   M3_MX_NORMED  x [rows, k] normed with norm_weight [k] and eps as by m3_add_rmsnorm_mx without a residual
+ *   M3_MX_GATED   x [rows, 2 k] as m3_mx_quantize takes it when gated
+ * For the sizes for which m3_mx_linear_takes_tensor returns 1 (at most 16 rows of together at most 32768 padded
+ * elements, and so few columns that m3_mx_linear takes its kernel for few rows; normed or gated, out_dtype equal to x_dtype, and
+ * normed at most 2048 columns); others are unsupported. norm_weight and eps are read only when normed.
  */
-int m3_mx_linear_takes_tensor(int64_t rows, int32_t n, int32_t k, int32_t out_dtype);
-int m3_mx_linear_tensor(int64_t rows, int32_t n, int32_t k, int32_t x_dtype, int32_t out_dtype, const void* x, const void* w_data,
-                        const void* w_scales, const void* residual, float scale, void* out, void* stream);
+enum m3_mx_before { M3_MX_AS_IS = 0, M3_MX_NORMED = 1, M3_MX_GATED = 2 };
+int m3_mx_linear_takes_tensor(int64_t rows, int32_t n, int32_t k, int32_t x_dtype, int32_t out_dtype, int32_t before);
+int m3_mx_linear_tensor(int64_t rows, int32_t n, int32_t k, int32_t x_dtype, int32_t out_dtype, int32_t before, const void* x,
+                        const void* norm_weight, float eps, const void* w_data, const void* w_scales, const void* residual,
+                        float scale, void* out, void* stream);
 
 /*
  * The next token of each row of logits [rows, vocab] from a random number u [rows] in [0, 1) (mamba3/block.py:208-222

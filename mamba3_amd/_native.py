@@ -208,8 +208,8 @@ def _declare(lib: ctypes.CDLL) -> None:
             ("m3_add_rmsnorm_bwd_workspace_size", [_i64, _i32, size_p]),
             ("m3_add_rmsnorm_bwd", [_i64, _i32, _i32] + [_vp] * 5 + [f32] + [_vp] * 4 + [ctypes.c_size_t, _vp]),
             ("m3_mx_linear", [_i64] + [_i32] * 4 + [_vp] * 5 + [f32] + [_vp] * 2),
-            ("m3_mx_linear_takes_tensor", [_i64] + [_i32] * 3),
-            ("m3_mx_linear_tensor", [_i64] + [_i32] * 4 + [_vp] * 4 + [f32] + [_vp] * 2),
+            ("m3_mx_linear_takes_tensor", [_i64] + [_i32] * 5),
+            ("m3_mx_linear_tensor", [_i64] + [_i32] * 5 + [_vp] * 2 + [f32] + [_vp] * 3 + [f32] + [_vp] * 2),
             ("m3_sample_tokens", [_i64, _i32, _i32, _vp, _vp, _vp, ctypes.c_double, _vp, _i64, _vp, ctypes.c_double, _vp,
                                   ctypes.c_double, _vp, _vp, _vp])):
         fn = getattr(lib, name)
@@ -644,15 +644,21 @@ def mx_linear(x_data, x_scales, x_format: str, w_data, w_scales, k: int, residua
         check(st, "m3_mx_linear")
 
 
-def mx_linear_takes_tensor(rows: int, n: int, k: int, out_dtype: torch.dtype) -> bool:
-    return bool(lib().m3_mx_linear_takes_tensor(rows, n, k, dtype_code(out_dtype)))
+# What happens to a tensor before it is quantised and multiplied.
+MX_AS_IS, MX_NORMED, MX_GATED = range(3)
 
 
-def mx_linear_tensor(x, w_data, w_scales, residual, scale: float, out) -> None:
-    """m3_mx_linear_tensor on contiguous x (rows, k) into contiguous out (rows, n)."""
+def mx_linear_takes_tensor(rows: int, n: int, k: int, x_dtype: torch.dtype, out_dtype: torch.dtype, before: int) -> bool:
+    return bool(lib().m3_mx_linear_takes_tensor(rows, n, k, dtype_code(x_dtype), dtype_code(out_dtype), before))
+
+
+def mx_linear_tensor(x, norm_weight, eps: float, gated: bool, w_data, w_scales, residual, scale: float, out) -> None:
+    """m3_mx_linear_tensor on contiguous x (rows, k), gated (rows, 2 k), into contiguous out (rows, n)."""
     rows, n = out.shape
-    st = lib().m3_mx_linear_tensor(rows, n, x.shape[1], dtype_code(x.dtype), dtype_code(out.dtype), x.data_ptr(),
-                                   w_data.data_ptr(), w_scales.data_ptr(), ptr(residual), scale, out.data_ptr(), stream_of(out))
+    before = MX_GATED if gated else MX_AS_IS if norm_weight is None else MX_NORMED
+    st = lib().m3_mx_linear_tensor(rows, n, x.shape[1] // 2 if gated else x.shape[1], dtype_code(x.dtype), dtype_code(out.dtype), before, x.data_ptr(),
+                                   ptr(norm_weight), eps, w_data.data_ptr(), w_scales.data_ptr(), ptr(residual), scale, out.data_ptr(),
+                                   stream_of(out))
     if st:
         check(st, "m3_mx_linear_tensor")
 

@@ -21,6 +21,8 @@ from . import _native, ops
 from .layer import KulaMamba, RMSNorm
 from .loss import linear_cross_entropy
 from .mlp import swiglu_mlp
+from .mx import MXTensor, mx_linear, quantize_mx
+from .sample import sample_tokens
 
 
 def add_scaled_linear(x: torch.Tensor, lin: nn.Linear, inp: torch.Tensor, scale: float,
@@ -55,6 +57,23 @@ def _as_written(m: nn.Module, cls: type) -> bool:
 def _only_weight(lin: nn.Module) -> bool:
     """Calling `lin` is x W^T."""
     return _as_written(lin, nn.Linear) and lin.bias is None
+
+
+def _mx_copy(owner: nn.Module, name: str, *weights: torch.Tensor) -> MXTensor:
+    """The 4-bit copy of the weights, one below the other, that `owner` keeps: made when first asked for and again after one
+    was replaced or changed in place (which their version counters tell). The copy holds on to the weights' memory, so an address
+    is not another weight's as long as it is compared."""
+    key = tuple((w.data_ptr(), 0 if w.is_inference() else w._version, w.dtype, w.device) for w in weights)
+    kept = owner.__dict__.get(name)
+    if kept is None or kept[0] != key:
+        if weights[0].is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a graph is being captured and the 4-bit weights are not there yet: run the model once before")
+        with torch.no_grad():
+            mx = quantize_mx(weights[0] if len(weights) == 1 else torch.cat(weights))
+        # from here on any stream may read them
+        torch.cuda.current_stream(mx.device).synchronize()
+        kept = owner.__dict__[name] = (key, mx, [w.detach() for w in weights])
+    return kept[1]
 
 
 class SwiGLU(nn.Module):
@@ -149,6 +168,40 @@ class KulaMambaBlock(nn.Module):
     # roundings differ (g, u and, in the backward, dh are not rounded to bf16).
     fused_mlp: bool = False
 
+    # Without gradients, multiply by 4-bit copies of the weights (KulaMambaLM.quantize_mx). Off by default.
+    mx_weights: bool = False
+
+    def _mx_projections(self) -> tuple[MXTensor, ...]:
+        """in_proj, out_proj and with an MLP [w_gate; w_up] and w_down in 4 bits."""
+        lins = [self.ssm.in_proj, self.ssm.out_proj]
+        whole = isinstance(self.ssm, KulaMamba) and _as_written(self.ssm_norm, RMSNorm) and self.ssm_norm.dim == -1
+        if self.use_mlp:
+            mlp = self.mlp
+            whole = whole and _as_written(mlp, SwiGLU) and _as_written(self.mlp_norm, RMSNorm) and self.mlp_norm.dim == -1
+            if whole:
+                lins += [mlp.w_gate, mlp.w_up, mlp.w_down]
+        if not whole or not all(_only_weight(lin) for lin in lins):
+            raise RuntimeError("4-bit weights need projections without bias and norms of the last dimension, without hooks or forwards of "
+                               "their own")
+        w = [lin.weight for lin in lins]
+        copies = (_mx_copy(lins[0], "_mx", w[0]), _mx_copy(lins[1], "_mx", w[1]))
+        return copies if not self.use_mlp else (*copies, _mx_copy(self.mlp, "_mx", w[2], w[3]), _mx_copy(lins[4], "_mx", w[4]))
+
+    def _mx_on(self) -> bool:
+        return self.mx_weights and not torch.is_grad_enabled()
+
+    @torch.compiler.disable
+    def _mx_block(self, x: torch.Tensor, ssd):
+        """The block on 4-bit weights: what is normed, gated and given out by the SSD is rounded to 8 bits as the next product's
+        input, the residual stays in x's type. ssd: in_proj's output -> (out_proj's input, state)."""
+        w, s = self._mx_projections(), self.residual_scale
+        y, state = ssd(mx_linear(x, w[0], norm_weight=self.ssm_norm.weight, eps=self.ssm_norm.eps))
+        x = mx_linear(y.view(*x.shape[:-1], -1), w[1], x, s)
+        if self.use_mlp:
+            gate_up = mx_linear(x, w[2], norm_weight=self.mlp_norm.weight, eps=self.mlp_norm.eps)
+            x = mx_linear(gate_up, w[3], x, s, gated=True)
+        return x, state
+
     def _ssm_forward(self, x_normed):
         return self.ssm(x_normed)
 
@@ -163,6 +216,8 @@ class KulaMambaBlock(nn.Module):
         """_own_input (internal): x is an intermediate of the caller's forward
         (KulaMambaLM), so without autograd the first residual add may overwrite it. The
         second add overwrites the first one's output whenever no autograd graph needs it."""
+        if self._mx_on():
+            return self._mx_block(x, self.ssm.ssd_from_proj)[0]
         ckpt = self.gradient_checkpointing and self.training
         nograd = not torch.is_grad_enabled()
         if ckpt:
@@ -220,6 +275,8 @@ class KulaMambaBlock(nn.Module):
         return x
 
     def step(self, x: torch.Tensor, ssm_state: dict):
+        if self._mx_on():
+            return self._mx_block(x, lambda proj: self.ssm._step_from_proj(proj, ssm_state))
         if self._small_step_usable(x):
             proj = ops.small_linear_fast(x, self.ssm_norm.weight, float(self.ssm_norm.eps),
                                     self.ssm.in_proj.weight, None, 1.0)
@@ -233,6 +290,8 @@ class KulaMambaBlock(nn.Module):
 
     def prefill(self, x: torch.Tensor, _own_input: bool = False):
         """_own_input as in forward."""
+        if self._mx_on():
+            return self._mx_block(x, lambda proj: self.ssm.ssd_from_proj(proj, return_state=True))
         nograd = not torch.is_grad_enabled()
         y, state = self.ssm._pre_out(self.ssm_norm(x), return_state=True)
         x = add_scaled_linear(x, self.ssm.out_proj, y, self.residual_scale,
@@ -306,6 +365,42 @@ class KulaMambaLM(nn.Module):
             layer.fused_mlp = on
         return self
 
+    # Without gradients, multiply by 4-bit copies of the weights (quantize_mx). Off by default.
+    mx_weights: bool = False
+
+    def quantize_mx(self, on: bool = True) -> "KulaMambaLM":
+        """Switches products without gradients (generate, and forward, loss, prefill and step under torch.no_grad()) to 4-bit
+        copies of the weights and activations in 8 bits, both microscaled (quantize_mx, mx_linear), or back and frees
+        the copies. Gradients and the embedding use the weights themselves, which stay. A copy is made anew when its weight was
+        replaced or changed in place; after changes through `.data`, which leave no trace, call this again. Needs projections
+        without bias."""
+        for m in self.modules():
+            m.__dict__.pop("_mx", None)
+        self.mx_weights = on
+        for layer in self.layers:
+            layer.mx_weights = on
+        if on:
+            try:
+                for layer in self.layers:
+                    layer._mx_projections()
+                self._mx_head()
+            except Exception:
+                self.quantize_mx(False)
+                raise
+        return self
+
+    def _mx_on(self) -> bool:
+        return self.mx_weights and not torch.is_grad_enabled()
+
+    def _mx_head(self) -> MXTensor:
+        if not (_only_weight(self.lm_head) and _as_written(self.norm, RMSNorm) and self.norm.dim == -1):
+            raise RuntimeError("4-bit weights need a head without bias and a norm of the last dimension, without hooks or forwards of their own")
+        return _mx_copy(self.lm_head, "_mx", self.lm_head.weight)
+
+    @torch.compiler.disable
+    def _mx_logits(self, x: torch.Tensor) -> torch.Tensor:
+        return mx_linear(x, self._mx_head(), norm_weight=self.norm.weight, eps=self.norm.eps)
+
     def loss(self, input_ids: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
         """The mean next-token cross entropy that forward returns as "loss" (fp32), without the
         logits: the head and the loss are one operator (linear_cross_entropy), so a training step
@@ -321,6 +416,8 @@ class KulaMambaLM(nn.Module):
         # the hidden states
         target = torch.full_like(labels, ignore_index)
         target[:, :-1] = labels[:, 1:]
+        if self._mx_on():
+            return F.cross_entropy(self._mx_logits(x).flatten(0, -2).float(), target.flatten(), ignore_index=ignore_index)
         x = self.norm(x)
         if not _only_weight(self.lm_head):
             return F.cross_entropy(self.lm_head(x).flatten(0, -2).float(), target.flatten(), ignore_index=ignore_index)
@@ -330,7 +427,7 @@ class KulaMambaLM(nn.Module):
         x = self.embedding(input_ids)
         for layer in self.layers:
             x = layer(x, _own_input=True)
-        logits = self.lm_head(self.norm(x))
+        logits = self._mx_logits(x) if self._mx_on() else self.lm_head(self.norm(x))
         result = {"logits": logits}
         if labels is not None:
             pred = logits[:, :-1].contiguous()
@@ -344,20 +441,37 @@ class KulaMambaLM(nn.Module):
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int = 100,
-                 temperature: float = 1.0, top_k: int | None = None) -> torch.Tensor:
+                 temperature: float = 1.0, top_k: int | None = None, top_p: float | None = None,
+                 min_p: float | None = None, generator: torch.Generator | None = None) -> torch.Tensor:
         """Parallel prefill of the prompt, then one `step` per new token
-        (mamba3/block.py:195-231). temperature=0 is greedy argmax."""
+        (mamba3/block.py:195-231). temperature=0 is greedy argmax.
+
+        With top_p, min_p or a generator (of the ids' device) tokens are drawn by sample_tokens from one random number a row, else
+        with torch.multinomial. There, a row whose logits are all NaN or -inf gives -1 and goes on with token 0; top_k keeps
+        exactly as many, ties from the lowest index."""
+        own = top_p is not None or min_p is not None or generator is not None
+        if own:
+            top_p, min_p = 1.0 if top_p is None else float(top_p), 0.0 if min_p is None else float(min_p)
+            if not (0.0 <= top_p <= 1.0 and 0.0 <= min_p <= 1.0 and temperature >= 0.0 and (top_k is None or top_k > 0)):
+                raise ValueError(f"need top_p and min_p in [0, 1], temperature of at least 0 and top_k of at least 1, got {top_p}, {min_p}, "
+                                 f"{temperature} and {top_k}")
         x = self.embedding(input_ids)
         states = []
         for layer in self.layers:
             x, st = layer.prefill(x, _own_input=True)
             states.append(st)
-        logits = self.lm_head(self.norm(x)[:, -1])
+        logits = self._mx_logits(x[:, -1]) if self._mx_on() else self.lm_head(self.norm(x)[:, -1])
         out = [input_ids]
         graph = None
         if self.decode_graph and max_new_tokens > 1 and input_ids.is_cuda:
             graph = _DecodeGraph(self, states, input_ids.shape[0])
         for _ in range(max_new_tokens):
+            if own:
+                u = torch.rand(logits.shape[0], device=logits.device, generator=generator)
+                nxt = sample_tokens(logits, u, temperature, top_k or 0, top_p, min_p).unsqueeze(1)
+                out.append(nxt)
+                logits = self._next_logits(nxt.squeeze(1).clamp(min=0), states, graph)
+                continue
             scores = logits / temperature if temperature > 0 else logits
             if top_k is not None:
                 kth = torch.topk(scores, min(top_k, scores.size(-1))).values[:, -1:]
@@ -367,30 +481,40 @@ class KulaMambaLM(nn.Module):
             else:
                 nxt = scores.argmax(dim=-1, keepdim=True)
             out.append(nxt)
-            if graph is not None:
-                logits = graph(nxt.squeeze(1))
-                continue
-            x = self.embedding(nxt.squeeze(1))
-            for i, layer in enumerate(self.layers):
-                x, states[i] = layer.step(x, states[i])
-            logits = _lm_logits(self, x)
+            logits = self._next_logits(nxt.squeeze(1), states, graph)
         return torch.cat(out, dim=1)
+
+    def _next_logits(self, tokens: torch.Tensor, states: list, graph: "_DecodeGraph | None") -> torch.Tensor:
+        """One step of decoding; without a graph `states` are replaced by the new ones."""
+        if graph is not None:
+            return graph(tokens)
+        x = self.embedding(tokens)
+        for i, layer in enumerate(self.layers):
+            x, states[i] = layer.step(x, states[i])
+        return _lm_logits(self, x)
 
 
 def _block_step_into(block: KulaMambaBlock, x: torch.Tensor, st_in: dict, st_out: dict):
     """KulaMambaBlock.step (mamba3/block.py:94-100) with the SSM step written into the
     caller's state buffers `st_out` (which must not alias `st_in`)."""
     ssm = block.ssm
+
+    def step(proj):
+        y = torch.empty(x.shape[0], ssm.d_inner, device=x.device, dtype=proj.dtype)
+        ops.step_into(proj, *ssm._small_params(), None, st_in["h"], st_in["prev_BX"],
+                      st_in["angle"], y, st_out["h"], st_out["prev_BX"], st_out["angle"],
+                      *ops.layer_args(ssm))
+        return y
+
+    if block._mx_on():
+        return block._mx_block(x, lambda proj: (step(proj), None))[0]
     small = block._small_step_usable(x)
     if small:
         proj = ops.small_linear_fast(x, block.ssm_norm.weight, float(block.ssm_norm.eps),
                                 ssm.in_proj.weight, None, 1.0)
     else:
         proj = ssm.in_proj(block.ssm_norm(x))
-    y = torch.empty(x.shape[0], ssm.d_inner, device=x.device, dtype=proj.dtype)
-    ops.step_into(proj, *ssm._small_params(), None, st_in["h"], st_in["prev_BX"],
-                  st_in["angle"], y, st_out["h"], st_out["prev_BX"], st_out["angle"],
-                  *ops.layer_args(ssm))
+    y = step(proj)
     if small:
         return block._small_step_tail(x, y)
     x = add_scaled_linear(x, ssm.out_proj, y, block.residual_scale)
@@ -402,6 +526,8 @@ def _block_step_into(block: KulaMambaBlock, x: torch.Tensor, st_in: dict, st_out
 def _lm_logits(lm: "KulaMambaLM", x: torch.Tensor) -> torch.Tensor:
     """lm_head(norm(x)) for decode rows x (B, d_model): one small-batch kernel (norm in its
     prologue) when it applies (mamba3/block.py:182-183)."""
+    if lm._mx_on():
+        return lm._mx_logits(x)
     w = lm.lm_head.weight
     if (lm.lm_head.bias is None and lm.norm.dim in (-1, 1)
             and ops.small_proj_usable(x, lm.norm.weight, w, norm=True)):

@@ -864,22 +864,27 @@ int m3_mx_linear(int64_t rows, int32_t n, int32_t k, int32_t x_format, int32_t o
                                 as_stream(stream));
 }
 
-int m3_mx_linear_takes_tensor(int64_t rows, int32_t n, int32_t k, int32_t out_dtype) {
-    return rows > 0 && n > 0 && k > 0 && m3::mx_linear_takes_tensor(rows, n, k, out_dtype) ? 1 : 0;
+int m3_mx_linear_takes_tensor(int64_t rows, int32_t n, int32_t k, int32_t x_dtype, int32_t out_dtype, int32_t before) {
+    return rows > 0 && n > 0 && k > 0 && m3::mx_linear_takes_tensor(rows, n, k, x_dtype, out_dtype, before) ? 1 : 0;
 }
 
-int m3_mx_linear_tensor(int64_t rows, int32_t n, int32_t k, int32_t x_dtype, int32_t out_dtype, const void* x, const void* w_data,
-                        const void* w_scales, const void* residual, float scale, void* out, void* stream) {
+int m3_mx_linear_tensor(int64_t rows, int32_t n, int32_t k, int32_t x_dtype, int32_t out_dtype, int32_t before, const void* x,
+                        const void* norm_weight, float eps, const void* w_data, const void* w_scales, const void* residual,
+                        float scale, void* out, void* stream) {
+    if (before < M3_MX_AS_IS || before > M3_MX_GATED) return M3_ERR_UNSUPPORTED;
+    if (before == M3_MX_NORMED && !norm_weight) return M3_ERR_NULL_POINTER;
     if (!x || !w_data || !w_scales || !out) return M3_ERR_NULL_POINTER;
     if (rows <= 0 || n <= 0 || k <= 0) return M3_ERR_INVALID_SHAPE;
     int st = check_dtype(x_dtype);
     if (st == M3_OK) st = check_dtype(out_dtype);
     if (st != M3_OK) return st;
-    if (n > (1 << 26) || !m3::mx_linear_takes_tensor(rows, n, k, out_dtype)) return M3_ERR_UNSUPPORTED;
+    if (n > (1 << 26) || !m3::mx_linear_takes_tensor(rows, n, k, x_dtype, out_dtype, before)) return M3_ERR_UNSUPPORTED;
+    if (before == M3_MX_NORMED && !aligned(norm_weight, size_of(x_dtype))) return M3_ERR_MISALIGNED;
     if (!aligned(x, size_of(x_dtype)) || !aligned(w_data, 16) || !aligned(w_scales, 4) || !aligned(out, size_of(out_dtype)) ||
         (residual && !aligned(residual, size_of(out_dtype))))
         return M3_ERR_MISALIGNED;
-    return m3::launch_mx_linear_tensor(x, x_dtype, w_data, w_scales, residual, scale, out, out_dtype, (int)rows, n, k, as_stream(stream));
+    return m3::launch_mx_linear_tensor(x, x_dtype, before, norm_weight, eps, w_data, w_scales, residual, scale, out, out_dtype, (int)rows, n, k,
+                                       as_stream(stream));
 }
 
 static int check_sample(int64_t rows, int32_t vocab) {

@@ -251,10 +251,11 @@ int launch_add_norm_bwd(const void* total, const void* w, const float* rstd, con
 int launch_mx_linear(const void* x, const void* xs, int x_format, const void* w, const void* ws,
                      const void* res, float scale, void* out, int out_dtype, int m, int n, int k,
                      hipStream_t stream);
-// ... of a tensor that is quantised to e4m3 on the way, where one launch does both: the same bits.
-bool mx_linear_takes_tensor(int64_t m, int64_t n, int64_t k, int out_dtype);
-int launch_mx_linear_tensor(const void* x, int x_dtype, const void* w, const void* ws, const void* res,
-                            float scale, void* out, int out_dtype, int m, int n, int k, hipStream_t stream);
+// ... of a tensor that is quantised to e4m3 on the way, behind its norm or gate (`before`: enum m3_mx_before), where one launch
+// does it all: the same bits.
+bool mx_linear_takes_tensor(int64_t m, int64_t n, int64_t k, int x_dtype, int out_dtype, int before);
+int launch_mx_linear_tensor(const void* x, int x_dtype, int before, const void* norm, float eps, const void* w, const void* ws,
+                            const void* res, float scale, void* out, int out_dtype, int m, int n, int k, hipStream_t stream);
 
 // The next token of each row of logits (m3_sample.hip): settings by row, or where their pointer is
 // NULL one for all (m3_status).

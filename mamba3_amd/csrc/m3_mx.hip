@@ -6,18 +6,13 @@
 #include "m3_common.h"
 #include "m3_kernels.h"
 #include "m3_mx.h"
+#include "m3_row.h"
 #include "mamba3_amd.h"
 
 namespace m3 {
 
 constexpr int kMxThreads = 256;
 constexpr int kMxUnits = 2;  // eights a thread
-
-// silu without the overflow of exp(-g): e = exp(-|g|) is at most 1.
-__device__ __forceinline__ float silu_any(float g) {
-    const float e = expf(-fabsf(g));
-    return (g < 0.f ? g * e : g) / (1.f + e);
-}
 
 template <typename T, int F, bool kGated>
 __global__ __launch_bounds__(kMxThreads) void mx_quantize_kernel(const T* __restrict__ x, uint8_t* __restrict__ data,

@@ -17,6 +17,7 @@
 #include "m3_common.h"
 #include "m3_kernels.h"
 #include "m3_mx.h"
+#include "m3_row.h"
 #include "mamba3_amd.h"
 
 namespace m3 {
@@ -30,6 +31,10 @@ struct MxLinearArgs {
     void* out;
     float scale;
     int M, N, steps;  // steps of 128 k
+};
+struct MxBefore {  // of a tensor: its norm's weight
+    const void* norm;
+    float eps;
 };
 
 __device__ __forceinline__ i32x8 wide(i32x4 lo, i32x4 hi) {
@@ -183,11 +188,14 @@ __global__ __launch_bounds__(kMlWaves * 64) void mx_linear_few_kernel(MxLinearAr
 
 // The same for at most 16 rows of a tensor, which each block quantises to e4m3 into LDS first: one launch less, and the
 // weights' first reads are on their way meanwhile. Rows of LDS are XOR-swizzled in 16-byte pieces. The sums are those of
-// the kernel above on the quantised rows, bit for bit.
+// the kernel above on the quantised rows, bit for bit. In front of the rounding may stand the norm (a wave takes a row as
+// m3_add_norm.hip's does: the same sums) or silu(gate) * up.
 constexpr int kMlRawRows = 16;
 constexpr int kMlRawBytes = 32768;  // of quantised elements (with more, quantising in every block takes longer than the launch)
-template <typename T, int FN, typename TO>
-__global__ __launch_bounds__(kMlWaves * 64) void mx_linear_raw_kernel(MxLinearArgs a, int k, bool whole) {
+constexpr int kMlNormPieces = 4;    // of 512 columns: a wave's row
+enum { kAsIs, kNormed, kGated };
+template <typename T, int kPre, int FN, typename TO>
+__global__ __launch_bounds__(kMlWaves * 64) void mx_linear_raw_kernel(MxLinearArgs a, MxBefore before, int k, bool whole) {
     constexpr bool kExact = sizeof(TO) == 4;
     extern __shared__ __align__(16) char mx_smem[];  // [M][kp] elements, [M][kp / 32] scales
     __shared__ f32x4 part[kMlWaves][FN][64];
@@ -204,12 +212,45 @@ __global__ __launch_bounds__(kMlWaves * 64) void mx_linear_raw_kernel(MxLinearAr
     }
     uint8_t* xs = reinterpret_cast<uint8_t*>(mx_smem) + a.M * kp;
     const int units = kp / 8;
-    for (int i = threadIdx.x; i < a.M * units; i += kMlWaves * 64) {  // whole groups of four: units come in sixteens
-        const int row = i / units, unit = i - row * units;
-        float v[8];
-        load8(reinterpret_cast<const T*>(a.x) + (int64_t)row * k, unit * 8, k, v);
+    auto put = [&](float (&v)[8], int row, int unit) __attribute__((always_inline)) {
         const int at = (unit >> 1 ^ (row & 7)) * 2 + (unit & 1);  // its 16-byte piece
         mx_store8_at<kE4m3>(v, reinterpret_cast<uint8_t*>(mx_smem) + row * kp + at * 8, xs + row * (kp / 32) + (unit >> 2), (unit & 3) == 0);
+    };
+    if constexpr (kPre == kNormed) {
+        float nw[kMlNormPieces][8], t[kMlNormPieces][8];
+#pragma unroll
+        for (int p = 0; p < kMlNormPieces; ++p) load8(reinterpret_cast<const T*>(before.norm), (lane + p * 64) * 8, k, nw[p]);
+        for (int row = wave; row < a.M; row += kMlWaves) {
+            float ss = 0.f;
+#pragma unroll
+            for (int p = 0; p < kMlNormPieces; ++p) load8(reinterpret_cast<const T*>(a.x) + (int64_t)row * k, (lane + p * 64) * 8, k, t[p]);
+#pragma unroll
+            for (int p = 0; p < kMlNormPieces; ++p)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ss = fmaf(t[p][e], t[p][e], ss);
+            const float rs = inv_sqrt((float)(wave_sum_f64((double)ss) / k + (double)before.eps));
+#pragma unroll
+            for (int p = 0; p < kMlNormPieces; ++p) {
+                if (lane + p * 64 >= units) continue;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) t[p][e] = t[p][e] * rs * nw[p][e];
+                put(t[p], row, lane + p * 64);
+            }
+        }
+    } else {
+        for (int i = threadIdx.x; i < a.M * units; i += kMlWaves * 64) {  // whole groups of four: units come in sixteens
+            const int row = i / units, unit = i - row * units;
+            const T* x = reinterpret_cast<const T*>(a.x) + (int64_t)row * k * (kPre == kGated ? 2 : 1);
+            float v[8];
+            load8(x, unit * 8, k, v);
+            if constexpr (kPre == kGated) {
+                float u[8];
+                load8(x + k, unit * 8, k, u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = silu_any(v[e]) * u[e];
+            }
+            put(v, row, unit);
+        }
     }
     __syncthreads();
     f32x4 acc[1][FN];
@@ -259,18 +300,25 @@ static int few_m(const MxLinearArgs& a, hipStream_t stream) {
     if (fn == 2) return few_t<FA, FM, 2, TO>(a, stream);
     return few_t<FA, FM, 4, TO>(a, stream);
 }
-template <typename T, int FN, typename TO>
-static int raw_t(const MxLinearArgs& a, int k, hipStream_t stream) {
+template <typename T, int kPre, int FN, typename TO>
+static int raw_t(const MxLinearArgs& a, const MxBefore& before, int k, hipStream_t stream) {
     const int lds = a.M * a.steps * (kMxStep + 4);
-    hipLaunchKernelGGL((mx_linear_raw_kernel<T, FN, TO>), dim3((unsigned)((a.N + 16 * FN - 1) / (16 * FN))), dim3(kMlWaves * 64), lds, stream, a, k, out4<TO>(a));
+    hipLaunchKernelGGL((mx_linear_raw_kernel<T, kPre, FN, TO>), dim3((unsigned)((a.N + 16 * FN - 1) / (16 * FN))), dim3(kMlWaves * 64), lds, stream, a, before,
+                       k, out4<TO>(a));
     return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH;
 }
-template <typename T, typename TO>
-static int raw_n(const MxLinearArgs& a, int k, hipStream_t stream) {
+template <typename T, int kPre, typename TO>
+static int raw_n(const MxLinearArgs& a, const MxBefore& before, int k, hipStream_t stream) {
     const int fn = few_columns(a, 16);
-    if (fn == 1) return raw_t<T, 1, TO>(a, k, stream);
-    if (fn == 2) return raw_t<T, 2, TO>(a, k, stream);
-    return raw_t<T, 4, TO>(a, k, stream);
+    if (fn == 1) return raw_t<T, kPre, 1, TO>(a, before, k, stream);
+    if (fn == 2) return raw_t<T, kPre, 2, TO>(a, before, k, stream);
+    return raw_t<T, kPre, 4, TO>(a, before, k, stream);
+}
+template <typename T>
+static int raw_pre(const MxLinearArgs& a, int pre, const MxBefore& before, int k, hipStream_t stream) {
+    if (pre == kNormed) return raw_n<T, kNormed, T>(a, before, k, stream);
+    if (pre == kGated) return raw_n<T, kGated, T>(a, before, k, stream);
+    return raw_n<T, kAsIs, T>(a, before, k, stream);
 }
 
 // Many rows: tiles through LDS, as in m3_gemm.h. A block of WGM x WGN waves owns a BM x BN tile (a wave 32 FM x 64)
@@ -651,16 +699,19 @@ static MxLinearArgs linear_args(const void* x, const void* xs, const void* w, co
     const auto b = [](const void* p) { return reinterpret_cast<const uint8_t*>(p); };
     return MxLinearArgs{b(x), b(xs), b(w), b(ws), res, out, scale, m, n, (int)(mx_padded(k) / kMxStep)};
 }
-bool mx_linear_takes_tensor(int64_t m, int64_t n, int64_t k, int out_dtype) {
+bool mx_linear_takes_tensor(int64_t m, int64_t n, int64_t k, int x_dtype, int out_dtype, int before) {
     if (m > kMlRawRows || m * mx_padded(k) > kMlRawBytes) return false;
+    if (before != kAsIs && x_dtype != out_dtype) return false;
+    if (before == kNormed && k > kMlNormPieces * 512) return false;
     const MxLinearArgs a = linear_args(nullptr, nullptr, nullptr, nullptr, nullptr, 1.f, nullptr, (int)m, (int)n, (int)k);
     return out_dtype != M3_DTYPE_BF16 || !takes_tiles(a);
 }
-int launch_mx_linear_tensor(const void* x, int x_dtype, const void* w, const void* ws, const void* res, float scale, void* out,
-                            int out_dtype, int m, int n, int k, hipStream_t stream) {
+int launch_mx_linear_tensor(const void* x, int x_dtype, int before, const void* norm, float eps, const void* w, const void* ws, const void* res,
+                            float scale, void* out, int out_dtype, int m, int n, int k, hipStream_t stream) {
     const MxLinearArgs a = linear_args(x, nullptr, w, ws, res, scale, out, m, n, k);
-    if (x_dtype == M3_DTYPE_BF16) return out_dtype == M3_DTYPE_BF16 ? raw_n<bf16, bf16>(a, k, stream) : raw_n<bf16, float>(a, k, stream);
-    return out_dtype == M3_DTYPE_BF16 ? raw_n<float, bf16>(a, k, stream) : raw_n<float, float>(a, k, stream);
+    const MxBefore b{norm, eps};
+    if (x_dtype == out_dtype) return x_dtype == M3_DTYPE_BF16 ? raw_pre<bf16>(a, before, b, k, stream) : raw_pre<float>(a, before, b, k, stream);
+    return x_dtype == M3_DTYPE_BF16 ? raw_n<bf16, kAsIs, float>(a, b, k, stream) : raw_n<float, kAsIs, bf16>(a, b, k, stream);
 }
 int launch_mx_linear(const void* x, const void* xs, int x_format, const void* w, const void* ws, const void* res, float scale,
                      void* out, int out_dtype, int m, int n, int k, hipStream_t stream) {

@@ -679,7 +679,7 @@ __global__ __launch_bounds__(kSpThreads) void sample_kernel(SampleArgs a, int he
         }
         return;
     }
-    const SampleScale scale{(double)top, kSpPerT / r.t, a.shift};
+    const SampleScale scale{(double)top, fmin(kSpPerT / r.t, 1e300), a.shift};  // finite: the first lies at 0 times it
 
     // masses, and counts where a count is asked for
     const bool counts = r.k < (int64_t)a.vocab;

@@ -91,10 +91,14 @@ def silu_mul_mx(gate_up: torch.Tensor, format: str = "e4m3") -> MXTensor:
 
 
 def mx_linear(x: MXTensor | torch.Tensor, weight: MXTensor, residual: torch.Tensor | None = None, scale: float = 1.0,
-              out_dtype: torch.dtype | None = None) -> torch.Tensor:
+              out_dtype: torch.dtype | None = None, norm_weight: torch.Tensor | None = None, eps: float = 1e-5,
+              gated: bool = False) -> torch.Tensor:
     """[residual +] scale * x weight^T for weight (n, k) in e2m1 and x (..., k): microscaled in either format, or
     a tensor, which is quantised to e4m3 on the way. The result (..., n) has out_dtype: by default the residual's type,
     x's, or bf16. No backward.
+
+    A tensor is first normed where norm_weight (k,) is given (add_rms_norm_mx with eps and without a residual), or with `gated`
+    is (..., 2 k) and enters as silu_mul_mx gives it. The results are those of the separate calls; for few rows one launch does it.
 
     Sums are fp32. For a bf16 result the matrix instructions align the 128 products that they add at a time at about
     2^-13 of the largest where x is e4m3; an fp32 result has no such step."""
@@ -107,8 +111,17 @@ def mx_linear(x: MXTensor | torch.Tensor, weight: MXTensor, residual: torch.Tens
             raise ValueError("mx_linear expects x (..., k)")
         refuse_gradients("mx_linear", x)
         _native.dtype_code(x.dtype)
-    if x.shape[-1] != k or n < 1:
-        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit (..., k) and (n, k)")
+    elif gated or norm_weight is not None:
+        raise ValueError("norm_weight and gated are for a tensor, x is microscaled already")
+    if x.shape[-1] != (2 * k if gated else k) or n < 1:
+        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit (..., {'2 k' if gated else 'k'}) and (n, k)")
+    if norm_weight is not None:
+        if gated:
+            raise ValueError("either norm_weight or gated")
+        if norm_weight.shape != (k,) or norm_weight.dtype != x.dtype or norm_weight.device != x.device:
+            raise ValueError(f"norm_weight must be {x.dtype} of shape {(k,)} on {x.device}, got {norm_weight.dtype} "
+                             f"{tuple(norm_weight.shape)} on {norm_weight.device}")
+        refuse_gradients("mx_linear", norm_weight)
     if out_dtype is None:
         out_dtype = residual.dtype if residual is not None else x.dtype if plain else torch.bfloat16
     _native.dtype_code(out_dtype)
@@ -122,9 +135,16 @@ def mx_linear(x: MXTensor | torch.Tensor, weight: MXTensor, residual: torch.Tens
             raise ValueError(f"residual must be {out_dtype} of shape {shape} on {x.device}, got {residual.dtype} "
                              f"{tuple(residual.shape)} on {residual.device}")
         refuse_gradients("mx_linear", residual)
-    if plain and ops.mx_linear_takes_tensor(x, n, out_dtype):
-        out = ops.mx_linear_tensor_fast(x, weight.data, weight.scales, residual, float(scale), out_dtype)
+    before = _native.MX_GATED if gated else _native.MX_AS_IS if norm_weight is None else _native.MX_NORMED
+    if plain and ops.mx_linear_takes_tensor(x, n, k, out_dtype, before):
+        out = ops.mx_linear_tensor_fast(x, norm_weight, float(eps), gated, weight.data, weight.scales, residual, float(scale), out_dtype)
     else:
-        q = quantize_mx(x, "e4m3") if plain else x
+        q = x
+        if gated:
+            q = silu_mul_mx(x)
+        elif norm_weight is not None:
+            q = _mx(*ops.add_rmsnorm_mx_fast(x, None, norm_weight, 1.0, float(eps), "e4m3")[1:], x.shape, "e4m3")
+        elif plain:
+            q = quantize_mx(x, "e4m3")
         out = ops.mx_linear_fast(q.data, q.scales, q.format, weight.data, weight.scales, k, residual, float(scale), out_dtype)
     return out if len(shape) == 2 else out.view(shape)

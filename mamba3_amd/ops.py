@@ -1206,24 +1206,25 @@ def _(x_data, x_scales, x_format, w_data, w_scales, k, residual, scale, dtype):
 
 
 @functools.lru_cache(maxsize=1024)
-def _takes_tensor(rows: int, n: int, k: int, dtype: torch.dtype) -> bool:
-    return _native.mx_linear_takes_tensor(rows, n, k, dtype)
+def _takes_tensor(rows: int, n: int, k: int, x_dtype: torch.dtype, dtype: torch.dtype, before: int) -> bool:
+    return _native.mx_linear_takes_tensor(rows, n, k, x_dtype, dtype, before)
 
 
-def mx_linear_takes_tensor(x: torch.Tensor, n: int, dtype: torch.dtype) -> bool:
-    """True where one launch quantises x and multiplies (sizes alone decide; under torch.compile these may be
-    symbolic, and two launches run)."""
-    return not _is_compiling() and x.numel() > 0 and _takes_tensor(x.numel() // x.shape[-1], n, x.shape[-1], dtype)
+def mx_linear_takes_tensor(x: torch.Tensor, n: int, k: int, dtype: torch.dtype, before: int) -> bool:
+    """True where one launch quantises x, behind its norm or gate, and multiplies (sizes and types alone decide; under
+    torch.compile sizes may be symbolic, and two launches run)."""
+    return not _is_compiling() and x.numel() > 0 and _takes_tensor(x.numel() // x.shape[-1], n, k, x.dtype, dtype, before)
 
 
-def _mx_linear_tensor_eager(x: torch.Tensor, w_data: torch.Tensor, w_scales: torch.Tensor, residual: Optional[torch.Tensor],
-                            scale: float, dtype: torch.dtype) -> torch.Tensor:
+def _mx_linear_tensor_eager(x: torch.Tensor, norm_weight: Optional[torch.Tensor], eps: float, gated: bool, w_data: torch.Tensor,
+                            w_scales: torch.Tensor, residual: Optional[torch.Tensor], scale: float, dtype: torch.dtype) -> torch.Tensor:
     """m3_mx_linear_tensor: (rows, n) in `dtype`."""
-    _native.require_gpu(x, w_data, w_scales, residual)
+    _native.require_gpu(x, norm_weight, w_data, w_scales, residual)
     with on_device(x):
         x2 = _rows_of(x)
         out = torch.empty((x2.shape[0], w_data.shape[0]), device=x.device, dtype=dtype)
-        _native.mx_linear_tensor(x2, w_data, w_scales, None if residual is None else _rows_of(residual), scale, out)
+        _native.mx_linear_tensor(x2, None if norm_weight is None else norm_weight.contiguous(), eps, gated, w_data, w_scales,
+                                 None if residual is None else _rows_of(residual), scale, out)
     return out
 
 
@@ -1231,7 +1232,7 @@ mx_linear_tensor = torch.library.custom_op(f"{NS}::mx_linear_tensor", _mx_linear
 
 
 @mx_linear_tensor.register_fake
-def _(x, w_data, w_scales, residual, scale, dtype):
+def _(x, norm_weight, eps, gated, w_data, w_scales, residual, scale, dtype):
     return x.new_empty((x.numel() // x.shape[-1], w_data.shape[0]), dtype=dtype)
 
 
@@ -1286,9 +1287,9 @@ def mx_linear_fast(x_data, x_scales, x_format, w_data, w_scales, k, residual, sc
     return fn(x_data, x_scales, x_format, w_data, w_scales, k, residual, scale, dtype)
 
 
-def mx_linear_tensor_fast(x, w_data, w_scales, residual, scale, dtype):
-    fn = _mx_linear_tensor_eager if _plain(x, w_data, w_scales, residual) else mx_linear_tensor
-    return fn(x, w_data, w_scales, residual, scale, dtype)
+def mx_linear_tensor_fast(x, norm_weight, eps, gated, w_data, w_scales, residual, scale, dtype):
+    fn = _mx_linear_tensor_eager if _plain(x, norm_weight, w_data, w_scales, residual) else mx_linear_tensor
+    return fn(x, norm_weight, eps, gated, w_data, w_scales, residual, scale, dtype)
 
 
 def sample_tokens_fast(logits, u, temperatures, temperature, top_ks, top_k, top_ps, top_p, min_ps, min_p, logprob):

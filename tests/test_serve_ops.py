@@ -162,3 +162,40 @@ def test_mxtensor_refuses_what_does_not_fit():
 def test_header_names_the_stored_layout():
     assert [_native.mx_padded(k) for k in (1, 128, 129, 500)] == [128, 128, 256, 512]
     assert _native.mx_row_bytes(500, "e4m3") == 512 and _native.mx_row_bytes(500, "e2m1") == 256
+
+
+def test_python_refuses_what_does_not_go_in_front_of_a_product():
+    x = torch.randn(4, 64)
+    w = MXTensor(torch.zeros(8, 64, dtype=torch.uint8), torch.zeros(8, 4, dtype=torch.uint8), (8, 64), "e2m1")
+    for call in (lambda: mamba3_amd.mx_linear(w, w, gated=True), lambda: mamba3_amd.mx_linear(w, w, norm_weight=x[0]), lambda: mamba3_amd.mx_linear(x, w, gated=True),
+                 lambda: mamba3_amd.mx_linear(torch.randn(4, 128), w, norm_weight=x[0], gated=True), lambda: mamba3_amd.mx_linear(x, w, norm_weight=x[0, :63]),
+                 lambda: mamba3_amd.mx_linear(x, w, norm_weight=x), lambda: mamba3_amd.mx_linear(x, w, norm_weight=x[0].bfloat16())):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(RuntimeError, match="no backward"):
+        mamba3_amd.mx_linear(x, w, norm_weight=x[0].clone().requires_grad_())
+
+
+def test_mx_linear_tensor_refuses_bad_arguments(lib):
+    def go(rows=4, n=8, k=64, x_dtype=0, out_dtype=0, before=0, x=FAKE, norm=None, w=FAKE, ws=FAKE, res=None, out=FAKE):
+        return lib.m3_mx_linear_tensor(rows, n, k, x_dtype, out_dtype, before, x, norm, 1e-5, w, ws, res, 1.0, out, None)
+
+    assert go(x=None) == go(w=None) == go(ws=None) == go(out=None) == go(before=1) == 1
+    assert go(rows=0) == go(n=0) == go(k=0) == 2
+    assert go(before=3) == go(before=-1) == go(x_dtype=2) == go(out_dtype=2) == go(rows=17) == go(k=8193) == go(n=(1 << 26) + 1) == 3
+    assert go(before=1, norm=FAKE, k=2049) == go(before=1, norm=FAKE, out_dtype=1) == go(before=2, out_dtype=1) == 3
+    assert go(x=FAKE + 2) == go(w=FAKE + 8) == go(ws=FAKE + 2) == go(out=FAKE + 2) == go(res=FAKE + 1) == go(before=1, norm=FAKE + 1) == 5
+
+
+def test_model_refuses_what_it_cannot_serve():
+    lm = mamba3_amd.KulaMambaLM(50, 64, n_layers=1, d_state=16, headdim=16, mimo_rank=1)
+    with pytest.raises(RuntimeError, match="GPU"):
+        lm.quantize_mx()
+    assert not lm.mx_weights and not lm.layers[0].mx_weights
+    biased = mamba3_amd.KulaMambaLM(50, 64, n_layers=1, d_state=16, headdim=16, mimo_rank=1, bias=True)
+    with pytest.raises(RuntimeError, match="bias"):
+        biased.quantize_mx()
+    ids = torch.zeros(1, 3, dtype=torch.long)
+    for bad in (dict(top_p=1.5), dict(min_p=-0.1), dict(top_p=0.5, top_k=0), dict(top_p=0.5, temperature=-1.0), dict(min_p=math.nan)):
+        with pytest.raises(ValueError, match="top_p"):
+            lm.generate(ids, 1, **bad)
