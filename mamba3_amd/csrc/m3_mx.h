@@ -144,11 +144,14 @@ __device__ __forceinline__ void mx_unpack8(u32x2 w, float (&v)[8]) {
 template <typename T>
 __device__ __forceinline__ void load8(const T* row, int c, int n, float (&v)[8]) {
     T t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] = (T)0.f;
     if (c + 8 <= n) {
         __builtin_memcpy(t, row + c, 8 * sizeof(T));
-    } else {
+    } else if (c < n) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t[e] = c + e < n ? row[c + e] : (T)0.f;
+        for (int e = 0; e < 8; ++e)
+            if (c + e < n) t[e] = row[c + e];
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = (float)t[e];

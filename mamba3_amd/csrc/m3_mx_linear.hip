@@ -191,7 +191,10 @@ __global__ __launch_bounds__(kMlWaves * 64) void mx_linear_few_kernel(MxLinearAr
 // the kernel above on the quantised rows, bit for bit. In front of the rounding may stand the norm (a wave takes a row as
 // m3_add_norm.hip's does: the same sums) or silu(gate) * up.
 constexpr int kMlRawRows = 16;
-constexpr int kMlRawBytes = 32768;  // of quantised elements (with more, quantising in every block takes longer than the launch)
+// The work that is worth a launch less when every block does it (bf16, us in a graph, one launch against two): quantising
+// 8 x 1536 elements 4.9 against 5.6, 8 x 2048 6.2 against 6.1, 16 x 1536 7.3 against 5.8; gating 4 x 1536 5.5 against 6.3,
+// 4 x 2048 7.0 against 6.8; a norm of 4 rows, one a wave, of 768 5.2 against 5.6, of 8 rows 6.7 against 5.8.
+constexpr int kMlRawElements = 16384, kMlGatedElements = 6144, kMlNormRows = kMlWaves;
 constexpr int kMlNormPieces = 4;    // of 512 columns: a wave's row
 enum { kAsIs, kNormed, kGated };
 template <typename T, int kPre, int FN, typename TO>
@@ -219,11 +222,12 @@ __global__ __launch_bounds__(kMlWaves * 64) void mx_linear_raw_kernel(MxLinearAr
     if constexpr (kPre == kNormed) {
         float nw[kMlNormPieces][8], t[kMlNormPieces][8];
 #pragma unroll
-        for (int p = 0; p < kMlNormPieces; ++p) load8(reinterpret_cast<const T*>(before.norm), (lane + p * 64) * 8, k, nw[p]);
-        for (int row = wave; row < a.M; row += kMlWaves) {
+        for (int p = 0; p < kMlNormPieces; ++p) {
+            load8(reinterpret_cast<const T*>(a.x) + (int64_t)(wave < a.M ? wave : 0) * k, (lane + p * 64) * 8, k, t[p]);
+            load8(reinterpret_cast<const T*>(before.norm), (lane + p * 64) * 8, k, nw[p]);
+        }
+        if (const int row = wave; row < a.M) {
             float ss = 0.f;
-#pragma unroll
-            for (int p = 0; p < kMlNormPieces; ++p) load8(reinterpret_cast<const T*>(a.x) + (int64_t)row * k, (lane + p * 64) * 8, k, t[p]);
 #pragma unroll
             for (int p = 0; p < kMlNormPieces; ++p)
 #pragma unroll
@@ -700,9 +704,9 @@ static MxLinearArgs linear_args(const void* x, const void* xs, const void* w, co
     return MxLinearArgs{b(x), b(xs), b(w), b(ws), res, out, scale, m, n, (int)(mx_padded(k) / kMxStep)};
 }
 bool mx_linear_takes_tensor(int64_t m, int64_t n, int64_t k, int x_dtype, int out_dtype, int before) {
-    if (m > kMlRawRows || m * mx_padded(k) > kMlRawBytes) return false;
+    if (m > kMlRawRows || m * mx_padded(k) > (before == kGated ? kMlGatedElements : kMlRawElements)) return false;
     if (before != kAsIs && x_dtype != out_dtype) return false;
-    if (before == kNormed && k > kMlNormPieces * 512) return false;
+    if (before == kNormed && (m > kMlNormRows || k > kMlNormPieces * 512)) return false;
     const MxLinearArgs a = linear_args(nullptr, nullptr, nullptr, nullptr, nullptr, 1.f, nullptr, (int)m, (int)n, (int)k);
     return out_dtype != M3_DTYPE_BF16 || !takes_tiles(a);
 }
