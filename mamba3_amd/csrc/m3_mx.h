@@ -142,8 +142,7 @@ __device__ __forceinline__ void mx_unpack8(u32x2 w, float (&v)[8]) {
 // Eight elements of a row from column c on, those at or past `n` as zero. Whole eights are one or two
 // 16-byte reads at the element type's alignment.
 template <typename T>
-__device__ __forceinline__ void load8(const T* row, int c, int n, float (&v)[8]) {
-    T t[8];
+__device__ __forceinline__ void read8(const T* row, int c, int n, T (&t)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) t[e] = (T)0.f;
     if (c + 8 <= n) {
@@ -153,6 +152,12 @@ __device__ __forceinline__ void load8(const T* row, int c, int n, float (&v)[8])
         for (int e = 0; e < 8; ++e)
             if (c + e < n) t[e] = row[c + e];
     }
+}
+// ... as fp32.
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, int c, int n, float (&v)[8]) {
+    T t[8];
+    read8(row, c, n, t);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = (float)t[e];
 }

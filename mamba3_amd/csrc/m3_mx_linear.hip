@@ -100,10 +100,11 @@ __device__ __forceinline__ void mx_out4(const MxLinearArgs& a, int m, int n, f32
     }
 }
 
-// Few rows: a block takes 16 FM rows and 16 FN columns, its four waves every fourth step of k, straight from memory to
-// registers; their sums meet in LDS. Bound by the latency of its few reads, and by the weights' read. Reading two steps
-// ahead, and eight waves a block, gained nothing (4 x 768 x 3696 in a graph 2.6 us; 3.0 and 2.7).
-constexpr int kMlWaves = 4;
+// Few rows: a block takes 16 FM rows and 16 FN columns, its kW waves every kW-th step of k, straight from memory to
+// registers; their sums meet in LDS. Bound by the latency of its few reads, and by the weights' read. Up to 16 rows eight waves,
+// or 16 where a row has 4096 columns or more and the block 16 (few_waves): weights that come from HBM, as a model's do,
+// are then on their way at once (1 x 768 x 3696 2.8 us in a graph, 3.2 with four waves; 1 x 5504 x 2048 5.0, 5.7 with eight, 8.2 with
+// four; 1 x 2048 x 8800 7.8, 6.9 with four). More rows hold more sums: four waves.
 
 // Adds w x^T of one step of k.
 template <int FA, int FM, int FN, bool kExact>
@@ -134,26 +135,26 @@ __device__ __forceinline__ void few_step(const MxFrag<kE2m1> (&w)[FN], const MxF
     }
 }
 // The waves' sums and their store.
-template <int FM, int FN, typename TO>
-__device__ __forceinline__ void few_store(const MxLinearArgs& a, f32x4 (&part)[kMlWaves][FM * FN][64], const f32x4 (&acc)[FM][FN], int m0, int n0, bool whole) {
+template <int kW, int FM, int FN, typename TO>
+__device__ __forceinline__ void few_store(const MxLinearArgs& a, f32x4* part, const f32x4 (&acc)[FM][FN], int m0, int n0, bool whole) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) part[wave][i * FN + j][lane] = acc[i][j];
+        for (int j = 0; j < FN; ++j) part[(wave * FM * FN + i * FN + j) * 64 + lane] = acc[i][j];
     __syncthreads();
-    for (int f = wave; f < FM * FN; f += kMlWaves) {
-        f32x4 v = part[0][f][lane];
+    for (int f = wave; f < FM * FN; f += kW) {
+        f32x4 v = part[f * 64 + lane];
 #pragma unroll
-        for (int q = 1; q < kMlWaves; ++q) v += part[q][f][lane];
+        for (int q = 1; q < kW; ++q) v += part[(q * FM * FN + f) * 64 + lane];
         mx_out4<TO>(a, m0 + f / FN * 16 + (lane & 15), n0 + f % FN * 16 + (lane >> 4) * 4, v, whole);
     }
 }
 
-template <int FA, int FM, int FN, typename TO>
-__global__ __launch_bounds__(kMlWaves * 64) void mx_linear_few_kernel(MxLinearArgs a, int tiles_n, bool whole) {
+template <int kW, int FA, int FM, int FN, typename TO>
+__global__ __launch_bounds__(kW * 64) void mx_linear_few_kernel(MxLinearArgs a, int tiles_n, bool whole) {
     constexpr bool kExact = sizeof(TO) == 4;
-    __shared__ f32x4 part[kMlWaves][FM * FN][64];
+    extern __shared__ __align__(16) char mx_smem[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
     const int tm = (int)blockIdx.x / tiles_n, tn = (int)blockIdx.x - tm * tiles_n;
     const int m0 = tm * 16 * FM, n0 = tn * 16 * FN;
@@ -174,7 +175,7 @@ __global__ __launch_bounds__(kMlWaves * 64) void mx_linear_few_kernel(MxLinearAr
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int step = wave; step < a.steps; step += kMlWaves) {
+    for (int step = wave; step < a.steps; step += kW) {
         MxFrag<FA> x[FM];
         MxFrag<kE2m1> w[FN];
 #pragma unroll
@@ -183,7 +184,7 @@ __global__ __launch_bounds__(kMlWaves * 64) void mx_linear_few_kernel(MxLinearAr
         for (int i = 0; i < FM; ++i) x[i].template load<kExact>(xp[i], xsp[i], step, g);
         few_step<FA, FM, FN, kExact>(w, x, acc);
     }
-    few_store<FM, FN, TO>(a, part, acc, m0, n0, whole);
+    few_store<kW, FM, FN, TO>(a, reinterpret_cast<f32x4*>(mx_smem), acc, m0, n0, whole);
 }
 
 // The same for at most 16 rows of a tensor, which each block quantises to e4m3 into LDS first: one launch less, and the
@@ -192,68 +193,80 @@ __global__ __launch_bounds__(kMlWaves * 64) void mx_linear_few_kernel(MxLinearAr
 // m3_add_norm.hip's does: the same sums) or silu(gate) * up.
 constexpr int kMlRawRows = 16;
 // The work that is worth a launch less when every block does it (bf16, us in a graph, one launch against two): quantising
-// 8 x 1536 elements 4.9 against 5.6, 8 x 2048 6.2 against 6.1, 16 x 1536 7.3 against 5.8; gating 4 x 1536 5.5 against 6.3,
-// 4 x 2048 7.0 against 6.8; a norm of 4 rows, one a wave, of 768 5.2 against 5.6, of 8 rows 6.7 against 5.8.
-constexpr int kMlRawElements = 16384, kMlGatedElements = 6144, kMlNormRows = kMlWaves;
+// 8 x 2112 elements 5.0 against 5.6, 16 x 1536 6.2 against 5.8; gating 4 x 2112 6.1 against 6.5, 8 x 1536 7.0 against 6.5; a norm
+// of 8 rows, one a wave, of 768 4.4 against 5.7, of 2048 6.3 against 8.6.
+constexpr int kMlRawElements = 20480, kMlGatedElements = 10240, kMlNormRows = 8;
 constexpr int kMlNormPieces = 4;    // of 512 columns: a wave's row
 enum { kAsIs, kNormed, kGated };
-template <typename T, int kPre, int FN, typename TO>
-__global__ __launch_bounds__(kMlWaves * 64) void mx_linear_raw_kernel(MxLinearArgs a, MxBefore before, int k, bool whole) {
+template <int kW, typename T, int kPre, int FN, typename TO>
+__global__ __launch_bounds__(kW * 64) void mx_linear_raw_kernel(MxLinearArgs a, MxBefore before, int k, bool whole) {
     constexpr bool kExact = sizeof(TO) == 4;
-    extern __shared__ __align__(16) char mx_smem[];  // [M][kp] elements, [M][kp / 32] scales
-    __shared__ f32x4 part[kMlWaves][FN][64];
+    extern __shared__ __align__(16) char mx_smem[];  // [M][kp] elements, [M][kp / 32] scales; then the waves' sums
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
     const int n0 = (int)blockIdx.x * 16 * FN, kp = a.steps * kMxStep;
     const int64_t wb = (int64_t)a.steps * 64, sb = (int64_t)a.steps * 4;
     const uint8_t *wp[FN], *wsp[FN];
     MxFrag<kE2m1> w[FN];
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-        const int n = n0 + j * 16 + r < a.N ? n0 + j * 16 + r : a.N - 1;
-        wp[j] = a.w + n * wb, wsp[j] = a.ws + n * sb;
-        w[j].template load<kExact>(wp[j], wsp[j], wave < a.steps ? wave : a.steps - 1, g);
-    }
     uint8_t* xs = reinterpret_cast<uint8_t*>(mx_smem) + a.M * kp;
     const int units = kp / 8;
     auto put = [&](float (&v)[8], int row, int unit) __attribute__((always_inline)) {
         const int at = (unit >> 1 ^ (row & 7)) * 2 + (unit & 1);  // its 16-byte piece
         mx_store8_at<kE4m3>(v, reinterpret_cast<uint8_t*>(mx_smem) + row * kp + at * 8, xs + row * (kp / 32) + (unit >> 2), (unit & 3) == 0);
     };
+    // the weights' first step, asked for behind x's first elements: memory answers in order, and these are nearer
+    auto ask = [&]() __attribute__((always_inline)) {
+        M3_FENCE();
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            const int n = n0 + j * 16 + r < a.N ? n0 + j * 16 + r : a.N - 1;
+            wp[j] = a.w + n * wb, wsp[j] = a.ws + n * sb;
+            w[j].template load<kExact>(wp[j], wsp[j], wave < a.steps ? wave : a.steps - 1, g);
+        }
+        M3_FENCE();
+    };
     if constexpr (kPre == kNormed) {
-        float nw[kMlNormPieces][8], t[kMlNormPieces][8];
+        T nw[kMlNormPieces][8], tt[kMlNormPieces][8];
 #pragma unroll
         for (int p = 0; p < kMlNormPieces; ++p) {
-            load8(reinterpret_cast<const T*>(a.x) + (int64_t)(wave < a.M ? wave : 0) * k, (lane + p * 64) * 8, k, t[p]);
-            load8(reinterpret_cast<const T*>(before.norm), (lane + p * 64) * 8, k, nw[p]);
+            read8(reinterpret_cast<const T*>(a.x) + (int64_t)(wave < a.M ? wave : 0) * k, (lane + p * 64) * 8, k, tt[p]);
+            read8(reinterpret_cast<const T*>(before.norm), (lane + p * 64) * 8, k, nw[p]);
         }
+        ask();
         if (const int row = wave; row < a.M) {
-            float ss = 0.f;
+            float t[kMlNormPieces][8], ss = 0.f;
 #pragma unroll
             for (int p = 0; p < kMlNormPieces; ++p)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) ss = fmaf(t[p][e], t[p][e], ss);
+                for (int e = 0; e < 8; ++e) t[p][e] = (float)tt[p][e], ss = fmaf(t[p][e], t[p][e], ss);
             const float rs = inv_sqrt((float)(wave_sum_f64((double)ss) / k + (double)before.eps));
 #pragma unroll
             for (int p = 0; p < kMlNormPieces; ++p) {
                 if (lane + p * 64 >= units) continue;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) t[p][e] = t[p][e] * rs * nw[p][e];
+                for (int e = 0; e < 8; ++e) t[p][e] = t[p][e] * rs * (float)nw[p][e];
                 put(t[p], row, lane + p * 64);
             }
         }
     } else {
-        for (int i = threadIdx.x; i < a.M * units; i += kMlWaves * 64) {  // whole groups of four: units come in sixteens
+        // whole groups of four: units come in sixteens
+        constexpr int kHalves = kPre == kGated ? 2 : 1;
+        const int all = a.M * units;
+        T v[8], u[8];
+        auto read = [&](int i) __attribute__((always_inline)) {
             const int row = i / units, unit = i - row * units;
-            const T* x = reinterpret_cast<const T*>(a.x) + (int64_t)row * k * (kPre == kGated ? 2 : 1);
-            float v[8];
-            load8(x, unit * 8, k, v);
-            if constexpr (kPre == kGated) {
-                float u[8];
-                load8(x + k, unit * 8, k, u);
+            const T* x = reinterpret_cast<const T*>(a.x) + (int64_t)row * k * kHalves;
+            read8(x, unit * 8, k, v);
+            if constexpr (kPre == kGated) read8(x + k, unit * 8, k, u);
+        };
+        if ((int)threadIdx.x < all) read(threadIdx.x);
+        ask();
+        for (int i = threadIdx.x; i < all; i += kW * 64) {
+            const int row = i / units, unit = i - row * units;
+            float f[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = silu_any(v[e]) * u[e];
-            }
-            put(v, row, unit);
+            for (int e = 0; e < 8; ++e) f[e] = kPre == kGated ? silu_any((float)v[e]) * (float)u[e] : (float)v[e];
+            if (i + kW * 64 < all) read(i + kW * 64);
+            put(f, row, unit);
         }
     }
     __syncthreads();
@@ -263,7 +276,7 @@ __global__ __launch_bounds__(kMlWaves * 64) void mx_linear_raw_kernel(MxLinearAr
     const int m = r < a.M ? r : a.M - 1;
     const char* xr = mx_smem + m * kp;
     const uint8_t* xsr = xs + m * (kp / 32);
-    for (int step = wave; step < a.steps; step += kMlWaves) {
+    for (int step = wave; step < a.steps; step += kW) {
         if (step != wave) {
 #pragma unroll
             for (int j = 0; j < FN; ++j) w[j].template load<kExact>(wp[j], wsp[j], step, g);
@@ -275,7 +288,8 @@ __global__ __launch_bounds__(kMlWaves * 64) void mx_linear_raw_kernel(MxLinearAr
         x[0].s = xsr[step * 4 + g];
         few_step<kE4m3, 1, FN, kExact>(w, x, acc);
     }
-    few_store<1, FN, TO>(a, part, acc, 0, n0, whole);
+    __syncthreads();  // the rows have been read
+    few_store<kW, 1, FN, TO>(a, reinterpret_cast<f32x4*>(mx_smem), acc, 0, n0, whole);
 }
 
 // Rows of the result are whole pieces of four.
@@ -284,11 +298,23 @@ static bool out4(const MxLinearArgs& a) {
     const size_t piece = 4 * sizeof(TO);
     return a.N % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % piece == 0 && (!a.res || reinterpret_cast<uintptr_t>(a.res) % piece == 0);
 }
+// Waves of a block (the measurements: above).
+template <int FM, int FN, typename F>
+static void few_waves(const MxLinearArgs& a, F launch) {
+    if constexpr (FM == 1 && FN == 1) {
+        if (a.steps >= 32) return launch(std::integral_constant<int, 16>{});
+    }
+    launch(std::integral_constant<int, FM == 1 ? 8 : 4>{});
+}
 template <int FA, int FM, int FN, typename TO>
 static int few_t(const MxLinearArgs& a, hipStream_t stream) {
     const int64_t tn = (a.N + 16 * FN - 1) / (16 * FN), tm = (a.M + 16 * FM - 1) / (16 * FM);
     if (tn * tm > 0x7fffffff) return M3_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((mx_linear_few_kernel<FA, FM, FN, TO>), dim3((unsigned)(tn * tm)), dim3(kMlWaves * 64), 0, stream, a, (int)tn, out4<TO>(a));
+    few_waves<FM, FN>(a, [&](auto w) {
+        constexpr int kW = decltype(w)::value;
+        hipLaunchKernelGGL((mx_linear_few_kernel<kW, FA, FM, FN, TO>), dim3((unsigned)(tn * tm)), dim3(kW * 64), kW * FM * FN * 1024, stream, a, (int)tn,
+                           out4<TO>(a));
+    });
     return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH;
 }
 // Columns of a block: the fewest with which at most 256 blocks (one a CU) cover the result, since every block reads its rows
@@ -306,9 +332,12 @@ static int few_m(const MxLinearArgs& a, hipStream_t stream) {
 }
 template <typename T, int kPre, int FN, typename TO>
 static int raw_t(const MxLinearArgs& a, const MxBefore& before, int k, hipStream_t stream) {
-    const int lds = a.M * a.steps * (kMxStep + 4);
-    hipLaunchKernelGGL((mx_linear_raw_kernel<T, kPre, FN, TO>), dim3((unsigned)((a.N + 16 * FN - 1) / (16 * FN))), dim3(kMlWaves * 64), lds, stream, a, before,
-                       k, out4<TO>(a));
+    few_waves<1, FN>(a, [&](auto w) {
+        constexpr int kW = decltype(w)::value;
+        const int lds = std::max(a.M * a.steps * (kMxStep + 4), kW * FN * 1024);
+        hipLaunchKernelGGL((mx_linear_raw_kernel<kW, T, kPre, FN, TO>), dim3((unsigned)((a.N + 16 * FN - 1) / (16 * FN))), dim3(kW * 64), lds, stream, a, before,
+                           k, out4<TO>(a));
+    });
     return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH;
 }
 template <typename T, int kPre, typename TO>
