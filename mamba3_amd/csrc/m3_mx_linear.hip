@@ -301,10 +301,11 @@ static bool out4(const MxLinearArgs& a) {
 // Waves of a block (the measurements: above).
 template <int FM, int FN, typename F>
 static void few_waves(const MxLinearArgs& a, F launch) {
-    if constexpr (FM == 1 && FN == 1) {
-        if (a.steps >= 32) return launch(std::integral_constant<int, 16>{});
+    // at most 64 KB of sums
+    if constexpr (FM * FN <= 4) {
+        if (FN == 1 && a.steps >= 32) return launch(std::integral_constant<int, 16>{});
     }
-    launch(std::integral_constant<int, FM == 1 ? 8 : 4>{});
+    launch(std::integral_constant<int, FM * FN <= 8 ? 8 : 4>{});
 }
 template <int FA, int FM, int FN, typename TO>
 static int few_t(const MxLinearArgs& a, hipStream_t stream) {
