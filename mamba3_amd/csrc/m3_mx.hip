@@ -36,10 +36,7 @@ __global__ __launch_bounds__(kMxThreads) void mx_quantize_kernel(const T* __rest
 #pragma unroll
     for (int i = 0; i < kMxUnits; ++i) {
         if (at + i * kMxThreads >= units) continue;  // whole blocks of 32: units of a row come in sixteens
-        if constexpr (kGated) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] = silu_any(v[i][e]) * u[i][e];
-        }
+        if constexpr (kGated) silu_mul8(v[i], u[i]);
         mx_store8<F>(v[i], data + (int64_t)row[i] * (F == kE4m3 ? kp : kp / 2), scales + (int64_t)row[i] * (kp / 32), unit[i]);
     }
 }

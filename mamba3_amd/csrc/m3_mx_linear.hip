@@ -262,10 +262,14 @@ __global__ __launch_bounds__(kW * 64) void mx_linear_raw_kernel(MxLinearArgs a, 
         ask();
         for (int i = threadIdx.x; i < all; i += kW * 64) {
             const int row = i / units, unit = i - row * units;
-            float f[8];
+            float f[8], h[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = kPre == kGated ? silu_any((float)v[e]) * (float)u[e] : (float)v[e];
+            for (int e = 0; e < 8; ++e) {
+                f[e] = (float)v[e];
+                if constexpr (kPre == kGated) h[e] = (float)u[e];
+            }
             if (i + kW * 64 < all) read(i + kW * 64);
+            if constexpr (kPre == kGated) silu_mul8(f, h);
             put(f, row, unit);
         }
     }
@@ -723,8 +727,11 @@ static int linear_t(const MxLinearArgs& a, hipStream_t stream) {
             return large >= 192 && a.steps >= 12 && a.M > 128 ? tile_t<MxTile<FA, 256, 256, 2, 4, 2, 32>>(a, stream) : tile_t<MxTile<FA, 128, 128, 2, 2, 2, 32>>(a, stream);
         }
     }
-    if (a.M <= 16) return few_m<FA, 1, TO>(a, stream);
-    if (a.M <= 32) return few_m<FA, 2, TO>(a, stream);
+    // rows of a block: the fewest with which 256 blocks of 16 columns do (64 x 2112 x 768 3.6, 4.7 and 7.1 us with 16, 32 and 64,
+    // 32 x 5504 x 2048 6.1 and 8.6 with 16 and 32), and not 64 for 32
+    const int64_t tn = (a.N + 15) / 16;
+    if (a.M <= 16 || (a.M + 15) / 16 * tn <= 256) return few_m<FA, 1, TO>(a, stream);
+    if (a.M <= 32 || (a.M + 31) / 32 * tn <= 256) return few_m<FA, 2, TO>(a, stream);
     return few_m<FA, 4, TO>(a, stream);
 }
 

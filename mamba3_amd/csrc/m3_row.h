@@ -31,10 +31,34 @@ __device__ __forceinline__ float inv_sqrt(float m) {
     return fabsf(e) <= 1.f ? fmaf(0.5f * r, e, r) : r;
 }
 
-// silu without the overflow of exp(-g): e = exp(-|g|) is at most 1.
-__device__ __forceinline__ float silu_any(float g) {
-    const float e = expf(-fabsf(g));
-    return (g < 0.f ? g * e : g) / (1.f + e);
+// v = silu(v) u. With e = exp(-|g|), at most 1: silu = (g < 0 ? g e : g) / (1 + e), which does not overflow. For |g| < 80
+// e comes from the hardware's power of two, with the rounding of its argument put right, and 1 / (1 + e) from its reciprocal
+// (about 2 units in the last place together); beyond, where e nears the smallest numbers, from the library. With expf and a
+// division throughout, gating 8192 x 2112 took 26 us instead of 20.
+__device__ __forceinline__ void silu_mul8(float (&v)[8], const float (&u)[8]) {
+    float most = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
+    bool near = most < 80.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) near &= v[e] == v[e];
+    if (near) {
+        constexpr float kHi = 1.44269502f, kLo = 1.92596299e-8f, kLn2 = 0.693147182f;  // log2 e = kHi + kLo
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float g = v[i], a = -fabsf(g), x = a * kHi;
+            const float rest = fmaf(a, kLo, fmaf(a, kHi, -x));
+            float e = __builtin_amdgcn_exp2f(x);
+            e = fmaf(e * kLn2, rest, e);
+            v[i] = (g < 0.f ? g * e : g) * __builtin_amdgcn_rcpf(1.f + e) * u[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float g = v[i], e = expf(-fabsf(g));
+            v[i] = (g < 0.f ? g * e : g) / (1.f + e) * u[i];
+        }
+    }
 }
 
 }  // namespace m3
