@@ -161,6 +161,25 @@ __device__ __forceinline__ void load8(const T* row, int c, int n, float (&v)[8])
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = (float)t[e];
 }
+// bf16 as it lies in memory, for values that wait in registers.
+__device__ __forceinline__ u32x4 raw8(const bf16* row, int c, int n) {
+    u32x4 o{0, 0, 0, 0};
+    if (c + 8 <= n) {
+        __builtin_memcpy(&o, row + c, 16);
+    } else if (c < n) {
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e / 2] |= c + e < n ? (unsigned)p[c + e] << e % 2 * 16 : 0u;
+    }
+    return o;
+}
+__device__ __forceinline__ void values8(const u32x4& r, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const unsigned w = r[e / 2];
+        v[e] = __builtin_bit_cast(float, e % 2 ? w & 0xffff0000u : w << 16);
+    }
+}
 template <typename T>
 __device__ __forceinline__ void store8(T* row, int c, int n, const float (&v)[8]) {
     T t[8];
