@@ -12,12 +12,14 @@
 // until it fits.
 // With q = 64 (max z - z) / T in 64 bits, a token's mass is exp(-b / 64) exp(-r / 64), b the bin and r < 1: the bins add up
 // exp(-r / 64), four terms of its series to 1e-11, as whole numbers of 2^-45 or so, so that sums do not depend on their
-// order; exp(-b / 64) comes in once a bin. (An exponential for each token took three times as long.) What lies past the last bin
-// but one, below exp(-32) of the likeliest, is counted but has no mass. A border is missed with a probability of about
-// 1e-10 a row, as with 64-bit sums over sorted probabilities.
-// Bound by the reads and the bins' atomics for large batches (256 rows of 128000 fp32 logits, a setting for each row: 78 us, where one
-// read of them takes 23), by the chain of passes and barriers for few (4 rows of 32000: 23-26 us, of which greedy choice and
-// launch take 6). 16 waves a block: with 8, which leaves the compiler more registers, 97 us and the same 23-26.
+// order; exp(-b / 64), of two table values, comes in once a bin. (An exponential for each token took three times as long.) What lies
+// past the last bin but one, below exp(-32) of the likeliest, is counted but has no mass. A border is missed with a probability of
+// about 1e-10 a row, as with 64-bit sums over sorted probabilities.
+// Bound by the reads and the bins' atomics for large batches (256 rows of 128000 fp32 logits, a setting for each row: 76 us, where one
+// read of them takes 22; a row alone on its CU takes 50-60), by the chain of passes, barriers and first fetches of code for few
+// (4 rows of 32000: 18-20 us, of which greedy choice and launch take 6). After the bins one wave does what is left but
+// gathering and sorting: with all 16 and their barriers, and the library's exponential at each place that needs one, 23-26 us. 16 waves a
+// block: with 8, which leaves the compiler more registers, the large case took 97 us for 78.
 #include <algorithm>
 #include <atomic>
 
@@ -34,6 +36,7 @@ constexpr int kSpWaves = kSpThreads / 64;
 constexpr int kSpBins = 2048;
 constexpr double kSpPerT = 64.0;  // bins of T / 64
 constexpr int kSpList = 1024;
+constexpr int kSpShare = kSpBins / kSpWaves;  // a wave's bins
 constexpr int kSpParts = 1024;  // of a bin's keys
 constexpr int kSpHeld = 112 << 10;  // bytes of a row in LDS
 
@@ -84,11 +87,34 @@ constexpr double kSpWhole = 4503599627370496.0;  // 2^52: what is added to it is
 __device__ __forceinline__ u64 sp_whole(double v) {  // of 0 <= v < 2^52
     return __builtin_bit_cast(u64, v + kSpWhole) & 0x000fffffffffffffull;
 }
-// A token's mass, and that times 2^shift as a whole number (shift <= 51), none past the last bin but one.
-__device__ __forceinline__ double sp_exp(const SampleScale& s, float z) { return exp(s.far(z) * (-1.0 / kSpPerT)); }
-__device__ __forceinline__ u64 sp_mass(const SampleScale& s, float z) {
+// exp(-i) and exp(-i / 64): a bin's mass is a product of two, and a token's that times four terms of exp(-d / 64)'s series for
+// what it lies behind its bin's start (to 1e-11).
+struct SampleTables {
+    double whole[kSpBins / 64], part[64];
+};
+constexpr double sp_exp_of(double x) {  // Taylor's series for |x| <= 1
+    double term = 1.0, sum = 1.0;
+    for (int i = 1; i < 24; ++i) term *= x / i, sum += term;
+    return sum;
+}
+constexpr SampleTables sp_tables() {
+    SampleTables t{};
+    for (int i = 0; i < kSpBins / 64; ++i) t.whole[i] = i == 0 ? 1.0 : t.whole[i - 1] * sp_exp_of(-1.0);
+    for (int i = 0; i < 64; ++i) t.part[i] = sp_exp_of(-i / 64.0);
+    return t;
+}
+__constant__ const SampleTables kSpTables = sp_tables();
+__device__ __forceinline__ double sp_series(double d) {
+    constexpr double c1 = -1.0 / kSpPerT, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4;
+    return fma(fma(fma(fma(c4, d, c3), d, c2), d, c1), d, 1.0);
+}
+__device__ __forceinline__ double sp_bin_mass(const SampleTables& t, int b) { return t.whole[b >> 6] * t.part[b & 63]; }
+// A token's mass times 2^shift as a whole number (shift <= 51), none past the last bin but one.
+__device__ __forceinline__ u64 sp_mass(const SampleTables& t, const SampleScale& s, float z) {
     const double q = s.far(z);
-    return q < (double)(kSpBins - 1) ? sp_whole(ldexp(exp(q * (-1.0 / kSpPerT)), s.shift)) : 0;
+    if (!(q < (double)(kSpBins - 1))) return 0;
+    const int b = (int)q;
+    return sp_whole(ldexp(sp_bin_mass(t, b) * sp_series(q - (double)b), s.shift));
 }
 
 struct SampleRow {
@@ -203,9 +229,28 @@ struct SamplePlace {
     int index;        // -1: not known yet
 };
 
+// What the first wave finds out from the bins.
+struct SamplePlan {
+    static constexpr int kSpans = 3;  // k's; p's and min_p's; the token's
+    int from[kSpans], to[kSpans];     // of bins
+    int skipped[kSpans];              // bins before a span that are in none
+    float lo[kSpans], hi[kSpans];
+    double parts;                     // of the sort, a bin
+    bool by_k, by_p, by_m;
+    int k_bin, m_from, m_to;
+    unsigned some;                    // tokens of the spans (without counts, at least)
+    u64 total, kept, before_m;
+};
+
 // The block's working memory.
 struct SampleShared {
-    u64 mass[kSpBins + 64];  // of the row's bins, and a place for each lane's tokens without mass; then of all bins up to each
+    SampleTables tables;
+    SamplePlan plan;
+    u64 begin_mass[kSpWaves];  // of all bins before a wave's share of them
+    unsigned begin_count[kSpWaves];
+    unsigned tail;
+    // of the row's bins, and a place for each lane's tokens without mass; then of a wave's share of bins up to each
+    u64 mass[kSpBins + 64];
     unsigned count[kSpBins + 64];
     union {
         struct {
@@ -225,7 +270,7 @@ struct SampleShared {
     SamplePlace place;
 };
 
-// Inclusive sums over a wave's lanes, by lane moves.
+// Sums over a wave's lanes, by lane moves.
 template <int kCtrl, int kRows>
 __device__ __forceinline__ unsigned sp_move(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, kRows, 0xf, true); }
 template <int kCtrl, int kRows = 0xf>
@@ -250,17 +295,24 @@ __device__ __forceinline__ unsigned sp_max(unsigned v) {
     }
     return v;
 }
+// Inclusive sums over rows of 16 lanes, and over a wave.
+__device__ __forceinline__ void sp_row_scan(unsigned& c, u64& m) {
+    sp_add<kRowShr + 1>(c, m);
+    sp_add<kRowShr + 2>(c, m);
+    sp_add<kRowShr + 4>(c, m);
+    sp_add<kRowShr + 8>(c, m);
+}
+__device__ __forceinline__ void sp_wave_scan(unsigned& c, u64& m) {
+    sp_row_scan(c, m);
+    sp_add<kRowBcast15, 0xa>(c, m);
+    sp_add<kRowBcast31, 0xc>(c, m);
+}
 // Exclusive sums of c and m over the block's threads, in their order, and all of them.
 __device__ __forceinline__ void sp_scan(SampleShared& s, unsigned& c, u64& m, unsigned& all_c, u64& all_m) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     unsigned ic = c;
     u64 im = m;
-    sp_add<kRowShr + 1>(ic, im);
-    sp_add<kRowShr + 2>(ic, im);
-    sp_add<kRowShr + 4>(ic, im);
-    sp_add<kRowShr + 8>(ic, im);
-    sp_add<kRowBcast15, 0xa>(ic, im);
-    sp_add<kRowBcast31, 0xc>(ic, im);
+    sp_wave_scan(ic, im);
     __syncthreads();
     if (lane == 63) s.wcount[wave] = ic, s.wmass[wave] = im;
     __syncthreads();
@@ -343,6 +395,7 @@ __device__ __forceinline__ void sp_span(SampleShared& s, unsigned& lo, unsigned&
 // Sorts the first n of the list from the largest key (and the lowest index) down: by 1024 parts, and within
 // a part by counting the larger ones; where a part has more than 48 (equal logits), all by exchanges of pairs.
 // place(key): its part, below 1024, not falling as keys fall; with kByKeys parts of the keys' span.
+// (Counting alone, without parts: sp_count_sort.)
 template <bool kByKeys, typename F>
 __device__ __forceinline__ void sp_sort(SampleShared& s, unsigned n, F place) {
     constexpr int kPer = kSpList / kSpThreads;
@@ -422,6 +475,17 @@ __device__ __forceinline__ void sp_sort(SampleShared& s, unsigned n, F place) {
     }
     __syncthreads();
 }
+constexpr unsigned kSpCounted = 256;
+__device__ __forceinline__ void sp_count_sort(SampleShared& s, unsigned n) {  // of at most so many, into s.parted
+    if (threadIdx.x < n) {
+        const u64 mine = s.list[threadIdx.x];
+        unsigned above = 0;
+#pragma unroll 4
+        for (unsigned j = 0; j < n; ++j) above += s.list[j] > mine;
+        s.parted[above] = mine;
+    }
+    __syncthreads();
+}
 // A thread's part of the sorted list: each token's count and mass before it, and the mass up to it.
 struct SampleWalk {
     static constexpr int kPer = kSpList / kSpThreads;
@@ -435,7 +499,7 @@ struct SampleWalk {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const unsigned j = threadIdx.x * kPer + i;
-            m[i] = j < n ? sp_mass(scale, sp_logit((unsigned)(s.list[j] >> 32))) : 0;
+            m[i] = j < n ? sp_mass(s.tables, scale, sp_logit((unsigned)(s.list[j] >> 32))) : 0;
             at += m[i];
         }
         sp_scan(s, tc, at, all_c, all_m);
@@ -447,54 +511,13 @@ struct SampleWalk {
             after[i] = at += m[i];
         }
     }
-    // Of the tokens of whole bins that need not follow each other, by the bins' running sums: a bin's last
-    // token ends where the bin does. (The masses of a bin, added up at once, may differ from its tokens' in the last bits.) The
-    // running sums are lost.
-    __device__ __forceinline__ void start_bins(SampleShared& s, unsigned n_, const SampleScale& scale) {
-        start(s, n_, scale, 0, 0);
-        int bin[kPer], of_before = -1;
-        u64 end[kPer], begin[kPer];
-        unsigned begin_c[kPer];
-        bool first[kPer], last[kPer];
-        auto bin_of = [&](unsigned j) __attribute__((always_inline)) { return sp_bin(scale.far(sp_logit((unsigned)(s.list[j] >> 32)))); };
-        if (threadIdx.x * kPer < n && threadIdx.x > 0) of_before = bin_of(threadIdx.x * kPer - 1);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const unsigned j = threadIdx.x * kPer + i;
-            bin[i] = j < n ? bin_of(j) : -1;
-            first[i] = bin[i] != of_before;
-            of_before = bin[i];
-            const int b = bin[i] > 0 ? bin[i] : 0;
-            end[i] = s.mass[b];
-            begin[i] = b ? s.mass[b - 1] : 0, begin_c[i] = b ? s.count[b - 1] : 0;
-        }
-        const unsigned next = (threadIdx.x + 1) * kPer;
-        const int of_next = next < n ? bin_of(next) : -1;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) last[i] = bin[i] != (i + 1 < kPer ? bin[i + 1 < kPer ? i + 1 : 0] : of_next);
-        __syncthreads();
-        // what to add to the list's own sums in this bin
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if (bin[i] >= 0 && first[i]) s.mass[bin[i]] = begin[i] - before[i], s.count[bin[i]] = begin_c[i] - (threadIdx.x * kPer + i);
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int b = bin[i] > 0 ? bin[i] : 0;
-            const u64 more = s.mass[b];
-            count[i] = s.count[b] + (threadIdx.x * kPer + i);
-            before[i] += more, after[i] += more;
-            if (before[i] > end[i]) before[i] = end[i];
-            if (after[i] > end[i] || last[i]) after[i] = end[i];
-        }
-    }
-    // the token that the goal falls on, in s.place, or with kLast the last where none reaches it (the caller waits)
-    template <bool kLast>
+    // the token that the goal falls on, in s.place, or the last where none reaches it: the masses of a bin, added up at once,
+    // may differ from its tokens' in the last bits (the caller waits)
     __device__ __forceinline__ void find(SampleShared& s, const SampleGoal& goal) const {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const unsigned j = threadIdx.x * kPer + i;
-            if (j < n && !goal.reached(count[i], before[i]) && ((kLast && j + 1 == n) || goal.reached(count[i] + 1, after[i]))) {
+            if (j < n && !goal.reached(count[i], before[i]) && (j + 1 == n || goal.reached(count[i] + 1, after[i]))) {
                 const unsigned key = (unsigned)(s.list[j] >> 32);
                 unsigned less = 0, more = j;  // the first of its ties
                 while (less < more) {
@@ -537,7 +560,7 @@ __device__ __forceinline__ void sp_locate(SampleShared& s, const L& z, const Sam
             sp_sort<true>(s, n, [](unsigned) { return 0u; });
             SampleWalk walk;
             walk.start(s, n, scale, base_c, base_m);
-            walk.find<true>(s, goal);
+            walk.find(s, goal);
             few = false;
             continue;
         }
@@ -555,7 +578,7 @@ __device__ __forceinline__ void sp_locate(SampleShared& s, const L& z, const Sam
         if (klo == khi) {
             // equal logits: which of them, by division
             if (threadIdx.x == 0) {
-                const u64 own = sp_mass(scale, sp_logit(khi));
+                const u64 own = sp_mass(s.tables, scale, sp_logit(khi));
                 int64_t before = 0, with = n;  // not reached with `before` of them, reached with `with`
                 while (with - before > 1) {
                     const int64_t mid = (before + with) / 2;
@@ -574,7 +597,7 @@ __device__ __forceinline__ void sp_locate(SampleShared& s, const L& z, const Sam
             if (x > -INFINITY && sp_in(scale.far(x), bin)) {
                 const int b = (int)((khi - sp_key(x)) >> parts);
                 atomicAdd(&s.scount[b], 1u);
-                atomicAdd(&s.smass[b], sp_mass(scale, x));
+                atomicAdd(&s.smass[b], sp_mass(s.tables, scale, x));
             }
         });
         __syncthreads();
@@ -630,6 +653,8 @@ __global__ __launch_bounds__(kSpThreads) void sample_kernel(SampleArgs a, int he
     const SampleLogits<T> z{reinterpret_cast<u32x4*>(sp_smem), reinterpret_cast<const T*>(a.z) + row * a.vocab, a.vocab, held};
     const SampleRow r = sp_row(a, row);
     for (int b = threadIdx.x; b < kSpBins + 64; b += kSpThreads) s.mass[b] = 0, s.count[b] = 0;
+    if (threadIdx.x < sizeof(SampleTables) / 8) reinterpret_cast<double*>(&s.tables)[threadIdx.x] = reinterpret_cast<const double*>(&kSpTables)[threadIdx.x];
+    if (threadIdx.x == 0) s.tail = s.n = 0;
 
     // the largest logit (NaN is none), for a greedy choice its lowest index
     float top = -INFINITY;
@@ -652,8 +677,17 @@ __global__ __launch_bounds__(kSpThreads) void sample_kernel(SampleArgs a, int he
     }
     if ((threadIdx.x & 63) == 0) s.wmass[threadIdx.x >> 6] = best;
     __syncthreads();
+    static_assert(kSpWaves == 16, "a value for each lane of a row of 16");
+    best = s.wmass[threadIdx.x & 15];
+    if (greedy) {
 #pragma unroll
-    for (int w = 0; w < kSpWaves; ++w) best = s.wmass[w] > best ? s.wmass[w] : best;
+        for (int off = 8; off > 0; off >>= 1) {
+            const u64 o = __shfl_xor(best, off, kWave);
+            best = o > best ? o : best;
+        }
+    } else {
+        best = (u64)sp_max((unsigned)(best >> 32)) << 32;
+    }
     top = sp_logit((unsigned)(best >> 32));
     if (greedy || top == -INFINITY) {
         if (threadIdx.x == 0) {
@@ -685,9 +719,8 @@ __global__ __launch_bounds__(kSpThreads) void sample_kernel(SampleArgs a, int he
     const bool counts = r.k < (int64_t)a.vocab;
     unsigned tail = 0;  // tokens of the last bin, which have no mass
     {
-        // exp(-r / 64) 2^shift: the series' terms, -1 / 64 to the i over i!
         const double unit = ldexp(1.0, a.shift), c1 = unit * (-1.0 / kSpPerT), c2 = c1 * (-1.0 / (2 * kSpPerT)), c3 = c2 * (-1.0 / (3 * kSpPerT)),
-                     c4 = c3 * (-1.0 / (4 * kSpPerT));
+                     c4 = c3 * (-1.0 / (4 * kSpPerT));  // sp_series, times 2^shift
         const int aside = kSpBins + ((int)threadIdx.x & 63);
         auto add = [&](float x, auto counted) __attribute__((always_inline)) {
             // without a branch: what has no mass (NaN, too) goes where nobody looks
@@ -701,42 +734,35 @@ __global__ __launch_bounds__(kSpThreads) void sample_kernel(SampleArgs a, int he
                 tail += !in & (x > -INFINITY);
             }
         };
-        if (counts) z.template each<false>([&](float x, int) __attribute__((always_inline)) { add(x, std::true_type{}); });
-        else z.template each<false>([&](float x, int) __attribute__((always_inline)) { add(x, std::false_type{}); });
+        if (counts) {
+            z.template each<false>([&](float x, int) __attribute__((always_inline)) { add(x, std::true_type{}); });
+            if (tail) atomicAdd(&s.tail, tail);
+        } else z.template each<false>([&](float x, int) __attribute__((always_inline)) { add(x, std::false_type{}); });
     }
     __syncthreads();
-    u64 total;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    SamplePlan& plan = s.plan;
     {
-        // without counts, at least so many tokens are in a bin
-        unsigned all_c;
-        u64 all;
-        if (counts) {
-            u64 none = 0;
-            sp_scan(s, tail, none, all_c, all);
-            if (threadIdx.x == 0) s.count[kSpBins - 1] = all_c;
+        // running sums of each wave's share of bins
+        constexpr int kPer = kSpBins / kSpThreads;
+        unsigned c[kPer], ic = 0;
+        u64 m[kPer], im = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int b = (int)threadIdx.x * kPer + i;
+            const u64 raw = s.mass[b];
+            // without counts, at least so many tokens are in a bin
+            c[i] = ic += !counts ? (unsigned)((raw + ((u64)1 << a.shift) - 1) >> a.shift) : b == kSpBins - 1 ? s.tail : s.count[b];
+            m[i] = im += (u64)((double)raw * sp_bin_mass(s.tables, b) + 0.5);
         }
-        for (int b = threadIdx.x; b < kSpBins; b += kSpThreads) {
-            const u64 m = s.mass[b];
-            if (!counts) s.count[b] = (unsigned)((m + ((u64)1 << a.shift) - 1) >> a.shift);
-            s.mass[b] = (u64)((double)m * exp((double)b * (-1.0 / kSpPerT)) + 0.5);
-        }
-        __syncthreads();
-        sp_run<kSpBins>(s, s.mass, s.count, all_c, total);
+        const unsigned own_c = ic;
+        const u64 own_m = im;
+        sp_wave_scan(ic, im);
+        if (lane == 63) s.wcount[wave] = ic, s.wmass[wave] = im;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) s.count[threadIdx.x * kPer + i] = ic - own_c + c[i], s.mass[threadIdx.x * kPer + i] = im - own_m + m[i];
     }
-    bool by_p = r.p < 1.0;
-    const double min_p = r.m < 1.0 ? r.m : 1.0;
-    // min_p keeps what is nearer than this; rounding of the logarithm matters to tokens that are as near as makes no
-    // difference to a bin, and these are asked for their mass itself
-    const double far_m = r.m > 0.0 ? log(min_p) * -kSpPerT : (double)kSpBins;
-    bool by_m = far_m < (double)(kSpBins - 2);  // what is beyond has no mass
-    auto kept_by_m = [&](float x) __attribute__((always_inline)) {
-        const double q = scale.far(x);
-        return q < far_m - 1e-6 || (q < far_m + 1e-6 && sp_exp(scale, x) >= min_p);
-    };
-
-    // The bins in which the answers lie: the k-th token's, that in which p of the k's mass is reached, the bound of min_p and the
-    // token's. What is known of a mass is that it lies between those of all before its bin and of all up to its end.
-    auto mass_to = [&](int bin) __attribute__((always_inline)) { return bin < 0 ? (u64)0 : s.mass[bin]; };
+    __syncthreads();
     const auto share = [&](u64 of) __attribute__((always_inline)) {  // the token that reaches p is the last; the first stays whatever p is
         const double m = r.p > 0.0 ? r.p * (double)of : 0.0;
         return SampleGoal{kReach, 0, m > 1.0 ? m : 1.0};
@@ -745,66 +771,108 @@ __global__ __launch_bounds__(kSpThreads) void sample_kernel(SampleArgs a, int he
         const double m = u > 0.0 ? u * (double)of : 0.0, most = (double)of * (1.0 - 0x1p-30);
         return SampleGoal{kPass, 0, m < most ? m : most};
     };
-    constexpr int kSpans = 3;
-    int from[kSpans] = {0, 0, 0}, to[kSpans] = {-1, -1, -1};  // of bins: k's; p's and min_p's; the token's
-    const int m_from = by_m ? (int)fmax(far_m - 1e-6, 0.0) : 0, m_to = by_m ? (int)(far_m + 1e-6) : -1;
-    u64 low = total, high = total, kept = total;
-    bool by_k = counts;
-    if (by_k) {
-        const SampleGoal goal{kCount, (u64)r.k, 0.0};
-        sp_find_bins<kSpBins>(s, s.mass, s.count, 0, 0, goal, goal, -1);
-        by_k = s.at >= 0;  // the row has so many tokens
+    // min_p keeps what is nearer than this; rounding of the logarithm matters to tokens that are as near as makes no
+    // difference to a bin, and these are asked for their mass itself
+    const double min_p = r.m < 1.0 ? r.m : 1.0;
+    const double far_m = r.m > 0.0 ? log(min_p) * -kSpPerT : (double)kSpBins;
+    auto kept_by_m = [&](float x) __attribute__((always_inline)) {
+        const double q = scale.far(x);
+        return q < far_m - 1e-6 || (q < far_m + 1e-6 && exp(q * (-1.0 / kSpPerT)) >= min_p);
+    };
+    auto mass_to = [&](int bin) __attribute__((always_inline)) { return bin < 0 ? (u64)0 : s.begin_mass[bin / kSpShare] + s.mass[bin]; };
+    auto count_to = [&](int bin) __attribute__((always_inline)) { return bin < 0 ? 0u : s.begin_count[bin / kSpShare] + s.count[bin]; };
+    if (wave == 0) {
+        // The bins in which the answers lie: the k-th token's, that in which p of the k's mass is reached, the bound of min_p and
+        // the token's. What is known of a mass is that it lies between those of all before its bin and of all up to its end.
+        unsigned ic = s.wcount[lane & 15];
+        u64 im = s.wmass[lane & 15];
+        const unsigned own_c = ic;
+        const u64 own_m = im;
+        sp_row_scan(ic, im);
+        if (lane < kSpWaves) s.begin_mass[lane] = im - own_m, s.begin_count[lane] = ic - own_c;
+        const u64 total = __shfl(im, 15, kWave);
+        __builtin_amdgcn_wave_barrier();
+        // the bin whose end reaches the goal and whose start does not
+        auto find = [&](const SampleGoal& goal, int otherwise) __attribute__((always_inline)) {
+            const u64 shares = __ballot(goal.reached(ic, im)) & 0xffffu;
+            if (!shares) return otherwise;
+            const int first = __builtin_ctzll(shares), at = first * kSpShare + 2 * lane;
+            const u64 bm = s.begin_mass[first];
+            const unsigned bc = s.begin_count[first];
+            const bool r0 = goal.reached((u64)bc + s.count[at], bm + s.mass[at]), r1 = goal.reached((u64)bc + s.count[at + 1], bm + s.mass[at + 1]);
+            const u64 m0 = __ballot(r0), m1 = __ballot(r1);
+            if (!m1) return otherwise;
+            const int l = __builtin_ctzll(m1);
+            return first * kSpShare + 2 * l + ((m0 >> l & 1) ? 0 : 1);
+        };
+        static_assert(kSpShare == 128, "two bins a lane");
+        constexpr int kSpans = SamplePlan::kSpans;
+        int from[kSpans] = {0, 0, 0}, to[kSpans] = {-1, -1, -1};
+        u64 low = total, high = total, kept = total, before_m = 0;
+        int k_bin = 0;
+        bool by_k = counts, by_p = r.p < 1.0, by_m = far_m < (double)(kSpBins - 2);  // what is beyond has no mass
         if (by_k) {
-            from[0] = to[0] = s.at;
-            low = mass_to(s.at - 1), high = mass_to(s.at);
-            if (low == high) by_k = false, to[0] = -1, kept = low;  // whichever it is
+            const int at = find(SampleGoal{kCount, (u64)r.k, 0.0}, -1);
+            by_k = at >= 0;  // the row has so many tokens
+            if (by_k) {
+                from[0] = to[0] = k_bin = at;
+                low = mass_to(at - 1), high = mass_to(at);
+                if (low == high) by_k = false, to[0] = -1, kept = low;  // whichever it is
+            }
         }
-    }
-    if (by_p) {
-        __syncthreads();
-        sp_find_bins<kSpBins>(s, s.mass, s.count, 0, 0, share(low), share(high), kSpBins - 1);
-        from[1] = s.at, to[1] = s.to;
-        low = mass_to(from[1] - 1), high = mass_to(to[1]);
-    }
-    u64 before_m = 0;
-    if (by_m) {
-        before_m = mass_to(m_from - 1);
-        const u64 up_to_m = mass_to(m_to);
-        if (before_m >= high) {  // the others leave less
-            by_m = false;
-        } else if (up_to_m <= low) {  // more, of which min_p leaves a part
-            by_k = by_p = false;
-            from[0] = 0, to[0] = -1, from[1] = m_from, to[1] = m_to;
-            kept = total, low = before_m, high = up_to_m;
-        } else {
-            // side by side with p's, a span holds both
-            from[1] = to[1] < 0 ? m_from : min(from[1], m_from), to[1] = max(to[1], m_to);
-            low = min(low, before_m), high = min(high, up_to_m);
+        if (by_p) {
+            from[1] = find(share(low), kSpBins - 1), to[1] = find(share(high), kSpBins - 1);
+            low = mass_to(from[1] - 1), high = mass_to(to[1]);
+        }
+        const int m_from = by_m ? (int)fmax(far_m - 1e-6, 0.0) : 0, m_to = by_m ? (int)(far_m + 1e-6) : -1;
+        if (by_m) {
+            before_m = mass_to(m_from - 1);
+            const u64 up_to_m = mass_to(m_to);
+            if (before_m >= high) {  // the others leave less
+                by_m = false;
+            } else if (up_to_m <= low) {  // more, of which min_p leaves a part
+                by_k = by_p = false;
+                from[0] = 0, to[0] = -1, from[1] = m_from, to[1] = m_to;
+                kept = total, low = before_m, high = up_to_m;
+            } else {
+                // side by side with p's, a span holds both
+                from[1] = to[1] < 0 ? m_from : min(from[1], m_from), to[1] = max(to[1], m_to);
+                low = min(low, before_m), high = min(high, up_to_m);
+            }
+        }
+        from[2] = find(draw(low), kSpBins - 1), to[2] = find(draw(high), kSpBins - 1);
+        // the spans one after the other: the token's, p's and min_p's, k's
+        int bins = 0;
+        unsigned some = 0;
+#pragma unroll
+        for (int i = kSpans - 1, done = 0; i >= 0; --i) {
+            from[i] = max(from[i], done);
+            const bool is = to[i] >= from[i];
+            if (lane == 0) {
+                plan.from[i] = from[i], plan.to[i] = to[i], plan.skipped[i] = from[i] - bins;
+                plan.lo[i] = !is ? INFINITY : to[i] < kSpBins - 1 ? scale.near((double)(to[i] + 1)) : -INFINITY;
+                plan.hi[i] = !is ? -INFINITY : from[i] > 0 ? scale.beyond((double)from[i]) : INFINITY;
+            }
+            if (is) {
+                bins += to[i] - from[i] + 1, done = to[i] + 1;
+                some += count_to(to[i]) - count_to(from[i] - 1);
+            }
+        }
+        if (lane == 0) {
+            plan.parts = (double)kSpList / (double)bins;
+            plan.k_bin = k_bin;
+            plan.by_k = by_k, plan.by_p = by_p, plan.by_m = by_m, plan.m_from = m_from, plan.m_to = m_to;
+            plan.some = some, plan.total = total, plan.kept = kept, plan.before_m = before_m;
         }
     }
     __syncthreads();
-    sp_find_bins<kSpBins>(s, s.mass, s.count, 0, 0, draw(low), draw(high), kSpBins - 1);
-    from[2] = s.at, to[2] = s.to;
-    // the spans one after the other: the token's, p's and min_p's, k's
-    int skipped[kSpans], bins = 0;  // bins that lie before a span and are in none
-    unsigned some = 0;
-    float lo[kSpans], hi[kSpans];
-#pragma unroll
-    for (int i = kSpans - 1, done = 0; i >= 0; --i) {
-        from[i] = max(from[i], done);
-        skipped[i] = from[i] - bins;
-        lo[i] = INFINITY, hi[i] = -INFINITY;
-        if (to[i] < from[i]) continue;
-        bins += to[i] - from[i] + 1, done = to[i] + 1;
-        some += s.count[to[i]] - (from[i] ? s.count[from[i] - 1] : 0);
-        lo[i] = done < kSpBins ? scale.near((double)done) : -INFINITY;
-        hi[i] = from[i] > 0 ? scale.beyond((double)from[i]) : INFINITY;
-    }
     unsigned n = kSpList + 1;
-    if (some <= (unsigned)kSpList) {
-        __syncthreads();
-        if (threadIdx.x == 0) s.n = 0;
-        __syncthreads();
+    if (plan.some <= (unsigned)kSpList) {
+        constexpr int kSpans = SamplePlan::kSpans;
+        float lo[kSpans], hi[kSpans];
+        int from[kSpans], to[kSpans];
+#pragma unroll
+        for (int i = 0; i < kSpans; ++i) lo[i] = plan.lo[i], hi[i] = plan.hi[i], from[i] = plan.from[i], to[i] = plan.to[i];
         z.template each_in<kSpans>(lo, hi, [&](float x, int v) __attribute__((always_inline)) {
             const int b = sp_bin(scale.far(x));
             bool in = false;
@@ -819,60 +887,115 @@ __global__ __launch_bounds__(kSpThreads) void sample_kernel(SampleArgs a, int he
         n = s.n;
     }
 
+    u64 kept = plan.kept;
     float logit;
     int index;
     if (n <= (unsigned)kSpList) {
-        const double parts = (double)kSpList / (double)bins;
-        sp_sort<false>(s, n, [&](unsigned key) __attribute__((always_inline)) {
-            const double q = scale.far(sp_logit(key));
-            const int b = sp_bin(q);
-            const int less = b <= to[2] ? skipped[2] : b <= to[1] ? skipped[1] : skipped[0];
-            return (unsigned)fmin(fmax((q - (double)less) * parts, 0.0), (double)(kSpList - 1));
-        });
-        SampleWalk walk;
-        walk.start_bins(s, n, scale);
-        if (by_k) {
-            walk.find<false>(s, SampleGoal{kCount, (u64)r.k, 0.0});
-            __syncthreads();
-            kept = s.place.mass + s.place.own;
-            __syncthreads();
+        const u64* list = s.list;
+        u64* after = s.parted;  // the mass up to each token of the list
+        if (n <= kSpCounted) {
+            sp_count_sort(s, n);
+            list = s.parted, after = s.list;
+        } else {
+            // its parts: the spans' bins one after the other, without those between
+            sp_sort<false>(s, n, [&](unsigned key) __attribute__((always_inline)) {
+                const double q = scale.far(sp_logit(key));
+                const int b = sp_bin(q);
+                const int less = b <= plan.to[2] ? plan.skipped[2] : b <= plan.to[1] ? plan.skipped[1] : plan.skipped[0];
+                return (unsigned)fmin(fmax((q - (double)less) * plan.parts, 0.0), (double)(kSpList - 1));
+            });
         }
-        if (by_p) {
-            walk.find<false>(s, share(kept));
-            __syncthreads();
-            kept = s.place.mass + s.place.own;
-            __syncthreads();
-        }
-        if (by_m) {
-            u64 mine = 0, all_m;
-            unsigned none = 0, all_c;
-#pragma unroll
-            for (int i = 0; i < SampleWalk::kPer; ++i) {
-                const unsigned j = threadIdx.x * SampleWalk::kPer + i;
-                if (j >= n) continue;
-                const float x = sp_logit((unsigned)(s.list[j] >> 32));
-                const int b = sp_bin(scale.far(x));
-                if (b >= m_from && b <= m_to && kept_by_m(x)) mine += walk.after[i] - walk.before[i];
+        if (wave != 0) return;
+        // The first wave reads the answers off. A bin's first token starts where the bin does, its last ends where the bin does
+        // (the masses of a bin, added up at once, may differ from its tokens' in the last bits); a lane takes `per`
+        // tokens in a row.
+        const unsigned per = (n + 63) / 64, j0 = lane * per, j1 = min(j0 + per, n);
+        auto far_of = [&](unsigned j) __attribute__((always_inline)) { return scale.far(sp_logit((unsigned)(list[j] >> 32))); };
+        u64 v = 0;
+        bool known = false;  // v is the mass of all before, not only of this lane's
+        int b_before = j0 > 0 && j0 < n ? sp_bin(far_of(j0 - 1)) : -1;
+        {
+            int pb = b_before;
+#pragma unroll 1
+            for (unsigned j = j0; j < j1; ++j) {
+                const int b = sp_bin(far_of(j));
+                const u64 m = sp_mass(s.tables, scale, sp_logit((unsigned)(list[j] >> 32)));
+                if (b != pb) v = mass_to(b - 1), known = true;
+                v += m, pb = b;
+                after[j] = m;
             }
-            sp_scan(s, none, mine, all_c, all_m);
-            kept = min(kept, before_m + all_m);
         }
-        walk.find<false>(s, draw(kept));
-        __syncthreads();
-        logit = sp_logit(s.place.key), index = s.place.index;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const u64 ov = __shfl_up(v, off, kWave);
+            const bool ok = __shfl_up((int)known, off, kWave);
+            if (lane >= off && !known) v += ov, known = ok;
+        }
+        v = __shfl_up(v, 1, kWave);  // up to this lane's first
+        {
+            int pb = b_before, b = j0 < n ? sp_bin(far_of(j0)) : -1;
+#pragma unroll 1
+            for (unsigned j = j0; j < j1; ++j) {
+                const int next = j + 1 < n ? sp_bin(far_of(j + 1)) : -1;
+                if (b != pb) v = mass_to(b - 1);
+                v += after[j];
+                const u64 end = mass_to(b);
+                after[j] = next != b || v > end ? end : v;
+                pb = b, b = next;
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        // the first token that reaches a goal (not a count)
+        auto find = [&](const SampleGoal& goal) __attribute__((always_inline)) {
+            const u64 lanes = __ballot(j0 < n && goal.reached(0, after[j1 - 1]));
+            if (!lanes) return n - 1;
+            const unsigned at = __builtin_ctzll(lanes) * per + lane;
+            const u64 places = __ballot(lane < per && at < n && goal.reached(0, after[at < n ? at : n - 1]));
+            return (unsigned)(at - lane) + (unsigned)__builtin_ctzll(places);
+        };
+        if (plan.by_k) {
+            // it is so many behind its bin's start; the list may lack tokens before that
+            const int bin = plan.k_bin;
+            unsigned nearer = 0;
+#pragma unroll 1
+            for (unsigned j = j0; j < j1; ++j) nearer += sp_bin(far_of(j)) < bin;
+            u64 none = 0;
+            sp_wave_scan(nearer, none);
+            kept = after[min(__shfl(nearer, 63, kWave) + (unsigned)(r.k - 1 - count_to(bin - 1)), n - 1)];
+        }
+        if (plan.by_p) kept = after[find(share(kept))];
+        if (plan.by_m) {
+            int last = -1;
+#pragma unroll 1
+            for (unsigned j = j0; j < j1; ++j) {
+                const float x = sp_logit((unsigned)(list[j] >> 32));
+                const int b = sp_bin(scale.far(x));
+                if (b >= plan.m_from && b <= plan.m_to && kept_by_m(x)) last = (int)j;
+            }
+            last = (int)sp_max((unsigned)(last + 1)) - 1;
+            kept = min(kept, last < 0 ? plan.before_m : after[last]);
+        }
+        const unsigned at = find(draw(kept));
+        logit = sp_logit((unsigned)(list[at] >> 32)), index = (int)~(unsigned)list[at];
     } else {
+        // the running sums of all bins
+        constexpr int kPer = kSpBins / kSpThreads;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) s.count[threadIdx.x * kPer + i] += s.begin_count[wave], s.mass[threadIdx.x * kPer + i] += s.begin_mass[wave];
+        const bool by_k = plan.by_k, by_p = plan.by_p;
         SamplePlace q;
         for (int step = by_k ? 0 : by_p ? 1 : 2; step < 3; step = step == 0 && !by_p ? 2 : step + 1) {
-            if (step == 2 && by_m) {
+            if (step == 2 && plan.by_m) {
                 u64 mine = 0, all_m;
                 unsigned none = 0, all_c;
+                const int m_from = plan.m_from, m_to = plan.m_to;
                 const float least[1] = {scale.near((double)(m_to + 1))}, most[1] = {m_from > 0 ? scale.beyond((double)m_from) : INFINITY};
                 z.template each_in<1>(least, most, [&](float x, int) __attribute__((always_inline)) {
                     const int b = sp_bin(scale.far(x));
-                    if (b >= m_from && b <= m_to && kept_by_m(x)) mine += sp_mass(scale, x);
+                    if (b >= m_from && b <= m_to && kept_by_m(x)) mine += sp_mass(s.tables, scale, x);
                 });
                 sp_scan(s, none, mine, all_c, all_m);
-                kept = min(kept, before_m + all_m);
+                kept = min(kept, plan.before_m + all_m);
             }
             sp_locate(s, z, scale, step == 0 ? SampleGoal{kCount, (u64)r.k, 0.0} : step == 1 ? share(kept) : draw(kept));
             q = s.place;
@@ -884,7 +1007,7 @@ __global__ __launch_bounds__(kSpThreads) void sample_kernel(SampleArgs a, int he
     if (threadIdx.x == 0) {
         a.token[row] = index;
         if (a.logprob)
-            a.logprob[row] = (float)((logit == top ? 0.0 : ((double)logit - (double)top) / r.t) - log(ldexp((double)kept, -a.shift)));
+            a.logprob[row] = (float)(scale.far(logit) * (-1.0 / kSpPerT) - (double)logf((float)ldexp((double)kept, -a.shift)));
     }
 }
 
