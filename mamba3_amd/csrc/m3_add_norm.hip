@@ -8,7 +8,8 @@
 //
 // A row is taken by one wave (to 2048 columns) or by a block's four (to 8192), eight consecutive
 // columns a lane and piece, so that four lanes hold a block of 32; wider rows are read a second time.
-// Squares are added in fp32 within a lane (at most 32 of them) and in fp64 across lanes.
+// Squares are added in fp32 within a lane (at most 32 of them) and in fp64 across lanes; for microscaled results in fp64
+// from eight on, and the product is rounded once (m3_row.h).
 #include <algorithm>
 
 #include "m3_common.h"
@@ -67,6 +68,7 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_kernel(AddNormArgs a) {
             if constexpr (kRes) load8(reinterpret_cast<const T*>(a.res) + base, c, d, r[p]);
         }
         float ss = 0.f;
+        double squares = 0.0;
 #pragma unroll
         for (int p = 0; p < kNp; ++p) {
             if constexpr (kRes) {
@@ -75,10 +77,16 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_kernel(AddNormArgs a) {
                 const int c = (lane + p * kLanes) * 8;
                 if (c < d) store8(reinterpret_cast<T*>(a.total) + base, c, d, t[p]);
             }
+            if constexpr (kF != kSame) {
+                squares = add_squares(squares, t[p]);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss = fmaf(t[p][e], t[p][e], ss);
+                for (int e = 0; e < 8; ++e) ss = fmaf(t[p][e], t[p][e], ss);
+            }
         }
-        const float rs = inv_sqrt((float)(row_sum<kWpr>((double)ss, red) / d + (double)a.eps));
+        const double mean = row_sum<kWpr>(kF != kSame ? squares : (double)ss, red) / d + (double)a.eps;
+        const RowScale r2 = row_scale(mean);
+        const float rs = r2.hi;
         if (a.rstd && lane == 0) a.rstd[row] = rs;
 #pragma unroll
         for (int p = 0; p < kNp; ++p) {
@@ -86,7 +94,7 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_kernel(AddNormArgs a) {
             if (unit >= units) continue;
             float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = t[p][e] * rs * w[p][e];
+            for (int e = 0; e < 8; ++e) v[e] = kF != kSame ? norm_odd<T>(t[p][e], w[p][e], r2) : t[p][e] * rs * w[p][e];
             if constexpr (kF == kSame) store8(reinterpret_cast<T*>(a.y) + base, unit * 8, d, v);
             else mx_store8<kF>(v, a.data + row * (kF == kE4m3 ? a.kp : a.kp / 2), a.scales + row * (a.kp / 32), unit);
         }
@@ -110,18 +118,23 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_wide_kernel(AddNormArgs a
                 for (int e = 0; e < 8; ++e) t[e] = (float)(T)fmaf(a.scale, t[e], r[e]);
                 store8(reinterpret_cast<T*>(a.total) + base, unit * 8, d, t);
             }
+            if constexpr (kF != kSame) {
+                sum = add_squares(sum, t);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss = fmaf(t[e], t[e], ss);
-            sum += (double)ss;
+                for (int e = 0; e < 8; ++e) ss = fmaf(t[e], t[e], ss);
+                sum += (double)ss;
+            }
         }
-        const float rs = inv_sqrt((float)(row_sum<kAnWaves>(sum, red) / d + (double)a.eps));
+        const RowScale r2 = row_scale(row_sum<kAnWaves>(sum, red) / d + (double)a.eps);
+        const float rs = r2.hi;
         if (a.rstd && threadIdx.x == 0) a.rstd[row] = rs;
         for (int unit = threadIdx.x; unit < units; unit += kAnThreads) {
             float t[8], w[8];  // t: what this thread wrote above
             load8(reinterpret_cast<const T*>(kRes ? a.total : a.x) + base, unit * 8, d, t);
             load8(reinterpret_cast<const T*>(a.w), unit * 8, d, w);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) t[e] = t[e] * rs * w[e];
+            for (int e = 0; e < 8; ++e) t[e] = kF != kSame ? norm_odd<T>(t[e], w[e], r2) : t[e] * rs * w[e];
             if constexpr (kF == kSame) store8(reinterpret_cast<T*>(a.y) + base, unit * 8, d, t);
             else mx_store8<kF>(t, a.data + row * (kF == kE4m3 ? a.kp : a.kp / 2), a.scales + row * (a.kp / 32), unit);
         }

@@ -233,17 +233,20 @@ __global__ __launch_bounds__(kW * 64) void mx_linear_raw_kernel(MxLinearArgs a, 
         }
         ask();
         if (const int row = wave; row < a.M) {
-            float t[kMlNormPieces][8], ss = 0.f;
+            float t[kMlNormPieces][8];
+            double squares = 0.0;
 #pragma unroll
-            for (int p = 0; p < kMlNormPieces; ++p)
+            for (int p = 0; p < kMlNormPieces; ++p) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) t[p][e] = (float)tt[p][e], ss = fmaf(t[p][e], t[p][e], ss);
-            const float rs = inv_sqrt((float)(wave_sum_f64((double)ss) / k + (double)before.eps));
+                for (int e = 0; e < 8; ++e) t[p][e] = (float)tt[p][e];
+                squares = add_squares(squares, t[p]);
+            }
+            const RowScale rs = row_scale(wave_sum_f64(squares) / k + (double)before.eps);
 #pragma unroll
             for (int p = 0; p < kMlNormPieces; ++p) {
                 if (lane + p * 64 >= units) continue;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) t[p][e] = t[p][e] * rs * (float)nw[p][e];
+                for (int e = 0; e < 8; ++e) t[p][e] = norm_odd<T>(t[p][e], (float)nw[p][e], rs);
                 put(t[p], row, lane + p * 64);
             }
         }

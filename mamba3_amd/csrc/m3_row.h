@@ -31,6 +31,33 @@ __device__ __forceinline__ float inv_sqrt(float m) {
     return fabsf(e) <= 1.f ? fmaf(0.5f * r, e, r) : r;
 }
 
+// For results that are rounded to 8 bits and fewer: 1 / sqrt(m) in two parts, and t r w as fp32 rounded to odd (to the odd one of
+// its two neighbours where it is none), so that the next rounding falls as the exact product's would. Rounded to nearest,
+// about one e4m3 element in a million would fall on the other side of a tie.
+struct RowScale {
+    float hi, lo;
+};
+__device__ __forceinline__ RowScale row_scale(double m) {
+    const float r = inv_sqrt((float)m);
+    const double e = fma(-m * (double)r, (double)r, 1.0);
+    return RowScale{r, fabs(e) < 1e-3 ? (float)(0.5 * (double)r * e) : 0.f};  // (m of 0, infinity or NaN: hi is the answer)
+}
+template <typename T>
+__device__ __forceinline__ float norm_odd(float t, float w, RowScale r) {
+    const float p = t * w, hi = p * r.hi;
+    float rest = fmaf(p, r.lo, fmaf(p, r.hi, -hi));
+    if constexpr (sizeof(T) == 4) rest = fmaf(fmaf(t, w, -p), r.hi, rest);  // (a product of two bf16 is exact)
+    const unsigned b = __builtin_bit_cast(unsigned, hi), toward = (__builtin_bit_cast(unsigned, rest) ^ b) >> 31;  // 1: toward zero
+    return __builtin_bit_cast(float, fabsf(rest) > 0.f ? (b - toward) | 1u : b);
+}
+// The sum of eight squares added to s. (Their roundings to fp32 average out over a row: about 2^-28 of its sum.)
+__device__ __forceinline__ double add_squares(double s, const float (&t)[8]) {
+    float q = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q = fmaf(t[e], t[e], q);
+    return s + (double)q;
+}
+
 // v = silu(v) u. With e = exp(-|g|), at most 1: silu = (g < 0 ? g e : g) / (1 + e), which does not overflow. For |g| < 80
 // e comes from the hardware's power of two, with the rounding of its argument put right, and 1 / (1 + e) from its reciprocal
 // (about 2 units in the last place together); beyond, where e nears the smallest numbers, from the library. With expf and a
