@@ -61,15 +61,20 @@ def _only_weight(lin: nn.Module) -> bool:
 
 def _mx_copy(owner: nn.Module, name: str, *weights: torch.Tensor) -> MXTensor:
     """The 4-bit copy of the weights, one below the other, that `owner` keeps: made when first asked for and again after one
-    was replaced or changed in place (which their version counters tell). The copy holds on to the weights' memory, so an address
-    is not another weight's as long as it is compared."""
+    was replaced or changed in place (which their version counters tell), into the same memory where it fits, so that graphs
+    captured with the copy go on with the new weights. The copy holds on to the weights' memory, so an address is not another
+    weight's as long as it is compared."""
     key = tuple((w.data_ptr(), 0 if w.is_inference() else w._version, w.dtype, w.device) for w in weights)
     kept = owner.__dict__.get(name)
     if kept is None or kept[0] != key:
         if weights[0].is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a graph is being captured and the 4-bit weights are not there yet: run the model once before")
-        with torch.no_grad():
+        with torch.inference_mode(False), torch.no_grad():  # copies outlive the mode that they are made in
             mx = quantize_mx(weights[0] if len(weights) == 1 else torch.cat(weights))
+            if kept is not None and kept[1].shape == mx.shape and kept[1].device == mx.device:
+                kept[1].data.copy_(mx.data)
+                kept[1].scales.copy_(mx.scales)
+                mx = kept[1]
         # from here on any stream may read them
         torch.cuda.current_stream(mx.device).synchronize()
         kept = owner.__dict__[name] = (key, mx, [w.detach() for w in weights])
@@ -217,6 +222,7 @@ class KulaMambaBlock(nn.Module):
         (KulaMambaLM), so without autograd the first residual add may overwrite it. The
         second add overwrites the first one's output whenever no autograd graph needs it."""
         if self._mx_on():
+            self.ssm._check_sequence(x)
             return self._mx_block(x, self.ssm.ssd_from_proj)[0]
         ckpt = self.gradient_checkpointing and self.training
         nograd = not torch.is_grad_enabled()
@@ -276,7 +282,8 @@ class KulaMambaBlock(nn.Module):
 
     def step(self, x: torch.Tensor, ssm_state: dict):
         if self._mx_on():
-            return self._mx_block(x, lambda proj: self.ssm._step_from_proj(proj, ssm_state))
+            y, state = self._mx_block(self.ssm._check_token(x), lambda proj: self.ssm._step_from_proj(proj, ssm_state))
+            return y.view(x.shape), state
         if self._small_step_usable(x):
             proj = ops.small_linear_fast(x, self.ssm_norm.weight, float(self.ssm_norm.eps),
                                     self.ssm.in_proj.weight, None, 1.0)
@@ -291,6 +298,7 @@ class KulaMambaBlock(nn.Module):
     def prefill(self, x: torch.Tensor, _own_input: bool = False):
         """_own_input as in forward."""
         if self._mx_on():
+            self.ssm._check_sequence(x)
             return self._mx_block(x, lambda proj: self.ssm.ssd_from_proj(proj, return_state=True))
         nograd = not torch.is_grad_enabled()
         y, state = self.ssm._pre_out(self.ssm_norm(x), return_state=True)

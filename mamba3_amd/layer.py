@@ -155,14 +155,27 @@ class KulaMamba(nn.Module):
         return dt_scale.to(device=device, dtype=torch.float32).expand(shape).contiguous()
 
     # ------------------------------------------------------------------ forward paths
-    def _pre_out(self, x: torch.Tensor, dt_scale=None, return_state: bool = False):
-        """in_proj and the SSD core: x (B,T,d_model) -> (out_proj's input (B,T,d_inner),
-        state or None)."""
+    @staticmethod
+    def _check_sequence(x: torch.Tensor) -> None:
         if x.dim() != 3:
             raise ValueError(f"expected (batch, seqlen, d_model), got {tuple(x.shape)}")
         if x.shape[1] <= 0:
             raise ValueError(f"Sequence length must be positive, got {x.shape[1]}")
         _native.require_gpu(x)
+
+    @staticmethod
+    def _check_token(x: torch.Tensor) -> torch.Tensor:
+        """x (B, d_model) or (B, 1, d_model) as (B, d_model)."""
+        rows = x if x.dim() == 2 else x.squeeze(1)
+        if rows.dim() != 2:
+            raise ValueError(f"expected (B, d_model) or (B, 1, d_model), got {tuple(x.shape)}")
+        _native.require_gpu(rows)
+        return rows
+
+    def _pre_out(self, x: torch.Tensor, dt_scale=None, return_state: bool = False):
+        """in_proj and the SSD core: x (B,T,d_model) -> (out_proj's input (B,T,d_inner),
+        state or None)."""
+        self._check_sequence(x)
         # A 3-D input whose batch rows are not adjacent would send the projection down
         # torch's batched bf16 GEMM with a transposed weight view, which returned wrong rows
         # on this GPU; a contiguous input folds to one 2-D GEMM.
@@ -248,10 +261,7 @@ class KulaMamba(nn.Module):
 
     def _step_pre_out(self, hidden_states: torch.Tensor, ssm_state: dict, dt_scale=None):
         """in_proj and the step kernel: (out_proj's input (B, d_inner), new state)."""
-        x_in = hidden_states if hidden_states.dim() == 2 else hidden_states.squeeze(1)
-        if x_in.dim() != 2:
-            raise ValueError(f"expected (B, d_model) or (B, 1, d_model), got {tuple(hidden_states.shape)}")
-        _native.require_gpu(x_in)
+        x_in = self._check_token(hidden_states)
         w = self.in_proj.weight
         if self.in_proj.bias is None and ops.small_proj_usable(x_in, w):
             proj = ops.small_linear_fast(x_in, None, 0.0, w, None, 1.0)

@@ -364,3 +364,80 @@ def test_many_results():
     u = torch.rand(1000, generator=torch.Generator().manual_seed(2)).cuda()
     tokens = sample_tokens(got, u.repeat(70), 1.0, 50, 0.9)
     assert same(tokens[-1000:], sample_tokens(want, u, 1.0, 50, 0.9))
+
+
+# ---------------------------------------------------------------- shapes that a block takes and refuses
+@torch.no_grad()
+def test_block_shapes_quantised():
+    block = small_lm().quantize_mx().layers[0]
+    x = normal((3, 1, 128), 0, torch.bfloat16)
+    state = block.ssm.allocate_inference_state(3)
+    y, after = block.step(x[:, 0], state)
+    y3, after3 = block.step(x, state)
+    assert y3.shape == x.shape and same(y3[:, 0], y) and all(same(after[k], after3[k]) for k in after)
+    for bad in (lambda: block(x[:, 0]), lambda: block.prefill(x[:, 0]), lambda: block(x[:, :0]), lambda: block.step(normal((3, 2, 128), 1, torch.bfloat16), state),
+                lambda: block.step(x[:2], state), lambda: block(x[..., :64])):
+        with pytest.raises(ValueError):
+            bad()
+    wide = normal((3, 2, 9, 128), 2, torch.bfloat16)[:, 0]  # rows of a batch that do not follow each other
+    assert same(block(wide), block(wide.contiguous()))
+
+
+@torch.no_grad()
+def test_prefill_then_steps_quantised_against_the_forward():
+    """The state that a prompt leaves carries the model on: logits of the last tokens, decoded one by one, against those of one
+    forward over all. Both round the same activations to 8 bits, but for those that bf16's roundings of the two orders of summing
+    set apart: an element that falls to the other side of a tie is off by at most 2^-4 of itself, few do."""
+    lm = small_lm(torch.float32).quantize_mx()
+    ids = torch.randint(0, 500, (2, 40), generator=torch.Generator().manual_seed(1)).cuda()
+    want = lm(ids)["logits"]
+    x, states = lm.embedding(ids[:, :32]), []
+    for layer in lm.layers:
+        x, st = layer.prefill(x)
+        states.append(st)
+    assert same(lm._mx_logits(x), want[:, :32]) or (lm._mx_logits(x) - want[:, :32]).norm() < 2 ** -4 * want.norm()
+    for t in range(32, 40):
+        got = lm._next_logits(ids[:, t], states, None)
+        assert ((got - want[:, t]).norm() / want[:, t].norm()).item() < 2 ** -4
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=5), dict(top_p=0.9), dict(min_p=0.01)])
+def test_sample_odd_settings(kw):
+    """Temperatures that a division or an exponential would overflow at, and views with steps."""
+    z = normal((4, 1000), 0, std=3.0)
+    z[:, 17] = 20.0
+    u = torch.tensor([0.0, 0.3, 0.6, 0.999]).cuda()
+    for t in (1e-320, 1e-45, 1e-30, 1e-6):
+        assert same(sample_tokens(z, u, t, **kw), torch.full((4,), 17, device="cuda"))
+    for t in (1e30, float("inf")):
+        tokens, lp = sample_tokens(z, u, t, return_logprob=True, **kw)
+        assert ((tokens >= 0) & (tokens < 1000)).all() and torch.isfinite(lp).all()
+        if not kw:  # all masses are alike: the tokens in the order of their logits, ties of the mass or not
+            order = z.sort(dim=1, descending=True, stable=True).indices
+            assert same(tokens, order.gather(1, (u.double() * 1000).long()[:, None])[:, 0])
+    wide = normal((4, 3, 1000), 1)
+    assert same(sample_tokens(wide[:, 1], u, **kw), sample_tokens(wide[:, 1].contiguous(), u, **kw))
+    assert same(sample_tokens(wide[:, 1], u[1:2].expand(4), **kw), sample_tokens(wide[:, 1], torch.full((4,), 0.3).cuda(), **kw))
+    assert same(sample_tokens(wide, u[:, None].expand(4, 3), **kw), sample_tokens(wide.flatten(0, 1), u.repeat_interleave(3), **kw).view(4, 3))
+
+
+def test_a_captured_graph_follows_the_weights():
+    lm = small_lm().quantize_mx()
+    x = normal((2, 128), 0, torch.bfloat16)
+    with torch.inference_mode():
+        first = lm._mx_logits(x).clone()
+    with torch.no_grad():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = lm._mx_logits(x)
+        graph.replay()
+        assert same(got, first)
+        lm.lm_head.weight.mul_(3.0)
+        want = lm._mx_logits(x)  # makes the copy anew
+        graph.replay()
+        assert same(got, want) and not torch.equal(got, first)
+    with torch.inference_mode():
+        lm.lm_head.weight.mul_(0.5)
+        want = lm._mx_logits(x).clone()
+    with torch.no_grad():
+        assert same(lm._mx_logits(x), want)
