@@ -708,25 +708,34 @@ static int tile_t(const MxLinearArgs& a, hipStream_t stream) {
     if (tm * tn > (1 << 30) || a.N > (1 << 25)) return M3_ERR_UNSUPPORTED;  // 32 rows of results within a descriptor
     static std::atomic<uint64_t> done{0};
     if (!allow_lds(reinterpret_cast<const void*>(&mx_linear_tile_kernel<Tile>), Tile::kLds, done)) return M3_ERR_LAUNCH;
-    const int64_t most = 256 * (Tile::NT >= 512 ? 1 : 2);  // blocks at once
+    const int64_t most = 256 * std::min(2, (160 << 10) / Tile::kLds);  // blocks at once
     hipLaunchKernelGGL((mx_linear_tile_kernel<Tile>), dim3((unsigned)std::min(tm * tn, most)), dim3(Tile::NT), Tile::kLds, stream, a,
                        (int)tm, (int)tn);
     return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH;
 }
-// Which kernel, by the number of 128 x 128 and 256 x 256 tiles (us in a graph, e4m3, few rows' kernel and 128 x 128 tiles):
-// 16 x 2048 x 11008 7.3 and 9.3, x 128000 41 and 29; 32 x 2048 x 11008 9.1 and 9.2, 32 x 768 x 32000 6.6 and 5.9;
-// 64 x 2048 x 11008 12.4 and 9.8, 64 x 768 x 3696 4.4 and 5.6, 256 x 768 x 3696 6.5 and 5.9, 1000 x 768 x 4224 19 and 9.1.
-// 128 x 128 and 256 x 256 tiles: 8192 x 768 x 4224 32 and 37, 8192 x 2112 x 768 19 and 27, 8192 x 5504 x 2048 105 and 76,
-// 16 x 2048 x 128000 29 and 45.
+// Which kernel, by the number of tiles of 128 columns and the steps of k (us in a graph of weights from HBM, e4m3, few
+// rows' kernel and tiles of 64 x 128, which have four steps on their way):
+//   8 rows: 2048 x 128000 41.9 and 38.8, 2048 x 25600 11.8 and 11.5, 1024 x 128000 21.7 and 21.9
+//   16 rows: 2048 x 128000 46.1 and 39.4, 2048 x 25600 12.8 and 11.6, 1536 x 32000 9.9 and 10.1, 768 x 128000 16.6 and 18.3, 2048 x 16000 8.8 and 10.7
+//   32 rows: 2048 x 25600 16.2 and 12.0, 1024 x 32000 9.8 and 8.2, 768 x 32000 7.1 and 7.4, 768 x 128000 22 and 18, 2048 x 16000 9.7 and 10.8
+//   64 rows: 2048 x 11000 14.3 and 11.4, 768 x 11000 7.9 and 6.9, 768 x 7168 5.4 and 6.7
+// and with tiles of 128 x 128 (weights from the caches) 256 x 768 x 3696 6.5 and 5.9, 1000 x 768 x 4224 19 and 9.1. Tiles of 128 x 128 for
+// 64 rows: 2048 x 11000 14.3, 2048 x 128000 45 (42.6). 128 x 128 and 256 x 256 tiles: 8192 x 768 x 4224 32 and 37,
+// 8192 x 2112 x 768 19 and 27, 8192 x 5504 x 2048 105 and 76.
 static bool takes_tiles(const MxLinearArgs& a) {
     const int64_t tiles = (int64_t)((a.M + 127) / 128) * ((a.N + 127) / 128);
-    return tiles >= (a.M <= 16 ? 512 : a.M <= 32 ? 200 : 56);
+    if (a.M > 64) return tiles >= 56;
+    if (a.M > 32) return tiles >= 72;
+    if (a.M > 16) return tiles >= (a.steps >= 8 ? 200 : 512);
+    if (a.M > 8) return tiles >= (a.steps >= 12 ? 200 : 512) && a.steps >= 8;
+    return tiles >= 512 && a.steps >= 16;
 }
 template <int FA, typename TO>
 static int linear_t(const MxLinearArgs& a, hipStream_t stream) {
     if constexpr (sizeof(TO) == 2) {
         if (takes_tiles(a)) {
             const int64_t large = (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256);
+            if (a.M <= 64) return tile_t<MxTile<FA, 64, 128, 1, 2, 4, 32>>(a, stream);
             return large >= 192 && a.steps >= 12 && a.M > 128 ? tile_t<MxTile<FA, 256, 256, 2, 4, 2, 32>>(a, stream) : tile_t<MxTile<FA, 128, 128, 2, 2, 2, 32>>(a, stream);
         }
     }

@@ -532,3 +532,19 @@ def test_sample_follows_the_masses():
     want = share[kept] / share[kept].sum()
     count = torch.bincount(token, minlength=50).double() / n
     assert (count[kept] - want).abs().max() <= 2 / n and abs(count.sum() - count[kept].sum()) == 0
+
+
+@pytest.mark.parametrize("rows,n,k", [(33, 9999, 64), (40, 9304, 300), (50, 9222, 2050), (64, 9217, 129), (12, 25700, 1600), (25, 25704, 1100), (5, 65600, 2048)])
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+def test_mx_linear_few_rows_many_columns(rows, n, k, fmt):
+    x, w = mx_pair(rows, n, k, fmt, 11)
+    a, b = x.dequantize(torch.float32).double(), w.dequantize(torch.float32).double()
+    want, size = a @ b.t(), a.abs() @ b.abs().t()
+    top = lambda v: torch.nn.functional.pad(v.abs(), (0, -k % 128)).unflatten(-1, (-1, 128)).amax(-1)  # noqa: E731
+    step = 2.0 ** -11 * (top(a) @ top(b).t()) if fmt == "e4m3" else 0.0
+    off = step + k * 2.0 ** -24 * size
+    assert ((mamba3_amd.mx_linear(x, w).double() - want).abs() <= half(torch.bfloat16) * want.abs() + off).all()
+    r = normal((rows, n), 3, torch.bfloat16).cuda()
+    want = r.double() - 0.75 * want
+    assert ((mamba3_amd.mx_linear(x, w, r, -0.75).double() - want).abs()
+            <= half(torch.bfloat16) * want.abs() + 0.75 * off + 2.0 ** -22 * (r.abs().double() + 2 * want.abs())).all()
