@@ -523,6 +523,16 @@ int m3_mx_linear(int64_t rows, int32_t n, int32_t k, int32_t x_format, int32_t o
                  void* stream);
 
 /*
+ * The same for fp32 results of many rows (residual and out fp32): both operands are written to the workspace in bf16, which holds
+ * them exactly, and multiplied from there. m3_mx_linear_exact_workspace_size gives its bytes, or 0 where m3_mx_linear is the
+ * faster one; then the call is unsupported.
+ */
+int m3_mx_linear_exact_workspace_size(int64_t rows, int32_t n, int32_t k, size_t* bytes);
+int m3_mx_linear_exact(int64_t rows, int32_t n, int32_t k, int32_t x_format, const void* x_data, const void* x_scales, const void* w_data,
+                       const void* w_scales, const float* residual, float scale, float* out, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/*
  * The same for a tensor x in x_dtype, quantised to e4m3 on the way: the bits of the two calls, in one launch. `before`:
  *   M3_MX_AS_IS   x [rows, k] as m3_mx_quantize takes it
  *   M3_MX_NORMED  x [rows, k] normed with norm_weight [k] and eps as by m3_add_rmsnorm_mx without a residual

@@ -66,6 +66,8 @@ EXPORTED_SYMBOLS = (
     "m3_add_rmsnorm_bwd_workspace_size",
     "m3_add_rmsnorm_bwd",
     "m3_mx_linear",
+    "m3_mx_linear_exact",
+    "m3_mx_linear_exact_workspace_size",
     "m3_mx_linear_takes_tensor",
     "m3_mx_linear_tensor",
     "m3_sample_tokens",
@@ -208,6 +210,8 @@ def _declare(lib: ctypes.CDLL) -> None:
             ("m3_add_rmsnorm_bwd_workspace_size", [_i64, _i32, size_p]),
             ("m3_add_rmsnorm_bwd", [_i64, _i32, _i32] + [_vp] * 5 + [f32] + [_vp] * 4 + [ctypes.c_size_t, _vp]),
             ("m3_mx_linear", [_i64] + [_i32] * 4 + [_vp] * 5 + [f32] + [_vp] * 2),
+            ("m3_mx_linear_exact", [_i64] + [_i32] * 3 + [_vp] * 5 + [f32] + [_vp] * 2 + [ctypes.c_size_t, _vp]),
+            ("m3_mx_linear_exact_workspace_size", [_i64] + [_i32] * 2 + [ctypes.POINTER(ctypes.c_size_t)]),
             ("m3_mx_linear_takes_tensor", [_i64] + [_i32] * 5),
             ("m3_mx_linear_tensor", [_i64] + [_i32] * 5 + [_vp] * 2 + [f32] + [_vp] * 3 + [f32] + [_vp] * 2),
             ("m3_sample_tokens", [_i64, _i32, _i32, _vp, _vp, _vp, ctypes.c_double, _vp, _i64, _vp, ctypes.c_double, _vp,
@@ -635,9 +639,21 @@ def add_rmsnorm_bwd(total, weight, rstd, dtotal, dy, scale: float, dx, dresidual
                                    stream_of(total)), "m3_add_rmsnorm_bwd")
 
 
+@functools.lru_cache(maxsize=1024)
+def _mx_exact_bytes(rows: int, n: int, k: int) -> int:
+    return _bytes_of("m3_mx_linear_exact_workspace_size", rows, n, k)
+
+
 def mx_linear(x_data, x_scales, x_format: str, w_data, w_scales, k: int, residual, scale: float, out) -> None:
-    """m3_mx_linear into contiguous out (rows, n)."""
+    """m3_mx_linear into contiguous out (rows, n), or m3_mx_linear_exact where it is the faster one; allocates its workspace."""
     rows, n = out.shape
+    if out.dtype is torch.float32:
+        size = _mx_exact_bytes(rows, n, k)
+        if size:
+            ws = _workspace(size, out.device)
+            check(lib().m3_mx_linear_exact(rows, n, k, MX_FORMATS[x_format], x_data.data_ptr(), x_scales.data_ptr(), w_data.data_ptr(), w_scales.data_ptr(),
+                                           ptr(residual), scale, out.data_ptr(), ptr(ws), size, stream_of(out)), "m3_mx_linear_exact")
+            return
     st = lib().m3_mx_linear(rows, n, k, MX_FORMATS[x_format], dtype_code(out.dtype), x_data.data_ptr(), x_scales.data_ptr(),
                             w_data.data_ptr(), w_scales.data_ptr(), ptr(residual), scale, out.data_ptr(), stream_of(out))
     if st:

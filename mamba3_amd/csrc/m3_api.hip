@@ -864,6 +864,34 @@ int m3_mx_linear(int64_t rows, int32_t n, int32_t k, int32_t x_format, int32_t o
                                 as_stream(stream));
 }
 
+static int check_exact(int64_t rows, int32_t n, int32_t k) {
+    if (rows <= 0 || n <= 0 || k <= 0) return M3_ERR_INVALID_SHAPE;
+    return rows > (1 << 26) || n > (1 << 26) || k > (1 << 20) ? M3_ERR_UNSUPPORTED : M3_OK;
+}
+
+int m3_mx_linear_exact_workspace_size(int64_t rows, int32_t n, int32_t k, size_t* bytes) {
+    if (!bytes) return M3_ERR_NULL_POINTER;
+    const int st = check_exact(rows, n, k);
+    if (st == M3_OK) *bytes = m3::mx_linear_exact_workspace(rows, n, k);
+    return st;
+}
+
+int m3_mx_linear_exact(int64_t rows, int32_t n, int32_t k, int32_t x_format, const void* x_data, const void* x_scales, const void* w_data,
+                       const void* w_scales, const float* residual, float scale, float* out, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+    if (!x_data || !x_scales || !w_data || !w_scales || !out) return M3_ERR_NULL_POINTER;
+    int st = check_exact(rows, n, k);
+    if (st == M3_OK) st = check_mx(rows, k, x_format);
+    if (st != M3_OK) return st;
+    const size_t bytes = m3::mx_linear_exact_workspace(rows, n, k);
+    if (!bytes) return M3_ERR_UNSUPPORTED;
+    if (!aligned(x_data, 16) || !aligned(w_data, 16) || !aligned(x_scales, 4) || !aligned(w_scales, 4) || !aligned(out, 4) || (residual && !aligned(residual, 4)))
+        return M3_ERR_MISALIGNED;
+    st = check_workspace(workspace, workspace_bytes, bytes);
+    if (st != M3_OK) return st;
+    return m3::launch_mx_linear_exact(x_data, x_scales, x_format, w_data, w_scales, residual, scale, out, (int)rows, n, k, workspace, as_stream(stream));
+}
+
 int m3_mx_linear_takes_tensor(int64_t rows, int32_t n, int32_t k, int32_t x_dtype, int32_t out_dtype, int32_t before) {
     return rows > 0 && n > 0 && k > 0 && m3::mx_linear_takes_tensor(rows, n, k, x_dtype, out_dtype, before) ? 1 : 0;
 }

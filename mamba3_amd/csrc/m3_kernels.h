@@ -251,6 +251,10 @@ int launch_add_norm_bwd(const void* total, const void* w, const float* rstd, con
 int launch_mx_linear(const void* x, const void* xs, int x_format, const void* w, const void* ws,
                      const void* res, float scale, void* out, int out_dtype, int m, int n, int k,
                      hipStream_t stream);
+// fp32 results of many rows, by way of bf16 copies in a workspace (m3_mx_exact.hip; 0 bytes: not worth it).
+size_t mx_linear_exact_workspace(int64_t m, int64_t n, int64_t k);
+int launch_mx_linear_exact(const void* x, const void* xs, int x_format, const void* w, const void* ws, const float* res, float scale,
+                           float* out, int m, int n, int k, void* workspace, hipStream_t stream);
 // ... of a tensor that is quantised to e4m3 on the way, behind its norm or gate (`before`: enum m3_mx_before), where one launch
 // does it all: the same bits.
 bool mx_linear_takes_tensor(int64_t m, int64_t n, int64_t k, int x_dtype, int out_dtype, int before);

@@ -548,3 +548,22 @@ def test_mx_linear_few_rows_many_columns(rows, n, k, fmt):
     want = r.double() - 0.75 * want
     assert ((mamba3_amd.mx_linear(x, w, r, -0.75).double() - want).abs()
             <= half(torch.bfloat16) * want.abs() + 0.75 * off + 2.0 ** -22 * (r.abs().double() + 2 * want.abs())).all()
+
+
+@pytest.mark.parametrize("rows,n,k", [(256, 20001, 2000), (700, 7501, 2000), (1100, 9101, 1003), (8200, 9602, 130)])
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+def test_mx_linear_many_rows_fp32(rows, n, k, fmt):
+    from mamba3_amd import _native
+    assert _native._mx_exact_bytes(rows, n, k) > 0  # sizes that go by way of bf16 copies
+    x, w = mx_pair(rows, n, k, fmt, 13)
+    a, b = x.dequantize(torch.float32).double(), w.dequantize(torch.float32).double()
+    want, size = a @ b.t(), a.abs() @ b.abs().t()
+    off = k * 2.0 ** -24 * size
+    y = mamba3_amd.mx_linear(x, w, out_dtype=torch.float32)
+    assert y.dtype == torch.float32 and ((y.double() - want).abs() <= half(torch.float32) * want.abs() + off).all()
+    r = normal((rows * n + 1,), 3).cuda()[1:].view(rows, n)  # four bytes past an aligned address
+    want = r.double() + 0.25 * want
+    assert ((mamba3_amd.mx_linear(x, w, r, 0.25).double() - want).abs() <= 2.0 ** -23 * (want.abs() + r.abs()) + 0.25 * off).all()
+    x.scales[3, 0] = 255
+    y = mamba3_amd.mx_linear(x, w, out_dtype=torch.float32)
+    assert torch.isnan(y[3]).all() and torch.isfinite(y[:3]).all() and torch.isfinite(y[4:]).all()

@@ -199,3 +199,20 @@ def test_model_refuses_what_it_cannot_serve():
     for bad in (dict(top_p=1.5), dict(min_p=-0.1), dict(top_p=0.5, top_k=0), dict(top_p=0.5, temperature=-1.0), dict(min_p=math.nan)):
         with pytest.raises(ValueError, match="top_p"):
             lm.generate(ids, 1, **bad)
+
+
+def test_mx_linear_exact_refuses_bad_arguments(lib):
+    import ctypes
+    size = ctypes.c_size_t(0)
+    assert lib.m3_mx_linear_exact_workspace_size(1024, 10000, 1024, ctypes.byref(size)) == 0 and size.value == (1024 + 10000) * 1024 * 2
+    assert lib.m3_mx_linear_exact_workspace_size(255, 1 << 20, 1024, ctypes.byref(size)) == 0 and size.value == 0
+    assert lib.m3_mx_linear_exact_workspace_size(0, 1024, 1024, ctypes.byref(size)) == 2 and lib.m3_mx_linear_exact_workspace_size(1024, 1024, 1024, None) == 1
+
+    def go(rows=1024, n=10000, k=1024, fmt=1, x=FAKE, xs=FAKE, w=FAKE, ws=FAKE, res=None, out=FAKE, room=FAKE, bytes_=1 << 30):
+        return lib.m3_mx_linear_exact(rows, n, k, fmt, x, xs, w, ws, res, 1.0, out, room, bytes_, None)
+
+    assert go(x=None) == go(xs=None) == go(w=None) == go(ws=None) == go(out=None) == 1
+    assert go(rows=0) == go(n=-1) == go(k=0) == 2
+    assert go(rows=16) == go(n=8) == go(fmt=2) == go(k=(1 << 20) + 1) == 3
+    assert go(x=FAKE + 8) == go(w=FAKE + 8) == go(xs=FAKE + 2) == go(ws=FAKE + 1) == go(out=FAKE + 2) == go(res=FAKE + 2) == 5
+    assert go(room=None) != 0 and go(bytes_=100) != 0
