@@ -21,8 +21,10 @@ def check_format(fmt: str) -> None:
 
 
 def refuse_gradients(what: str, *tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no backward: call it under torch.no_grad(), or detach its inputs")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no backward: call it under torch.no_grad(), or detach its inputs")
 
 
 class MXTensor:
@@ -38,10 +40,14 @@ class MXTensor:
         shape = torch.Size(shape)
         if len(shape) < 1 or shape[-1] < 1:
             raise ValueError(f"MXTensor needs a last dimension of at least 1, got shape {tuple(shape)}")
-        rows, k = math.prod(shape[:-1]), shape[-1]
-        for name, t, cols in (("data", data, _native.mx_row_bytes(k, format)), ("scales", scales, _native.mx_padded(k) // 32)):
-            if t.dtype is not torch.uint8 or t.shape != (rows, cols) or not t.is_contiguous():
-                raise ValueError(f"{name} must be contiguous uint8 of shape {(rows, cols)}, got {t.dtype} {tuple(t.shape)}")
+        k = shape[-1]
+        rows, kp = shape[0] if len(shape) == 2 else math.prod(shape[:-1]), _native.mx_padded(k)
+        if data.shape != (rows, kp if format == "e4m3" else kp // 2) or scales.shape != (rows, kp // 32):
+            raise ValueError(f"data and scales must have shapes {(rows, _native.mx_row_bytes(k, format))} and {(rows, kp // 32)}, got {tuple(data.shape)} "
+                             f"and {tuple(scales.shape)}")
+        for name, t in (("data", data), ("scales", scales)):
+            if t.dtype is not torch.uint8 or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous uint8, got {t.dtype} with strides {t.stride()}")
         if data.device != scales.device:
             raise ValueError(f"data is on {data.device}, scales on {scales.device}")
         if data.is_cuda and not torch.compiler.is_compiling() and (data.data_ptr() % 16 or scales.data_ptr() % 4):
@@ -65,18 +71,19 @@ class MXTensor:
 def _mx(data: torch.Tensor, scales: torch.Tensor, shape, format: str) -> MXTensor:
     """An MXTensor of what the kernels wrote."""
     t = MXTensor.__new__(MXTensor)
-    t.data, t.scales, t.shape, t.format = data, scales, torch.Size(shape), format
+    t.data, t.scales, t.shape, t.format = data, scales, shape if type(shape) is torch.Size else torch.Size(shape), format
     return t
 
 
 def quantize_mx(x: torch.Tensor, format: str = "e2m1") -> MXTensor:
     """x (..., k), fp32 or bf16 on a GPU, as microscaled values. No backward."""
     check_format(format)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"quantize_mx needs a last dimension of at least 1, got shape {tuple(x.shape)}")
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"quantize_mx needs a last dimension of at least 1, got shape {tuple(shape)}")
     _native.dtype_code(x.dtype)
     refuse_gradients("quantize_mx", x)
-    return _mx(*ops.mx_quantize_fast(x, format, False), x.shape, format)
+    return _mx(*ops.mx_quantize_fast(x, format, False), shape, format)
 
 
 def silu_mul_mx(gate_up: torch.Tensor, format: str = "e4m3") -> MXTensor:
@@ -105,16 +112,16 @@ def mx_linear(x: MXTensor | torch.Tensor, weight: MXTensor, residual: torch.Tens
     if not isinstance(weight, MXTensor) or weight.format != "e2m1" or len(weight.shape) != 2:
         raise ValueError("mx_linear needs a two-dimensional e2m1 MXTensor as weight")
     n, k = weight.shape
-    plain = not isinstance(x, MXTensor)
+    plain, given = not isinstance(x, MXTensor), x.shape
     if plain:
-        if x.dim() < 1:
+        if len(given) < 1:
             raise ValueError("mx_linear expects x (..., k)")
         refuse_gradients("mx_linear", x)
         _native.dtype_code(x.dtype)
     elif gated or norm_weight is not None:
         raise ValueError("norm_weight and gated are for a tensor, x is microscaled already")
-    if x.shape[-1] != (2 * k if gated else k) or n < 1:
-        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit (..., {'2 k' if gated else 'k'}) and (n, k)")
+    if given[-1] != (2 * k if gated else k) or n < 1:
+        raise ValueError(f"x {tuple(given)} and weight {tuple(weight.shape)} do not fit (..., {'2 k' if gated else 'k'}) and (n, k)")
     if norm_weight is not None:
         if gated:
             raise ValueError("either norm_weight or gated")
@@ -125,13 +132,14 @@ def mx_linear(x: MXTensor | torch.Tensor, weight: MXTensor, residual: torch.Tens
     if out_dtype is None:
         out_dtype = residual.dtype if residual is not None else x.dtype if plain else torch.bfloat16
     _native.dtype_code(out_dtype)
-    if x.device != weight.device:
+    at = weight.data.device
+    if (x if plain else x.data).device != at:
         # a tensor on the host is refused for what it is
         _native.require_gpu(x if plain else x.data)
-        raise ValueError(f"x is on {x.device}, weight on {weight.device}")
-    shape = (*x.shape[:-1], n)
+        raise ValueError(f"x is on {x.device}, weight on {at}")
+    shape = (given[0], n) if len(given) == 2 else (*given[:-1], n)
     if residual is not None:
-        if residual.shape != shape or residual.dtype != out_dtype or residual.device != weight.device:
+        if residual.shape != shape or residual.dtype != out_dtype or residual.device != at:
             raise ValueError(f"residual must be {out_dtype} of shape {shape} on {x.device}, got {residual.dtype} "
                              f"{tuple(residual.shape)} on {residual.device}")
         refuse_gradients("mx_linear", residual)

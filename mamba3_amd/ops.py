@@ -1011,9 +1011,9 @@ def _rows_of(t: torch.Tensor) -> torch.Tensor:
 
 def _mx_empty(rows: int, k: int, fmt: str, like: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Room for (rows, k) microscaled values: (data, scales)."""
-    device, kp = like.device, _native.mx_padded(k)
-    return (torch.empty((rows, kp if fmt == "e4m3" else kp // 2), dtype=torch.uint8, device=device),
-            torch.empty((rows, kp // 32), dtype=torch.uint8, device=device))
+    kp = _native.mx_padded(k)
+    return (like.new_empty((rows, kp if fmt == "e4m3" else kp // 2), dtype=torch.uint8),
+            like.new_empty((rows, kp // 32), dtype=torch.uint8))
 
 
 def _mx_quantize_eager(x: torch.Tensor, fmt: str, gated: bool) -> tuple[torch.Tensor, torch.Tensor]:
@@ -1021,8 +1021,9 @@ def _mx_quantize_eager(x: torch.Tensor, fmt: str, gated: bool) -> tuple[torch.Te
     _native.require_gpu(x)
     with on_device(x):
         x2 = _rows_of(x)
-        out = _mx_empty(x2.shape[0], x2.shape[1] // 2 if gated else x2.shape[1], fmt, x2)
-        if x2.shape[0]:
+        rows, k = x2.shape
+        out = _mx_empty(rows, k // 2 if gated else k, fmt, x2)
+        if rows:
             _native.mx_quantize(x2, fmt, gated, *out)
     return out
 
@@ -1040,8 +1041,9 @@ def _mx_dequantize_eager(data: torch.Tensor, scales: torch.Tensor, fmt: str, k: 
     """m3_mx_dequantize: (rows, k) in `dtype`."""
     _native.require_gpu(data, scales)
     with on_device(data):
-        out = torch.empty((data.shape[0], k), device=data.device, dtype=dtype)
-        if out.shape[0]:
+        rows = data.shape[0]
+        out = data.new_empty((rows, k), dtype=dtype)
+        if rows:
             _native.mx_dequantize(data, scales, fmt, out)
     return out
 
@@ -1164,11 +1166,12 @@ def _add_rmsnorm_mx_eager(x: torch.Tensor, residual: Optional[torch.Tensor], wei
     with on_device(x):
         x2 = _rows_of(x)
         total = None if residual is None else torch.empty_like(x2)
-        data, scales = _mx_empty(*x2.shape, fmt, x2)
-        if x2.shape[0]:
+        rows, d = x2.shape
+        data, scales = _mx_empty(rows, d, fmt, x2)
+        if rows:
             _native.add_rmsnorm_mx(x2, None if residual is None else _rows_of(residual), weight.contiguous(), scale, eps,
                                    total, fmt, data, scales)
-    return None if total is None else total.view(x.shape), data, scales
+    return total if total is None or x2 is x else total.view(x.shape), data, scales
 
 
 @torch.library.custom_op(f"{NS}::add_rmsnorm_mx", mutates_args=())
@@ -1190,8 +1193,9 @@ def _mx_linear_eager(x_data: torch.Tensor, x_scales: torch.Tensor, x_format: str
     """m3_mx_linear: (rows, n) in `dtype`, the residual's where one is given."""
     _native.require_gpu(x_data, x_scales, w_data, w_scales, residual)
     with on_device(x_data):
-        out = torch.empty((x_data.shape[0], w_data.shape[0]), device=x_data.device, dtype=dtype)
-        if out.numel():
+        rows, n = x_data.shape[0], w_data.shape[0]
+        out = x_data.new_empty((rows, n), dtype=dtype)
+        if rows and n:
             _native.mx_linear(x_data, x_scales, x_format, w_data, w_scales, k,
                               None if residual is None else _rows_of(residual), scale, out)
     return out
@@ -1222,7 +1226,7 @@ def _mx_linear_tensor_eager(x: torch.Tensor, norm_weight: Optional[torch.Tensor]
     _native.require_gpu(x, norm_weight, w_data, w_scales, residual)
     with on_device(x):
         x2 = _rows_of(x)
-        out = torch.empty((x2.shape[0], w_data.shape[0]), device=x.device, dtype=dtype)
+        out = x2.new_empty((x2.shape[0], w_data.shape[0]), dtype=dtype)
         _native.mx_linear_tensor(x2, None if norm_weight is None else norm_weight.contiguous(), eps, gated, w_data, w_scales,
                                  None if residual is None else _rows_of(residual), scale, out)
     return out
@@ -1244,8 +1248,8 @@ def _sample_tokens_eager(logits: torch.Tensor, u: torch.Tensor, temperatures: Op
     _native.require_gpu(logits, u, temperatures, top_ks, top_ps, min_ps)
     with on_device(logits):
         rows = logits.shape[0]
-        token = torch.empty(rows, device=logits.device, dtype=torch.int64)
-        lp = torch.empty(rows if logprob else 0, device=logits.device, dtype=torch.float32)
+        token = logits.new_empty(rows, dtype=torch.int64)
+        lp = logits.new_empty(rows if logprob else 0, dtype=torch.float32)
         each = [n if t is None else t.contiguous()
                 for t, n in ((temperatures, temperature), (top_ks, top_k), (top_ps, top_p), (min_ps, min_p))]
         if rows:

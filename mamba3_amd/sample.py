@@ -22,7 +22,7 @@ def _setting(name: str, v, least: float, most: float, shape, device, dtype) -> t
         if v.dtype != dtype:
             raise TypeError(f"{name} by row must be {dtype}, got {v.dtype}")
         return v.reshape(-1), 0
-    v = int(v) if dtype == torch.int32 else float(v)
+    v = int(v) if dtype is torch.int32 else float(v)
     if not least <= v <= most:
         raise ValueError(f"{name} must lie in [{least}, {most}], got {v}")
     return None, v
@@ -59,5 +59,9 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
                                  ("top_p", top_p, 1.0, torch.float32), ("min_p", min_p, 1.0, torch.float32)):
         args += _setting(name, v, 0, most, shape, logits.device, dtype)
     _native.require_gpu(logits)
-    token, lp = ops.sample_tokens_fast(logits.detach().reshape(-1, logits.shape[-1]), u.reshape(-1), *args, return_logprob)
+    z = logits.detach() if logits.requires_grad else logits
+    if len(shape) == 1:
+        got = ops.sample_tokens_fast(z, u, *args, return_logprob)
+        return got if return_logprob else got[0]
+    token, lp = ops.sample_tokens_fast(z.reshape(-1, z.shape[-1]), u.reshape(-1), *args, return_logprob)
     return (token.view(shape), lp.view(shape)) if return_logprob else token.view(shape)
