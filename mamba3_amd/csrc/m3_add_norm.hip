@@ -94,7 +94,7 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_kernel(AddNormArgs a) {
             if (unit >= units) continue;
             float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = kF != kSame ? norm_odd<T>(t[p][e], w[p][e], r2) : t[p][e] * rs * w[p][e];
+            for (int e = 0; e < 8; ++e) v[e] = kF != kSame ? norm_odd(t[p][e], w[p][e], r2) : t[p][e] * rs * w[p][e];
             if constexpr (kF == kSame) store8(reinterpret_cast<T*>(a.y) + base, unit * 8, d, v);
             else mx_store8<kF>(v, a.data + row * (kF == kE4m3 ? a.kp : a.kp / 2), a.scales + row * (a.kp / 32), unit);
         }
@@ -134,7 +134,7 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_wide_kernel(AddNormArgs a
             load8(reinterpret_cast<const T*>(kRes ? a.total : a.x) + base, unit * 8, d, t);
             load8(reinterpret_cast<const T*>(a.w), unit * 8, d, w);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) t[e] = kF != kSame ? norm_odd<T>(t[e], w[e], r2) : t[e] * rs * w[e];
+            for (int e = 0; e < 8; ++e) t[e] = kF != kSame ? norm_odd(t[e], w[e], r2) : t[e] * rs * w[e];
             if constexpr (kF == kSame) store8(reinterpret_cast<T*>(a.y) + base, unit * 8, d, t);
             else mx_store8<kF>(t, a.data + row * (kF == kE4m3 ? a.kp : a.kp / 2), a.scales + row * (a.kp / 32), unit);
         }

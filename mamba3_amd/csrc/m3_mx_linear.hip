@@ -246,7 +246,7 @@ __global__ __launch_bounds__(kW * 64) void mx_linear_raw_kernel(MxLinearArgs a, 
             for (int p = 0; p < kMlNormPieces; ++p) {
                 if (lane + p * 64 >= units) continue;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) t[p][e] = norm_odd<T>(t[p][e], (float)nw[p][e], rs);
+                for (int e = 0; e < 8; ++e) t[p][e] = norm_odd(t[p][e], (float)nw[p][e], rs);
                 put(t[p], row, lane + p * 64);
             }
         }

@@ -42,11 +42,9 @@ __device__ __forceinline__ RowScale row_scale(double m) {
     const double e = fma(-m * (double)r, (double)r, 1.0);
     return RowScale{r, fabs(e) < 1e-3 ? (float)(0.5 * (double)r * e) : 0.f};  // (m of 0, infinity or NaN: hi is the answer)
 }
-template <typename T>
 __device__ __forceinline__ float norm_odd(float t, float w, RowScale r) {
-    const float p = t * w, hi = p * r.hi;
-    float rest = fmaf(p, r.lo, fmaf(p, r.hi, -hi));
-    if constexpr (sizeof(T) == 4) rest = fmaf(fmaf(t, w, -p), r.hi, rest);  // (a product of two bf16 is exact)
+    const float p = t * r.hi, hi = p * w;  // (t w first could overflow)
+    const float rest = fmaf(fmaf(t, r.lo, fmaf(t, r.hi, -p)), w, fmaf(p, w, -hi));
     const unsigned b = __builtin_bit_cast(unsigned, hi), toward = (__builtin_bit_cast(unsigned, rest) ^ b) >> 31;  // 1: toward zero
     return __builtin_bit_cast(float, fabsf(rest) > 0.f ? (b - toward) | 1u : b);
 }

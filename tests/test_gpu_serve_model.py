@@ -441,3 +441,13 @@ def test_a_captured_graph_follows_the_weights():
         want = lm._mx_logits(x).clone()
     with torch.no_grad():
         assert same(lm._mx_logits(x), want)
+
+
+@torch.no_grad()
+def test_compiled_model_runs_its_4_bit_blocks_as_they_are():
+    torch._dynamo.reset()
+    lm = small_lm().quantize_mx()
+    ids = torch.randint(0, 500, (2, 9), generator=torch.Generator().manual_seed(1)).cuda()
+    want = lm(ids)["logits"]
+    assert same(torch.compile(lm, backend="aot_eager")(ids)["logits"], want)
+    torch._dynamo.reset()

@@ -567,3 +567,24 @@ def test_mx_linear_many_rows_fp32(rows, n, k, fmt):
     x.scales[3, 0] = 255
     y = mamba3_amd.mx_linear(x, w, out_dtype=torch.float32)
     assert torch.isnan(y[3]).all() and torch.isfinite(y[:3]).all() and torch.isfinite(y[4:]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_add_rms_norm_mx_large_and_small_values(dtype):
+    """Rows whose products with the weight alone would overflow or vanish; and each element on the side of a tie where the formula in
+    64 bits has it."""
+    x = normal((6, 384), 0, torch.float64) * torch.tensor([1e18, 1e-18, 1.0, 1e15, 1e-10, 3.0])[:, None].double()
+    w = normal((384,), 1, torch.float64) * torch.tensor([1e22, 1e-20, 1.0]).repeat(128).double()
+    x, w = x.to(dtype), w.to(dtype)
+    q = mamba3_amd.add_rms_norm_mx(x.cuda(), None, w.cuda(), eps=1e-30)[1]
+    t = x.double()
+    y = t / torch.sqrt(t.square().mean(1, keepdim=True) + 1e-30) * w.double()
+    assert torch.equal(q.dequantize(torch.float32).cpu().double(), ref_values(y, "e4m3").float().double())
+    big = normal((3000, 512), 2, dtype)
+    w = normal((512,), 3, dtype)
+    for fmt in ("e4m3", "e2m1"):
+        v = mamba3_amd.add_rms_norm_mx(big.cuda(), None, w.cuda(), 1.0, 1e-5, fmt)[1].dequantize(torch.float32).cpu().double()
+        t = big.double()
+        want = ref_values(t / torch.sqrt(t.square().mean(1, keepdim=True) + 1e-5) * w.double(), fmt)
+        # a row's reciprocal root is 2^-28 or so from exact: of 1.5 million elements one may be that near to a tie
+        assert (v != want).sum() <= 2
