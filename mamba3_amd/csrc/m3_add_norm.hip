@@ -4,8 +4,10 @@
 // the inputs' type or to microscaled elements (m3_mx.h). The squares are of t as it is stored, since
 // that is what the next block adds to. Backward, with g = w dy and a = sum g t:
 //   dt = dtotal + r g - t r^3 a / d,   dresidual = dt,   dx = s dt,   dw = sum over rows of dy t r
-// Bound by HBM: x, residual, t and y once each; backward t, dtotal, dy, dx and dresidual once each.
+// Bound by HBM: x, residual, t and y once each; backward t, dtotal, dy, dx and dresidual once each. bf16, 16384 x 2048: forward
+// 51 us (5.2 TB/s), to e4m3 58 (4.1 TB/s: the roundings below cost 4 us), backward 64 and 5 for dw (5.2 TB/s); fp32 107 and 138.
 //
+// One wave a row where it holds it: no barriers, and the rows of a block's four waves hide one another's latency.
 // A row is taken by one wave (to 2048 columns) or by a block's four (to 8192), eight consecutive
 // columns a lane and piece, so that four lanes hold a block of 32; wider rows are read a second time.
 // Squares are added in fp32 within a lane (at most 32 of them) and in fp64 across lanes; for microscaled results in fp64

@@ -1,5 +1,6 @@
 // Microscaled quantisation (m3_mx.h), with silu(gate) * up in front of it, and its inverse.
-// Bound by HBM: one read and one write. A lane takes eight elements (one 16-byte read of bf16), four
+// Bound by HBM: one read and one write; gated by the gate's arithmetic as well. 32000 x 768 in bf16 to e2m1 14.5 us (4.3 TB/s), gated
+// 8192 x 2112 to e4m3 21.6 us (4.0 TB/s), its values 9.6 (5.5 TB/s, read from the caches). A lane takes eight elements (one 16-byte read of bf16), four
 // lanes a block of 32, whose largest magnitude they find with two lane moves.
 #include <algorithm>
 

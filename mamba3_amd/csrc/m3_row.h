@@ -46,7 +46,8 @@ __device__ __forceinline__ float norm_odd(float t, float w, RowScale r) {
     const float p = t * r.hi, hi = p * w;  // (t w first could overflow)
     const float rest = fmaf(fmaf(t, r.lo, fmaf(t, r.hi, -p)), w, fmaf(p, w, -hi));
     const unsigned b = __builtin_bit_cast(unsigned, hi), toward = (__builtin_bit_cast(unsigned, rest) ^ b) >> 31;  // 1: toward zero
-    return __builtin_bit_cast(float, fabsf(rest) > 0.f ? (b - toward) | 1u : b);
+    constexpr int kNumber = 0x198;  // but for 0, infinity and NaN
+    return __builtin_bit_cast(float, __builtin_amdgcn_classf(rest, kNumber) ? (b - toward) | 1u : b);
 }
 // The sum of eight squares added to s. (Their roundings to fp32 average out over a row: about 2^-28 of its sum.)
 __device__ __forceinline__ double add_squares(double s, const float (&t)[8]) {

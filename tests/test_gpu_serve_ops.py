@@ -588,3 +588,13 @@ def test_add_rms_norm_mx_large_and_small_values(dtype):
         want = ref_values(t / torch.sqrt(t.square().mean(1, keepdim=True) + 1e-5) * w.double(), fmt)
         # a row's reciprocal root is 2^-28 or so from exact: of 1.5 million elements one may be that near to a tie
         assert (v != want).sum() <= 2
+
+
+def test_add_rms_norm_mx_past_the_largest_number():
+    x, w = normal((4, 128), 5), torch.full((128,), 2.5e38)
+    w[64:] = 1.0
+    y = (x.double() / torch.sqrt(x.double().square().mean(1, keepdim=True))) * w.double()
+    past = (y.abs() > torch.finfo(torch.float32).max).view(4, 4, 32).any(-1)
+    assert past.any() and not past.all()
+    v = mamba3_amd.add_rms_norm_mx(x.cuda(), None, w.cuda(), eps=0.0)[1]
+    assert torch.equal(v.scales.cpu() == 255, past)  # an infinity makes its block NaN
