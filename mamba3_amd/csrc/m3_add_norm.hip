@@ -57,25 +57,29 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_kernel(AddNormArgs a) {
     __shared__ double red[kAnWaves];
     const int lane = threadIdx.x % kLanes;
     const int d = a.d, units = (kF == kSame ? d + 7 : a.kp) / 8;
-    float w[kNp][8];
+    Held8<T> w[kNp];
 #pragma unroll
-    for (int p = 0; p < kNp; ++p) load8(reinterpret_cast<const T*>(a.w), (lane + p * kLanes) * 8, d, w[p]);
+    for (int p = 0; p < kNp; ++p) w[p].load(reinterpret_cast<const T*>(a.w), (lane + p * kLanes) * 8, d);
     for (int64_t row = (int64_t)blockIdx.x * kRpb + threadIdx.x / kLanes; row < a.rows; row += (int64_t)gridDim.x * kRpb) {
         const int64_t base = row * d;
-        float t[kNp][8], r[kRes ? kNp : 1][8];
+        float t[kNp][8];
+        Held8<T> x[kNp], r[kRes ? kNp : 1];
 #pragma unroll
         for (int p = 0; p < kNp; ++p) {
             const int c = (lane + p * kLanes) * 8;
-            load8(reinterpret_cast<const T*>(a.x) + base, c, d, t[p]);
-            if constexpr (kRes) load8(reinterpret_cast<const T*>(a.res) + base, c, d, r[p]);
+            x[p].load(reinterpret_cast<const T*>(a.x) + base, c, d);
+            if constexpr (kRes) r[p].load(reinterpret_cast<const T*>(a.res) + base, c, d);
         }
         float ss = 0.f;
         double squares = 0.0;
 #pragma unroll
         for (int p = 0; p < kNp; ++p) {
+            x[p].values(t[p]);
             if constexpr (kRes) {
+                float v[8];
+                r[p].values(v);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) t[p][e] = (float)(T)fmaf(a.scale, t[p][e], r[p][e]);
+                for (int e = 0; e < 8; ++e) t[p][e] = (float)(T)fmaf(a.scale, t[p][e], v[e]);
                 const int c = (lane + p * kLanes) * 8;
                 if (c < d) store8(reinterpret_cast<T*>(a.total) + base, c, d, t[p]);
             }
@@ -95,8 +99,9 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_kernel(AddNormArgs a) {
             const int unit = lane + p * kLanes;
             if (unit >= units) continue;
             float v[8];
+            w[p].values(v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = kF != kSame ? norm_odd(t[p][e], w[p][e], r2) : t[p][e] * rs * w[p][e];
+            for (int e = 0; e < 8; ++e) v[e] = kF != kSame ? norm_odd(t[p][e], v[e], r2) : t[p][e] * rs * v[e];
             if constexpr (kF == kSame) store8(reinterpret_cast<T*>(a.y) + base, unit * 8, d, v);
             else mx_store8<kF>(v, a.data + row * (kF == kE4m3 ? a.kp : a.kp / 2), a.scales + row * (a.kp / 32), unit);
         }

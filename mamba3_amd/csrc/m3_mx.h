@@ -180,6 +180,25 @@ __device__ __forceinline__ void values8(const u32x4& r, float (&v)[8]) {
         v[e] = __builtin_bit_cast(float, e % 2 ? w & 0xffff0000u : w << 16);
     }
 }
+// Eight elements that stay in registers: bf16 in half as many.
+template <typename T> struct Held8;
+template <> struct Held8<bf16> {
+    u32x4 raw;
+    __device__ __forceinline__ void load(const bf16* row, int c, int n) { raw = raw8(row, c, n); }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+        u32x4 r = raw;
+        asm volatile("" : "+v"(r));  // not hoisted out of a loop, where the values would be held after all
+        values8(r, v);
+    }
+};
+template <> struct Held8<float> {
+    float raw[8];
+    __device__ __forceinline__ void load(const float* row, int c, int n) { load8(row, c, n, raw); }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = raw[e];
+    }
+};
 template <typename T>
 __device__ __forceinline__ void store8(T* row, int c, int n, const float (&v)[8]) {
     T t[8];
