@@ -1,6 +1,6 @@
 // Microscaled quantisation (m3_mx.h), with silu(gate) * up in front of it, and its inverse.
-// Bound by HBM: one read and one write; gated by the gate's arithmetic as well. 32000 x 768 in bf16 to e2m1 14.5 us (4.3 TB/s), gated
-// 8192 x 2112 to e4m3 21.6 us (4.0 TB/s), its values 9.6 (5.5 TB/s, read from the caches). A lane takes eight elements (one 16-byte read of bf16), four
+// Bound by HBM: one read and one write; gated by the gate's arithmetic as well. 32000 x 768 in bf16 to e2m1 13.4 us (4.6 TB/s), gated
+// 8192 x 2112 to e4m3 17.5 us (5.0 TB/s), its values 10.2 (5.1 TB/s). A lane takes eight elements (one 16-byte read of bf16), four
 // lanes a block of 32, whose largest magnitude they find with two lane moves.
 #include <algorithm>
 
@@ -13,64 +13,47 @@
 namespace m3 {
 
 constexpr int kMxThreads = 256;
-constexpr int kMxUnits = 2;  // eights a thread
 
+// A thread an eight: two or four a thread, asked for at once, took longer (gated 8192 x 2112 17.5 us, 19.7 and 25).
 template <typename T, int F, bool kGated>
 __global__ __launch_bounds__(kMxThreads) void mx_quantize_kernel(const T* __restrict__ x, uint8_t* __restrict__ data,
                                                                  uint8_t* __restrict__ scales, unsigned units, int k,
                                                                  int kp, FastDiv per_row) {
-    const unsigned at = blockIdx.x * (kMxThreads * kMxUnits) + threadIdx.x;
-    float v[kMxUnits][8], u[kGated ? kMxUnits : 1][8];
-    unsigned row[kMxUnits];
-    int unit[kMxUnits];
-#pragma unroll
-    for (int i = 0; i < kMxUnits; ++i) {
-        const unsigned id = at + i * kMxThreads;
-        row[i] = per_row.div(id);
-        unit[i] = (int)(id - row[i] * per_row.d);
-        if (id < units) {
-            const T* r = x + (int64_t)row[i] * (kGated ? 2 * (int64_t)k : k);
-            load8(r, unit[i] * 8, k, v[i]);
-            if constexpr (kGated) load8(r + k, unit[i] * 8, k, u[i]);
-        }
+    const unsigned id = blockIdx.x * kMxThreads + threadIdx.x;
+    if (id >= units) return;  // whole blocks of 32: units of a row come in sixteens
+    const unsigned row = per_row.div(id);
+    const int unit = (int)(id - row * per_row.d);
+    const T* r = x + (int64_t)row * (kGated ? 2 * (int64_t)k : k);
+    Held8<T> x8, u8;
+    x8.load(r, unit * 8, k);
+    if constexpr (kGated) u8.load(r + k, unit * 8, k);
+    float v[8];
+    x8.values(v);
+    if constexpr (kGated) {
+        float u[8];
+        u8.values(u);
+        silu_mul8(v, u);
     }
-#pragma unroll
-    for (int i = 0; i < kMxUnits; ++i) {
-        if (at + i * kMxThreads >= units) continue;  // whole blocks of 32: units of a row come in sixteens
-        if constexpr (kGated) silu_mul8(v[i], u[i]);
-        mx_store8<F>(v[i], data + (int64_t)row[i] * (F == kE4m3 ? kp : kp / 2), scales + (int64_t)row[i] * (kp / 32), unit[i]);
-    }
+    mx_store8<F>(v, data + (int64_t)row * (F == kE4m3 ? kp : kp / 2), scales + (int64_t)row * (kp / 32), unit);
 }
 
 template <typename T, int F>
 __global__ __launch_bounds__(kMxThreads) void mx_dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales,
                                                                    T* __restrict__ out, unsigned units, int k, int kp, FastDiv per_row) {
-    const unsigned at = blockIdx.x * (kMxThreads * kMxUnits) + threadIdx.x;
-    u32x2 w[kMxUnits];
-    unsigned row[kMxUnits], s[kMxUnits];
-    int unit[kMxUnits];
+    const unsigned id = blockIdx.x * kMxThreads + threadIdx.x;
+    if (id >= units) return;
+    const unsigned row = per_row.div(id);
+    const int unit = (int)(id - row * per_row.d);
+    const uint8_t* p = data + (int64_t)row * (F == kE4m3 ? kp : kp / 2);
+    u32x2 w;
+    if constexpr (F == kE4m3) w = *reinterpret_cast<const u32x2*>(p + unit * 8);
+    else w = u32x2{*reinterpret_cast<const unsigned*>(p + unit * 4), 0};
+    const float f = mx_factor(scales[(int64_t)row * (kp / 32) + (unit >> 2)]);
+    float v[8];
+    mx_unpack8<F>(w, v);
 #pragma unroll
-    for (int i = 0; i < kMxUnits; ++i) {
-        const unsigned id = at + i * kMxThreads;
-        row[i] = per_row.div(id);
-        unit[i] = (int)(id - row[i] * per_row.d);
-        if (id < units) {
-            const uint8_t* p = data + (int64_t)row[i] * (F == kE4m3 ? kp : kp / 2);
-            if constexpr (F == kE4m3) w[i] = *reinterpret_cast<const u32x2*>(p + unit[i] * 8);
-            else w[i] = u32x2{*reinterpret_cast<const unsigned*>(p + unit[i] * 4), 0};
-            s[i] = scales[(int64_t)row[i] * (kp / 32) + (unit[i] >> 2)];
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < kMxUnits; ++i) {
-        if (at + i * kMxThreads >= units) continue;
-        float v[8];
-        mx_unpack8<F>(w[i], v);
-        const float f = mx_factor(s[i]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= f;
-        store8(out + (int64_t)row[i] * k, unit[i] * 8, k, v);
-    }
+    for (int e = 0; e < 8; ++e) v[e] *= f;
+    store8(out + (int64_t)row * k, unit * 8, k, v);
 }
 
 // Launches of fewer than 2^31 units.
@@ -79,7 +62,7 @@ static int mx_rows(int64_t rows, int64_t per_row, Launch launch) {
     const int64_t most = (((int64_t)1 << 31) - 1) / per_row;
     for (int64_t r = 0; r < rows; r += most) {
         const unsigned units = (unsigned)(std::min(most, rows - r) * per_row);
-        launch(r, units, dim3((units + kMxThreads * kMxUnits - 1) / (kMxThreads * kMxUnits)));
+        launch(r, units, dim3((units + kMxThreads - 1) / kMxThreads));
         if (hipGetLastError() != hipSuccess) return M3_ERR_LAUNCH;
     }
     return M3_OK;

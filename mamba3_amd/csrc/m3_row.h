@@ -60,7 +60,7 @@ __device__ __forceinline__ double add_squares(double s, const float (&t)[8]) {
 // v = silu(v) u. With e = exp(-|g|), at most 1: silu = (g < 0 ? g e : g) / (1 + e), which does not overflow. For |g| < 80
 // e comes from the hardware's power of two, with the rounding of its argument put right, and 1 / (1 + e) from its reciprocal
 // (about 2 units in the last place together); beyond, where e nears the smallest numbers, from the library. With expf and a
-// division throughout, gating 8192 x 2112 took 26 us instead of 20.
+// division throughout, gating 8192 x 2112 took 26 us instead of 20 (17.5 with an eight a thread).
 __device__ __forceinline__ void silu_mul8(float (&v)[8], const float (&u)[8]) {
     float most = 0.f;
 #pragma unroll
