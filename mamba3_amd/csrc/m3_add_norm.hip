@@ -5,7 +5,9 @@
 // that is what the next block adds to. Backward, with g = w dy and a = sum g t:
 //   dt = dtotal + r g - t r^3 a / d,   dresidual = dt,   dx = s dt,   dw = sum over rows of dy t r
 // Bound by HBM: x, residual, t and y once each; backward t, dtotal, dy, dx and dresidual once each. bf16, 16384 x 2048: forward
-// 51 us (5.2 TB/s), to e4m3 58 (4.1 TB/s: the roundings below cost 4 us), backward 64 and 5 for dw (5.2 TB/s); fp32 107 and 138.
+// 43 us (6.2 TB/s, partly from the last-level cache), to e4m3 40 (5.9), backward 64 and 5 for dw (5.2 TB/s); fp32 107, 85 and 138. bf16 rows and
+// weights wait as they lie in memory and are taken apart where they are used: at half the registers, four to six waves a SIMD
+// instead of three or four (51 us and 58 as fp32).
 //
 // One wave a row where it holds it: no barriers, and the rows of a block's four waves hide one another's latency.
 // A row is taken by one wave (to 2048 columns) or by a block's four (to 8192), eight consecutive
