@@ -31,6 +31,7 @@ struct MxLinearArgs {
     void* out;
     float scale;
     int M, N, steps;  // steps of 128 k
+    int ld;           // columns of a row of out and res
 };
 struct MxBefore {  // of a tensor: its norm's weight
     const void* norm;
@@ -84,7 +85,7 @@ template <typename TO>
 __device__ __forceinline__ void mx_out4(const MxLinearArgs& a, int m, int n, f32x4 v, bool whole) {
     typedef TO T4 __attribute__((ext_vector_type(4)));
     if (m >= a.M || n >= a.N) return;
-    const int64_t at = (int64_t)m * a.N + n;
+    const int64_t at = (int64_t)m * a.ld + n;
     TO* out = reinterpret_cast<TO*>(a.out) + at;
     const TO* res = reinterpret_cast<const TO*>(a.res) + at;
     if (whole) {
@@ -303,7 +304,7 @@ __global__ __launch_bounds__(kW * 64) void mx_linear_raw_kernel(MxLinearArgs a, 
 template <typename TO>
 static bool out4(const MxLinearArgs& a) {
     const size_t piece = 4 * sizeof(TO);
-    return a.N % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % piece == 0 && (!a.res || reinterpret_cast<uintptr_t>(a.res) % piece == 0);
+    return a.ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % piece == 0 && (!a.res || reinterpret_cast<uintptr_t>(a.res) % piece == 0);
 }
 // Waves of a block (the measurements: above).
 template <int FM, int FN, typename F>
@@ -539,7 +540,7 @@ __global__ __launch_bounds__(Tile::NT, 2) void mx_linear_tile_kernel(MxLinearArg
 
     // ---- epilogue: ER rows of 64 columns at a time. Stores go out unconditionally, those past the end to an offset
     // that the descriptor drops, so that their number is known to the next wait.
-    const bool whole = a.N % 8 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && reinterpret_cast<uintptr_t>(a.res) % 16 == 0;
+    const bool whole = a.N % 8 == 0 && a.ld % 8 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && reinterpret_cast<uintptr_t>(a.res) % 16 == 0;
     auto epilogue = [&](int id, auto with_res) __attribute__((always_inline)) {
         constexpr bool kRes = decltype(with_res)::value;
         constexpr int ER = Tile::ER, T = ER / 8;
@@ -576,7 +577,7 @@ __global__ __launch_bounds__(Tile::NT, 2) void mx_linear_tile_kernel(MxLinearArg
 #pragma unroll
                 for (int t = 0; t < T; ++t) {
                     const int m = m0 + round * ER + t * 8 + rr;
-                    rv[kRes ? to : 0][t] = *reinterpret_cast<const bf16x8*>(res + (int64_t)(m < a.M ? m : a.M - 1) * a.N + (n < a.N ? n : a.N - 8));
+                    rv[kRes ? to : 0][t] = *reinterpret_cast<const bf16x8*>(res + (int64_t)(m < a.M ? m : a.M - 1) * a.ld + (n < a.N ? n : a.N - 8));
                 }
             };
             if constexpr (kRes) read_res(0, 0);
@@ -591,11 +592,11 @@ __global__ __launch_bounds__(Tile::NT, 2) void mx_linear_tile_kernel(MxLinearArg
                 }
                 combine(round);
                 const int m1 = m0 + round * ER, rows = a.M - m1 < ER ? a.M - m1 : ER;
-                const __amdgpu_buffer_rsrc_t to = make_rsrc(out + (int64_t)m1 * a.N, rows > 0 ? (int64_t)rows * a.N * 2 : 0);
+                const __amdgpu_buffer_rsrc_t to = make_rsrc(out + (int64_t)m1 * a.ld, rows > 0 ? (int64_t)rows * a.ld * 2 : 0);
 #pragma unroll
                 for (int t = 0; t < T; ++t) {
                     const u32x4 v = *reinterpret_cast<const u32x4*>(mine + (t * 8 + rr) * 128 + (((lane & 7) ^ rr) * 16));
-                    __builtin_amdgcn_raw_buffer_store_b128(v, to, n < a.N ? ((t * 8 + rr) * a.N + n) * 2 : (int)0x80000000u, 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b128(v, to, n < a.N ? ((t * 8 + rr) * a.ld + n) * 2 : (int)0x80000000u, 0, 0);
                 }
                 M3_LDS_FENCE();
             }
@@ -610,7 +611,7 @@ __global__ __launch_bounds__(Tile::NT, 2) void mx_linear_tile_kernel(MxLinearArg
                 if constexpr (kRes) {
                     bf16 v[ER];
 #pragma unroll
-                    for (int e = 0; e < ER; ++e) v[e] = res[(int64_t)(m1 + e < a.M ? m1 + e : a.M - 1) * a.N + nc];
+                    for (int e = 0; e < ER; ++e) v[e] = res[(int64_t)(m1 + e < a.M ? m1 + e : a.M - 1) * a.ld + nc];
 #pragma unroll
                     for (int e = 0; e < ER; ++e) *at(e) = v[e];
                     M3_LDS_FENCE();
@@ -619,7 +620,7 @@ __global__ __launch_bounds__(Tile::NT, 2) void mx_linear_tile_kernel(MxLinearArg
 #pragma unroll
                 for (int e = 0; e < ER; ++e) {
                     const bf16 v = *at(e);
-                    if (m1 + e < a.M && n < a.N) out[(int64_t)(m1 + e) * a.N + n] = v;
+                    if (m1 + e < a.M && n < a.N) out[(int64_t)(m1 + e) * a.ld + n] = v;
                 }
                 M3_LDS_FENCE();
             }
@@ -705,7 +706,7 @@ __global__ __launch_bounds__(Tile::NT, 2) void mx_linear_tile_kernel(MxLinearArg
 template <typename Tile>
 static int tile_t(const MxLinearArgs& a, hipStream_t stream) {
     const int64_t tm = (a.M + Tile::BM - 1) / Tile::BM, tn = (a.N + Tile::BN - 1) / Tile::BN;
-    if (tm * tn > (1 << 30) || a.N > (1 << 25)) return M3_ERR_UNSUPPORTED;  // 32 rows of results within a descriptor
+    if (tm * tn > (1 << 30) || a.ld > (1 << 25)) return M3_ERR_UNSUPPORTED;  // 32 rows of results within a descriptor
     static std::atomic<uint64_t> done{0};
     if (!allow_lds(reinterpret_cast<const void*>(&mx_linear_tile_kernel<Tile>), Tile::kLds, done)) return M3_ERR_LAUNCH;
     const int64_t most = 256 * std::min(2, (160 << 10) / Tile::kLds);  // blocks at once
@@ -734,9 +735,24 @@ template <int FA, typename TO>
 static int linear_t(const MxLinearArgs& a, hipStream_t stream) {
     if constexpr (sizeof(TO) == 2) {
         if (takes_tiles(a)) {
-            const int64_t large = (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256);
+            typedef MxTile<FA, 256, 256, 2, 4, 2, 32> Large;
+            typedef MxTile<FA, 128, 128, 2, 2, 2, 32> Middle;
             if (a.M <= 64) return tile_t<MxTile<FA, 64, 128, 1, 2, 4, 32>>(a, stream);
-            return large >= 192 && a.steps >= 12 && a.M > 128 ? tile_t<MxTile<FA, 256, 256, 2, 4, 2, 32>>(a, stream) : tile_t<MxTile<FA, 128, 128, 2, 2, 2, 32>>(a, stream);
+            const int64_t tm = (a.M + 255) / 256, large = tm * ((a.N + 255) / 256);
+            if (large < 192 || a.steps < 12 || a.M <= 128) return tile_t<Middle>(a, stream);
+            // Whole rounds of large tiles, one a CU, and for the columns that are left one round of the others, two a CU, if they
+            // fit it (us, all in large tiles and so: 1.2 rounds, 300 x 1700 x 40008, 43 and 38; 1.3, 2100 x 1600 x 9000, 45 and 42; 4.4, 8192 x 2048 x
+            // 8800, 138 and 134). After five rounds the power that idle CUs leave to the others is worth as much (5.4, 8192 x 2048 x 11008,
+            // 177 and 177, with a residual 210 and 218).
+            const int64_t cols = large / 256 * 256 / tm * 256, left = a.N - cols;
+            if (large >= 1280 || large % 256 == 0 || cols == 0 || (int64_t)((a.M + 127) / 128) * ((left + 127) / 128) > 512) return tile_t<Large>(a, stream);
+            MxLinearArgs rest = a, most = a;
+            most.N = (int)cols, rest.N = (int)left;
+            rest.w += cols * a.steps * 64, rest.ws += cols * a.steps * 4;
+            rest.out = reinterpret_cast<bf16*>(a.out) + cols;
+            if (a.res) rest.res = reinterpret_cast<const bf16*>(a.res) + cols;
+            const int st = tile_t<Large>(most, stream);
+            return st == M3_OK ? tile_t<Middle>(rest, stream) : st;
         }
     }
     // rows of a block: the fewest with which 256 blocks of 16 columns do (64 x 2112 x 768 3.6, 4.7 and 7.1 us with 16, 32 and 64,
@@ -750,7 +766,7 @@ static int linear_t(const MxLinearArgs& a, hipStream_t stream) {
 static MxLinearArgs linear_args(const void* x, const void* xs, const void* w, const void* ws, const void* res, float scale, void* out,
                                 int m, int n, int k) {
     const auto b = [](const void* p) { return reinterpret_cast<const uint8_t*>(p); };
-    return MxLinearArgs{b(x), b(xs), b(w), b(ws), res, out, scale, m, n, (int)(mx_padded(k) / kMxStep)};
+    return MxLinearArgs{b(x), b(xs), b(w), b(ws), res, out, scale, m, n, (int)(mx_padded(k) / kMxStep), n};
 }
 bool mx_linear_takes_tensor(int64_t m, int64_t n, int64_t k, int x_dtype, int out_dtype, int before) {
     if (m > kMlRawRows || m * mx_padded(k) > (before == kGated ? kMlGatedElements : kMlRawElements)) return false;

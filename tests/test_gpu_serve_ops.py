@@ -598,3 +598,19 @@ def test_add_rms_norm_mx_past_the_largest_number():
     assert past.any() and not past.all()
     v = mamba3_amd.add_rms_norm_mx(x.cuda(), None, w.cuda(), eps=0.0)[1]
     assert torch.equal(v.scales.cpu() == 255, past)  # an infinity makes its block NaN
+
+
+@pytest.mark.parametrize("rows,n,k", [(2100, 9000, 1600), (2100, 9001, 1600), (4000, 4616, 1536), (300, 40008, 1700)])
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+def test_mx_linear_rounds_of_tiles(rows, n, k, fmt):
+    """Sizes whose last columns may go to other tiles than the rest."""
+    x, w = mx_pair(rows, n, k, fmt, 17)
+    a, b = x.dequantize(torch.float32).double(), w.dequantize(torch.float32).double()
+    want, size = a @ b.t(), a.abs() @ b.abs().t()
+    top = lambda v: torch.nn.functional.pad(v.abs(), (0, -k % 128)).unflatten(-1, (-1, 128)).amax(-1)  # noqa: E731
+    off = k * 2.0 ** -24 * size + (2.0 ** -11 * (top(a) @ top(b).t()) if fmt == "e4m3" else 0.0)
+    assert ((mamba3_amd.mx_linear(x, w).double() - want).abs() <= half(torch.bfloat16) * want.abs() + off).all()
+    r = normal((rows, n), 3, torch.bfloat16).cuda()
+    want = r.double() - 0.75 * want
+    assert ((mamba3_amd.mx_linear(x, w, r, -0.75).double() - want).abs()
+            <= half(torch.bfloat16) * want.abs() + 0.75 * off + 2.0 ** -22 * (r.abs().double() + 2 * want.abs())).all()
