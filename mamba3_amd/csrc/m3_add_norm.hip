@@ -59,6 +59,7 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_kernel(AddNormArgs a) {
     __shared__ double red[kAnWaves];
     const int lane = threadIdx.x % kLanes;
     const int d = a.d, units = (kF == kSame ? d + 7 : a.kp) / 8;
+    const double share = 1.0 / d;
     Held8<T> w[kNp];
 #pragma unroll
     for (int p = 0; p < kNp; ++p) w[p].load(reinterpret_cast<const T*>(a.w), (lane + p * kLanes) * 8, d);
@@ -92,7 +93,7 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_kernel(AddNormArgs a) {
                 for (int e = 0; e < 8; ++e) ss = fmaf(t[p][e], t[p][e], ss);
             }
         }
-        const double mean = row_sum<kWpr>(kF != kSame ? squares : (double)ss, red) / d + (double)a.eps;
+        const double mean = row_sum<kWpr>(kF != kSame ? squares : (double)ss, red) * share + (double)a.eps;
         const RowScale r2 = row_scale(mean);
         const float rs = r2.hi;
         if (a.rstd && lane == 0) a.rstd[row] = rs;
@@ -135,7 +136,7 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_wide_kernel(AddNormArgs a
                 sum += (double)ss;
             }
         }
-        const RowScale r2 = row_scale(row_sum<kAnWaves>(sum, red) / d + (double)a.eps);
+        const RowScale r2 = row_scale(row_sum<kAnWaves>(sum, red) * (1.0 / d) + (double)a.eps);
         const float rs = r2.hi;
         if (a.rstd && threadIdx.x == 0) a.rstd[row] = rs;
         for (int unit = threadIdx.x; unit < units; unit += kAnThreads) {

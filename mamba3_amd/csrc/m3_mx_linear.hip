@@ -194,8 +194,8 @@ __global__ __launch_bounds__(kW * 64) void mx_linear_few_kernel(MxLinearArgs a, 
 // m3_add_norm.hip's does: the same sums) or silu(gate) * up.
 constexpr int kMlRawRows = 16;
 // The work that is worth a launch less when every block does it (bf16, us in a graph, one launch against two): quantising
-// 8 x 2112 elements 5.0 against 5.6, 16 x 1536 6.2 against 5.8; gating 4 x 2112 6.1 against 6.5, 8 x 1536 7.0 against 6.5; a norm
-// of 8 rows, one a wave, of 768 4.4 against 5.7, of 2048 6.3 against 8.6.
+// 8 x 2112 elements 5.1 against 5.5, 16 x 1536 6.2 against 5.8; gating 4 x 2112 5.4 against 5.5, 8 x 1536 7.0 against 6.5; a norm
+// of 8 rows, one a wave, of 768 4.9 against 5.6, of 2048 7.4 against 8.5, of 16 rows of 768 7.1 against 5.8.
 constexpr int kMlRawElements = 20480, kMlGatedElements = 10240, kMlNormRows = 8;
 constexpr int kMlNormPieces = 4;    // of 512 columns: a wave's row
 enum { kAsIs, kNormed, kGated };
@@ -226,28 +226,30 @@ __global__ __launch_bounds__(kW * 64) void mx_linear_raw_kernel(MxLinearArgs a, 
         M3_FENCE();
     };
     if constexpr (kPre == kNormed) {
-        T nw[kMlNormPieces][8], tt[kMlNormPieces][8];
+        Held8<T> nw[kMlNormPieces], tt[kMlNormPieces];
 #pragma unroll
         for (int p = 0; p < kMlNormPieces; ++p) {
-            read8(reinterpret_cast<const T*>(a.x) + (int64_t)(wave < a.M ? wave : 0) * k, (lane + p * 64) * 8, k, tt[p]);
-            read8(reinterpret_cast<const T*>(before.norm), (lane + p * 64) * 8, k, nw[p]);
+            tt[p].load(reinterpret_cast<const T*>(a.x) + (int64_t)(wave < a.M ? wave : 0) * k, (lane + p * 64) * 8, k);
+            nw[p].load(reinterpret_cast<const T*>(before.norm), (lane + p * 64) * 8, k);
         }
         ask();
+        const double share = 1.0 / k;  // while they are on their way
         if (const int row = wave; row < a.M) {
             float t[kMlNormPieces][8];
             double squares = 0.0;
 #pragma unroll
             for (int p = 0; p < kMlNormPieces; ++p) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) t[p][e] = (float)tt[p][e];
+                tt[p].values(t[p]);
                 squares = add_squares(squares, t[p]);
             }
-            const RowScale rs = row_scale(wave_sum_f64(squares) / k + (double)before.eps);
+            const RowScale rs = row_scale(wave_sum_f64(squares) * share + (double)before.eps);
 #pragma unroll
             for (int p = 0; p < kMlNormPieces; ++p) {
                 if (lane + p * 64 >= units) continue;
+                float w8[8];
+                nw[p].values(w8);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) t[p][e] = norm_odd(t[p][e], (float)nw[p][e], rs);
+                for (int e = 0; e < 8; ++e) t[p][e] = norm_odd(t[p][e], w8[e], rs);
                 put(t[p], row, lane + p * 64);
             }
         }
