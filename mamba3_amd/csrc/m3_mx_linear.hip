@@ -257,23 +257,20 @@ __global__ __launch_bounds__(kW * 64) void mx_linear_raw_kernel(MxLinearArgs a, 
         // whole groups of four: units come in sixteens
         constexpr int kHalves = kPre == kGated ? 2 : 1;
         const int all = a.M * units;
-        T v[8], u[8];
+        Held8<T> v, u;
         auto read = [&](int i) __attribute__((always_inline)) {
             const int row = i / units, unit = i - row * units;
             const T* x = reinterpret_cast<const T*>(a.x) + (int64_t)row * k * kHalves;
-            read8(x, unit * 8, k, v);
-            if constexpr (kPre == kGated) read8(x + k, unit * 8, k, u);
+            v.load(x, unit * 8, k);
+            if constexpr (kPre == kGated) u.load(x + k, unit * 8, k);
         };
         if ((int)threadIdx.x < all) read(threadIdx.x);
         ask();
         for (int i = threadIdx.x; i < all; i += kW * 64) {
             const int row = i / units, unit = i - row * units;
             float f[8], h[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                f[e] = (float)v[e];
-                if constexpr (kPre == kGated) h[e] = (float)u[e];
-            }
+            v.values(f);
+            if constexpr (kPre == kGated) u.values(h);
             if (i + kW * 64 < all) read(i + kW * 64);
             if constexpr (kPre == kGated) silu_mul8(f, h);
             put(f, row, unit);
