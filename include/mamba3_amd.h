@@ -537,8 +537,8 @@ int m3_mx_linear_exact(int64_t rows, int32_t n, int32_t k, int32_t x_format, con
  *   M3_MX_AS_IS   x [rows, k] as m3_mx_quantize takes it
  *   M3_MX_NORMED  x [rows, k] normed with norm_weight [k] and eps as by m3_add_rmsnorm_mx without a residual
  *   M3_MX_GATED   x [rows, 2 k] as m3_mx_quantize takes it when gated
- * For the sizes for which m3_mx_linear_takes_tensor returns 1 (at most 16 rows of together at most 20480 padded
- * elements, gated 10240, normed at most 8 rows of at most 2048; so few columns that m3_mx_linear takes its kernel for few rows;
+ * For the sizes for which m3_mx_linear_takes_tensor returns 1 (at most 16 rows of together at most 24576 padded
+ * elements, gated 12288, normed at most 8 rows of at most 2048; so few columns that m3_mx_linear takes its kernel for few rows;
  * and normed or gated, out_dtype equal to x_dtype); others are unsupported. norm_weight and eps are read only when normed.
  */
 enum m3_mx_before { M3_MX_AS_IS = 0, M3_MX_NORMED = 1, M3_MX_GATED = 2 };

@@ -182,7 +182,7 @@ def test_mx_linear_tensor_refuses_bad_arguments(lib):
 
     assert go(x=None) == go(w=None) == go(ws=None) == go(out=None) == go(before=1) == 1
     assert go(rows=0) == go(n=0) == go(k=0) == 2
-    assert go(before=3) == go(before=-1) == go(x_dtype=2) == go(out_dtype=2) == go(rows=17) == go(k=5121) == go(n=(1 << 26) + 1) == 3
+    assert go(before=3) == go(before=-1) == go(x_dtype=2) == go(out_dtype=2) == go(rows=17) == go(k=6145) == go(n=(1 << 26) + 1) == 3
     assert go(before=1, norm=FAKE, k=2049) == go(before=1, norm=FAKE, out_dtype=1) == go(before=2, out_dtype=1) == 3
     assert go(x=FAKE + 2) == go(w=FAKE + 8) == go(ws=FAKE + 2) == go(out=FAKE + 2) == go(res=FAKE + 1) == go(before=1, norm=FAKE + 1) == 5
 
