@@ -210,29 +210,48 @@ __device__ __forceinline__ void store_grads(const AddNormBwdArgs& a, int64_t bas
 }
 
 // A block's waves walk rows; each lane adds up dw of its columns, and the waves' sums meet in LDS. bf16 rows
-// wait as they lie in memory, the next one's while this one's are used (16384 x 2048 66 us and 5 for dw; 86 without, fp32, at twice
-// the bytes, 133 as it is; four blocks a CU instead of two made dw's sums longer and nothing shorter).
+// wait as they lie in memory, the next one's while this one's are used, and so do the weights (16384 x 2048 62 us and 5 for dw; 86
+// without; fp32, at twice the bytes, 137).
 template <typename T, int kWpr, int kNp>
 __global__ __launch_bounds__(kAnThreads) void add_norm_bwd_kernel(AddNormBwdArgs a) {
     constexpr int kLanes = kWpr * 64, kRpb = kAnWaves / kWpr;
     __shared__ double red[kAnWaves];
     __shared__ float sum[kWpr == 1 ? kAnWaves * 64 * 8 : 1];
     const int lane = threadIdx.x % kLanes, d = a.d;
-    float w[kNp][8], dw[kNp][8];
+    Held8<T> w[kNp];
+    float dw[kNp][8];
 #pragma unroll
     for (int p = 0; p < kNp; ++p) {
-        load8(reinterpret_cast<const T*>(a.w), (lane + p * kLanes) * 8, d, w[p]);
+        w[p].load(reinterpret_cast<const T*>(a.w), (lane + p * kLanes) * 8, d);
 #pragma unroll
         for (int e = 0; e < 8; ++e) dw[p][e] = 0.f;
     }
     constexpr bool kHalf = sizeof(T) == 2, kAhead = kHalf && kWpr * kNp < 16;  // (more would take more than half the registers)
     u32x4 tr[kNp], gr[kNp], dr[kNp];
     float rr;
+    // A row's last columns, where eight do not divide it, are read from `late` columns before and moved when they are used: a read
+    // of single elements is waited for at once (16384 x 2050 99 us, 89 as it is; 65536 x 500 105 and 75).
+    auto late = [&](int p) __attribute__((always_inline)) {
+        const int c = (lane + p * kLanes) * 8;
+        return c < d && c + 8 > d && d >= 8 ? c + 8 - d : 0;
+    };
+    auto values = [&](u32x4 raw, int p, float (&v)[8]) __attribute__((always_inline)) {
+        if (const int by = late(p)) {
+            // down by so many halves
+            if (by & 4) raw = u32x4{raw[2], raw[3], 0, 0};
+            if (by & 2) raw = u32x4{raw[1], raw[2], raw[3], 0};
+            if (by & 1) {
+                const unsigned a = raw[0], b = raw[1], c = raw[2], e = raw[3];
+                raw = u32x4{a >> 16 | b << 16, b >> 16 | c << 16, c >> 16 | e << 16, e >> 16};
+            }
+        }
+        values8(raw, v);
+    };
     auto read = [&](int64_t row) __attribute__((always_inline)) {
         const int64_t base = row * d;
 #pragma unroll
         for (int p = 0; p < kNp; ++p) {
-            const int c = (lane + p * kLanes) * 8;
+            const int c = (lane + p * kLanes) * 8 - late(p);
             tr[p] = raw8(reinterpret_cast<const bf16*>(a.t) + base, c, d);
             gr[p] = raw8(reinterpret_cast<const bf16*>(a.dy) + base, c, d);
             dr[p] = a.dtotal ? raw8(reinterpret_cast<const bf16*>(a.dtotal) + base, c, d) : u32x4{0, 0, 0, 0};
@@ -248,7 +267,7 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_bwd_kernel(AddNormBwdArgs
         if constexpr (kHalf) {
             if constexpr (!kAhead) read(row);
 #pragma unroll
-            for (int p = 0; p < kNp; ++p) values8(tr[p], t[p]), values8(gr[p], g[p]), values8(dr[p], dt[p]);
+            for (int p = 0; p < kNp; ++p) values(tr[p], p, t[p]), values(gr[p], p, g[p]), values(dr[p], p, dt[p]);
         } else {
 #pragma unroll
             for (int p = 0; p < kNp; ++p) {
@@ -268,13 +287,16 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_bwd_kernel(AddNormBwdArgs
         if (kAhead && row + step < a.rows) read(row + step);
         float dot = 0.f;
 #pragma unroll
-        for (int p = 0; p < kNp; ++p)
+        for (int p = 0; p < kNp; ++p) {
+            float w8[8];
+            w[p].values(w8);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 dw[p][e] = fmaf(g[p][e], t[p][e] * rs, dw[p][e]);
-                g[p][e] *= w[p][e];
+                g[p][e] *= w8[e];
                 dot = fmaf(g[p][e], t[p][e], dot);
             }
+        }
         const float mean = (float)(row_sum<kWpr>((double)dot, red) / d * (double)rs * (double)rs);
 #pragma unroll
         for (int p = 0; p < kNp; ++p) {
@@ -374,10 +396,12 @@ __global__ __launch_bounds__(1024) void add_norm_dw_kernel(const float* __restri
     }
 }
 
-constexpr int64_t kAnParts = 512;  // blocks of the backward: two a CU
-constexpr int kAnNarrow = 8192;    // columns that stay in registers
+constexpr int kAnNarrow = 8192;  // columns that stay in registers
+// Blocks of the backward: as many as run at once, by the registers that a row's pieces take (65536 x 768 122 us with two a CU, 103
+// with three, 133 with four; 16384 x 2048 67 with two).
 static int64_t add_norm_parts(int64_t rows, int d) {
-    return std::min(kAnParts, d <= 2048 ? (rows + kAnWaves - 1) / kAnWaves : rows);
+    const int64_t most = 256 * (d <= 512 ? 4 : d <= 1024 ? 3 : d > 2048 && d <= 4096 ? 3 : 2);
+    return std::min(most, d <= 2048 ? (rows + kAnWaves - 1) / kAnWaves : rows);
 }
 size_t add_norm_bwd_workspace(int64_t rows, int d) { return (size_t)add_norm_parts(rows, d) * d * sizeof(float); }
 

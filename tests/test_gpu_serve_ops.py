@@ -199,6 +199,28 @@ def test_add_rms_norm(rows, d, dtype):
     assert ((grads[2].cpu().double() - dw).abs() <= half(dtype) * dw.abs() + (small + rows * 2.0 ** -24) * parts.abs().sum(0)).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,d", [(9001, 41), (9002, 42), (9003, 43), (9004, 44), (9005, 45), (9006, 46), (9007, 47), (8300, 513),
+                                    (4999, 767), (4100, 1027), (1700, 2051), (1601, 4094), (1100, 4099), (1050, 8190)])
+def test_add_rms_norm_gradients_of_more_rows_than_run_at_once(rows, d, dtype):
+    x, r, w = normal((rows, d), 1, dtype).cuda(), normal((rows, d), 2, dtype, 3.0).cuda(), normal((d,), 3, dtype).cuda()
+    dt, dy = normal((rows, d), 4, dtype).cuda(), normal((rows, d), 5, dtype).cuda()
+    ins = [t.requires_grad_() for t in (x, r, w)]
+    total, y = mamba3_amd.add_rms_norm(*ins, 0.3, 1e-5)
+    dx, dr, dw = torch.autograd.grad([total, y], ins, [dt, dy])
+    t, w64, dy64, dt64 = total.detach().double(), w.detach().double(), dy.double(), dt.double()
+    rs = 1 / torch.sqrt(t.square().mean(1, keepdim=True) + 1e-5)
+    g = dy64 * w64
+    d64 = dt64 + rs * g - t * rs ** 3 * (g * t).sum(1, keepdim=True) / d
+    size = dt64.abs() + rs * g.abs() + t.abs() * rs ** 3 * (g * t).abs().sum(1, keepdim=True) / d
+    small = 2.0 ** -20  # fp32 sums and products
+    for got, s in ((dr, 1.0), (dx, 0.3)):
+        assert ((got.double() - s * d64).abs() <= half(dtype) * (s * d64).abs() + small * s * size).all()
+    parts = dy64 * t * rs
+    want = parts.sum(0)
+    assert ((dw.double() - want).abs() <= half(dtype) * want.abs() + (small + rows * 2.0 ** -24) * parts.abs().sum(0)).all()
+
+
 @pytest.mark.parametrize("which", ["total", "y", "x", "residual", "weight"])
 def test_add_rms_norm_one_result_or_one_gradient(which):
     x, r, w = (normal(s, i, torch.float32).cuda() for i, s in enumerate([(3, 70), (3, 70), (70,)]))
