@@ -66,7 +66,7 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_kernel(AddNormArgs a) {
     for (int64_t row = (int64_t)blockIdx.x * kRpb + threadIdx.x / kLanes; row < a.rows; row += (int64_t)gridDim.x * kRpb) {
         const int64_t base = row * d;
         float t[kNp][8];
-        Held8<T> x[kNp], r[kRes ? kNp : 1];
+        Held8<T, kF == kSame> x[kNp], r[kRes ? kNp : 1];
 #pragma unroll
         for (int p = 0; p < kNp; ++p) {
             const int c = (lane + p * kLanes) * 8;
@@ -229,29 +229,11 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_bwd_kernel(AddNormBwdArgs
     constexpr bool kHalf = sizeof(T) == 2, kAhead = kHalf && kWpr * kNp < 16;  // (more would take more than half the registers)
     u32x4 tr[kNp], gr[kNp], dr[kNp];
     float rr;
-    // A row's last columns, where eight do not divide it, are read from `late` columns before and moved when they are used: a read
-    // of single elements is waited for at once (16384 x 2050 99 us, 89 as it is; 65536 x 500 105 and 75).
-    auto late = [&](int p) __attribute__((always_inline)) {
-        const int c = (lane + p * kLanes) * 8;
-        return c < d && c + 8 > d && d >= 8 ? c + 8 - d : 0;
-    };
-    auto values = [&](u32x4 raw, int p, float (&v)[8]) __attribute__((always_inline)) {
-        if (const int by = late(p)) {
-            // down by so many halves
-            if (by & 4) raw = u32x4{raw[2], raw[3], 0, 0};
-            if (by & 2) raw = u32x4{raw[1], raw[2], raw[3], 0};
-            if (by & 1) {
-                const unsigned a = raw[0], b = raw[1], c = raw[2], e = raw[3];
-                raw = u32x4{a >> 16 | b << 16, b >> 16 | c << 16, c >> 16 | e << 16, e >> 16};
-            }
-        }
-        values8(raw, v);
-    };
     auto read = [&](int64_t row) __attribute__((always_inline)) {
         const int64_t base = row * d;
 #pragma unroll
         for (int p = 0; p < kNp; ++p) {
-            const int c = (lane + p * kLanes) * 8 - late(p);
+            const int c0 = (lane + p * kLanes) * 8, c = c0 - late8(c0, d);
             tr[p] = raw8(reinterpret_cast<const bf16*>(a.t) + base, c, d);
             gr[p] = raw8(reinterpret_cast<const bf16*>(a.dy) + base, c, d);
             dr[p] = a.dtotal ? raw8(reinterpret_cast<const bf16*>(a.dtotal) + base, c, d) : u32x4{0, 0, 0, 0};
@@ -267,7 +249,10 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_bwd_kernel(AddNormBwdArgs
         if constexpr (kHalf) {
             if constexpr (!kAhead) read(row);
 #pragma unroll
-            for (int p = 0; p < kNp; ++p) values(tr[p], p, t[p]), values(gr[p], p, g[p]), values(dr[p], p, dt[p]);
+            for (int p = 0; p < kNp; ++p) {
+                const int late = late8((lane + p * kLanes) * 8, d);
+                values8_late(tr[p], late, t[p]), values8_late(gr[p], late, g[p]), values8_late(dr[p], late, dt[p]);
+            }
         } else {
 #pragma unroll
             for (int p = 0; p < kNp; ++p) {

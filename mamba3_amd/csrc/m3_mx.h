@@ -180,18 +180,34 @@ __device__ __forceinline__ void values8(const u32x4& r, float (&v)[8]) {
         v[e] = __builtin_bit_cast(float, e % 2 ? w & 0xffff0000u : w << 16);
     }
 }
-// Eight elements that stay in registers: bf16 in half as many.
-template <typename T> struct Held8;
-template <> struct Held8<bf16> {
+// A row's last columns, where eight do not divide it, are read from late8 columns before and moved by values8_late when they are
+// used: a read of single elements is waited for at once (the norm's backward, 16384 x 2050: 99 us, 89 as it is).
+__device__ __forceinline__ int late8(int c, int n) { return c < n && c + 8 > n && n >= 8 ? c + 8 - n : 0; }
+__device__ __forceinline__ void values8_late(u32x4 r, int late, float (&v)[8]) {
+    if (late) {  // down by so many halves
+        if (late & 4) r = u32x4{r[2], r[3], 0, 0};
+        if (late & 2) r = u32x4{r[1], r[2], r[3], 0};
+        if (late & 1) r = u32x4{r[0] >> 16 | r[1] << 16, r[1] >> 16 | r[2] << 16, r[2] >> 16 | r[3] << 16, r[3] >> 16};
+    }
+    values8(r, v);
+}
+// Eight elements that stay in registers: bf16 in half as many. kLate: read late8 columns before (the norm, 16384 x 2050: 67 us, 58
+// with it; to microscaled values it stays off, whose registers it takes: 4096 x 8192 43 and 51).
+template <typename T, bool kLate = false> struct Held8;
+template <bool kLate> struct Held8<bf16, kLate> {
     u32x4 raw;
-    __device__ __forceinline__ void load(const bf16* row, int c, int n) { raw = raw8(row, c, n); }
+    int late;
+    __device__ __forceinline__ void load(const bf16* row, int c, int n) {
+        late = kLate ? late8(c, n) : 0;
+        raw = raw8(row, c - late, n);
+    }
     __device__ __forceinline__ void values(float (&v)[8]) const {
         u32x4 r = raw;
         asm volatile("" : "+v"(r));  // not hoisted out of a loop, where the values would be held after all
-        values8(r, v);
+        values8_late(r, kLate ? late : 0, v);
     }
 };
-template <> struct Held8<float> {
+template <bool kLate> struct Held8<float, kLate> {
     float raw[8];
     __device__ __forceinline__ void load(const float* row, int c, int n) { load8(row, c, n, raw); }
     __device__ __forceinline__ void values(float (&v)[8]) const {

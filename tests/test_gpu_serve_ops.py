@@ -202,7 +202,7 @@ def test_add_rms_norm(rows, d, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,d", [(9001, 41), (9002, 42), (9003, 43), (9004, 44), (9005, 45), (9006, 46), (9007, 47), (8300, 513),
                                     (4999, 767), (4100, 1027), (1700, 2051), (1601, 4094), (1100, 4099), (1050, 8190)])
-def test_add_rms_norm_gradients_of_more_rows_than_run_at_once(rows, d, dtype):
+def test_add_rms_norm_of_more_rows_than_run_at_once(rows, d, dtype):
     x, r, w = normal((rows, d), 1, dtype).cuda(), normal((rows, d), 2, dtype, 3.0).cuda(), normal((d,), 3, dtype).cuda()
     dt, dy = normal((rows, d), 4, dtype).cuda(), normal((rows, d), 5, dtype).cuda()
     ins = [t.requires_grad_() for t in (x, r, w)]
@@ -210,6 +210,10 @@ def test_add_rms_norm_gradients_of_more_rows_than_run_at_once(rows, d, dtype):
     dx, dr, dw = torch.autograd.grad([total, y], ins, [dt, dy])
     t, w64, dy64, dt64 = total.detach().double(), w.detach().double(), dy.double(), dt.double()
     rs = 1 / torch.sqrt(t.square().mean(1, keepdim=True) + 1e-5)
+    sum64 = r.detach().double() + 0.3 * x.detach().double()
+    assert ((t - sum64).abs() <= half(dtype) * sum64.abs() + 2.0 ** -22 * (r.detach().abs() + x.detach().abs()).double()).all()
+    y64 = t * rs * w64
+    assert ((y.detach().double() - y64).abs() <= (half(dtype) + 2.0 ** -20) * y64.abs()).all()
     g = dy64 * w64
     d64 = dt64 + rs * g - t * rs ** 3 * (g * t).sum(1, keepdim=True) / d
     size = dt64.abs() + rs * g.abs() + t.abs() * rs ** 3 * (g * t).abs().sum(1, keepdim=True) / d
