@@ -212,11 +212,11 @@ __device__ __forceinline__ void store_grads(const AddNormBwdArgs& a, int64_t bas
 // A block's waves walk rows; each lane adds up dw of its columns, and the waves' sums meet in LDS. bf16 rows
 // wait as they lie in memory, the next one's while this one's are used, and so do the weights (16384 x 2048 62 us and 5 for dw; 86
 // without; fp32, at twice the bytes, 137).
-template <typename T, int kWpr, int kNp>
-__global__ __launch_bounds__(kAnThreads) void add_norm_bwd_kernel(AddNormBwdArgs a) {
-    constexpr int kLanes = kWpr * 64, kRpb = kAnWaves / kWpr;
-    __shared__ double red[kAnWaves];
-    __shared__ float sum[kWpr == 1 ? kAnWaves * 64 * 8 : 1];
+template <typename T, int kWaves, int kWpr, int kNp>
+__global__ __launch_bounds__(kWaves * 64) void add_norm_bwd_kernel(AddNormBwdArgs a) {
+    constexpr int kLanes = kWpr * 64, kRpb = kWaves / kWpr;
+    __shared__ double red[kWaves];
+    __shared__ float sum[kWpr == 1 ? kWaves * 64 * 8 : 1];
     const int lane = threadIdx.x % kLanes, d = a.d;
     Held8<T> w[kNp];
     float dw[kNp][8];
@@ -300,10 +300,10 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_bwd_kernel(AddNormBwdArgs
             __syncthreads();
             store8(sum + (threadIdx.x >> 6) * 512, lane * 8, 512, dw[p]);
             __syncthreads();
-            for (int c = threadIdx.x; c < 512; c += kAnThreads) {
+            for (int c = threadIdx.x; c < 512; c += kWaves * 64) {
                 float v = sum[c];
 #pragma unroll
-                for (int i = 1; i < kAnWaves; ++i) v += sum[i * 512 + c];
+                for (int i = 1; i < kWaves; ++i) v += sum[i * 512 + c];
                 if (p * 512 + c < d) out[p * 512 + c] = v;
             }
         } else {
@@ -382,26 +382,28 @@ __global__ __launch_bounds__(1024) void add_norm_dw_kernel(const float* __restri
 }
 
 constexpr int kAnNarrow = 8192;  // columns that stay in registers
-// Blocks of the backward: as many as run at once, by the registers that a row's pieces take (65536 x 768 122 us with two a CU, 103
-// with three, 133 with four; 16384 x 2048 67 with two).
+// Blocks of the backward: as many waves as run at once by the registers that a row's pieces take (65536 x 768: eight waves a CU
+// 122 us, twelve 106), in few blocks, since each has its line in dw's sum (32768 x 512: four waves a block 34.4, eight 32.4).
+static int add_norm_bwd_waves(int d) { return d <= 512 ? 8 : d <= 1024 ? 12 : 4; }
 static int64_t add_norm_parts(int64_t rows, int d) {
-    const int64_t most = 256 * (d <= 512 ? 4 : d <= 1024 ? 3 : d > 2048 && d <= 4096 ? 3 : 2);
-    return std::min(most, d <= 2048 ? (rows + kAnWaves - 1) / kAnWaves : rows);
+    const int waves = add_norm_bwd_waves(d);
+    if (d <= 1024) return std::min<int64_t>(d <= 512 ? 512 : 256, (rows + waves - 1) / waves);
+    return d <= 2048 ? std::min<int64_t>(512, (rows + waves - 1) / waves) : std::min<int64_t>(d <= 4096 ? 768 : 512, rows);
 }
 size_t add_norm_bwd_workspace(int64_t rows, int d) { return (size_t)add_norm_parts(rows, d) * d * sizeof(float); }
 
 template <typename T>
 static int add_norm_bwd_t(AddNormBwdArgs a, void* dw, hipStream_t stream) {
     const int64_t parts = add_norm_parts(a.rows, a.d);
-    const dim3 grid((unsigned)parts), block(kAnThreads);
-    if (a.d <= 512) hipLaunchKernelGGL((add_norm_bwd_kernel<T, 1, 1>), grid, block, 0, stream, a);
-    else if (a.d <= 1024) hipLaunchKernelGGL((add_norm_bwd_kernel<T, 1, 2>), grid, block, 0, stream, a);
-    else if (a.d <= 2048) hipLaunchKernelGGL((add_norm_bwd_kernel<T, 1, 4>), grid, block, 0, stream, a);
-    else if (a.d <= 4096) hipLaunchKernelGGL((add_norm_bwd_kernel<T, 4, 2>), grid, block, 0, stream, a);
-    else if (a.d <= kAnNarrow) hipLaunchKernelGGL((add_norm_bwd_kernel<T, 4, 4>), grid, block, 0, stream, a);
+    const dim3 grid((unsigned)parts), block(64 * add_norm_bwd_waves(a.d));
+    if (a.d <= 512) hipLaunchKernelGGL((add_norm_bwd_kernel<T, 8, 1, 1>), grid, block, 0, stream, a);
+    else if (a.d <= 1024) hipLaunchKernelGGL((add_norm_bwd_kernel<T, 12, 1, 2>), grid, block, 0, stream, a);
+    else if (a.d <= 2048) hipLaunchKernelGGL((add_norm_bwd_kernel<T, 4, 1, 4>), grid, block, 0, stream, a);
+    else if (a.d <= 4096) hipLaunchKernelGGL((add_norm_bwd_kernel<T, 4, 4, 2>), grid, block, 0, stream, a);
+    else if (a.d <= kAnNarrow) hipLaunchKernelGGL((add_norm_bwd_kernel<T, 4, 4, 4>), grid, block, 0, stream, a);
     else {
         if (a.dx || a.dres)
-            hipLaunchKernelGGL((add_norm_bwd_wide_kernel<T>), dim3((unsigned)std::min(a.rows, kAnMaxBlocks)), block, 0, stream, a);
+            hipLaunchKernelGGL((add_norm_bwd_wide_kernel<T>), dim3((unsigned)std::min(a.rows, kAnMaxBlocks)), dim3(kAnThreads), 0, stream, a);
         if (dw) {
             const int64_t each = (a.rows + parts - 1) / parts;
             hipLaunchKernelGGL((add_norm_dw_wide_kernel<T>), dim3((unsigned)((a.d + 511) / 512), (unsigned)parts), dim3(64), 0, stream, a, each);
