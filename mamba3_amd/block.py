@@ -10,6 +10,7 @@ equal the reference's so seeded models hold identical weights.
 from __future__ import annotations
 
 import math
+import weakref
 
 import torch
 import torch.nn as nn
@@ -59,26 +60,46 @@ def _only_weight(lin: nn.Module) -> bool:
     return _as_written(lin, nn.Linear) and lin.bias is None
 
 
-def _mx_copy(owner: nn.Module, name: str, *weights: torch.Tensor) -> MXTensor:
+class _MXCopy:
+    """The 4-bit copy of some weights, and which weights at which versions. It holds on to their memory, so that an address is not
+    another weight's as long as it is compared; their objects are compared too, since a new parameter of the same memory counts
+    its versions anew. Copied or pickled it is empty: the other module's weights are others."""
+
+    __slots__ = ("mx", "of", "key", "memory")
+
+    def __init__(self, mx: MXTensor | None = None, weights: tuple[torch.Tensor, ...] = ()):
+        self.mx, self.key = mx, self._key(weights)
+        self.of, self.memory = [weakref.ref(w) for w in weights], [w.detach() for w in weights]
+
+    def __reduce__(self):
+        return _MXCopy, ()
+
+    @staticmethod
+    def _key(weights: tuple[torch.Tensor, ...]) -> list[tuple]:
+        return [(w.data_ptr(), 0 if w.is_inference() else w._version, w.dtype, w.device) for w in weights]
+
+    def is_of(self, weights: tuple[torch.Tensor, ...]) -> bool:
+        return len(self.of) == len(weights) and all(r() is w for r, w in zip(self.of, weights)) and self.key == self._key(weights)
+
+
+def _mx_copy(owner: nn.Module, *weights: torch.Tensor) -> MXTensor:
     """The 4-bit copy of the weights, one below the other, that `owner` keeps: made when first asked for and again after one
     was replaced or changed in place (which their version counters tell), into the same memory where it fits, so that graphs
-    captured with the copy go on with the new weights. The copy holds on to the weights' memory, so an address is not another
-    weight's as long as it is compared."""
-    key = tuple((w.data_ptr(), 0 if w.is_inference() else w._version, w.dtype, w.device) for w in weights)
-    kept = owner.__dict__.get(name)
-    if kept is None or kept[0] != key:
+    captured with the copy go on with the new weights."""
+    kept = owner.__dict__.get("_mx")
+    if kept is None or not kept.is_of(weights):
         if weights[0].is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a graph is being captured and the 4-bit weights are not there yet: run the model once before")
         with torch.inference_mode(False), torch.no_grad():  # copies outlive the mode that they are made in
             mx = quantize_mx(weights[0] if len(weights) == 1 else torch.cat(weights))
-            if kept is not None and kept[1].shape == mx.shape and kept[1].device == mx.device:
-                kept[1].data.copy_(mx.data)
-                kept[1].scales.copy_(mx.scales)
-                mx = kept[1]
+            if kept is not None and kept.mx is not None and kept.mx.shape == mx.shape and kept.mx.device == mx.device:
+                kept.mx.data.copy_(mx.data)
+                kept.mx.scales.copy_(mx.scales)
+                mx = kept.mx
         # from here on any stream may read them
         torch.cuda.current_stream(mx.device).synchronize()
-        kept = owner.__dict__[name] = (key, mx, [w.detach() for w in weights])
-    return kept[1]
+        kept = owner.__dict__["_mx"] = _MXCopy(mx, weights)
+    return kept.mx
 
 
 class SwiGLU(nn.Module):
@@ -189,8 +210,8 @@ class KulaMambaBlock(nn.Module):
             raise RuntimeError("4-bit weights need projections without bias and norms of the last dimension, without hooks or forwards of "
                                "their own")
         w = [lin.weight for lin in lins]
-        copies = (_mx_copy(lins[0], "_mx", w[0]), _mx_copy(lins[1], "_mx", w[1]))
-        return copies if not self.use_mlp else (*copies, _mx_copy(self.mlp, "_mx", w[2], w[3]), _mx_copy(lins[4], "_mx", w[4]))
+        copies = (_mx_copy(lins[0], w[0]), _mx_copy(lins[1], w[1]))
+        return copies if not self.use_mlp else (*copies, _mx_copy(self.mlp, w[2], w[3]), _mx_copy(lins[4], w[4]))
 
     def _mx_on(self) -> bool:
         return self.mx_weights and not torch.is_grad_enabled()
@@ -403,7 +424,7 @@ class KulaMambaLM(nn.Module):
     def _mx_head(self) -> MXTensor:
         if not (_only_weight(self.lm_head) and _as_written(self.norm, RMSNorm) and self.norm.dim == -1):
             raise RuntimeError("4-bit weights need a head without bias and a norm of the last dimension, without hooks or forwards of their own")
-        return _mx_copy(self.lm_head, "_mx", self.lm_head.weight)
+        return _mx_copy(self.lm_head, self.lm_head.weight)
 
     @torch.compiler.disable
     def _mx_logits(self, x: torch.Tensor) -> torch.Tensor:

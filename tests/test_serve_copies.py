@@ -1,0 +1,94 @@
+"""When the language model makes its 4-bit copies of the weights anew, and into which memory: on the host, with a quantisation
+that keeps the weights' numbers and a GPU that notes what it is asked."""
+
+from __future__ import annotations
+
+import copy
+import pickle
+
+import pytest
+import torch
+from torch import nn
+
+from mamba3_amd import MXTensor, block
+
+def kept_numbers(w, format="e2m1"):
+    rows, k = w.shape
+    data = torch.zeros(rows, -(-k // 128) * 64, dtype=torch.uint8)
+    data[:, :k] = w.to(torch.uint8)
+    return MXTensor(data, torch.full((rows, -(-k // 128) * 4), 127, dtype=torch.uint8), (rows, k), format)
+
+
+class Gpu:
+    """What _mx_copy asks of torch.cuda."""
+
+    def __init__(self):
+        self.asked, self.capturing = [], False
+
+    def current_stream(self, device=None):
+        return self
+
+    def synchronize(self, device=None):
+        self.asked.append("wait")
+
+    def is_current_stream_capturing(self):
+        return self.capturing
+
+
+@pytest.fixture
+def gpu(monkeypatch):
+    gpu = Gpu()
+    monkeypatch.setattr(block, "quantize_mx", kept_numbers)
+    for name in ("current_stream", "synchronize", "is_current_stream_capturing"):
+        monkeypatch.setattr(torch.cuda, name, getattr(gpu, name))
+    return gpu
+
+
+def linear(start=0, rows=3, k=20):
+    lin = nn.Linear(k, rows, bias=False)
+    with torch.no_grad():
+        lin.weight.copy_((torch.arange(rows * k) + start).view(rows, k))
+    return lin
+
+
+def get(lin):
+    return block._mx_copy(lin, lin.weight)
+
+
+def fresh(lin):
+    return torch.equal(get(lin).data, kept_numbers(lin.weight.detach()).data)
+
+
+@torch.no_grad()
+def test_a_copy_follows_a_new_parameter_of_the_same_memory(gpu):
+    """It counts its versions anew, so that address and version are the old parameter's while the numbers are others."""
+    lin = linear()
+    assert fresh(lin)
+    old = lin.weight
+    lin.weight = nn.Parameter(old.data)
+    assert lin.weight._version < old._version and lin.weight.data_ptr() == old.data_ptr()
+    while lin.weight._version < old._version:
+        lin.weight.add_(1.0)
+    assert fresh(lin)
+    lin.weight.add_(1.0)
+    assert fresh(lin)
+
+
+@torch.no_grad()
+def test_a_copied_or_pickled_module_makes_its_own(gpu):
+    lin = linear()
+    mine = get(lin)
+    for other in (copy.deepcopy(lin), pickle.loads(pickle.dumps(lin))):
+        assert fresh(other) and get(other).data.data_ptr() != mine.data.data_ptr()
+        other.weight.add_(5.0)
+        assert fresh(other) and fresh(lin) and get(lin) is mine
+
+
+@torch.no_grad()
+def test_a_copy_is_made_once(gpu):
+    lin = linear()
+    first = get(lin)
+    waits = len(gpu.asked)
+    assert all(get(lin) is first for _ in range(3)) and len(gpu.asked) == waits
+    lin.to(torch.bfloat16)
+    assert fresh(lin)
