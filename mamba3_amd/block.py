@@ -76,7 +76,7 @@ class _MXCopy:
 
     @staticmethod
     def _key(weights: tuple[torch.Tensor, ...]) -> list[tuple]:
-        return [(w.data_ptr(), 0 if w.is_inference() else w._version, w.dtype, w.device) for w in weights]
+        return [(w.data_ptr(), w._version, w.dtype, w.device) for w in weights]
 
     def is_of(self, weights: tuple[torch.Tensor, ...]) -> bool:
         return len(self.of) == len(weights) and all(r() is w for r, w in zip(self.of, weights)) and self.key == self._key(weights)
@@ -88,6 +88,9 @@ def _mx_copy(owner: nn.Module, *weights: torch.Tensor) -> MXTensor:
     captured with the copy go on with the new weights."""
     kept = owner.__dict__.get("_mx")
     if kept is None or not kept.is_of(weights):
+        if any(w.is_inference() for w in weights):
+            raise RuntimeError("4-bit weights need parameters that count their changes; those made in torch.inference_mode() do not: make or load "
+                               "the model outside of it")
         if weights[0].is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a graph is being captured and the 4-bit weights are not there yet: run the model once before")
         with torch.inference_mode(False), torch.no_grad():  # copies outlive the mode that they are made in
@@ -401,7 +404,8 @@ class KulaMambaLM(nn.Module):
         """Switches products without gradients (generate, and forward, loss, prefill and step under torch.no_grad()) to 4-bit
         copies of the weights and activations in 8 bits, both microscaled (quantize_mx, mx_linear), or back and frees
         the copies. Gradients and the embedding use the weights themselves, which stay. A copy is made anew when its weight was
-        replaced or changed in place; after changes through `.data`, which leave no trace, call this again. Needs projections
+        replaced or changed in place; after changes that leave no trace (through `.data`, or by a graph's replay, as of a captured
+        optimizer step), call this again. Weights made in torch.inference_mode() count no changes and are refused. Needs projections
         without bias."""
         for m in self.modules():
             m.__dict__.pop("_mx", None)

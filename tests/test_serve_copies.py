@@ -92,3 +92,21 @@ def test_a_copy_is_made_once(gpu):
     assert all(get(lin) is first for _ in range(3)) and len(gpu.asked) == waits
     lin.to(torch.bfloat16)
     assert fresh(lin)
+
+
+def test_weights_that_do_not_count_their_changes_are_refused(gpu):
+    with torch.inference_mode():
+        made = linear()
+        with pytest.raises(RuntimeError, match="inference_mode"):
+            get(made)
+    with pytest.raises(RuntimeError, match="inference_mode"):
+        get(made)
+    lin = linear()
+    first = get(lin)
+    with torch.inference_mode():  # the mode itself is no matter: other parameters count their changes in it
+        assert get(lin) is first
+        lin.weight.add_(3.0)
+        assert fresh(lin)
+        lin.weight = nn.Parameter(lin.weight + 1)
+        with pytest.raises(RuntimeError, match="inference_mode"):
+            get(lin)
