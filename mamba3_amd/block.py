@@ -82,12 +82,12 @@ class _MXCopy:
         return len(self.of) == len(weights) and all(r() is w for r, w in zip(self.of, weights)) and self.key == self._key(weights)
 
 
-def _mx_copy(owner: nn.Module, *weights: torch.Tensor) -> MXTensor:
+def _mx_copy(owner: nn.Module, *weights: torch.Tensor, anew: bool = False) -> MXTensor:
     """The 4-bit copy of the weights, one below the other, that `owner` keeps: made when first asked for and again after one
-    was replaced or changed in place (which their version counters tell), into the same memory where it fits, so that graphs
-    captured with the copy go on with the new weights."""
+    was replaced or changed in place (which their version counters tell) or when asked for `anew`, into the same memory where it
+    fits, so that graphs captured with the copy go on with the new weights."""
     kept = owner.__dict__.get("_mx")
-    if kept is None or not kept.is_of(weights):
+    if kept is None or anew or not kept.is_of(weights):
         if any(w.is_inference() for w in weights):
             raise RuntimeError("4-bit weights need parameters that count their changes; those made in torch.inference_mode() do not: make or load "
                                "the model outside of it")
@@ -200,7 +200,7 @@ class KulaMambaBlock(nn.Module):
     # Without gradients, multiply by 4-bit copies of the weights (KulaMambaLM.quantize_mx). Off by default.
     mx_weights: bool = False
 
-    def _mx_projections(self) -> tuple[MXTensor, ...]:
+    def _mx_projections(self, anew: bool = False) -> tuple[MXTensor, ...]:
         """in_proj, out_proj and with an MLP [w_gate; w_up] and w_down in 4 bits."""
         lins = [self.ssm.in_proj, self.ssm.out_proj]
         whole = isinstance(self.ssm, KulaMamba) and _as_written(self.ssm_norm, RMSNorm) and self.ssm_norm.dim == -1
@@ -213,8 +213,8 @@ class KulaMambaBlock(nn.Module):
             raise RuntimeError("4-bit weights need projections without bias and norms of the last dimension, without hooks or forwards of "
                                "their own")
         w = [lin.weight for lin in lins]
-        copies = (_mx_copy(lins[0], w[0]), _mx_copy(lins[1], w[1]))
-        return copies if not self.use_mlp else (*copies, _mx_copy(self.mlp, w[2], w[3]), _mx_copy(lins[4], w[4]))
+        copies = (_mx_copy(lins[0], w[0], anew=anew), _mx_copy(lins[1], w[1], anew=anew))
+        return copies if not self.use_mlp else (*copies, _mx_copy(self.mlp, w[2], w[3], anew=anew), _mx_copy(lins[4], w[4], anew=anew))
 
     def _mx_on(self) -> bool:
         return self.mx_weights and not torch.is_grad_enabled()
@@ -403,32 +403,35 @@ class KulaMambaLM(nn.Module):
     def quantize_mx(self, on: bool = True) -> "KulaMambaLM":
         """Switches products without gradients (generate, and forward, loss, prefill and step under torch.no_grad()) to 4-bit
         copies of the weights and activations in 8 bits, both microscaled (quantize_mx, mx_linear), or back and frees
-        the copies. Gradients and the embedding use the weights themselves, which stay. A copy is made anew when its weight was
-        replaced or changed in place; after changes that leave no trace (through `.data`, or by a graph's replay, as of a captured
-        optimizer step), call this again. Weights made in torch.inference_mode() count no changes and are refused. Needs projections
-        without bias."""
-        for m in self.modules():
-            m.__dict__.pop("_mx", None)
-        self.mx_weights = on
-        for layer in self.layers:
-            layer.mx_weights = on
+        the copies: graphs captured with them are not to be replayed after that. Gradients and the embedding use the weights
+        themselves, which stay. A copy is made anew when the model runs and its weight was replaced or changed in place; after changes
+        that leave no trace (through `.data`, or by a graph's replay, as of a captured optimizer step), call this again. Either way it
+        stays in its memory, where captured graphs find it. Weights made in torch.inference_mode() count no changes and are
+        refused. Needs projections without bias."""
         if on:
             try:
                 for layer in self.layers:
-                    layer._mx_projections()
-                self._mx_head()
+                    layer._mx_projections(anew=True)
+                self._mx_head(anew=True)
             except Exception:
-                self.quantize_mx(False)
+                if not self.mx_weights:
+                    self.quantize_mx(False)
                 raise
+        else:
+            for m in self.modules():
+                m.__dict__.pop("_mx", None)
+        self.mx_weights = on
+        for layer in self.layers:
+            layer.mx_weights = on
         return self
 
     def _mx_on(self) -> bool:
         return self.mx_weights and not torch.is_grad_enabled()
 
-    def _mx_head(self) -> MXTensor:
+    def _mx_head(self, anew: bool = False) -> MXTensor:
         if not (_only_weight(self.lm_head) and _as_written(self.norm, RMSNorm) and self.norm.dim == -1):
             raise RuntimeError("4-bit weights need a head without bias and a norm of the last dimension, without hooks or forwards of their own")
-        return _mx_copy(self.lm_head, self.lm_head.weight)
+        return _mx_copy(self.lm_head, self.lm_head.weight, anew=anew)
 
     @torch.compiler.disable
     def _mx_logits(self, x: torch.Tensor) -> torch.Tensor:

@@ -10,12 +10,13 @@ import pytest
 import torch
 from torch import nn
 
-from mamba3_amd import MXTensor, block
+from mamba3_amd import KulaMambaLM, MXTensor, block
+
 
 def kept_numbers(w, format="e2m1"):
     rows, k = w.shape
     data = torch.zeros(rows, -(-k // 128) * 64, dtype=torch.uint8)
-    data[:, :k] = w.to(torch.uint8)
+    data[:, :k] = w[:, :data.shape[1]].to(torch.uint8)
     return MXTensor(data, torch.full((rows, -(-k // 128) * 4), 127, dtype=torch.uint8), (rows, k), format)
 
 
@@ -110,3 +111,40 @@ def test_weights_that_do_not_count_their_changes_are_refused(gpu):
         lin.weight = nn.Parameter(lin.weight + 1)
         with pytest.raises(RuntimeError, match="inference_mode"):
             get(lin)
+
+
+def copies(lm):
+    return [m.__dict__["_mx"].mx for m in lm.modules() if "_mx" in m.__dict__]
+
+
+def small_lm(**kw):
+    return KulaMambaLM(50, 64, n_layers=2, d_state=16, headdim=16, mimo_rank=1, **kw)
+
+
+@torch.no_grad()
+def test_quantising_again_makes_the_copies_anew_in_their_memory(gpu):
+    """Graphs that were captured with them read it."""
+    lm = small_lm().quantize_mx()
+    at = [(c.data.data_ptr(), c.scales.data_ptr()) for c in copies(lm)]
+    assert len(at) == 9  # four a block and the head's
+    for p in lm.parameters():
+        p.data.fill_(7.0)  # leaves no trace
+    assert lm.quantize_mx() is lm
+    assert [(c.data.data_ptr(), c.scales.data_ptr()) for c in copies(lm)] == at
+    assert all((c.data[:, 0] == 7).all() for c in copies(lm))
+    assert not copies(lm.quantize_mx(False)) and not lm.mx_weights and not lm.layers[1].mx_weights
+
+
+@torch.no_grad()
+def test_a_call_that_fails_leaves_the_model_as_it_was(gpu):
+    lm = small_lm().quantize_mx()
+    mine = copies(lm)
+    hook = lm.lm_head.register_forward_hook(lambda *a: None)
+    with pytest.raises(RuntimeError, match="hooks"):
+        lm.quantize_mx()
+    hook.remove()
+    assert lm.mx_weights and lm.layers[0].mx_weights and all(a is b for a, b in zip(copies(lm), mine))
+    biased = small_lm(bias=True)
+    with pytest.raises(RuntimeError, match="bias"):
+        biased.quantize_mx()
+    assert not biased.mx_weights and not copies(biased)
