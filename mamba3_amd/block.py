@@ -65,11 +65,13 @@ class _MXCopy:
     another weight's as long as it is compared; their objects are compared too, since a new parameter of the same memory counts
     its versions anew. Copied or pickled it is empty: the other module's weights are others."""
 
-    __slots__ = ("mx", "of", "key", "memory")
+    __slots__ = ("mx", "of", "key", "memory", "streams", "in_graph")
 
-    def __init__(self, mx: MXTensor | None = None, weights: tuple[torch.Tensor, ...] = ()):
+    def __init__(self, mx: MXTensor | None = None, weights: tuple[torch.Tensor, ...] = (), in_graph: bool = False):
         self.mx, self.key = mx, self._key(weights)
         self.of, self.memory = [weakref.ref(w) for w in weights], [w.detach() for w in weights]
+        self.streams = set() if mx is None else {_native.stream_of(mx.data)}  # that the allocator knows as its readers
+        self.in_graph = in_graph  # a captured graph reads it
 
     def __reduce__(self):
         return _MXCopy, ()
@@ -81,11 +83,24 @@ class _MXCopy:
     def is_of(self, weights: tuple[torch.Tensor, ...]) -> bool:
         return len(self.of) == len(weights) and all(r() is w for r, w in zip(self.of, weights)) and self.key == self._key(weights)
 
+    def read(self) -> MXTensor:
+        """The copy for work on the current stream. Once another has taken its place the allocator keeps its memory until the
+        streams that read it have come to that point."""
+        if not self.in_graph and torch.cuda.is_current_stream_capturing():
+            self.in_graph = True
+        if not self.in_graph and _native.stream_of(self.mx.data) not in self.streams:
+            stream = torch.cuda.current_stream(self.mx.device)
+            self.mx.data.record_stream(stream)
+            self.mx.scales.record_stream(stream)
+            self.streams.add(_native.stream_of(self.mx.data))
+        return self.mx
+
 
 def _mx_copy(owner: nn.Module, *weights: torch.Tensor, anew: bool = False) -> MXTensor:
     """The 4-bit copy of the weights, one below the other, that `owner` keeps: made when first asked for and again after one
-    was replaced or changed in place (which their version counters tell) or when asked for `anew`, into the same memory where it
-    fits, so that graphs captured with the copy go on with the new weights."""
+    was replaced or changed in place (which their version counters tell) or when asked for `anew`. It goes to memory of its own, so
+    that work under way keeps what it reads; where a captured graph reads the old one, into that one's memory behind all work on the
+    GPU, so that the graph goes on with the new weights."""
     kept = owner.__dict__.get("_mx")
     if kept is None or anew or not kept.is_of(weights):
         if any(w.is_inference() for w in weights):
@@ -95,14 +110,16 @@ def _mx_copy(owner: nn.Module, *weights: torch.Tensor, anew: bool = False) -> MX
             raise RuntimeError("a graph is being captured and the 4-bit weights are not there yet: run the model once before")
         with torch.inference_mode(False), torch.no_grad():  # copies outlive the mode that they are made in
             mx = quantize_mx(weights[0] if len(weights) == 1 else torch.cat(weights))
-            if kept is not None and kept.mx is not None and kept.mx.shape == mx.shape and kept.mx.device == mx.device:
+            in_graph = kept is not None and kept.in_graph and kept.mx.shape == mx.shape and kept.mx.device == mx.device
+            if in_graph:
+                torch.cuda.synchronize(mx.device)
                 kept.mx.data.copy_(mx.data)
                 kept.mx.scales.copy_(mx.scales)
                 mx = kept.mx
         # from here on any stream may read them
         torch.cuda.current_stream(mx.device).synchronize()
-        kept = owner.__dict__["_mx"] = _MXCopy(mx, weights)
-    return kept.mx
+        kept = owner.__dict__["_mx"] = _MXCopy(mx, weights, in_graph)
+    return kept.read()
 
 
 class SwiGLU(nn.Module):
@@ -405,8 +422,8 @@ class KulaMambaLM(nn.Module):
         copies of the weights and activations in 8 bits, both microscaled (quantize_mx, mx_linear), or back and frees
         the copies: graphs captured with them are not to be replayed after that. Gradients and the embedding use the weights
         themselves, which stay. A copy is made anew when the model runs and its weight was replaced or changed in place; after changes
-        that leave no trace (through `.data`, or by a graph's replay, as of a captured optimizer step), call this again. Either way it
-        stays in its memory, where captured graphs find it. Weights made in torch.inference_mode() count no changes and are
+        that leave no trace (through `.data`, or by a graph's replay, as of a captured optimizer step), call this again. Copies that
+        captured graphs read stay in their memory, behind all work on the GPU, and others go to new memory. Weights made in torch.inference_mode() count no changes and are
         refused. Needs projections without bias."""
         if on:
             try:

@@ -47,3 +47,36 @@ def test_a_captured_graph_follows_a_second_quantisation():
         torch.cuda.synchronize()
         assert torch.equal(got, want)
         del junk
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("captured", [False, True])
+def test_weights_are_replaced_while_another_stream_reads_the_copy(captured):
+    """The other stream's products, still waiting behind long work, keep the weights that they were launched with."""
+    lm, x = small_lm(20000, 256).quantize_mx(), rows(64, 256, 0)
+    if captured:
+        lm._mx_logits(x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = lm._mx_logits(x)
+    side, long = torch.cuda.Stream(), torch.zeros(8192, 8192, device="cuda", dtype=torch.bfloat16)
+    for i in range(3):
+        old = lm.lm_head.weight
+        first = logits(lm, x)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for _ in range(20):
+                long = long @ long
+            if captured:
+                graph.replay()
+                kept = got.clone()
+            else:
+                kept = lm._mx_logits(x)
+        lm.lm_head.weight = torch.nn.Parameter(old.flip(0) * (1.5 + i))
+        now = lm._mx_logits(x)
+        torch.cuda.synchronize()
+        assert torch.equal(kept, first) and torch.equal(now, logits(lm, x)) and not torch.equal(now, first)
+        if captured:
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, now)

@@ -24,13 +24,14 @@ class Gpu:
     """What _mx_copy asks of torch.cuda."""
 
     def __init__(self):
-        self.asked, self.capturing = [], False
+        self.asked, self.capturing, self.stream, self.on_wait = [], False, 0, lambda: None
 
     def current_stream(self, device=None):
         return self
 
     def synchronize(self, device=None):
-        self.asked.append("wait")
+        self.asked.append("wait" if device is None else "wait for all")
+        self.on_wait()
 
     def is_current_stream_capturing(self):
         return self.capturing
@@ -42,6 +43,8 @@ def gpu(monkeypatch):
     monkeypatch.setattr(block, "quantize_mx", kept_numbers)
     for name in ("current_stream", "synchronize", "is_current_stream_capturing"):
         monkeypatch.setattr(torch.cuda, name, getattr(gpu, name))
+    monkeypatch.setattr(block._native, "stream_of", lambda t: gpu.stream)
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, stream: gpu.asked.append(("reads", t.data_ptr(), gpu.stream)))
     return gpu
 
 
@@ -125,6 +128,9 @@ def small_lm(**kw):
 def test_quantising_again_makes_the_copies_anew_in_their_memory(gpu):
     """Graphs that were captured with them read it."""
     lm = small_lm().quantize_mx()
+    gpu.capturing = True
+    lm._mx_head(), [layer._mx_projections() for layer in lm.layers]
+    gpu.capturing = False
     at = [(c.data.data_ptr(), c.scales.data_ptr()) for c in copies(lm)]
     assert len(at) == 9  # four a block and the head's
     for p in lm.parameters():
@@ -138,13 +144,53 @@ def test_quantising_again_makes_the_copies_anew_in_their_memory(gpu):
 @torch.no_grad()
 def test_a_call_that_fails_leaves_the_model_as_it_was(gpu):
     lm = small_lm().quantize_mx()
-    mine = copies(lm)
+    mine = [lm._mx_head()]
     hook = lm.lm_head.register_forward_hook(lambda *a: None)
     with pytest.raises(RuntimeError, match="hooks"):
         lm.quantize_mx()
     hook.remove()
-    assert lm.mx_weights and lm.layers[0].mx_weights and all(a is b for a, b in zip(copies(lm), mine))
+    assert lm.mx_weights and lm.layers[0].mx_weights and len(copies(lm)) == 9 and mine[0] in copies(lm)
     biased = small_lm(bias=True)
     with pytest.raises(RuntimeError, match="bias"):
         biased.quantize_mx()
     assert not biased.mx_weights and not copies(biased)
+
+
+@torch.no_grad()
+def test_a_new_copy_leaves_the_old_one_to_work_under_way(gpu):
+    lin = linear()
+    mine = get(lin)
+    numbers = mine.data.clone()
+    other = nn.Parameter(lin.weight + 9.0)
+    for change in (lambda: lin.weight.add_(1.0), lambda: setattr(lin, "weight", other)):
+        change()
+        assert fresh(lin) and get(lin) is not mine and torch.equal(mine.data, numbers)
+    mine = get(lin)
+    numbers = mine.data.clone()
+    assert block._mx_copy(lin, lin.weight, anew=True) is not mine and torch.equal(mine.data, numbers)
+
+
+@torch.no_grad()
+def test_a_copy_that_a_graph_reads_is_overwritten_behind_all_work(gpu):
+    lin = linear()
+    get(lin)
+    gpu.capturing = True
+    mine = get(lin)
+    gpu.capturing = False
+    for i in range(3):
+        lin.weight.add_(1.0)
+        numbers, seen = mine.data.clone(), []
+        gpu.on_wait = lambda: seen.append((gpu.asked[-1], torch.equal(mine.data, numbers)))
+        assert get(lin) is mine and not torch.equal(mine.data, numbers) and fresh(lin)
+        assert seen == [("wait for all", True), ("wait", False)]
+
+
+@torch.no_grad()
+def test_the_allocator_learns_each_stream_that_reads_a_copy(gpu):
+    lin = linear()
+    mine = get(lin)
+    assert not [a for a in gpu.asked if a[0] == "reads"]  # the stream it was made on it knows
+    for gpu.stream in (0, 5, 5, 6, 0, 5):
+        get(lin)
+    want = [("reads", t.data_ptr(), stream) for stream in (5, 6) for t in (mine.data, mine.scales)]
+    assert [a for a in gpu.asked if a[0] == "reads"] == want
