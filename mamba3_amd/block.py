@@ -10,6 +10,7 @@ equal the reference's so seeded models hold identical weights.
 from __future__ import annotations
 
 import math
+import threading
 import weakref
 
 import torch
@@ -67,11 +68,11 @@ class _MXCopy:
 
     __slots__ = ("mx", "of", "key", "memory", "streams", "in_graph")
 
-    def __init__(self, mx: MXTensor | None = None, weights: tuple[torch.Tensor, ...] = (), in_graph: bool = False):
-        self.mx, self.key = mx, self._key(weights)
+    def __init__(self, *weights: torch.Tensor):
+        self.mx, self.key = None, self._key(weights)
         self.of, self.memory = [weakref.ref(w) for w in weights], [w.detach() for w in weights]
-        self.streams = set() if mx is None else {_native.stream_of(mx.data)}  # that the allocator knows as its readers
-        self.in_graph = in_graph  # a captured graph reads it
+        self.streams = set()   # that the allocator knows as its readers
+        self.in_graph = False  # a captured graph reads it
 
     def __reduce__(self):
         return _MXCopy, ()
@@ -103,23 +104,37 @@ def _mx_copy(owner: nn.Module, *weights: torch.Tensor, anew: bool = False) -> MX
     GPU, so that the graph goes on with the new weights."""
     kept = owner.__dict__.get("_mx")
     if kept is None or anew or not kept.is_of(weights):
-        if any(w.is_inference() for w in weights):
-            raise RuntimeError("4-bit weights need parameters that count their changes; those made in torch.inference_mode() do not: make or load "
-                               "the model outside of it")
-        if weights[0].is_cuda and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("a graph is being captured and the 4-bit weights are not there yet: run the model once before")
-        with torch.inference_mode(False), torch.no_grad():  # copies outlive the mode that they are made in
-            mx = quantize_mx(weights[0] if len(weights) == 1 else torch.cat(weights))
-            in_graph = kept is not None and kept.in_graph and kept.mx.shape == mx.shape and kept.mx.device == mx.device
-            if in_graph:
-                torch.cuda.synchronize(mx.device)
-                kept.mx.data.copy_(mx.data)
-                kept.mx.scales.copy_(mx.scales)
-                mx = kept.mx
-        # from here on any stream may read them
-        torch.cuda.current_stream(mx.device).synchronize()
-        kept = owner.__dict__["_mx"] = _MXCopy(mx, weights, in_graph)
+        with _MX_LOCK:
+            kept = owner.__dict__.get("_mx")
+            if kept is None or anew or not kept.is_of(weights):
+                kept = owner.__dict__["_mx"] = _mx_made(kept, weights)
     return kept.read()
+
+
+_MX_LOCK = threading.RLock()  # copies are made by one thread at a time
+
+
+def _mx_made(kept: _MXCopy | None, weights: tuple[torch.Tensor, ...]) -> _MXCopy:
+    """The copy of the weights in the place of `kept`."""
+    if any(w.is_inference() for w in weights):
+        raise RuntimeError("4-bit weights need parameters that count their changes; those made in torch.inference_mode() do not: make or load "
+                           "the model outside of it")
+    if weights[0].is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a graph is being captured and the 4-bit weights are not there yet: run the model once before")
+    made = _MXCopy(*weights)  # of the versions before they are read
+    with torch.inference_mode(False), torch.no_grad():  # copies outlive the mode that they are made in
+        mx = quantize_mx(weights[0] if len(weights) == 1 else torch.cat(weights))
+        made.in_graph = kept is not None and kept.in_graph and kept.mx.shape == mx.shape and kept.mx.device == mx.device
+        if made.in_graph:
+            torch.cuda.synchronize(mx.device)
+            kept.mx.data.copy_(mx.data)
+            kept.mx.scales.copy_(mx.scales)
+            mx = kept.mx
+    made.mx = mx
+    made.streams.add(_native.stream_of(mx.data))
+    # from here on any stream may read it
+    torch.cuda.current_stream(mx.device).synchronize()
+    return made
 
 
 class SwiGLU(nn.Module):

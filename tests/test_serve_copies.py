@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import copy
 import pickle
+import threading
 
 import pytest
 import torch
@@ -194,3 +195,45 @@ def test_the_allocator_learns_each_stream_that_reads_a_copy(gpu):
         get(lin)
     want = [("reads", t.data_ptr(), stream) for stream in (5, 6) for t in (mine.data, mine.scales)]
     assert [a for a in gpu.asked if a[0] == "reads"] == want
+
+
+@torch.no_grad()
+def test_threads_that_find_a_copy_stale_make_it_once(gpu, monkeypatch):
+    lin, made, meet = linear(), [], threading.Barrier(4)
+
+    def slow(w, format="e2m1"):
+        made.append(threading.get_ident())
+        threading.Event().wait(0.05)
+        return kept_numbers(w, format)
+
+    monkeypatch.setattr(block, "quantize_mx", slow)
+    got = [None] * 4
+
+    def one(i):
+        with torch.no_grad():
+            meet.wait()
+            got[i] = get(lin)
+
+    for turn in range(2):
+        threads = [threading.Thread(target=one, args=(i,)) for i in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert len(made) == turn + 1 and all(g is got[0] for g in got) and fresh(lin)
+        lin.weight.add_(1.0)
+
+
+@torch.no_grad()
+def test_a_change_while_a_copy_is_made_is_not_missed(gpu, monkeypatch):
+    lin = linear()
+
+    def changed_meanwhile(w, format="e2m1"):
+        numbers = kept_numbers(w, format)
+        lin.weight.add_(1.0)
+        return numbers
+
+    monkeypatch.setattr(block, "quantize_mx", changed_meanwhile)
+    get(lin)
+    monkeypatch.setattr(block, "quantize_mx", kept_numbers)
+    assert fresh(lin)
