@@ -1016,8 +1016,18 @@ static int sample_t(const SampleArgs& a, hipStream_t stream) {
     const int pieces = (int)(((int64_t)a.vocab * (int)sizeof(T) + 15) / 16), held = std::min(pieces, kSpHeld / 16);
     static std::atomic<uint64_t> done{0};
     if (!allow_lds(reinterpret_cast<const void*>(&sample_kernel<T>), kSpHeld, done)) return M3_ERR_LAUNCH;
-    hipLaunchKernelGGL((sample_kernel<T>), dim3((unsigned)a.rows), dim3(kSpThreads), held * 16, stream, a, held);
-    return hipGetLastError() == hipSuccess ? M3_OK : M3_ERR_LAUNCH;
+    // a grid holds less than 2^32 threads
+    constexpr int64_t kRows = ((int64_t)1 << 32) / kSpThreads / 2;
+    for (int64_t r = 0; r < a.rows; r += kRows) {
+        SampleArgs b = a;
+        const auto from = [&](auto* p) { return p ? p + r : p; };
+        b.z = reinterpret_cast<const T*>(a.z) + r * a.vocab;
+        b.u = from(a.u), b.temperature = from(a.temperature), b.top_p = from(a.top_p), b.min_p = from(a.min_p), b.top_k = from(a.top_k);
+        b.token = from(a.token), b.logprob = from(a.logprob);
+        hipLaunchKernelGGL((sample_kernel<T>), dim3((unsigned)std::min(kRows, a.rows - r)), dim3(kSpThreads), held * 16, stream, b, held);
+        if (hipGetLastError() != hipSuccess) return M3_ERR_LAUNCH;
+    }
+    return M3_OK;
 }
 
 int launch_sample(const void* logits, int dtype, int64_t rows, int vocab, const float* u, const float* temperature,
