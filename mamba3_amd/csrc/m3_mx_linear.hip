@@ -318,7 +318,7 @@ static void few_waves(const MxLinearArgs& a, F launch) {
 template <int FA, int FM, int FN, typename TO>
 static int few_t(const MxLinearArgs& a, hipStream_t stream) {
     const int64_t tn = (a.N + 16 * FN - 1) / (16 * FN), tm = (a.M + 16 * FM - 1) / (16 * FM);
-    if (tn * tm > 0x7fffffff) return M3_ERR_UNSUPPORTED;
+    if (tn * tm >= (1 << 24)) return M3_ERR_UNSUPPORTED;  // a grid holds less than 2^32 threads, and 256 a block where there are so many
     few_waves<FM, FN>(a, [&](auto w) {
         constexpr int kW = decltype(w)::value;
         hipLaunchKernelGGL((mx_linear_few_kernel<kW, FA, FM, FN, TO>), dim3((unsigned)(tn * tm)), dim3(kW * 64), kW * FM * FN * 1024, stream, a, (int)tn,
@@ -703,10 +703,12 @@ __global__ __launch_bounds__(Tile::NT, 2) void mx_linear_tile_kernel(MxLinearArg
     wait(std::integral_constant<int, 0>{});
 }
 
+constexpr int kMlTileLd = 1 << 25;  // 32 rows of fewer columns are below 2^31 bytes, the end of a descriptor
+
 template <typename Tile>
 static int tile_t(const MxLinearArgs& a, hipStream_t stream) {
     const int64_t tm = (a.M + Tile::BM - 1) / Tile::BM, tn = (a.N + Tile::BN - 1) / Tile::BN;
-    if (tm * tn > (1 << 30) || a.ld > (1 << 25)) return M3_ERR_UNSUPPORTED;  // 32 rows of results within a descriptor
+    if (tm * tn > (1 << 30) || a.ld >= kMlTileLd) return M3_ERR_UNSUPPORTED;
     static std::atomic<uint64_t> done{0};
     if (!allow_lds(reinterpret_cast<const void*>(&mx_linear_tile_kernel<Tile>), Tile::kLds, done)) return M3_ERR_LAUNCH;
     const int64_t most = 256 * std::min(2, (160 << 10) / Tile::kLds);  // blocks at once
@@ -724,6 +726,7 @@ static int tile_t(const MxLinearArgs& a, hipStream_t stream) {
 // 64 rows: 2048 x 11000 14.3, 2048 x 128000 45 (42.6). 128 x 128 and 256 x 256 tiles: 8192 x 768 x 4224 32 and 37,
 // 8192 x 2112 x 768 19 and 27, 8192 x 5504 x 2048 105 and 76.
 static bool takes_tiles(const MxLinearArgs& a) {
+    if (a.ld >= kMlTileLd) return false;
     const int64_t tiles = (int64_t)((a.M + 127) / 128) * ((a.N + 127) / 128);
     if (a.M > 64) return tiles >= 56;
     if (a.M > 32) return tiles >= 72;

@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from mamba3_amd import _native, sample_tokens
+from mamba3_amd import MXTensor, _native, mx_linear, quantize_mx, sample_tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +33,20 @@ def test_more_rows_than_a_grid_has_room_for(each, dtype):
         want = sample_tokens(z[part], u[part], *(v[part] if each else v for v in settings), return_logprob=True)
         assert torch.equal(tokens[part], want[0]) and torch.equal(lp[part], want[1])
     assert ((tokens >= 0) & (tokens < vocab)).all() and torch.isfinite(lp).all()
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("rows,n", [(40, 1 << 25), (70, (1 << 25) + 70), (3, (1 << 26) - 5)])
+def test_more_columns_than_tiles_take(rows, n):
+    """From 2^25 columns on, 32 rows of bf16 results reach the end of what a descriptor bounds."""
+    k, gen = 100, torch.Generator("cuda").manual_seed(0)
+    w = MXTensor(torch.randint(256, (n, 64), device="cuda", generator=gen, dtype=torch.uint8),
+                 torch.randint(120, 130, (n, 4), device="cuda", generator=gen, dtype=torch.uint8), (n, k), "e2m1")
+    x = torch.randn(rows, k, device="cuda", generator=gen).bfloat16()
+    res = torch.empty(rows, n, device="cuda", dtype=torch.bfloat16).normal_(generator=gen)
+    for given in (x, quantize_mx(x, "e4m3")):
+        y = mx_linear(given, w, res, 0.5)
+        for at in (0, 1 << 24, n - 333):
+            part = slice(at, at + 333)
+            want = mx_linear(given, MXTensor(w.data[part], w.scales[part], (333, k), "e2m1"), res[:, part], 0.5)
+            assert torch.equal(y[:, part], want)
