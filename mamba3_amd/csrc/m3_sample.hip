@@ -1006,8 +1006,8 @@ __global__ __launch_bounds__(kSpThreads) void sample_kernel(SampleArgs a, int he
     }
     if (threadIdx.x == 0) {
         a.token[row] = index;
-        if (a.logprob)
-            a.logprob[row] = (float)(scale.far(logit) * (-1.0 / kSpPerT) - (double)logf((float)ldexp((double)kept, -a.shift)));
+        // the likeliest token's mass is 1: what the others add may be far below it
+        if (a.logprob) a.logprob[row] = (float)(scale.far(logit) * (-1.0 / kSpPerT) - log1p(ldexp((double)(int64_t)(kept - ((u64)1 << a.shift)), -a.shift)));
     }
 }
 
