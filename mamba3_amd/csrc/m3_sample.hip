@@ -11,10 +11,12 @@
 // more (equal logits, low temperatures), each question gathers the one bin that it falls in, which is split by its keys' bits
 // until it fits.
 // With q = 64 (max z - z) / T in 64 bits, a token's mass is exp(-b / 64) exp(-r / 64), b the bin and r < 1: the bins add up
-// exp(-r / 64), four terms of its series to 1e-11, as whole numbers of 2^-45 or so, so that sums do not depend on their
-// order; exp(-b / 64), of two table values, comes in once a bin. (An exponential for each token took three times as long.) What lies
-// past the last bin but one, below exp(-32) of the likeliest, is counted but has no mass. A border is missed with a probability of
-// about 1e-10 a row, as with 64-bit sums over sorted probabilities.
+// exp(-r / 64), five terms of its series to 2e-14, as whole numbers of 2^-45 (131072 tokens; 2^-51 to 2048), so that sums do not depend
+// on their order; exp(-b / 64), of two table values, comes in once a bin. (An exponential for each token took three times as long.) What
+// lies past the last bin but one, below exp(-32) of the likeliest, is counted but has no mass. A running mass of n tokens is off by
+// about 2e-14 of itself and sqrt(n) 2^-47 of the likeliest's (2e-14 and 3e-12 at 131072 tokens, to 2048 below 2e-14), where sums of
+// 64-bit floating numbers would be off by about 1e-14 and depend on their order. That is how probable it is for a border that u falls
+// on its other side.
 // Bound by the reads and the bins' atomics for large batches (256 rows of 128000 fp32 logits, a setting for each row: 76 us, where one
 // read of them takes 22; a row alone on its CU takes 50-60), by the chain of passes, barriers and first fetches of code for few
 // (4 rows of 32000: 18-20 us, of which greedy choice and launch take 6). After the bins one wave does what is left but
@@ -87,8 +89,8 @@ constexpr double kSpWhole = 4503599627370496.0;  // 2^52: what is added to it is
 __device__ __forceinline__ u64 sp_whole(double v) {  // of 0 <= v < 2^52
     return __builtin_bit_cast(u64, v + kSpWhole) & 0x000fffffffffffffull;
 }
-// exp(-i) and exp(-i / 64): a bin's mass is a product of two, and a token's that times four terms of exp(-d / 64)'s series for
-// what it lies behind its bin's start (to 1e-11).
+// exp(-i) and exp(-i / 64): a bin's mass is a product of two, and a token's that times five terms of exp(-d / 64)'s series for
+// what it lies behind its bin's start (to 2e-14).
 struct SampleTables {
     double whole[kSpBins / 64], part[64];
 };
@@ -105,8 +107,8 @@ constexpr SampleTables sp_tables() {
 }
 __constant__ const SampleTables kSpTables = sp_tables();
 __device__ __forceinline__ double sp_series(double d) {
-    constexpr double c1 = -1.0 / kSpPerT, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4;
-    return fma(fma(fma(fma(c4, d, c3), d, c2), d, c1), d, 1.0);
+    constexpr double c1 = -1.0 / kSpPerT, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4, c5 = c4 * c1 / 5;
+    return fma(fma(fma(fma(fma(c5, d, c4), d, c3), d, c2), d, c1), d, 1.0);
 }
 __device__ __forceinline__ double sp_bin_mass(const SampleTables& t, int b) { return t.whole[b >> 6] * t.part[b & 63]; }
 // A token's mass times 2^shift as a whole number (shift <= 51), none past the last bin but one.
@@ -720,7 +722,7 @@ __global__ __launch_bounds__(kSpThreads) void sample_kernel(SampleArgs a, int he
     unsigned tail = 0;  // tokens of the last bin, which have no mass
     {
         const double unit = ldexp(1.0, a.shift), c1 = unit * (-1.0 / kSpPerT), c2 = c1 * (-1.0 / (2 * kSpPerT)), c3 = c2 * (-1.0 / (3 * kSpPerT)),
-                     c4 = c3 * (-1.0 / (4 * kSpPerT));  // sp_series, times 2^shift
+                     c4 = c3 * (-1.0 / (4 * kSpPerT)), c5 = c4 * (-1.0 / (5 * kSpPerT));  // sp_series, times 2^shift
         const int aside = kSpBins + ((int)threadIdx.x & 63);
         auto add = [&](float x, auto counted) __attribute__((always_inline)) {
             // without a branch: what has no mass (NaN, too) goes where nobody looks
@@ -728,7 +730,7 @@ __global__ __launch_bounds__(kSpThreads) void sample_kernel(SampleArgs a, int he
             const bool in = q < (double)(kSpBins - 1);
             const int b = (int)q, at = in ? b : aside;
             const double d = q - (double)b;
-            atomicAdd(&s.mass[at], sp_whole(fma(fma(fma(fma(c4, d, c3), d, c2), d, c1), d, unit)));
+            atomicAdd(&s.mass[at], sp_whole(fma(fma(fma(fma(fma(c5, d, c4), d, c3), d, c2), d, c1), d, unit)));
             if constexpr (decltype(counted)::value) {
                 atomicAdd(&s.count[at], 1u);
                 tail += !in & (x > -INFINITY);

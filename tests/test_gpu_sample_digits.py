@@ -2,6 +2,9 @@
 
 from __future__ import annotations
 
+import math
+from decimal import Decimal, getcontext
+
 import pytest
 import torch
 
@@ -44,3 +47,29 @@ def test_log_probabilities_are_the_64_bit_ones_rounded():
         want = torch.log_softmax(masses, 1).gather(1, token.cpu()[:, None])[:, 0]
         # a mass is off by 2^-36 of itself at most and by 2^-50
         assert ((lp.cpu().double() - want).abs() <= 2.0 ** -24 * want.abs() + 2.0 ** -35).all()
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("vocab", [2, 1500])
+@pytest.mark.parametrize("off", [6e-13, -6e-13])
+def test_masses_next_to_a_border(off, vocab):
+    """Two tokens, of masses 1 and m: u is just before or past the end of the first, 1 / (1 + m), by less than the fifth term of
+    exp's series where m lies at the end of a bin (7.8e-12 of m, a quarter of that here)."""
+    getcontext().prec = 40
+    z = torch.full((8, vocab), -float("inf"))
+    gap = 2.0 ** -6 + 2.0 ** -20 * torch.arange(8)
+    z[:, 0], z[:, 1] = 0.0, -gap
+    u, temperature, want = [], [], []
+    for g in gap.tolist():
+        one = torch.tensor(1 / (1 + math.exp(-1 / 64.001))).item()
+        u.append(one)
+        # the temperature that puts the border at u (1 + off): exp(-g / t) = 1 / border - 1
+        border = Decimal(one) * (1 + Decimal(off))
+        temperature.append(float(-Decimal(g) / (1 / border - 1).ln()))
+        real = 1 / (1 + (-Decimal(g) / Decimal(temperature[-1])).exp())
+        assert abs(real / border - 1) < Decimal("2e-16")
+        want.append(1 if Decimal(one) >= real else 0)
+    assert want == [0 if off > 0 else 1] * 8
+    # the series to 2e-14 of m and whole numbers of 2^-51: 1e-14 of the whole
+    got = [sample_tokens(z[i:i + 1].cuda(), torch.tensor(u[i:i + 1]).cuda(), t).item() for i, t in enumerate(temperature)]
+    assert got == want
