@@ -268,7 +268,7 @@ struct SampleShared {
     u64 wmass[kSpWaves];
     unsigned wcount[kSpWaves];
     unsigned n;
-    int at, to;
+    int at;
     SamplePlace place;
 };
 
@@ -358,24 +358,20 @@ __device__ __forceinline__ void sp_run(SampleShared& s, u64* mass, unsigned* cou
     for (int i = 0; i < kPer; ++i) count[threadIdx.x * kPer + i] = tc + c[i], mass[threadIdx.x * kPer + i] = tm + m[i];
     __syncthreads();
 }
-// The bins (s.at, s.to) whose end reaches the goals and whose start does not, or where none does `otherwise` (-1: none). `to` is
-// not easier to reach than `at`.
+// The bin s.at whose end reaches the goal and whose start does not, or where none does `otherwise` (-1: none).
 template <int kBins>
-__device__ __forceinline__ void sp_find_bins(SampleShared& s, const u64* mass, const unsigned* count, u64 base_c, u64 base_m, const SampleGoal& at,
-                                             const SampleGoal& to, int otherwise) {
+__device__ __forceinline__ void sp_find_bin(SampleShared& s, const u64* mass, const unsigned* count, u64 base_c, u64 base_m, const SampleGoal& goal,
+                                            int otherwise) {
     constexpr int kPer = kBins / kSpThreads;
-    if (threadIdx.x == 0) s.at = s.to = otherwise;
+    if (threadIdx.x == 0) s.at = otherwise;
     const int first = (int)threadIdx.x * kPer;
-    u64 c = base_c + (first ? count[first - 1] : 0), m = base_m + (first ? mass[first - 1] : 0);
-    bool at_before = at.reached(c, m), to_before = to.reached(c, m);
+    bool before = goal.reached(base_c + (first ? count[first - 1] : 0), base_m + (first ? mass[first - 1] : 0));
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        c = base_c + count[first + i], m = base_m + mass[first + i];
-        const bool at_now = at.reached(c, m), to_now = to.reached(c, m);
-        if (at_now & !at_before) s.at = first + i;
-        if (to_now & !to_before) s.to = first + i;
-        at_before = at_now, to_before = to_now;
+        const bool now = goal.reached(base_c + count[first + i], base_m + mass[first + i]);
+        if (now & !before) s.at = first + i;
+        before = now;
     }
     __syncthreads();
 }
@@ -538,7 +534,7 @@ struct SampleWalk {
 template <typename L>
 __device__ __forceinline__ void sp_locate(SampleShared& s, const L& z, const SampleScale& scale, const SampleGoal& goal) {
     __syncthreads();
-    sp_find_bins<kSpBins>(s, s.mass, s.count, 0, 0, goal, goal, -1);
+    sp_find_bin<kSpBins>(s, s.mass, s.count, 0, 0, goal, -1);
     const int bin = s.at;
     u64 base_c = bin > 0 ? s.count[bin - 1] : 0, base_m = bin > 0 ? s.mass[bin - 1] : 0;
     // first what may lie in the bin, by one comparison each way
@@ -606,7 +602,7 @@ __device__ __forceinline__ void sp_locate(SampleShared& s, const L& z, const Sam
         unsigned all_c;
         u64 all_m;
         sp_run<kSpParts>(s, s.smass, s.scount, all_c, all_m);
-        sp_find_bins<kSpParts>(s, s.smass, s.scount, base_c, base_m, goal, goal, (int)((khi - klo) >> parts));
+        sp_find_bin<kSpParts>(s, s.smass, s.scount, base_c, base_m, goal, (int)((khi - klo) >> parts));
         const unsigned b = (unsigned)s.at;
         if (b) base_c += s.scount[b - 1], base_m += s.smass[b - 1];
         const unsigned new_hi = khi - (b << parts), span = (1u << parts) - 1u;
