@@ -484,8 +484,8 @@ enum m3_mx_format {
  * E + 127, 4-byte aligned, 255 for a block that held an infinity or NaN (it is NaN). E is the smallest exponent,
  * from -127 on, under which the block's largest magnitude rounds to an element (none saturates); 0 for a block
  * of zeros. Elements round to nearest, ties to even.
- * m3_mx_quantize: x [rows, k], or with `gated` of silu(x[:, :k]) * x[:, k:] for x [rows, 2 k] (computed in fp32,
- * mamba3/block.py:16-26). m3_mx_dequantize: out [rows, k] (exact in bf16 but for results below 2^-126 or past the largest number).
+ * m3_mx_quantize: x [rows, k], or with `gated` of silu(x[:, :k]) * x[:, k:] for x [rows, 2 k] (rounded as the
+ * exact product would be, mamba3/block.py:16-26). m3_mx_dequantize: out [rows, k] (exact in bf16 but for results below 2^-126 or past the largest number).
  * rows <= 2^32, k <= 2^24. No result of these and the calls below may overlap an input.
  */
 int m3_mx_quantize(int64_t rows, int32_t k, int32_t dtype, int32_t gated, int32_t format, const void* x, void* data,

@@ -194,8 +194,8 @@ __global__ __launch_bounds__(kW * 64) void mx_linear_few_kernel(MxLinearArgs a, 
 // m3_add_norm.hip's does: the same sums) or silu(gate) * up.
 constexpr int kMlRawRows = 16;
 // The work that is worth a launch less when every block does it (bf16, us in a graph, one launch against two): quantising
-// 4 x 5504 elements 5.7 against 6.9, 16 x 1536 5.5 against 5.8, 16 x 2048 6.8 against 6.5; gating 2 x 5504 6.1 against 6.9, 8 x 1536 5.5
-// against 5.5, 8 x 2112 7.1 against 5.6; a norm
+// 4 x 5504 elements 5.7 against 6.9, 16 x 1536 5.5 against 5.8, 16 x 2048 6.8 against 6.5; gating 2 x 5504 6.6 against 7.0, 8 x 1536 5.8
+// against 5.7, 8 x 2112 (the gate in 32 bits alone) 7.1 against 5.6; a norm
 // of 8 rows, one a wave, of 768 4.9 against 5.6, of 2048 7.4 against 8.5, of 16 rows of 768 7.1 against 5.8.
 constexpr int kMlRawElements = 24576, kMlGatedElements = 12288, kMlNormRows = 8;
 constexpr int kMlNormPieces = 4;    // of 512 columns: a wave's row

@@ -88,7 +88,7 @@ def quantize_mx(x: torch.Tensor, format: str = "e2m1") -> MXTensor:
 
 def silu_mul_mx(gate_up: torch.Tensor, format: str = "e4m3") -> MXTensor:
     """silu(gate) * up as microscaled values, from gate_up (..., 2 k) that holds the gate in its first half
-    (mamba3/block.py:16-26 between its products): computed in fp32 and rounded once. No backward."""
+    (mamba3/block.py:16-26 between its products), rounded as the exact product would be. No backward."""
     check_format(format)
     if gate_up.dim() < 1 or gate_up.shape[-1] < 2 or gate_up.shape[-1] % 2:
         raise ValueError(f"silu_mul_mx needs an even last dimension of at least 2, got shape {tuple(gate_up.shape)}")
