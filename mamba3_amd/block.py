@@ -87,14 +87,20 @@ class _MXCopy:
     def read(self) -> MXTensor:
         """The copy for work on the current stream. Once another has taken its place the allocator keeps its memory until the
         streams that read it have come to that point."""
-        if not self.in_graph and torch.cuda.is_current_stream_capturing():
+        known = _native.stream_of(self.mx.data) in self.streams
+        if not (known and self.in_graph) and torch.cuda.is_current_stream_capturing():
             self.in_graph = True
-        if not self.in_graph and _native.stream_of(self.mx.data) not in self.streams:
+        elif not known:
             stream = torch.cuda.current_stream(self.mx.device)
             self.mx.data.record_stream(stream)
             self.mx.scales.record_stream(stream)
             self.streams.add(_native.stream_of(self.mx.data))
         return self.mx
+
+    def release(self) -> None:
+        """Waits for graphs that read the copy, whose memory is about to be given back: the allocator does not know their streams."""
+        if self.in_graph:
+            torch.cuda.synchronize(self.mx.device)
 
 
 def _mx_copy(owner: nn.Module, *weights: torch.Tensor, anew: bool = False) -> MXTensor:
@@ -124,12 +130,13 @@ def _mx_made(kept: _MXCopy | None, weights: tuple[torch.Tensor, ...]) -> _MXCopy
     made = _MXCopy(*weights)  # of the versions before they are read
     with torch.inference_mode(False), torch.no_grad():  # copies outlive the mode that they are made in
         mx = quantize_mx(weights[0] if len(weights) == 1 else torch.cat(weights))
+        if kept is not None:
+            kept.release()
         made.in_graph = kept is not None and kept.in_graph and kept.mx.shape == mx.shape and kept.mx.device == mx.device
         if made.in_graph:
-            torch.cuda.synchronize(mx.device)
             kept.mx.data.copy_(mx.data)
             kept.mx.scales.copy_(mx.scales)
-            mx = kept.mx
+            mx, made.streams = kept.mx, kept.streams
     made.mx = mx
     made.streams.add(_native.stream_of(mx.data))
     # from here on any stream may read it
@@ -451,7 +458,9 @@ class KulaMambaLM(nn.Module):
                 raise
         else:
             for m in self.modules():
-                m.__dict__.pop("_mx", None)
+                kept = m.__dict__.pop("_mx", None)
+                if kept is not None:
+                    kept.release()
         self.mx_weights = on
         for layer in self.layers:
             layer.mx_weights = on

@@ -237,3 +237,41 @@ def test_a_change_while_a_copy_is_made_is_not_missed(gpu, monkeypatch):
     get(lin)
     monkeypatch.setattr(block, "quantize_mx", kept_numbers)
     assert fresh(lin)
+
+
+@torch.no_grad()
+def test_readers_of_a_copy_that_a_graph_reads_too_are_known(gpu):
+    lin = linear()
+    mine = get(lin)
+    gpu.stream, gpu.capturing = 3, True
+    get(lin)
+    gpu.capturing = False
+    gpu.asked.clear()
+    for turn in range(2):
+        for gpu.stream in (0, 5, 3, 5):
+            assert get(lin) is mine
+        lin.weight.add_(1.0)
+    reads = [a for a in gpu.asked if a[0] == "reads"]
+    assert reads == [("reads", t.data_ptr(), stream) for stream in (5, 3) for t in (mine.data, mine.scales)]
+
+
+@torch.no_grad()
+def test_memory_that_a_graph_reads_is_given_back_behind_all_work(gpu):
+    lm = small_lm().quantize_mx()
+    gpu.asked.clear()
+    lm.quantize_mx(False).quantize_mx()
+    assert "wait for all" not in gpu.asked  # the allocator knows the other readers
+    gpu.capturing = True
+    lm._mx_head()
+    gpu.capturing = False
+    gpu.asked.clear()
+    lm.quantize_mx(False)
+    assert gpu.asked == ["wait for all"] and not copies(lm)
+    lin = linear()
+    get(lin)
+    gpu.capturing = True
+    old = get(lin)
+    gpu.capturing = False
+    gpu.asked.clear()
+    lin.weight = nn.Parameter(torch.ones(5, 40))  # no room for it in the old one's memory
+    assert get(lin) is not old and gpu.asked == ["wait for all", "wait"] and fresh(lin)
