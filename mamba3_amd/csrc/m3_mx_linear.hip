@@ -102,10 +102,10 @@ __device__ __forceinline__ void mx_out4(const MxLinearArgs& a, int m, int n, f32
 }
 
 // Few rows: a block takes 16 FM rows and 16 FN columns, its kW waves every kW-th step of k, straight from memory to
-// registers; their sums meet in LDS. Bound by the latency of its few reads, and by the weights' read. Up to 16 rows eight waves,
-// or 16 where a row has 4096 columns or more and the block 16 (few_waves): weights that come from HBM, as a model's do,
-// are then on their way at once (1 x 768 x 3696 2.8 us in a graph, 3.2 with four waves; 1 x 5504 x 2048 5.0, 5.7 with eight, 8.2 with
-// four; 1 x 2048 x 8800 7.8, 6.9 with four). More rows hold more sums: four waves.
+// registers; their sums meet in LDS. Bound by the latency of its few reads, and by the weights' read. Eight waves where FM FN is at
+// most eight, or 16 where k is above 3968 and the block takes 16 columns (few_waves): weights that come from
+// HBM, as a model's do, are then on their way at once (1 x 768 x 3696 2.8 us in a graph, 3.2 with four waves; 1 x 5504 x 2048 5.0, 5.7
+// with eight, 8.2 with four; 1 x 2048 x 8800 7.8, 6.9 with four). Blocks of 64 x 64 hold more sums: four waves.
 
 // Adds w x^T of one step of k.
 template <int FA, int FM, int FN, bool kExact>
@@ -364,7 +364,7 @@ static int raw_pre(const MxLinearArgs& a, int pre, const MxBefore& before, int k
 }
 
 // Many rows: tiles through LDS, as in m3_gemm.h. A block of WGM x WGN waves owns a BM x BN tile (a wave 32 FM x 64)
-// and walks k in steps of 128, fetched straight to LDS three steps ahead; operand rows past the end come as zeros by
+// and walks k in steps of 128, fetched straight to LDS as many steps ahead as it has stages (two or four); operand rows past the end come as zeros by
 // the descriptors' bounds. The 32 x 32 x 64 instruction takes a step in two halves; half s of a step takes the step's blocks
 // of 32 s and 2 + s, so that a lane's two scales of an operand row are one 16-bit read: group g = lane / 32 holds
 // block 2 g + s (e2m1) or 16 elements of either block (e4m3), and the scale of block 2 g + s.
@@ -375,7 +375,7 @@ static int raw_pre(const MxLinearArgs& a, int pre, const MxBefore& before, int k
 //
 // A step is 2 FM groups of two instructions, each with a fragment of x; fragments are read two groups ahead, into a ring of
 // four. The barrier lies before the last two groups: by then all waves have read the step, whose place is refilled with
-// the one three further on, and the next step has landed. (With a whole half's fragments ahead the 256 x 256 tile spilled 94
+// the one so many stages further on, and the next step has landed. (With a whole half's fragments ahead the 256 x 256 tile spilled 94
 // registers.) Blocks stay for further tiles, whose first steps are fetched by the last steps of the tile before; the
 // epilogue turns the results into whole rows in a part of LDS of each wave's own.
 template <int FA_, int BM_, int BN_, int WGM_, int WGN_, int STAGES_, int ER_>
