@@ -66,36 +66,38 @@ class _MXCopy:
     another weight's as long as it is compared; their objects are compared too, since a new parameter of the same memory counts
     its versions anew. Copied or pickled it is empty: the other module's weights are others."""
 
-    __slots__ = ("mx", "of", "key", "memory", "streams", "in_graph")
+    __slots__ = ("mx", "of", "memory", "streams", "in_graph")
 
     def __init__(self, *weights: torch.Tensor):
-        self.mx, self.key = None, self._key(weights)
-        self.of, self.memory = [weakref.ref(w) for w in weights], [w.detach() for w in weights]
+        self.mx = None
+        self.of, self.memory = [(weakref.ref(w), w.data_ptr(), w._version, w.dtype) for w in weights], [w.detach() for w in weights]
         self.streams = set()   # that the allocator knows as its readers
         self.in_graph = False  # a captured graph reads it
 
     def __reduce__(self):
         return _MXCopy, ()
 
-    @staticmethod
-    def _key(weights: tuple[torch.Tensor, ...]) -> list[tuple]:
-        return [(w.data_ptr(), w._version, w.dtype, w.device) for w in weights]
-
     def is_of(self, weights: tuple[torch.Tensor, ...]) -> bool:
-        return len(self.of) == len(weights) and all(r() is w for r, w in zip(self.of, weights)) and self.key == self._key(weights)
+        if len(self.of) != len(weights):
+            return False
+        for (ref, address, version, dtype), w in zip(self.of, weights):
+            if ref() is not w or w._version != version or w.data_ptr() != address or w.dtype != dtype:
+                return False
+        return True
 
     def read(self) -> MXTensor:
         """The copy for work on the current stream. Once another has taken its place the allocator keeps its memory until the
         streams that read it have come to that point."""
-        known = _native.stream_of(self.mx.data) in self.streams
+        mx = self.mx
+        known = _native.stream_of(mx.data) in self.streams
         if not (known and self.in_graph) and torch.cuda.is_current_stream_capturing():
             self.in_graph = True
         elif not known:
-            stream = torch.cuda.current_stream(self.mx.device)
-            self.mx.data.record_stream(stream)
-            self.mx.scales.record_stream(stream)
-            self.streams.add(_native.stream_of(self.mx.data))
-        return self.mx
+            stream = torch.cuda.current_stream(mx.device)
+            mx.data.record_stream(stream)
+            mx.scales.record_stream(stream)
+            self.streams.add(_native.stream_of(mx.data))
+        return mx
 
     def release(self) -> None:
         """Waits for graphs that read the copy, whose memory is about to be given back: the allocator does not know their streams."""
