@@ -448,7 +448,8 @@ class KulaMambaLM(nn.Module):
         themselves, which stay. A copy is made anew when the model runs and its weight was replaced or changed in place; after changes
         that leave no trace (through `.data`, or by a graph's replay, as of a captured optimizer step), call this again. Copies that
         captured graphs read stay in their memory, behind all work on the GPU, and others go to new memory. Weights made in torch.inference_mode() count no changes and are
-        refused. Needs projections without bias."""
+        refused. Needs projections without bias. A block inside a reentrant checkpoint runs its forward without gradients: switch
+        back before training with one."""
         if on:
             try:
                 for layer in self.layers:

@@ -17,11 +17,11 @@
 // about 2e-14 of itself and sqrt(n) 2^-47 of the likeliest's (2e-14 and 3e-12 at 131072 tokens, to 2048 below 2e-14), where sums of
 // 64-bit floating numbers would be off by about 1e-14 and depend on their order. That is how probable it is for a border that u falls
 // on its other side.
-// Bound by the reads and the bins' atomics for large batches (256 rows of 128000 fp32 logits, a setting for each row: 76 us, where one
+// Bound by the reads and the bins' atomics for large batches (256 rows of 128000 fp32 logits, a setting for each row: 80 us, where one
 // read of them takes 22; a row alone on its CU takes 50-60), by the chain of passes, barriers and first fetches of code for few
-// (4 rows of 32000: 18-20 us, of which greedy choice and launch take 6). After the bins one wave does what is left but
+// (4 rows of 32000: 20-21 us, of which greedy choice and launch take 6). After the bins one wave does what is left but
 // gathering and sorting: with all 16 and their barriers, and the library's exponential at each place that needs one, 23-26 us. 16 waves a
-// block: with 8, which leaves the compiler more registers, the large case took 97 us for 78.
+// block: with 8, which leaves the compiler more registers, the large case took 97 us for 78 (with four terms of the series).
 #include <algorithm>
 #include <atomic>
 
