@@ -139,8 +139,9 @@ def _mx_made(kept: _MXCopy | None, weights: tuple[torch.Tensor, ...]) -> _MXCopy
             kept.mx.data.copy_(mx.data)
             kept.mx.scales.copy_(mx.scales)
             mx, made.streams = kept.mx, kept.streams
+        else:
+            made.streams.add(_native.stream_of(mx.data))  # it was allocated on
     made.mx = mx
-    made.streams.add(_native.stream_of(mx.data))
     # from here on any stream may read it
     torch.cuda.current_stream(mx.device).synchronize()
     return made

@@ -251,8 +251,10 @@ def test_readers_of_a_copy_that_a_graph_reads_too_are_known(gpu):
         for gpu.stream in (0, 5, 3, 5):
             assert get(lin) is mine
         lin.weight.add_(1.0)
+    gpu.stream = 9  # makes the copy anew in the graph's memory, and reads it
+    assert get(lin) is mine
     reads = [a for a in gpu.asked if a[0] == "reads"]
-    assert reads == [("reads", t.data_ptr(), stream) for stream in (5, 3) for t in (mine.data, mine.scales)]
+    assert reads == [("reads", t.data_ptr(), stream) for stream in (5, 3, 9) for t in (mine.data, mine.scales)]
 
 
 @torch.no_grad()
