@@ -89,15 +89,16 @@ __device__ __forceinline__ float silu_mul_odd(float gate, float u) {
 // two, with the rounding of its argument put right, 1 / (1 + e) from its reciprocal. That is off by at most 4.5 2^-23 of the
 // product (e 1.5, the sum 0.5, the reciprocal 1, three products 1.5), nine steps of fp32, which matters next to a tie only. Ties, and
 // what the scale turns on, have at most five significant bits whatever the scale: their last 19 bits are zeros. Products within
-// kNear steps of such a number (1 in 25000) are computed again, and those of |g| >= 80, where e nears the smallest numbers. (Products
-// and gates below 2^-126 fp32 itself holds in fewer bits.) Gating 8192 x 2112 in bf16: 18.7 us, 17.5 in 32 bits alone, 31 in 64 throughout. In 32 bits
-// alone 83 of 104 million e4m3 elements fell on the other side of a tie, with expf and a division 70.
+// kNear steps of such a number (1 in 25000) are computed again. So are those of g < -80, where e nears the smallest numbers, unless the
+// lane holds a product that makes zeros of them; and those of |g| > 2^127, whose exponent overflows: they come out as NaN, whose last bits
+// are zeros, too. (Products and gates below 2^-126 fp32 itself holds in fewer bits.) Gating 8192 x 2112 in bf16: 18.3 us, 17.5 in 32 bits
+// alone, 31 in 64 throughout. In 32 bits alone 83 of 104 million e4m3 elements fell on the other side of a tie, with expf and a division 70.
 __device__ __forceinline__ void silu_mul8(float (&v)[8], const float (&u)[8]) {
     constexpr float kHi = 1.44269502f, kLo = 1.92596299e-8f, kLn2 = 0.693147182f;  // log2 e = kHi + kLo
     constexpr unsigned kNear = 10u;
     const auto close = [](float x) __attribute__((always_inline)) { return (__builtin_bit_cast(unsigned, x) + kNear) << 13; };
-    float g[8], most = 0.f;
-    unsigned nearest = ~0u;
+    float g[8], low = 0.f;
+    unsigned nearest = ~0u, any = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         g[i] = v[i];
@@ -107,12 +108,18 @@ __device__ __forceinline__ void silu_mul8(float (&v)[8], const float (&u)[8]) {
         e = fmaf(e * kLn2, rest, e);
         v[i] = (g[i] < 0.f ? g[i] * e : g[i]) * __builtin_amdgcn_rcpf(1.f + e) * u[i];
         nearest = min(nearest, close(v[i]));
-        most = fmaxf(most, fabsf(g[i]));
+        any |= __builtin_bit_cast(unsigned, v[i]);
+        low = fminf(low, g[i]);
     }
-    if ((nearest <= 2 * kNear << 13 && most > 0.f) || most >= 80.f) {  // (behind a row's end all are zeros)
+    if ((nearest <= 2 * kNear << 13 && any << 1) || low < -80.f) {  // (behind a row's end all are zeros)
+        // |g| exp(-|g|) is below 2^-109 for g < -80: times u an element is half its smallest step where it is 2^-19 of the largest
+        float top = 0.f, up = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i])), up = fmaxf(up, fabsf(u[i]));
+        const bool zeros = top >= 0x1p-50f && up <= 0x1p30f;
         unsigned marks = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) marks |= (close(v[i]) <= 2 * kNear << 13 && v[i] != 0.f) || fabsf(g[i]) >= 80.f ? 1u << i : 0u;
+        for (int i = 0; i < 8; ++i) marks |= g[i] < -80.f ? (zeros ? 0u : 1u << i) : close(v[i]) <= 2 * kNear << 13 && v[i] != 0.f ? 1u << i : 0u;
         while (marks) {
             const unsigned at = __builtin_ctz(marks);
             marks &= marks - 1;

@@ -87,3 +87,27 @@ def test_gates_of_any_size():
     bad = torch.zeros(4, 64, device="cuda")
     bad[0, 3], bad[1, 3], bad[2, 3], bad[:, 35] = float("inf"), float("nan"), -float("inf"), 1.0
     assert torch.isnan(silu_mul_mx(bad).dequantize()[:3]).all() and (silu_mul_mx(bad).dequantize()[3] == 0).all()
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+def test_far_negative_gates_beside_others(fmt):
+    """Gates below -80 next to products of any size, up to factors that bring them back."""
+    gen = torch.Generator("cuda").manual_seed(3)
+    rows = 20_000
+    g = torch.randn(rows, 32, device="cuda", generator=gen, dtype=torch.float64) * 60
+    u = torch.randn(rows, 32, device="cuda", generator=gen, dtype=torch.float64) * torch.exp2(torch.randint(-60, 100, (rows, 1), device="cuda", generator=gen).double())
+    far = torch.rand(rows, 1, device="cuda", generator=gen) < 0.3
+    g = torch.where(far, -80 - 20 * torch.rand(rows, 32, device="cuda", generator=gen, dtype=torch.float64), g).float()  # rows that hold nothing else
+    u = u.float()
+    h = g.double() * torch.exp(torch.nn.functional.logsigmoid(g.double())) * u.double()
+    t = silu_mul_mx(torch.cat([g, u], 1), fmt)
+    got, scale = t.dequantize(torch.float32).double(), torch.exp2(t.scales[:, :1].double() - 127)
+    # half a step: of an element 2^-4 (e4m3) or 2^-2 of it, of the smallest ones 2^-10 or 2^-2 of the scale
+    off = 2.0 ** -4 * h.abs() + 2.0 ** -10 * scale if fmt == "e4m3" else 2.0 ** -2 * h.abs() + 2.0 ** -2 * scale
+    assert ((got - h).abs() <= off * (1 + 2.0 ** -20) + 2.0 ** -148).all()
+    top = h.abs().amax(1)
+    last = 464.0 if fmt == "e4m3" else 7.0
+    # the smallest scale under which the largest product rounds to an element
+    sure = (top > 2.0 ** -110)
+    assert (top <= last * scale[:, 0] * (1 + 2.0 ** -20))[sure].all() and (top >= last / 2 * scale[:, 0] * (1 - 2.0 ** -20))[sure].all()
