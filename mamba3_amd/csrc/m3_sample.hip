@@ -11,10 +11,10 @@
 // more (equal logits, low temperatures), each question gathers the one bin that it falls in, which is split by its keys' bits
 // until it fits.
 // With q = 64 (max z - z) / T in 64 bits, a token's mass is exp(-b / 64) exp(-r / 64), b the bin and r < 1: the bins add up
-// exp(-r / 64), five terms of its series to 2e-14, as whole numbers of 2^-45 (131072 tokens; 2^-51 to 2048), so that sums do not depend
+// exp(-r / 64), five terms of its series to 2e-14, as whole numbers of 2^-45 (131072 tokens; 2^-51 to 2048, 2^-40 for 2^22), so that sums do not depend
 // on their order; exp(-b / 64), of two table values, comes in once a bin. (An exponential for each token took three times as long.) What
 // lies past the last bin but one, below exp(-32) of the likeliest, is counted but has no mass. A running mass of n tokens is off by
-// about 2e-14 of itself and sqrt(n) 2^-47 of the likeliest's (2e-14 and 3e-12 at 131072 tokens, to 2048 below 2e-14), where sums of
+// about 2e-14 of itself and a quarter of sqrt(n) of these units (3e-12 of the likeliest's mass at 131072 tokens, to 2048 below 2e-14), where sums of
 // 64-bit floating numbers would be off by about 1e-14 and depend on their order. That is how probable it is for a border that u falls
 // on its other side.
 // Bound by the reads and the bins' atomics for large batches (256 rows of 128000 fp32 logits, a setting for each row: 80 us, where one
