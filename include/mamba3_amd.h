@@ -516,8 +516,8 @@ int m3_add_rmsnorm_bwd(int64_t rows, int32_t d, int32_t dtype, const void* total
  * out = [residual +] scale * (x w^T) for microscaled x [rows, k] (either format) and w [n, k] (e2m1); residual and
  * out [rows, n] in out_dtype. bf16 results come from the instructions that take the elements and scales as they
  * are, whose sums align e4m3 products at about 2^-13 of the largest of 128; fp32 results from bf16
- * instructions (the elements with their scales are exact in bf16) with fp32 sums. rows, n <= 2^26, k <= 2^20; for n >= 2^25 the
- * result has fewer than 2^24 pieces of 64 x 64.
+ * instructions (the elements with their scales are exact in bf16) with fp32 sums. rows, n <= 2^26, k <= 2^20; fp32
+ * results, and bf16 ones of n >= 2^25, have fewer than 2^24 pieces of 64 x 64.
  */
 int m3_mx_linear(int64_t rows, int32_t n, int32_t k, int32_t x_format, int32_t out_dtype, const void* x_data,
                  const void* x_scales, const void* w_data, const void* w_scales, const void* residual, float scale, void* out,
